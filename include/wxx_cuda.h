@@ -410,6 +410,55 @@ int wxx_adamw_device_multi(int n, float* const* p, const float* const* g, float*
 /* step (one device int) += 1, then bc = {1 - beta1^step, 1 - beta2^step} (computed in double). */
 int wxx_adamw_advance(int* step, float* bc, double beta1, double beta2);
 
+/* ---------------------------------------------------------------- recurrence, distillation, selection
+ * No reference counterpart: training and decoding a recurrent language model
+ * (functional.gated_recurrence / distill_loss / topk / beam_select / beam_reorder). */
+/* a = sigmoid(gate), h_t = a_t h_{t-1} + (1 - a_t) x_t over x (B, T, D) and gate (B, T, H), H
+ * dividing D (head i's gate serves channels i D/H .. (i+1) D/H - 1); both with unit stride inside
+ * and the given batch / time strides.  h0 (B, D): the state before position 0 (NULL: zero); reset
+ * (B, T) u32: where it is not zero the state before that position is zero (NULL: nowhere).
+ * Outputs h (B, T, D) and h_last (B, D), the state after the last position. */
+int wxx_gated_recurrence(float* h, float* h_last, const float* x, int64_t x_bs, int64_t x_ts,
+                         const float* gate, int64_t g_bs, int64_t g_ts, const float* h0,
+                         const uint32_t* reset, int64_t B, int64_t T, int64_t D, int64_t H);
+/* Its gradients dx (B, T, D), dgate (B, T, H) and dh0 (B, D; NULL: not wanted) from dh (B, T, D),
+ * the gradient of h_last dlast (B, D; NULL: zero), the forward's inputs and its output h. */
+int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0, const float* dh,
+                                  const float* dlast, const float* x, int64_t x_bs, int64_t x_ts,
+                                  const float* gate, int64_t g_bs, int64_t g_ts, const float* h,
+                                  const float* h0, const uint32_t* reset, int64_t B, int64_t T,
+                                  int64_t D, int64_t H);
+/* One position per sequence, in place: state (B, D) <- a state + (1 - a) x; x (B, D) and gate
+ * (B, H) with row strides x_ld and g_ld. */
+int wxx_gated_recurrence_step(float* state, const float* x, int64_t x_ld, const float* gate,
+                              int64_t g_ld, int64_t B, int64_t D, int64_t H);
+/* Distillation from a teacher's K stored logits per row: loss (N) = tau^2 KL(softmax(top / tau) ||
+ * softmax(logits / tau)) and the row statistics stats (N, 2) of the backward; logits (N, V) with
+ * row stride ld, top and ids (N, K), 1 <= K <= 1024.  A stored logit of -inf is an absent entry; a
+ * row without entries has loss 0; an id >= V is an absent entry and sets the device error word. */
+int wxx_distill_loss(float* loss, float* stats, const float* logits, int64_t ld, const float* top,
+                     const uint32_t* ids, int64_t N, int64_t V, int K, float tau);
+/* dz (N, V) from the gradient grad (N) of the losses. */
+int wxx_distill_backward(float* dz, const float* grad, const float* logits, int64_t ld,
+                         const float* top, const uint32_t* ids, const float* stats, int64_t N,
+                         int64_t V, int K, float tau);
+/* values and ids (N, K): the K (<= min(V, 256)) largest of each row of x (N, V; row stride ld), in
+ * descending order, equal values by the lower id first, NaN above every number. */
+int wxx_topk(float* values, uint32_t* ids, const float* x, int64_t ld, int64_t N, int64_t V, int K);
+/* One selection step of beam search, W <= 16 beams: the W best continuations of each batch item by
+ * scores[b, w] + log softmax(logits[b W + w])[token] over logits (B W, V; row stride ld).  finished
+ * (B, W; NULL with new_finished): such a beam is carried on by the token `stop` alone, at no cost.
+ * Outputs (B, W), best first: scores, parents (beam of the same item), tokens, finished. */
+int wxx_beam_select(float* new_scores, uint32_t* parents, uint32_t* tokens, uint32_t* new_finished,
+                    const float* logits, int64_t ld, const float* scores,
+                    const uint32_t* finished, int64_t B, int W, int64_t V, uint32_t stop);
+/* Row b W + w of every state takes, in place, what row b W + parents[b, w] had.  state (n device
+ * pointers in a host array), B W rows of row[i] 4-byte words each; with cur_len (one device word)
+ * only the first *cur_len * unit[i] words of a row move (unit[i] = 0: the whole row).  A parent >= W
+ * leaves its row and sets the device error word. */
+int wxx_beam_reorder(int n, uint32_t* const* state, const int64_t* row, const int64_t* unit,
+                     const uint32_t* parents, int64_t B, int W, const uint32_t* cur_len);
+
 /* ---------------------------------------------------------------- NCCL
  * No reference counterpart (the reference drives one WebGPU device): the
  * all-gather of batch-sharded outputs across the GPUs of one node. */

@@ -1,0 +1,312 @@
+"""The gated linear recurrence on the GPU against its 64-bit restatement.
+
+Tolerances.  With u = 2^-24 a step h + z (x - h) rounds x - h, the gate's z
+(a few u of itself; 32 u allows for a short exponential) and the result, so it
+adds at most u (64 z + 4) M with M the largest |x| or |h0|; an error decays by
+a = 1 - z a step, so it is multiplied by at most L = min(T, 1 / smallest z).
+That gives u M (64 + 8 L), the 8 also covering the products of a that join
+pieces of a row.  The gradients obey the same recursion with the largest total
+gradient G in the place of M.  In the 2-norm independent roundings grow with
+the root of L: 4 sqrt(L) u < 1e-5 for every L here.
+"""
+
+import numpy as np
+import pytest
+
+from oracle import recurrent
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def _F():
+    import wxx_b200 as wxx
+
+    return wxx.functional
+
+
+def up(a, dtype=np.float32):
+    return None if a is None else _F().from_numpy(np.asarray(a), dtype=dtype)
+
+
+def close(got, ref, bound):
+    got, ref = np.asarray(got, np.float64), np.asarray(ref, np.float64)
+    assert got.shape == ref.shape
+    if ref.size == 0:
+        return
+    assert np.isfinite(got).all()
+    assert np.abs(got - ref).max() <= bound, (np.abs(got - ref).max(), bound)
+    norm = np.linalg.norm(ref)
+    assert np.linalg.norm(got - ref) <= 1e-5 * norm or norm < bound
+
+
+def inputs(rng, B, T, D, H, with_h0, with_reset):
+    x = rng.standard_normal((B, T, D)).astype(np.float32)
+    gate = np.clip(rng.standard_normal((B, T, H)) * 1.5 + 2, -6, 6).astype(np.float32)
+    h0 = rng.standard_normal((B, D)).astype(np.float32) if with_h0 else None
+    reset = None
+    if with_reset:
+        reset = (rng.random((B, T)) < 0.02).astype(np.uint32) * 7     # any non-zero value
+        if T:
+            reset[0, 0] = 1
+    return x, gate, h0, reset
+
+
+def reach(gate, T):
+    z = 1 / (1 + np.exp(np.asarray(gate, np.float64)))
+    return min(max(T, 1), 1 / z.min()) if z.size else 1.0, z
+
+
+SHAPES = [
+    # B, T, D, H
+    (1, 1, 1, 1), (2, 1, 5, 5), (1, 2, 3, 1), (3, 7, 33, 33), (2, 16, 32, 32), (2, 17, 64, 2),
+    (1, 127, 40, 8), (2, 128, 31, 31), (1, 129, 96, 3), (4, 255, 30, 6), (1, 1000, 250, 250),
+    (2, 300, 70, 7), (1, 513, 256, 4), (1, 200, 192, 1), (3, 4097, 34, 17), (1, 20000, 32, 32),
+    (5, 640, 128, 128), (1, 9000, 65, 13), (2, 2048, 160, 5), (16, 130, 4, 4),
+]
+
+
+@pytest.mark.parametrize("B,T,D,H", SHAPES)
+@pytest.mark.parametrize("h0,reset", [(False, False), (True, True)])
+def test_forward_and_backward(B, T, D, H, h0, reset, rng):
+    F = _F()
+    x, gate, h0, reset = inputs(rng, B, T, D, H, h0, reset)
+    L, z = reach(gate, T)
+    M = max(np.abs(x).max(), 0 if h0 is None else np.abs(h0).max())
+    tx, tg, th0, tr = up(x), up(gate), up(h0), up(reset, np.uint32)
+    h, last = F.gated_recurrence(tx, tg, th0, tr)
+    rh, rlast = recurrent.recurrence(x, gate, h0, reset)
+    bound = U * M * (64 + 8 * L)
+    close(h.numpy(), rh, bound)
+    assert np.array_equal(last.numpy(), h.numpy()[:, -1])
+
+    dh = rng.standard_normal((B, T, D)).astype(np.float32)
+    dlast = rng.standard_normal((B, D)).astype(np.float32) if h0 is not None else None
+    dx, dg, dh0 = F.gated_recurrence_backward(up(dh), tx, tg, h, th0, tr, up(dlast))
+    rdx, rdg, rdh0 = recurrent.recurrence_backward(dh, x, gate, h0, reset, dlast)
+    G = np.abs(rdx / np.repeat(z, D // H, -1)).max()
+    bound = U * G * (64 + 8 * L)
+    close(dx.numpy(), rdx, bound)
+    close(dg.numpy(), rdg, bound * 2 * max(M, 1) * (D // H))
+    if h0 is None:
+        assert dh0 is None
+    else:
+        close(dh0.numpy(), rdh0, bound)
+
+
+def test_gradient_against_differences(rng):
+    """The kernels' own forward, differenced: the loss is linear in x and h0, so a
+    wide step loses nothing there; in the gate the truncation is step^2 / 6 of the
+    third derivative (below 1/2 a step)."""
+    F = _F()
+    B, T, D, H = 1, 6, 4, 2
+    x, gate, h0, _ = inputs(rng, B, T, D, H, True, False)
+    dh = rng.standard_normal((B, T, D)).astype(np.float32)
+
+    def value(x, gate, h0):
+        h = F.gated_recurrence(up(x), up(gate), up(h0))[0].numpy()
+        return (h.astype(np.float64) * dh).sum()
+
+    h, _ = F.gated_recurrence(up(x), up(gate), up(h0))
+    got = F.gated_recurrence_backward(up(dh), up(x), up(gate), h, up(h0))
+    step = 2.0 ** -4
+    M, W = max(np.abs(x).max(), np.abs(h0).max()) + step, np.abs(dh).sum()
+    for k, v in enumerate((x, gate, h0)):
+        ref = np.zeros(v.shape)
+        for i in np.ndindex(v.shape):
+            at = [x.copy(), gate.copy(), h0.copy()]
+            at[k][i] += step
+            hi = value(*at)
+            at[k][i] -= 2 * step
+            ref[i] = (hi - value(*at)) / (2 * step)
+        rounding = U * M * W * (64 + 8 * T) / step
+        truncation = step ** 2 / 6 * 0.5 * M * W if k == 1 else 0.0
+        assert np.abs(got[k].numpy() - ref).max() <= rounding + truncation
+
+
+def test_step_continues_the_scan(rng):
+    F = _F()
+    B, T, D, H = 3, 70, 48, 6
+    x, gate, h0, _ = inputs(rng, B, T, D, H, True, False)
+    L, _ = reach(gate, T)
+    bound = U * max(np.abs(x).max(), np.abs(h0).max()) * (64 + 8 * L)
+    ref, _ = recurrent.recurrence(x, gate, h0)
+    _, state = F.gated_recurrence(up(x[:, :50]), up(gate[:, :50]), up(h0))
+    version = state.buffer.version
+    for t in range(50, T):
+        out = F.gated_recurrence_step(up(x[:, t]), up(gate[:, t]), state)
+        assert out is state
+        close(state.numpy(), ref[:, t], bound)
+    assert state.buffer.version > version
+
+
+@pytest.mark.parametrize("B,D,H", [(1, 1, 1), (3, 5, 5), (2, 1024, 16), (257, 36, 12), (64, 4096, 4096)])
+def test_step_sizes(B, D, H, rng):
+    F = _F()
+    x, gate, h0, _ = inputs(rng, B, 1, D, H, True, False)
+    state = up(h0)
+    F.gated_recurrence_step(up(x[:, 0]), up(gate[:, 0]), state)
+    ref, _ = recurrent.recurrence(x, gate, h0)
+    close(state.numpy(), ref[:, 0], U * max(np.abs(x).max(), np.abs(h0).max()) * 72)
+
+
+def test_strided_operands(rng):
+    """x and the gate as column slices of one projection, time-major storage,
+    a broadcast gate (time stride 0) and an offset base."""
+    F = _F()
+    B, T, D = 2, 150, 24
+    both = rng.standard_normal((B, T, 3 * D)).astype(np.float32)
+    t = up(both)
+    x, gate = t[..., 1:1 + D], t[..., 2 * D:]
+    h, last = F.gated_recurrence(x, gate)
+    same, same_last = F.gated_recurrence(up(both[..., 1:1 + D]), up(both[..., 2 * D:]))
+    assert np.array_equal(h.numpy(), same.numpy())
+    assert np.array_equal(last.numpy(), same_last.numpy())
+    dh = up(rng.standard_normal((B, T, D)))
+    got = F.gated_recurrence_backward(dh, x, gate, h)
+    ref = F.gated_recurrence_backward(dh, up(both[..., 1:1 + D]), up(both[..., 2 * D:]), same)
+    for a, b in zip(got[:2], ref[:2]):
+        assert np.array_equal(a.numpy(), b.numpy())
+    # (T, B, D) storage read as (B, T, D), and x with a strided last axis (copied)
+    tm = up(np.ascontiguousarray(both[..., :D].transpose(1, 0, 2)))
+    a = F.gated_recurrence(tm.permute(1, 0, 2), gate)[0].numpy()
+    assert np.array_equal(a, F.gated_recurrence(up(both[..., :D]), gate)[0].numpy())
+    a = F.gated_recurrence(t[..., 0:2 * D:2], gate)[0].numpy()
+    assert np.array_equal(a, F.gated_recurrence(up(both[..., 0:2 * D:2]), gate)[0].numpy())
+
+
+def test_saturated_gates_and_foreign_values(rng):
+    """Gates of +-inf keep or replace the state exactly; NaN and infinities of one
+    document or channel do not reach another."""
+    F = _F()
+    B, T, D = 1, 400, 37
+    x, gate, h0, _ = inputs(rng, B, T, D, D, True, False)
+    gate[0, :, 0], gate[0, :, 1] = np.inf, -np.inf
+    gate[0, :, 2], gate[0, :, 3] = 200.0, -200.0
+    h = F.gated_recurrence(up(x), up(gate), up(h0))[0].numpy()
+    assert (h[0, :, 0] == h0[0, 0]).all() and np.array_equal(h[0, :, 1], x[0, :, 1])
+    assert (h[0, :, 2] == h0[0, 2]).all() and np.array_equal(h[0, :, 3], x[0, :, 3])
+
+    x, gate, h0, _ = inputs(rng, B, T, D, D, True, False)
+    clean = x.copy()
+    reset = np.zeros((B, T), np.uint32)
+    reset[0, [150, 320]] = 1
+    x[0, 100, 5] = np.nan
+    x[0, 200, 6] = np.inf
+    h, last = F.gated_recurrence(up(x), up(gate), up(h0), up(reset, np.uint32))
+    ref, _ = F.gated_recurrence(up(clean), up(gate), up(h0), up(reset, np.uint32))
+    h, ref = h.numpy(), ref.numpy()
+    assert np.isnan(h[0, 100:150, 5]).all() and not np.isfinite(h[0, 200:320, 6]).any()
+    h[0, 100:150, 5], h[0, 200:320, 6] = ref[0, 100:150, 5], ref[0, 200:320, 6]
+    assert np.array_equal(h, ref)
+    assert np.isfinite(last.numpy()).all()
+    # backwards: a NaN gradient stays within its document and channel
+    dh = rng.standard_normal((B, T, D)).astype(np.float32)
+    th = F.gated_recurrence(up(clean), up(gate), up(h0), up(reset, np.uint32))[0]
+    ref = [v.numpy() for v in F.gated_recurrence_backward(up(dh), up(clean), up(gate), th, up(h0),
+                                                          up(reset, np.uint32))]
+    dh[0, 200, 9] = np.nan
+    got = [v.numpy() for v in F.gated_recurrence_backward(up(dh), up(clean), up(gate), th, up(h0),
+                                                          up(reset, np.uint32))]
+    for a, b in zip(got[:2], ref[:2]):
+        assert np.isnan(a[0, 150:201, 9]).all()
+        a[0, 150:201, 9] = b[0, 150:201, 9]
+        assert np.array_equal(a, b)
+    assert np.array_equal(got[2], ref[2])
+
+
+@pytest.mark.parametrize("B,T,D", [(2, 0, 5), (0, 4, 5), (2, 3, 0)])
+def test_empty(B, T, D, rng):
+    F = _F()
+    H = max(D, 1)
+    x, gate = np.zeros((B, T, D), np.float32), np.zeros((B, T, H if D else 0), np.float32)
+    h0 = rng.standard_normal((B, D)).astype(np.float32)
+    h, last = F.gated_recurrence(up(x), up(gate), up(h0))
+    assert h.shape == [B, T, D]
+    dx, dg, dh0 = F.gated_recurrence_backward(up(x), up(x), up(gate), h, up(h0), None, up(h0))
+    if T == 0:
+        assert np.array_equal(last.numpy(), h0) and np.array_equal(dh0.numpy(), h0)
+        assert not F.gated_recurrence(up(x), up(gate))[1].numpy().any()
+
+
+def test_same_bits_every_time(rng):
+    """The join of a row's pieces has one order, whatever runs first."""
+    F = _F()
+    x, gate, h0, reset = inputs(rng, 2, 9000, 96, 3, True, True)
+    dh = up(rng.standard_normal(x.shape))
+    t = up(x), up(gate), up(h0), up(reset, np.uint32)
+    first = None
+    for _ in range(5):
+        h, last = F.gated_recurrence(*t)
+        out = [h, last, *F.gated_recurrence_backward(dh, t[0], t[1], h, t[2], t[3])]
+        out = [v.numpy() for v in out]
+        if first is None:
+            first = out
+        for a, b in zip(first, out):
+            assert np.array_equal(a, b)
+
+
+def test_offsets_past_32_bits():
+    """A sequence batch whose last rows lie past 2^32 bytes and 2^31 elements."""
+    F = _F()
+    import wxx_b200 as wxx
+
+    B, T, D = 3, 24000, 32768
+    x = wxx.Tensor((1, T, D), value=0.5)
+    gate = wxx.Tensor((1, T, 1), value=1.0)
+    # stride 0 over the batch: only the output is large (9.4 GB)
+    xb = wxx.Tensor((B, T, D), buffer=x.buffer, stride=(0, D, 1))
+    gb = wxx.Tensor((B, T, 1), buffer=gate.buffer, stride=(0, 1, 1))
+    h, last = F.gated_recurrence(xb, gb)
+    a = 1 / (1 + np.exp(-1.0))
+    tail = h[B - 1, T - 3:].numpy()
+    assert np.abs(tail - 0.5).max() < 1e-6 and np.abs(last.numpy() - 0.5).max() < 1e-6
+    head = h[B - 1, :3, ::4096].numpy()
+    ref = 0.5 * (1 - a ** np.arange(1, 4))[:, None]
+    assert np.abs(head - ref).max() < 1e-6
+
+
+def test_recorded_in_a_graph(rng):
+    F = _F()
+    import wxx_b200 as wxx
+
+    x, gate, h0, reset = inputs(rng, 2, 1500, 40, 40, True, True)
+    t = up(x), up(gate), up(h0), up(reset, np.uint32)
+    dh = up(rng.standard_normal(x.shape))
+
+    def step():
+        h, last = F.gated_recurrence(*t)
+        return (h, last, *F.gated_recurrence_backward(dh, t[0], t[1], h, t[2], t[3]))
+
+    ref = [v.numpy() for v in step()]
+    g = wxx.graph.capture(step)
+    for _ in range(3):
+        out = g.replay()
+    for a, b in zip(out, ref):
+        assert np.array_equal(a.numpy(), b)
+    x2 = rng.standard_normal(x.shape).astype(np.float32)
+    F.assign(t[0], up(x2))
+    out = [v.numpy() for v in g.replay()]
+    for a, b in zip(out, step()):
+        assert np.array_equal(a, b.numpy())
+    g.close()
+    assert wxx.backend.device_status() == 0
+
+
+def test_autograd(rng):
+    import wxx_b200 as wxx
+    from wxx_b200 import autograd
+
+    B, T, D, H = 2, 40, 12, 3
+    x, gate, h0, _ = inputs(rng, B, T, D, H, True, False)
+    w = rng.standard_normal((B, T, D)).astype(np.float32)
+    leaves = [wxx.Parameter(up(v)) for v in (x, gate, h0)]
+    h = autograd.gated_recurrence(*leaves).forward(*leaves)
+    (h * up(w)).sum().backward()
+    ref = recurrent.recurrence_backward(w, x, gate, h0)
+    L, z = reach(gate, T)
+    G = np.abs(ref[0] / np.repeat(z, D // H, -1)).max()
+    bound = U * G * (64 + 8 * L)
+    for leaf, r, k in zip(leaves, ref, (1, 2 * max(1, np.abs(x).max()) * (D // H), 1)):
+        close(leaf.grad.numpy(), r, bound * k)

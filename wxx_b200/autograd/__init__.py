@@ -483,6 +483,39 @@ class CrossEntropyLoss(Function):
         return (dz,) + (None,) * (len(self.inputs) - 1)
 
 
+class DistillLoss(Function):
+    """Per-row distillation loss (N, 1) of the student's logits against a
+    teacher's stored top logits and ids, which receive no gradient."""
+
+    def forward(self, logits, top_logits, top_ids, temperature=1.0):
+        loss, stats = functional.distill_loss(logits, top_logits, top_ids, temperature)
+        if any(self.needs_input_grad):
+            self.saved = (logits, top_logits, top_ids, stats, temperature)
+        return self._track(loss)
+
+    def backward(self, grad_output):
+        saved, self.saved = self.saved, None
+        d = functional.distill_loss_backward(grad_output, *saved)
+        return (d,) + (None,) * (len(self.inputs) - 1)
+
+
+class gated_recurrence(Function):
+    """The states of the gated linear recurrence (batch, time, channels);
+    constructed with x, the gate and, when it needs a gradient, h0."""
+
+    def forward(self, x, gate, h0=None, reset=None):
+        h, _ = functional.gated_recurrence(x, gate, h0, reset)
+        if any(self.needs_input_grad):
+            self.saved = (x, gate, h, h0, reset)
+        return self._track(h)
+
+    def backward(self, grad_output):
+        saved, self.saved = self.saved, None
+        grads = functional.gated_recurrence_backward(grad_output, *saved)
+        need = self.needs_input_grad
+        return tuple(g if n else None for g, n in zip(grads, need))
+
+
 def _training_op(name):
     class _T(Function):
         def forward(self, *args, **kwargs):

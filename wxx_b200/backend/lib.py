@@ -149,6 +149,20 @@ SIGNATURES = {
     "wxx_adamw_advance": [c_void_p, c_void_p, ctypes.c_double, ctypes.c_double],
     "wxx_adamw_device_multi": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
                               + [c_float] * 5 + [c_void_p],
+    "wxx_gated_recurrence": [c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_void_p, c_i64, c_i64,
+                             c_void_p, c_void_p, c_i64, c_i64, c_i64, c_i64],
+    "wxx_gated_recurrence_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_i64, c_i64, c_void_p, c_i64, c_i64, c_void_p, c_void_p,
+                                      c_void_p, c_i64, c_i64, c_i64, c_i64],
+    "wxx_gated_recurrence_step": [c_void_p, c_void_p, c_i64, c_void_p, c_i64, c_i64, c_i64, c_i64],
+    "wxx_distill_loss": [c_void_p, c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_i64, c_i64,
+                         c_int, c_float],
+    "wxx_distill_backward": [c_void_p, c_void_p, c_void_p, c_i64, c_void_p, c_void_p, c_void_p,
+                             c_i64, c_i64, c_int, c_float],
+    "wxx_topk": [c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64, c_int],
+    "wxx_beam_select": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_void_p,
+                        c_void_p, c_i64, c_int, c_i64, c_u32],
+    "wxx_beam_reorder": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_int, c_void_p],
     "wxx_nccl_unique_id": [P_u8],
     "wxx_nccl_init": [P_u8, c_int, c_int],
     "wxx_nccl_allgather": [c_void_p, c_void_p, c_u64],

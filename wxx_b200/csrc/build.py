@@ -35,6 +35,9 @@ SOURCES = [
     "attention.cu",
     "generate.cu",
     "train.cu",
+    "recurrence.cu",
+    "distill.cu",
+    "select.cu",
     "pool.cu",
     "nccl.cu",
 ]

@@ -139,6 +139,13 @@ from .training import (  # noqa: E402
     meanvarnormdg,
     softmax_backward,
 )
+from .distill import distill_loss, distill_loss_backward  # noqa: E402
+from .recurrence import (  # noqa: E402
+    gated_recurrence,
+    gated_recurrence_backward,
+    gated_recurrence_step,
+)
+from .selection import beam_reorder, beam_select, topk  # noqa: E402
 
 
 __all__ = [name for name in dir() if not name.startswith("__")]

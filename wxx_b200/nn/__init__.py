@@ -33,7 +33,7 @@ from .module import (
     RMSNorm,
     Sequential,
 )
-from .loss import CCELoss, MAELoss, loss
+from .loss import CCELoss, DistillLoss, MAELoss, loss
 from .optimizer import AdamW, Optimizer, SGD
 from .resnet import ResBlock, ResNet18
 
@@ -43,5 +43,5 @@ __all__ = [
     "HyenaBlock", "HyenaOperator", "ImplicitFilter", "LayerNorm", "Linear", "MaxPool1d",
     "MaxPool2d", "Module", "ModuleList", "MultiHeadAttention", "PositionalEncoding", "RMSNorm",
     "ResBlock", "ResNet18", "Sequential", "Sine", "SwiGLU", "TiedLinear",
-    "loss", "CCELoss", "MAELoss", "Optimizer", "SGD", "AdamW",
+    "loss", "CCELoss", "DistillLoss", "MAELoss", "Optimizer", "SGD", "AdamW",
 ]
