@@ -17,6 +17,11 @@
 #include <stdint.h>
 
 #include "common.cuh"
+#include "tc_gemm.cuh"
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <mutex>
 
 WXX_EXPORT int wxx_malloc(void** out, uint64_t nbytes);
 WXX_EXPORT int wxx_free(void* p);
@@ -25,11 +30,19 @@ WXX_EXPORT int wxx_reduce(float* out, const float* x, int64_t outer, int64_t red
 
 namespace {
 
+using wxx_tc::mbar_arrive_expect_tx;
+using wxx_tc::mbar_init;
+using wxx_tc::mbar_wait;
+using wxx_tc::smem_u32;
+using wxx_tc::tma_load_3d;
+
 constexpr int kT = 256;
 constexpr int kSteps = 16;          // positions of a thread
 constexpr int kWarps = 8;           // pieces of a tile, at most
 constexpr int kGroup = 32;          // tiles joined without a chain
 constexpr int kSeg = kGroup / kWarps;
+constexpr int kTile = kWarps * kSteps * 32;                // floats of a tile's operand
+constexpr int kForwardBlocks = 3, kBackwardBlocks = 2;     // resident on an SM
 constexpr int kWaitLimit = 1 << 21; // polls of a published word (about a second)
 
 // A gate as its smaller weight (<= 1/2) with the sign telling which it is:
@@ -38,8 +51,9 @@ constexpr int kWaitLimit = 1 << 21; // polls of a published word (about a second
 // (e^(-|g|) carries half an ulp of |g| log2 e).
 __device__ __forceinline__ float gate_weight(float g) {
   const float e = fast_exp2(fabsf(g) * -1.4426950408889634f);
-  const float w = __fdividef(e, 1.0f + e);
-  return copysignf(w, g);          // a NaN stays one
+  float r;                         // 1 + e is in [1, 2]: the approximate reciprocal
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));   // is good to an ulp
+  return copysignf(e * r, g);      // a NaN stays one
 }
 __device__ __forceinline__ bool keeps(float w) { return __float_as_int(w) >= 0; }
 __device__ __forceinline__ float weight_a(float w) { return keeps(w) ? 1.0f - w : -w; }
@@ -68,19 +82,31 @@ __device__ __forceinline__ Stretch join(Stretch first, Stretch then) {
   return {cuts(then.A) ? then.A : first.A * then.A, through(then, first.b)};
 }
 
+struct Yes {
+  static constexpr bool value = true;
+};
+struct No {
+  static constexpr bool value = false;
+};
+
 struct Operand {            // (B, T, ...) with unit stride inside
   const float* p;
   int64_t bs, ts;
 };
 
-// Scratch of a row of tiles, zero at launch.  Every published number travels
-// with a flag in the upper half of its 64-bit word, so a reader needs no fence.
+// The tiles of a scan and their scratch, zero at launch.  Every published number
+// travels with a flag in the upper half of its 64-bit word, so a reader needs no
+// fence.
 struct Chain {
   unsigned* ticket;
-  ulonglong2* tile;         // {A, b} of a tile, 32 channels
+  ulonglong2* tile;           // {A, b} of a tile, 32 channels
   unsigned long long* group;  // the state after each group of kGroup tiles
-  int64_t blocks;           // blocks of 32 channels
-  int tiles;                // tiles of a row
+  unsigned blocks;            // blocks of 32 channels, all sequences
+  unsigned row_blocks;        // of one sequence
+  int tiles;                  // tiles of a row
+  unsigned total;             // tiles of all rows
+  int per;                    // channels of a gate
+  int gates;                  // gates that 32 channels can have, at most
   int* err;
 };
 
@@ -109,7 +135,7 @@ __device__ __forceinline__ bool peek(const ulonglong2* p, Stretch& s) {
   return (u >> 32) != 0 && (v >> 32) != 0;
 }
 // Polls end when every lane has its words, or give up: at the limit (error word
-// set) or as soon as another block has given up.  Returns whether to stop.
+// set) or as soon as another block has given up.
 __device__ __forceinline__ bool poll_over(bool ready, int& n, int* err) {
   if (__all_sync(0xffffffffu, ready)) return true;
   ++n;
@@ -120,260 +146,452 @@ __device__ __forceinline__ bool poll_over(bool ready, int& n, int* err) {
   return (n & 1023) == 0 && *reinterpret_cast<volatile int*>(err) == WXX_DEV_ERR_MBAR_TIMEOUT;
 }
 
-struct Joint {               // shared memory of a tile's join
-  Stretch piece[kWarps][32];
+struct Joint {                    // shared memory of a block
+  Stretch piece[2][kWarps][32];   // by turns: a warp may start the next tile early
   Stretch before[kWarps][32];
   float group[32];
-  int tile;
+  uint64_t full;                  // barrier: a tile's inputs have come
+  unsigned next;
+  int abort[2];                   // a wait for them has given up, by turns
 };
 
-// The tile that this block takes.  Tiles are handed out in the order of their
-// rows' join, so whoever a block waits for has started before it.
-__device__ __forceinline__ int64_t take_tile(const Chain& c, Joint& s) {
-  if (c.tiles == 1) return blockIdx.x;
-  if (threadIdx.x == 0) s.tile = (int)atomicAdd(c.ticket, 1u);
-  __syncthreads();
-  return s.tile;
+// A block works through tiles, the next one's inputs on their way while this
+// one is joined and written.  Where tiles wait for one another they are handed
+// out by a ticket in the order of the join, and every block takes its own in that
+// order, so whoever a block waits for is already being worked on.
+__device__ __forceinline__ unsigned take_ticket(const Chain& c) { return atomicAdd(c.ticket, 1u); }
+
+// Where a thread's piece lies: lane = one of 32 channels, warp = a piece of
+// kSteps positions.  Divisions are of 32-bit numbers (the host checks that they
+// fit): in 64 bits they cost as much as the piece itself.
+struct Place {
+  unsigned q, b, j;           // channel block (all sequences), sequence, place in the row
+  int d, i, row, t0, left;    // channel, place of the piece, its row in the tile, its first
+};                            // position, positions there are
+__device__ __forceinline__ Place place_of(const Chain& c, unsigned id, bool backwards, int T,
+                                          int D) {
+  Place p;
+  const int warps = blockDim.x >> 5;
+  p.j = c.tiles == 1 ? 0 : id / c.blocks;
+  p.q = id - p.j * c.blocks;
+  p.b = p.q / c.row_blocks;
+  p.d = (int)(p.q - p.b * c.row_blocks) * 32 + (threadIdx.x & 31);
+  p.i = threadIdx.x >> 5;
+  p.row = (backwards ? warps - 1 - p.i : p.i) * kSteps;
+  p.t0 = (backwards ? c.tiles - 1 - (int)p.j : (int)p.j) * warps * kSteps + p.row;
+  p.left = p.d < D ? max(0, min(kSteps, T - p.t0)) : 0;
+  return p;
+}
+
+// A tile's inputs come to shared memory as [position][32 channels].  With kTma
+// one thread asks for a box of each operand (what lies outside the tensor reads as
+// zero); rows that are not 16-byte aligned are copied by the threads, float by
+// float, and so is a gate of several channels, as [position][gates].
+__device__ __forceinline__ void copy_float(float* dst, const float* src, bool here) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(here ? 4 : 0)
+               : "memory");
+}
+// The barrier takes this thread's arrival when its copies are done.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// This thread's piece of an operand, `back` positions earlier (zero before
+// position 0 and after the last).
+__device__ __forceinline__ void copy_piece(float* tile, const Operand& o, const Place& p,
+                                           int back) {
+  float* dst = tile + p.row * 32 + (threadIdx.x & 31);
+  const float* src = o.p + p.b * o.bs + (p.t0 - back) * o.ts + p.d;
+#pragma unroll 4
+  for (int k = 0; k < kSteps; ++k) {
+    const bool here = k < p.left && p.t0 + k >= back;
+    copy_float(dst + k * 32, here ? src : o.p, here);
+    src += o.ts;
+  }
+}
+__device__ __forceinline__ int first_gate(const Chain& c, const Place& p) {
+  return (p.d - (int)(threadIdx.x & 31)) / c.per;
+}
+__device__ __forceinline__ void copy_gates(float* tile, const Operand& g, const Chain& c,
+                                           const Place& p, int T, int D) {
+  const int d0 = p.d - (threadIdx.x & 31), first = d0 / c.per;
+  const int n = min(d0 + 31, D - 1) / c.per - first + 1;
+  const int t0 = p.t0 - p.row, steps = (blockDim.x >> 5) * kSteps;
+  const float* src = g.p + p.b * g.bs + first;
+  for (int e = threadIdx.x; e < steps * n; e += blockDim.x) {
+    const int t = e / n, k = e - t * n;
+    const bool here = t0 + t < T;
+    copy_float(tile + t * c.gates + k, here ? src + (t0 + t) * g.ts + k : g.p, here);
+  }
 }
 
 // Joins the pieces of a tile (warp i of the order holds piece `mine`) with
 // everything before it.  j: the tile's place in its row, q: its channel block.
 // Returns the state before this warp's piece.  The order of the additions
 // depends on j alone: the tiles of the same group so far, in kWarps segments,
-// then the state after the group before.
-__device__ float join_tile(const Chain& c, Joint& s, int i, Stretch mine, int j, int64_t q,
-                           float start) {
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  s.piece[i][lane] = mine;
+// then the state after the group before.  fetch_next is called once, when every
+// warp has taken its inputs from shared memory.
+template <class F>
+__device__ __forceinline__ float join_tile(const Chain& c, Joint& s, int turn, const Place& p,
+                                           Stretch mine, float start, F fetch_next) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, i = p.i;
+  auto& piece = s.piece[turn];
+  piece[i][lane] = mine;
   __syncthreads();
-  if (c.tiles == 1) {
-    float h = start;
-    for (int k = 0; k < i; ++k) h = through(s.piece[k][lane], h);
+  if (c.tiles > 1 && i == 0) {
+    Stretch all = mine;
+    for (int k = 1; k < warps; ++k) all = join(all, piece[k][lane]);
+    publish(c.tile + ((int64_t)p.q * c.tiles + p.j) * 32 + lane, all);
+  }
+  fetch_next();
+  float h = start;
+  if (c.tiles > 1) {
+    const int r = p.j % kGroup, g = p.j / kGroup;
+    const int64_t groups = (c.tiles + kGroup - 1) / kGroup;
+    const ulonglong2* row = c.tile + ((int64_t)p.q * c.tiles + g * kGroup + i * kSeg) * 32 + lane;
+    // segment i: tiles i kSeg .. of the group, those before r
+    Stretch seg[kSeg];
+    int n = 0;
+    while (true) {
+      bool ready = true;
+#pragma unroll
+      for (int k = 0; k < kSeg; ++k) {
+        seg[k] = {1.0f, 0.0f};
+        if (i * kSeg + k < r) ready = peek(row + k * 32, seg[k]) && ready;
+      }
+      if (poll_over(ready, n, c.err)) break;
+    }
+    Stretch before = seg[0];
+#pragma unroll
+    for (int k = 1; k < kSeg; ++k) before = join(before, seg[k]);
+    s.before[i][lane] = before;
+    if (i == 0) {
+      if (g > 0) {
+        n = 0;
+        while (!poll_over(peek(c.group + (p.q * groups + g - 1) * 32 + lane, h), n, c.err)) {
+        }
+      }
+      s.group[lane] = h;
+    }
+    __syncthreads();
+    h = s.group[lane];
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) h = through(s.before[k][lane], h);
+    for (int k = 0; k < i; ++k) h = through(piece[k][lane], h);
+    if (i == warps - 1 && r == kGroup - 1)
+      publish(c.group + (p.q * groups + g) * 32 + lane, through(mine, h));
     return h;
   }
-  const int r = j % kGroup, g = j / kGroup;
-  const int64_t row = q * c.tiles;
-  if (i == 0) {
-    Stretch all = mine;
-    for (int k = 1; k < warps; ++k) all = join(all, s.piece[k][lane]);
-    publish(c.tile + (row + j) * 32 + lane, all);
-  }
-  // segment i: tiles i kSeg .. of the group, those before r
-  Stretch seg[kSeg];
-  int n = 0;
-  while (true) {
-    bool ready = true;
-#pragma unroll
-    for (int k = 0; k < kSeg; ++k) {
-      seg[k] = {1.0f, 0.0f};
-      if (i * kSeg + k < r)
-        ready = peek(c.tile + (row + g * kGroup + i * kSeg + k) * 32 + lane, seg[k]) && ready;
-    }
-    if (poll_over(ready, n, c.err)) break;
-  }
-  Stretch before = seg[0];
-#pragma unroll
-  for (int k = 1; k < kSeg; ++k) before = join(before, seg[k]);
-  s.before[i][lane] = before;
-  if (i == 0) {
-    float h = start;
-    if (g > 0) {
-      n = 0;
-      while (!poll_over(peek(c.group + (q * ((c.tiles + kGroup - 1) / kGroup) + g - 1) * 32 + lane, h),
-                        n, c.err)) {
-      }
-    }
-    s.group[lane] = h;
-  }
-  __syncthreads();
-  float h = s.group[lane];
-#pragma unroll
-  for (int k = 0; k < kWarps; ++k) h = through(s.before[k][lane], h);
-  for (int k = 0; k < i; ++k) h = through(s.piece[k][lane], h);
-  if (i == warps - 1 && r == kGroup - 1)
-    publish(c.group + (q * ((c.tiles + kGroup - 1) / kGroup) + g) * 32 + lane, through(mine, h));
+  for (int k = 0; k < i; ++k) h = through(piece[k][lane], h);
   return h;
 }
 
-__device__ __forceinline__ int positions_left(int64_t T, int64_t t0) {
-  const int64_t n = T - t0;
-  return n < 0 ? 0 : n < kSteps ? (int)n : kSteps;
-}
-
-// Positions t0 .. t0 + kSteps - 1 of sequence b that start a document, as bits.
-__device__ __forceinline__ unsigned reset_bits(const uint32_t* __restrict__ reset, int64_t b,
-                                               int64_t T, int64_t t0, bool in) {
-  if (!reset) return 0u;
+// The document starts of this warp's piece: lane k's word is position k's.
+__device__ __forceinline__ uint32_t reset_word(const uint32_t* __restrict__ reset, const Place& p,
+                                               int T) {
   const int lane = threadIdx.x & 31;
-  const int64_t b0 = __shfl_sync(0xffffffffu, b, 0);
-  if (__all_sync(0xffffffffu, !in || b == b0))   // one sequence: a lane per position
-    return __ballot_sync(0xffffffffu,
-                         lane < kSteps && t0 + lane < T && reset[b0 * T + t0 + lane] != 0);
-  unsigned bits = 0;
-  if (in)
-    for (int k = 0; k < kSteps; ++k)
-      bits |= (unsigned)(t0 + k < T && reset[b * T + t0 + k] != 0) << k;
-  return bits;
+  return reset && lane < kSteps && p.t0 + lane < T ? reset[(int64_t)p.b * T + p.t0 + lane] : 0u;
 }
 
-// A tile is 32 channels (of the batch x channels rows side by side) by up to
-// kWarps pieces of kSteps positions, one piece a warp: the piece's inputs stay in
-// registers while the state before it is found, so each is read once and h is
-// written once, 12 bytes a position.  A piece is first run from a zero state for
-// its (A, b), then once more from the state that the join gives.
-__global__ void __launch_bounds__(kT)
-    recurrence_forward_kernel(float* __restrict__ h, float* __restrict__ h_last, Operand x,
-                              Operand g, const float* __restrict__ h0,
-                              const uint32_t* __restrict__ reset, int64_t B, int64_t T, int64_t D,
-                              int64_t per, Chain c) {
+// A block's way through its tiles, the same in both directions.  fetch asks for
+// a tile's inputs, work is called with a tile when they are there and calls back
+// (with the place of the next) once it has taken them.
+template <bool kBackwards, class Fetch, class Work>
+__device__ __forceinline__ void through_tiles(const Chain& c, Joint& s, unsigned arrivals,
+                                              const uint32_t* reset, int T, int D, Fetch fetch,
+                                              Work work) {
+  if (threadIdx.x == 0) {
+    mbar_init(&s.full, arrivals);
+    wxx_tc::fence_barrier_init();
+    s.abort[0] = s.abort[1] = 0;
+    if (c.tiles > 1) s.next = take_ticket(c);
+  }
+  __syncthreads();
+  unsigned id = c.tiles == 1 ? blockIdx.x : s.next;
+  if (id >= c.total) return;
+  Place p = place_of(c, id, kBackwards, T, D);
+  fetch(p);
+  uint32_t starts = reset_word(reset, p, T);
+  __syncthreads();             // s.next has been read
+  int turn = 0;
+  for (;; turn ^= 1) {
+    if (c.tiles > 1 && threadIdx.x == 0) s.next = take_ticket(c);
+    const unsigned cut = __ballot_sync(0xffffffffu, starts != 0);
+    mbar_wait(&s.full, turn, &s.abort[turn], c.err);
+    Place after = p;
+    work(p, cut, turn, [&] {
+      // after a wait that gave up nothing more is asked for: the tile's numbers
+      // are wrong, the error word says so, and no copy is in flight but its own
+      id = s.abort[turn] ? c.total : c.tiles == 1 ? id + gridDim.x : s.next;
+      if (id >= c.total) return;
+      after = place_of(c, id, kBackwards, T, D);
+      fetch(after);
+      starts = reset_word(reset, after, T);
+    });
+    if (id >= c.total) break;
+    p = after;
+  }
+  // a last wait for the copies of a tile that did not come, before the block's
+  // shared memory goes to another
+  if (s.abort[turn])
+    for (int n = 0; n < kWaitLimit && !wxx_tc::mbar_try_wait(smem_u32(&s.full), turn); ++n) {
+    }
+}
+
+__device__ __forceinline__ float* aligned_smem(float* p) {
+  return reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(p) + 127) & ~uintptr_t(127));
+}
+
+// A tile is 32 channels by up to kWarps pieces of kSteps positions.  A piece's
+// inputs come through shared memory into registers and stay there while the
+// state before it is found, so each is read once and h is written once, 12 bytes
+// a position.  A piece is first run from a zero state for its (A, b), then once
+// more from the state that the join gives.  A warp whose piece is whole and holds
+// no reset (nearly all) runs without the tests for them.
+template <bool kTma>
+__global__ void __launch_bounds__(kT, kForwardBlocks)
+    recurrence_forward_kernel(float* __restrict__ h, float* __restrict__ h_last,
+                              const __grid_constant__ CUtensorMap map_x,
+                              const __grid_constant__ CUtensorMap map_g, Operand x, Operand g,
+                              const float* __restrict__ h0, const uint32_t* __restrict__ reset,
+                              int T, int D, Chain c) {
+  extern __shared__ float s_raw[];
   __shared__ Joint s;
-  const int64_t id = take_tile(c, s);
-  const int j = (int)(id / c.blocks);
-  const int64_t q = id - j * c.blocks, ch = q * 32 + (threadIdx.x & 31);
-  const int i = threadIdx.x >> 5;
-  const int64_t t0 = ((int64_t)j * (blockDim.x >> 5) + i) * kSteps;
-  const bool in = ch < B * D;
-  const int64_t b = in ? ch / D : 0, d = in ? ch - b * D : 0;
-  const float* xp = x.p + b * x.bs + t0 * x.ts + d;
-  const float* gp = g.p + b * g.bs + t0 * g.ts + d / per;
-  const int left = in ? positions_left(T, t0) : 0;
-  float xv[kSteps], w[kSteps];
+  float *s_x = aligned_smem(s_raw), *s_g = s_x + kTile;
+  const bool own_gate = c.per == 1;
+  const unsigned box = (blockDim.x >> 5) * kSteps * 32 * sizeof(float);
+  auto fetch = [&](const Place& p) {
+    if (kTma && threadIdx.x == 0) {
+      mbar_arrive_expect_tx(&s.full, own_gate ? 2 * box : box);
+      tma_load_3d(smem_u32(s_x), &map_x, &s.full, p.d, p.t0 - p.row, p.b);
+      if (own_gate) tma_load_3d(smem_u32(s_g), &map_g, &s.full, p.d, p.t0 - p.row, p.b);
+    }
+    if (!kTma) copy_piece(s_x, x, p, 0);
+    if (!kTma && own_gate) copy_piece(s_g, g, p, 0);
+    if (!own_gate) copy_gates(s_g, g, c, p, T, D);
+    if (!kTma || !own_gate) copies_arrive(&s.full);
+  };
+  const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !own_gate ? blockDim.x : 0);
+  through_tiles<false>(c, s, arrivals, reset, T, D, fetch, [&](const Place& p, unsigned cut,
+                                                               int turn, auto next) {
+    const bool whole = __all_sync(0xffffffffu, p.left == kSteps && cut == 0);
+    const int stride = own_gate ? 32 : c.gates;
+    const float* sx = s_x + p.row * 32 + (threadIdx.x & 31);
+    const float* sg = s_g + p.row * stride +
+                      (own_gate ? (int)(threadIdx.x & 31)
+                                : min(p.d, D - 1) / c.per - first_gate(c, p));
+    float xv[kSteps], w[kSteps];
+    Stretch mine = {1.0f, 0.0f};
+    auto first_run = [&](auto plain) {
+      constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    xv[k] = k < left ? *xp : 0.f;
-    w[k] = k < left ? *gp : INFINITY;         // past the end: keep the state
-    xp += x.ts;
-    gp += g.ts;
-  }
-  const unsigned cut = reset_bits(reset, b, T, t0, in);
-  Stretch mine = {1.0f, 0.0f};
+      for (int k = 0; k < kSteps; ++k) {
+        xv[k] = sx[k * 32];
+        w[k] = gate_weight(kPlain || k < p.left ? sg[k * stride] : INFINITY);  // past the end:
+        if (!kPlain && k >= p.left) xv[k] = 0.f;                               // keep the state
+        if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
+        mine.b = mix(w[k], mine.b, xv[k]);
+        mine.A *= weight_a(w[k]);
+      }
+    };
+    if (whole) first_run(Yes{}); else first_run(No{});
+    const int64_t state = (int64_t)p.b * D + p.d;
+    float v = join_tile(c, s, turn, p, mine, h0 && p.d < D && p.j < kGroup ? h0[state] : 0.f, next);
+    float* hp = h + ((int64_t)p.b * T + p.t0) * D + p.d;
+    auto second_run = [&](auto plain) {
+      constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    w[k] = gate_weight(w[k]);
-    if (cut >> k & 1) mine = {-0.0f, 0.0f};
-    mine.b = mix(w[k], mine.b, xv[k]);
-    mine.A *= weight_a(w[k]);
-  }
-  float v = join_tile(c, s, i, mine, j, q, in && h0 ? h0[ch] : 0.f);
-  float* hp = h + (b * T + t0) * D + d;
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    if (cut >> k & 1) v = 0.f;
-    v = mix(w[k], v, xv[k]);
-    if (k < left) *hp = v;
-    if (k == left - 1 && t0 + left == T) h_last[ch] = v;
-    hp += D;
-  }
+      for (int k = 0; k < kSteps; ++k) {
+        if (!kPlain && (cut >> k & 1)) v = 0.f;
+        v = mix(w[k], v, xv[k]);
+        if (kPlain || k < p.left) *hp = v;
+        if (!kPlain && k == p.left - 1 && p.t0 + p.left == T) h_last[state] = v;
+        hp += D;
+      }
+      if (kPlain && p.t0 + kSteps == T) h_last[state] = v;
+    };
+    if (whole) second_run(Yes{}); else second_run(No{});
+  });
 }
 
 // The same tiles with time reversed: c_t = a_t r_t (dh_t + c_{t+1}) is what
 // position t hands to t - 1.  Reads dh, x, gate, h, writes dx, dgate: 24 bytes a
 // position.  DG: where the gate's gradient goes -- 1: sums over the `per` lanes
-// of a head (a power of two up to 32; lane 0 of them writes), 32: sums over the
+// of a head (a power of two up to 32; the first of them writes), 32: sums over the
 // warp, one partial sum per block of 32 channels; 0: every channel's own.
-template <int DG>
-__global__ void __launch_bounds__(kT)
+template <bool kTma, int DG>
+__global__ void __launch_bounds__(kT, kBackwardBlocks)
     recurrence_backward_kernel(float* __restrict__ dx, float* __restrict__ dg,
-                               float* __restrict__ dh0, const float* __restrict__ dh,
-                               const float* __restrict__ dlast, Operand x, Operand g,
-                               const float* __restrict__ h, const float* __restrict__ h0,
-                               const uint32_t* __restrict__ reset, int64_t B, int64_t T, int64_t D,
-                               int64_t per, Chain c) {
+                               float* __restrict__ dh0,
+                               const __grid_constant__ CUtensorMap map_x,
+                               const __grid_constant__ CUtensorMap map_g,
+                               const __grid_constant__ CUtensorMap map_d,
+                               const __grid_constant__ CUtensorMap map_h, Operand x, Operand g,
+                               Operand dh, Operand h, const float* __restrict__ dlast,
+                               const float* __restrict__ h0, const uint32_t* __restrict__ reset,
+                               int T, int D, Chain c) {
+  extern __shared__ float s_raw[];
   __shared__ Joint s;
-  const int64_t id = take_tile(c, s);
-  const int j = (int)(id / c.blocks);
-  const int64_t q = id - j * c.blocks, ch = q * 32 + (threadIdx.x & 31);
-  const int warps = blockDim.x >> 5, i = threadIdx.x >> 5;
-  // the order runs from the last position: warp i holds piece i of it
-  const int64_t t0 = ((int64_t)(c.tiles - 1 - j) * warps + (warps - 1 - i)) * kSteps;
-  const bool in = ch < B * D;
-  const int64_t b = in ? ch / D : 0, d = in ? ch - b * D : 0;
-  const int64_t at = (b * T + t0) * D + d;
-  const float* xp = x.p + b * x.bs + t0 * x.ts + d;
-  const float* gp = g.p + b * g.bs + t0 * g.ts + d / per;
-  const int left = in ? positions_left(T, t0) : 0;
-  const float *dp = dh + at, *hp = h + at;
-  float u[kSteps], w[kSteps], gv[kSteps], xv[kSteps];
-  u[0] = left == 0 ? 0.f : t0 > 0 ? *(hp - D) : h0 ? h0[ch] : 0.f;
-#pragma unroll
-  for (int k = 0; k < kSteps; ++k) {
-    w[k] = k < left ? *gp : INFINITY;
-    gv[k] = k < left ? *dp : 0.f;
-    xv[k] = k < left ? *xp : 0.f;
-    if (k + 1 < kSteps) u[k + 1] = k + 1 < left ? *hp : 0.f;
-    gp += g.ts;
-    dp += D;
-    xp += x.ts;
-    hp += D;
-  }
-  const unsigned cut = reset_bits(reset, b, T, t0, in);
-  Stretch mine = {1.0f, 0.0f};
-#pragma unroll
-  for (int k = kSteps - 1; k >= 0; --k) {
-    w[k] = gate_weight(w[k]);
-    const float a = weight_a(w[k]);
-    mine.b = a * (gv[k] + mine.b);
-    mine.A *= a;
-    if (cut >> k & 1) {
-      mine = {-0.0f, 0.0f};
-      u[k] = 0.f;
+  float *s_x = aligned_smem(s_raw), *s_d = s_x + kTile, *s_h = s_d + kTile, *s_g = s_h + kTile;
+  const bool own_gate = c.per == 1;
+  const unsigned box = (blockDim.x >> 5) * kSteps * 32 * sizeof(float);
+  auto fetch = [&](const Place& p) {
+    if (kTma && threadIdx.x == 0) {
+      const int t0 = p.t0 - p.row;
+      mbar_arrive_expect_tx(&s.full, own_gate ? 4 * box : 3 * box);
+      tma_load_3d(smem_u32(s_x), &map_x, &s.full, p.d, t0, p.b);
+      tma_load_3d(smem_u32(s_d), &map_d, &s.full, p.d, t0, p.b);
+      tma_load_3d(smem_u32(s_h), &map_h, &s.full, p.d, t0 - 1, p.b);
+      if (own_gate) tma_load_3d(smem_u32(s_g), &map_g, &s.full, p.d, t0, p.b);
     }
-    // d a / d gate = a z
-    u[k] = (u[k] - xv[k]) * (fabsf(w[k]) * (1.0f - fabsf(w[k])));
-  }
-  float v = join_tile(c, s, i, mine, j, q, in && dlast ? dlast[ch] : 0.f);
-  const int64_t heads = DG == 1 ? D / per : DG == 32 ? D / 32 : D;
-  const int64_t lanes = DG == 1 ? per : DG == 32 ? 32 : 1;
-  float* xo = dx + at + (kSteps - 1) * D;
-  float* go = dg + (b * T + t0 + kSteps - 1) * heads + d / lanes;
-#pragma unroll
-  for (int k = kSteps - 1; k >= 0; --k) {
-    const float G = gv[k] + v;
-    if (k < left) *xo = weight_z(w[k]) * G;
-    float e = G * u[k];
-    if (DG == 1) {
-      for (int o = 1; o < per; o <<= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
-    } else if (DG == 32) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
+    if (!kTma) {
+      copy_piece(s_x, x, p, 0);
+      copy_piece(s_d, dh, p, 0);
+      copy_piece(s_h, h, p, 1);
+      if (own_gate) copy_piece(s_g, g, p, 0);
     }
-    if (k < left && (DG == 0 || d % lanes == 0)) *go = e;
-    v = cut >> k & 1 ? 0.f : weight_a(w[k]) * G;
-    xo -= D;
-    go -= heads;
-  }
-  if (dh0 && in && t0 == 0) dh0[ch] = v;
+    if (!own_gate) copy_gates(s_g, g, c, p, T, D);
+    if (!kTma || !own_gate) copies_arrive(&s.full);
+  };
+  const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !own_gate ? blockDim.x : 0);
+  const int lanes = DG == 1 ? c.per : DG == 32 ? 32 : 1, heads = DG == 0 ? D : D / lanes;
+  through_tiles<true>(c, s, arrivals, reset, T, D, fetch, [&](const Place& p, unsigned cut,
+                                                              int turn, auto next) {
+    const bool whole = __all_sync(0xffffffffu, p.left == kSteps && cut == 0 && p.t0 > 0);
+    const int stride = own_gate ? 32 : c.gates, at = p.row * 32 + (threadIdx.x & 31);
+    const float* sg = s_g + p.row * stride +
+                      (own_gate ? (int)(threadIdx.x & 31)
+                                : min(p.d, D - 1) / c.per - first_gate(c, p));
+    const int64_t state = (int64_t)p.b * D + p.d;
+    float u[kSteps], w[kSteps], gv[kSteps];
+    Stretch mine = {1.0f, 0.0f};
+    auto first_run = [&](auto plain) {
+      constexpr bool kPlain = decltype(plain)::value;
+#pragma unroll
+      for (int k = kSteps - 1; k >= 0; --k) {
+        const bool here = kPlain || k < p.left;
+        w[k] = gate_weight(here ? sg[k * stride] : INFINITY);
+        gv[k] = here ? s_d[at + k * 32] : 0.f;
+        float before = s_h[at + k * 32];
+        if (!kPlain && p.t0 + k == 0) before = h0 && here ? h0[state] : 0.f;
+        if (!kPlain && (cut >> k & 1)) before = 0.f;
+        // d a / d gate = a z
+        u[k] = (before - s_x[at + k * 32]) * (fabsf(w[k]) - w[k] * w[k]);
+        const float a = weight_a(w[k]);
+        mine.b = a * (gv[k] + mine.b);
+        mine.A *= a;
+        if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
+      }
+    };
+    if (whole) first_run(Yes{}); else first_run(No{});
+    float v = join_tile(c, s, turn, p, mine, dlast && p.d < D && p.j < kGroup ? dlast[state] : 0.f,
+                        next);
+    const int64_t last = (int64_t)p.b * T + p.t0 + kSteps - 1;
+    float* xo = dx + last * D + p.d;
+    float* go = dg + last * heads + (DG == 0 ? p.d : p.d / lanes);
+    const bool writes = DG == 0 || p.d % lanes == 0;
+    auto second_run = [&](auto plain) {
+      constexpr bool kPlain = decltype(plain)::value;
+#pragma unroll
+      for (int k = kSteps - 1; k >= 0; --k) {
+        const float G = gv[k] + v;
+        if (kPlain || k < p.left) *xo = weight_z(w[k]) * G;
+        float e = G * u[k];
+        if (DG == 1) {
+          if (!kPlain && k >= p.left) e = 0.f;
+          for (int o = 1; o < lanes; o <<= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
+        } else if (DG == 32) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
+        }
+        if ((kPlain || k < p.left) && writes) *go = e;
+        v = !kPlain && (cut >> k & 1) ? 0.f : weight_a(w[k]) * G;
+        xo -= D;
+        go -= heads;
+      }
+    };
+    if (whole) second_run(Yes{}); else second_run(No{});
+    if (dh0 && p.left && p.t0 == 0) dh0[state] = v;
+  });
 }
 
 __global__ void recurrence_step_kernel(float* __restrict__ state, const float* __restrict__ x,
                                        int64_t x_ld, const float* __restrict__ g, int64_t g_ld,
-                                       int64_t n, int64_t D, int64_t per) {
+                                       int64_t n, unsigned D, unsigned per) {
   for (int64_t i = (int64_t)blockIdx.x * kT + threadIdx.x; i < n;
        i += (int64_t)gridDim.x * kT) {
-    const int64_t b = i / D, d = i - b * D;
+    const unsigned b = (unsigned)i / D, d = (unsigned)i - b * D;
     state[i] = mix(gate_weight(g[b * g_ld + d / per]), state[i], x[b * x_ld + d]);
   }
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 get_encode_scan() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
+                                         &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    cudaGetLastError();
+  });
+  return fn;
+}
+
+// A map of boxes of 32 channels by `steps` positions over an operand, where the
+// copy engine takes it: 16-byte aligned base and strides, time inside batch.
+bool encode_operand(CUtensorMap* map, const Operand& o, int64_t B, int64_t T, int64_t D,
+                    unsigned steps) {
+  auto enc = get_encode_scan();
+  const int64_t bs = B > 1 ? o.bs : T * o.ts;
+  if (!enc || (reinterpret_cast<uintptr_t>(o.p) & 15) || o.ts % 4 || bs % 4 || o.ts < D ||
+      bs < T * o.ts || bs >= (int64_t(1) << 37))
+    return false;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)B};
+  cuuint64_t strides[2] = {(cuuint64_t)o.ts * 4, (cuuint64_t)bs * 4};
+  cuuint32_t box[3] = {32, steps, 1}, ones[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(o.p), dims, strides, box,
+             ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int check_sizes(const char* what, int64_t B, int64_t T, int64_t D, int64_t H) {
+  WXX_REQUIRE(B >= 0 && T >= 0 && D >= 0 && H >= 0, "%s: negative size", what);
+  WXX_REQUIRE(D == 0 || (H > 0 && D % H == 0), "%s: %lld channels are not a multiple of %lld heads",
+              what, (long long)D, (long long)H);
+  // positions, channels and rows are numbered in 32 bits (offsets are not)
+  WXX_REQUIRE(B < (int64_t(1) << 31) && T < (int64_t(1) << 31) - 256 &&
+                  D < (int64_t(1) << 31) - 32 && B * D < (int64_t(1) << 31),
+              "%s: time or batch times channels is 2^31 or more", what);
+  return WXX_OK;
+}
+
 // Threads and blocks of a scan, and its scratch (freed by the caller).
-int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, Chain& c, unsigned& threads,
-              unsigned& grid, void** scratch) {
+int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, int64_t H, int resident, Chain& c,
+              unsigned& threads, unsigned& grid, void** scratch) {
   const int64_t pieces = (T + kSteps - 1) / kSteps;
   const int64_t warps = pieces < kWarps ? pieces : kWarps;
+  c = Chain{};
   c.tiles = (int)((pieces + warps - 1) / warps);
-  c.blocks = (B * D + 31) / 32;
+  c.row_blocks = (unsigned)((D + 31) / 32);
+  c.per = (int)(D / H);
+  c.gates = c.per >= 32 ? 2 : 31 / c.per + 2;
   c.err = wxx::device_error_word();
-  c.ticket = nullptr;
-  c.tile = nullptr;
-  c.group = nullptr;
   *scratch = nullptr;
   threads = (unsigned)(warps * 32);
-  WXX_REQUIRE(c.blocks * c.tiles < (int64_t(1) << 31), "%s: too many elements", what);
-  grid = (unsigned)(c.blocks * c.tiles);
+  const int64_t blocks = B * c.row_blocks, total = blocks * c.tiles;
+  WXX_REQUIRE(total < (int64_t(1) << 31), "%s: too many elements", what);
+  c.blocks = (unsigned)blocks;
+  c.total = (unsigned)total;
+  const int64_t most = (int64_t)wxx::num_sms() * resident;
+  grid = (unsigned)(total < most ? total : most);
   if (c.tiles == 1) return WXX_OK;
   const int64_t groups = (c.tiles + kGroup - 1) / kGroup;
-  const size_t tile_bytes = (size_t)c.blocks * c.tiles * 32 * sizeof(ulonglong2);
-  const size_t bytes = 256 + tile_bytes + (size_t)c.blocks * groups * 32 * 8;
+  const size_t tile_bytes = (size_t)total * 32 * sizeof(ulonglong2);
+  const size_t bytes = 256 + tile_bytes + (size_t)(blocks * groups) * 32 * 8;
   if (int st = wxx_malloc(scratch, bytes)) return st;
   char* p = static_cast<char*>(*scratch);
   c.ticket = reinterpret_cast<unsigned*>(p);
@@ -382,8 +600,23 @@ int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, Chain& c, unsig
   cudaError_t e = cudaMemsetAsync(p, 0, bytes, wxx::stream());
   if (e != cudaSuccess) {
     wxx_free(*scratch);
+    *scratch = nullptr;
     wxx::set_error("%s: clearing the scratch failed: %s", what, cudaGetErrorString(e));
     return WXX_E_CUDA;
+  }
+  return WXX_OK;
+}
+
+// Room for the kernel's tiles, asked for once for each kernel.
+template <class K>
+int allow_smem(K kernel, int bytes) {
+  static K done[8] = {};           // kernels of this type that have it
+  for (K& k : done) {
+    if (k == kernel) return WXX_OK;
+    if (k) continue;
+    WXX_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    k = kernel;
+    return WXX_OK;
   }
   return WXX_OK;
 }
@@ -395,15 +628,6 @@ int copy_state(float* to, const float* from, int64_t n) {
                                    wxx::stream()));
   else
     WXX_CUDA_CHECK(cudaMemsetAsync(to, 0, (size_t)n * sizeof(float), wxx::stream()));
-  return WXX_OK;
-}
-
-int check_sizes(const char* what, int64_t B, int64_t T, int64_t D, int64_t H) {
-  WXX_REQUIRE(B >= 0 && T >= 0 && D >= 0 && H >= 0, "%s: negative size", what);
-  WXX_REQUIRE(D == 0 || (H > 0 && D % H == 0), "%s: %lld channels are not a multiple of %lld heads",
-              what, (long long)D, (long long)H);
-  WXX_REQUIRE(B < (int64_t(1) << 31) && T < (int64_t(1) << 31) && D < (int64_t(1) << 31),
-              "%s: a size is 2^31 or more", what);
   return WXX_OK;
 }
 
@@ -420,13 +644,26 @@ WXX_EXPORT int wxx_gated_recurrence(float* h, float* h_last, const float* x, int
   if (int st = check_sizes("wxx_gated_recurrence", B, T, D, H)) return st;
   if (B * D == 0) return WXX_OK;
   if (T == 0) return copy_state(h_last, h0, B * D);
+  const Operand ox{x, x_bs, x_ts}, og{gate, g_bs, g_ts};
   Chain c;
   unsigned threads, grid;
   void* scratch;
-  if (int st = plan_scan("wxx_gated_recurrence", B, T, D, c, threads, grid, &scratch)) return st;
-  recurrence_forward_kernel<<<grid, threads, 0, wxx::stream()>>>(
-      h, h_last, Operand{x, x_bs, x_ts}, Operand{gate, g_bs, g_ts}, h0, reset, B, T, D, D / H, c);
-  const int st = wxx::after_launch(__FILE__, __LINE__);
+  if (int st = plan_scan("wxx_gated_recurrence", B, T, D, H, kForwardBlocks, c, threads, grid,
+                         &scratch))
+    return st;
+  constexpr int kBytes = 2 * kTile * sizeof(float) + 128;
+  CUtensorMap mx{}, mg{};
+  const unsigned steps = threads / 32 * kSteps;
+  const bool tma = encode_operand(&mx, ox, B, T, D, steps) &&
+                   (c.per > 1 || encode_operand(&mg, og, B, T, D, steps));
+  auto launch = [&](auto kernel) {
+    if (int st = allow_smem(kernel, kBytes)) return st;
+    kernel<<<grid, threads, kBytes, wxx::stream()>>>(h, h_last, mx, mg, ox, og, h0, reset, (int)T,
+                                                     (int)D, c);
+    return wxx::after_launch(__FILE__, __LINE__);
+  };
+  const int st = tma ? launch(recurrence_forward_kernel<true>)
+                     : launch(recurrence_forward_kernel<false>);
   if (scratch) wxx_free(scratch);
   return st;
 }
@@ -450,23 +687,38 @@ WXX_EXPORT int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0
   const int64_t per = D / H;
   const bool inside = per <= 32 && (per & (per - 1)) == 0, partial = per > 32 && per % 32 == 0;
   const int64_t parts = partial ? per / 32 : per;
-  float* sums = dgate;
-  void *scratch = nullptr, *wide = nullptr;
+  const Operand ox{x, x_bs, x_ts}, og{gate, g_bs, g_ts}, od{dh, T * D, D}, oh{h, T * D, D};
   Chain c;
   unsigned threads, grid;
+  void *scratch = nullptr, *wide = nullptr;
+  float* sums = dgate;
   if (!inside) {
     if (int st = wxx_malloc(&wide, (uint64_t)(B * T * H * parts) * sizeof(float))) return st;
     sums = static_cast<float*>(wide);
   }
-  int st = plan_scan("wxx_gated_recurrence_backward", B, T, D, c, threads, grid, &scratch);
+  int st = plan_scan("wxx_gated_recurrence_backward", B, T, D, H, kBackwardBlocks, c, threads, grid,
+                     &scratch);
   if (st == WXX_OK) {
-    auto kernel = per == 1 || (!inside && !partial) ? recurrence_backward_kernel<0>
-                  : inside                          ? recurrence_backward_kernel<1>
-                                                    : recurrence_backward_kernel<32>;
-    kernel<<<grid, threads, 0, wxx::stream()>>>(dx, sums, dh0, dh, dlast, Operand{x, x_bs, x_ts},
-                                                Operand{gate, g_bs, g_ts}, h, h0, reset, B, T, D,
-                                                per, c);
-    st = wxx::after_launch(__FILE__, __LINE__);
+    constexpr int kBytes = 4 * kTile * sizeof(float) + 128;
+    CUtensorMap mx{}, mg{}, md{}, mh{};
+    const unsigned steps = threads / 32 * kSteps;
+    const bool tma = encode_operand(&mx, ox, B, T, D, steps) &&
+                     encode_operand(&md, od, B, T, D, steps) &&
+                     encode_operand(&mh, oh, B, T, D, steps) &&
+                     (c.per > 1 || encode_operand(&mg, og, B, T, D, steps));
+    auto launch = [&](auto kernel) {
+      if (int e = allow_smem(kernel, kBytes)) return e;
+      kernel<<<grid, threads, kBytes, wxx::stream()>>>(dx, sums, dh0, mx, mg, md, mh, ox, og, od,
+                                                       oh, dlast, h0, reset, (int)T, (int)D, c);
+      return wxx::after_launch(__FILE__, __LINE__);
+    };
+    auto pick = [&](auto t) {
+      constexpr bool kTma = decltype(t)::value;
+      return per == 1 || (!inside && !partial) ? launch(recurrence_backward_kernel<kTma, 0>)
+             : inside                          ? launch(recurrence_backward_kernel<kTma, 1>)
+                                               : launch(recurrence_backward_kernel<kTma, 32>);
+    };
+    st = tma ? pick(Yes{}) : pick(No{});
     if (st == WXX_OK && wide) st = wxx_reduce(dgate, sums, B * T * H, parts, 1, 0);
   }
   if (scratch) wxx_free(scratch);
@@ -483,8 +735,8 @@ WXX_EXPORT int wxx_gated_recurrence_step(float* state, const float* x, int64_t x
   if (int st = check_sizes("wxx_gated_recurrence_step", B, 1, D, H)) return st;
   const int64_t n = B * D;
   if (n == 0) return WXX_OK;
-  recurrence_step_kernel<<<wxx::grid_for(n, kT), kT, 0, wxx::stream()>>>(state, x, x_ld, gate, g_ld,
-                                                                         n, D, D / H);
+  recurrence_step_kernel<<<wxx::grid_for(n, kT), kT, 0, wxx::stream()>>>(
+      state, x, x_ld, gate, g_ld, n, (unsigned)D, (unsigned)(D / H));
   WXX_LAUNCH_CHECK();
   return WXX_OK;
 }
