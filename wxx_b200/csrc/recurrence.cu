@@ -45,27 +45,30 @@ constexpr int kTile = kWarps * kSteps * 32;                // floats of a tile's
 constexpr int kForwardBlocks = 3, kBackwardBlocks = 2;     // resident on an SM
 constexpr int kWaitLimit = 1 << 21; // polls of a published word (about a second)
 
-// A gate as its smaller weight (<= 1/2) with the sign telling which it is:
-// positive: z = 1 - a, the state is kept for the most part; negative: a.  With
-// e = exp(-|g|) the smaller weight is e / (1 + e), good to a few ulp of itself
-// (e^(-|g|) carries half an ulp of |g| log2 e).
-__device__ __forceinline__ float gate_weight(float g) {
+// A gate as the smaller of its weights a and z = 1 - a, which says how much of
+// the other value is mixed in, and whether the state is the one that is kept.
+// With e = exp(-|g|) the smaller weight is e / (1 + e), good to a few ulp of
+// itself (e^(-|g|) carries half an ulp of |g| log2 e).
+struct Gate {
+  float w;
+  bool keep;
+};
+__device__ __forceinline__ Gate gate_of(float g) {
   const float e = fast_exp2(fabsf(g) * -1.4426950408889634f);
   float r;                         // 1 + e is in [1, 2]: the approximate reciprocal
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));   // is good to an ulp
-  return copysignf(e * r, g);      // a NaN stays one
+  return {e * r, g >= 0.f};        // a NaN gives one
 }
-__device__ __forceinline__ bool keeps(float w) { return __float_as_int(w) >= 0; }
-__device__ __forceinline__ float weight_a(float w) { return keeps(w) ? 1.0f - w : -w; }
-__device__ __forceinline__ float weight_z(float w) { return keeps(w) ? w : 1.0f + w; }
+__device__ __forceinline__ float weight_a(Gate g) { return g.keep ? 1.0f - g.w : g.w; }
+__device__ __forceinline__ float weight_z(Gate g) { return g.keep ? g.w : 1.0f - g.w; }
 
 // a h + z x as the larger-weighted of the two plus the smaller weight times
 // their difference: a constant gate's fixed point stays where it is (a and z,
 // each rounded, do not add up to 1: at z = 1e-3 that error is multiplied by
 // 1000), and a saturated gate keeps or replaces h exactly.
-__device__ __forceinline__ float mix(float w, float h, float x) {
-  const float base = keeps(w) ? h : x, other = keeps(w) ? x : h;
-  return fmaf(fabsf(w), other - base, base);
+__device__ __forceinline__ float mix(Gate g, float h, float x) {
+  const float base = g.keep ? h : x, other = g.keep ? x : h;
+  return fmaf(g.w, other - base, base);
 }
 
 // What a stretch of positions does to the state before it: h -> A h + b.  A
@@ -94,6 +97,19 @@ struct Operand {            // (B, T, ...) with unit stride inside
   int64_t bs, ts;
 };
 
+// n / d for n < 2^31 as a product: d <= 2^s, m = ceil(2^(31 + s) / d) < 2^32.
+struct Divider {
+  unsigned m, s, d;
+  static Divider of(unsigned d) {
+    unsigned s = 0;
+    while ((1ull << s) < d) ++s;
+    return {(unsigned)(((1ull << (31 + s)) + d - 1) / d), 31 + s, d};
+  }
+  __device__ __forceinline__ unsigned operator()(unsigned n) const {
+    return (unsigned)(((unsigned long long)n * m) >> s);
+  }
+};
+
 // The tiles of a scan and their scratch, zero at launch.  Every published number
 // travels with a flag in the upper half of its 64-bit word, so a reader needs no
 // fence.
@@ -101,8 +117,8 @@ struct Chain {
   unsigned* ticket;
   ulonglong2* tile;           // {A, b} of a tile, 32 channels
   unsigned long long* group;  // the state after each group of kGroup tiles
-  unsigned blocks;            // blocks of 32 channels, all sequences
-  unsigned row_blocks;        // of one sequence
+  Divider blocks;             // blocks of 32 channels, all sequences
+  Divider row_blocks;         // of one sequence
   int tiles;                  // tiles of a row
   unsigned total;             // tiles of all rows
   int per;                    // channels of a gate
@@ -162,8 +178,9 @@ struct Joint {                    // shared memory of a block
 __device__ __forceinline__ unsigned take_ticket(const Chain& c) { return atomicAdd(c.ticket, 1u); }
 
 // Where a thread's piece lies: lane = one of 32 channels, warp = a piece of
-// kSteps positions.  Divisions are of 32-bit numbers (the host checks that they
-// fit): in 64 bits they cost as much as the piece itself.
+// kSteps positions.  Tiles, channels and positions are numbered in 32 bits (the
+// host checks that they fit) and divided by products: 64-bit divisions cost as
+// much as the piece itself.
 struct Place {
   unsigned q, b, j;           // channel block (all sequences), sequence, place in the row
   int d, i, row, t0, left;    // channel, place of the piece, its row in the tile, its first
@@ -172,10 +189,10 @@ __device__ __forceinline__ Place place_of(const Chain& c, unsigned id, bool back
                                           int D) {
   Place p;
   const int warps = blockDim.x >> 5;
-  p.j = c.tiles == 1 ? 0 : id / c.blocks;
-  p.q = id - p.j * c.blocks;
-  p.b = p.q / c.row_blocks;
-  p.d = (int)(p.q - p.b * c.row_blocks) * 32 + (threadIdx.x & 31);
+  p.j = c.blocks(id);
+  p.q = id - p.j * c.blocks.d;
+  p.b = c.row_blocks(p.q);
+  p.d = (int)(p.q - p.b * c.row_blocks.d) * 32 + (threadIdx.x & 31);
   p.i = threadIdx.x >> 5;
   p.row = (backwards ? warps - 1 - p.i : p.i) * kSteps;
   p.t0 = (backwards ? c.tiles - 1 - (int)p.j : (int)p.j) * warps * kSteps + p.row;
@@ -346,9 +363,10 @@ __device__ __forceinline__ float* aligned_smem(float* p) {
 // A tile is 32 channels by up to kWarps pieces of kSteps positions.  A piece's
 // inputs come through shared memory into registers and stay there while the
 // state before it is found, so each is read once and h is written once, 12 bytes
-// a position.  A piece is first run from a zero state for its (A, b), then once
-// more from the state that the join gives.  A warp whose piece is whole and holds
-// no reset (nearly all) runs without the tests for them.
+// a position.  A piece is run from a zero state: what it gives at every position,
+// and the product of the weights up to there, which then takes the state that the
+// join gives.  A warp whose piece is whole and holds no reset (nearly all) runs
+// without the tests for them.
 template <bool kTma>
 __global__ void __launch_bounds__(kT, kForwardBlocks)
     recurrence_forward_kernel(float* __restrict__ h, float* __restrict__ h_last,
@@ -381,35 +399,33 @@ __global__ void __launch_bounds__(kT, kForwardBlocks)
     const float* sg = s_g + p.row * stride +
                       (own_gate ? (int)(threadIdx.x & 31)
                                 : min(p.d, D - 1) / c.per - first_gate(c, p));
-    float xv[kSteps], w[kSteps];
+    Stretch upto[kSteps];            // the piece's positions up to each
     Stretch mine = {1.0f, 0.0f};
     auto first_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
-        xv[k] = sx[k * 32];
-        w[k] = gate_weight(kPlain || k < p.left ? sg[k * stride] : INFINITY);  // past the end:
-        if (!kPlain && k >= p.left) xv[k] = 0.f;                               // keep the state
+        // past the end: keep the state
+        const Gate gate = gate_of(kPlain || k < p.left ? sg[k * stride] : INFINITY);
         if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
-        mine.b = mix(w[k], mine.b, xv[k]);
-        mine.A *= weight_a(w[k]);
+        mine.b = mix(gate, mine.b, kPlain || k < p.left ? sx[k * 32] : 0.f);
+        mine.A *= weight_a(gate);
+        upto[k] = mine;
       }
     };
     if (whole) first_run(Yes{}); else first_run(No{});
     const int64_t state = (int64_t)p.b * D + p.d;
-    float v = join_tile(c, s, turn, p, mine, h0 && p.d < D && p.j < kGroup ? h0[state] : 0.f, next);
+    const float v = join_tile(c, s, turn, p, mine, h0 && p.d < D && p.j < kGroup ? h0[state] : 0.f, next);
     float* hp = h + ((int64_t)p.b * T + p.t0) * D + p.d;
     auto second_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
-        if (!kPlain && (cut >> k & 1)) v = 0.f;
-        v = mix(w[k], v, xv[k]);
-        if (kPlain || k < p.left) *hp = v;
-        if (!kPlain && k == p.left - 1 && p.t0 + p.left == T) h_last[state] = v;
+        const float now = kPlain ? fmaf(upto[k].A, v, upto[k].b) : through(upto[k], v);
+        if (kPlain || k < p.left) *hp = now;
+        if (k == (kPlain ? kSteps : p.left) - 1 && p.t0 + k == T - 1) h_last[state] = now;
         hp += D;
       }
-      if (kPlain && p.t0 + kSteps == T) h_last[state] = v;
     };
     if (whole) second_run(Yes{}); else second_run(No{});
   });
@@ -464,40 +480,45 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
                       (own_gate ? (int)(threadIdx.x & 31)
                                 : min(p.d, D - 1) / c.per - first_gate(c, p));
     const int64_t state = (int64_t)p.b * D + p.d;
-    float u[kSteps], w[kSteps], gv[kSteps];
+    // the total gradient from a zero carry, dx and dgate per unit of it
+    float G[kSteps], z[kSteps], u[kSteps];
     Stretch mine = {1.0f, 0.0f};
     auto first_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
       for (int k = kSteps - 1; k >= 0; --k) {
         const bool here = kPlain || k < p.left;
-        w[k] = gate_weight(here ? sg[k * stride] : INFINITY);
-        gv[k] = here ? s_d[at + k * 32] : 0.f;
+        const Gate gate = gate_of(here ? sg[k * stride] : INFINITY);
         float before = s_h[at + k * 32];
         if (!kPlain && p.t0 + k == 0) before = h0 && here ? h0[state] : 0.f;
         if (!kPlain && (cut >> k & 1)) before = 0.f;
         // d a / d gate = a z
-        u[k] = (before - s_x[at + k * 32]) * (fabsf(w[k]) - w[k] * w[k]);
-        const float a = weight_a(w[k]);
-        mine.b = a * (gv[k] + mine.b);
+        u[k] = (before - s_x[at + k * 32]) * fmaf(-gate.w, gate.w, gate.w);
+        z[k] = weight_z(gate);
+        G[k] = mine.b + (here ? s_d[at + k * 32] : 0.f);
+        const float a = weight_a(gate);
+        mine.b = a * G[k];
         mine.A *= a;
         if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
       }
     };
     if (whole) first_run(Yes{}); else first_run(No{});
-    float v = join_tile(c, s, turn, p, mine, dlast && p.d < D && p.j < kGroup ? dlast[state] : 0.f,
+    const float v = join_tile(c, s, turn, p, mine, dlast && p.d < D && p.j < kGroup ? dlast[state] : 0.f,
                         next);
     const int64_t last = (int64_t)p.b * T + p.t0 + kSteps - 1;
     float* xo = dx + last * D + p.d;
     float* go = dg + last * heads + (DG == 0 ? p.d : p.d / lanes);
     const bool writes = DG == 0 || p.d % lanes == 0;
+    // What the join gives reaches position k through the weights after it: 1 - z
+    // is a to 2^-24, which is enough for a product that only scales the carry.
+    float carried = v;
     auto second_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
       for (int k = kSteps - 1; k >= 0; --k) {
-        const float G = gv[k] + v;
-        if (kPlain || k < p.left) *xo = weight_z(w[k]) * G;
-        float e = G * u[k];
+        const float total = G[k] + carried;
+        if (kPlain || k < p.left) *xo = z[k] * total;
+        float e = u[k] * total;
         if (DG == 1) {
           if (!kPlain && k >= p.left) e = 0.f;
           for (int o = 1; o < lanes; o <<= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
@@ -506,13 +527,14 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
           for (int o = 16; o > 0; o >>= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
         }
         if ((kPlain || k < p.left) && writes) *go = e;
-        v = !kPlain && (cut >> k & 1) ? 0.f : weight_a(w[k]) * G;
+        carried *= 1.0f - z[k];
+        if (!kPlain && (cut >> k & 1)) carried = 0.f;
         xo -= D;
         go -= heads;
       }
     };
     if (whole) second_run(Yes{}); else second_run(No{});
-    if (dh0 && p.left && p.t0 == 0) dh0[state] = v;
+    if (dh0 && p.left && p.t0 == 0) dh0[state] = mine.b + carried;
   });
 }
 
@@ -522,7 +544,7 @@ __global__ void recurrence_step_kernel(float* __restrict__ state, const float* _
   for (int64_t i = (int64_t)blockIdx.x * kT + threadIdx.x; i < n;
        i += (int64_t)gridDim.x * kT) {
     const unsigned b = (unsigned)i / D, d = (unsigned)i - b * D;
-    state[i] = mix(gate_weight(g[b * g_ld + d / per]), state[i], x[b * x_ld + d]);
+    state[i] = mix(gate_of(g[b * g_ld + d / per]), state[i], x[b * x_ld + d]);
   }
 }
 
@@ -576,15 +598,15 @@ int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, int64_t H, int 
   const int64_t warps = pieces < kWarps ? pieces : kWarps;
   c = Chain{};
   c.tiles = (int)((pieces + warps - 1) / warps);
-  c.row_blocks = (unsigned)((D + 31) / 32);
+  c.row_blocks = Divider::of((unsigned)((D + 31) / 32));
   c.per = (int)(D / H);
   c.gates = c.per >= 32 ? 2 : 31 / c.per + 2;
   c.err = wxx::device_error_word();
   *scratch = nullptr;
   threads = (unsigned)(warps * 32);
-  const int64_t blocks = B * c.row_blocks, total = blocks * c.tiles;
+  const int64_t blocks = B * c.row_blocks.d, total = blocks * c.tiles;
   WXX_REQUIRE(total < (int64_t(1) << 31), "%s: too many elements", what);
-  c.blocks = (unsigned)blocks;
+  c.blocks = Divider::of((unsigned)blocks);
   c.total = (unsigned)total;
   const int64_t most = (int64_t)wxx::num_sms() * resident;
   grid = (unsigned)(total < most ? total : most);
