@@ -7,12 +7,10 @@
 // a beam whose log-probabilities are NaN the score -inf.
 
 #include <cuda_runtime.h>
+#include <cooperative_groups.h>
 #include <stdint.h>
 
 #include "common.cuh"
-
-WXX_EXPORT int wxx_malloc(void** out, uint64_t nbytes);
-WXX_EXPORT int wxx_free(void* p);
 
 namespace {
 
@@ -20,126 +18,363 @@ constexpr int kT = 256;
 constexpr int kMaxTopk = 256;
 constexpr int kMaxBeams = 16;
 constexpr int kMaxStates = 128;
+constexpr int kCandidates = 2048;     // of a row, in shared memory
+constexpr int kClusterBlocks = 8;     // blocks that share a batch item's rows
 
-// A (value, index) pair as one number that is larger for the better pair:
-// the value's order-preserving bits above the inverted index.  nan_key is what
-// a NaN counts as.
-__device__ __forceinline__ uint64_t pair_key(float v, uint32_t i, uint32_t nan_key) {
-  const uint32_t u = __float_as_uint(v + 0.0f);          // -0 becomes +0
-  uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  if (v != v) k = nan_key;
-  return ((uint64_t)k << 32) | (uint32_t)~i;
-}
-constexpr uint32_t kNanHighest = 0xfffffffeu;             // above +inf, and no pair is all ones
+// The order-preserving bits of a value (-0 counts as +0); nan_key is what a NaN
+// counts as.
+constexpr uint32_t kNanHighest = 0xfffffffeu;            // above +inf
 constexpr uint32_t kNanLowest = 0x007fffffu;             // the key of -inf
-
+__device__ __forceinline__ uint32_t value_key(float v, uint32_t nan_key) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return v != v ? nan_key : k;
+}
+// A (value, index) pair as one number that is larger for the better pair: the
+// value's key above the inverted index.  0 is below every pair.
+__device__ __forceinline__ uint64_t pair_key(float v, uint32_t i, uint32_t nan_key) {
+  return ((uint64_t)value_key(v, nan_key) << 32) | (uint32_t)~i;
+}
 __device__ __forceinline__ uint32_t key_index(uint64_t k) { return ~(uint32_t)k; }
 
-__device__ __forceinline__ uint64_t block_max_key(uint64_t v, uint64_t* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = w > v ? w : v;
-  }
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-#pragma unroll
-  for (int w = 1; w < kT / 32; ++w) v = red[w] > v ? red[w] : v;
-  __syncthreads();
-  return v;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
 
-// The best pair of the row that is below `under`.
-__device__ uint64_t next_best(const float* __restrict__ row, int V, uint64_t under,
-                              uint32_t nan_key, uint64_t* red) {
-  uint64_t best = 0;
-  for (int c = threadIdx.x; c < V; c += kT) {
-    const uint64_t k = pair_key(row[c], c, nan_key);
-    if (k < under && k > best) best = k;
-  }
-  return block_max_key(best, red);
-}
+struct Select {                       // shared memory of a row's selection
+  uint64_t pair[kCandidates];
+  unsigned hist[256];
+  float tau[32];
+  float sum[32], top[32];
+  unsigned count, digit, rest;
+};
 
-__global__ void __launch_bounds__(kT)
-    topk_kernel(float* __restrict__ values, uint32_t* __restrict__ ids,
-                const float* __restrict__ x, int64_t ld, int V, int K) {
-  __shared__ uint64_t red[kT / 32];
-  const int64_t row = blockIdx.x;
-  const float* z = x + row * ld;
-  uint64_t under = ~0ull;
-  for (int k = 0; k < K; ++k) {
-    under = next_best(z, V, under, kNanHighest, red);
-    if (threadIdx.x == 0) {
-      const uint32_t i = key_index(under);
-      ids[row * K + k] = i;
-      values[row * K + k] = z[i];
+// A row split over THREADS threads: 16-byte groups in the aligned middle, thread
+// t taking groups t, t + THREADS, ..., and up to six single entries at its ends,
+// one each for the first threads.
+struct Row {
+  const float* p;
+  const float4* mid;
+  int V, head, groups, single;        // single: this thread's single entry, -1 for none
+  __device__ Row(const float* row, int n) : p(row), V(n) {
+    head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / 4);
+    groups = (n - head) / 4;
+    mid = reinterpret_cast<const float4*>(row + head);
+    const int tail = n - head - 4 * groups, t = threadIdx.x;
+    single = t < head ? t : t < head + tail ? n - tail + (t - head) : -1;
+  }
+  template <int THREADS, class F>
+  __device__ __forceinline__ void each(F f) const {
+    if (single >= 0) f(p[single], single);
+    for (int i = threadIdx.x; i < groups; i += THREADS) {
+      const float4 v = mid[i];
+      const int at = head + 4 * i;
+      f(v.x, at);
+      f(v.y, at + 1);
+      f(v.z, at + 2);
+      f(v.w, at + 3);
     }
   }
+};
+
+// The r-th largest (from 1) of key(entry) over the row's entries that `among`
+// lets in, by 8-bit digits from the top; rest: how many of the entries equal to it
+// are needed to make up r.
+template <int THREADS, class Key, class Among>
+__device__ uint32_t nth_key(const Row& row, Select& s, unsigned r, unsigned& rest, Key key,
+                            Among among) {
+  uint32_t prefix = 0, mask = 0;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = threadIdx.x; i < 256; i += THREADS) s.hist[i] = 0;
+    __syncthreads();
+    row.each<THREADS>([&](float v, int i) {
+      const uint32_t k = key(v, i);
+      if (among(v, i) && (k & mask) == prefix) atomicAdd(&s.hist[k >> shift & 255u], 1u);
+    });
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      unsigned above = 0;
+      int d = 255;
+      while (d > 0 && above + s.hist[d] < r) above += s.hist[d--];
+      s.digit = d;
+      s.rest = r - above;
+    }
+    __syncthreads();
+    prefix |= s.digit << shift;
+    mask |= 255u << shift;
+    r = s.rest;
+    __syncthreads();
+  }
+  rest = r;
+  return prefix;
 }
 
-// Candidates of one beam: its W best tokens by logit with their scores.
-__global__ void __launch_bounds__(kT)
-    beam_rows_kernel(float* __restrict__ cand, uint32_t* __restrict__ tokens,
-                     const float* __restrict__ logits, int64_t ld,
-                     const float* __restrict__ scores, const uint32_t* __restrict__ finished,
-                     int W, int V, uint32_t stop) {
-  __shared__ uint64_t red[kT / 32];
-  __shared__ float s_sum[kT / 32];
-  const int64_t row = blockIdx.x;
-  const float* z = logits + row * ld;
-  const float score = scores[row];
-  if (finished && finished[row]) {
-    if (threadIdx.x < W) {
-      cand[row * W + threadIdx.x] = threadIdx.x == 0 && score == score ? score : -INFINITY;
-      tokens[row * W + threadIdx.x] = stop;
+// Puts the row's K best pairs, and perhaps more of its best, into s.pair and
+// returns how many (K <= V).  With SUM, top and sum come to hold the row's largest
+// number and the sum of exp(v - top).
+//
+// One pass over the row gives every thread its largest entry.  The ceil(K / warps)
+// th largest of a warp's, the smallest of that over the warps, is a value that at
+// least K entries reach, and few more do: about 3 K of 50304 at K = 64 and 32
+// warps.  The threads whose largest reaches it read their entries again (from
+// L2) and keep those that do.  Where too many do (long runs of one value, or large
+// ones crowded into a few threads), the exact K-th pair is found digit by digit.
+template <int THREADS, uint32_t NAN_KEY, bool SUM>
+__device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& sum) {
+  constexpr int kWarps = THREADS / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float m = row.single >= 0 ? row.p[row.single] : -INFINITY;
+  if (NAN_KEY == kNanLowest && m != m) m = -INFINITY;
+  float part = 0.f;
+  if (SUM && row.single >= 0 && row.p[row.single] != -INFINITY) part = expf(row.p[row.single] - m);
+  auto larger = [](float a, float b) {
+    return NAN_KEY == kNanHighest ? max_nan(a, b) : fmaxf(a, b);
+  };
+#pragma unroll 4
+  for (int i = threadIdx.x; i < row.groups; i += THREADS) {
+    const float4 v = row.mid[i];
+    const float n = larger(larger(m, v.x), larger(larger(v.y, v.z), v.w));
+    if (SUM && n != -INFINITY) {
+      if (n > m) part *= fast_exp2((m - n) * 1.4426950408889634f);
+      part += (fast_exp2((v.x - n) * 1.4426950408889634f) +
+               fast_exp2((v.y - n) * 1.4426950408889634f)) +
+              (fast_exp2((v.z - n) * 1.4426950408889634f) +
+               fast_exp2((v.w - n) * 1.4426950408889634f));
+    } else if (SUM) {
+      part += (v.x + v.y) + (v.z + v.w) == -INFINITY ? 0.f : NAN;   // nothing but -inf, or NaN
+    }
+    m = n;
+  }
+  // the warp's lanes in descending order of their largest entries
+  float o = m != m ? INFINITY : m;
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, o, j);
+      const bool first = (lane & j) == 0, down = (lane & k) == 0;
+      o = first == down ? fmaxf(o, other) : fminf(o, other);
+    }
+  const float reach = __shfl_sync(0xffffffffu, o, (K + kWarps - 1) / kWarps - 1);
+  if (SUM) {
+    const float w = __shfl_sync(0xffffffffu, o, 0);
+    part *= m == -INFINITY || m == w ? 1.0f : expf(m - w);
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) part += __shfl_xor_sync(0xffffffffu, part, k);
+    if (lane == 0) {
+      s.top[warp] = w;
+      s.sum[warp] = part;
+    }
+  }
+  if (lane == 0) s.tau[warp] = reach;
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+  float tau = INFINITY;
+  for (int w = 0; w < kWarps; ++w) tau = fminf(tau, s.tau[w]);
+  if (SUM) {
+    top = -INFINITY;
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s.top[w]);
+    sum = 0.f;
+    for (int w = 0; w < kWarps; ++w)
+      sum += s.top[w] == top ? s.sum[w] : s.sum[w] * expf(s.top[w] - top);
+  }
+  auto keep = [&](float v, int i) {
+    const unsigned at = atomicAdd(&s.count, 1u);
+    if (at < kCandidates) s.pair[at] = pair_key(v, i, NAN_KEY);
+  };
+  // all pairs of a short row, else those that reach tau (NaN counts as reaching
+  // where it is the highest; where it is the lowest, tau = -inf is left to the
+  // digits, which know where it stands)
+  const bool all = row.V <= kCandidates && tau == -INFINITY;
+  const bool plain = all || tau > -INFINITY || NAN_KEY == kNanHighest;
+  if (plain && (all || !(m < tau)))
+    row.each<THREADS>([&](float v, int i) {
+      if (all || (NAN_KEY == kNanHighest ? !(v < tau) : v >= tau)) keep(v, i);
+    });
+  __syncthreads();
+  const unsigned n = s.count;
+  if (plain && n <= kCandidates) return (int)n;
+  __syncthreads();
+  unsigned rest, none;
+  const uint32_t cut = nth_key<THREADS>(
+      row, s, K, rest, [](float v, int) { return value_key(v, NAN_KEY); },
+      [](float, int) { return true; });
+  const uint32_t last = ~nth_key<THREADS>(
+      row, s, rest, none, [](float, int i) { return ~(uint32_t)i; },
+      [&](float v, int) { return value_key(v, NAN_KEY) == cut; });
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+  row.each<THREADS>([&](float v, int i) {
+    const uint32_t k = value_key(v, NAN_KEY);
+    if (k > cut || (k == cut && (uint32_t)i <= last)) keep(v, i);
+  });
+  __syncthreads();
+  return K;
+}
+
+// Calls put(rank, pair) for the K best of the n pairs in s.pair (all different).
+// Up to 256 of them are counted against each other; more are sorted, a pair a
+// thread, where there are threads for that.
+template <int THREADS, class F>
+__device__ void in_order(Select& s, int n, int K, F put) {
+  const int t = threadIdx.x;
+  if (n <= 256 || n > THREADS) {
+    for (int i = t; i < n; i += THREADS) {
+      const uint64_t mine = s.pair[i];
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) rank += s.pair[j] > mine;
+      if (rank < K) put(rank, mine);
     }
     return;
   }
-  uint64_t under = next_best(z, V, ~0ull, kNanLowest, red);
-  const float m = z[key_index(under)];
-  float s = 0.f;
-  for (int c = threadIdx.x; c < V; c += kT) s += expf(z[c] - m);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = s;
-  __syncthreads();
-  s = 0.f;
-#pragma unroll
-  for (int w = 0; w < kT / 32; ++w) s += s_sum[w];
-  const float log_s = logf(s);
-  for (int k = 0; k < W; ++k) {
-    if (threadIdx.x == 0) {
-      const uint32_t i = key_index(under);
-      const float c = k < V ? score + ((z[i] - m) - log_s) : -INFINITY;
-      cand[row * W + k] = c == c ? c : -INFINITY;
-      tokens[row * W + k] = k < V ? i : 0u;
+  int size = 512;
+  while (size < n) size <<= 1;
+  uint64_t mine = t < n ? s.pair[t] : 0;
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      uint64_t other;
+      if (j >= 32) {
+        __syncthreads();
+        if (t < size) s.pair[t] = mine;
+        __syncthreads();
+        other = t < size ? s.pair[t ^ j] : 0;
+      } else {
+        other = __shfl_xor_sync(0xffffffffu, mine, j);
+      }
+      const bool first = (t & j) == 0, down = (t & k) == 0;
+      mine = (first == down) == (mine > other) ? mine : other;
     }
-    if (k + 1 < V) under = next_best(z, V, under, kNanLowest, red);
-  }
+  if (t < K) put(t, mine);
 }
 
-// The W best candidates of a batch item, by score, then beam, then rank.
-__global__ void beam_merge_kernel(float* __restrict__ new_scores, uint32_t* __restrict__ parents,
-                                  uint32_t* __restrict__ new_tokens,
-                                  uint32_t* __restrict__ new_finished,
-                                  const float* __restrict__ cand,
-                                  const uint32_t* __restrict__ tokens,
-                                  const uint32_t* __restrict__ finished, int W, uint32_t stop) {
-  const int64_t b = blockIdx.x;
-  const int i = threadIdx.x, n = W * W;
-  if (i >= n) return;
-  const float* c = cand + b * n;
-  const uint64_t mine = pair_key(c[i], i, kNanLowest);
-  int rank = 0;
-  for (int j = 0; j < n; ++j) rank += pair_key(c[j], j, kNanLowest) > mine;
-  if (rank >= W) return;
-  const int64_t o = b * W + rank;
-  new_scores[o] = c[i];
-  parents[o] = i / W;
-  const uint32_t t = tokens[b * n + i];
-  new_tokens[o] = t;
-  if (new_finished) new_finished[o] = finished[b * W + i / W] != 0 || t == stop;
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 2048 / THREADS)
+    topk_kernel(float* __restrict__ values, uint32_t* __restrict__ ids,
+                const float* __restrict__ x, int64_t ld, int V, int K) {
+  __shared__ Select s;
+  const int64_t at = blockIdx.x;
+  const Row row(x + at * ld, V);
+  float top, sum;
+  const int n = best_pairs<THREADS, kNanHighest, false>(row, K, s, top, sum);
+  in_order<THREADS>(s, n, K, [&](int rank, uint64_t pair) {
+    const uint32_t i = key_index(pair);
+    ids[at * K + rank] = i;
+    values[at * K + rank] = row.p[i];
+  });
+}
+
+// One selection step.  A cluster takes a batch item; its rows, or `parts` pieces
+// of each where there are few, go to its blocks in turn.  Each leaves the piece's
+// best W pairs, its largest logit and its sum of exponentials in shared memory,
+// and the first block merges them all:
+//   score = scores[w] + ((z - top_w) - log sum_w)
+struct Piece {
+  uint64_t pair[kMaxBeams];           // 0: no pair
+  float top, sum;
+};
+struct Merge {
+  Select s;
+  Piece piece[2];                     // pieces rank, rank + blocks
+  uint64_t first[kMaxBeams * kMaxBeams], second[kMaxBeams * kMaxBeams];
+  float top[kMaxBeams], log_sum[kMaxBeams];
+};
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS)
+    beam_select_kernel(float* __restrict__ new_scores, uint32_t* __restrict__ parents,
+                       uint32_t* __restrict__ new_tokens, uint32_t* __restrict__ new_finished,
+                       const float* __restrict__ logits, int64_t ld,
+                       const float* __restrict__ scores, const uint32_t* __restrict__ finished,
+                       int W, int V, int parts, uint32_t stop) {
+  __shared__ Merge s;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = cluster.block_rank(), blocks = cluster.num_blocks();
+  const int64_t b = blockIdx.x / blocks;
+  const int t = threadIdx.x, pieces = W * parts;
+  // a piece's length, a multiple of 4 so that all start where the first does
+  const int length = parts == 1 ? V : ((V + parts - 1) / parts + 3) / 4 * 4;
+  for (int q = rank, turn = 0; q < pieces; q += blocks, ++turn) {
+    Piece& piece = s.piece[turn];
+    const int w = q / parts, from = (q - w * parts) * length;
+    const int n = min(length, V - from), K = min(W, n);
+    if (t < W) piece.pair[t] = 0;
+    __syncthreads();
+    if (finished && finished[b * W + w]) continue;
+    const Row row(logits + (b * W + w) * ld + from, n);
+    float top, sum;
+    const int found = best_pairs<THREADS, kNanLowest, true>(row, K, s.s, top, sum);
+    in_order<THREADS>(s.s, found, K, [&](int r, uint64_t pair) {
+      piece.pair[r] = pair - (uint32_t)from;        // the inverted index of the row
+    });
+    if (t == 0) {
+      piece.top = top;
+      piece.sum = sum;
+    }
+    __syncthreads();
+  }
+  cluster.sync();
+  if (rank == 0) {
+    auto piece_of = [&](int q) -> const Piece* {
+      return cluster.map_shared_rank(&s.piece[q / blocks], q % blocks);
+    };
+    if (t < W) {
+      float top = -INFINITY, sum = 0.f;
+      if (!(finished && finished[b * W + t])) {
+        for (int k = 0; k < parts; ++k) top = fmaxf(top, piece_of(t * parts + k)->top);
+        for (int k = 0; k < parts; ++k) {
+          const Piece* p = piece_of(t * parts + k);
+          sum += p->top == top ? p->sum : p->sum * expf(p->top - top);
+        }
+      }
+      s.top[t] = top;
+      s.log_sum[t] = logf(sum);
+    }
+    __syncthreads();
+    // Every beam's W best pairs of all its pieces compete: by score, then the lower
+    // beam, then the better pair of it.
+    const int n = pieces * W;
+    for (int i = t; i < n; i += THREADS) {
+      const int q = i / W, r = i - q * W, w = q / parts;
+      const float score = scores[b * W + w];
+      uint64_t pair = piece_of(q)->pair[r];
+      float c = -INFINITY;
+      if (finished && finished[b * W + w]) {
+        if (q == w * parts && r == 0) {
+          c = score;
+          pair = 1;
+        }
+      } else if (pair) {
+        const float z = logits[(b * W + w) * ld + key_index(pair)];
+        c = score + ((z - s.top[w]) - s.log_sum[w]);
+      }
+      s.first[i] = (uint64_t)value_key(c, kNanLowest) << 32 | (uint32_t)(kMaxBeams - w);
+      s.second[i] = pair;
+    }
+    __syncthreads();
+    for (int i = t; i < n; i += THREADS) {
+      const uint64_t f = s.first[i], g = s.second[i];
+      int place = 0;
+      for (int j = 0; j < n; ++j) {
+        const uint64_t fj = s.first[j], gj = s.second[j];
+        place += fj > f || (fj == f && (gj > g || (gj == g && j < i)));
+      }
+      if (place >= W) continue;
+      const int w = i / W / parts;
+      const bool done = finished && finished[b * W + w];
+      const uint32_t token = done ? stop : g ? key_index(g) : 0u;
+      const uint32_t k = (uint32_t)(f >> 32);
+      const int64_t o = b * W + place;
+      new_scores[o] = __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+      parents[o] = w;
+      new_tokens[o] = token;
+      if (new_finished) new_finished[o] = done || token == stop;
+    }
+  }
+  cluster.sync();                     // the pieces stay until they have been read
 }
 
 struct StateTable {
@@ -188,7 +423,12 @@ WXX_EXPORT int wxx_topk(float* values, uint32_t* ids, const float* x, int64_t ld
   WXX_REQUIRE(K >= 1 && K <= kMaxTopk && K <= V, "wxx_topk: k = %d outside [1, min(%lld, %d)]", K,
               (long long)V, kMaxTopk);
   if (N == 0) return WXX_OK;
-  topk_kernel<<<(unsigned)N, kT, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
+  // 256 threads see a short row in a few loads; a long one, or a K that would take
+  // many of each warp's entries, is worth 1024
+  if (V <= 4096 && K <= 64)
+    topk_kernel<256><<<(unsigned)N, 256, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
+  else
+    topk_kernel<1024><<<(unsigned)N, 1024, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
   WXX_LAUNCH_CHECK();
   return WXX_OK;
 }
@@ -208,21 +448,27 @@ WXX_EXPORT int wxx_beam_select(float* new_scores, uint32_t* parents, uint32_t* t
   WXX_REQUIRE((finished == nullptr) == (new_finished == nullptr),
               "wxx_beam_select: finished and new_finished go together");
   if (B == 0) return WXX_OK;
-  void* scratch = nullptr;
-  const int64_t n = B * W * W;
-  if (int st = wxx_malloc(&scratch, (uint64_t)n * 8)) return st;
-  float* cand = static_cast<float*>(scratch);
-  uint32_t* toks = reinterpret_cast<uint32_t*>(cand + n);
-  beam_rows_kernel<<<(unsigned)(B * W), kT, 0, wxx::stream()>>>(cand, toks, logits, ld, scores,
-                                                                finished, W, (int)V, stop);
-  int st = wxx::after_launch(__FILE__, __LINE__);
-  if (st == WXX_OK) {
-    beam_merge_kernel<<<(unsigned)B, 256, 0, wxx::stream()>>>(
-        new_scores, parents, tokens, new_finished, cand, toks, finished, W, stop);
-    st = wxx::after_launch(__FILE__, __LINE__);
-  }
-  wxx_free(scratch);
-  return st;
+  // long rows of few beams are split so that the cluster's blocks all have a piece
+  const bool wide = V > 4096;
+  const int parts = wide && W < kClusterBlocks ? kClusterBlocks / W : 1;
+  const int blocks = W * parts < kClusterBlocks ? W * parts : kClusterBlocks;
+  WXX_REQUIRE(B * blocks < (int64_t(1) << 31), "wxx_beam_select: too many rows");
+  auto launch = [&](auto kernel, int threads) -> int {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(B * blocks));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = wxx::stream();
+    cudaLaunchAttribute at = {};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim = {(unsigned)blocks, 1, 1};
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    WXX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, new_scores, parents, tokens, new_finished,
+                                      logits, ld, scores, finished, W, (int)V, parts, stop));
+    WXX_LAUNCH_CHECK();
+    return WXX_OK;
+  };
+  return wide ? launch(beam_select_kernel<1024>, 1024) : launch(beam_select_kernel<256>, 256);
 }
 
 // Moves the rows of n state tensors in place: row b W + w of each takes what
