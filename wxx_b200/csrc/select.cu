@@ -10,6 +10,8 @@
 #include <cooperative_groups.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace {
@@ -384,31 +386,59 @@ struct StateTable {
   int64_t unit[kMaxStates];    // words of one position (0: the whole row moves)
 };
 
-// Every thread owns a word position of a batch item: it reads it from all the
-// beams, then writes it to all, so the move is in place.
-__global__ void beam_reorder_kernel(const __grid_constant__ StateTable tab,
-                                    const uint32_t* __restrict__ parents,
-                                    const uint32_t* __restrict__ cur_len, int W, int* err) {
+// Every thread owns a place in the rows of a batch item: it reads it from every
+// beam that someone else follows, then writes it to the followers, so the move is
+// in place and a beam is read once however many follow it.  Beams that follow
+// themselves are not touched.  MAX: beams, at most; four words at a time where the
+// rows are 16-byte aligned.
+template <int MAX>
+__global__ void __launch_bounds__(kT)
+    beam_reorder_kernel(const __grid_constant__ StateTable tab,
+                        const uint32_t* __restrict__ parents,
+                        const uint32_t* __restrict__ cur_len, int W, int* err) {
+  __shared__ unsigned s_followers[MAX];
   const int64_t b = blockIdx.y;
-  const int s = blockIdx.z;
-  int64_t n = tab.row[s];
+  const int s = blockIdx.z, t = threadIdx.x;
+  const int64_t row = tab.row[s];
+  int64_t n = row;
   if (cur_len && tab.unit[s]) {
     const int64_t used = (int64_t)*cur_len * tab.unit[s];
     n = used < n ? used : n;
   }
-  uint32_t* base = tab.p[s] + b * W * tab.row[s];
-  for (int64_t i = (int64_t)blockIdx.x * kT + threadIdx.x; i < n; i += (int64_t)gridDim.x * kT) {
-    uint32_t v[kMaxBeams];
-    for (int w = 0; w < W; ++w) v[w] = base[w * tab.row[s] + i];
-    for (int w = 0; w < W; ++w) {
-      const uint32_t p = parents[b * W + w];
-      if (p >= (uint32_t)W) {
-        wxx_device_fail(err, WXX_DEV_ERR_BAD_INDEX);
-        continue;
-      }
-      base[w * tab.row[s] + i] = v[p];
+  if (t < 32) {
+    const uint32_t parent = t < W ? parents[b * W + t] : (uint32_t)t;
+    if (t < W && parent >= (uint32_t)W) wxx_device_fail(err, WXX_DEV_ERR_BAD_INDEX);
+    for (int p = 0; p < MAX; ++p) {
+      const unsigned who = __ballot_sync(0xffffffffu, t < W && parent == (uint32_t)p && t != p);
+      if (t == 0) s_followers[p] = who;
     }
   }
+  __syncthreads();
+  unsigned followers[MAX];
+  unsigned any = 0;
+#pragma unroll
+  for (int p = 0; p < MAX; ++p) any |= followers[p] = s_followers[p];
+  if (!any) return;
+  uint32_t* base = tab.p[s] + b * W * row;
+  auto move = [&](auto* at, int64_t step, int64_t i) {
+    auto* column = at + i;
+    std::remove_reference_t<decltype(*at)> v[MAX];
+#pragma unroll
+    for (int p = 0; p < MAX; ++p)
+      if (followers[p]) v[p] = column[p * step];
+#pragma unroll
+    for (int p = 0; p < MAX; ++p)
+      for (unsigned who = followers[p]; who; who &= who - 1)
+        column[(__ffs(who) - 1) * step] = v[p];
+  };
+  int64_t done = 0;
+  if (row % 4 == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0) {
+    for (int64_t i = (int64_t)blockIdx.x * kT + t; i < n / 4; i += (int64_t)gridDim.x * kT)
+      move(reinterpret_cast<uint4*>(base), row / 4, i);
+    done = n / 4 * 4;
+  }
+  for (int64_t i = done + (int64_t)blockIdx.x * kT + t; i < n; i += (int64_t)gridDim.x * kT)
+    move(base, row, i);
 }
 
 }  // namespace
@@ -498,11 +528,14 @@ WXX_EXPORT int wxx_beam_reorder(int n, uint32_t* const* state, const int64_t* ro
       longest = longest < row[i] ? row[i] : longest;
     }
     if (tab.n == 0) continue;
-    int64_t blocks = (longest + kT - 1) / kT;
-    if (blocks > 1024) blocks = 1024;
-    dim3 grid((unsigned)blocks, (unsigned)B, (unsigned)tab.n);
-    beam_reorder_kernel<<<grid, kT, 0, wxx::stream()>>>(tab, parents, cur_len, W,
-                                                        wxx::device_error_word());
+    // about eight blocks an SM in all, more where a row gives each thread work
+    const int64_t groups = (longest / 4 + kT - 1) / kT, rest = B * tab.n;
+    int64_t blocks = (wxx::num_sms() * 32 + rest - 1) / rest;
+    blocks = blocks < groups ? blocks : groups;
+    const dim3 grid((unsigned)(blocks < 1 ? 1 : blocks), (unsigned)B, (unsigned)tab.n);
+    auto kernel = W <= 4 ? beam_reorder_kernel<4> : W <= 8 ? beam_reorder_kernel<8>
+                                                          : beam_reorder_kernel<16>;
+    kernel<<<grid, kT, 0, wxx::stream()>>>(tab, parents, cur_len, W, wxx::device_error_word());
     WXX_LAUNCH_CHECK();
   }
   return WXX_OK;
