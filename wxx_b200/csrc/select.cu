@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "common.cuh"
 
@@ -38,6 +39,10 @@ __device__ __forceinline__ uint64_t pair_key(float v, uint32_t i, uint32_t nan_k
   return ((uint64_t)value_key(v, nan_key) << 32) | (uint32_t)~i;
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t k) { return ~(uint32_t)k; }
+__device__ __forceinline__ float key_float(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ float key_value(uint64_t k) { return key_float((uint32_t)(k >> 32)); }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
@@ -45,12 +50,33 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The lanes' values in descending order.
+__device__ __forceinline__ uint32_t descending(uint32_t v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, v, j);
+      const bool first = (lane & j) == 0, down = (lane & k) == 0;
+      v = first == down ? max(v, other) : min(v, other);
+    }
+  return v;
+}
+
 struct Select {                       // shared memory of a row's selection
   uint64_t pair[kCandidates];
   unsigned hist[256];
-  float tau[32];
+  uint32_t reach[32];
   float sum[32], top[32];
-  unsigned count, digit, rest;
+  int warp[32];
+  unsigned digit, rest;
 };
 
 // A row split over THREADS threads: 16-byte groups in the aligned middle, thread
@@ -70,13 +96,21 @@ struct Row {
   template <int THREADS, class F>
   __device__ __forceinline__ void each(F f) const {
     if (single >= 0) f(p[single], single);
-    for (int i = threadIdx.x; i < groups; i += THREADS) {
-      const float4 v = mid[i];
-      const int at = head + 4 * i;
-      f(v.x, at);
-      f(v.y, at + 1);
-      f(v.z, at + 2);
-      f(v.w, at + 3);
+    constexpr int kAhead = 4;         // loads in flight: they come from L2
+    for (int i = threadIdx.x; i < groups; i += kAhead * THREADS) {
+      float4 v[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (i + k * THREADS < groups) v[k] = mid[i + k * THREADS];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (i + k * THREADS >= groups) break;
+        const int at = head + 4 * (i + k * THREADS);
+        f(v[k].x, at);
+        f(v[k].y, at + 1);
+        f(v[k].z, at + 2);
+        f(v[k].w, at + 3);
+      }
     }
   }
 };
@@ -113,16 +147,76 @@ __device__ uint32_t nth_key(const Row& row, Select& s, unsigned r, unsigned& res
   return prefix;
 }
 
+// Puts the pairs of the entries that wanted() lets in into s.pair, in an order that
+// depends on the row alone, and returns how many there are (the first kCandidates
+// are kept); threads with look = false have none.  A thread marks 64 of its
+// entries at a time, the marks are counted over the block, and only the marked
+// entries are read again: a counter in shared memory that every pair takes a turn
+// at cost 12,000 cycles for 228 pairs.
+template <int THREADS, uint32_t NAN_KEY, class Wanted>
+__device__ int collect(const Row& row, Select& s, bool look, Wanted wanted) {
+  constexpr int kWarps = THREADS / 32, kAhead = 4, kRound = 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int total = 0;
+  for (int g0 = threadIdx.x; g0 - (int)threadIdx.x < max(row.groups, 1); g0 += kRound * THREADS) {
+    unsigned long long marks = 0;
+    const bool lone = look && g0 == threadIdx.x && row.single >= 0 &&
+                      wanted(row.p[row.single], row.single);
+    if (look)
+#pragma unroll
+      for (int k0 = 0; k0 < kRound; k0 += kAhead) {
+        if (g0 + k0 * THREADS >= row.groups) break;
+        float4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+          if (g0 + (k0 + k) * THREADS < row.groups) v[k] = row.mid[g0 + (k0 + k) * THREADS];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int g = g0 + (k0 + k) * THREADS, at = row.head + 4 * g;
+          if (g >= row.groups) break;
+          const unsigned four = (unsigned)wanted(v[k].x, at) | (unsigned)wanted(v[k].y, at + 1) << 1 |
+                                (unsigned)wanted(v[k].z, at + 2) << 2 |
+                                (unsigned)wanted(v[k].w, at + 3) << 3;
+          marks |= (unsigned long long)four << 4 * (k0 + k);
+        }
+      }
+    const int mine = __popcll(marks) + (int)lone;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int before = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += before;
+    }
+    __syncthreads();                  // s.warp has been read
+    if (lane == 31) s.warp[warp] = upto;
+    __syncthreads();
+    const int w = lane < kWarps ? s.warp[lane] : 0;
+    int at = total + upto - mine + __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
+    total += __reduce_add_sync(0xffffffffu, w);
+    if (lone && at < kCandidates)
+      s.pair[at] = pair_key(row.p[row.single], row.single, NAN_KEY);
+    at += lone;
+    for (; marks; marks &= marks - 1, ++at) {
+      const int k = __ffsll(marks) - 1;
+      const int i = row.head + 4 * (g0 + (k >> 2) * THREADS) + (k & 3);
+      if (at < kCandidates) s.pair[at] = pair_key(row.p[i], i, NAN_KEY);
+    }
+  }
+  __syncthreads();
+  return total;
+}
+
 // Puts the row's K best pairs, and perhaps more of its best, into s.pair and
 // returns how many (K <= V).  With SUM, top and sum come to hold the row's largest
 // number and the sum of exp(v - top).
 //
-// One pass over the row gives every thread its largest entry.  The ceil(K / warps)
-// th largest of a warp's, the smallest of that over the warps, is a value that at
-// least K entries reach, and few more do: about 3 K of 50304 at K = 64 and 32
-// warps.  The threads whose largest reaches it read their entries again (from
-// L2) and keep those that do.  Where too many do (long runs of one value, or large
-// ones crowded into a few threads), the exact K-th pair is found digit by digit.
+// One pass over the row gives every thread its largest entry.  Of the jth largest
+// of each warp's, the mth largest over the warps is a value tau that at least
+// j m >= K entries reach, and few more do where m is about 2/3 of the warps: about
+// 125 entries at K = 64 (with j = K / warps and the smallest over the warps it was
+// 228).  The threads whose largest reaches tau read their entries again (from L2)
+// and keep those that do.  Where too many do (long runs of one value, or large ones
+// crowded into a few threads), the exact K-th pair is found digit by digit.
 template <int THREADS, uint32_t NAN_KEY, bool SUM>
 __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& sum) {
   constexpr int kWarps = THREADS / 32;
@@ -134,7 +228,7 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
   auto larger = [](float a, float b) {
     return NAN_KEY == kNanHighest ? max_nan(a, b) : fmaxf(a, b);
   };
-#pragma unroll 4
+#pragma unroll(SUM ? 8 : 4)
   for (int i = threadIdx.x; i < row.groups; i += THREADS) {
     const float4 v = row.mid[i];
     const float n = larger(larger(m, v.x), larger(larger(v.y, v.z), v.w));
@@ -149,56 +243,48 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
     }
     m = n;
   }
-  // the warp's lanes in descending order of their largest entries
-  float o = m != m ? INFINITY : m;
-#pragma unroll
-  for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      const float other = __shfl_xor_sync(0xffffffffu, o, j);
-      const bool first = (lane & j) == 0, down = (lane & k) == 0;
-      o = first == down ? fmaxf(o, other) : fminf(o, other);
-    }
-  const float reach = __shfl_sync(0xffffffffu, o, (K + kWarps - 1) / kWarps - 1);
+  // the nth largest of the warp's lanes (of their largest entries)
+  uint32_t o = value_key(m, NAN_KEY);
+  constexpr int kMost = kWarps * 2 / 3;
+  const int nth = (K + kMost - 1) / kMost < 32 ? (K + kMost - 1) / kMost : 32;
+  const int mth = (K + nth - 1) / nth;         // <= warps: K <= 32 warps
+  uint32_t reach = __reduce_max_sync(0xffffffffu, o);
   if (SUM) {
-    const float w = __shfl_sync(0xffffffffu, o, 0);
+    const float w = key_float(reach);
     part *= m == -INFINITY || m == w ? 1.0f : expf(m - w);
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) part += __shfl_xor_sync(0xffffffffu, part, k);
+    part = warp_sum(part);
     if (lane == 0) {
       s.top[warp] = w;
       s.sum[warp] = part;
     }
   }
-  if (lane == 0) s.tau[warp] = reach;
-  if (threadIdx.x == 0) s.count = 0;
-  __syncthreads();
-  float tau = INFINITY;
-  for (int w = 0; w < kWarps; ++w) tau = fminf(tau, s.tau[w]);
-  if (SUM) {
-    top = -INFINITY;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s.top[w]);
-    sum = 0.f;
-    for (int w = 0; w < kWarps; ++w)
-      sum += s.top[w] == top ? s.sum[w] : s.sum[w] * expf(s.top[w] - top);
+  if (nth <= 4) {
+    for (int k = 1; k < nth; ++k) {      // without the lane that had it
+      if (lane == __ffs(__ballot_sync(0xffffffffu, o == reach)) - 1) o = 0;
+      reach = __reduce_max_sync(0xffffffffu, o);
+    }
+  } else {
+    reach = __shfl_sync(0xffffffffu, descending(o), nth - 1);
   }
-  auto keep = [&](float v, int i) {
-    const unsigned at = atomicAdd(&s.count, 1u);
-    if (at < kCandidates) s.pair[at] = pair_key(v, i, NAN_KEY);
-  };
+  if (lane == 0) s.reach[warp] = reach;
+  __syncthreads();
+  const float tau = key_float(
+      __shfl_sync(0xffffffffu, descending(lane < kWarps ? s.reach[lane] : 0u), mth - 1));
+  if (SUM) {
+    const float w = lane < kWarps ? s.top[lane] : -INFINITY;
+    top = key_float(__reduce_max_sync(0xffffffffu, value_key(w, NAN_KEY)));
+    sum = warp_sum(lane < kWarps ? s.sum[lane] * (w == top ? 1.0f : expf(w - top)) : 0.f);
+  }
   // all pairs of a short row, else those that reach tau (NaN counts as reaching
   // where it is the highest; where it is the lowest, tau = -inf is left to the
   // digits, which know where it stands)
   const bool all = row.V <= kCandidates && tau == -INFINITY;
-  const bool plain = all || tau > -INFINITY || NAN_KEY == kNanHighest;
-  if (plain && (all || !(m < tau)))
-    row.each<THREADS>([&](float v, int i) {
-      if (all || (NAN_KEY == kNanHighest ? !(v < tau) : v >= tau)) keep(v, i);
+  if (all || tau > -INFINITY || NAN_KEY == kNanHighest) {
+    const int n = collect<THREADS, NAN_KEY>(row, s, all || !(m < tau), [&](float v, int) {
+      return all || (NAN_KEY == kNanHighest ? !(v < tau) : v >= tau);
     });
-  __syncthreads();
-  const unsigned n = s.count;
-  if (plain && n <= kCandidates) return (int)n;
-  __syncthreads();
+    if (n <= kCandidates) return n;
+  }
   unsigned rest, none;
   const uint32_t cut = nth_key<THREADS>(
       row, s, K, rest, [](float v, int) { return value_key(v, NAN_KEY); },
@@ -206,49 +292,72 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
   const uint32_t last = ~nth_key<THREADS>(
       row, s, rest, none, [](float, int i) { return ~(uint32_t)i; },
       [&](float v, int) { return value_key(v, NAN_KEY) == cut; });
-  if (threadIdx.x == 0) s.count = 0;
-  __syncthreads();
-  row.each<THREADS>([&](float v, int i) {
+  return collect<THREADS, NAN_KEY>(row, s, true, [&](float v, int i) {
     const uint32_t k = value_key(v, NAN_KEY);
-    if (k > cut || (k == cut && (uint32_t)i <= last)) keep(v, i);
+    return k > cut || (k == cut && (uint32_t)i <= last);
   });
-  __syncthreads();
-  return K;
 }
 
-// Calls put(rank, pair) for the K best of the n pairs in s.pair (all different).
-// Up to 256 of them are counted against each other; more are sorted, a pair a
-// thread, where there are threads for that.
-template <int THREADS, class F>
-__device__ void in_order(Select& s, int n, int K, F put) {
+// Sorts the first SIZE pairs (0 past n) in descending order, one a thread, by the
+// first SIZE threads of the block; returns this thread's.
+template <int SIZE>
+__device__ __forceinline__ uint64_t sorted_pair(Select& s, int n) {
   const int t = threadIdx.x;
-  if (n <= 256 || n > THREADS) {
-    for (int i = t; i < n; i += THREADS) {
-      const uint64_t mine = s.pair[i];
-      int rank = 0;
-#pragma unroll 8
-      for (int j = 0; j < n; ++j) rank += s.pair[j] > mine;
-      if (rank < K) put(rank, mine);
-    }
-    return;
-  }
-  int size = 512;
-  while (size < n) size <<= 1;
   uint64_t mine = t < n ? s.pair[t] : 0;
-  for (int k = 2; k <= size; k <<= 1)
+#pragma unroll
+  for (int k = 2; k <= SIZE; k <<= 1)
+#pragma unroll
     for (int j = k >> 1; j > 0; j >>= 1) {
       uint64_t other;
       if (j >= 32) {
-        __syncthreads();
-        if (t < size) s.pair[t] = mine;
-        __syncthreads();
-        other = t < size ? s.pair[t ^ j] : 0;
+        asm volatile("bar.sync 1, %0;" ::"n"(SIZE) : "memory");
+        s.pair[t] = mine;
+        asm volatile("bar.sync 1, %0;" ::"n"(SIZE) : "memory");
+        other = s.pair[t ^ j];
       } else {
         other = __shfl_xor_sync(0xffffffffu, mine, j);
       }
       const bool first = (t & j) == 0, down = (t & k) == 0;
       mine = (first == down) == (mine > other) ? mine : other;
     }
+  return mine;
+}
+
+// Calls put(rank, pair) for the K best of the n pairs in s.pair (all different).
+// Up to 64 of them are counted against each other, a few neighbouring threads
+// sharing a pair's count; more are sorted, a pair a thread (n^2 / 32 reads of
+// shared memory by a warp against log^2 n / 2 exchanges), or counted where threads
+// are too few.
+template <int THREADS, class F>
+__device__ __forceinline__ void in_order(Select& s, int n, int K, F put) {
+  const int t = threadIdx.x;
+  if (n <= 64 || n > THREADS) {
+    int share = 1;
+    while (share < 32 && n * share * 2 <= THREADS) share <<= 1;
+    const int lane = t & (share - 1);
+    for (int at = 0; at < n; at += THREADS / share) {
+      const int i = at + t / share;
+      const uint64_t mine = i < n ? s.pair[i] : 0;
+      int rank = 0;
+#pragma unroll 4
+      for (int j = lane; j < n; j += share) rank += s.pair[j] > mine;
+      for (int o = 1; o < share; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      if (i < n && lane == 0 && rank < K) put(rank, mine);
+    }
+    return;
+  }
+  uint64_t mine = 0;
+  if (n <= 128) {
+    if (t < 128) mine = sorted_pair<128>(s, n);
+  } else if (n <= 256) {
+    if (t < 256) mine = sorted_pair<256>(s, n);
+  } else if (THREADS > 256) {
+    if (n <= 512) {
+      if (t < 512) mine = sorted_pair<512>(s, n);
+    } else {
+      mine = sorted_pair<THREADS>(s, n);
+    }
+  }
   if (t < K) put(t, mine);
 }
 
@@ -262,26 +371,23 @@ __global__ void __launch_bounds__(THREADS, 2048 / THREADS)
   float top, sum;
   const int n = best_pairs<THREADS, kNanHighest, false>(row, K, s, top, sum);
   in_order<THREADS>(s, n, K, [&](int rank, uint64_t pair) {
-    const uint32_t i = key_index(pair);
+    const uint32_t i = key_index(pair), v = (uint32_t)(pair >> 32);
     ids[at * K + rank] = i;
-    values[at * K + rank] = row.p[i];
+    // a key gives its value back, but for the sign of zero and a NaN's bits
+    values[at * K + rank] = v == 0x80000000u || v == kNanHighest ? row.p[i] : key_float(v);
   });
 }
 
 // One selection step.  A cluster takes a batch item; its rows, or `parts` pieces
-// of each where there are few, go to its blocks in turn.  Each leaves the piece's
-// best W pairs, its largest logit and its sum of exponentials in shared memory,
-// and the first block merges them all:
+// of each where there are few, go to its blocks in turn.  Each sends the piece's
+// best W pairs, its largest logit and its sum of exponentials to the first block,
+// which merges them all:
 //   score = scores[w] + ((z - top_w) - log sum_w)
-struct Piece {
-  uint64_t pair[kMaxBeams];           // 0: no pair
-  float top, sum;
-};
+constexpr int kMostPieces = kMaxBeams > kClusterBlocks ? kMaxBeams : kClusterBlocks;
 struct Merge {
-  Select s;
-  Piece piece[2];                     // pieces rank, rank + blocks
-  uint64_t first[kMaxBeams * kMaxBeams], second[kMaxBeams * kMaxBeams];
-  float top[kMaxBeams], log_sum[kMaxBeams];
+  uint64_t pair[kMostPieces * kMaxBeams];       // 0: no pair
+  float top[kMostPieces], sum[kMostPieces];
+  uint64_t key[kMostPieces * kMaxBeams];
 };
 
 template <int THREADS>
@@ -291,92 +397,87 @@ __global__ void __launch_bounds__(THREADS)
                        const float* __restrict__ logits, int64_t ld,
                        const float* __restrict__ scores, const uint32_t* __restrict__ finished,
                        int W, int V, int parts, uint32_t stop) {
-  __shared__ Merge s;
+  __shared__ Select s;
+  __shared__ Merge s_merge;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
+  auto started = cluster.barrier_arrive();
+  bool met = false;                  // the cluster's blocks have all started
+  auto meet = [&] {
+    if (!met) cluster.barrier_wait(std::move(started));
+    met = true;
+  };
   const int rank = cluster.block_rank(), blocks = cluster.num_blocks();
   const int64_t b = blockIdx.x / blocks;
-  const int t = threadIdx.x, pieces = W * parts;
+  const int t = threadIdx.x, pieces = W * parts, n = pieces * W;
+  Merge* merge = cluster.map_shared_rank(&s_merge, 0);
+  // a thread of the merge: proposal r of piece t / W
+  const int my_piece = t / W, my_beam = my_piece / parts, my_rank = t - my_piece * W;
+  const bool mine = rank == 0 && t < n;
+  const float score = mine ? scores[b * W + my_beam] : 0.f;
+  const bool done = mine && finished && finished[b * W + my_beam];
   // a piece's length, a multiple of 4 so that all start where the first does
   const int length = parts == 1 ? V : ((V + parts - 1) / parts + 3) / 4 * 4;
-  for (int q = rank, turn = 0; q < pieces; q += blocks, ++turn) {
-    Piece& piece = s.piece[turn];
+  for (int q = rank; q < pieces; q += blocks) {
     const int w = q / parts, from = (q - w * parts) * length;
-    const int n = min(length, V - from), K = min(W, n);
-    if (t < W) piece.pair[t] = 0;
-    __syncthreads();
+    const int len = min(length, V - from), K = min(W, len);
     if (finished && finished[b * W + w]) continue;
-    const Row row(logits + (b * W + w) * ld + from, n);
+    const Row row(logits + (b * W + w) * ld + from, len);
     float top, sum;
-    const int found = best_pairs<THREADS, kNanLowest, true>(row, K, s.s, top, sum);
-    in_order<THREADS>(s.s, found, K, [&](int r, uint64_t pair) {
-      piece.pair[r] = pair - (uint32_t)from;        // the inverted index of the row
+    const int found = best_pairs<THREADS, kNanLowest, true>(row, K, s, top, sum);
+    meet();
+    in_order<THREADS>(s, found, K, [&](int r, uint64_t pair) {
+      merge->pair[q * W + r] = pair - (uint32_t)from;          // the inverted index of the row
     });
+    if (t < W && t >= K) merge->pair[q * W + t] = 0;
     if (t == 0) {
-      piece.top = top;
-      piece.sum = sum;
+      merge->top[q] = top;
+      merge->sum[q] = sum;
     }
-    __syncthreads();
+    __syncthreads();                 // s is used again
   }
+  meet();
   cluster.sync();
-  if (rank == 0) {
-    auto piece_of = [&](int q) -> const Piece* {
-      return cluster.map_shared_rank(&s.piece[q / blocks], q % blocks);
-    };
-    if (t < W) {
+  if (rank != 0) return;
+  // Every beam's W best pairs of all its pieces compete: by score, then the lower
+  // beam, then the better pair of it.
+  uint64_t pair = 0;
+  uint64_t key = 0;                  // no proposal
+  if (mine) {
+    float c = -INFINITY;
+    int place = my_rank;             // among the beam's
+    if (done) {
+      c = my_piece == my_beam * parts && my_rank == 0 ? score : -INFINITY;
+    } else {
+      pair = s_merge.pair[t];
+      const int first = my_beam * parts;
       float top = -INFINITY, sum = 0.f;
-      if (!(finished && finished[b * W + t])) {
-        for (int k = 0; k < parts; ++k) top = fmaxf(top, piece_of(t * parts + k)->top);
-        for (int k = 0; k < parts; ++k) {
-          const Piece* p = piece_of(t * parts + k);
-          sum += p->top == top ? p->sum : p->sum * expf(p->top - top);
-        }
+      for (int k = first; k < first + parts; ++k) top = fmaxf(top, s_merge.top[k]);
+      for (int k = first; k < first + parts; ++k)
+        sum += s_merge.sum[k] * (s_merge.top[k] == top ? 1.0f : expf(s_merge.top[k] - top));
+      if (pair) c = score + ((key_value(pair) - top) - logf(sum));
+      if (parts > 1) {
+        place = 0;
+        for (int k = first * W; k < (first + parts) * W; ++k) place += s_merge.pair[k] > pair;
       }
-      s.top[t] = top;
-      s.log_sum[t] = logf(sum);
     }
-    __syncthreads();
-    // Every beam's W best pairs of all its pieces compete: by score, then the lower
-    // beam, then the better pair of it.
-    const int n = pieces * W;
-    for (int i = t; i < n; i += THREADS) {
-      const int q = i / W, r = i - q * W, w = q / parts;
-      const float score = scores[b * W + w];
-      uint64_t pair = piece_of(q)->pair[r];
-      float c = -INFINITY;
-      if (finished && finished[b * W + w]) {
-        if (q == w * parts && r == 0) {
-          c = score;
-          pair = 1;
-        }
-      } else if (pair) {
-        const float z = logits[(b * W + w) * ld + key_index(pair)];
-        c = score + ((z - s.top[w]) - s.log_sum[w]);
-      }
-      s.first[i] = (uint64_t)value_key(c, kNanLowest) << 32 | (uint32_t)(kMaxBeams - w);
-      s.second[i] = pair;
-    }
-    __syncthreads();
-    for (int i = t; i < n; i += THREADS) {
-      const uint64_t f = s.first[i], g = s.second[i];
-      int place = 0;
-      for (int j = 0; j < n; ++j) {
-        const uint64_t fj = s.first[j], gj = s.second[j];
-        place += fj > f || (fj == f && (gj > g || (gj == g && j < i)));
-      }
-      if (place >= W) continue;
-      const int w = i / W / parts;
-      const bool done = finished && finished[b * W + w];
-      const uint32_t token = done ? stop : g ? key_index(g) : 0u;
-      const uint32_t k = (uint32_t)(f >> 32);
-      const int64_t o = b * W + place;
-      new_scores[o] = __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-      parents[o] = w;
-      new_tokens[o] = token;
-      if (new_finished) new_finished[o] = done || token == stop;
-    }
+    if (place < W && !(done && my_piece != my_beam * parts))
+      key = (uint64_t)value_key(c, kNanLowest) << 32 | (uint32_t)(kMaxBeams - my_beam) << 8 |
+            (uint32_t)(255 - place);
+    s_merge.key[t] = key;
   }
-  cluster.sync();                     // the pieces stay until they have been read
+  __syncthreads();
+  if (!mine || key == 0) return;
+  int place = 0;
+#pragma unroll 8
+  for (int j = 0; j < n; ++j) place += s_merge.key[j] > key;
+  if (place >= W) return;
+  const uint32_t token = done ? stop : pair ? key_index(pair) : 0u;
+  const int64_t o = b * W + place;
+  new_scores[o] = key_value(key);
+  parents[o] = my_beam;
+  new_tokens[o] = token;
+  if (new_finished) new_finished[o] = done || token == stop;
 }
 
 struct StateTable {
