@@ -433,7 +433,7 @@ int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0, const flo
 int wxx_gated_recurrence_step(float* state, const float* x, int64_t x_ld, const float* gate,
                               int64_t g_ld, int64_t B, int64_t D, int64_t H);
 /* Distillation from a teacher's K stored logits per row: loss (N) = tau^2 KL(softmax(top / tau) ||
- * softmax(logits / tau)) and the row statistics stats (N, 2) of the backward; logits (N, V) with
+ * softmax(logits / tau)) and the row statistics stats (N, 4) of the backward; logits (N, V) with
  * row stride ld, top and ids (N, K), 1 <= K <= 1024.  A stored logit of -inf is an absent entry; a
  * row without entries has loss 0; an id >= V is an absent entry and sets the device error word. */
 int wxx_distill_loss(float* loss, float* stats, const float* logits, int64_t ld, const float* top,

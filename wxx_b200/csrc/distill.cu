@@ -10,27 +10,24 @@
 // vocabulary raises WXX_DEV_ERR_BAD_INDEX and its entry counts as not there.
 
 #include <cuda_runtime.h>
+#include <cooperative_groups.h>
 #include <stdint.h>
 
+#include <cmath>
+
 #include "common.cuh"
+#include "rows.cuh"
 
 namespace {
 
-constexpr int kT = 256;
-constexpr int kMaxK = 1024;
+using wxx_rows::Row;
+using wxx_rows::warp_sum;
 
-template <int THREADS>
-__device__ __forceinline__ float block_sum(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.f;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) v += red[w];
-  __syncthreads();
-  return v;
-}
+constexpr int kT = 256;
+constexpr int kWarps = kT / 32;
+constexpr int kMaxK = 1024;
+constexpr int kMaxParts = 8;          // blocks that share a row, at most
+constexpr int kStats = 4;             // largest logit, sum of exp; the teacher's two
 
 // The maximum, NaN if there is one.
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -38,134 +35,272 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-
-template <int THREADS>
-__device__ __forceinline__ float block_max(float v, float* red) {
+__device__ __forceinline__ float warp_max_nan(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+// Over the block, in an order that depends on nothing but the values' places.
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = warp_sum(v);
+  __syncthreads();                    // red has been read
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = red[0];
 #pragma unroll
-  for (int w = 1; w < THREADS / 32; ++w) v = max_nan(v, red[w]);
+  for (int w = 1; w < kWarps; ++w) v += red[w];
+  return v;
+}
+__device__ __forceinline__ float block_max_nan(float v, float* red) {
+  v = warp_max_nan(v);
   __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) v = max_nan(v, red[w]);
   return v;
 }
 
-// The teacher's side of a row: s_t[k] = (t_k - max) / tau, s_p[k] = p_k; returns
-// whether the row has an entry, and log of the sum in log_sum.
-template <int THREADS>
-__device__ bool teacher_row(const float* __restrict__ top, const uint32_t* __restrict__ ids, int K,
-                            uint32_t V, float inv_tau, float* s_t, float* s_p, float* red,
-                            float& log_sum, int* err) {
-  float m = -INFINITY;
-  for (int k = threadIdx.x; k < K; k += THREADS) {
-    float t = top[k];
-    if (t != -INFINITY && ids[k] >= V) {
-      wxx_device_fail(err, WXX_DEV_ERR_BAD_INDEX);
-      t = -INFINITY;
-    }
-    s_t[k] = t;
-    m = max_nan(m, t);
-  }
-  m = block_max<THREADS>(m, red);
-  const bool some = m != -INFINITY;
-  float s = 0.f;
-  for (int k = threadIdx.x; k < K; k += THREADS) {
-    const float t = some ? (s_t[k] - m) * inv_tau : 0.f;
-    const float e = some ? expf(t) : 0.f;
-    s_t[k] = t;
-    s_p[k] = e;
-    s += e;
-  }
-  s = block_sum<THREADS>(s, red);
-  log_sum = some ? logf(s) : 0.f;
-  const float inv = some ? 1.0f / s : 0.f;
-  for (int k = threadIdx.x; k < K; k += THREADS) s_p[k] *= inv;
-  __syncthreads();
-  return some;
+// 2^((v - m) c), c = log2(e) / tau: exp of the logits' distance over tau.
+__device__ __forceinline__ float scaled_exp(float v, float m, float c) {
+  return fast_exp2((v - m) * c);
 }
 
+// A stored teacher logit, -inf where the entry is not there.
+__device__ __forceinline__ float stored(float t, uint32_t id, uint32_t V, int* err) {
+  if (t == -INFINITY || id < V) return t;
+  wxx_device_fail(err, WXX_DEV_ERR_BAD_INDEX);
+  return -INFINITY;
+}
+
+struct Sum {
+  float top, sum;                     // the largest so far, the sum of exp(v - top)
+};
+__device__ __forceinline__ Sum plus(Sum a, Sum b, float c) {
+  const float top = max_nan(a.top, b.top);
+  return {top, (a.top == top ? a.sum : a.sum * scaled_exp(a.top, top, c)) +
+                   (b.top == top ? b.sum : b.sum * scaled_exp(b.top, top, c))};
+}
+
+// One pass over a row's piece: 16 logits at a time, their largest against the
+// thread's so far, one rescaling of its sum where they exceed it.  4 bytes and
+// one exponential a logit; the loads are what bounds it.
+__device__ Sum piece_sum(const Row& row, float c, Sum* red) {
+  Sum s{-INFINITY, 0.f};
+  auto add = [&](float v) {
+    if (v != -INFINITY) s = plus(s, {v, 1.0f}, c);
+  };
+  if (row.single >= 0) add(row.p[row.single]);
+  constexpr int kAhead = 4;
+  int i = threadIdx.x;
+  for (; i + (kAhead - 1) * kT < row.groups; i += kAhead * kT) {
+    float4 v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) v[k] = row.mid[i + k * kT];
+    float n = s.top;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      n = max_nan(max_nan(n, max_nan(v[k].x, v[k].y)), max_nan(v[k].z, v[k].w));
+    if (n == -INFINITY) continue;
+    float e = s.top == n ? s.sum : s.sum * scaled_exp(s.top, n, c);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      e += (scaled_exp(v[k].x, n, c) + scaled_exp(v[k].y, n, c)) +
+           (scaled_exp(v[k].z, n, c) + scaled_exp(v[k].w, n, c));
+    s = {n, e};
+  }
+  for (; i < row.groups; i += kT) {
+    const float4 v = row.mid[i];
+    const float n = max_nan(max_nan(s.top, max_nan(v.x, v.y)), max_nan(v.z, v.w));
+    if (n == -INFINITY) continue;
+    s = {n, (s.top == n ? s.sum : s.sum * scaled_exp(s.top, n, c)) +
+                ((scaled_exp(v.x, n, c) + scaled_exp(v.y, n, c)) +
+                 (scaled_exp(v.z, n, c) + scaled_exp(v.w, n, c)))};
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    s = plus(s, {__shfl_xor_sync(0xffffffffu, s.top, o), __shfl_xor_sync(0xffffffffu, s.sum, o)}, c);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = red[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) s = plus(s, red[w], c);
+  return s;
+}
+
+// A row's blocks (a cluster where there are several) each take a piece of it; the
+// first has the teacher's entries meanwhile, then joins the pieces' sums.
 __global__ void __launch_bounds__(kT)
     distill_forward_kernel(float* __restrict__ loss, float* __restrict__ stats,
                            const float* __restrict__ logits, int64_t ld,
                            const float* __restrict__ top, const uint32_t* __restrict__ ids, int V,
-                           int K, float inv_tau, float tau2, int* err) {
-  __shared__ float s_t[kMaxK], s_p[kMaxK], red[kT / 32];
-  const int64_t row = blockIdx.x;
-  const float* z = logits + row * ld;
-  float log_sum;
-  const bool some = teacher_row<kT>(top + row * K, ids + row * K, K, V, inv_tau, s_t, s_p, red,
-                                    log_sum, err);
-  float m = -INFINITY;
-  for (int c = threadIdx.x; c < V; c += kT) m = max_nan(m, z[c]);
-  m = block_max<kT>(m, red);
-  float s = 0.f;
-  for (int c = threadIdx.x; c < V; c += kT) s += expf((z[c] - m) * inv_tau);
-  s = block_sum<kT>(s, red);
-  const float log_s = logf(s);
-  float part = 0.f;
-  for (int k = threadIdx.x; k < K; k += kT) {
-    const float p = s_p[k];
-    if (!(p == 0.f))
-      part += p * ((s_t[k] - log_sum) - ((z[ids[row * K + k]] - m) * inv_tau - log_s));
+                           int K, int parts, int length, float inv_tau, float c, float tau2,
+                           int* err) {
+  namespace cg = cooperative_groups;
+  __shared__ float s_t[kMaxK], red[kWarps];
+  __shared__ Sum s_red[kWarps], s_part[kMaxParts];
+  const int part = blockIdx.x % parts;
+  const int64_t at = blockIdx.x / parts;
+  const float* z = logits + at * ld;
+  if (parts > 1) cg::this_cluster().barrier_arrive();
+  float t_top = -INFINITY, t_sum = 0.f;
+  if (part == 0) {
+    for (int k = threadIdx.x; k < K; k += kT) {
+      const float t = stored(top[at * K + k], ids[at * K + k], V, err);
+      s_t[k] = t;
+      t_top = max_nan(t_top, t);
+    }
+    t_top = block_max_nan(t_top, red);
+    for (int k = threadIdx.x; k < K; k += kT)
+      if (t_top != -INFINITY) t_sum += expf((s_t[k] - t_top) * inv_tau);
+    t_sum = block_sum(t_sum, red);
   }
-  part = block_sum<kT>(part, red);
+  const int from = part * length;
+  Sum s = piece_sum(Row(z + from, min(length, V - from)), c, s_red);
+  if (parts > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.barrier_wait();          // the first block is there
+    if (threadIdx.x == 0) *cluster.map_shared_rank(&s_part[part], 0) = s;
+    cluster.sync();
+    if (part != 0) return;
+    s = s_part[0];
+    for (int k = 1; k < parts; ++k) s = plus(s, s_part[k], c);
+  }
+  const bool some = t_top != -INFINITY;
+  const float log_s = logf(s.sum), log_t = logf(t_sum), inv = 1.0f / t_sum;
+  float sum = 0.f;
+  if (some)
+    for (int k = threadIdx.x; k < K; k += kT) {
+      const float t = (s_t[k] - t_top) * inv_tau, p = expf(t) * inv;
+      if (!(p == 0.f))
+        sum += p * ((t - log_t) - ((z[ids[at * K + k]] - s.top) * inv_tau - log_s));
+    }
+  sum = block_sum(sum, red);
   if (threadIdx.x == 0) {
-    loss[row] = some ? tau2 * part : 0.f;
-    stats[2 * row] = m;
-    stats[2 * row + 1] = s;
+    loss[at] = some ? tau2 * sum : 0.f;
+    float* o = stats + at * kStats;
+    o[0] = s.top;
+    o[1] = s.sum;
+    o[2] = t_top;
+    o[3] = t_sum;
   }
 }
 
+// dz over a piece of a row: g tau q everywhere, then the stored entries that lie in
+// it.  8 bytes a logit.  kAligned: logits and dz have the same place in their 16
+// bytes, so both go four at a time.
+template <bool kAligned>
 __global__ void __launch_bounds__(kT)
     distill_backward_kernel(float* __restrict__ dz, const float* __restrict__ grad,
                             const float* __restrict__ logits, int64_t ld,
                             const float* __restrict__ top, const uint32_t* __restrict__ ids,
-                            const float* __restrict__ stats, int V, int K, float tau,
-                            float inv_tau, int* err) {
-  __shared__ float s_t[kMaxK], s_p[kMaxK], red[kT / 32];
-  const int64_t row = blockIdx.x;
-  const float* z = logits + row * ld;
-  const uint32_t* id = ids + row * K;
-  float* out = dz + row * V;
-  float log_sum;
-  const bool some = teacher_row<kT>(top + row * K, id, K, V, inv_tau, s_t, s_p, red, log_sum, err);
-  const float m = stats[2 * row], inv = 1.0f / stats[2 * row + 1], g = grad[row] * tau;
-  for (int c = threadIdx.x; c < V; c += kT)
-    out[c] = some ? g * (expf((z[c] - m) * inv_tau) * inv) : 0.f;
-  __syncthreads();
-  // the first entry of an id takes all that have it
-  for (int k = threadIdx.x; k < K; k += kT) {
-    if (s_p[k] == 0.f || !some) continue;
-    const uint32_t c = id[k];
-    float p = s_p[k];
-    bool first = true;
-    for (int j = 0; j < k; ++j) first = first && !(id[j] == c && s_p[j] != 0.f);
-    if (!first) continue;
-    for (int j = k + 1; j < K; ++j)
-      if (id[j] == c) p += s_p[j];
-    out[c] = g * (expf((z[c] - m) * inv_tau) * inv - p);
+                            const float* __restrict__ stats, int V, int K, int parts, int length,
+                            float tau, float inv_tau, float c, int* err) {
+  __shared__ float s_p[kMaxK];
+  __shared__ uint32_t s_id[kMaxK];
+  const int part = blockIdx.x % parts;
+  const int64_t at = blockIdx.x / parts;
+  const int from = part * length, n = min(length, V - from);
+  const float* z = logits + at * ld + from;
+  float* out = dz + at * V + from;
+  const float4 st = *reinterpret_cast<const float4*>(stats + at * kStats);
+  const bool some = st.w != 0.f;     // the teacher's sum: 0 without entries
+  const float m = st.x, inv = 1.0f / st.y, g = grad[at] * tau;
+  if (some) {
+    const float inv_t = 1.0f / st.w;
+    for (int k = threadIdx.x; k < K; k += kT) {
+      const uint32_t j = ids[at * K + k];
+      const float t = stored(top[at * K + k], j, V, part == 0 ? err : nullptr);
+      s_id[k] = j;
+      s_p[k] = expf((t - st.z) * inv_tau) * inv_t;
+    }
   }
+  auto value = [&](float v) { return some ? g * (scaled_exp(v, m, c) * inv) : 0.f; };
+  if (kAligned) {
+    const Row row(z, n);
+    if (row.single >= 0) out[row.single] = value(z[row.single]);
+    float4* to = reinterpret_cast<float4*>(out + row.head);
+    constexpr int kAhead = 4;
+    int i = threadIdx.x;
+    for (; i + (kAhead - 1) * kT < row.groups; i += kAhead * kT) {
+      float4 v[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) v[k] = row.mid[i + k * kT];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        to[i + k * kT] = make_float4(value(v[k].x), value(v[k].y), value(v[k].z), value(v[k].w));
+    }
+    for (; i < row.groups; i += kT) {
+      const float4 v = row.mid[i];
+      to[i] = make_float4(value(v.x), value(v.y), value(v.z), value(v.w));
+    }
+  } else {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += kT) out[i] = value(z[i]);
+  }
+  if (!some) return;
+  __syncthreads();                   // the stored entries overwrite what is there
+  for (int k = threadIdx.x; k < K; k += kT) {
+    const uint32_t j = s_id[k];
+    if (j < (uint32_t)from || j - (uint32_t)from >= (uint32_t)n) continue;
+    // the first entry of an id takes all that have it
+    float p = 0.f;
+    bool first = true;
+#pragma unroll 8
+    for (int o = 0; o < K; ++o) {
+      const bool same = s_id[o] == j;
+      first = first && !(same && o < k);
+      p += same && o >= k ? s_p[o] : 0.f;
+    }
+    if (first) out[j - from] = g * (scaled_exp(z[j - from], m, c) * inv - p);
+  }
+}
+
+int check_sizes(const char* what, int64_t N, int64_t V, int K, float tau) {
+  WXX_REQUIRE(N >= 0 && N < (int64_t(1) << 28) && V >= 1 && V < (int64_t(1) << 31) - 4 * kT,
+              "%s: bad sizes", what);
+  WXX_REQUIRE(K >= 1 && K <= kMaxK, "%s: %d stored logits outside [1, %d]", what, K, kMaxK);
+  WXX_REQUIRE(tau > 0.f && tau < INFINITY, "%s: the temperature must be positive", what);
+  return WXX_OK;
+}
+
+// Pieces of a row, so that few long rows still give every SM two blocks; a piece is
+// a multiple of 4 logits, at least 2048.
+void split_row(int64_t N, int64_t V, int& parts, int& length) {
+  const int64_t wanted = (2 * wxx::num_sms() + N - 1) / N, most = (V + 2047) / 2048;
+  int64_t n = wanted < most ? wanted : most;
+  n = n < kMaxParts ? n : kMaxParts;
+  length = (int)(((V + n - 1) / n + 3) / 4 * 4);
+  parts = (int)((V + length - 1) / length);
 }
 
 }  // namespace
 
-// loss (N) and the row statistics stats (N, 2: the largest logit and the sum of
-// exp((z - largest) / tau)) that wxx_distill_backward takes; logits (N, V) with
-// row stride ld, top and ids (N, K).
+// loss (N) and the row statistics stats (N, 4: the largest logit and the sum of
+// exp((z - largest) / tau), the same two of the teacher's entries) that
+// wxx_distill_backward takes; logits (N, V) with row stride ld, top and ids (N, K).
 WXX_EXPORT int wxx_distill_loss(float* loss, float* stats, const float* logits, int64_t ld,
                                 const float* top, const uint32_t* ids, int64_t N, int64_t V, int K,
                                 float tau) {
   WXX_REQUIRE_INIT();
-  WXX_REQUIRE(N >= 0 && N < (int64_t(1) << 31) && V >= 1 && V < (int64_t(1) << 31),
-              "wxx_distill_loss: bad sizes");
-  WXX_REQUIRE(K >= 1 && K <= kMaxK, "wxx_distill_loss: %d stored logits outside [1, %d]", K, kMaxK);
-  WXX_REQUIRE(tau > 0.f && tau < INFINITY, "wxx_distill_loss: the temperature must be positive");
+  if (int st = check_sizes("wxx_distill_loss", N, V, K, tau)) return st;
   if (N == 0) return WXX_OK;
-  distill_forward_kernel<<<(unsigned)N, kT, 0, wxx::stream()>>>(
-      loss, stats, logits, ld, top, ids, (int)V, K, 1.0f / tau, tau * tau,
-      wxx::device_error_word());
+  int parts, length;
+  split_row(N, V, parts, length);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(N * parts));
+  cfg.blockDim = dim3(kT);
+  cfg.stream = wxx::stream();
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim = {(unsigned)parts, 1, 1};
+  cfg.attrs = &at;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
+  WXX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, distill_forward_kernel, loss, stats, logits, ld, top, ids,
+                                    (int)V, K, parts, length, 1.0f / tau,
+                                    (float)(1.4426950408889634 / (double)tau), tau * tau,
+                                    wxx::device_error_word()));
   WXX_LAUNCH_CHECK();
   return WXX_OK;
 }
@@ -175,15 +310,18 @@ WXX_EXPORT int wxx_distill_backward(float* dz, const float* grad, const float* l
                                     const float* top, const uint32_t* ids, const float* stats,
                                     int64_t N, int64_t V, int K, float tau) {
   WXX_REQUIRE_INIT();
-  WXX_REQUIRE(N >= 0 && N < (int64_t(1) << 31) && V >= 1 && V < (int64_t(1) << 31),
-              "wxx_distill_backward: bad sizes");
-  WXX_REQUIRE(K >= 1 && K <= kMaxK, "wxx_distill_backward: %d stored logits outside [1, %d]", K,
-              kMaxK);
-  WXX_REQUIRE(tau > 0.f && tau < INFINITY,
-              "wxx_distill_backward: the temperature must be positive");
+  if (int st = check_sizes("wxx_distill_backward", N, V, K, tau)) return st;
   if (N == 0) return WXX_OK;
-  distill_backward_kernel<<<(unsigned)N, kT, 0, wxx::stream()>>>(
-      dz, grad, logits, ld, top, ids, stats, (int)V, K, tau, 1.0f / tau, wxx::device_error_word());
+  WXX_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0,
+              "wxx_distill_backward: the statistics must be 16-byte aligned");
+  int parts, length;
+  split_row(N, V, parts, length);
+  const bool aligned = ((reinterpret_cast<uintptr_t>(dz) - reinterpret_cast<uintptr_t>(logits)) &
+                        15) == 0 && (ld - V) % 4 == 0;
+  auto kernel = aligned ? distill_backward_kernel<true> : distill_backward_kernel<false>;
+  kernel<<<(unsigned)(N * parts), kT, 0, wxx::stream()>>>(
+      dz, grad, logits, ld, top, ids, stats, (int)V, K, parts, length, tau, 1.0f / tau,
+      (float)(1.4426950408889634 / (double)tau), wxx::device_error_word());
   WXX_LAUNCH_CHECK();
   return WXX_OK;
 }

@@ -14,8 +14,12 @@
 #include <utility>
 
 #include "common.cuh"
+#include "rows.cuh"
 
 namespace {
+
+using wxx_rows::Row;
+using wxx_rows::warp_sum;
 
 constexpr int kT = 256;
 constexpr int kMaxTopk = 256;
@@ -44,16 +48,16 @@ __device__ __forceinline__ float key_float(uint32_t k) {
 }
 __device__ __forceinline__ float key_value(uint64_t k) { return key_float((uint32_t)(k >> 32)); }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
+// The largest of three; a NaN wins where it is the highest and loses where it is
+// the lowest.
+template <uint32_t NAN_KEY>
+__device__ __forceinline__ float largest(float a, float b, float c) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  if (NAN_KEY == kNanHighest)
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  else
+    d = fmax3(a, b, c);
   return d;
-}
-
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
 }
 
 // The lanes' values in descending order.
@@ -76,43 +80,9 @@ struct Select {                       // shared memory of a row's selection
   uint32_t reach[32];
   float sum[32], top[32];
   int warp[32];
+  unsigned char looks[32][32];
+  float tau;
   unsigned digit, rest;
-};
-
-// A row split over THREADS threads: 16-byte groups in the aligned middle, thread
-// t taking groups t, t + THREADS, ..., and up to six single entries at its ends,
-// one each for the first threads.
-struct Row {
-  const float* p;
-  const float4* mid;
-  int V, head, groups, single;        // single: this thread's single entry, -1 for none
-  __device__ Row(const float* row, int n) : p(row), V(n) {
-    head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / 4);
-    groups = (n - head) / 4;
-    mid = reinterpret_cast<const float4*>(row + head);
-    const int tail = n - head - 4 * groups, t = threadIdx.x;
-    single = t < head ? t : t < head + tail ? n - tail + (t - head) : -1;
-  }
-  template <int THREADS, class F>
-  __device__ __forceinline__ void each(F f) const {
-    if (single >= 0) f(p[single], single);
-    constexpr int kAhead = 4;         // loads in flight: they come from L2
-    for (int i = threadIdx.x; i < groups; i += kAhead * THREADS) {
-      float4 v[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (i + k * THREADS < groups) v[k] = mid[i + k * THREADS];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        if (i + k * THREADS >= groups) break;
-        const int at = head + 4 * (i + k * THREADS);
-        f(v[k].x, at);
-        f(v[k].y, at + 1);
-        f(v[k].z, at + 2);
-        f(v[k].w, at + 3);
-      }
-    }
-  }
 };
 
 // The r-th largest (from 1) of key(entry) over the row's entries that `among`
@@ -149,38 +119,49 @@ __device__ uint32_t nth_key(const Row& row, Select& s, unsigned r, unsigned& res
 
 // Puts the pairs of the entries that wanted() lets in into s.pair, in an order that
 // depends on the row alone, and returns how many there are (the first kCandidates
-// are kept); threads with look = false have none.  A thread marks 64 of its
-// entries at a time, the marks are counted over the block, and only the marked
-// entries are read again: a counter in shared memory that every pair takes a turn
-// at cost 12,000 cycles for 228 pairs.
+// are kept); threads with look = false have none.  A warp goes through the 16-byte
+// groups of its looking threads with all its lanes, marks what is wanted, and reads
+// the marked entries again once the marks are counted over the block (a counter in
+// shared memory that every pair takes a turn at cost 12,000 cycles for 228 pairs).
 template <int THREADS, uint32_t NAN_KEY, class Wanted>
 __device__ int collect(const Row& row, Select& s, bool look, Wanted wanted) {
-  constexpr int kWarps = THREADS / 32, kAhead = 4, kRound = 16;
+  constexpr int kWarps = THREADS / 32, kAhead = 4, kRounds = 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned looking = __ballot_sync(0xffffffffu, look);
+  const int n = __popc(looking);
+  if (look) s.looks[warp][__popc(looking & ((1u << lane) - 1))] = (unsigned char)lane;
+  __syncwarp();
+  const int each = (row.groups + THREADS - 1) / THREADS;     // groups of a thread
+  const bool lone = look && row.single >= 0 && wanted(row.p[row.single], row.single);
+  // the group of this lane in round r, or past the end
+  auto group_of = [&](int r) {
+    const int i = r * 32 + lane, g = n ? i / n : each;
+    return g < each ? warp * 32 + s.looks[warp][i - g * n] + g * THREADS : row.groups;
+  };
   int total = 0;
-  for (int g0 = threadIdx.x; g0 - (int)threadIdx.x < max(row.groups, 1); g0 += kRound * THREADS) {
+  for (int r0 = 0; r0 < max(each, 1); r0 += kRounds) {       // each * 32 groups at most
     unsigned long long marks = 0;
-    const bool lone = look && g0 == threadIdx.x && row.single >= 0 &&
-                      wanted(row.p[row.single], row.single);
-    if (look)
 #pragma unroll
-      for (int k0 = 0; k0 < kRound; k0 += kAhead) {
-        if (g0 + k0 * THREADS >= row.groups) break;
-        float4 v[kAhead];
+    for (int k0 = 0; k0 < kRounds; k0 += kAhead) {
+      if ((r0 + k0) * 32 >= n * each) break;
+      float4 v[kAhead];
+      int g[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-          if (g0 + (k0 + k) * THREADS < row.groups) v[k] = row.mid[g0 + (k0 + k) * THREADS];
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          const int g = g0 + (k0 + k) * THREADS, at = row.head + 4 * g;
-          if (g >= row.groups) break;
-          const unsigned four = (unsigned)wanted(v[k].x, at) | (unsigned)wanted(v[k].y, at + 1) << 1 |
-                                (unsigned)wanted(v[k].z, at + 2) << 2 |
-                                (unsigned)wanted(v[k].w, at + 3) << 3;
-          marks |= (unsigned long long)four << 4 * (k0 + k);
-        }
+      for (int k = 0; k < kAhead; ++k) {
+        g[k] = (r0 + k0 + k) * 32 < n * each ? group_of(r0 + k0 + k) : row.groups;
+        if (g[k] < row.groups) v[k] = row.mid[g[k]];
       }
-    const int mine = __popcll(marks) + (int)lone;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int at = row.head + 4 * g[k];
+        if (g[k] >= row.groups) continue;
+        const unsigned four = (unsigned)wanted(v[k].x, at) | (unsigned)wanted(v[k].y, at + 1) << 1 |
+                              (unsigned)wanted(v[k].z, at + 2) << 2 |
+                              (unsigned)wanted(v[k].w, at + 3) << 3;
+        marks |= (unsigned long long)four << 4 * (k0 + k);
+      }
+    }
+    const int mine = __popcll(marks) + (int)(lone && r0 == 0);
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -193,12 +174,13 @@ __device__ int collect(const Row& row, Select& s, bool look, Wanted wanted) {
     const int w = lane < kWarps ? s.warp[lane] : 0;
     int at = total + upto - mine + __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
     total += __reduce_add_sync(0xffffffffu, w);
-    if (lone && at < kCandidates)
-      s.pair[at] = pair_key(row.p[row.single], row.single, NAN_KEY);
-    at += lone;
+    if (lone && r0 == 0) {
+      if (at < kCandidates) s.pair[at] = pair_key(row.p[row.single], row.single, NAN_KEY);
+      ++at;
+    }
     for (; marks; marks &= marks - 1, ++at) {
       const int k = __ffsll(marks) - 1;
-      const int i = row.head + 4 * (g0 + (k >> 2) * THREADS) + (k & 3);
+      const int i = row.head + 4 * group_of(r0 + (k >> 2)) + (k & 3);
       if (at < kCandidates) s.pair[at] = pair_key(row.p[i], i, NAN_KEY);
     }
   }
@@ -225,13 +207,10 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
   if (NAN_KEY == kNanLowest && m != m) m = -INFINITY;
   float part = 0.f;
   if (SUM && row.single >= 0 && row.p[row.single] != -INFINITY) part = expf(row.p[row.single] - m);
-  auto larger = [](float a, float b) {
-    return NAN_KEY == kNanHighest ? max_nan(a, b) : fmaxf(a, b);
-  };
-#pragma unroll(SUM ? 8 : 4)
+#pragma unroll 4
   for (int i = threadIdx.x; i < row.groups; i += THREADS) {
     const float4 v = row.mid[i];
-    const float n = larger(larger(m, v.x), larger(larger(v.y, v.z), v.w));
+    const float n = largest<NAN_KEY>(largest<NAN_KEY>(m, v.x, v.y), v.z, v.w);
     if (SUM && n != -INFINITY) {
       if (n > m) part *= fast_exp2((m - n) * 1.4426950408889634f);
       part += (fast_exp2((v.x - n) * 1.4426950408889634f) +
@@ -268,13 +247,17 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
   }
   if (lane == 0) s.reach[warp] = reach;
   __syncthreads();
-  const float tau = key_float(
-      __shfl_sync(0xffffffffu, descending(lane < kWarps ? s.reach[lane] : 0u), mth - 1));
+  if (warp == 0) {
+    const uint32_t order = descending(lane < kWarps ? s.reach[lane] : 0u);
+    if (lane == mth - 1) s.tau = key_float(order);
+  }
   if (SUM) {
     const float w = lane < kWarps ? s.top[lane] : -INFINITY;
     top = key_float(__reduce_max_sync(0xffffffffu, value_key(w, NAN_KEY)));
     sum = warp_sum(lane < kWarps ? s.sum[lane] * (w == top ? 1.0f : expf(w - top)) : 0.f);
   }
+  __syncthreads();
+  const float tau = s.tau;
   // all pairs of a short row, else those that reach tau (NaN counts as reaching
   // where it is the highest; where it is the lowest, tau = -inf is left to the
   // digits, which know where it stands)

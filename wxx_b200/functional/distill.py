@@ -43,12 +43,12 @@ def _operands(what, logits, top_logits, top_ids, temperature):
 def distill_loss(logits, top_logits, top_ids, temperature=1.0):
     """``(loss, stats)``: the loss (N, 1) of every row of the student's
     ``logits`` (N, V) against the teacher's stored ``top_logits`` (N, K) of the
-    ids ``top_ids`` (N, K) u32, and the row statistics (N, 2) that
+    ids ``top_ids`` (N, K) u32, and the row statistics (N, 4) that
     ``distill_loss_backward`` takes.  An id outside [0, V) sets the device
     error word and counts as absent."""
     z, t, ids, tau, N, V, K = _operands("distill_loss", logits, top_logits, top_ids, temperature)
     loss = empty((N, 1))
-    stats = empty((N, 2))
+    stats = empty((N, 4))
     check(F.wxx_distill_loss(loss.buffer.ptr, stats.buffer.ptr, z.ptr, z.stride[0], t.ptr, ids.ptr,
                              N, V, K, tau), "distill_loss")
     return loss, stats
@@ -59,7 +59,7 @@ def distill_loss_backward(grad, logits, top_logits, top_ids, stats, temperature=
     losses: ``grad temperature (q_j - sum of p_k over id_k = j)``."""
     z, t, ids, tau, N, V, K = _operands("distill_loss_backward", logits, top_logits, top_ids,
                                         temperature)
-    for name, v, shape in (("grad", grad, (N, 1)), ("stats", stats, (N, 2))):
+    for name, v, shape in (("grad", grad, (N, 1)), ("stats", stats, (N, 4))):
         if v.type != "f32":
             raise TypeError(f"distill_loss_backward expects f32 {name}, got {v.type!r}")
         if tuple(v.shape) != shape:
