@@ -25,8 +25,6 @@
 
 WXX_EXPORT int wxx_malloc(void** out, uint64_t nbytes);
 WXX_EXPORT int wxx_free(void* p);
-WXX_EXPORT int wxx_reduce(float* out, const float* x, int64_t outer, int64_t reduce, int64_t inner,
-                          int mode);
 
 namespace {
 
@@ -121,7 +119,7 @@ struct Chain {
   Divider row_blocks;         // of one sequence
   int tiles;                  // tiles of a row
   unsigned total;             // tiles of all rows
-  int per;                    // channels of a gate
+  Divider per;                // channels of a gate
   int gates;                  // gates that 32 channels can have, at most
   int* err;
 };
@@ -227,20 +225,18 @@ __device__ __forceinline__ void copy_piece(float* tile, const Operand& o, const 
     src += o.ts;
   }
 }
+// Two threads a position; the block's first gate is gate 0 of the tile.
 __device__ __forceinline__ int first_gate(const Chain& c, const Place& p) {
-  return (p.d - (int)(threadIdx.x & 31)) / c.per;
+  return c.per(p.d - (threadIdx.x & 31));
 }
 __device__ __forceinline__ void copy_gates(float* tile, const Operand& g, const Chain& c,
                                            const Place& p, int T, int D) {
-  const int d0 = p.d - (threadIdx.x & 31), first = d0 / c.per;
-  const int n = min(d0 + 31, D - 1) / c.per - first + 1;
-  const int t0 = p.t0 - p.row, steps = (blockDim.x >> 5) * kSteps;
-  const float* src = g.p + p.b * g.bs + first;
-  for (int e = threadIdx.x; e < steps * n; e += blockDim.x) {
-    const int t = e / n, k = e - t * n;
-    const bool here = t0 + t < T;
-    copy_float(tile + t * c.gates + k, here ? src + (t0 + t) * g.ts + k : g.p, here);
-  }
+  const int d0 = p.d - (threadIdx.x & 31), first = first_gate(c, p);
+  const int n = c.per(min(d0 + 31, D - 1)) - first + 1;
+  const int row = threadIdx.x >> 1, t = p.t0 - p.row + row;
+  const float* src = g.p + p.b * g.bs + t * g.ts + first;
+  for (int k = threadIdx.x & 1; k < n; k += 2)
+    copy_float(tile + row * c.gates + k, t < T ? src + k : g.p, t < T);
 }
 
 // Joins the pieces of a tile (warp i of the order holds piece `mine`) with
@@ -377,7 +373,7 @@ __global__ void __launch_bounds__(kT, kForwardBlocks)
   extern __shared__ float s_raw[];
   __shared__ Joint s;
   float *s_x = aligned_smem(s_raw), *s_g = s_x + kTile;
-  const bool own_gate = c.per == 1;
+  const bool own_gate = c.per.d == 1;
   const unsigned box = (blockDim.x >> 5) * kSteps * 32 * sizeof(float);
   auto fetch = [&](const Place& p) {
     if (kTma && threadIdx.x == 0) {
@@ -398,7 +394,7 @@ __global__ void __launch_bounds__(kT, kForwardBlocks)
     const float* sx = s_x + p.row * 32 + (threadIdx.x & 31);
     const float* sg = s_g + p.row * stride +
                       (own_gate ? (int)(threadIdx.x & 31)
-                                : min(p.d, D - 1) / c.per - first_gate(c, p));
+                                : (int)c.per(min(p.d, D - 1)) - first_gate(c, p));
     Stretch upto[kSteps];            // the piece's positions up to each
     Stretch mine = {1.0f, 0.0f};
     auto first_run = [&](auto plain) {
@@ -434,8 +430,8 @@ __global__ void __launch_bounds__(kT, kForwardBlocks)
 // The same tiles with time reversed: c_t = a_t r_t (dh_t + c_{t+1}) is what
 // position t hands to t - 1.  Reads dh, x, gate, h, writes dx, dgate: 24 bytes a
 // position.  DG: where the gate's gradient goes -- 1: sums over the `per` lanes
-// of a head (a power of two up to 32; the first of them writes), 32: sums over the
-// warp, one partial sum per block of 32 channels; 0: every channel's own.
+// of a head (a power of two below 32; the first of them writes), 32: sums over the
+// warp, one per block of 32 channels; 0: every channel's own.
 template <bool kTma, int DG>
 __global__ void __launch_bounds__(kT, kBackwardBlocks)
     recurrence_backward_kernel(float* __restrict__ dx, float* __restrict__ dg,
@@ -450,7 +446,7 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
   extern __shared__ float s_raw[];
   __shared__ Joint s;
   float *s_x = aligned_smem(s_raw), *s_d = s_x + kTile, *s_h = s_d + kTile, *s_g = s_h + kTile;
-  const bool own_gate = c.per == 1;
+  const bool own_gate = c.per.d == 1;
   const unsigned box = (blockDim.x >> 5) * kSteps * 32 * sizeof(float);
   auto fetch = [&](const Place& p) {
     if (kTma && threadIdx.x == 0) {
@@ -471,14 +467,14 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
     if (!kTma || !own_gate) copies_arrive(&s.full);
   };
   const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !own_gate ? blockDim.x : 0);
-  const int lanes = DG == 1 ? c.per : DG == 32 ? 32 : 1, heads = DG == 0 ? D : D / lanes;
+  const int lanes = DG == 1 ? c.per.d : DG == 32 ? 32 : 1, heads = DG == 0 ? D : D / lanes;
   through_tiles<true>(c, s, arrivals, reset, T, D, fetch, [&](const Place& p, unsigned cut,
                                                               int turn, auto next) {
     const bool whole = __all_sync(0xffffffffu, p.left == kSteps && cut == 0 && p.t0 > 0);
     const int stride = own_gate ? 32 : c.gates, at = p.row * 32 + (threadIdx.x & 31);
     const float* sg = s_g + p.row * stride +
                       (own_gate ? (int)(threadIdx.x & 31)
-                                : min(p.d, D - 1) / c.per - first_gate(c, p));
+                                : (int)c.per(min(p.d, D - 1)) - first_gate(c, p));
     const int64_t state = (int64_t)p.b * D + p.d;
     // the total gradient from a zero carry, dx and dgate per unit of it
     float G[kSteps], z[kSteps], u[kSteps];
@@ -519,14 +515,15 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
         const float total = G[k] + carried;
         if (kPlain || k < p.left) *xo = z[k] * total;
         float e = u[k] * total;
-        if (DG == 1) {
-          if (!kPlain && k >= p.left) e = 0.f;
-          for (int o = 1; o < lanes; o <<= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
-        } else if (DG == 32) {
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
+        if (DG == 32) {
+          u[k] = e;
+        } else {
+          if (DG == 1) {
+            if (!kPlain && k >= p.left) e = 0.f;
+            for (int o = 1; o < lanes; o <<= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
+          }
+          if ((kPlain || k < p.left) && writes) *go = e;
         }
-        if ((kPlain || k < p.left) && writes) *go = e;
         carried *= 1.0f - z[k];
         if (!kPlain && (cut >> k & 1)) carried = 0.f;
         xo -= D;
@@ -534,8 +531,36 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
       }
     };
     if (whole) second_run(Yes{}); else second_run(No{});
+    if (DG == 32) {
+      // 16 sums over 32 lanes: every exchange halves the sums that a lane still
+      // carries, 16 exchanges in all where one sum at a time takes 80
+      const int lane = threadIdx.x & 31;
+#pragma unroll
+      for (int n = kSteps / 2, o = 16; n > 0; n >>= 1, o >>= 1)
+#pragma unroll
+        for (int k = 0; k < n; ++k) {
+          const bool upper = lane & o;
+          const float keep = upper ? u[k + n] : u[k], send = upper ? u[k] : u[k + n];
+          u[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+      const float sum = u[0] + __shfl_xor_sync(0xffffffffu, u[0], 1);
+      const int k = lane >> 1, left = __shfl_sync(0xffffffffu, p.left, 0);
+      if ((lane & 1) == 0 && k < left)
+        dg[((int64_t)p.b * T + p.t0 + k) * heads + (p.d - lane) / 32] = sum;
+    }
     if (dh0 && p.left && p.t0 == 0) dh0[state] = mine.b + carried;
   });
+}
+
+// out[i] = the sum of in[i parts .. (i + 1) parts - 1], in that order.
+__global__ void sum_parts_kernel(float* __restrict__ out, const float* __restrict__ in, int64_t n,
+                                 int parts) {
+  for (int64_t i = (int64_t)blockIdx.x * kT + threadIdx.x; i < n; i += (int64_t)gridDim.x * kT) {
+    const float* p = in + i * parts;
+    float v = p[0];
+    for (int k = 1; k < parts; ++k) v += p[k];
+    out[i] = v;
+  }
 }
 
 __global__ void recurrence_step_kernel(float* __restrict__ state, const float* __restrict__ x,
@@ -599,8 +624,8 @@ int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, int64_t H, int 
   c = Chain{};
   c.tiles = (int)((pieces + warps - 1) / warps);
   c.row_blocks = Divider::of((unsigned)((D + 31) / 32));
-  c.per = (int)(D / H);
-  c.gates = c.per >= 32 ? 2 : 31 / c.per + 2;
+  c.per = Divider::of((unsigned)(D / H));
+  c.gates = c.per.d >= 32 ? 2 : 31 / c.per.d + 2;
   c.err = wxx::device_error_word();
   *scratch = nullptr;
   threads = (unsigned)(warps * 32);
@@ -677,7 +702,7 @@ WXX_EXPORT int wxx_gated_recurrence(float* h, float* h_last, const float* x, int
   CUtensorMap mx{}, mg{};
   const unsigned steps = threads / 32 * kSteps;
   const bool tma = encode_operand(&mx, ox, B, T, D, steps) &&
-                   (c.per > 1 || encode_operand(&mg, og, B, T, D, steps));
+                   (c.per.d > 1 || encode_operand(&mg, og, B, T, D, steps));
   auto launch = [&](auto kernel) {
     if (int st = allow_smem(kernel, kBytes)) return st;
     kernel<<<grid, threads, kBytes, wxx::stream()>>>(h, h_last, mx, mg, ox, og, h0, reset, (int)T,
@@ -707,8 +732,9 @@ WXX_EXPORT int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0
   // they lie in one warp's 32 neighbours, by partial sums per 32 channels where
   // they are several warps', and from every channel's own otherwise.
   const int64_t per = D / H;
-  const bool inside = per <= 32 && (per & (per - 1)) == 0, partial = per > 32 && per % 32 == 0;
-  const int64_t parts = partial ? per / 32 : per;
+  const bool warp = per % 32 == 0, lanes = per < 32 && (per & (per - 1)) == 0;
+  const bool inside = lanes || per == 32;
+  const int64_t parts = warp ? per / 32 : per;
   const Operand ox{x, x_bs, x_ts}, og{gate, g_bs, g_ts}, od{dh, T * D, D}, oh{h, T * D, D};
   Chain c;
   unsigned threads, grid;
@@ -727,7 +753,7 @@ WXX_EXPORT int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0
     const bool tma = encode_operand(&mx, ox, B, T, D, steps) &&
                      encode_operand(&md, od, B, T, D, steps) &&
                      encode_operand(&mh, oh, B, T, D, steps) &&
-                     (c.per > 1 || encode_operand(&mg, og, B, T, D, steps));
+                     (c.per.d > 1 || encode_operand(&mg, og, B, T, D, steps));
     auto launch = [&](auto kernel) {
       if (int e = allow_smem(kernel, kBytes)) return e;
       kernel<<<grid, threads, kBytes, wxx::stream()>>>(dx, sums, dh0, mx, mg, md, mh, ox, og, od,
@@ -736,12 +762,16 @@ WXX_EXPORT int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0
     };
     auto pick = [&](auto t) {
       constexpr bool kTma = decltype(t)::value;
-      return per == 1 || (!inside && !partial) ? launch(recurrence_backward_kernel<kTma, 0>)
-             : inside                          ? launch(recurrence_backward_kernel<kTma, 1>)
-                                               : launch(recurrence_backward_kernel<kTma, 32>);
+      return warp                  ? launch(recurrence_backward_kernel<kTma, 32>)
+             : lanes && per > 1    ? launch(recurrence_backward_kernel<kTma, 1>)
+                                   : launch(recurrence_backward_kernel<kTma, 0>);
     };
     st = tma ? pick(Yes{}) : pick(No{});
-    if (st == WXX_OK && wide) st = wxx_reduce(dgate, sums, B * T * H, parts, 1, 0);
+    if (st == WXX_OK && wide) {
+      sum_parts_kernel<<<wxx::grid_for(B * T * H, kT), kT, 0, wxx::stream()>>>(
+          dgate, sums, B * T * H, (int)parts);
+      st = wxx::after_launch(__FILE__, __LINE__);
+    }
   }
   if (scratch) wxx_free(scratch);
   if (wide) wxx_free(wide);

@@ -33,6 +33,17 @@ def dense(t):
     return contiguous(t)
 
 
+def compact(t):
+    """``dense`` where the check is a good part of a short call: the strides are
+    compared in place instead of being built first."""
+    n = 1
+    for d, s in zip(reversed(t.shape), reversed(t.stride)):
+        if d != 1 and s != n:
+            return dense(t)
+        n *= d
+    return t
+
+
 def ptr_or_none(t):
     return None if t is None else t.ptr
 
@@ -83,6 +94,7 @@ def rng():
 __all__ = [
     "arr64",
     "check",
+    "compact",
     "dense",
     "empty",
     "F",

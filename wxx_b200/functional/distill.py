@@ -12,7 +12,7 @@ with none has loss 0 and gradient 0.
 
 import math
 
-from ._common import F, check, dense, empty
+from ._common import F, check, compact, empty
 
 _MAX_STORED = 1024
 
@@ -36,8 +36,8 @@ def _operands(what, logits, top_logits, top_ids, temperature):
     if not 0.0 < temperature < math.inf:
         raise ValueError(f"{what}: the temperature must be positive, got {temperature}")
     if logits.stride[1] != 1 or logits.stride[0] < V:
-        logits = dense(logits)
-    return logits, dense(top_logits), dense(top_ids), temperature, N, V, K
+        logits = compact(logits)
+    return logits, compact(top_logits), compact(top_ids), temperature, N, V, K
 
 
 def distill_loss(logits, top_logits, top_ids, temperature=1.0):
@@ -64,7 +64,7 @@ def distill_loss_backward(grad, logits, top_logits, top_ids, stats, temperature=
             raise TypeError(f"distill_loss_backward expects f32 {name}, got {v.type!r}")
         if tuple(v.shape) != shape:
             raise ValueError(f"distill_loss_backward: {name} {tuple(v.shape)} is not {shape}")
-    grad, stats = dense(grad), dense(stats)
+    grad, stats = compact(grad), compact(stats)
     dz = empty((N, V))
     check(F.wxx_distill_backward(dz.buffer.ptr, grad.ptr, z.ptr, z.stride[0], t.ptr, ids.ptr,
                                  stats.ptr, N, V, K, tau), "distill_loss_backward")

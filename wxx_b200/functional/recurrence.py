@@ -10,7 +10,7 @@ u32, marks positions where a new document starts: the state before such a
 position is zero, so documents packed into one row do not see each other.
 """
 
-from ._common import F, check, dense, empty, ptr_or_none
+from ._common import F, check, compact, empty, ptr_or_none
 from .utils import mark_written
 
 
@@ -22,7 +22,7 @@ def _typed(name, t, dtype):
 def _inner_dense(t):
     """``t`` when its rows are dense (any other strides: a column slice of a
     projection's output is read in place), else a dense copy."""
-    return t if t.shape[-1] <= 1 or t.stride[-1] == 1 and min(t.stride) >= 0 else dense(t)
+    return t if t.shape[-1] <= 1 or t.stride[-1] == 1 and min(t.stride) >= 0 else compact(t)
 
 
 def _operands(x, gate, h0, reset):
@@ -42,12 +42,12 @@ def _operands(x, gate, h0, reset):
         _typed("h0", h0, "f32")
         if tuple(h0.shape) != (B, D):
             raise ValueError(f"gated_recurrence: h0 {tuple(h0.shape)} is not {(B, D)}")
-        h0 = dense(h0)
+        h0 = compact(h0)
     if reset is not None:
         _typed("reset", reset, "u32")
         if tuple(reset.shape) != (B, T):
             raise ValueError(f"gated_recurrence: reset {tuple(reset.shape)} is not {(B, T)}")
-        reset = dense(reset)
+        reset = compact(reset)
     return _inner_dense(x), _inner_dense(gate), h0, reset, B, T, D, H
 
 
@@ -78,8 +78,8 @@ def gated_recurrence_backward(grad, x, gate, h, h0=None, reset=None, grad_last=N
         _typed(name, t, "f32")
         if tuple(t.shape) != shape:
             raise ValueError(f"gated_recurrence_backward: {name} {tuple(t.shape)} is not {shape}")
-    grad, h = dense(grad), dense(h)
-    grad_last = None if grad_last is None else dense(grad_last)
+    grad, h = compact(grad), compact(h)
+    grad_last = None if grad_last is None else compact(grad_last)
     dx = empty((B, T, D))
     dgate = empty((B, T, H))
     dh0 = None if h0 is None else empty((B, D))

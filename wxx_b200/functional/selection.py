@@ -8,7 +8,7 @@ the results are the same on every run.
 import ctypes
 
 from .. import validation
-from ._common import F, check, dense, empty, ptr_or_none
+from ._common import F, check, compact, empty, ptr_or_none
 from .utils import mark_written
 
 _MAX_TOPK = 256
@@ -28,7 +28,7 @@ def topk(x, k):
     if not 1 <= k <= min(V, _MAX_TOPK):
         raise ValueError(f"topk: k = {k} outside [1, {min(V, _MAX_TOPK)}] for {V} entries")
     if not (len(x.shape) == 2 and x.stride[1] == 1 and x.stride[0] >= V):
-        x = dense(x)
+        x = compact(x)
     lead = list(x.shape[:-1])
     N = validation.numel(lead)
     values = empty(lead + [k])
@@ -75,10 +75,10 @@ def beam_select(logits, scores, finished=None, stop_token=None):
             raise ValueError(f"beam_select: finished {tuple(finished.shape)} is not {(B, W)}")
         if not 0 <= int(stop_token) < V:
             raise ValueError(f"beam_select: stop_token {stop_token} outside [0, {V})")
-        finished = dense(finished)
-    scores = dense(scores)
+        finished = compact(finished)
+    scores = compact(scores)
     if logits.stride[1] != 1 or logits.stride[0] < V:
-        logits = dense(logits)
+        logits = compact(logits)
     new_scores = empty((B, W))
     parents = empty((B, W), "u32")
     tokens = empty((B, W), "u32")
@@ -126,7 +126,7 @@ def beam_reorder(states, parents, cur_len=None):
         # each would move rows that the other is moving
         if rows[i] and rows[j] and (ptrs[i] or 0) + 4 * B * W * rows[i] > (ptrs[j] or 0):
             raise ValueError(f"beam_reorder: states {i} and {j} overlap in memory")
-    parents = dense(parents)
+    parents = compact(parents)
     check(F.wxx_beam_reorder(n, ptrs, rows, units, parents.ptr, B, W, ptr_or_none(cur_len)),
           "beam_reorder")
     for t in states:
