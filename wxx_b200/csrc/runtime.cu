@@ -341,7 +341,11 @@ WXX_EXPORT int wxx_free(void* p) {
             g_arenas.erase(g_arenas.begin() + i);
             break;
           }
-        cudaFreeAsync(a->base, wxx::stream());
+        // as for a pool block below: not inside another graph's capture
+        if (g_capture != nullptr)
+          g_capture->deferred.push_back(a->base);
+        else
+          cudaFreeAsync(a->base, wxx::stream());
         delete a;
       }
       return WXX_OK;
