@@ -120,9 +120,20 @@ class Tensor:
     @classmethod
     def _empty(cls, shape, dtype="f32", requires_grad=False):
         """Uninitialised dense tensor (internal: every op's output)."""
-        n = validation.numel(shape)
-        buf = _dev.DeviceBuffer(max(n * _itemsize(dtype), 4), "Tensor")
-        return cls._wrap(shape, buf, dtype, requires_grad)
+        t = object.__new__(cls)
+        t.shape = list(shape)
+        n, stride = 1, [1] * len(t.shape)
+        for axis in range(len(t.shape) - 1, -1, -1):
+            stride[axis] = n
+            n *= int(t.shape[axis])
+        t.stride = tuple(stride)
+        t.type = dtype
+        t.nbytes = n * _itemsize(dtype)
+        t.buffer = _dev.DeviceBuffer(max(t.nbytes, 4), "Tensor")
+        t.offset = 0
+        t._base = t.creator = t.grad = None
+        t.requires_grad = requires_grad
+        return t
 
     @property
     def ptr(self):

@@ -8,6 +8,7 @@ import numpy as np
 
 from .. import validation
 from ..Tensor import Tensor
+from ..backend.device import DeviceBuffer
 from ..backend.lib import F, check
 
 i64 = ctypes.c_int64
@@ -20,6 +21,17 @@ def arr64(values):
 
 def empty(shape, dtype="f32", requires_grad=False):
     return Tensor._empty(list(shape), dtype, requires_grad)
+
+
+def empty_group(*specs):
+    """Uninitialised dense tensors, each a (shape, dtype), in one allocation (kept
+    while any of them is): for the results of one call that are used together."""
+    total, at = 0, []
+    for shape, _ in specs:
+        at.append(total)
+        total += (4 * validation.numel(shape) + 255) // 256 * 256
+    buf = DeviceBuffer(max(total, 4), "Tensor")
+    return [Tensor._wrap(shape, buf, dtype, offset=o // 4) for (shape, dtype), o in zip(specs, at)]
 
 
 def dense(t):
@@ -97,6 +109,7 @@ __all__ = [
     "compact",
     "dense",
     "empty",
+    "empty_group",
     "F",
     "get_matmul_mode",
     "manual_seed",

@@ -12,7 +12,7 @@ with none has loss 0 and gradient 0.
 
 import math
 
-from ._common import F, check, compact, empty
+from ._common import F, check, compact, empty, empty_group
 
 _MAX_STORED = 1024
 
@@ -47,9 +47,8 @@ def distill_loss(logits, top_logits, top_ids, temperature=1.0):
     ``distill_loss_backward`` takes.  An id outside [0, V) sets the device
     error word and counts as absent."""
     z, t, ids, tau, N, V, K = _operands("distill_loss", logits, top_logits, top_ids, temperature)
-    loss = empty((N, 1))
-    stats = empty((N, 4))
-    check(F.wxx_distill_loss(loss.buffer.ptr, stats.buffer.ptr, z.ptr, z.stride[0], t.ptr, ids.ptr,
+    stats, loss = empty_group(((N, 4), "f32"), ((N, 1), "f32"))
+    check(F.wxx_distill_loss(loss.ptr, stats.ptr, z.ptr, z.stride[0], t.ptr, ids.ptr,
                              N, V, K, tau), "distill_loss")
     return loss, stats
 

@@ -8,7 +8,7 @@ the results are the same on every run.
 import ctypes
 
 from .. import validation
-from ._common import F, check, compact, empty, ptr_or_none
+from ._common import F, check, compact, empty_group, ptr_or_none
 from .utils import mark_written
 
 _MAX_TOPK = 256
@@ -31,9 +31,8 @@ def topk(x, k):
         x = compact(x)
     lead = list(x.shape[:-1])
     N = validation.numel(lead)
-    values = empty(lead + [k])
-    ids = empty(lead + [k], "u32")
-    check(F.wxx_topk(values.buffer.ptr, ids.buffer.ptr, x.ptr,
+    values, ids = empty_group((lead + [k], "f32"), (lead + [k], "u32"))
+    check(F.wxx_topk(values.ptr, ids.ptr, x.ptr,
                      x.stride[0] if len(lead) == 1 else V, N, V, k), "topk")
     return values, ids
 
@@ -79,11 +78,11 @@ def beam_select(logits, scores, finished=None, stop_token=None):
     scores = compact(scores)
     if logits.stride[1] != 1 or logits.stride[0] < V:
         logits = compact(logits)
-    new_scores = empty((B, W))
-    parents = empty((B, W), "u32")
-    tokens = empty((B, W), "u32")
-    new_finished = None if finished is None else empty((B, W), "u32")
-    check(F.wxx_beam_select(new_scores.buffer.ptr, parents.buffer.ptr, tokens.buffer.ptr,
+    whole = ((B, W), "u32")
+    new_scores, parents, tokens, *more = empty_group(
+        ((B, W), "f32"), whole, whole, *([] if finished is None else [whole]))
+    new_finished = more[0] if more else None
+    check(F.wxx_beam_select(new_scores.ptr, parents.ptr, tokens.ptr,
                             ptr_or_none(new_finished), logits.ptr, logits.stride[0], scores.ptr,
                             ptr_or_none(finished), B, W, V, int(stop_token or 0)), "beam_select")
     return new_scores, parents, tokens, new_finished
