@@ -37,8 +37,6 @@ using wxx_tc::tma_load_3d;
 constexpr int kT = 256;
 constexpr int kSteps = 16;          // positions of a thread
 constexpr int kWarps = 8;           // pieces of a tile, at most
-constexpr int kGroup = 32;          // tiles joined without a chain
-constexpr int kSeg = kGroup / kWarps;
 constexpr int kTile = kWarps * kSteps * 32;                // floats of a tile's operand
 constexpr int kForwardBlocks = 3, kBackwardBlocks = 2;     // resident on an SM
 constexpr int kWaitLimit = 1 << 21; // polls of a published word (about a second)
@@ -114,7 +112,7 @@ struct Divider {
 struct Chain {
   unsigned* ticket;
   ulonglong2* tile;           // {A, b} of a tile, 32 channels
-  unsigned long long* group;  // the state after each group of kGroup tiles
+  unsigned long long* group;  // the state after each group of tiles
   Divider blocks;             // blocks of 32 channels, all sequences
   Divider row_blocks;         // of one sequence
   int tiles;                  // tiles of a row
@@ -242,10 +240,10 @@ __device__ __forceinline__ void copy_gates(float* tile, const Operand& g, const 
 // Joins the pieces of a tile (warp i of the order holds piece `mine`) with
 // everything before it.  j: the tile's place in its row, q: its channel block.
 // Returns the state before this warp's piece.  The order of the additions
-// depends on j alone: the tiles of the same group so far, in kWarps segments,
-// then the state after the group before.  fetch_next is called once, when every
+// depends on j alone: the tiles of the same group (kWarps segments of kSeg tiles,
+// one looked at by each warp) so far, then the state after the group before.  fetch_next is called once, when every
 // warp has taken its inputs from shared memory.
-template <class F>
+template <int kSeg, class F>
 __device__ __forceinline__ float join_tile(const Chain& c, Joint& s, int turn, const Place& p,
                                            Stretch mine, float start, F fetch_next) {
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, i = p.i;
@@ -260,6 +258,7 @@ __device__ __forceinline__ float join_tile(const Chain& c, Joint& s, int turn, c
   fetch_next();
   float h = start;
   if (c.tiles > 1) {
+    constexpr int kGroup = kSeg * kWarps;
     const int r = p.j % kGroup, g = p.j / kGroup;
     const int64_t groups = (c.tiles + kGroup - 1) / kGroup;
     const ulonglong2* row = c.tile + ((int64_t)p.q * c.tiles + g * kGroup + i * kSeg) * 32 + lane;
@@ -347,9 +346,10 @@ __device__ __forceinline__ void through_tiles(const Chain& c, Joint& s, unsigned
   }
   // a last wait for the copies of a tile that did not come, before the block's
   // shared memory goes to another
-  if (s.abort[turn])
-    for (int n = 0; n < kWaitLimit && !wxx_tc::mbar_try_wait(smem_u32(&s.full), turn); ++n) {
-    }
+  if (s.abort[turn]) {
+    int given_up = 0;
+    mbar_wait(&s.full, turn, &given_up, c.err);
+  }
 }
 
 __device__ __forceinline__ float* aligned_smem(float* p) {
@@ -363,7 +363,7 @@ __device__ __forceinline__ float* aligned_smem(float* p) {
 // and the product of the weights up to there, which then takes the state that the
 // join gives.  A warp whose piece is whole and holds no reset (nearly all) runs
 // without the tests for them.
-template <bool kTma>
+template <bool kTma, int kSeg>
 __global__ void __launch_bounds__(kT, kForwardBlocks)
     recurrence_forward_kernel(float* __restrict__ h, float* __restrict__ h_last,
                               const __grid_constant__ CUtensorMap map_x,
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kT, kForwardBlocks)
     };
     if (whole) first_run(Yes{}); else first_run(No{});
     const int64_t state = (int64_t)p.b * D + p.d;
-    const float v = join_tile(c, s, turn, p, mine, h0 && p.d < D && p.j < kGroup ? h0[state] : 0.f, next);
+    const float v = join_tile<kSeg>(c, s, turn, p, mine, h0 && p.d < D && p.j < kSeg * kWarps ? h0[state] : 0.f, next);
     float* hp = h + ((int64_t)p.b * T + p.t0) * D + p.d;
     auto second_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kT, kForwardBlocks)
 // position.  DG: where the gate's gradient goes -- 1: sums over the `per` lanes
 // of a head (a power of two below 32; the first of them writes), 32: sums over the
 // warp, one per block of 32 channels; 0: every channel's own.
-template <bool kTma, int DG>
+template <bool kTma, int kSeg, int DG>
 __global__ void __launch_bounds__(kT, kBackwardBlocks)
     recurrence_backward_kernel(float* __restrict__ dx, float* __restrict__ dg,
                                float* __restrict__ dh0,
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
       }
     };
     if (whole) first_run(Yes{}); else first_run(No{});
-    const float v = join_tile(c, s, turn, p, mine, dlast && p.d < D && p.j < kGroup ? dlast[state] : 0.f,
+    const float v = join_tile<kSeg>(c, s, turn, p, mine, dlast && p.d < D && p.j < kSeg * kWarps ? dlast[state] : 0.f,
                         next);
     const int64_t last = (int64_t)p.b * T + p.t0 + kSteps - 1;
     float* xo = dx + last * D + p.d;
@@ -616,6 +616,13 @@ int check_sizes(const char* what, int64_t B, int64_t T, int64_t D, int64_t H) {
   return WXX_OK;
 }
 
+// Tiles of a group.  Looking at more tiles costs every tile, a hop between groups
+// costs the row: at 64 tiles a row forward and backward took 78 + 139 us in groups of
+// 8, 84 + 160 in groups of 32; at 512 tiles a row the forward took 73 and 54 us.
+constexpr int kShortSeg = 1, kLongSeg = 4;
+bool long_rows(const Chain& c) { return c.tiles > 128; }
+int group_tiles(const Chain& c) { return kWarps * (long_rows(c) ? kLongSeg : kShortSeg); }
+
 // Threads and blocks of a scan, and its scratch (freed by the caller).
 int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, int64_t H, int resident, Chain& c,
               unsigned& threads, unsigned& grid, void** scratch) {
@@ -636,7 +643,7 @@ int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, int64_t H, int 
   const int64_t most = (int64_t)wxx::num_sms() * resident;
   grid = (unsigned)(total < most ? total : most);
   if (c.tiles == 1) return WXX_OK;
-  const int64_t groups = (c.tiles + kGroup - 1) / kGroup;
+  const int64_t size = group_tiles(c), groups = (c.tiles + size - 1) / size;
   const size_t tile_bytes = (size_t)total * 32 * sizeof(ulonglong2);
   const size_t bytes = 256 + tile_bytes + (size_t)(blocks * groups) * 32 * 8;
   if (int st = wxx_malloc(scratch, bytes)) return st;
@@ -657,7 +664,7 @@ int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, int64_t H, int 
 // Room for the kernel's tiles, asked for once for each kernel.
 template <class K>
 int allow_smem(K kernel, int bytes) {
-  static K done[8] = {};           // kernels of this type that have it
+  static K done[16] = {};           // kernels of this type that have it
   for (K& k : done) {
     if (k == kernel) return WXX_OK;
     if (k) continue;
@@ -709,8 +716,11 @@ WXX_EXPORT int wxx_gated_recurrence(float* h, float* h_last, const float* x, int
                                                      (int)D, c);
     return wxx::after_launch(__FILE__, __LINE__);
   };
-  const int st = tma ? launch(recurrence_forward_kernel<true>)
-                     : launch(recurrence_forward_kernel<false>);
+  const int st =
+      long_rows(c) ? (tma ? launch(recurrence_forward_kernel<true, kLongSeg>)
+                          : launch(recurrence_forward_kernel<false, kLongSeg>))
+                   : (tma ? launch(recurrence_forward_kernel<true, kShortSeg>)
+                          : launch(recurrence_forward_kernel<false, kShortSeg>));
   if (scratch) wxx_free(scratch);
   return st;
 }
@@ -760,13 +770,15 @@ WXX_EXPORT int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0
                                                        oh, dlast, h0, reset, (int)T, (int)D, c);
       return wxx::after_launch(__FILE__, __LINE__);
     };
-    auto pick = [&](auto t) {
+    auto pick = [&](auto t, auto seg) {
       constexpr bool kTma = decltype(t)::value;
-      return warp                  ? launch(recurrence_backward_kernel<kTma, 32>)
-             : lanes && per > 1    ? launch(recurrence_backward_kernel<kTma, 1>)
-                                   : launch(recurrence_backward_kernel<kTma, 0>);
+      constexpr int kSeg = decltype(seg)::value ? kLongSeg : kShortSeg;
+      return warp                  ? launch(recurrence_backward_kernel<kTma, kSeg, 32>)
+             : lanes && per > 1    ? launch(recurrence_backward_kernel<kTma, kSeg, 1>)
+                                   : launch(recurrence_backward_kernel<kTma, kSeg, 0>);
     };
-    st = tma ? pick(Yes{}) : pick(No{});
+    st = long_rows(c) ? (tma ? pick(Yes{}, Yes{}) : pick(No{}, Yes{}))
+                      : (tma ? pick(Yes{}, No{}) : pick(No{}, No{}));
     if (st == WXX_OK && wide) {
       sum_parts_kernel<<<wxx::grid_for(B * T * H, kT), kT, 0, wxx::stream()>>>(
           dgate, sums, B * T * H, (int)parts);
