@@ -458,6 +458,10 @@ int wxx_beam_select(float* new_scores, uint32_t* parents, uint32_t* tokens, uint
  * leaves its row and sets the device error word. */
 int wxx_beam_reorder(int n, uint32_t* const* state, const int64_t* row, const int64_t* unit,
                      const uint32_t* parents, int64_t B, int W, const uint32_t* cur_len);
+/* ids[r, *cur_len] = tokens[r] for the rows of ids (rows, most; row stride ld), then *cur_len += 1
+ * (one device word).  At *cur_len >= most nothing is written and the device error word is set. */
+int wxx_beam_append(uint32_t* ids, int64_t ld, int64_t rows, const uint32_t* tokens,
+                    uint32_t* cur_len, int64_t most);
 
 /* ---------------------------------------------------------------- NCCL
  * No reference counterpart (the reference drives one WebGPU device): the

@@ -135,3 +135,61 @@ def beam_reorder(state, parents, used=None):
     else:
         out[:, :used] = state[rows, :used]
     return out
+
+
+# ------------------------------------------------------------------ the model
+
+
+def _layernorm(x, g, b):
+    mu = x.mean(-1, keepdims=True)
+    return (x - mu) / np.sqrt(((x - mu) ** 2).mean(-1, keepdims=True) + 1e-5) * g + b
+
+
+def _gelu(x):
+    return 0.5 * x * (1 + np.tanh(0.7978845608 * (x + 0.044715 * x ** 3)))
+
+
+def lm_forward(sd, ids, n_layers, reset=None):
+    """Logits (batch, time, vocab) of the recurrent language model."""
+    sd = {k: np.asarray(v, np.float64) for k, v in sd.items()}
+    x = sd["tok_emb.weight"][np.asarray(ids, np.int64)]
+    for i in range(n_layers):
+        p = f"blocks.{i}."
+        u = _layernorm(x, sd[p + "ln1.weightg"], sd[p + "ln1.weightb"])
+        gate = u @ sd[p + "mixer.gate.weight"] + sd[p + "mixer.gate.bias"]
+        h, _ = recurrence(u @ sd[p + "mixer.value.weight"], gate, None, reset)
+        x = x + (h * _gelu(u @ sd[p + "mixer.mix.weight"])) @ sd[p + "mixer.out.weight"]
+        u = _layernorm(x, sd[p + "ln2.weightg"], sd[p + "ln2.weightb"])
+        u = _gelu(u @ sd[p + "mlp.0.weight"] + sd[p + "mlp.0.bias"])
+        x = x + u @ sd[p + "mlp.2.weight"] + sd[p + "mlp.2.bias"]
+    return _layernorm(x, sd["ln_f.weightg"], sd["ln_f.weightb"]) @ sd["tok_emb.weight"].T
+
+
+def beam_search(logits_of, prompt, beams, n_new, stop=None):
+    """(ids (batch, beams, seq + n), scores): every step re-runs ``logits_of`` on
+    whole prefixes; finished beams are filled up with ``stop``.  ``gap`` is the
+    smallest distance between neighbouring proposals around any cut or order."""
+    out_ids, out_scores, gap = [], [], np.inf
+    for row in np.asarray(prompt):
+        live = [(0.0, list(row), False)]
+        for _ in range(n_new):
+            if all(f for _, _, f in live):
+                live = [(s, ids + [stop], f) for s, ids, f in live]
+                continue
+            found = []
+            for w, (s, ids, f) in enumerate(live):
+                if f:
+                    found.append((s, w, 0, stop))
+                    continue
+                z = np.asarray(logits_of(np.array([ids])), np.float64)[0, -1]
+                logp = z - z.max() - np.log(np.exp(z - z.max()).sum())
+                best = np.argsort(-logp, kind="stable")[:beams + 1]
+                found += [(s + logp[t], w, r, int(t)) for r, t in enumerate(best)]
+            found.sort(key=lambda c: (-c[0], c[1], c[2]))
+            top = np.array([c[0] for c in found[:beams + 1]])
+            gap = min(gap, np.abs(np.diff(top)).min())
+            live = [(s, live[w][1] + [t], live[w][2] or (stop is not None and t == stop))
+                    for s, w, _, t in found[:beams]]
+        out_ids.append([ids for _, ids, _ in live])
+        out_scores.append([s for s, _, _ in live])
+    return np.array(out_ids), np.array(out_scores), gap

@@ -163,6 +163,7 @@ SIGNATURES = {
     "wxx_beam_select": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_void_p,
                         c_void_p, c_i64, c_int, c_i64, c_u32],
     "wxx_beam_reorder": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_int, c_void_p],
+    "wxx_beam_append": [c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_i64],
     "wxx_nccl_unique_id": [P_u8],
     "wxx_nccl_init": [P_u8, c_int, c_int],
     "wxx_nccl_allgather": [c_void_p, c_void_p, c_u64],

@@ -525,6 +525,21 @@ __global__ void __launch_bounds__(kT)
     move(base, row, i);
 }
 
+// The rows' next tokens behind their first *cur_len ids; the block that writes them
+// all advances the length.
+__global__ void beam_append_kernel(uint32_t* __restrict__ ids, int64_t ld, int64_t rows,
+                                   const uint32_t* __restrict__ tokens, uint32_t* cur_len,
+                                   uint32_t most, int* err) {
+  const uint32_t n = *cur_len;
+  __syncthreads();
+  if (n >= most) {
+    if (threadIdx.x == 0) wxx_device_fail(err, WXX_DEV_ERR_BAD_INDEX);
+    return;
+  }
+  for (int64_t r = threadIdx.x; r < rows; r += blockDim.x) ids[r * ld + n] = tokens[r];
+  if (threadIdx.x == 0) *cur_len = n + 1;
+}
+
 }  // namespace
 
 // values and ids (N, K): the K largest of each row of x (N, V; row stride ld)
@@ -622,5 +637,19 @@ WXX_EXPORT int wxx_beam_reorder(int n, uint32_t* const* state, const int64_t* ro
     kernel<<<grid, kT, 0, wxx::stream()>>>(tab, parents, cur_len, W, wxx::device_error_word());
     WXX_LAUNCH_CHECK();
   }
+  return WXX_OK;
+}
+
+// ids[r, *cur_len] = tokens[r] for the rows of ids (rows, most; row stride ld), then
+// *cur_len += 1.  A full table is left as it is and sets the device error word.
+WXX_EXPORT int wxx_beam_append(uint32_t* ids, int64_t ld, int64_t rows, const uint32_t* tokens,
+                               uint32_t* cur_len, int64_t most) {
+  WXX_REQUIRE_INIT();
+  WXX_REQUIRE(rows >= 0 && most >= 0 && most < (int64_t(1) << 32) && ld >= most,
+              "wxx_beam_append: bad sizes");
+  if (rows == 0) return WXX_OK;
+  beam_append_kernel<<<1, kT, 0, wxx::stream()>>>(ids, ld, rows, tokens, cur_len, (uint32_t)most,
+                                                  wxx::device_error_word());
+  WXX_LAUNCH_CHECK();
   return WXX_OK;
 }

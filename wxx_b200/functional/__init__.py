@@ -145,7 +145,7 @@ from .recurrence import (  # noqa: E402
     gated_recurrence_backward,
     gated_recurrence_step,
 )
-from .selection import beam_reorder, beam_select, topk  # noqa: E402
+from .selection import beam_append, beam_reorder, beam_select, topk  # noqa: E402
 
 
 __all__ = [name for name in dir() if not name.startswith("__")]

@@ -131,3 +131,25 @@ def beam_reorder(states, parents, cur_len=None):
     for t in states:
         mark_written(t)
     return states
+
+
+def beam_append(ids, tokens, cur_len):
+    """Writes the chosen tokens behind the beams' ids: ``ids[r, cur_len] =
+    tokens[r]`` for the rows of ``ids`` (rows, most) u32, ``tokens`` of as many
+    u32 elements, then ``cur_len`` (a u32 tensor of one element) grows by one,
+    all on the device.  A full ``ids`` is left and sets the device error word."""
+    for name, t in (("ids", ids), ("tokens", tokens), ("cur_len", cur_len)):
+        if t.type != "u32":
+            raise TypeError(f"beam_append expects u32 {name}, got {t.type!r}")
+    if len(ids.shape) != 2 or ids.stride[1] != 1 or ids.stride[0] < ids.shape[1]:
+        raise ValueError("beam_append: ids are written in place and must be rows of neighbouring "
+                         f"elements, got shape {tuple(ids.shape)} stride {tuple(ids.stride)}")
+    if validation.numel(tokens.shape) != ids.shape[0] or validation.numel(cur_len.shape) != 1:
+        raise ValueError(f"beam_append: {tuple(tokens.shape)} tokens and cur_len "
+                         f"{tuple(cur_len.shape)} for {ids.shape[0]} rows")
+    tokens = compact(tokens)
+    check(F.wxx_beam_append(ids.ptr, ids.stride[0], ids.shape[0], tokens.ptr, cur_len.ptr,
+                            ids.shape[1]), "beam_append")
+    mark_written(ids)
+    mark_written(cur_len)
+    return ids

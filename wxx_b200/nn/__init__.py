@@ -35,6 +35,7 @@ from .module import (
 )
 from .loss import CCELoss, DistillLoss, MAELoss, loss
 from .optimizer import AdamW, Optimizer, SGD
+from .recurrent import GatedRecurrence, RecurrentBlock, RecurrentLM
 from .resnet import ResBlock, ResNet18
 
 __all__ = [
@@ -44,4 +45,5 @@ __all__ = [
     "MaxPool2d", "Module", "ModuleList", "MultiHeadAttention", "PositionalEncoding", "RMSNorm",
     "ResBlock", "ResNet18", "Sequential", "Sine", "SwiGLU", "TiedLinear",
     "loss", "CCELoss", "DistillLoss", "MAELoss", "Optimizer", "SGD", "AdamW",
+    "GatedRecurrence", "RecurrentBlock", "RecurrentLM",
 ]

@@ -169,5 +169,13 @@ class GPT2(Module):
         return generate(self, prompt, max_new_tokens=max_new_tokens, temperature=temperature,
                         top_k=top_k, stop_token=stop_token, rng=rng)
 
+    def beam_search(self, prompt, beams=4, max_new_tokens=64, stop_token=None, length_penalty=0.0):
+        """Beam search from ``prompt``, at most ``max_len`` tokens in total (see
+        ``nn.generation.beam_search``; no reference counterpart)."""
+        from .generation import beam_search
+
+        return beam_search(self, prompt, beams=beams, max_new_tokens=max_new_tokens,
+                           stop_token=stop_token, length_penalty=length_penalty)
+
 
 __all__ = ["GPT2", "GPT2Block"]
