@@ -188,6 +188,62 @@ __device__ int collect(const Row& row, Select& s, bool look, Wanted wanted) {
   return total;
 }
 
+// The warps' largest entries and sums of exponentials, and their join (the row's).
+__device__ __forceinline__ void warp_sums(Select& s, float warp_top, float m, float part) {
+  part = warp_sum(part * (m == -INFINITY || m == warp_top ? 1.0f : expf(m - warp_top)));
+  if ((threadIdx.x & 31) == 0) {
+    s.top[threadIdx.x >> 5] = warp_top;
+    s.sum[threadIdx.x >> 5] = part;
+  }
+}
+template <int WARPS>
+__device__ __forceinline__ void join_sums(Select& s, float& top, float& sum) {
+  const int lane = threadIdx.x & 31;
+  const float w = lane < WARPS ? s.top[lane] : -INFINITY;
+  top = key_float(__reduce_max_sync(0xffffffffu, value_key(w, kNanLowest)));
+  sum = warp_sum(lane < WARPS ? s.sum[lane] * (w == top ? 1.0f : expf(w - top)) : 0.f);
+}
+
+// best_pairs for a short row and a few pairs: a thread has at most five entries, so
+// every warp takes its K best one after the other (two reductions each), and those
+// of all warps are the result.  Half the time of a threshold at K = 4.
+template <int THREADS, uint32_t NAN_KEY, bool SUM>
+__device__ __forceinline__ int warp_bests(const Row& row, int K, Select& s, float m, float part,
+                                          float& top, float& sum) {
+  constexpr int kWarps = THREADS / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = threadIdx.x;
+  uint32_t key[5];                    // 0: no entry
+  uint32_t at[5];
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (t < row.groups) v = row.mid[t];
+  const float values[5] = {v.x, v.y, v.z, v.w, row.single >= 0 ? row.p[row.single] : 0.f};
+#pragma unroll
+  for (int k = 0; k < 5; ++k) {
+    const bool here = k < 4 ? t < row.groups : row.single >= 0;
+    key[k] = here ? value_key(values[k], NAN_KEY) : 0u;
+    at[k] = k < 4 ? (uint32_t)(row.head + 4 * t + k) : (uint32_t)row.single;
+  }
+  for (int r = 0; r < K; ++r) {
+    uint32_t best = key[0], i = at[0];
+#pragma unroll
+    for (int k = 1; k < 5; ++k)
+      if (key[k] > best || (key[k] == best && key[k] != 0 && at[k] < i)) {
+        best = key[k];
+        i = at[k];
+      }
+    const uint32_t first = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t where = __reduce_min_sync(0xffffffffu, best == first ? i : 0xffffffffu);
+    if (SUM && r == 0) warp_sums(s, first ? key_float(first) : -INFINITY, m, part);
+    if (lane == 0) s.pair[warp * K + r] = first ? ((uint64_t)first << 32) | (uint32_t)~where : 0;
+#pragma unroll
+    for (int k = 0; k < 5; ++k)
+      if (key[k] == first && at[k] == where) key[k] = 0;
+  }
+  __syncthreads();
+  if (SUM) join_sums<kWarps>(s, top, sum);
+  return kWarps * K;
+}
+
 // Puts the row's K best pairs, and perhaps more of its best, into s.pair and
 // returns how many (K <= V).  With SUM, top and sum come to hold the row's largest
 // number and the sum of exp(v - top).
@@ -222,21 +278,15 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
     }
     m = n;
   }
+  if (row.groups <= THREADS && K <= kMaxBeams && K * kWarps <= 256)
+    return warp_bests<THREADS, NAN_KEY, SUM>(row, K, s, m, part, top, sum);
   // the nth largest of the warp's lanes (of their largest entries)
   uint32_t o = value_key(m, NAN_KEY);
   constexpr int kMost = kWarps * 2 / 3;
   const int nth = (K + kMost - 1) / kMost < 32 ? (K + kMost - 1) / kMost : 32;
   const int mth = (K + nth - 1) / nth;         // <= warps: K <= 32 warps
   uint32_t reach = __reduce_max_sync(0xffffffffu, o);
-  if (SUM) {
-    const float w = key_float(reach);
-    part *= m == -INFINITY || m == w ? 1.0f : expf(m - w);
-    part = warp_sum(part);
-    if (lane == 0) {
-      s.top[warp] = w;
-      s.sum[warp] = part;
-    }
-  }
+  if (SUM) warp_sums(s, key_float(reach), m, part);
   if (nth <= 4) {
     for (int k = 1; k < nth; ++k) {      // without the lane that had it
       if (lane == __ffs(__ballot_sync(0xffffffffu, o == reach)) - 1) o = 0;
@@ -251,11 +301,7 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
     const uint32_t order = descending(lane < kWarps ? s.reach[lane] : 0u);
     if (lane == mth - 1) s.tau = key_float(order);
   }
-  if (SUM) {
-    const float w = lane < kWarps ? s.top[lane] : -INFINITY;
-    top = key_float(__reduce_max_sync(0xffffffffu, value_key(w, NAN_KEY)));
-    sum = warp_sum(lane < kWarps ? s.sum[lane] * (w == top ? 1.0f : expf(w - top)) : 0.f);
-  }
+  if (SUM) join_sums<kWarps>(s, top, sum);
   __syncthreads();
   const float tau = s.tau;
   // all pairs of a short row, else those that reach tau (NaN counts as reaching
@@ -306,7 +352,8 @@ __device__ __forceinline__ uint64_t sorted_pair(Select& s, int n) {
   return mine;
 }
 
-// Calls put(rank, pair) for the K best of the n pairs in s.pair (all different).
+// Calls put(rank, pair) for the K best of the n pairs in s.pair (all different, but
+// for zeros in the place of missing ones, which rank behind K pairs).
 // Up to 64 of them are counted against each other, a few neighbouring threads
 // sharing a pair's count; more are sorted, a pair a thread (n^2 / 32 reads of
 // shared memory by a warp against log^2 n / 2 exchanges), or counted where threads
