@@ -26,7 +26,7 @@ constexpr int kMaxTopk = 256;
 constexpr int kMaxBeams = 16;
 constexpr int kMaxStates = 128;
 constexpr int kCandidates = 2048;     // of a row, in shared memory
-constexpr int kClusterBlocks = 8;     // blocks that share a batch item's rows
+constexpr int kClusterBlocks = 8;     // blocks that share a batch item's rows, at most
 
 // The order-preserving bits of a value (-0 counts as +0); nan_key is what a NaN
 // counts as.
@@ -263,18 +263,32 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
   if (NAN_KEY == kNanLowest && m != m) m = -INFINITY;
   float part = 0.f;
   if (SUM && row.single >= 0 && row.p[row.single] != -INFINITY) part = expf(row.p[row.single] - m);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < row.groups; i += THREADS) {
-    const float4 v = row.mid[i];
-    const float n = largest<NAN_KEY>(largest<NAN_KEY>(m, v.x, v.y), v.z, v.w);
-    if (SUM && n != -INFINITY) {
+  // four groups at a time: their largest against the thread's so far, one rescaling
+  // of its sum of exponentials
+  constexpr int kAhead = 4;
+  for (int i = threadIdx.x; i < row.groups; i += kAhead * THREADS) {
+    float4 v[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      v[k] = i + k * THREADS < row.groups
+                 ? row.mid[i + k * THREADS]
+                 : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    float n = m;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      n = largest<NAN_KEY>(largest<NAN_KEY>(n, v[k].x, v[k].y), v[k].z, v[k].w);
+    if (SUM) {
+      // nothing but -inf (and perhaps NaN) so far: shifted by any number, they are 0
+      const float shift = n == -INFINITY ? 0.f : n;
       if (n > m) part *= fast_exp2((m - n) * 1.4426950408889634f);
-      part += (fast_exp2((v.x - n) * 1.4426950408889634f) +
-               fast_exp2((v.y - n) * 1.4426950408889634f)) +
-              (fast_exp2((v.z - n) * 1.4426950408889634f) +
-               fast_exp2((v.w - n) * 1.4426950408889634f));
-    } else if (SUM) {
-      part += (v.x + v.y) + (v.z + v.w) == -INFINITY ? 0.f : NAN;   // nothing but -inf, or NaN
+      float e = 0.f;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        e += (fast_exp2((v[k].x - shift) * 1.4426950408889634f) +
+              fast_exp2((v[k].y - shift) * 1.4426950408889634f)) +
+             (fast_exp2((v[k].z - shift) * 1.4426950408889634f) +
+              fast_exp2((v[k].w - shift) * 1.4426950408889634f));
+      part += e;
     }
     m = n;
   }
@@ -414,6 +428,7 @@ __global__ void __launch_bounds__(THREADS, 2048 / THREADS)
 // which merges them all:
 //   score = scores[w] + ((z - top_w) - log sum_w)
 constexpr int kMostPieces = kMaxBeams > kClusterBlocks ? kMaxBeams : kClusterBlocks;
+static_assert(kMostPieces * kMaxBeams <= 256, "a thread a proposal");
 struct Merge {
   uint64_t pair[kMostPieces * kMaxBeams];       // 0: no pair
   float top[kMostPieces], sum[kMostPieces];
@@ -624,7 +639,9 @@ WXX_EXPORT int wxx_beam_select(float* new_scores, uint32_t* parents, uint32_t* t
   WXX_REQUIRE((finished == nullptr) == (new_finished == nullptr),
               "wxx_beam_select: finished and new_finished go together");
   if (B == 0) return WXX_OK;
-  // long rows of few beams are split so that the cluster's blocks all have a piece
+  // Long rows of few beams are split so that all blocks of the cluster have a piece
+  // (with clusters of 16 blocks, which are not portable, a step of 8 beams over 50304
+  // tokens took 9 us longer).
   const bool wide = V > 4096;
   const int parts = wide && W < kClusterBlocks ? kClusterBlocks / W : 1;
   const int blocks = W * parts < kClusterBlocks ? W * parts : kClusterBlocks;
@@ -644,7 +661,7 @@ WXX_EXPORT int wxx_beam_select(float* new_scores, uint32_t* parents, uint32_t* t
     WXX_LAUNCH_CHECK();
     return WXX_OK;
   };
-  return wide ? launch(beam_select_kernel<1024>, 1024) : launch(beam_select_kernel<256>, 256);
+  return wide ? launch(beam_select_kernel<512>, 512) : launch(beam_select_kernel<256>, 256);
 }
 
 // Moves the rows of n state tensors in place: row b W + w of each takes what
