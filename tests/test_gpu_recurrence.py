@@ -95,6 +95,33 @@ def test_forward_and_backward(B, T, D, H, h0, reset, rng):
         close(dh0.numpy(), rdh0, bound)
 
 
+# enough tiles for two channels a lane: even and odd widths, gates of 1, 2, 3, 25 and 64
+# channels, rows of more than 128 tiles, a last block with one channel or none whole
+MANY = [(8, 2100, 190, 190), (4, 4097, 131, 131), (7, 3001, 128, 64), (3, 17000, 66, 22),
+        (17, 1025, 100, 4), (6, 3100, 192, 3), (40, 900, 65, 65), (38, 129, 256, 256)]
+
+
+@pytest.mark.parametrize("B,T,D,H", MANY)
+@pytest.mark.parametrize("h0,reset", [(False, False), (True, True)])
+def test_many_tiles(B, T, D, H, h0, reset, rng):
+    test_forward_and_backward(B, T, D, H, h0, reset, rng)
+
+
+def test_many_tiles_strided(rng):
+    """Column slices at odd and even offsets, and an odd number of channels."""
+    F = _F()
+    B, T, D = 9, 1500, 102
+    both = rng.standard_normal((B, T, 3 * D)).astype(np.float32)
+    t = up(both)
+    for a, b, n in ((0, 2 * D, D), (1, 2 * D, D), (2, D + 1, D - 1), (4, 2 * D, D - 2)):
+        x, gate = t[..., a:a + n], t[..., b:b + n]
+        h, last = F.gated_recurrence(x, gate)
+        same, same_last = F.gated_recurrence(up(both[..., a:a + n]), up(both[..., b:b + n]))
+        assert np.array_equal(h.numpy(), same.numpy())
+        assert np.array_equal(last.numpy(), same_last.numpy())
+        assert np.array_equal(last.numpy(), h.numpy()[:, -1])
+
+
 def test_gradient_against_differences(rng):
     """The kernels' own forward, differenced: the loss is linear in x and h0, so a
     wide step loses nothing there; in the gate the truncation is step^2 / 6 of the
