@@ -274,6 +274,61 @@ def test_same_bits_every_time(rng):
             assert np.array_equal(a, b)
 
 
+def test_scans_of_all_sizes_one_after_another(rng):
+    """What one call leaves in the scan's scratch means nothing to the next, larger or
+    smaller, forward or backward, recorded or not."""
+    F = _F()
+    import wxx_b200 as wxx
+
+    sizes = [(1, 300, 40), (2, 20000, 32), (1, 129, 33), (3, 4100, 70), (1, 300, 40), (6, 2050, 256)]
+    t = [tuple(up(v) for v in inputs(rng, B, T, D, D, True, True)[:3]) for B, T, D in sizes]
+
+    def one(k):
+        h, last = F.gated_recurrence(*t[k])
+        return [h, last, *F.gated_recurrence_backward(t[k][0], t[k][0], t[k][1], h, t[k][2])]
+
+    ref = [[v.numpy() for v in one(k)] for k in range(len(sizes))]
+    graphs = [wxx.graph.capture(one, k) for k in (3, 1)]
+    for _ in range(3):
+        for k in rng.permutation(len(sizes)):
+            out = one(int(k))
+            graphs[0].replay()
+            graphs[1].replay()
+            for a, b in zip(out, ref[k]):
+                assert np.array_equal(a.numpy(), b)
+    for g, k in zip(graphs, (3, 1)):
+        for a, b in zip(g.output, ref[k]):
+            assert np.array_equal(a.numpy(), b)
+        g.close()
+    assert wxx.backend.device_status() == 0
+
+
+def test_on_another_stream(rng):
+    """The library stream changed between calls: each stream has its own scratch."""
+    import torch
+
+    F = _F()
+    import wxx_b200 as wxx
+    from wxx_b200.backend.lib import F as C, check
+
+    x, gate, h0, _ = inputs(rng, 2, 5000, 64, 64, True, False)
+    a = up(x), up(gate), up(h0)
+    ref = F.gated_recurrence(*a)[0].numpy()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    try:
+        for k in range(6):
+            check(C.wxx_sync())
+            check(C.wxx_set_stream(streams[k % 2].cuda_stream))
+            h = F.gated_recurrence(*a)[0]
+            assert np.array_equal(h.numpy(), ref)
+            del h
+            check(C.wxx_sync())
+    finally:
+        check(C.wxx_set_stream(None))
+    assert np.array_equal(F.gated_recurrence(*a)[0].numpy(), ref)
+    assert wxx.backend.device_status() == 0
+
+
 def test_offsets_past_32_bits():
     """A sequence batch whose last rows lie past 2^32 bytes and 2^31 elements."""
     F = _F()
