@@ -201,6 +201,33 @@ def test_strided_logits_and_empty_batch(rng):
                                    up(ids[:0], np.uint32), stats).shape == [0, 101]
 
 
+def test_offsets_past_32_bits(rng):
+    """43000 x 50304 logits (2^31 of them, 8.7 GB): the last rows against the same
+    rows on their own."""
+    F = _F()
+    import wxx_b200 as wxx
+
+    N, V, K, n = 43000, 50304, 4, 3
+    z, top, ids = problem(rng, n, V, K, False)
+    big = wxx.Tensor((N, V), value=0.25)
+    F.assign(big.narrow(0, N - n, n), up(z))
+    all_top, all_ids = np.zeros((N, K), np.float32), np.tile(np.arange(K, dtype=np.uint32), (N, 1))
+    all_top[N - n:], all_ids[N - n:] = top, ids
+    loss, stats = F.distill_loss(big, up(all_top), up(all_ids, np.uint32))
+    ref, rstats = F.distill_loss(up(z), up(top), up(ids, np.uint32))
+    # (a row on its own may be summed in more pieces)
+    bl, bg = bounds(z, top, 1.0)
+    assert np.abs(loss.numpy()[N - n:] - ref.numpy()).max() <= 2 * bl
+    # uniform student over V against uniform teacher over K
+    assert np.abs(loss.numpy()[0] - np.log(V / K)) <= bl
+    grad = np.ones((N, 1), np.float32)
+    d = F.distill_loss_backward(up(grad), big, up(all_top), up(all_ids, np.uint32), stats)
+    tail = d.narrow(0, N - n, n).numpy()
+    rd = F.distill_loss_backward(up(grad[:n]), up(z), up(top), up(ids, np.uint32), rstats).numpy()
+    assert np.abs(tail - rd).max() <= 2 * bg
+    assert wxx.backend.device_status() == 0
+
+
 def test_module_with_mask_trains_the_logits(rng):
     import wxx_b200 as wxx
 

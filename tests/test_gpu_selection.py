@@ -96,6 +96,39 @@ def test_topk_shapes(rng):
     assert F.topk(up(np.zeros((0, 9))), 3)[0].shape == [0, 3]
 
 
+def test_topk_offsets_past_32_bits(rng):
+    """43000 x 50304 entries (2^31 of them, 8.7 GB): rows of one value, and the last."""
+    F = _F()
+    import wxx_b200 as wxx
+
+    N, V, n = 43000, 50304, 2
+    x = rng.standard_normal((n, V)).astype(np.float32)
+    big = wxx.Tensor((N, V), value=-1.5)
+    F.assign(big.narrow(0, N - n, n), up(x))
+    values, ids = F.topk(big, 3)
+    rv, ri = recurrent.topk(x, 3)
+    assert np.array_equal(ids.numpy()[N - n:], ri) and np.array_equal(values.numpy()[N - n:], rv)
+    assert np.array_equal(ids.numpy()[:N - n], np.tile([0, 1, 2], (N - n, 1)))
+    assert wxx.backend.device_status() == 0
+
+
+def test_reorder_offsets_past_32_bits(rng):
+    """States of 3 x 1.5 GB rows: the last words of the last beam."""
+    F = _F()
+    import wxx_b200 as wxx
+
+    row = 400_000_000
+    t = wxx.Tensor((3, row), value=0.0)
+    for w in range(3):
+        F.assign(t.narrow(0, w, 1), float(w + 1))
+        F.assign(t.narrow(0, w, 1).narrow(1, row - 5, 5), float(10 * (w + 1)))
+    F.beam_reorder([t], up([[2, 2, 0]], np.uint32))
+    for w, p in enumerate((2, 2, 0)):
+        assert np.all(t.narrow(0, w, 1).narrow(1, row - 9, 4).numpy() == p + 1)
+        assert np.all(t.narrow(0, w, 1).narrow(1, row - 5, 5).numpy() == 10 * (p + 1))
+    assert wxx.backend.device_status() == 0
+
+
 def beams(rng, B, W, V, done):
     z = (rng.standard_normal((B * W, V)) * 3).astype(np.float32)
     s = (-10 - 2 * rng.random((B, W))).astype(np.float32)

@@ -85,11 +85,15 @@ class DeviceBuffer:
     __slots__ = ("ptr", "size", "label", "uid", "version", "__weakref__")
 
     def __init__(self, nbytes, label="Tensor"):
-        ensure_init()
+        if not _ctx.ready:
+            _ctx.init()
         p = ctypes.c_void_p()
-        check(F.wxx_malloc(ctypes.byref(p), int(nbytes)), f"wxx_malloc({nbytes})")
+        nbytes = int(nbytes)
+        status = F.wxx_malloc(ctypes.byref(p), nbytes)
+        if status:
+            check(status, f"wxx_malloc({nbytes})")
         self.ptr = p.value
-        self.size = int(nbytes)
+        self.size = nbytes
         self.label = label
         self.uid = next(_buffer_uids)
         self.version = 0

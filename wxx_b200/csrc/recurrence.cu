@@ -21,9 +21,7 @@
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
-#include <map>
 #include <mutex>
-#include <utility>
 
 WXX_EXPORT int wxx_malloc(void** out, uint64_t nbytes);
 WXX_EXPORT int wxx_free(void* p);
@@ -256,9 +254,10 @@ __device__ __forceinline__ void copy_gates(float* tile, const Operand& g, const 
 // Joins the pieces of a tile (warp i of the order holds piece `mine`) with
 // everything before it.  j: the tile's place in its row, q: its channel block.
 // Returns the state before this warp's piece.  The order of the additions
-// depends on j alone: the tiles of the same group (kWarps segments of kSeg tiles,
-// one looked at by each warp) so far, then the state after the group before.  fetch_next is called once, when every
-// warp has taken its inputs from shared memory.
+// depends on j alone: the state after the group before, the tiles of the same group
+// so far (kWarps segments of kSeg tiles, one looked at by each warp), the pieces.
+// fetch_next is called once, when every warp has taken its inputs from shared
+// memory.
 template <int kSeg, class F>
 __device__ __forceinline__ float join_tile(const Chain& c, Joint& s, int turn, const Place& p,
                                            Stretch mine, float start, F fetch_next) {
@@ -648,16 +647,33 @@ int group_tiles(const Chain& c) { return kWarps * (long_rows(c) ? kLongSeg : kSh
 
 // Scratch of at least `bytes`.  Each stream keeps its own, zero when it is new, so
 // scans on two streams do not meet.  A recorded launch may be replayed beside
-// either, so it has scratch of its own in the recording, cleared before it: *own,
-// for the caller to free.
+// either, so it has scratch of its own in the recording, cleared before it; so has
+// a launch on a stream past the sixteenth.  *own is such scratch, for the caller to
+// free.
 int scan_scratch(size_t bytes, char** p, void** own) {
+  struct Kept {
+    cudaStream_t stream;
+    char* p;
+    size_t size;
+  };
   static std::mutex mu;
-  static std::map<cudaStream_t, std::pair<char*, size_t>> kept;
+  static Kept kept[16];
+  static int n = 0;
   cudaStream_t stream = wxx::stream();
   *own = nullptr;
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
   WXX_CUDA_CHECK(cudaStreamIsCapturing(stream, &cs));
-  if (cs != cudaStreamCaptureStatusNone) {
+  std::lock_guard<std::mutex> lock(mu);
+  Kept* mine = nullptr;
+  if (cs == cudaStreamCaptureStatusNone) {
+    for (int i = 0; i < n && !mine; ++i)
+      if (kept[i].stream == stream) mine = &kept[i];
+    if (!mine && n < 16) {
+      mine = &kept[n++];
+      *mine = {stream, nullptr, 0};
+    }
+  }
+  if (!mine) {
     if (int st = wxx_malloc(own, bytes)) return st;
     *p = static_cast<char*>(*own);
     cudaError_t e = cudaMemsetAsync(*p, 0, bytes, stream);
@@ -667,19 +683,25 @@ int scan_scratch(size_t bytes, char** p, void** own) {
     wxx::set_error("clearing a scan's scratch failed: %s", cudaGetErrorString(e));
     return WXX_E_CUDA;
   }
-  std::lock_guard<std::mutex> lock(mu);
-  auto& mine = kept[stream];
-  if (mine.second < bytes) {
+  if (mine->size < bytes) {
     size_t size = 1 << 20;
     while (size < bytes) size <<= 1;
-    if (mine.first) WXX_CUDA_CHECK(cudaFreeAsync(mine.first, stream));
-    mine = {nullptr, 0};
+    char* old = mine->p;
+    mine->p = nullptr;
+    mine->size = 0;
+    if (old) WXX_CUDA_CHECK(cudaFreeAsync(old, stream));
     char* fresh = nullptr;
     WXX_CUDA_CHECK(cudaMallocAsync(reinterpret_cast<void**>(&fresh), size, stream));
-    WXX_CUDA_CHECK(cudaMemsetAsync(fresh, 0, size, stream));
-    mine = {fresh, size};
+    cudaError_t e = cudaMemsetAsync(fresh, 0, size, stream);
+    if (e != cudaSuccess) {
+      cudaFreeAsync(fresh, stream);
+      wxx::set_error("clearing a scan's scratch failed: %s", cudaGetErrorString(e));
+      return WXX_E_CUDA;
+    }
+    mine->p = fresh;
+    mine->size = size;
   }
-  *p = mine.first;
+  *p = mine->p;
   return WXX_OK;
 }
 

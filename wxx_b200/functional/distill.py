@@ -17,18 +17,25 @@ from ._common import F, check, compact, empty, empty_group
 _MAX_STORED = 1024
 
 
-def _operands(what, logits, top_logits, top_ids, temperature):
+def _refuse(what, logits, top_logits, top_ids):
+    """The message for operands that do not fit together."""
     for name, t, dtype in (("logits", logits, "f32"), ("top_logits", top_logits, "f32"),
                            ("top_ids", top_ids, "u32")):
         if t.type != dtype:
             raise TypeError(f"{what} expects {dtype} {name}, got {t.type!r}")
         if len(t.shape) != 2:
             raise ValueError(f"{what} expects a matrix of {name}, got {tuple(t.shape)}")
+    raise ValueError(f"{what}: top_logits {tuple(top_logits.shape)} and top_ids "
+                     f"{tuple(top_ids.shape)} do not match logits {tuple(logits.shape)}")
+
+
+def _operands(what, logits, top_logits, top_ids, temperature):
+    if (logits.type != "f32" or top_logits.type != "f32" or top_ids.type != "u32"
+            or len(logits.shape) != 2 or len(top_logits.shape) != 2
+            or top_ids.shape != top_logits.shape or top_logits.shape[0] != logits.shape[0]):
+        _refuse(what, logits, top_logits, top_ids)
     N, V = logits.shape
     K = top_logits.shape[1]
-    if top_logits.shape[0] != N or tuple(top_ids.shape) != (N, K):
-        raise ValueError(f"{what}: top_logits {tuple(top_logits.shape)} and top_ids "
-                         f"{tuple(top_ids.shape)} do not match logits {(N, V)}")
     if V < 1 or not 1 <= K <= _MAX_STORED:
         raise ValueError(f"{what}: needs at least one logit and 1 to {_MAX_STORED} stored ones, "
                          f"got {V} and {K}")

@@ -26,8 +26,9 @@ def _inner_dense(t):
 
 
 def _operands(x, gate, h0, reset):
-    _typed("x", x, "f32")
-    _typed("gate", gate, "f32")
+    if x.type != "f32" or gate.type != "f32":
+        _typed("x", x, "f32")
+        _typed("gate", gate, "f32")
     if len(x.shape) != 3 or len(gate.shape) != 3:
         raise ValueError(f"gated_recurrence expects x (batch, time, channels) and gate (batch, "
                          f"time, heads), got {tuple(x.shape)} and {tuple(gate.shape)}")
