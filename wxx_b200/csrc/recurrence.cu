@@ -639,10 +639,13 @@ int check_sizes(const char* what, int64_t B, int64_t T, int64_t D, int64_t H) {
 }
 
 // Tiles of a group.  Looking at more tiles costs every tile, a hop between groups
-// costs the row: at 64 tiles a row forward and backward took 78 + 139 us in groups of
-// 8, 84 + 160 in groups of 32; at 512 tiles a row the forward took 73 and 54 us.
+// (about 1.5 us) costs the row.  The rows are joined side by side, so the hops of
+// groups of 8 are hidden where the tiles of 8 positions of all rows take longer than
+// one: from about 24 blocks of 32 channels.  Forward in groups of 8 against 32: 72 and
+// 53 us with 8 blocks of 512 tiles, 40 and 39 us with 16 of 192, 46 and 47 us with 32 of
+// 128, 78 and 84 us with 128 of 64.
 constexpr int kShortSeg = 1, kLongSeg = 4;
-bool long_rows(const Chain& c) { return c.tiles > 128; }
+bool long_rows(const Chain& c) { return c.blocks.d < 24; }
 int group_tiles(const Chain& c) { return kWarps * (long_rows(c) ? kLongSeg : kShortSeg); }
 
 // Scratch of at least `bytes`.  Each stream keeps its own, zero when it is new, so

@@ -296,8 +296,9 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
     return warp_bests<THREADS, NAN_KEY, SUM>(row, K, s, m, part, top, sum);
   // the nth largest of the warp's lanes (of their largest entries)
   uint32_t o = value_key(m, NAN_KEY);
-  constexpr int kMost = kWarps * 2 / 3;
-  const int nth = (K + kMost - 1) / kMost < 32 ? (K + kMost - 1) / kMost : 32;
+  // (of the warps that have entries; tau is -inf where they are too few)
+  const int active = min(kWarps, (row.groups + 31) / 32), most = max(1, active * 2 / 3);
+  const int nth = min(32, (K + most - 1) / most);
   const int mth = (K + nth - 1) / nth;         // <= warps: K <= 32 warps
   uint32_t reach = __reduce_max_sync(0xffffffffu, o);
   if (SUM) warp_sums(s, key_float(reach), m, part);
@@ -614,10 +615,15 @@ WXX_EXPORT int wxx_topk(float* values, uint32_t* ids, const float* x, int64_t ld
   WXX_REQUIRE(K >= 1 && K <= kMaxTopk && K <= V, "wxx_topk: k = %d outside [1, min(%lld, %d)]", K,
               (long long)V, kMaxTopk);
   if (N == 0) return WXX_OK;
-  // 256 threads see a short row in a few loads; a long one, or a K that would take
-  // many of each warp's entries, is worth 1024
-  if (V <= 4096 && K <= 64)
+  // Small blocks hide one another's steps, but more rows are then under way and what
+  // is read again no longer comes from L2, and a large K takes most entries of few
+  // threads.  256 against 1024 threads: 1024 rows of 4096 at K = 32 12 and 29 us, of
+  // 16384 at K = 64 21 and 26 us, 4096 rows of 50304 247 and 150 us; 256, 512 and 1024
+  // threads for 1024 rows of 4096 at K = 128 64, 25 and 33 us.
+  if (V <= 16384 && K <= 64)
     topk_kernel<256><<<(unsigned)N, 256, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
+  else if (V <= 16384 && K <= 128)
+    topk_kernel<512><<<(unsigned)N, 512, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
   else
     topk_kernel<1024><<<(unsigned)N, 1024, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
   WXX_LAUNCH_CHECK();
@@ -639,11 +645,14 @@ WXX_EXPORT int wxx_beam_select(float* new_scores, uint32_t* parents, uint32_t* t
   WXX_REQUIRE((finished == nullptr) == (new_finished == nullptr),
               "wxx_beam_select: finished and new_finished go together");
   if (B == 0) return WXX_OK;
-  // Long rows of few beams are split so that all blocks of the cluster have a piece
-  // (with clusters of 16 blocks, which are not portable, a step of 8 beams over 50304
-  // tokens took 9 us longer).
-  const bool wide = V > 4096;
-  const int parts = wide && W < kClusterBlocks ? kClusterBlocks / W : 1;
+  // Where rows are long and few, those of fewer beams than the cluster has blocks are
+  // split, and blocks have 512 threads.  1 item of 4 beams over 50304 tokens took 10 us
+  // (12 us with a block of 256 threads a row), 8 of 8 beams 12 us (14 us); 32 of 4
+  // beams, more than one block an SM, 14 us with a block of 256 a row and 23 us split.
+  // (With clusters of 16 blocks, which are not portable, 8 of 8 beams took 9 us more.)
+  const bool few = V > 16384 && B * (W < kClusterBlocks ? kClusterBlocks / W * W : kClusterBlocks)
+                                    <= wxx::num_sms();
+  const int parts = few && W < kClusterBlocks ? kClusterBlocks / W : 1;
   const int blocks = W * parts < kClusterBlocks ? W * parts : kClusterBlocks;
   WXX_REQUIRE(B * blocks < (int64_t(1) << 31), "wxx_beam_select: too many rows");
   auto launch = [&](auto kernel, int threads) -> int {
@@ -661,7 +670,7 @@ WXX_EXPORT int wxx_beam_select(float* new_scores, uint32_t* parents, uint32_t* t
     WXX_LAUNCH_CHECK();
     return WXX_OK;
   };
-  return wide ? launch(beam_select_kernel<512>, 512) : launch(beam_select_kernel<256>, 256);
+  return few ? launch(beam_select_kernel<512>, 512) : launch(beam_select_kernel<256>, 256);
 }
 
 // Moves the rows of n state tensors in place: row b W + w of each takes what
