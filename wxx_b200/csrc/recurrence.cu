@@ -41,22 +41,39 @@ constexpr int kTile = kWarps * kSteps * 32;                // floats of a tile's
 constexpr int kForwardBlocks = 3, kBackwardBlocks = 2;     // resident on an SM
 constexpr int kWaitLimit = 1 << 21; // polls of a published word (about a second)
 
-// A gate as the smaller of its weights a and z = 1 - a, which says how much of
-// the other value is mixed in, and whether the state is the one that is kept.
-// With e = exp(-|g|) the smaller weight is e / (1 + e), good to a few ulp of
-// itself (e^(-|g|) carries half an ulp of |g| log2 e).
+// The weights of two gates (of neighbouring positions, so that the additions and
+// products go in pairs): with e = exp(-g), a = 1 / (1 + e) and z = 1 - a = e a, each
+// good to a few ulp of itself (e carries half an ulp of g log2 e, and 1 + e >= 1 is
+// what the approximate reciprocal takes to an ulp).  Where e overflows, a is 0 and z
+// is NaN unless kBounded, which keeps e at 2^126: then a is 2^-126 and z is 1.
+struct Weights {
+  float a, z;
+};
+template <bool kBounded>
+__device__ __forceinline__ void weights2(float g0, float g1, Weights& w0, Weights& w1) {
+  float y0, y1, e0, e1, s0, s1;
+  mul2(y0, y1, g0, g1, -1.4426950408889634f, -1.4426950408889634f);
+  if (kBounded) {
+    asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(y0) : "f"(y0));
+    asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(y1) : "f"(y1));
+  }
+  e0 = fast_exp2(y0);
+  e1 = fast_exp2(y1);
+  add2(s0, s1, e0, e1, 1.0f, 1.0f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(w0.a) : "f"(s0));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(w1.a) : "f"(s1));
+  mul2(w0.z, w1.z, e0, e1, w0.a, w1.a);
+}
+
+// A gate as the smaller of its weights, which says how much of the other value is
+// mixed in, and whether the state is the one that is kept.
 struct Gate {
   float w;
   bool keep;
 };
-__device__ __forceinline__ Gate gate_of(float g) {
-  const float e = fast_exp2(fabsf(g) * -1.4426950408889634f);
-  float r;                         // 1 + e is in [1, 2]: the approximate reciprocal
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));   // is good to an ulp
-  return {e * r, g >= 0.f};        // a NaN gives one
+__device__ __forceinline__ Gate gate_of(float g, Weights w) {
+  return {g >= 0.f ? w.z : w.a, g >= 0.f};       // a NaN gives one
 }
-__device__ __forceinline__ float weight_a(Gate g) { return g.keep ? 1.0f - g.w : g.w; }
-__device__ __forceinline__ float weight_z(Gate g) { return g.keep ? g.w : 1.0f - g.w; }
 
 // a h + z x as the larger-weighted of the two plus the smaller weight times
 // their difference: a constant gate's fixed point stays where it is (a and z,
@@ -422,13 +439,21 @@ __global__ void __launch_bounds__(kT, kForwardBlocks)
     auto first_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        // past the end: keep the state
-        const Gate gate = gate_of(kPlain || k < p.left ? sg[k * stride] : INFINITY);
-        if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
-        mine.b = mix(gate, mine.b, kPlain || k < p.left ? sx[k * 32] : 0.f);
-        mine.A *= weight_a(gate);
-        upto[k] = mine;
+      for (int k0 = 0; k0 < kSteps; k0 += 2) {
+        float g[2];
+        Weights w[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)              // past the end: keep the state
+          g[k] = kPlain || k0 + k < p.left ? sg[(k0 + k) * stride] : INFINITY;
+        weights2<false>(g[0], g[1], w[0], w[1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int k = k0 + e;
+          if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
+          mine.b = mix(gate_of(g[e], w[e]), mine.b, kPlain || k < p.left ? sx[k * 32] : 0.f);
+          mine.A *= w[e].a;
+          upto[k] = mine;
+        }
       }
     };
     if (whole) first_run(Yes{}); else first_run(No{});
@@ -504,20 +529,27 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
     auto first_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
-      for (int k = kSteps - 1; k >= 0; --k) {
-        const bool here = kPlain || k < p.left;
-        const Gate gate = gate_of(here ? sg[k * stride] : INFINITY);
-        float before = s_h[at + k * 32];
-        if (!kPlain && p.t0 + k == 0) before = h0 && here ? h0[state] : 0.f;
-        if (!kPlain && (cut >> k & 1)) before = 0.f;
-        // d a / d gate = a z
-        u[k] = (before - s_x[at + k * 32]) * fmaf(-gate.w, gate.w, gate.w);
-        z[k] = weight_z(gate);
-        G[k] = mine.b + (here ? s_d[at + k * 32] : 0.f);
-        const float a = weight_a(gate);
-        mine.b = a * G[k];
-        mine.A *= a;
-        if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
+      for (int k0 = kSteps - 2; k0 >= 0; k0 -= 2) {
+        float g[2], slope[2];
+        Weights w[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) g[k] = kPlain || k0 + k < p.left ? sg[(k0 + k) * stride] : INFINITY;
+        weights2<true>(g[0], g[1], w[0], w[1]);
+        mul2(slope[0], slope[1], w[0].a, w[1].a, w[0].z, w[1].z);    // d a / d gate
+#pragma unroll
+        for (int e = 1; e >= 0; --e) {
+          const int k = k0 + e;
+          const bool here = kPlain || k < p.left;
+          float before = s_h[at + k * 32];
+          if (!kPlain && p.t0 + k == 0) before = h0 && here ? h0[state] : 0.f;
+          if (!kPlain && (cut >> k & 1)) before = 0.f;
+          u[k] = (before - s_x[at + k * 32]) * slope[e];
+          z[k] = w[e].z;
+          G[k] = mine.b + (here ? s_d[at + k * 32] : 0.f);
+          mine.b = w[e].a * G[k];
+          mine.A *= w[e].a;
+          if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
+        }
       }
     };
     if (whole) first_run(Yes{}); else first_run(No{});
@@ -591,7 +623,10 @@ __global__ void recurrence_step_kernel(float* __restrict__ state, const float* _
   for (int64_t i = (int64_t)blockIdx.x * kT + threadIdx.x; i < n;
        i += (int64_t)gridDim.x * kT) {
     const unsigned b = (unsigned)i / D, d = (unsigned)i - b * D;
-    state[i] = mix(gate_of(g[b * g_ld + d / per]), state[i], x[b * x_ld + d]);
+    const float gate = g[b * g_ld + d / per];
+    Weights w, same;
+    weights2<false>(gate, gate, w, same);
+    state[i] = mix(gate_of(gate, w), state[i], x[b * x_ld + d]);
   }
 }
 
