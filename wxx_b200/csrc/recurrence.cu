@@ -557,8 +557,7 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
                         next);
     const int64_t last = (int64_t)p.b * T + p.t0 + kSteps - 1;
     float* xo = dx + last * D + p.d;
-    float* go = dg + last * heads + (DG == 0 ? p.d : p.d / lanes);
-    const bool writes = DG == 0 || p.d % lanes == 0;
+    float* go = DG == 0 ? dg + last * D + p.d : nullptr;
     // What the join gives reaches position k through the weights after it: 1 - z
     // is a to 2^-24, which is enough for a product that only scales the carry.
     float carried = v;
@@ -568,26 +567,43 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
       for (int k = kSteps - 1; k >= 0; --k) {
         const float total = G[k] + carried;
         if (kPlain || k < p.left) *xo = z[k] * total;
-        float e = u[k] * total;
-        if (DG == 32) {
-          u[k] = e;
-        } else {
-          if (DG == 1) {
-            if (!kPlain && k >= p.left) e = 0.f;
-            for (int o = 1; o < lanes; o <<= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
-          }
-          if ((kPlain || k < p.left) && writes) *go = e;
-        }
+        u[k] *= total;
+        if (DG == 0 && (kPlain || k < p.left)) *go = u[k];
         carried *= 1.0f - z[k];
         if (!kPlain && (cut >> k & 1)) carried = 0.f;
         xo -= D;
-        go -= heads;
+        if (DG == 0) go -= D;
       }
     };
     if (whole) second_run(Yes{}); else second_run(No{});
+    if (DG == 1) {
+      // 16 sums over the lanes of a head: every exchange halves the sums that a lane
+      // still carries (14 exchanges over 8 lanes where one sum at a time takes 48);
+      // positions past the end are 0, their weight z a being so
+      const int lane = threadIdx.x & 31;
+      int first = 0, n_mine = kSteps;          // the lane's positions
+#pragma unroll
+      for (int n = kSteps / 2, step = 1; n > 0; n >>= 1, ++step) {
+        const int o = lanes >> step;
+        if (o == 0) break;
+        const bool upper = lane & o;
+#pragma unroll
+        for (int k = 0; k < n; ++k) {
+          const float keep = upper ? u[k + n] : u[k], send = upper ? u[k] : u[k + n];
+          u[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+        first += upper ? n : 0;
+        n_mine = n;
+      }
+      float* out = dg + ((int64_t)p.b * T + p.t0 + first) * heads + p.d / lanes;
+#pragma unroll
+      for (int k = 0; k < kSteps / 2; ++k) {
+        if (k < n_mine && first + k < p.left) *out = u[k];
+        out += heads;
+      }
+    }
     if (DG == 32) {
-      // 16 sums over 32 lanes: every exchange halves the sums that a lane still
-      // carries, 16 exchanges in all where one sum at a time takes 80
+      // the same over the whole warp: 16 exchanges where one sum at a time takes 80
       const int lane = threadIdx.x & 31;
 #pragma unroll
       for (int n = kSteps / 2, o = 16; n > 0; n >>= 1, o >>= 1)
