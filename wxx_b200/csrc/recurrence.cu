@@ -38,7 +38,12 @@ constexpr int kT = 256;
 constexpr int kSteps = 16;          // positions of a thread
 constexpr int kWarps = 8;           // pieces of a tile, at most
 constexpr int kTile = kWarps * kSteps * 32;                // floats of a tile's operand
-constexpr int kForwardBlocks = 3, kBackwardBlocks = 2;     // resident on an SM
+// Blocks resident on an SM.  Four of the forward's leave 64 registers a thread (two
+// are spilled).  Measured with four and with three: 68 and 70 us over (32, 1024, 1024)
+// with a gate per 64 channels, 18.5 and 20.4 over (64, 128, 1024); but 60 and 54 over
+// (1, 65536, 256), whose groups are longer, and 21 and 20 without the copy engine.
+constexpr int forward_blocks(bool tma, int seg) { return tma && seg == 1 ? 4 : 3; }
+constexpr int kBackwardBlocks = 2;
 constexpr int kWaitLimit = 1 << 21; // polls of a published word (about a second)
 
 // The weights of two gates (of neighbouring positions, so that the additions and
@@ -412,7 +417,7 @@ __device__ __forceinline__ float* aligned_smem(float* p) {
 // (85 us: the tiles it holds back are the ones that others wait for), pieces of 8 (95
 // us) and 32 positions (76 us forward, 151 backward), groups of groups (83 and 66 us).
 template <bool kTma, int kSeg>
-__global__ void __launch_bounds__(kT, kForwardBlocks)
+__global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
     recurrence_forward_kernel(float* __restrict__ h, float* __restrict__ h_last,
                               const __grid_constant__ CUtensorMap map_x,
                               const __grid_constant__ CUtensorMap map_g, Operand x, Operand g,
@@ -770,9 +775,14 @@ int scan_scratch(size_t bytes, char** p, void** own) {
   return WXX_OK;
 }
 
-// Threads and blocks of a scan, and its scratch (*own is freed by the caller).
-int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, int64_t H, int resident, Chain& c,
-              unsigned& threads, unsigned& grid, void** own) {
+unsigned scan_grid(const Chain& c, int resident) {
+  const unsigned most = (unsigned)(wxx::num_sms() * resident);
+  return c.total < most ? c.total : most;
+}
+
+// Threads and tiles of a scan, and its scratch (*own is freed by the caller).
+int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, int64_t H, Chain& c,
+              unsigned& threads, void** own) {
   const int64_t pieces = (T + kSteps - 1) / kSteps;
   const int64_t warps = pieces < kWarps ? pieces : kWarps;
   c = Chain{};
@@ -787,8 +797,6 @@ int plan_scan(const char* what, int64_t B, int64_t T, int64_t D, int64_t H, int 
   WXX_REQUIRE(total < (int64_t(1) << 31), "%s: too many elements", what);
   c.blocks = Divider::of((unsigned)blocks);
   c.total = (unsigned)total;
-  const int64_t most = (int64_t)wxx::num_sms() * resident;
-  grid = (unsigned)(total < most ? total : most);
   if (c.tiles == 1) return WXX_OK;
   const int64_t size = group_tiles(c), groups = (c.tiles + size - 1) / size;
   const size_t tile_bytes = (size_t)total * 32 * sizeof(ulonglong2);
@@ -840,27 +848,27 @@ WXX_EXPORT int wxx_gated_recurrence(float* h, float* h_last, const float* x, int
   if (T == 0) return copy_state(h_last, h0, B * D);
   const Operand ox{x, x_bs, x_ts}, og{gate, g_bs, g_ts};
   Chain c;
-  unsigned threads, grid;
+  unsigned threads;
   void* scratch;
-  if (int st = plan_scan("wxx_gated_recurrence", B, T, D, H, kForwardBlocks, c, threads, grid,
-                         &scratch))
-    return st;
+  if (int st = plan_scan("wxx_gated_recurrence", B, T, D, H, c, threads, &scratch)) return st;
   constexpr int kBytes = 2 * kTile * sizeof(float) + 128;
   CUtensorMap mx{}, mg{};
   const unsigned steps = threads / 32 * kSteps;
   const bool tma = encode_operand(&mx, ox, B, T, D, steps) &&
                    (c.per.d > 1 || encode_operand(&mg, og, B, T, D, steps));
-  auto launch = [&](auto kernel) {
+  auto launch = [&](auto kernel, int resident) {
     if (int st = allow_smem(kernel, kBytes)) return st;
-    kernel<<<grid, threads, kBytes, wxx::stream()>>>(h, h_last, mx, mg, ox, og, h0, reset, (int)T,
-                                                     (int)D, c);
+    kernel<<<scan_grid(c, resident), threads, kBytes, wxx::stream()>>>(
+        h, h_last, mx, mg, ox, og, h0, reset, (int)T, (int)D, c);
     return wxx::after_launch(__FILE__, __LINE__);
   };
-  const int st =
-      long_rows(c) ? (tma ? launch(recurrence_forward_kernel<true, kLongSeg>)
-                          : launch(recurrence_forward_kernel<false, kLongSeg>))
-                   : (tma ? launch(recurrence_forward_kernel<true, kShortSeg>)
-                          : launch(recurrence_forward_kernel<false, kShortSeg>));
+  auto pick = [&](auto t, auto seg) {
+    constexpr bool kTma = decltype(t)::value;
+    constexpr int kSeg = decltype(seg)::value ? kLongSeg : kShortSeg;
+    return launch(recurrence_forward_kernel<kTma, kSeg>, forward_blocks(kTma, kSeg));
+  };
+  const int st = long_rows(c) ? (tma ? pick(Yes{}, Yes{}) : pick(No{}, Yes{}))
+                              : (tma ? pick(Yes{}, No{}) : pick(No{}, No{}));
   if (scratch) wxx_free(scratch);
   return st;
 }
@@ -887,15 +895,14 @@ WXX_EXPORT int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0
   const int64_t parts = warp ? per / 32 : per;
   const Operand ox{x, x_bs, x_ts}, og{gate, g_bs, g_ts}, od{dh, T * D, D}, oh{h, T * D, D};
   Chain c;
-  unsigned threads, grid;
+  unsigned threads;
   void *scratch = nullptr, *wide = nullptr;
   float* sums = dgate;
   if (!inside) {
     if (int st = wxx_malloc(&wide, (uint64_t)(B * T * H * parts) * sizeof(float))) return st;
     sums = static_cast<float*>(wide);
   }
-  int st = plan_scan("wxx_gated_recurrence_backward", B, T, D, H, kBackwardBlocks, c, threads, grid,
-                     &scratch);
+  int st = plan_scan("wxx_gated_recurrence_backward", B, T, D, H, c, threads, &scratch);
   if (st == WXX_OK) {
     constexpr int kBytes = 4 * kTile * sizeof(float) + 128;
     CUtensorMap mx{}, mg{}, md{}, mh{};
@@ -906,8 +913,8 @@ WXX_EXPORT int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0
                      (c.per.d > 1 || encode_operand(&mg, og, B, T, D, steps));
     auto launch = [&](auto kernel) {
       if (int e = allow_smem(kernel, kBytes)) return e;
-      kernel<<<grid, threads, kBytes, wxx::stream()>>>(dx, sums, dh0, mx, mg, md, mh, ox, og, od,
-                                                       oh, dlast, h0, reset, (int)T, (int)D, c);
+      kernel<<<scan_grid(c, kBackwardBlocks), threads, kBytes, wxx::stream()>>>(
+          dx, sums, dh0, mx, mg, md, mh, ox, og, od, oh, dlast, h0, reset, (int)T, (int)D, c);
       return wxx::after_launch(__FILE__, __LINE__);
     };
     auto pick = [&](auto t, auto seg) {
