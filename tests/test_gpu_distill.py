@@ -182,6 +182,37 @@ def test_id_outside_the_vocabulary(rng):
     assert wxx.backend.device_status() == 0
 
 
+def test_absent_entries_beside_foreign_ones(rng):
+    """A NaN or an infinity among a row's stored logits makes its loss NaN, and the
+    gradient where it is stored; the entries that are not there stay without effect,
+    whatever their ids."""
+    F = _F()
+    N, V, K = 6, 5000, 40
+    z, top, ids = problem(rng, N, V, K, False)
+    top[:, 20:] = -np.inf
+    ids[:, 20:] = np.uint32(0xFFFFFFFF)
+    ids[3, 20:] = np.argsort(z[3])[:20]
+    top[1, 0] = top[3, 7] = np.nan
+    top[2, 3] = np.inf
+    loss, stats = F.distill_loss(up(z), up(top), up(ids, np.uint32), 2.0)
+    grad = np.ones((N, 1), np.float32)
+    d = F.distill_loss_backward(up(grad), up(z), up(top), up(ids, np.uint32), stats, 2.0).numpy()
+    loss = loss.numpy()
+    safe = np.where(top == -np.inf, 0, ids)
+    for n in range(N):
+        if n not in (1, 2, 3):
+            want = recurrent.distill(z[n:n + 1], top[n:n + 1], safe[n:n + 1], 2.0)[0]
+            assert abs(loss[n, 0] - want[0, 0]) <= 4 * bounds(z[n:n + 1], top[n:n + 1], 2.0)[0]
+            continue
+        assert np.isnan(loss[n, 0])
+        stored = np.zeros(V, bool)
+        stored[ids[n, :20]] = True
+        assert np.isnan(d[n, stored]).all() and np.isfinite(d[n, ~stored]).all()
+    import wxx_b200 as wxx
+
+    assert wxx.backend.device_status() == 0
+
+
 def test_strided_logits_and_empty_batch(rng):
     F = _F()
     z, top, ids = problem(rng, 6, 101, 9, False)

@@ -174,7 +174,8 @@ __global__ void __launch_bounds__(kT)
   if (some)
     for (int k = threadIdx.x; k < K; k += kT) {
       const float t = (s_t[k] - t_top) * inv_tau, p = expf(t) * inv;
-      if (!(p == 0.f))
+      // an entry that is not there may have any id, and a p of NaN from one that is
+      if (s_t[k] != -INFINITY && !(p == 0.f))
         sum += p * ((t - log_t) - ((z[ids[at * K + k]] - s.top) * inv_tau - log_s));
     }
   sum = block_sum(sum, red);
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(kT)
       const uint32_t j = ids[at * K + k];
       const float t = stored(top[at * K + k], j, V, part == 0 ? err : nullptr);
       s_id[k] = j;
-      s_p[k] = expf((t - st.z) * inv_tau) * inv_t;
+      s_p[k] = t == -INFINITY ? 0.f : expf((t - st.z) * inv_tau) * inv_t;
     }
   }
   auto value = [&](float v) { return some ? g * (scaled_exp(v, m, c) * inv) : 0.f; };
