@@ -262,6 +262,24 @@ def test_beam_reorder_bad_parent(rng):
     assert np.array_equal(t.numpy(), v[[1, 1, 0, 3]])
 
 
+@pytest.mark.parametrize("W", [1, 3, 5, 7, 9, 15])
+def test_beam_reorder_parent_just_outside(W, rng):
+    """A parent of beams or a little more leaves its row as it was: the next item's
+    rows, or what lies behind the last one's, are not read."""
+    F = _F()
+    import wxx_b200 as wxx
+
+    v = rng.standard_normal((2 * W, 20)).astype(np.float32)
+    for bad in (W, 16):
+        parents = np.tile(np.arange(W)[::-1], (2, 1)).astype(np.uint32)
+        parents[0, 0] = parents[1, W // 2] = bad
+        t = up(v)
+        F.beam_reorder([t], up(parents, np.uint32))
+        assert wxx.backend.device_status() == 2
+        kept = np.where(parents < W, parents, np.arange(W, dtype=np.uint32))
+        assert np.array_equal(t.numpy(), recurrent.beam_reorder(v, kept))
+
+
 def test_steps_in_a_graph(rng):
     F = _F()
     import wxx_b200 as wxx

@@ -560,8 +560,11 @@ __global__ void __launch_bounds__(kT)
     n = used < n ? used : n;
   }
   if (t < 32) {
-    const uint32_t parent = t < W ? parents[b * W + t] : (uint32_t)t;
-    if (t < W && parent >= (uint32_t)W) wxx_device_fail(err, WXX_DEV_ERR_BAD_INDEX);
+    uint32_t parent = t < W ? parents[b * W + t] : (uint32_t)t;
+    if (t < W && parent >= (uint32_t)W) {        // also where it is below MAX
+      wxx_device_fail(err, WXX_DEV_ERR_BAD_INDEX);
+      parent = (uint32_t)t;
+    }
     for (int p = 0; p < MAX; ++p) {
       const unsigned who = __ballot_sync(0xffffffffu, t < W && parent == (uint32_t)p && t != p);
       if (t == 0) s_followers[p] = who;
