@@ -243,6 +243,42 @@ def test_saturated_gates_and_foreign_values(rng):
     assert np.array_equal(got[2], ref[2])
 
 
+def test_infinities_and_the_largest_numbers(rng):
+    """An infinite x makes the states infinite from its position on, as the formula
+    has it (gates of 0 to 4: no product of 128 weights is zero); opposite infinities
+    meet in NaN; opposite numbers near the largest stay finite."""
+    F = _F()
+    B, T, D = 1, 300, 40
+    x = rng.standard_normal((B, T, D)).astype(np.float32)
+    gate = (rng.random((B, T, D)) * 4).astype(np.float32)
+    gate[0, :, 8:12] *= -1
+    for c in range(16):
+        x[0, 37 + 16 * c, c] = np.inf if c % 2 else -np.inf
+    x[0, 250, 3] = -np.inf
+    x[0, :, 16:24] = np.where(rng.random((T, 8)) < 0.5, -3e38, 3e38)
+    gate[0, :, 20:24] *= -1
+    with np.errstate(invalid="ignore"):
+        ref = recurrent.recurrence(x, gate)[0]
+    h, last = F.gated_recurrence(up(x), up(gate))
+    h, last = h.numpy(), last.numpy()
+    far = ~np.isfinite(ref)
+    assert far[0, -1, :16].all() and np.isnan(ref[0, -1, 3])
+    bound = U * (64 + 8 * reach(gate, T)[0])
+    state, steps = up(np.zeros((B, D))), np.empty_like(h)
+    for t in range(T):
+        steps[:, t] = F.gated_recurrence_step(up(x[:, t]), up(gate[:, t]), state).numpy()
+    for got in (h, steps):
+        # states 128 positions and more behind an infinity, negative gates: products of
+        # their weights may be zero, so infinite or NaN
+        near = np.ones(got.shape, bool)
+        near[0, :, 8:12] = np.arange(T)[:, None] < 37 + 16 * np.arange(8, 12) + 1
+        assert np.array_equal(got[far & near], ref[far & near].astype(np.float32), equal_nan=True)
+        assert not np.isfinite(got[far]).any()
+        largest = np.broadcast_to(np.where(np.arange(D) // 8 == 2, 3e38, 5.0), got.shape)
+        assert (np.abs(got[~far] - ref[~far]) <= bound * largest[~far]).all()
+    assert np.array_equal(last, h[:, -1], equal_nan=True)
+
+
 @pytest.mark.parametrize("B,T,D", [(2, 0, 5), (0, 4, 5), (2, 3, 0)])
 def test_empty(B, T, D, rng):
     F = _F()

@@ -39,8 +39,8 @@ constexpr int kSteps = 16;          // positions of a thread
 constexpr int kWarps = 8;           // pieces of a tile, at most
 constexpr int kTile = kWarps * kSteps * 32;                // floats of a tile's operand
 // Blocks resident on an SM.  Four of the forward's leave 64 registers a thread (two
-// are spilled).  Measured with four and with three: 68 and 70 us over (32, 1024, 1024)
-// with a gate per 64 channels, 18.5 and 20.4 over (64, 128, 1024); but 60 and 54 over
+// are spilled).  Measured with four and with three: 70 and 72 us over (32, 1024, 1024)
+// with a gate per 64 channels, 18.5 and 20.5 over (64, 128, 1024); but 60 and 54 over
 // (1, 65536, 256), whose groups are longer, and 21 and 20 without the copy engine.
 constexpr int forward_blocks(bool tma, int seg) { return tma && seg == 1 ? 4 : 3; }
 constexpr int kBackwardBlocks = 2;
@@ -87,6 +87,13 @@ __device__ __forceinline__ Gate gate_of(float g, Weights w) {
 __device__ __forceinline__ float mix(Gate g, float h, float x) {
   const float base = g.keep ? h : x, other = g.keep ? x : h;
   return fmaf(g.w, other - base, base);
+}
+// The same where the difference may be more than the type holds: an infinity, or
+// values of about 1e38 and opposite signs.
+__device__ __forceinline__ float mix_any(Gate g, float h, float x) {
+  const float base = g.keep ? h : x, other = g.keep ? x : h, apart = other - base;
+  return fabsf(apart) < INFINITY ? fmaf(g.w, apart, base)
+                                 : fmaf(g.w, other, (1.0f - g.w) * base);
 }
 
 // What a stretch of positions does to the state before it: h -> A h + b.  A
@@ -406,10 +413,12 @@ __device__ __forceinline__ float* aligned_smem(float* p) {
 // a position.  A piece is run from a zero state: what it gives at every position,
 // and the product of the weights up to there, which then takes the state that the
 // join gives.  A warp whose piece is whole and holds no reset (nearly all) runs
-// without the tests for them.
+// without the tests for them, and runs it again with them where it comes out
+// infinite or NaN: a difference of two values may have passed the largest number
+// (asking costs 1 us at (16, 8192, 256)).
 //
-// A row of 8192 positions has 64 tiles, so (16, 8192, 256) gives 8192 tiles for 444
-// blocks: 78 us, 5.2 TB/s of its 403 MB, the join's looks at other tiles and the
+// A row of 8192 positions has 64 tiles, so (16, 8192, 256) gives 8192 tiles for 592
+// blocks: 79 us, 5.1 TB/s of its 403 MB, the join's looks at other tiles and the
 // latency of a tile's steps taking what a plain copy would not (without any join 73
 // us).  (1, 65536, 256) has 8 rows of tiles side by side and waits for its hops: 54 us,
 // 3.7 TB/s.  Measured and not kept: two channels a lane (80 and 61 us; a third of the
@@ -452,6 +461,7 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
     Stretch mine = {1.0f, 0.0f};
     auto first_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
+      mine = {1.0f, 0.0f};
 #pragma unroll
       for (int k0 = 0; k0 < kSteps; k0 += 2) {
         float g[2];
@@ -464,13 +474,16 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
         for (int e = 0; e < 2; ++e) {
           const int k = k0 + e;
           if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
-          mine.b = mix(gate_of(g[e], w[e]), mine.b, kPlain || k < p.left ? sx[k * 32] : 0.f);
+          const float now = kPlain || k < p.left ? sx[k * 32] : 0.f;
+          mine.b = kPlain ? mix(gate_of(g[e], w[e]), mine.b, now)
+                          : mix_any(gate_of(g[e], w[e]), mine.b, now);
           mine.A *= w[e].a;
           upto[k] = mine;
         }
       }
     };
-    if (whole) first_run(Yes{}); else first_run(No{});
+    if (whole) first_run(Yes{});
+    if (__any_sync(0xffffffffu, !whole || !(fabsf(mine.b) < INFINITY))) first_run(No{});
     const int64_t state = (int64_t)p.b * D + p.d;
     const float v = join_tile<kSeg>(c, s, turn, p, mine, h0 && p.d < D && p.j < kSeg * kWarps ? h0[state] : 0.f, next);
     float* hp = h + ((int64_t)p.b * T + p.t0) * D + p.d;
@@ -658,7 +671,7 @@ __global__ void recurrence_step_kernel(float* __restrict__ state, const float* _
     const float gate = g[b * g_ld + d / per];
     Weights w, same;
     weights2<false>(gate, gate, w, same);
-    state[i] = mix(gate_of(gate, w), state[i], x[b * x_ld + d]);
+    state[i] = mix_any(gate_of(gate, w), state[i], x[b * x_ld + d]);
   }
 }
 

@@ -7,7 +7,10 @@ sequence (no reference counterpart; kernels in ``csrc/recurrence.cu``).
 dividing the channels: a head's gate serves its channels / heads neighbouring
 channels (heads = channels: a gate per channel).  ``reset`` (batch, time),
 u32, marks positions where a new document starts: the state before such a
-position is zero, so documents packed into one row do not see each other.
+position is zero, so documents packed into one row do not see each other, not
+even their NaN.  Behind an infinite ``x`` a document's states are infinite as
+the formula has it, or NaN once the product of the gates since is too small
+for f32.
 """
 
 from ._common import F, check, compact, empty, ptr_or_none
