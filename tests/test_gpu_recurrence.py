@@ -339,6 +339,35 @@ def test_scans_of_all_sizes_one_after_another(rng):
     assert wxx.backend.device_status() == 0
 
 
+def test_scans_of_two_host_threads(rng):
+    """Two host threads on the library's stream, each asking for more scratch than the
+    other has had so far: neither's is freed under it."""
+    import threading
+
+    F = _F()
+    sizes = [(1, 300 + 700 * k, 32) for k in range(12)]
+    x = rng.standard_normal((1, 9000, 32)).astype(np.float32)
+    gate = (rng.standard_normal((1, 9000, 32)) + 2).astype(np.float32)
+    want = F.gated_recurrence(up(x), up(gate))[0].numpy()
+    wrong = []
+
+    def scans(order):
+        try:
+            for B, T, D in order:
+                h = F.gated_recurrence(up(x[:, :T]), up(gate[:, :T]))[0].numpy()
+                if not np.array_equal(h, want[:, :T]):
+                    wrong.append(T)
+        except Exception as e:              # handed to the test's own thread
+            wrong.append(e)
+
+    threads = [threading.Thread(target=scans, args=(o,)) for o in (sizes[::2] * 2, sizes[1::2] * 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_on_another_stream(rng):
     """The library stream changed between calls: each stream has its own scratch."""
     import torch

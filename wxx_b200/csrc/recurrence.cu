@@ -728,32 +728,37 @@ constexpr int kShortSeg = 1, kLongSeg = 4;
 bool long_rows(const Chain& c) { return c.blocks.d < 24; }
 int group_tiles(const Chain& c) { return kWarps * (long_rows(c) ? kLongSeg : kShortSeg); }
 
-// Scratch of at least `bytes`.  Each stream keeps its own, zero when it is new, so
-// scans on two streams do not meet.  A recorded launch may be replayed beside
-// either, so it has scratch of its own in the recording, cleared before it; so has
-// a launch on a stream past the sixteenth.  *own is such scratch, for the caller to
-// free.
+// Held from the choice of a scan's scratch to its launch: another host thread's
+// larger scan would free the scratch in between.
+std::mutex g_scan;
+
+// Scratch of at least `bytes` (under g_scan).  Each stream keeps its own, zero when it
+// is new, so scans on two streams do not meet; streams are told apart by their id,
+// which no later stream has again, as it may a handle.  A recorded launch may be
+// replayed beside either, so it has scratch of its own in the recording, cleared
+// before it; so has a launch on a stream past the sixteenth.  *own is such scratch,
+// for the caller to free.
 int scan_scratch(size_t bytes, char** p, void** own) {
   struct Kept {
-    cudaStream_t stream;
+    unsigned long long stream;
     char* p;
     size_t size;
   };
-  static std::mutex mu;
   static Kept kept[16];
   static int n = 0;
   cudaStream_t stream = wxx::stream();
   *own = nullptr;
   cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
   WXX_CUDA_CHECK(cudaStreamIsCapturing(stream, &cs));
-  std::lock_guard<std::mutex> lock(mu);
   Kept* mine = nullptr;
   if (cs == cudaStreamCaptureStatusNone) {
+    unsigned long long id = 0;
+    WXX_CUDA_CHECK(cudaStreamGetId(stream, &id));
     for (int i = 0; i < n && !mine; ++i)
-      if (kept[i].stream == stream) mine = &kept[i];
+      if (kept[i].stream == id) mine = &kept[i];
     if (!mine && n < 16) {
       mine = &kept[n++];
-      *mine = {stream, nullptr, 0};
+      *mine = {id, nullptr, 0};
     }
   }
   if (!mine) {
@@ -860,6 +865,7 @@ WXX_EXPORT int wxx_gated_recurrence(float* h, float* h_last, const float* x, int
   if (B * D == 0) return WXX_OK;
   if (T == 0) return copy_state(h_last, h0, B * D);
   const Operand ox{x, x_bs, x_ts}, og{gate, g_bs, g_ts};
+  std::lock_guard<std::mutex> lock(g_scan);
   Chain c;
   unsigned threads;
   void* scratch;
@@ -907,6 +913,7 @@ WXX_EXPORT int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0
   const bool inside = lanes || per == 32;
   const int64_t parts = warp ? per / 32 : per;
   const Operand ox{x, x_bs, x_ts}, og{gate, g_bs, g_ts}, od{dh, T * D, D}, oh{h, T * D, D};
+  std::lock_guard<std::mutex> lock(g_scan);
   Chain c;
   unsigned threads;
   void *scratch = nullptr, *wide = nullptr;
