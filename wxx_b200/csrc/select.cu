@@ -627,12 +627,13 @@ WXX_EXPORT int wxx_topk(float* values, uint32_t* ids, const float* x, int64_t ld
   if (N == 0) return WXX_OK;
   // Small blocks hide one another's steps, but more rows are then under way and what
   // is read again no longer comes from L2, and a large K takes most entries of few
-  // threads.  256 against 1024 threads: 1024 rows of 4096 at K = 32 12 and 29 us, of
-  // 16384 at K = 64 21 and 26 us, 4096 rows of 50304 247 and 150 us; 256, 512 and 1024
-  // threads for 1024 rows of 4096 at K = 128 64, 25 and 33 us.
+  // threads.  256, 512 and 1024 threads, 100 M entries: rows of 4096 at K = 32 179, 322
+  // and 631 us, of 16384 at K = 64 101, 109 and 152 and at K = 128 411, 156 and 191, of
+  // 24576 at K = 64 122, 91 and 119, of 32768 133, 84 and 98, of 50304 137, 106 and 84; at
+  // K = 256 rows of 4096 take 10569, 4570 and 997.  (A memory bound pass takes 64.)
   if (V <= 16384 && K <= 64)
     topk_kernel<256><<<(unsigned)N, 256, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
-  else if (V <= 16384 && K <= 128)
+  else if (V <= 32768 && K <= 128)
     topk_kernel<512><<<(unsigned)N, 512, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
   else
     topk_kernel<1024><<<(unsigned)N, 1024, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
