@@ -66,6 +66,27 @@ def test_topk_crowded_lanes(rng):
         check_topk(x, k)
 
 
+@pytest.mark.parametrize("V", [1, 31, 32, 33, 200, 256, 257, 511, 513, 1000, 1024, 1025, 2047, 2048,
+                               2049])
+def test_topk_short_rows(V, rng):
+    """Rows about the lengths where the kernel changes: random, of few values (more
+    equal entries than are looked at together), one lane's entries above all others,
+    infinities and NaN, falling and rising; every number of rows of a block."""
+    at = np.arange(V)
+    few = rng.integers(0, 3, V)
+    odd = rng.standard_normal(V)
+    odd[rng.integers(0, V, 5)] = [np.nan, np.inf, -np.inf, 0.0, -0.0]
+    rows = [rng.standard_normal(V), few, np.where(few == 2, rng.random(V) + 2, few),
+            np.where(at % 32 == 5, 10 + rng.random(V), rng.random(V)), odd, at, -at, np.zeros(V),
+            np.full(V, -np.inf), np.full(V, np.nan), np.where(at < V // 2, -np.inf, odd)]
+    x = np.stack(rows).astype(np.float32)
+    for k in (1, 7, 31, 32, 33, 63, 65, 128, 129, 160, 256):
+        if k <= V:
+            check_topk(x, k)
+            check_topk(x[:2], k)
+    check_topk(rng.standard_normal((601, V)).astype(np.float32), min(V, 40))
+
+
 def test_topk_foreign_values(rng):
     x = rng.standard_normal((6, 777)).astype(np.float32)
     x[0, [5, 700]] = np.nan

@@ -207,7 +207,7 @@ __device__ __forceinline__ void join_sums(Select& s, float& top, float& sum) {
 // best_pairs for a short row and a few pairs: a thread has at most five entries, so
 // every warp takes its K best one after the other (two reductions each), and those
 // of all warps are the result.  Half the time of a threshold at K = 4.
-template <int THREADS, uint32_t NAN_KEY, bool SUM>
+template <int THREADS, uint32_t NAN_KEY>
 __device__ __forceinline__ int warp_bests(const Row& row, int K, Select& s, float m, float part,
                                           float& top, float& sum) {
   constexpr int kWarps = THREADS / 32;
@@ -233,14 +233,14 @@ __device__ __forceinline__ int warp_bests(const Row& row, int K, Select& s, floa
       }
     const uint32_t first = __reduce_max_sync(0xffffffffu, best);
     const uint32_t where = __reduce_min_sync(0xffffffffu, best == first ? i : 0xffffffffu);
-    if (SUM && r == 0) warp_sums(s, first ? key_float(first) : -INFINITY, m, part);
+    if (r == 0) warp_sums(s, first ? key_float(first) : -INFINITY, m, part);
     if (lane == 0) s.pair[warp * K + r] = first ? ((uint64_t)first << 32) | (uint32_t)~where : 0;
 #pragma unroll
     for (int k = 0; k < 5; ++k)
       if (key[k] == first && at[k] == where) key[k] = 0;
   }
   __syncthreads();
-  if (SUM) join_sums<kWarps>(s, top, sum);
+  join_sums<kWarps>(s, top, sum);
   return kWarps * K;
 }
 
@@ -292,8 +292,10 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
     }
     m = n;
   }
-  if (row.groups <= THREADS && K <= kMaxBeams && K * kWarps <= 256)
-    return warp_bests<THREADS, NAN_KEY, SUM>(row, K, s, m, part, top, sum);
+  if constexpr (SUM) {
+    if (row.groups <= THREADS && K <= kMaxBeams && K * kWarps <= 256)
+      return warp_bests<THREADS, NAN_KEY>(row, K, s, m, part, top, sum);
+  }
   // the nth largest of the warp's lanes (of their largest entries)
   uint32_t o = value_key(m, NAN_KEY);
   // (of the warps that have entries; tau is -inf where they are too few)
@@ -408,8 +410,8 @@ __device__ __forceinline__ void in_order(Select& s, int n, int K, F put) {
 
 // A block a row.  4 bytes an entry: the top 64 of 4096 x 50304 in 150 us, 5.5 TB/s.
 // Two blocks of 1024 threads share an SM, one streams its row while the other picks;
-// what is left of the time is where both pick.  The top 32 of 1024 x 1024 take 8 us,
-// of which the launch is 3: the steps' latencies bound it, not the 4 MB.
+// what is left of the time is where both pick (asking L2 for a later block's row in
+// the meantime took the same rows from 150 to 178 us).
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS, 2048 / THREADS)
     topk_kernel(float* __restrict__ values, uint32_t* __restrict__ ids,
@@ -425,6 +427,157 @@ __global__ void __launch_bounds__(THREADS, 2048 / THREADS)
     // a key gives its value back, but for the sign of zero and a NaN's bits
     values[at * K + rank] = v == 0x80000000u || v == kNanHighest ? row.p[i] : key_float(v);
   });
+}
+
+// A warp a row, for short rows: its entries' keys stay in registers, entry 32 j + lane
+// in key[j].  Of every lane's NTH largest, the mth largest over the lanes is a key
+// that at least NTH m >= K entries reach.  From there the cut is raised by bisection
+// towards the largest key: over the registers while more reach it than shared memory
+// holds, then over those pairs until few more than K are left, which are counted
+// against each other.  A ballot counts entries in the order of their indices, so of
+// entries that a cut cannot tell apart the first are taken.
+// Bound by its instructions (about 700 a row of 1024 at K = 32) and, with few rows, by
+// their latency; there is no barrier: the top 32 of 1024 x 1024 take 6 us, of which the
+// launch is 3, of 4096 x 1024 10 us (16.8 MB, 1.6 TB/s).
+constexpr int kRowWarps = 4;
+
+template <int M>
+__device__ __forceinline__ int reaching(const uint32_t (&key)[M], uint32_t cut) {
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < M; ++j) n += key[j] >= cut;
+  return __reduce_add_sync(0xffffffffu, n);
+}
+
+// Raises the cut, which `left` >= K keys reach, until at most `most` do or it is the
+// K-th key itself.
+template <int M>
+__device__ __forceinline__ void raise(const uint32_t (&key)[M], int K, int most, uint32_t& cut,
+                                      uint32_t& high, int& left) {
+  while (left > most && cut < high) {
+    const uint32_t middle = cut + (high - cut + 1) / 2;
+    const int n = reaching(key, middle);
+    if (n >= K) {
+      cut = middle;
+      left = n;
+    } else {
+      high = middle - 1;
+    }
+  }
+}
+
+// put(j, place) for the keys that reach the cut or, where they are more than `most`,
+// for the K first of them (the cut is the K-th key then).  Returns how many.
+template <int M, class Put>
+__device__ __forceinline__ int take(const uint32_t (&key)[M], int K, int most, uint32_t cut,
+                                    int left, Put put) {
+  const unsigned lower = (1u << (threadIdx.x & 31)) - 1;
+  int n = 0;
+  if (left <= most) {
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      const unsigned who = __ballot_sync(0xffffffffu, key[j] >= cut);
+      if (key[j] >= cut) put(j, n + __popc(who & lower));
+      n += __popc(who);
+    }
+    return n;
+  }
+  int ties = K - reaching(key, cut + 1);
+#pragma unroll
+  for (int j = 0; j < M; ++j) {
+    const unsigned same = __ballot_sync(0xffffffffu, key[j] == cut);
+    const bool wanted = key[j] > cut || (key[j] == cut && __popc(same & lower) < ties);
+    const unsigned who = __ballot_sync(0xffffffffu, wanted);
+    if (wanted) put(j, n + __popc(who & lower));
+    ties -= __popc(same);
+    n += __popc(who);
+  }
+  return n;
+}
+
+template <int ITEMS, int NTH>
+__global__ void __launch_bounds__(kRowWarps * 32)
+    topk_rows_kernel(float* __restrict__ values, uint32_t* __restrict__ ids,
+                     const float* __restrict__ x, int64_t ld, int64_t N, int V, int K) {
+  constexpr int kMost = 40 * NTH;     // pairs to count: a quarter more than the largest K
+  constexpr int kPairs = NTH == 8 ? 512 : 256;
+  __shared__ uint64_t s_pair[kRowWarps][kPairs];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)blockIdx.x * kRowWarps + warp;
+  if (at >= N) return;
+  const float* row = x + at * ld;
+  uint64_t* pair = s_pair[warp];
+  uint32_t key[ITEMS];                // 0: no entry
+  {
+    float v[ITEMS];
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) v[j] = 32 * j + lane < V ? row[32 * j + lane] : 0.f;
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      key[j] = 32 * j + lane < V ? value_key(v[j], kNanHighest) : 0u;
+  }
+  uint32_t best[NTH] = {};
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    uint32_t rest = key[j];
+#pragma unroll
+    for (int i = 0; i < NTH; ++i) {
+      const uint32_t larger = max(best[i], rest);
+      rest = min(best[i], rest);
+      best[i] = larger;
+    }
+  }
+  const int m = (K + NTH - 1) / NTH;
+  uint32_t cut = m == 32 ? __reduce_min_sync(0xffffffffu, best[NTH - 1])
+                         : __shfl_sync(0xffffffffu, descending(best[NTH - 1]), m - 1);
+  uint32_t high = __reduce_max_sync(0xffffffffu, best[0]);
+  cut = max(cut, 1u);
+  int n = reaching(key, cut);
+  raise(key, K, kPairs, cut, high, n);
+  n = take(key, K, kPairs, cut, n, [&](int j, int place) {
+    pair[place] = (uint64_t)key[j] << 32 | (uint32_t)~(32 * j + lane);
+  });
+  __syncwarp();
+  constexpr int kOwn = (kMost + 31) / 32;
+  uint64_t own[kPairs / 32];
+  if (n > kMost) {
+    uint32_t part[kPairs / 32];
+#pragma unroll
+    for (int i = 0; i < kPairs / 32; ++i) {
+      own[i] = 32 * i + lane < n ? pair[32 * i + lane] : 0;
+      part[i] = (uint32_t)(own[i] >> 32);
+    }
+    __syncwarp();                     // all have been read
+    raise(part, K, kMost, cut, high, n);
+    n = take(part, K, kMost, cut, n, [&](int i, int place) { pair[place] = own[i]; });
+    __syncwarp();
+  }
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) own[i] = 32 * i + lane < n ? pair[32 * i + lane] : 0;
+  int rank[kOwn] = {};
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const uint64_t other = pair[j];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) rank[i] += other > own[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    if (own[i] == 0 || rank[i] >= K) continue;
+    const uint32_t entry = key_index(own[i]), k = (uint32_t)(own[i] >> 32);
+    ids[at * K + rank[i]] = entry;
+    values[at * K + rank[i]] = k == 0x80000000u || k == kNanHighest ? row[entry] : key_float(k);
+  }
+}
+
+template <int ITEMS>
+void topk_rows(float* values, uint32_t* ids, const float* x, int64_t ld, int64_t N, int V, int K) {
+  auto kernel = K <= 32    ? topk_rows_kernel<ITEMS, 1>
+                : K <= 64  ? topk_rows_kernel<ITEMS, 2>
+                : K <= 128 ? topk_rows_kernel<ITEMS, 4>
+                           : topk_rows_kernel<ITEMS, 8>;
+  kernel<<<(unsigned)((N + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, wxx::stream()>>>(
+      values, ids, x, ld, N, V, K);
 }
 
 // One selection step.  A cluster takes a batch item; its rows, or `parts` pieces
@@ -625,13 +778,24 @@ WXX_EXPORT int wxx_topk(float* values, uint32_t* ids, const float* x, int64_t ld
   WXX_REQUIRE(K >= 1 && K <= kMaxTopk && K <= V, "wxx_topk: k = %d outside [1, min(%lld, %d)]", K,
               (long long)V, kMaxTopk);
   if (N == 0) return WXX_OK;
+  // A warp a row against a block a row: 4096 rows of 1024 at K = 8, 32 and 128 8, 10 and
+  // 25 us and 37, 33 and 74 us, of 2048 12, 16 and 31 and 27, 33 and 74 us, 16 of 2048 6, 6
+  // and 10 and 6, 6 and 8 us.
   // Small blocks hide one another's steps, but more rows are then under way and what
   // is read again no longer comes from L2, and a large K takes most entries of few
   // threads.  256, 512 and 1024 threads, 100 M entries: rows of 4096 at K = 32 179, 322
   // and 631 us, of 16384 at K = 64 101, 109 and 152 and at K = 128 411, 156 and 191, of
   // 24576 at K = 64 122, 91 and 119, of 32768 133, 84 and 98, of 50304 137, 106 and 84; at
   // K = 256 rows of 4096 take 10569, 4570 and 997.  (A memory bound pass takes 64.)
-  if (V <= 16384 && K <= 64)
+  if (V <= 256)
+    topk_rows<8>(values, ids, x, ld, N, (int)V, K);
+  else if (V <= 512)
+    topk_rows<16>(values, ids, x, ld, N, (int)V, K);
+  else if (V <= 1024)
+    topk_rows<32>(values, ids, x, ld, N, (int)V, K);
+  else if (V <= 2048)
+    topk_rows<64>(values, ids, x, ld, N, (int)V, K);
+  else if (V <= 16384 && K <= 64)
     topk_kernel<256><<<(unsigned)N, 256, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
   else if (V <= 32768 && K <= 128)
     topk_kernel<512><<<(unsigned)N, 512, 0, wxx::stream()>>>(values, ids, x, ld, (int)V, K);
