@@ -76,6 +76,32 @@ def test_loss_and_gradient(N, V, K, tau, ragged, rng):
     assert (np.abs(d - rd) <= np.abs(grad) * tau * full * bg + 1e-37).all()
 
 
+@pytest.mark.parametrize("N,V,K", [(1500, 7, 7), (1030, 31, 20), (1024, 256, 64), (1025, 257, 33),
+                                   (1024, 500, 64), (1027, 513, 1), (1100, 1021, 40),
+                                   (1024, 1024, 65), (1024, 1025, 64), (6, 2048, 128),
+                                   (6, 2049, 128), (5, 2048, 129)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_many_short_rows(N, V, K, ragged, rng):
+    """Both sides of the lengths, entries and rows where the kernels change, ids
+    stored twice among them."""
+    tau = 1.5
+    F = _F()
+    z, top, ids = problem(rng, N, V, K, ragged)
+    ids[:, K // 2] = ids[:, 0]
+    ids[::3, K - 1] = ids[::3, K // 3]
+    loss, stats = F.distill_loss(up(z), up(top), up(ids, np.uint32), tau)
+    rloss, rp, rq = recurrent.distill(z, top, ids, tau)
+    bl, bg = bounds(z, top, tau)
+    assert np.abs(loss.numpy() - rloss).max() <= tau * tau * bl
+    grad = rng.standard_normal((N, 1)).astype(np.float32)
+    d = F.distill_loss_backward(up(grad), up(z), up(top), up(ids, np.uint32), stats, tau).numpy()
+    rd = recurrent.distill_backward(grad, z, top, ids, tau)
+    full = rq.copy()
+    for n in range(N):
+        np.add.at(full[n], ids[n].astype(np.int64), rp[n])
+    assert (np.abs(d - rd) <= np.abs(grad) * tau * full * bg + 1e-37).all()
+
+
 def test_gradient_against_differences(rng):
     """Central differences of the kernel's loss: the third derivative of the
     log-sum is below 1/4, so a step s is off by tau^2 s^2 / 24 / tau^3 and the
@@ -182,12 +208,13 @@ def test_id_outside_the_vocabulary(rng):
     assert wxx.backend.device_status() == 0
 
 
-def test_absent_entries_beside_foreign_ones(rng):
+@pytest.mark.parametrize("N,V", [(6, 5000), (6, 900), (1030, 300)])
+def test_absent_entries_beside_foreign_ones(N, V, rng):
     """A NaN or an infinity among a row's stored logits makes its loss NaN, and the
     gradient where it is stored; the entries that are not there stay without effect,
     whatever their ids."""
     F = _F()
-    N, V, K = 6, 5000, 40
+    K = 40
     z, top, ids = problem(rng, N, V, K, False)
     top[:, 20:] = -np.inf
     ids[:, 20:] = np.uint32(0xFFFFFFFF)

@@ -14,6 +14,7 @@
 #include <stdint.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "rows.cuh"
@@ -189,6 +190,28 @@ __global__ void __launch_bounds__(kT)
   }
 }
 
+// Whether entry k is the first with its id; p, its own, becomes the sum over all that
+// have the id.  (id is 16-byte aligned and filled to a multiple of four.)
+__device__ __forceinline__ bool first_of_its_id(const uint32_t* id, const float* ps, int K, int k,
+                                                float& p) {
+  const uint32_t j = id[k];
+  int same = 0;
+#pragma unroll 4
+  for (int o = 0; o < K; o += 4) {
+    const uint4 four = *reinterpret_cast<const uint4*>(id + o);
+    same += (four.x == j) + (four.y == j) + (four.z == j) + (four.w == j);
+  }
+  if (same == 1) return true;
+  p = 0.f;
+  bool first = true;
+  for (int o = 0; o < K; ++o) {
+    if (id[o] != j) continue;
+    first = first && o >= k;
+    p += ps[o];
+  }
+  return first;
+}
+
 // dz over a piece of a row: g tau q everywhere, then the stored entries that lie in
 // it.  8 bytes a logit: 4096 x 50304 in 279 us, 5.9 TB/s, the rate of reading and
 // writing at once.  (Cache hints for streaming did not help: 279 us on the stores,
@@ -202,7 +225,7 @@ __global__ void __launch_bounds__(kT)
                             const float* __restrict__ stats, int V, int K, int parts, int length,
                             float tau, float inv_tau, float c, int* err) {
   __shared__ float s_p[kMaxK];
-  __shared__ uint32_t s_id[kMaxK];
+  __shared__ __align__(16) uint32_t s_id[kMaxK];
   const int part = blockIdx.x % parts;
   const int64_t at = blockIdx.x / parts;
   const int from = part * length, n = min(length, V - from);
@@ -213,6 +236,7 @@ __global__ void __launch_bounds__(kT)
   const float m = st.x, inv = 1.0f / st.y, g = grad[at] * tau;
   if (some) {
     const float inv_t = 1.0f / st.w;
+    if (threadIdx.x < 4 && K + threadIdx.x < kMaxK) s_id[K + threadIdx.x] = 0xffffffffu;
     for (int k = threadIdx.x; k < K; k += kT) {
       const uint32_t j = ids[at * K + k];
       const float t = stored(top[at * K + k], j, V, part == 0 ? err : nullptr);
@@ -248,17 +272,137 @@ __global__ void __launch_bounds__(kT)
   for (int k = threadIdx.x; k < K; k += kT) {
     const uint32_t j = s_id[k];
     if (j < (uint32_t)from || j - (uint32_t)from >= (uint32_t)n) continue;
-    // the first entry of an id takes all that have it
-    float p = 0.f;
-    bool first = true;
-#pragma unroll 8
-    for (int o = 0; o < K; ++o) {
-      const bool same = s_id[o] == j;
-      first = first && !(same && o < k);
-      p += same && o >= k ? s_p[o] : 0.f;
-    }
-    if (first) out[j - from] = g * (scaled_exp(z[j - from], m, c) * inv - p);
+    const float q = scaled_exp(z[j - from], m, c) * inv;
+    float p = s_p[k];
+    if (first_of_its_id(s_id, s_p, K, k, p)) out[j - from] = g * (q - p);
   }
+}
+
+// Short rows: a warp a row, its logits in registers (entry 32 j + lane in v[j]) and a few
+// stored entries a lane, so there is no barrier and one exponential a logit.  Bound by
+// instructions and, with few rows, latencies: 4096 x 1021 logits with 64 stored take 6
+// us forward (a block a row 23) and 12 backward (14), 4096 x 200 4 and 8 us (21 and 12).
+// Backward, a warp is longer at comparing the stored ids with one another: 128 rows of
+// 1021 6 us against 4, 4096 with 128 stored 21 against 19, so it has many rows and at
+// most 64 stored entries.
+constexpr int kRowWarps = 4;
+constexpr int kForwardEntries = 4, kBackwardEntries = 2;       // of a lane
+constexpr int kForwardV = 2048, kBackwardV = 1024, kBackwardN = 1024;
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kRowWarps * 32)
+    distill_forward_rows_kernel(float* __restrict__ loss, float* __restrict__ stats,
+                                const float* __restrict__ logits, int64_t ld,
+                                const float* __restrict__ top, const uint32_t* __restrict__ ids,
+                                int64_t N, int V, int K, float inv_tau, float c, float tau2,
+                                int* err) {
+  const int lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  if (at >= N) return;
+  const float* z = logits + at * ld;
+  float v[ITEMS], t[kForwardEntries];
+  uint32_t id[kForwardEntries];          // V: not there
+#pragma unroll
+  for (int i = 0; i < kForwardEntries; ++i) {
+    const int k = 32 * i + lane;
+    id[i] = k < K ? ids[at * K + k] : 0u;
+    t[i] = k < K ? top[at * K + k] : -INFINITY;
+  }
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) v[j] = 32 * j + lane < V ? z[32 * j + lane] : -INFINITY;
+  float m = -INFINITY, t_top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kForwardEntries; ++i) {
+    t[i] = stored(t[i], id[i], V, err);
+    if (t[i] == -INFINITY) id[i] = V;
+    t_top = max_nan(t_top, t[i]);
+  }
+  t_top = warp_max_nan(t_top);
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) m = max_nan(m, v[j]);
+  m = warp_max_nan(m);
+  float s = 0.f, t_sum = 0.f;
+  if (m != -INFINITY) {
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) s += scaled_exp(v[j], m, c);
+  }
+  s = warp_sum(s);
+  const bool some = t_top != -INFINITY;
+  float p[kForwardEntries];
+#pragma unroll
+  for (int i = 0; i < kForwardEntries; ++i) {
+    t[i] = some ? (t[i] - t_top) * inv_tau : -INFINITY;
+    t_sum += p[i] = expf(t[i]);
+  }
+  t_sum = warp_sum(t_sum);
+  const float log_s = logf(s), log_t = logf(t_sum), inv = 1.0f / t_sum;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kForwardEntries; ++i) {
+    if (id[i] >= (uint32_t)V || p[i] * inv == 0.f) continue;
+    sum += p[i] * inv * ((t[i] - log_t) - ((z[id[i]] - m) * inv_tau - log_s));
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) {
+    loss[at] = some ? tau2 * sum : 0.f;
+    *reinterpret_cast<float4*>(stats + at * kStats) = make_float4(m, s, t_top, t_sum);
+  }
+}
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kRowWarps * 32)
+    distill_backward_rows_kernel(float* __restrict__ dz, const float* __restrict__ grad,
+                                 const float* __restrict__ logits, int64_t ld,
+                                 const float* __restrict__ top, const uint32_t* __restrict__ ids,
+                                 const float* __restrict__ stats, int64_t N, int V, int K,
+                                 float tau, float inv_tau, float c, int* err) {
+  __shared__ __align__(16) uint32_t s_id[kRowWarps][32 * kBackwardEntries];
+  __shared__ float s_p[kRowWarps][32 * kBackwardEntries];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t at = (int64_t)blockIdx.x * kRowWarps + warp;
+  if (at >= N) return;
+  const float* z = logits + at * ld;
+  float* out = dz + at * V;
+  const float4 st = *reinterpret_cast<const float4*>(stats + at * kStats);
+  const bool some = st.w != 0.f;     // the teacher's sum: 0 without entries
+  const float m = st.x, inv = 1.0f / st.y, inv_t = 1.0f / st.w, g = grad[at] * tau;
+  float v[ITEMS];
+  uint32_t id[kBackwardEntries];          // V: not there
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) v[j] = 32 * j + lane < V ? z[32 * j + lane] : 0.f;
+#pragma unroll
+  for (int i = 0; i < kBackwardEntries; ++i) {
+    const int k = 32 * i + lane;
+    id[i] = k < K ? ids[at * K + k] : 0u;
+    const float t = k < K ? stored(top[at * K + k], id[i], V, err) : -INFINITY;
+    if (t == -INFINITY) id[i] = V;
+    s_id[warp][k] = id[i];
+    s_p[warp][k] = t == -INFINITY ? 0.f : expf((t - st.z) * inv_tau) * inv_t;
+  }
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j)
+    if (32 * j + lane < V) out[32 * j + lane] = some ? g * (scaled_exp(v[j], m, c) * inv) : 0.f;
+  if (!some) return;
+  __syncwarp();                      // the stored entries overwrite what is there
+#pragma unroll
+  for (int i = 0; i < kBackwardEntries; ++i) {
+    if (32 * i >= K) break;
+    if (id[i] >= (uint32_t)V) continue;
+    const float q = scaled_exp(z[id[i]], m, c) * inv;
+    float p = s_p[warp][32 * i + lane];
+    if (first_of_its_id(s_id[warp], s_p[warp], K, 32 * i + lane, p)) out[id[i]] = g * (q - p);
+  }
+}
+
+// The kernel of a row length.
+template <int MOST, class F>
+int by_length(int64_t V, F launch) {
+  using std::integral_constant;
+  if (V <= 256) return launch(integral_constant<int, 8>{});
+  if (V <= 512) return launch(integral_constant<int, 16>{});
+  if constexpr (MOST > 1024)
+    if (V > 1024) return launch(integral_constant<int, MOST / 32>{});
+  return launch(integral_constant<int, 32>{});
 }
 
 int check_sizes(const char* what, int64_t N, int64_t V, int K, float tau) {
@@ -292,6 +436,16 @@ WXX_EXPORT int wxx_distill_loss(float* loss, float* stats, const float* logits, 
   WXX_REQUIRE_INIT();
   if (int st = check_sizes("wxx_distill_loss", N, V, K, tau)) return st;
   if (N == 0) return WXX_OK;
+  const float inv_tau = 1.0f / tau, c = (float)(1.4426950408889634 / (double)tau);
+  const bool wide = (reinterpret_cast<uintptr_t>(stats) & 15) == 0;
+  if (V <= kForwardV && K <= 32 * kForwardEntries && wide)
+    return by_length<kForwardV>(V, [&](auto items) {
+      distill_forward_rows_kernel<items.value>
+          <<<(unsigned)((N + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, wxx::stream()>>>(
+              loss, stats, logits, ld, top, ids, N, (int)V, K, inv_tau, c, tau * tau,
+              wxx::device_error_word());
+      return wxx::after_launch(__FILE__, __LINE__);
+    });
   int parts, length;
   split_row(N, V, parts, length);
   cudaLaunchConfig_t cfg = {};
@@ -304,8 +458,7 @@ WXX_EXPORT int wxx_distill_loss(float* loss, float* stats, const float* logits, 
   cfg.attrs = &at;
   cfg.numAttrs = parts > 1 ? 1 : 0;
   WXX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, distill_forward_kernel, loss, stats, logits, ld, top, ids,
-                                    (int)V, K, parts, length, 1.0f / tau,
-                                    (float)(1.4426950408889634 / (double)tau), tau * tau,
+                                    (int)V, K, parts, length, inv_tau, c, tau * tau,
                                     wxx::device_error_word()));
   WXX_LAUNCH_CHECK();
   return WXX_OK;
@@ -320,14 +473,23 @@ WXX_EXPORT int wxx_distill_backward(float* dz, const float* grad, const float* l
   if (N == 0) return WXX_OK;
   WXX_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0,
               "wxx_distill_backward: the statistics must be 16-byte aligned");
+  const float inv_tau = 1.0f / tau, c = (float)(1.4426950408889634 / (double)tau);
+  if (V <= kBackwardV && K <= 32 * kBackwardEntries && N >= kBackwardN)
+    return by_length<kBackwardV>(V, [&](auto items) {
+      distill_backward_rows_kernel<items.value>
+          <<<(unsigned)((N + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, wxx::stream()>>>(
+              dz, grad, logits, ld, top, ids, stats, N, (int)V, K, tau, inv_tau, c,
+              wxx::device_error_word());
+      return wxx::after_launch(__FILE__, __LINE__);
+    });
   int parts, length;
   split_row(N, V, parts, length);
   const bool aligned = ((reinterpret_cast<uintptr_t>(dz) - reinterpret_cast<uintptr_t>(logits)) &
                         15) == 0 && (ld - V) % 4 == 0;
   auto kernel = aligned ? distill_backward_kernel<true> : distill_backward_kernel<false>;
   kernel<<<(unsigned)(N * parts), kT, 0, wxx::stream()>>>(
-      dz, grad, logits, ld, top, ids, stats, (int)V, K, parts, length, tau, 1.0f / tau,
-      (float)(1.4426950408889634 / (double)tau), wxx::device_error_word());
+      dz, grad, logits, ld, top, ids, stats, (int)V, K, parts, length, tau, inv_tau, c,
+      wxx::device_error_word());
   WXX_LAUNCH_CHECK();
   return WXX_OK;
 }
