@@ -118,8 +118,9 @@ class Tensor:
         return t
 
     @classmethod
-    def _empty(cls, shape, dtype="f32", requires_grad=False):
-        """Uninitialised dense tensor (internal: every op's output)."""
+    def _empty(cls, shape, dtype="f32", requires_grad=False, buffer=None, offset=0):
+        """Uninitialised dense tensor (internal: every op's output), in its own buffer or
+        at an element offset of one."""
         t = object.__new__(cls)
         t.shape = list(shape)
         n, stride = 1, [1] * len(t.shape)
@@ -129,8 +130,8 @@ class Tensor:
         t.stride = tuple(stride)
         t.type = dtype
         t.nbytes = n * _itemsize(dtype)
-        t.buffer = _dev.DeviceBuffer(max(t.nbytes, 4), "Tensor")
-        t.offset = 0
+        t.buffer = _dev.DeviceBuffer(max(t.nbytes, 4)) if buffer is None else buffer
+        t.offset = offset
         t._base = t.creator = t.grad = None
         t.requires_grad = requires_grad
         return t

@@ -204,47 +204,6 @@ __device__ __forceinline__ void join_sums(Select& s, float& top, float& sum) {
   sum = warp_sum(lane < WARPS ? s.sum[lane] * (w == top ? 1.0f : expf(w - top)) : 0.f);
 }
 
-// best_pairs for a short row and a few pairs: a thread has at most five entries, so
-// every warp takes its K best one after the other (two reductions each), and those
-// of all warps are the result.  A threshold costs more at 4 beams (8 us against 6 for 4 x 1024
-// logits) and less at many: 12 beams 12 us against 17.
-template <int THREADS, uint32_t NAN_KEY>
-__device__ __forceinline__ int warp_bests(const Row& row, int K, Select& s, float m, float part,
-                                          float& top, float& sum) {
-  constexpr int kWarps = THREADS / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = threadIdx.x;
-  uint32_t key[5];                    // 0: no entry
-  uint32_t at[5];
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (t < row.groups) v = row.mid[t];
-  const float values[5] = {v.x, v.y, v.z, v.w, row.single >= 0 ? row.p[row.single] : 0.f};
-#pragma unroll
-  for (int k = 0; k < 5; ++k) {
-    const bool here = k < 4 ? t < row.groups : row.single >= 0;
-    key[k] = here ? value_key(values[k], NAN_KEY) : 0u;
-    at[k] = k < 4 ? (uint32_t)(row.head + 4 * t + k) : (uint32_t)row.single;
-  }
-  for (int r = 0; r < K; ++r) {
-    uint32_t best = key[0], i = at[0];
-#pragma unroll
-    for (int k = 1; k < 5; ++k)
-      if (key[k] > best || (key[k] == best && key[k] != 0 && at[k] < i)) {
-        best = key[k];
-        i = at[k];
-      }
-    const uint32_t first = __reduce_max_sync(0xffffffffu, best);
-    const uint32_t where = __reduce_min_sync(0xffffffffu, best == first ? i : 0xffffffffu);
-    if (r == 0) warp_sums(s, first ? key_float(first) : -INFINITY, m, part);
-    if (lane == 0) s.pair[warp * K + r] = first ? ((uint64_t)first << 32) | (uint32_t)~where : 0;
-#pragma unroll
-    for (int k = 0; k < 5; ++k)
-      if (key[k] == first && at[k] == where) key[k] = 0;
-  }
-  __syncthreads();
-  join_sums<kWarps>(s, top, sum);
-  return kWarps * K;
-}
-
 // Puts the row's K best pairs, and perhaps more of its best, into s.pair and
 // returns how many (K <= V).  With SUM, top and sum come to hold the row's largest
 // number and the sum of exp(v - top).
@@ -292,10 +251,6 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
       part += e;
     }
     m = n;
-  }
-  if constexpr (SUM) {
-    if (row.groups <= THREADS && K <= 4)
-      return warp_bests<THREADS, NAN_KEY>(row, K, s, m, part, top, sum);
   }
   // the nth largest of the warp's lanes (of their largest entries)
   uint32_t o = value_key(m, NAN_KEY);
@@ -370,8 +325,7 @@ __device__ __forceinline__ uint64_t sorted_pair(Select& s, int n) {
   return mine;
 }
 
-// Calls put(rank, pair) for the K best of the n pairs in s.pair (all different, but
-// for zeros in the place of missing ones, which rank behind K pairs).
+// Calls put(rank, pair) for the K best of the n pairs in s.pair, all different.
 // Up to 64 of them are counted against each other, a few neighbouring threads
 // sharing a pair's count; more are sorted, a pair a thread (n^2 / 32 reads of
 // shared memory by a warp against log^2 n / 2 exchanges), or counted where threads

@@ -2,6 +2,7 @@
 stride marshalling, the global matmul precision mode and the host RNG."""
 
 import ctypes
+import math
 import os
 
 import numpy as np
@@ -29,9 +30,9 @@ def empty_group(*specs):
     total, at = 0, []
     for shape, _ in specs:
         at.append(total)
-        total += (4 * validation.numel(shape) + 255) // 256 * 256
-    buf = DeviceBuffer(max(total, 4), "Tensor")
-    return [Tensor._wrap(shape, buf, dtype, offset=o // 4) for (shape, dtype), o in zip(specs, at)]
+        total += (math.prod(shape) + 63) // 64 * 64
+    buf = DeviceBuffer(max(4 * total, 4))
+    return [Tensor._empty(shape, dtype, False, buf, o) for (shape, dtype), o in zip(specs, at)]
 
 
 def dense(t):
