@@ -79,6 +79,9 @@ struct Gate {
 __device__ __forceinline__ Gate gate_of(float g, Weights w) {
   return {g >= 0.f ? w.z : w.a, g >= 0.f};       // a NaN gives one
 }
+__device__ __forceinline__ Gate gate_of(Weights w) {
+  return {w.z <= w.a ? w.z : w.a, w.z <= w.a};
+}
 
 // a h + z x as the larger-weighted of the two plus the smaller weight times
 // their difference: a constant gate's fixed point stays where it is (a and z,
@@ -280,6 +283,31 @@ __device__ __forceinline__ void copy_gates(float* tile, const Operand& g, const 
     copy_float(tile + row * c.gates + k, t < T ? src + k : g.p, t < T);
 }
 
+// A gate for all of a warp's channels: the first threads each load the gate of one
+// position of the tile (past the last: keep the state) and, by the time the tile is
+// begun, have put its weights into shared memory, where a pair of positions is one
+// read.  Their arrival is part of the tile's barrier.
+__device__ __forceinline__ float warp_gate(const Operand& g, const Chain& c, const Place& p,
+                                           int T) {
+  const int row = threadIdx.x, t = p.t0 - p.row + row;
+  if (row >= (int)(blockDim.x >> 5) * kSteps || t >= T) return INFINITY;
+  return g.p[p.b * g.bs + t * g.ts + first_gate(c, p)];
+}
+template <bool kBounded>
+__device__ __forceinline__ void weigh(float2* tile, float gate, uint64_t* bar) {
+  if (threadIdx.x >= (blockDim.x >> 5) * kSteps) return;
+  Weights w, same;
+  weights2<kBounded>(gate, gate, w, same);
+  tile[threadIdx.x] = make_float2(w.a, w.z);
+  wxx_tc::mbar_arrive(bar);
+}
+// The weights of positions k and k + 1 of a warp's piece.
+__device__ __forceinline__ void weighed(const float2* piece, int k, Weights& w0, Weights& w1) {
+  const float4 v = *reinterpret_cast<const float4*>(piece + k);
+  w0 = {v.x, v.y};
+  w1 = {v.z, v.w};
+}
+
 // Joins the pieces of a tile (warp i of the order holds piece `mine`) with
 // everything before it.  j: the tile's place in its row, q: its channel block.
 // Returns the state before this warp's piece.  The order of the additions
@@ -351,12 +379,12 @@ __device__ __forceinline__ uint32_t reset_word(const uint32_t* __restrict__ rese
 }
 
 // A block's way through its tiles, the same in both directions.  fetch asks for
-// a tile's inputs, work is called with a tile when they are there and calls back
-// (with the place of the next) once it has taken them.
-template <bool kBackwards, class Fetch, class Work>
+// a tile's inputs, ready is called before the wait for them, work with a tile when they
+// are there; it calls back (with the place of the next) once it has taken them.
+template <bool kBackwards, class Fetch, class Ready, class Work>
 __device__ __forceinline__ void through_tiles(const Chain& c, Joint& s, unsigned arrivals,
                                               const uint32_t* reset, int T, int D, Fetch fetch,
-                                              Work work) {
+                                              Ready ready, Work work) {
   if (threadIdx.x == 0) {
     mbar_init(&s.full, arrivals);
     wxx_tc::fence_barrier_init();
@@ -380,6 +408,7 @@ __device__ __forceinline__ void through_tiles(const Chain& c, Joint& s, unsigned
   for (;; turn ^= 1) {
     if (c.tiles > 1 && threadIdx.x == 0) s.next = take_ticket(c);
     const unsigned cut = __ballot_sync(0xffffffffu, starts != 0);
+    ready();
     mbar_wait(&s.full, turn, &s.abort[turn], c.err);
     Place after = p;
     work(p, cut, turn, [&] {
@@ -425,7 +454,7 @@ __device__ __forceinline__ float* aligned_smem(float* p) {
 // instructions less, but fewer warps to hide latencies), a second buffer of inputs
 // (85 us: the tiles it holds back are the ones that others wait for), pieces of 8 (95
 // us) and 32 positions (76 us forward, 151 backward), groups of groups (83 and 66 us).
-template <bool kTma, int kSeg>
+template <bool kTma, int kSeg, bool kWarpGate>
 __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
     recurrence_forward_kernel(float* __restrict__ h, float* __restrict__ h_last,
                               const __grid_constant__ CUtensorMap map_x,
@@ -435,7 +464,9 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
   extern __shared__ float s_raw[];
   __shared__ Joint s;
   float *s_x = aligned_smem(s_raw), *s_g = s_x + kTile;
-  const bool own_gate = c.per.d == 1;
+  float2* s_w = reinterpret_cast<float2*>(s_g);
+  float gate = 0.f;                 // kWarpGate: of this thread's position of the next tile
+  const bool own_gate = !kWarpGate && c.per.d == 1;
   const unsigned box = (blockDim.x >> 5) * kSteps * 32 * sizeof(float);
   auto fetch = [&](const Place& p) {
     if (kTma && threadIdx.x == 0) {
@@ -445,12 +476,17 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
     }
     if (!kTma) copy_piece(s_x, x, p, 0);
     if (!kTma && own_gate) copy_piece(s_g, g, p, 0);
-    if (!own_gate) copy_gates(s_g, g, c, p, T, D);
-    if (!kTma || !own_gate) copies_arrive(&s.full);
+    if (kWarpGate) gate = warp_gate(g, c, p, T);
+    else if (!own_gate) copy_gates(s_g, g, c, p, T, D);
+    if (!kTma || !(kWarpGate || own_gate)) copies_arrive(&s.full);
   };
-  const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !own_gate ? blockDim.x : 0);
-  through_tiles<false>(c, s, arrivals, reset, T, D, fetch, [&](const Place& p, unsigned cut,
-                                                               int turn, auto next) {
+  auto ready = [&] {
+    if (kWarpGate) weigh<false>(s_w, gate, &s.full);
+  };
+  const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !(kWarpGate || own_gate) ? blockDim.x : 0) +
+                            (kWarpGate ? blockDim.x / 2 : 0);
+  through_tiles<false>(c, s, arrivals, reset, T, D, fetch, ready, [&](const Place& p, unsigned cut,
+                                                                      int turn, auto next) {
     const bool whole = __all_sync(0xffffffffu, p.left == kSteps && cut == 0);
     const int stride = own_gate ? 32 : c.gates;
     const float* sx = s_x + p.row * 32 + (threadIdx.x & 31);
@@ -466,17 +502,21 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
       for (int k0 = 0; k0 < kSteps; k0 += 2) {
         float g[2];
         Weights w[2];
+        if (kWarpGate) {
+          weighed(s_w + p.row, k0, w[0], w[1]);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)              // past the end: keep the state
-          g[k] = kPlain || k0 + k < p.left ? sg[(k0 + k) * stride] : INFINITY;
-        weights2<false>(g[0], g[1], w[0], w[1]);
+          for (int k = 0; k < 2; ++k)            // past the end: keep the state
+            g[k] = kPlain || k0 + k < p.left ? sg[(k0 + k) * stride] : INFINITY;
+          weights2<false>(g[0], g[1], w[0], w[1]);
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int k = k0 + e;
           if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
           const float now = kPlain || k < p.left ? sx[k * 32] : 0.f;
-          mine.b = kPlain ? mix(gate_of(g[e], w[e]), mine.b, now)
-                          : mix_any(gate_of(g[e], w[e]), mine.b, now);
+          const Gate mixed = kWarpGate ? gate_of(w[e]) : gate_of(g[e], w[e]);
+          mine.b = kPlain ? mix(mixed, mine.b, now) : mix_any(mixed, mine.b, now);
           mine.A *= w[e].a;
           upto[k] = mine;
         }
@@ -521,7 +561,10 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
   extern __shared__ float s_raw[];
   __shared__ Joint s;
   float *s_x = aligned_smem(s_raw), *s_d = s_x + kTile, *s_h = s_d + kTile, *s_g = s_h + kTile;
-  const bool own_gate = c.per.d == 1;
+  float2* s_w = reinterpret_cast<float2*>(s_g);
+  constexpr bool kWarpGate = DG == 32;
+  float gate = 0.f;                 // kWarpGate: of this thread's position of the next tile
+  const bool own_gate = !kWarpGate && c.per.d == 1;
   const unsigned box = (blockDim.x >> 5) * kSteps * 32 * sizeof(float);
   auto fetch = [&](const Place& p) {
     if (kTma && threadIdx.x == 0) {
@@ -538,13 +581,18 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
       copy_piece(s_h, h, p, 1);
       if (own_gate) copy_piece(s_g, g, p, 0);
     }
-    if (!own_gate) copy_gates(s_g, g, c, p, T, D);
-    if (!kTma || !own_gate) copies_arrive(&s.full);
+    if (kWarpGate) gate = warp_gate(g, c, p, T);
+    else if (!own_gate) copy_gates(s_g, g, c, p, T, D);
+    if (!kTma || !(kWarpGate || own_gate)) copies_arrive(&s.full);
   };
-  const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !own_gate ? blockDim.x : 0);
+  auto ready = [&] {
+    if (kWarpGate) weigh<true>(s_w, gate, &s.full);
+  };
+  const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !(kWarpGate || own_gate) ? blockDim.x : 0) +
+                            (kWarpGate ? blockDim.x / 2 : 0);
   const int lanes = DG == 1 ? c.per.d : DG == 32 ? 32 : 1, heads = DG == 0 ? D : D / lanes;
-  through_tiles<true>(c, s, arrivals, reset, T, D, fetch, [&](const Place& p, unsigned cut,
-                                                              int turn, auto next) {
+  through_tiles<true>(c, s, arrivals, reset, T, D, fetch, ready, [&](const Place& p, unsigned cut,
+                                                                     int turn, auto next) {
     const bool whole = __all_sync(0xffffffffu, p.left == kSteps && cut == 0 && p.t0 > 0);
     const int stride = own_gate ? 32 : c.gates, at = p.row * 32 + (threadIdx.x & 31);
     const float* sg = s_g + p.row * stride +
@@ -558,11 +606,17 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
       constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
       for (int k0 = kSteps - 2; k0 >= 0; k0 -= 2) {
-        float g[2], slope[2];
+        float slope[2];
         Weights w[2];
+        if (kWarpGate) {
+          weighed(s_w + p.row, k0, w[0], w[1]);
+        } else {
+          float g[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) g[k] = kPlain || k0 + k < p.left ? sg[(k0 + k) * stride] : INFINITY;
-        weights2<true>(g[0], g[1], w[0], w[1]);
+          for (int k = 0; k < 2; ++k)
+            g[k] = kPlain || k0 + k < p.left ? sg[(k0 + k) * stride] : INFINITY;
+          weights2<true>(g[0], g[1], w[0], w[1]);
+        }
         mul2(slope[0], slope[1], w[0].a, w[1].a, w[0].z, w[1].z);    // d a / d gate
 #pragma unroll
         for (int e = 1; e >= 0; --e) {
@@ -884,7 +938,9 @@ WXX_EXPORT int wxx_gated_recurrence(float* h, float* h_last, const float* x, int
   auto pick = [&](auto t, auto seg) {
     constexpr bool kTma = decltype(t)::value;
     constexpr int kSeg = decltype(seg)::value ? kLongSeg : kShortSeg;
-    return launch(recurrence_forward_kernel<kTma, kSeg>, forward_blocks(kTma, kSeg));
+    constexpr int kBlocks = forward_blocks(kTma, kSeg);
+    return c.per.d % 32 == 0 ? launch(recurrence_forward_kernel<kTma, kSeg, true>, kBlocks)
+                             : launch(recurrence_forward_kernel<kTma, kSeg, false>, kBlocks);
   };
   const int st = long_rows(c) ? (tma ? pick(Yes{}, Yes{}) : pick(No{}, Yes{}))
                               : (tma ? pick(Yes{}, No{}) : pick(No{}, No{}));
