@@ -39,9 +39,11 @@ constexpr int kSteps = 16;          // positions of a thread
 constexpr int kWarps = 8;           // pieces of a tile, at most
 constexpr int kTile = kWarps * kSteps * 32;                // floats of a tile's operand
 // Blocks resident on an SM.  Four of the forward's leave 64 registers a thread (two
-// are spilled).  Measured with four and with three: 70 and 72 us over (32, 1024, 1024)
-// with a gate per 64 channels, 18.5 and 20.5 over (64, 128, 1024); but 60 and 54 over
-// (1, 65536, 256), whose groups are longer, and 21 and 20 without the copy engine.
+// are spilled).  Measured with four and with three, the gates being weighed in every
+// channel: 70 and 72 us over (32, 1024, 1024) with a gate per 64 channels, 18.5 and 20.5
+// over (64, 128, 1024); but 60 and 54 over (1, 65536, 256), whose groups are longer, and
+// 21 and 20 without the copy engine.  (Five, which only a gate of 32 channels leaves
+// registers for: 71 us against 62 over (32, 1024, 1024).)
 constexpr int forward_blocks(bool tma, int seg) { return tma && seg == 1 ? 4 : 3; }
 constexpr int kBackwardBlocks = 2;
 constexpr int kWaitLimit = 1 << 21; // polls of a published word (about a second)
@@ -286,7 +288,9 @@ __device__ __forceinline__ void copy_gates(float* tile, const Operand& g, const 
 // A gate for all of a warp's channels: the first threads each load the gate of one
 // position of the tile (past the last: keep the state) and, by the time the tile is
 // begun, have put its weights into shared memory, where a pair of positions is one
-// read.  Their arrival is part of the tile's barrier.
+// read, and for the forward the products of a over its piece (a piece is 16 lanes).
+// Their arrival is part of the tile's barrier.  Weighed in every channel, (32, 1024,
+// 1024) with a gate per 64 channels took 70 + 105 us, so 62 + 101.
 __device__ __forceinline__ float warp_gate(const Operand& g, const Chain& c, const Place& p,
                                            int T) {
   const int row = threadIdx.x, t = p.t0 - p.row + row;
@@ -294,11 +298,23 @@ __device__ __forceinline__ float warp_gate(const Operand& g, const Chain& c, con
   return g.p[p.b * g.bs + t * g.ts + first_gate(c, p)];
 }
 template <bool kBounded>
-__device__ __forceinline__ void weigh(float2* tile, float gate, uint64_t* bar) {
-  if (threadIdx.x >= (blockDim.x >> 5) * kSteps) return;
+__device__ __forceinline__ void weigh(float2* tile, float* upto, float gate, uint64_t* bar) {
+  const int rows = (blockDim.x >> 5) * kSteps, row = threadIdx.x;
+  if ((row & ~31) >= rows) return;
   Weights w, same;
   weights2<kBounded>(gate, gate, w, same);
-  tile[threadIdx.x] = make_float2(w.a, w.z);
+  if (upto) {
+    static_assert(kSteps == 16, "a piece is half a warp");
+    float A = w.a;
+#pragma unroll
+    for (int o = 1; o < kSteps; o <<= 1) {
+      const float before = __shfl_up_sync(0xffffffffu, A, o, kSteps);
+      if ((row & (kSteps - 1)) >= o) A *= before;
+    }
+    if (row < rows) upto[row] = A;
+  }
+  if (row >= rows) return;
+  tile[row] = make_float2(w.a, w.z);
   wxx_tc::mbar_arrive(bar);
 }
 // The weights of positions k and k + 1 of a warp's piece.
@@ -408,7 +424,7 @@ __device__ __forceinline__ void through_tiles(const Chain& c, Joint& s, unsigned
   for (;; turn ^= 1) {
     if (c.tiles > 1 && threadIdx.x == 0) s.next = take_ticket(c);
     const unsigned cut = __ballot_sync(0xffffffffu, starts != 0);
-    ready();
+    ready(turn);
     mbar_wait(&s.full, turn, &s.abort[turn], c.err);
     Place after = p;
     work(p, cut, turn, [&] {
@@ -464,7 +480,10 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
   extern __shared__ float s_raw[];
   __shared__ Joint s;
   float *s_x = aligned_smem(s_raw), *s_g = s_x + kTile;
+  // kWarpGate, by turns: the weights of a tile's positions, the products of a in a piece
+  constexpr int kRows = kWarps * kSteps;
   float2* s_w = reinterpret_cast<float2*>(s_g);
+  float* s_A = s_g + 4 * kRows;
   float gate = 0.f;                 // kWarpGate: of this thread's position of the next tile
   const bool own_gate = !kWarpGate && c.per.d == 1;
   const unsigned box = (blockDim.x >> 5) * kSteps * 32 * sizeof(float);
@@ -480,8 +499,8 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
     else if (!own_gate) copy_gates(s_g, g, c, p, T, D);
     if (!kTma || !(kWarpGate || own_gate)) copies_arrive(&s.full);
   };
-  auto ready = [&] {
-    if (kWarpGate) weigh<false>(s_w, gate, &s.full);
+  auto ready = [&](int turn) {
+    if (kWarpGate) weigh<false>(s_w + turn * kRows, s_A + turn * kRows, gate, &s.full);
   };
   const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !(kWarpGate || own_gate) ? blockDim.x : 0) +
                             (kWarpGate ? blockDim.x / 2 : 0);
@@ -493,7 +512,9 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
     const float* sg = s_g + p.row * stride +
                       (own_gate ? (int)(threadIdx.x & 31)
                                 : (int)c.per(min(p.d, D - 1)) - first_gate(c, p));
-    Stretch upto[kSteps];            // the piece's positions up to each
+    const float2* sw = s_w + turn * kRows + p.row;
+    const float* sA = s_A + turn * kRows + p.row;
+    Stretch upto[kSteps];            // the piece's positions up to each (kWarpGate: A is sA's)
     Stretch mine = {1.0f, 0.0f};
     auto first_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
@@ -503,7 +524,7 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
         float g[2];
         Weights w[2];
         if (kWarpGate) {
-          weighed(s_w + p.row, k0, w[0], w[1]);
+          weighed(sw, k0, w[0], w[1]);
         } else {
 #pragma unroll
           for (int k = 0; k < 2; ++k)            // past the end: keep the state
@@ -517,10 +538,12 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
           const float now = kPlain || k < p.left ? sx[k * 32] : 0.f;
           const Gate mixed = kWarpGate ? gate_of(w[e]) : gate_of(g[e], w[e]);
           mine.b = kPlain ? mix(mixed, mine.b, now) : mix_any(mixed, mine.b, now);
-          mine.A *= w[e].a;
+          if (!kWarpGate) mine.A *= w[e].a;
           upto[k] = mine;
         }
       }
+      if (kWarpGate && kPlain) mine.A = sA[kSteps - 1];
+      if (kWarpGate && !kPlain) mine.A = cut ? -0.0f : sA[kSteps - 1];
     };
     if (whole) first_run(Yes{});
     if (__any_sync(0xffffffffu, !whole || !(fabsf(mine.b) < INFINITY))) first_run(No{});
@@ -531,6 +554,10 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
       constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
+        if (kWarpGate) {
+          upto[k].A = sA[k];
+          if (!kPlain && (cut & ((2u << k) - 1))) upto[k].A = -0.0f;
+        }
         const float now = kPlain ? fmaf(upto[k].A, v, upto[k].b) : through(upto[k], v);
         if (kPlain || k < p.left) *hp = now;
         if (k == (kPlain ? kSteps : p.left) - 1 && p.t0 + k == T - 1) h_last[state] = now;
@@ -585,8 +612,8 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
     else if (!own_gate) copy_gates(s_g, g, c, p, T, D);
     if (!kTma || !(kWarpGate || own_gate)) copies_arrive(&s.full);
   };
-  auto ready = [&] {
-    if (kWarpGate) weigh<true>(s_w, gate, &s.full);
+  auto ready = [&](int) {
+    if (kWarpGate) weigh<true>(s_w, nullptr, gate, &s.full);
   };
   const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !(kWarpGate || own_gate) ? blockDim.x : 0) +
                             (kWarpGate ? blockDim.x / 2 : 0);
