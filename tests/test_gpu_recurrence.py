@@ -64,6 +64,7 @@ SHAPES = [
     (1, 127, 40, 8), (2, 128, 31, 31), (1, 129, 96, 3), (4, 255, 30, 6), (1, 1000, 250, 250),
     (2, 300, 70, 7), (1, 513, 256, 4), (1, 200, 192, 1), (3, 4097, 34, 17), (1, 20000, 32, 32),
     (5, 640, 128, 128), (1, 9000, 65, 13), (2, 2048, 160, 5), (16, 130, 4, 4),
+    (2, 150, 300, 1), (1, 140, 514, 2), (1, 33, 8192, 1),
 ]
 
 

@@ -742,6 +742,22 @@ __global__ void sum_parts_kernel(float* __restrict__ out, const float* __restric
   }
 }
 
+// The same for many parts: a warp has an output.  Backward over (4, 4096, 1000) with one
+// gate takes 77 us, 147 with a thread an output; with 100 channels a gate 99 and 91.
+constexpr int kManyParts = 256;
+__global__ void sum_many_parts_kernel(float* __restrict__ out, const float* __restrict__ in,
+                                      int64_t n, int parts) {
+  const int lane = threadIdx.x & 31, warps = kT / 32;
+  for (int64_t i = (int64_t)blockIdx.x * warps + (threadIdx.x >> 5); i < n;
+       i += (int64_t)gridDim.x * warps) {
+    float v = 0.f;
+    for (int k = lane; k < parts; k += 32) v += in[i * parts + k];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) out[i] = v;
+  }
+}
+
 // One position: 16 bytes a channel; (32, 1024) takes 3 us, a launch's own time.
 __global__ void recurrence_step_kernel(float* __restrict__ state, const float* __restrict__ x,
                                        int64_t x_ld, const float* __restrict__ g, int64_t g_ld,
@@ -1030,8 +1046,13 @@ WXX_EXPORT int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0
     st = long_rows(c) ? (tma ? pick(Yes{}, Yes{}) : pick(No{}, Yes{}))
                       : (tma ? pick(Yes{}, No{}) : pick(No{}, No{}));
     if (st == WXX_OK && wide) {
-      sum_parts_kernel<<<wxx::grid_for(B * T * H, kT), kT, 0, wxx::stream()>>>(
-          dgate, sums, B * T * H, (int)parts);
+      const int64_t n = B * T * H;
+      if (parts < kManyParts)
+        sum_parts_kernel<<<wxx::grid_for(n, kT), kT, 0, wxx::stream()>>>(dgate, sums, n,
+                                                                         (int)parts);
+      else
+        sum_many_parts_kernel<<<wxx::grid_for(n, kT / 32), kT, 0, wxx::stream()>>>(dgate, sums, n,
+                                                                                   (int)parts);
       st = wxx::after_launch(__FILE__, __LINE__);
     }
   }
