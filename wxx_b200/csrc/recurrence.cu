@@ -492,7 +492,9 @@ __device__ __forceinline__ float* aligned_smem(float* p) {
 // 3.7 TB/s.  Measured and not kept: two channels a lane (80 and 61 us; a third of the
 // instructions less, but fewer warps to hide latencies), a second buffer of inputs
 // (85 us: the tiles it holds back are the ones that others wait for), pieces of 8 (95
-// us) and 32 positions (76 us forward, 151 backward), groups of groups (83 and 66 us).
+// us) and 32 positions (76 us forward, 151 backward), groups of groups (83 and 66 us),
+// a look at the tiles before while the own one is still being put together (85 and 63
+// us: it is repeated more often, and the own tile is published later).
 template <bool kTma, int kSeg, bool kWarpGate>
 __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
     recurrence_forward_kernel(float* __restrict__ h, float* __restrict__ h_last,
