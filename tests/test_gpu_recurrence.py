@@ -458,3 +458,96 @@ def test_autograd(rng):
     bound = U * G * (64 + 8 * L)
     for leaf, r, k in zip(leaves, ref, (1, 2 * max(1, np.abs(x).max()) * (D // H), 1)):
         close(leaf.grad.numpy(), r, bound * k)
+
+
+# gates about the places where exp(-gate), 1 + exp(-gate) and its reciprocal leave
+# the normal numbers, and far beyond
+FAR = [1, 20, 60, 86, 87.3, 87.4, 87.6, 88, 88.5, 88.7, 88.8, 89, 103, 104, 110, 200, 1e30, 3e38,
+       np.inf]
+
+
+def amplified(a):
+    """How many unit errors, one a position, a state holds at most: e = a e + 1."""
+    e, out = np.zeros(a[:, 0].shape), np.empty_like(a)
+    for t in range(a.shape[1]):
+        e = a[:, t] * e + 1
+        out[:, t] = e
+    return out
+
+
+def far_gates(rng, T, per, mixed):
+    """A head for each of the far gates and its opposite, (mixed) also gates that jump
+    between them and moderate ones; a gate serves ``per`` channels."""
+    values = np.array(FAR + [-v for v in FAR], np.float32)
+    gate = np.broadcast_to(values, (1, T, values.size))
+    if mixed:
+        gate = np.concatenate([rng.choice(values, gate.shape),
+                               rng.uniform(-110, 110, gate.shape).astype(np.float32)], -1)
+    x = rng.standard_normal((1, T, gate.shape[-1] * per)).astype(np.float32)
+    h0 = rng.standard_normal((1, gate.shape[-1] * per)).astype(np.float32)
+    a = recurrent._sigmoid(np.repeat(gate.astype(np.float64), per, -1))
+    return x, np.ascontiguousarray(gate), h0, a
+
+
+@pytest.mark.parametrize("per", [1, 8, 25, 32, 64])
+@pytest.mark.parametrize("T", [1, 40, 300])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_gates_far_from_zero(T, per, mixed, rng):
+    """Forward, one position at a time and backward agree with the 64-bit form for
+    every gate.  The bound is that of the tolerances above, entry by entry, with the
+    errors' own amplification in the place of L."""
+    F = _F()
+    x, gate, h0, a = far_gates(rng, T, per, mixed)
+    M = max(np.abs(x).max(), np.abs(h0).max())
+    ref, _ = recurrent.recurrence(x, gate, h0)
+    ahead = amplified(a)
+    tx, tg, th0 = up(x), up(gate), up(h0)
+    h, last = F.gated_recurrence(tx, tg, th0)
+    assert (np.abs(h.numpy() - ref) <= U * M * (64 + 8 * ahead)).all()
+    assert np.array_equal(last.numpy(), h.numpy()[:, -1])
+    state = up(h0)
+    for t in range(min(T, 40)):
+        F.gated_recurrence_step(up(x[:, t]), up(gate[:, t]), state)
+        assert (np.abs(state.numpy() - ref[:, t]) <= U * M * (64 + 8 * ahead[:, t])).all()
+
+    dh = rng.standard_normal(x.shape).astype(np.float32)
+    dlast = rng.standard_normal(h0.shape).astype(np.float32)
+    got = [v.numpy() for v in F.gated_recurrence_backward(up(dh), tx, tg, h, th0, None, up(dlast))]
+    dx, dg, dh0 = recurrent.recurrence_backward(dh, x, gate, h0, None, dlast)
+    # the gradient reaching a position: through the weights behind it
+    behind = np.ones_like(a)
+    behind[:, :-1] = a[:, 1:]
+    back = amplified(behind[:, ::-1])[:, ::-1]
+    G = max(np.abs(dh).max(), np.abs(dlast).max()) * back.max((0, 1))
+    bound = U * G * (64 + 8 * back)
+    assert (np.abs(got[0] - dx) <= bound).all()
+    assert (np.abs(got[2] - dh0) <= bound[:, 0]).all()
+    over = (bound + U * G * (64 + 8 * ahead)) * 2 * max(M, 1)
+    assert (np.abs(got[1] - dg) <= over.reshape(1, T, -1, per).sum(-1)).all()
+
+
+@pytest.mark.parametrize("per", [8, 25, 32, 64])
+def test_foreign_values_of_shared_gates(per, rng):
+    """A NaN gate makes its own head's states NaN up to the next document, an infinite x
+    its own channel's infinite or NaN; everything else keeps its bits."""
+    F = _F()
+    B, T, H = 2, 300, 5
+    D = per * H
+    x, gate, h0, _ = inputs(rng, B, T, D, H, True, False)
+    reset = np.zeros((B, T), np.uint32)
+    reset[:, 150] = 1
+    tr = up(reset, np.uint32)
+    ref = F.gated_recurrence(up(x), up(gate), up(h0), tr)[0].numpy()
+    gate[0, 100, 1] = np.nan
+    x[1, 60, 2 * per] = np.inf
+    x[1, 200, 3 * per + 1] = -np.inf
+    h, last = F.gated_recurrence(up(x), up(gate), up(h0), tr)
+    h = h.numpy()
+    assert np.array_equal(last.numpy(), h[:, -1], equal_nan=True)
+    assert np.isnan(h[0, 100:150, per:2 * per]).all()
+    assert not np.isfinite(h[1, 60:150, 2 * per]).any()
+    assert not np.isfinite(h[1, 200:, 3 * per + 1]).any()
+    h[0, 100:150, per:2 * per] = ref[0, 100:150, per:2 * per]
+    h[1, 60:150, 2 * per] = ref[1, 60:150, 2 * per]
+    h[1, 200:, 3 * per + 1] = ref[1, 200:, 3 * per + 1]
+    assert np.array_equal(h, ref)

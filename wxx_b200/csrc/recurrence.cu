@@ -51,8 +51,9 @@ constexpr int kWaitLimit = 1 << 21; // polls of a published word (about a second
 // The weights of two gates (of neighbouring positions, so that the additions and
 // products go in pairs): with e = exp(-g), a = 1 / (1 + e) and z = 1 - a = e a, each
 // good to a few ulp of itself (e carries half an ulp of g log2 e, and 1 + e >= 1 is
-// what the approximate reciprocal takes to an ulp).  Where e overflows, a is 0 and z
-// is NaN unless kBounded, which keeps e at 2^126: then a is 2^-126 and z is 1.
+// what the approximate reciprocal takes to an ulp).  Past e = 2^126 a is 0, and z is 0
+// and, where e overflows, NaN -- unless kBounded, which keeps e at 2^126: then a is
+// 2^-126 and z is 1.
 struct Weights {
   float a, z;
 };
@@ -81,8 +82,10 @@ struct Gate {
 __device__ __forceinline__ Gate gate_of(float g, Weights w) {
   return {g >= 0.f ? w.z : w.a, g >= 0.f};       // a NaN gives one
 }
+// Where e is past 2^126 the reciprocal is flushed: a is 0 and z is 0 or NaN, and neither
+// is below a, so the state is replaced.
 __device__ __forceinline__ Gate gate_of(Weights w) {
-  return {w.z <= w.a ? w.z : w.a, w.z <= w.a};
+  return {w.z < w.a ? w.z : w.a, w.z < w.a};
 }
 
 // a h + z x as the larger-weighted of the two plus the smaller weight times
