@@ -551,3 +551,34 @@ def test_foreign_values_of_shared_gates(per, rng):
     h[1, 60:150, 2 * per] = ref[1, 60:150, 2 * per]
     h[1, 200:, 3 * per + 1] = ref[1, 200:, 3 * per + 1]
     assert np.array_equal(h, ref)
+
+
+@pytest.mark.parametrize("per", [1, 4, 25, 32, 64])
+@pytest.mark.parametrize("T", [1, 16, 40, 300])
+def test_gradient_of_the_last_state_alone(T, per, rng):
+    """With no other gradient everything is what the weights hand back from the last
+    position, so the error is relative, entry by entry: a weight is good to 40 u of
+    itself (gates to -30), a product of T of them and the roundings between to u (42 T +
+    64).  dgate also takes the forward's error of h.  1e-36: products that have left
+    the normal numbers."""
+    F = _F()
+    gate = np.linspace(-30, 6, 37, dtype=np.float32)
+    H = gate.size
+    gate = np.ascontiguousarray(np.broadcast_to(gate, (2, T, H)))
+    x = rng.standard_normal((2, T, H * per)).astype(np.float32)
+    h0 = rng.standard_normal((2, H * per)).astype(np.float32)
+    dlast = (rng.uniform(0.5, 2, h0.shape) * rng.choice([-1, 1], h0.shape)).astype(np.float32)
+    zero = np.zeros_like(x)
+    h, _ = F.gated_recurrence(up(x), up(gate), up(h0))
+    got = F.gated_recurrence_backward(up(zero), up(x), up(gate), h, up(h0), None, up(dlast))
+    dx, dg, dh0 = recurrent.recurrence_backward(zero, x, gate, h0, None, dlast)
+    rel = U * (42 * T + 64)
+    assert (np.abs(got[0].numpy() - dx) <= rel * np.abs(dx) + 1e-36).all()
+    assert (np.abs(got[2].numpy() - dh0) <= rel * np.abs(dh0) + 1e-36).all()
+    wide = np.repeat(gate.astype(np.float64), per, -1)
+    a, z = recurrent._sigmoid(wide), recurrent._sigmoid(-wide)
+    before = np.concatenate([h0[:, None], recurrent.recurrence(x, gate, h0)[0][:, :-1]], 1)
+    M = max(np.abs(x).max(), np.abs(h0).max())
+    terms = np.abs(dx) * a * ((rel + 90 * U) * (np.abs(before) + np.abs(x))
+                              + U * M * (64 + 8 * np.minimum(T, 1 / z)))
+    assert (np.abs(got[1].numpy() - dg) <= terms.reshape(2, T, H, per).sum(-1) + 1e-36).all()

@@ -73,6 +73,13 @@ __device__ __forceinline__ void weights2(float g0, float g1, Weights& w0, Weight
   mul2(w0.z, w1.z, e0, e1, w0.a, w1.a);
 }
 
+// A gate's two weights in one number, the smaller of them, which is good to a few ulp of
+// itself (with the sign set where that is a; a is not 0 here): the other is 1 less it.
+__device__ __forceinline__ float pack(Weights w) { return w.z <= w.a ? w.z : -w.a; }
+__device__ __forceinline__ Weights unpack(float v) {
+  return v >= 0.f ? Weights{1.0f - v, v} : Weights{-v, 1.0f + v};    // a NaN gives two
+}
+
 // A gate as the smaller of its weights, which says how much of the other value is
 // mixed in, and whether the state is the one that is kept.
 struct Gate {
@@ -616,6 +623,8 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
   extern __shared__ float s_raw[];
   __shared__ Joint s;
   float *s_x = aligned_smem(s_raw), *s_d = s_x + kTile, *s_h = s_d + kTile, *s_g = s_h + kTile;
+  // kWarpGate, by turns: the weights of a tile's positions
+  constexpr int kRows = kWarps * kSteps;
   float2* s_w = reinterpret_cast<float2*>(s_g);
   constexpr bool kWarpGate = DG == 32;
   float gate = 0.f;                 // kWarpGate: of this thread's position of the next tile
@@ -640,8 +649,8 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
     else if (!own_gate) copy_gates(s_g, g, c, p, T, D);
     if (!kTma || !(kWarpGate || own_gate)) copies_arrive(&s.full);
   };
-  auto ready = [&](int) {
-    if (kWarpGate) weigh<true>(s_w, nullptr, gate, &s.full);
+  auto ready = [&](int turn) {
+    if (kWarpGate) weigh<true>(s_w + turn * kRows, nullptr, gate, &s.full);
   };
   const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !(kWarpGate || own_gate) ? blockDim.x : 0) +
                             (kWarpGate ? blockDim.x / 2 : 0);
@@ -654,8 +663,9 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
                       (own_gate ? (int)(threadIdx.x & 31)
                                 : (int)c.per(min(p.d, D - 1)) - first_gate(c, p));
     const int64_t state = (int64_t)p.b * D + p.d;
-    // the total gradient from a zero carry, dx and dgate per unit of it
-    float G[kSteps], z[kSteps], u[kSteps];
+    const float2* sw = s_w + turn * kRows + p.row;
+    // the total gradient from a zero carry, the weights, dgate per unit of the total
+    float G[kSteps], gates[kSteps], u[kSteps];
     Stretch mine = {1.0f, 0.0f};
     auto first_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
@@ -664,7 +674,7 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
         float slope[2];
         Weights w[2];
         if (kWarpGate) {
-          weighed(s_w + p.row, k0, w[0], w[1]);
+          weighed(sw, k0, w[0], w[1]);
         } else {
           float g[2];
 #pragma unroll
@@ -681,7 +691,7 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
           if (!kPlain && p.t0 + k == 0) before = h0 && here ? h0[state] : 0.f;
           if (!kPlain && (cut >> k & 1)) before = 0.f;
           u[k] = (before - s_x[at + k * 32]) * slope[e];
-          z[k] = w[e].z;
+          if (!kWarpGate) gates[k] = pack(w[e]);
           G[k] = mine.b + (here ? s_d[at + k * 32] : 0.f);
           mine.b = w[e].a * G[k];
           mine.A *= w[e].a;
@@ -695,18 +705,26 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
     const int64_t last = (int64_t)p.b * T + p.t0 + kSteps - 1;
     float* xo = dx + last * D + p.d;
     float* go = DG == 0 ? dg + last * D + p.d : nullptr;
-    // What the join gives reaches position k through the weights after it: 1 - z
-    // is a to 2^-24, which is enough for a product that only scales the carry.
+    // What the join gives reaches position k through the weights after it.  They are
+    // good to a few ulp of themselves here too: where the only gradient comes from later
+    // positions (that of the last state, say), all there is goes through them.
     float carried = v;
     auto second_run = [&](auto plain) {
       constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
       for (int k = kSteps - 1; k >= 0; --k) {
+        Weights w;
+        if (kWarpGate) {
+          const float2 both = sw[k];
+          w = {both.x, both.y};
+        } else {
+          w = unpack(gates[k]);
+        }
         const float total = G[k] + carried;
-        if (kPlain || k < p.left) *xo = z[k] * total;
+        if (kPlain || k < p.left) *xo = w.z * total;
         u[k] *= total;
         if (DG == 0 && (kPlain || k < p.left)) *go = u[k];
-        carried *= 1.0f - z[k];
+        carried *= w.a;
         if (!kPlain && (cut >> k & 1)) carried = 0.f;
         xo -= D;
         if (DG == 0) go -= D;
