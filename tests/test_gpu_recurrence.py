@@ -582,3 +582,36 @@ def test_gradient_of_the_last_state_alone(T, per, rng):
     terms = np.abs(dx) * a * ((rel + 90 * U) * (np.abs(before) + np.abs(x))
                               + U * M * (64 + 8 * np.minimum(T, 1 / z)))
     assert (np.abs(got[1].numpy() - dg) <= terms.reshape(2, T, H, per).sum(-1) + 1e-36).all()
+
+
+@pytest.mark.parametrize("per", [1, 8, 32])
+def test_weights_to_their_last_bits(per, rng):
+    """One position from a state of 0 or 1 shows the smaller weight, its gradients both.
+    Relative, at every gate: 4 u for the exponential, 2 u for the reciprocal, a rounding
+    (u) each for the exponential's correction, its product, 1 + e, e a and the result
+    are 11 u; dgate has both weights."""
+    F = _F()
+    gate = np.linspace(-86, 86, 4001, dtype=np.float32)
+    H = gate.size
+    g = up(gate.reshape(1, 1, H))
+    a, z = recurrent._sigmoid(gate.astype(np.float64)), recurrent._sigmoid(-gate.astype(np.float64))
+    one, zero = np.ones((1, 1, H * per)), np.zeros((1, 1, H * per))
+
+    def near(got, ref, units):
+        got = got.numpy().astype(np.float64).reshape(H, -1)
+        off = np.abs(got / ref[:, None] - 1).max() / U
+        assert off <= units, off
+
+    for value, start, weight, use in ((one, zero, z, gate >= 0), (zero, one, a, gate < 0)):
+        h, _ = F.gated_recurrence(up(value), g, up(start[:, 0]))
+        state = up(start[:, 0])
+        F.gated_recurrence_step(up(value[:, 0]), up(gate.reshape(1, H)), state)
+        for got in (h, state):
+            smaller = np.where(use, weight, 1.0)
+            off = np.abs(got.numpy().reshape(H, per) / smaller[:, None] - 1)[use].max() / U
+            assert off <= 12, off
+    h, _ = F.gated_recurrence(up(zero), g, up(one[:, 0]))
+    dx, dg, dh0 = F.gated_recurrence_backward(up(one), up(zero), g, h, up(one[:, 0]))
+    near(dx, z, 13)
+    near(dh0, a, 13)
+    near(dg, a * z * per, 26 + 8)

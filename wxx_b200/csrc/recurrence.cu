@@ -48,36 +48,52 @@ constexpr int forward_blocks(bool tma, int seg) { return tma && seg == 1 ? 4 : 3
 constexpr int kBackwardBlocks = 2;
 constexpr int kWaitLimit = 1 << 21; // polls of a published word (about a second)
 
-// The weights of two gates (of neighbouring positions, so that the additions and
-// products go in pairs): with e = exp(-g), a = 1 / (1 + e) and z = 1 - a = e a, each
-// good to a few ulp of itself (e carries half an ulp of g log2 e, and 1 + e >= 1 is
-// what the approximate reciprocal takes to an ulp).  Past e = 2^126 a is 0, and z is 0
-// and, where e overflows, NaN -- unless kBounded, which keeps e at 2^126: then a is
-// 2^-126 and z is 1.
+// A gate's weights a = sigmoid(g) and z = 1 - a are, in one order or the other (z is
+// the smaller where g >= 0), small = e / (1 + e) and large = 1 / (1 + e) with e =
+// exp(-|g|) <= 1, so that nothing overflows.  Each is good to a few ulp of itself: e = 2^y
+// 2^r, y = -|g| log2 e rounded (alone it would cost e y half ulps, 60 at |g| = 80) and r
+// what the product and the constant lost, so little that 2^r is 1 + r log 2; 1 + e is
+// what the approximate reciprocal takes to an ulp.  From |g| = 88 on small is 0, and gates
+// past 104 are taken as that, so that y and r are finite.  For two gates (of
+// neighbouring positions), so that the additions and products go in pairs.
+struct Halves {
+  float small, large;
+};
+__device__ __forceinline__ float far(float g) {
+  float t;
+  asm("min.NaN.f32 %0, %1, 0f42D00000;" : "=f"(t) : "f"(fabsf(g)));   // 104
+  return t;
+}
+__device__ __forceinline__ void halves2(float g0, float g1, Halves& w0, Halves& w1) {
+  constexpr float kC = -1.4426950408889634f;                          // -log2 e, and what is
+  constexpr float kLow = (float)(-1.4426950408889634 - (double)kC);   // left of it
+  constexpr float kLog2 = 0.6931471805599453f;
+  const float t0 = far(g0), t1 = far(g1);
+  float y0, y1, r0, r1, e0, e1, s0, s1;
+  mul2(y0, y1, t0, t1, kC, kC);
+  fma2(r0, r1, t0, t1, kC, kC, -y0, -y1);
+  fma2(r0, r1, t0, t1, kLow, kLow, r0, r1);
+  fma2(r0, r1, r0, r1, kLog2, kLog2, 1.0f, 1.0f);
+  mul2(e0, e1, fast_exp2(y0), fast_exp2(y1), r0, r1);
+  add2(s0, s1, e0, e1, 1.0f, 1.0f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(w0.large) : "f"(s0));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(w1.large) : "f"(s1));
+  mul2(w0.small, w1.small, e0, e1, w0.large, w1.large);
+}
+
 struct Weights {
   float a, z;
 };
-template <bool kBounded>
-__device__ __forceinline__ void weights2(float g0, float g1, Weights& w0, Weights& w1) {
-  float y0, y1, e0, e1, s0, s1;
-  mul2(y0, y1, g0, g1, -1.4426950408889634f, -1.4426950408889634f);
-  if (kBounded) {
-    asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(y0) : "f"(y0));
-    asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(y1) : "f"(y1));
-  }
-  e0 = fast_exp2(y0);
-  e1 = fast_exp2(y1);
-  add2(s0, s1, e0, e1, 1.0f, 1.0f);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(w0.a) : "f"(s0));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(w1.a) : "f"(s1));
-  mul2(w0.z, w1.z, e0, e1, w0.a, w1.a);
+__device__ __forceinline__ Weights weights_of(float g, Halves w) {
+  return g >= 0.f ? Weights{w.large, w.small} : Weights{w.small, w.large};
 }
 
-// A gate's two weights in one number, the smaller of them, which is good to a few ulp of
-// itself (with the sign set where that is a; a is not 0 here): the other is 1 less it.
-__device__ __forceinline__ float pack(Weights w) { return w.z <= w.a ? w.z : -w.a; }
+// Both weights in one number: the smaller, with the sign set where that is a (which may
+// be 0).  The other is 1 less it.
+__device__ __forceinline__ float pack(float g, Halves w) { return g >= 0.f ? w.small : -w.small; }
 __device__ __forceinline__ Weights unpack(float v) {
-  return v >= 0.f ? Weights{1.0f - v, v} : Weights{-v, 1.0f + v};    // a NaN gives two
+  const float small = fabsf(v), large = 1.0f - small;
+  return __float_as_int(v) >= 0 ? Weights{large, small} : Weights{small, large};
 }
 
 // A gate as the smaller of its weights, which says how much of the other value is
@@ -86,13 +102,9 @@ struct Gate {
   float w;
   bool keep;
 };
-__device__ __forceinline__ Gate gate_of(float g, Weights w) {
-  return {g >= 0.f ? w.z : w.a, g >= 0.f};       // a NaN gives one
-}
-// Where e is past 2^126 the reciprocal is flushed: a is 0 and z is 0 or NaN, and neither
-// is below a, so the state is replaced.
+__device__ __forceinline__ Gate gate_of(float g, Halves w) { return {w.small, g >= 0.f}; }
 __device__ __forceinline__ Gate gate_of(Weights w) {
-  return {w.z < w.a ? w.z : w.a, w.z < w.a};
+  return {w.z < w.a ? w.z : w.a, w.z < w.a};     // a NaN gives one
 }
 
 // a h + z x as the larger-weighted of the two plus the smaller weight times
@@ -330,12 +342,12 @@ __device__ __forceinline__ float warp_gate(const Operand& g, const Chain& c, con
   if (row >= (int)(blockDim.x >> 5) * kSteps || t >= T) return INFINITY;
   return g.p[p.b * g.bs + t * g.ts + first_gate(c, p)];
 }
-template <bool kBounded>
 __device__ __forceinline__ void weigh(float2* tile, float* upto, float gate, uint64_t* bar) {
   const int rows = (blockDim.x >> 5) * kSteps, row = threadIdx.x;
   if ((row & ~31) >= rows) return;
-  Weights w, same;
-  weights2<kBounded>(gate, gate, w, same);
+  Halves half, same;
+  halves2(gate, gate, half, same);
+  const Weights w = weights_of(gate, half);
   if (upto) {
     static_assert(kSteps == 16, "a piece is half a warp");
     float A = w.a;
@@ -535,7 +547,7 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
     if (!kTma || !(kWarpGate || own_gate)) copies_arrive(&s.full);
   };
   auto ready = [&](int turn) {
-    if (kWarpGate) weigh<false>(s_w + turn * kRows, s_A + turn * kRows, gate, &s.full);
+    if (kWarpGate) weigh(s_w + turn * kRows, s_A + turn * kRows, gate, &s.full);
   };
   const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !(kWarpGate || own_gate) ? blockDim.x : 0) +
                             (kWarpGate ? blockDim.x / 2 : 0);
@@ -556,24 +568,33 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
       mine = {1.0f, 0.0f};
 #pragma unroll
       for (int k0 = 0; k0 < kSteps; k0 += 2) {
-        float g[2];
-        Weights w[2];
+        Gate gates[2];
+        float a[2];
         if (kWarpGate) {
+          Weights w[2];
           weighed(sw, k0, w[0], w[1]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) gates[e] = gate_of(w[e]);
         } else {
+          float g[2];
+          Halves w[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k)            // past the end: keep the state
             g[k] = kPlain || k0 + k < p.left ? sg[(k0 + k) * stride] : INFINITY;
-          weights2<false>(g[0], g[1], w[0], w[1]);
+          halves2(g[0], g[1], w[0], w[1]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            gates[e] = gate_of(g[e], w[e]);
+            a[e] = weights_of(g[e], w[e]).a;
+          }
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int k = k0 + e;
           if (!kPlain && (cut >> k & 1)) mine = {-0.0f, 0.0f};
           const float now = kPlain || k < p.left ? sx[k * 32] : 0.f;
-          const Gate mixed = kWarpGate ? gate_of(w[e]) : gate_of(g[e], w[e]);
-          mine.b = kPlain ? mix(mixed, mine.b, now) : mix_any(mixed, mine.b, now);
-          if (!kWarpGate) mine.A *= w[e].a;
+          mine.b = kPlain ? mix(gates[e], mine.b, now) : mix_any(gates[e], mine.b, now);
+          if (!kWarpGate) mine.A *= a[e];
           upto[k] = mine;
         }
       }
@@ -650,7 +671,7 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
     if (!kTma || !(kWarpGate || own_gate)) copies_arrive(&s.full);
   };
   auto ready = [&](int turn) {
-    if (kWarpGate) weigh<true>(s_w + turn * kRows, nullptr, gate, &s.full);
+    if (kWarpGate) weigh(s_w + turn * kRows, nullptr, gate, &s.full);
   };
   const unsigned arrivals = (kTma ? 1 : 0) + (!kTma || !(kWarpGate || own_gate) ? blockDim.x : 0) +
                             (kWarpGate ? blockDim.x / 2 : 0);
@@ -677,10 +698,16 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
           weighed(sw, k0, w[0], w[1]);
         } else {
           float g[2];
+          Halves half[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k)
             g[k] = kPlain || k0 + k < p.left ? sg[(k0 + k) * stride] : INFINITY;
-          weights2<true>(g[0], g[1], w[0], w[1]);
+          halves2(g[0], g[1], half[0], half[1]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            w[e] = weights_of(g[e], half[e]);
+            gates[k0 + e] = pack(g[e], half[e]);
+          }
         }
         mul2(slope[0], slope[1], w[0].a, w[1].a, w[0].z, w[1].z);    // d a / d gate
 #pragma unroll
@@ -691,7 +718,6 @@ __global__ void __launch_bounds__(kT, kBackwardBlocks)
           if (!kPlain && p.t0 + k == 0) before = h0 && here ? h0[state] : 0.f;
           if (!kPlain && (cut >> k & 1)) before = 0.f;
           u[k] = (before - s_x[at + k * 32]) * slope[e];
-          if (!kWarpGate) gates[k] = pack(w[e]);
           G[k] = mine.b + (here ? s_d[at + k * 32] : 0.f);
           mine.b = w[e].a * G[k];
           mine.A *= w[e].a;
@@ -812,8 +838,8 @@ __global__ void recurrence_step_kernel(float* __restrict__ state, const float* _
        i += (int64_t)gridDim.x * kT) {
     const unsigned b = (unsigned)i / D, d = (unsigned)i - b * D;
     const float gate = g[b * g_ld + d / per];
-    Weights w, same;
-    weights2<false>(gate, gate, w, same);
+    Halves w, same;
+    halves2(gate, gate, w, same);
     state[i] = mix_any(gate_of(gate, w), state[i], x[b * x_ld + d]);
   }
 }
