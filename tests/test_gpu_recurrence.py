@@ -615,3 +615,16 @@ def test_weights_to_their_last_bits(per, rng):
     near(dx, z, 13)
     near(dh0, a, 13)
     near(dg, a * z * per, 26 + 8)
+
+
+def test_gates_without_channels():
+    """Gates of no channels receive the sum over none: zero, not what the memory held."""
+    F = _F()
+    for _ in range(4):
+        used = up(np.full((2, 3, 5), 7.0))
+        del used
+        x, gate = up(np.zeros((2, 3, 0))), up(np.zeros((2, 3, 5)))
+        h, _ = F.gated_recurrence(x, gate)
+        dx, dg, dh0 = F.gated_recurrence_backward(x, x, gate, h)
+        assert dx.shape == [2, 3, 0] and dh0 is None
+        assert np.array_equal(dg.numpy(), np.zeros((2, 3, 5)))

@@ -1074,7 +1074,12 @@ WXX_EXPORT int wxx_gated_recurrence_backward(float* dx, float* dgate, float* dh0
                                              int64_t H) {
   WXX_REQUIRE_INIT();
   if (int st = check_sizes("wxx_gated_recurrence_backward", B, T, D, H)) return st;
-  if (B * D == 0) return WXX_OK;
+  if (B * D == 0) {                   // a gate of no channels: the sum over none
+    if (B * T * H > 0)
+      WXX_CUDA_CHECK(cudaMemsetAsync(dgate, 0, (size_t)(B * T * H) * sizeof(float),
+                                     wxx::stream()));
+    return WXX_OK;
+  }
   if (T == 0) return dh0 ? copy_state(dh0, dlast, B * D) : WXX_OK;
   // The gate's gradient is summed over a head's channels in the kernel where
   // they lie in one warp's 32 neighbours, by partial sums per 32 channels where
