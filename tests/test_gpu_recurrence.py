@@ -628,3 +628,15 @@ def test_gates_without_channels():
         dx, dg, dh0 = F.gated_recurrence_backward(x, x, gate, h)
         assert dx.shape == [2, 3, 0] and dh0 is None
         assert np.array_equal(dg.numpy(), np.zeros((2, 3, 5)))
+
+
+# both sides of the rules that choose a kernel: 23 and 24 blocks of 32 channels (groups of
+# 32 or 8 tiles), 255 partial sums of a gate and more (a thread or a warp adds them), from
+# single channels and from blocks of 32
+SIDES = [(1, 700, 736, 736), (1, 700, 737, 737), (1, 1100, 736, 23), (4, 1100, 192, 6),
+         (1, 150, 255, 1), (1, 150, 514, 2), (2, 140, 1000, 1), (1, 40, 8160, 1), (1, 40, 8192, 1)]
+
+
+@pytest.mark.parametrize("B,T,D,H", SIDES)
+def test_both_sides_of_the_rules(B, T, D, H, rng):
+    test_forward_and_backward(B, T, D, H, True, True, rng)
