@@ -304,3 +304,31 @@ def test_module_with_mask_trains_the_logits(rng):
         assert abs(loss.item() - (rows * w).sum() / w.sum()) <= 2 * tau * tau * bl
         ref = recurrent.distill_backward((w / w.sum())[:, None], z, top, ids, tau)
         assert np.abs(leaf.grad.numpy() - ref).max() <= 2 * tau * bg
+
+
+@pytest.mark.parametrize("N,V,sliced", [(1100, 300, False), (3, 1021, False), (4, 5001, False),
+                                        (4, 6001, True), (2, 60001, False)])
+@pytest.mark.parametrize("tau", [1.0, 1.5, 2.0])
+def test_probabilities_of_far_logits(N, V, sliced, tau, rng):
+    """Logits to 80 tau below the largest, which is 0, so that their distances are
+    exact: the gradient off the one stored entry is grad tau q.  Relative, entry by
+    entry: 4 u for the exponential, u each for its argument's correction and product,
+    the same for the terms of the sum and 16 u for adding them in a tree, u each for its
+    reciprocal and three products: 32 u."""
+    F = _F()
+    far = np.sort(rng.uniform(0, 80 * tau, (N, V)), -1)
+    far[:, 0] = 0
+    z = (-far).astype(np.float32)
+    order = rng.permutation(V)
+    z = np.ascontiguousarray(z[:, order])
+    best = np.full((N, 1), int(np.flatnonzero(order == 0)[0]), np.uint32)
+    tz = up(np.concatenate([z[:, :1], z, z[:, :2]], -1))[:, 1:1 + V] if sliced else up(z)
+    top, ids = up(np.zeros((N, 1))), up(best, np.uint32)
+    loss, stats = F.distill_loss(tz, top, ids, tau)
+    grad = rng.uniform(0.5, 2, (N, 1)).astype(np.float32)
+    d = F.distill_loss_backward(up(grad), tz, top, ids, stats, tau).numpy().astype(np.float64)
+    _, _, q = recurrent.distill(z, np.zeros((N, 1)), best, tau)
+    ref = q * grad.astype(np.float64) * tau
+    others = np.arange(V) != best[0, 0]
+    off = np.abs(d / ref - 1)[:, others].max() / U
+    assert off <= 32, off
