@@ -238,7 +238,10 @@ __device__ int best_pairs(const Row& row, int K, Select& s, float& top, float& s
     for (int k = 0; k < kAhead; ++k)
       n = largest<NAN_KEY>(largest<NAN_KEY>(n, v[k].x, v[k].y), v[k].z, v[k].w);
     if (SUM) {
-      // nothing but -inf (and perhaps NaN) so far: shifted by any number, they are 0
+      // exp(v - n) is 2^y with y = (v - n) log2 e rounded: y half ulps lost, but a term weighs
+      // its probability, over which the mean of y is log2 V at most, so the sum loses less
+      // than by being added up.
+      // Nothing but -inf (and perhaps NaN) so far: shifted by any number, they are 0.
       const float shift = n == -INFINITY ? 0.f : n;
       if (n > m) part *= fast_exp2((m - n) * 1.4426950408889634f);
       float e = 0.f;
