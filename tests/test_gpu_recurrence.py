@@ -631,10 +631,11 @@ def test_gates_without_channels():
 
 
 # both sides of the rules that choose a kernel: 23 and 24 blocks of 32 channels (groups of
-# 32 or 8 tiles), 255 partial sums of a gate and more (a thread or a warp adds them), from
-# single channels and from blocks of 32
+# 32 or 8 tiles), 99 partial sums of a gate and 100 and more (a thread or a warp adds them),
+# from single channels and from blocks of 32
 SIDES = [(1, 700, 736, 736), (1, 700, 737, 737), (1, 1100, 736, 23), (4, 1100, 192, 6),
-         (1, 150, 255, 1), (1, 150, 514, 2), (2, 140, 1000, 1), (1, 40, 8160, 1), (1, 40, 8192, 1)]
+         (1, 150, 99, 1), (1, 150, 202, 2), (3, 70, 300, 3), (1, 150, 255, 1), (2, 140, 1000, 1),
+         (1, 40, 3168, 1), (1, 40, 3200, 1), (1, 40, 8160, 1)]
 
 
 @pytest.mark.parametrize("B,T,D,H", SIDES)

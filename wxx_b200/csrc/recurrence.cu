@@ -814,9 +814,11 @@ __global__ void sum_parts_kernel(float* __restrict__ out, const float* __restric
   }
 }
 
-// The same for many parts: a warp has an output.  Backward over (4, 4096, 1000) with one
-// gate takes 77 us, 147 with a thread an output; with 100 channels a gate 99 and 91.
-constexpr int kManyParts = 256;
+// The same for many parts: a warp has an output.  Backward over (4, 4096, 1000) with a
+// thread and with a warp an output: 87 and 96 us with 50 parts, 93 and 84 with 100, 90 and
+// 75 with 250, 150 and 77 with 1000; over (1, 1024, 1000) 17 and 13 us with 100, 24 and 12
+// with 250.
+constexpr int kManyParts = 100;
 __global__ void sum_many_parts_kernel(float* __restrict__ out, const float* __restrict__ in,
                                       int64_t n, int parts) {
   const int lane = threadIdx.x & 31, warps = kT / 32;
