@@ -332,3 +332,10 @@ def test_probabilities_of_far_logits(N, V, sliced, tau, rng):
     others = np.arange(V) != best[0, 0]
     off = np.abs(d / ref - 1)[:, others].max() / U
     assert off <= 32, off
+
+
+@pytest.mark.parametrize("N", [511, 512])
+@pytest.mark.parametrize("V,K", [(1021, 17), (200, 64)])
+def test_both_sides_of_many_rows(N, V, K, rng):
+    """Short rows: a block a row below 512 of them, a warp a row from there."""
+    test_loss_and_gradient(N, V, K, 1.5, True, rng)

@@ -311,13 +311,17 @@ __global__ void __launch_bounds__(kT)
 // Short rows: a warp a row, its logits in registers (entry 32 j + lane in v[j]) and a few
 // stored entries a lane, so there is no barrier and one exponential a logit.  Bound by
 // instructions and, with few rows, latencies: 4096 x 1021 logits with 64 stored take 6
-// us forward (a block a row 23) and 12 backward (14), 4096 x 200 4 and 8 us (21 and 12).
-// Backward, a warp is longer at comparing the stored ids with one another: 128 rows of
-// 1021 6 us against 4, 4096 with 128 stored 21 against 19, so it has many rows and at
-// most 64 stored entries.
+// us forward (a block a row 23) and 9 backward (13), 4096 x 200 4 and 8 us (21 and 12; with
+// 17 stored backward 3 and 9).
+// Backward, a warp is longer at comparing the stored ids with one another.  A warp and a
+// block a row, 64 of 1021 stored: 128 rows 3.3 and 3.1 us, 512 rows 3.5 both, 768 rows 4.0
+// both, 1023 rows 4.0 and 4.4, 2048 rows 5.4 and 7.3; 17 stored: 128 rows 2.6 and 2.8, 1023
+// rows 3.0 and 4.0.  4096 rows with 128 stored took 21 and 19 us.  So it has 512 rows and
+// more, and at most 64 stored entries.  (Backward: one call after the other over the same
+// rows.)
 constexpr int kRowWarps = 4;
 constexpr int kForwardEntries = 4, kBackwardEntries = 2;       // of a lane
-constexpr int kForwardV = 2048, kBackwardV = 1024, kBackwardN = 1024;
+constexpr int kForwardV = 2048, kBackwardV = 1024, kBackwardN = 512;
 
 template <int ITEMS>
 __global__ void __launch_bounds__(kRowWarps * 32)
