@@ -311,8 +311,7 @@ __global__ void __launch_bounds__(kT)
 // Short rows: a warp a row, its logits in registers (entry 32 j + lane in v[j]) and a few
 // stored entries a lane, so there is no barrier and one exponential a logit.  Bound by
 // instructions and, with few rows, latencies: 4096 x 1021 logits with 64 stored take 6
-// us forward (a block a row 23) and 9 backward (13), 4096 x 200 4 and 8 us (21 and 12; with
-// 17 stored backward 3 and 9).
+// us forward (a block a row 23) and 12 backward (14), 4096 x 200 6 and 8 us (21 and 12).
 // Backward, a warp is longer at comparing the stored ids with one another.  A warp and a
 // block a row, 64 of 1021 stored: 128 rows 3.3 and 3.1 us, 512 rows 3.5 both, 768 rows 4.0
 // both, 1023 rows 4.0 and 4.4, 2048 rows 5.4 and 7.3; 17 stored: 128 rows 2.6 and 2.8, 1023

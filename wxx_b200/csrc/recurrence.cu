@@ -287,7 +287,7 @@ __device__ __forceinline__ void copies_arrive(uint64_t* bar) {
 // This warp's piece of an operand, `back` positions earlier (zero before position 0,
 // after the last and past the last channel).  Where rows and channels come in pairs of
 // floats, half the lanes copy a position each, two channels at a time: (16, 4096, 250)
-// 49 + 76 us, 53 + 88 float by float.
+// 53 + 91 us, 59 + 103 float by float.
 __device__ __forceinline__ void copy_piece(float* tile, const Operand& o, const Place& p,
                                            int back, int T, int D) {
   const int lane = threadIdx.x & 31;
@@ -335,7 +335,7 @@ __device__ __forceinline__ void copy_gates(float* tile, const Operand& g, const 
 // begun, have put its weights into shared memory, where a pair of positions is one
 // read, and for the forward the products of a over its piece (a piece is 16 lanes).
 // Their arrival is part of the tile's barrier.  Weighed in every channel, (32, 1024,
-// 1024) with a gate per 64 channels took 70 + 105 us, so 62 + 101.
+// 1024) with a gate per 64 channels took 70 us forward, so 60.
 __device__ __forceinline__ float warp_gate(const Operand& g, const Chain& c, const Place& p,
                                            int T) {
   const int row = threadIdx.x, t = p.t0 - p.row + row;
@@ -505,18 +505,19 @@ __device__ __forceinline__ float* aligned_smem(float* p) {
 // join gives.  A warp whose piece is whole and holds no reset (nearly all) runs
 // without the tests for them, and runs it again with them where it comes out
 // infinite or NaN: a difference of two values may have passed the largest number
-// (asking costs 1 us at (16, 8192, 256)).
+// (asking costs 1 us at (1, 65536, 256) at most).
 //
 // A row of 8192 positions has 64 tiles, so (16, 8192, 256) gives 8192 tiles for 592
-// blocks: 79 us, 5.1 TB/s of its 403 MB, the join's looks at other tiles and the
-// latency of a tile's steps taking what a plain copy would not (without any join 73
-// us).  (1, 65536, 256) has 8 rows of tiles side by side and waits for its hops: 54 us,
-// 3.7 TB/s.  Measured and not kept: two channels a lane (80 and 61 us; a third of the
+// blocks: 77 us, 5.2 TB/s of its 403 MB, the join's looks at other tiles and the
+// latency of a tile's steps taking what a plain copy would not (without any join 5 us
+// less).  (1, 65536, 256) has 8 rows of tiles side by side and waits for its hops: 55 us,
+// 3.7 TB/s.  Measured against 79 and 54 us and not kept: two channels a lane (80 and 61 us; a third of the
 // instructions less, but fewer warps to hide latencies), a second buffer of inputs
 // (85 us: the tiles it holds back are the ones that others wait for), pieces of 8 (95
-// us) and 32 positions (76 us forward, 151 backward), groups of groups (83 and 66 us),
-// a look at the tiles before while the own one is still being put together (85 and 63
-// us: it is repeated more often, and the own tile is published later).
+// us) and 32 positions (76 us forward, but 151 backward, 14 more, and the length is one
+// for both), groups of groups (83 and 66 us), a look at the tiles before while the own
+// one is still being put together (85 and 63 us: it is repeated more often, and the own
+// tile is published later).
 template <bool kTma, int kSeg, bool kWarpGate>
 __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
     recurrence_forward_kernel(float* __restrict__ h, float* __restrict__ h_last,
@@ -626,10 +627,10 @@ __global__ void __launch_bounds__(kT, forward_blocks(kTma, kSeg))
 
 // The same tiles with time reversed: c_t = a_t r_t (dh_t + c_{t+1}) is what
 // position t hands to t - 1.  Reads dh, x, gate, h, writes dx, dgate: 24 bytes a
-// position; (16, 8192, 256) takes 137 us, 5.9 TB/s of its 805 MB (135 us without any
-// join).  DG: where the gate's gradient goes -- 1: sums over the `per` lanes
-// of a head (a power of two below 32; the first of them writes), 32: sums over the
-// warp, one per block of 32 channels; 0: every channel's own.
+// position; (16, 8192, 256) takes 135 us, 5.9 TB/s of its 805 MB (138 us with documents;
+// without any join 2 us less).  DG: where the gate's gradient goes -- 1: sums over the
+// `per` lanes of a head (a power of two below 32; the first of them writes), 32: sums over
+// the warp, one per block of 32 channels; 0: every channel's own.
 template <bool kTma, int kSeg, int DG>
 __global__ void __launch_bounds__(kT, kBackwardBlocks)
     recurrence_backward_kernel(float* __restrict__ dx, float* __restrict__ dg,

@@ -366,10 +366,10 @@ __device__ __forceinline__ void in_order(Select& s, int n, int K, F put) {
   if (t < K) put(t, mine);
 }
 
-// A block a row.  4 bytes an entry: the top 64 of 4096 x 50304 in 150 us, 5.5 TB/s.
+// A block a row.  4 bytes an entry: the top 64 of 4096 x 50304 in 154 us, 5.4 TB/s.
 // Two blocks of 1024 threads share an SM, one streams its row while the other picks;
 // what is left of the time is where both pick (asking L2 for a later block's row in
-// the meantime took the same rows from 150 to 178 us).
+// the meantime took 28 us longer).
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS, 2048 / THREADS)
     topk_kernel(float* __restrict__ values, uint32_t* __restrict__ ids,
@@ -655,7 +655,9 @@ struct StateTable {
 // in place and a beam is read once however many follow it.  Beams that follow
 // themselves are not touched.  MAX: beams, at most; four words at a time where the
 // rows are 16-byte aligned.  Bound by memory: 8 items of 8 beams with four caches of 700
-// x 1024 floats (about 1.1 GB read and written) in 165 us, 6.5 TB/s.
+// x 1024 floats (about 1.1 GB read and written) in 165 us, 6.5 TB/s.  Of more than 8 beams a
+// thread holds twice as many (140 registers, one block an SM) and is further from it: 4
+// items of 16 beams (1.18 GB) 221 us, 5.3 TB/s, 6 of 9 (0.95 GB) 218 us, 4.4 TB/s.
 template <int MAX>
 __global__ void __launch_bounds__(kT)
     beam_reorder_kernel(const __grid_constant__ StateTable tab,
