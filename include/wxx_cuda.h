@@ -463,6 +463,54 @@ int wxx_beam_reorder(int n, uint32_t* const* state, const int64_t* row, const in
 int wxx_beam_append(uint32_t* ids, int64_t ld, int64_t rows, const uint32_t* tokens,
                     uint32_t* cur_len, int64_t most);
 
+/* ---------------------------------------------------------------- retention
+ * No reference counterpart: the parts of a retention mixer (functional.rotary /
+ * linear_attention / group_norm). */
+/* Rotary positions: y (B, T, heads * d) from x (unit stride inside, the given batch and time
+ * strides), the pairs among the first r channels of every head turned by position * turns full
+ * turns (turns: r / 2 doubles on the HOST, r <= 512) and multiplied by gain, the others copied.
+ * positions (T) with p_bs = 0 or (B, T) with p_bs = T, u32, NULL: 0, 1, ...; offset is added.
+ * apart: a pair is (i, i + r / 2), else (2 i, 2 i + 1).  back: the gradient's map. */
+int wxx_rotary(float* y, const float* x, int64_t x_bs, int64_t x_ts, const uint32_t* positions,
+               int64_t p_bs, int64_t offset, const double* turns, int r, float gain, int64_t B,
+               int64_t T, int64_t heads, int64_t d, int apart, int back);
+/* Linear attention with a decay l = exp(log_decay) for each head, S_t = l S_{t-1} + k_t v_t^T, o_t =
+ * scale S_t^T q_t: o (B, T, H dv) and the state after the last position, last (B, H, dk, dv), from q,
+ * k (B, T, H dk) and v (B, T, H dv), unit stride inside and the given batch and time strides.  h0:
+ * the state before position 0 (NULL: zero); reset (B, T) u32: where it is not zero the state before
+ * that position is zero (NULL: nowhere).  dk, dv <= 256. */
+int wxx_linear_attention(float* o, float* last, const float* q, int64_t q_bs, int64_t q_ts,
+                         const float* k, int64_t k_bs, int64_t k_ts, const float* v, int64_t v_bs,
+                         int64_t v_ts, const float* log_decay, const float* h0,
+                         const uint32_t* reset, int64_t B, int64_t T, int64_t H, int64_t dk,
+                         int64_t dv, float scale);
+/* Its gradients dq, dk_out (B, T, H dk), dv_out (B, T, H dv) and dh0 (NULL: not wanted) from d_o (B, T,
+ * H dv), the gradient of last dlast (NULL: zero) and the forward's inputs. */
+int wxx_linear_attention_backward(float* dq, float* dk_out, float* dv_out, float* dh0,
+                                  const float* d_o, const float* dlast, const float* q,
+                                  int64_t q_bs, int64_t q_ts, const float* k, int64_t k_bs,
+                                  int64_t k_ts, const float* v, int64_t v_bs, int64_t v_ts,
+                                  const float* log_decay, const float* h0, const uint32_t* reset,
+                                  int64_t B, int64_t T, int64_t H, int64_t dk, int64_t dv,
+                                  float scale);
+/* One position per sequence, in place: state (B, H, dk, dv) <- l state + k v^T, then o (B, H dv) =
+ * scale state^T q; q, k, v with row strides q_ld, k_ld, v_ld. */
+int wxx_linear_attention_step(float* o, float* state, const float* q, int64_t q_ld, const float* k,
+                              int64_t k_ld, const float* v, int64_t v_ld, const float* log_decay,
+                              int64_t B, int64_t H, int64_t dk, int64_t dv, float scale);
+/* Group norm over trailing channels: z = (x - mean) inv over each sample's G groups of C / G
+ * channels at all S positions of x (N, S, C), n = gamma z + beta (C; NULL: 1, 0), y = act(n) or, with
+ * gate (like x; NULL: none), n act(gate); activation 0 none, 1 ReLU, 2 SiLU, 3 GELU (tanh form).
+ * mean and inv = 1 / sqrt(var + eps) are (N, G). */
+int wxx_group_norm(float* y, float* mean, float* inv, const float* x, const float* gate,
+                   const float* gamma, const float* beta, int64_t N, int64_t S, int64_t C,
+                   int64_t G, int activation, float eps);
+/* Its gradients dx, dgate (like x; dgate NULL without a gate), dgamma and dbeta (C). */
+int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, float* dgate, const float* dy,
+                            const float* x, const float* gate, const float* gamma,
+                            const float* beta, const float* mean, const float* inv, int64_t N,
+                            int64_t S, int64_t C, int64_t G, int activation);
+
 /* ---------------------------------------------------------------- NCCL
  * No reference counterpart (the reference drives one WebGPU device): the
  * all-gather of batch-sharded outputs across the GPUs of one node. */

@@ -1,0 +1,135 @@
+"""64-bit restatements of rotary positions, linear attention with a decay for each head,
+and group norm with an activation, from their definitions (they have no counterpart in
+the reference)."""
+
+import numpy as np
+
+
+def rotary(x, heads, frequencies, gain=1.0, positions=None, offset=0, layout="half", back=False):
+    """x (B, T, D) with every head's first pairs turned by position * frequency."""
+    x = np.asarray(x, np.float64)
+    B, T, D = x.shape
+    r = 2 * len(frequencies)
+    p = np.arange(T) if positions is None else np.asarray(positions).astype(np.int64)
+    angle = np.broadcast_to((p + offset)[..., None] * np.asarray(frequencies), (B, T, r // 2))
+    c, s = gain * np.cos(angle)[:, :, None], gain * np.sin(angle)[:, :, None]
+    s = -s if back else s
+    y = x.reshape(B, T, heads, D // heads).copy()
+    i = np.arange(r // 2)
+    a, b = (i, i + r // 2) if layout == "half" else (2 * i, 2 * i + 1)
+    u, v = y[..., a], y[..., b]
+    y[..., a], y[..., b] = u * c - v * s, u * s + v * c
+    return y.reshape(B, T, D)
+
+
+def _heads(t, H):
+    t = np.asarray(t, np.float64)
+    return t.reshape(*t.shape[:-1], H, t.shape[-1] // H)
+
+
+def linear_attention(q, k, v, log_decay, h0=None, reset=None, scale=1.0):
+    """(o, last) of S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t."""
+    lam = np.exp(np.asarray(log_decay, np.float64))[None, :, None, None]
+    H = lam.shape[1]
+    q, k, v = (_heads(t, H) for t in (q, k, v))
+    B, T, _, dk = q.shape
+    S = np.zeros((B, H, dk, v.shape[-1])) if h0 is None else np.array(h0, np.float64)
+    o = np.empty((B, T, H, v.shape[-1]))
+    for t in range(T):
+        if reset is not None:
+            S = np.where(np.asarray(reset)[:, t, None, None, None] != 0, 0.0, lam * S)
+        else:
+            S = lam * S
+        S = S + k[:, t, :, :, None] * v[:, t, :, None, :]
+        o[:, t] = scale * np.einsum("bhp,bhpr->bhr", q[:, t], S)
+    return o.reshape(B, T, -1), S
+
+
+def linear_attention_backward(do, q, k, v, log_decay, h0=None, reset=None, dlast=None, scale=1.0):
+    """(dq, dk, dv, dh0): the states forwards, their gradients R backwards."""
+    lam = np.exp(np.asarray(log_decay, np.float64))[None, :, None, None]
+    H = lam.shape[1]
+    q, k, v, do = (_heads(t, H) for t in (q, k, v, do))
+    B, T, _, dk = q.shape
+    S = np.zeros((B, H, dk, v.shape[-1])) if h0 is None else np.array(h0, np.float64)
+    cut = np.zeros((B, T), bool) if reset is None else np.asarray(reset) != 0
+    dq, dkey, dval = np.empty_like(q), np.empty_like(k), np.empty_like(v)
+    for t in range(T):
+        S = np.where(cut[:, t, None, None, None], 0.0, lam * S)
+        S = S + k[:, t, :, :, None] * v[:, t, :, None, :]
+        dq[:, t] = scale * np.einsum("bhpr,bhr->bhp", S, do[:, t])
+    R = np.zeros_like(S) if dlast is None else np.array(dlast, np.float64)
+    for t in range(T - 1, -1, -1):
+        R = R + scale * q[:, t, :, :, None] * do[:, t, :, None, :]
+        dkey[:, t] = np.einsum("bhpr,bhr->bhp", R, v[:, t])
+        dval[:, t] = np.einsum("bhpr,bhp->bhr", R, k[:, t])
+        R = np.where(cut[:, t, None, None, None], 0.0, lam * R)
+    return dq.reshape(B, T, -1), dkey.reshape(B, T, -1), dval.reshape(B, T, -1), R
+
+
+def _logistic(v):
+    e = np.exp(-np.abs(v))
+    return np.where(v >= 0, 1 / (1 + e), e / (1 + e))
+
+
+_C = 0.7978845608
+
+
+def act(v, name):
+    if name is None:
+        return v
+    if name == "relu":
+        return np.maximum(v, 0)
+    if name == "silu":
+        return v * _logistic(v)
+    return 0.5 * v * (1 + np.tanh(_C * (v + 0.044715 * v ** 3)))
+
+
+def slope(v, name):
+    if name is None:
+        return np.ones_like(v)
+    if name == "relu":
+        return (v > 0).astype(np.float64)
+    if name == "silu":
+        p = _logistic(v)
+        return p + v * p * _logistic(-v)
+    t = np.tanh(_C * (v + 0.044715 * v ** 3))
+    return 0.5 * (1 + t) + 0.5 * v * (1 - t * t) * _C * (1 + 3 * 0.044715 * v * v)
+
+
+def _normalised(x, groups, gamma, beta, eps):
+    x = np.asarray(x, np.float64)
+    N, C = x.shape[0], x.shape[-1]
+    w = x.reshape(N, -1, groups, C // groups)
+    mean = w.mean((1, 3), keepdims=True)
+    inv = 1 / np.sqrt(((w - mean) ** 2).mean((1, 3), keepdims=True) + eps)
+    z = (w - mean) * inv
+    gamma = np.ones(C) if gamma is None else np.asarray(gamma, np.float64)
+    beta = np.zeros(C) if beta is None else np.asarray(beta, np.float64)
+    gamma, beta = gamma.reshape(groups, -1), beta.reshape(groups, -1)
+    return z, z * gamma + beta, gamma, mean, inv
+
+
+def group_norm(x, groups, gamma=None, beta=None, activation=None, gate=None, eps=1e-5):
+    """(y, mean, inv) over x (N, ..., C)."""
+    _, n, _, mean, inv = _normalised(x, groups, gamma, beta, eps)
+    n = n.reshape(x.shape)
+    y = act(n, activation) if gate is None else n * act(np.asarray(gate, np.float64), activation)
+    return y, mean[:, 0, :, 0], inv[:, 0, :, 0]
+
+
+def group_norm_backward(dy, x, groups, gamma=None, beta=None, activation=None, gate=None, eps=1e-5):
+    """(dx, dgamma, dbeta, dgate)."""
+    z, n, g, _, inv = _normalised(x, groups, gamma, beta, eps)
+    dy = np.asarray(dy, np.float64).reshape(z.shape)
+    dgate = None
+    if gate is None:
+        dn = dy * slope(n, activation)
+    else:
+        w = np.asarray(gate, np.float64).reshape(z.shape)
+        dn = dy * act(w, activation)
+        dgate = (dy * n * slope(w, activation)).reshape(x.shape)
+    u = dn * g
+    dx = inv * (u - u.mean((1, 3), keepdims=True) - z * (u * z).mean((1, 3), keepdims=True))
+    return (dx.reshape(x.shape), (dn * z).sum((0, 1)).reshape(-1), dn.sum((0, 1)).reshape(-1),
+            dgate)

@@ -164,6 +164,16 @@ SIGNATURES = {
                         c_void_p, c_i64, c_int, c_i64, c_u32],
     "wxx_beam_reorder": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_int, c_void_p],
     "wxx_beam_append": [c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_i64],
+    "wxx_rotary": [c_void_p, c_void_p, c_i64, c_i64, c_void_p, c_i64, c_i64, c_void_p, c_int,
+                   c_float, c_i64, c_i64, c_i64, c_i64, c_int, c_int],
+    "wxx_linear_attention": [c_void_p, c_void_p] + [c_void_p, c_i64, c_i64] * 3 + [c_void_p] * 3
+                            + [c_i64] * 5 + [c_float],
+    "wxx_linear_attention_backward": [c_void_p] * 6 + [c_void_p, c_i64, c_i64] * 3
+                                     + [c_void_p] * 3 + [c_i64] * 5 + [c_float],
+    "wxx_linear_attention_step": [c_void_p, c_void_p] + [c_void_p, c_i64] * 3 + [c_void_p]
+                                 + [c_i64] * 4 + [c_float],
+    "wxx_group_norm": [c_void_p] * 7 + [c_i64] * 4 + [c_int, c_float],
+    "wxx_group_norm_backward": [c_void_p] * 11 + [c_i64] * 4 + [c_int],
     "wxx_nccl_unique_id": [P_u8],
     "wxx_nccl_init": [P_u8, c_int, c_int],
     "wxx_nccl_allgather": [c_void_p, c_void_p, c_u64],

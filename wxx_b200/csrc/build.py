@@ -38,6 +38,9 @@ SOURCES = [
     "recurrence.cu",
     "distill.cu",
     "select.cu",
+    "rotary.cu",
+    "linear_attention.cu",
+    "group_norm.cu",
     "pool.cu",
     "nccl.cu",
 ]

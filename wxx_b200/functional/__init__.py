@@ -145,6 +145,18 @@ from .recurrence import (  # noqa: E402
     gated_recurrence_backward,
     gated_recurrence_step,
 )
+from .group_norm import group_norm, group_norm_backward  # noqa: E402
+from .linear_attention import (  # noqa: E402
+    linear_attention,
+    linear_attention_backward,
+    linear_attention_step,
+)
+from .rotary import (  # noqa: E402
+    RotaryFrequencies,
+    rotary,
+    rotary_backward,
+    rotary_frequencies,
+)
 from .selection import beam_append, beam_reorder, beam_select, topk  # noqa: E402
 
 
