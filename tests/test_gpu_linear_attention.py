@@ -214,7 +214,11 @@ def test_non_finite_values_stay_where_the_formula_has_them(dk, dv, bad, rng):
         ref = ref.reshape(B, T, H, dv)
         hit = ~np.isfinite(got)
         assert np.array_equal(hit, ~np.isfinite(ref))
-        assert np.array_equal(last, good_last)
+        # the other row and head to the bit; the document behind shares a chunk with the bad
+        # one, which may be added in another order: each within its room of the exact state,
+        # (3 * 2^-22 + (64 + 8 sqrt(1024)) u) of its terms, below 2e-6 of the largest state
+        assert np.array_equal(last[1], good_last[1]) and np.array_equal(last[0, 1], good_last[0, 1])
+        assert np.abs(last - good_last).max() < 2e-6 * np.abs(good_last).max()
         size = np.abs(good).max()
         assert np.abs(np.where(hit, 0, got) - np.where(hit, 0, good)).max() < 2e-6 * size
         if name == "q":

@@ -13,10 +13,18 @@
 // (x, y, z) = (q, k, v) for o; (do, v, k) for dq; and backwards in time (k, q, do) for dv
 // and (v, do, q) for dk: see Pass.
 
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
 #include "common.cuh"
+
+WXX_EXPORT int wxx_malloc(void** out, uint64_t nbytes);
+WXX_EXPORT int wxx_free(void* p);
 
 namespace {
 
@@ -49,12 +57,15 @@ constexpr int kT = 256;
 
 // One position's decay of a state, l X.  A decay near 1 is applied as X + (l - 1) X: l alone
 // is rounded to 2^-25, which n positions in a row make n 2^-25.
+// (An infinite state takes l itself: of the two terms' signs one is the other's opposite.)
 struct Decay {
-  float less, whole;
+  float l, less, whole;
   __device__ explicit Decay(float log_decay)
-      : less(log_decay > -0.5f ? expm1f(log_decay) : expf(log_decay)),
+      : l(expf(log_decay)), less(log_decay > -0.5f ? expm1f(log_decay) : l),
         whole(log_decay > -0.5f ? 1.f : 0.f) {}
-  __device__ __forceinline__ float operator()(float X) const { return fmaf(less, X, whole * X); }
+  __device__ __forceinline__ float operator()(float X) const {
+    return fabsf(X) < INFINITY ? fmaf(less, X, whole * X) : l * X;
+  }
 };
 
 // A block per sequence, head and 32 columns of X: lane = column, warp = every 8th row,
@@ -123,6 +134,752 @@ __global__ void __launch_bounds__(kT) sweep_kernel(const Pass a, const Shape s) 
   }
 }
 
+// ------------------------------------------------------------------ chunks
+//
+// A chunk of 64 positions at a time, so that the work is products of matrices.  With X the
+// state that applies to the chunk's first position (its decay and a reset there already
+// taken), i and j positions of the chunk and l^n powers of the decay, forwards:
+//
+//   out_i = l^i X^T x_i + sum over j <= i of l^(i - j) (x_i . y_j) z_j
+//   X' = l^n X + sum of l^(n - j) y_j z_j^T
+//
+// with every term left out that a reset separates; backwards the same from the chunk's
+// other end.
+//
+// Four products a chunk (x y^T, its result with z, x X, y^T z) of 26.6 thousand operations a
+// position at 64 channels, four times the bytes: on FP32 units (65 TFLOP/s measured) they
+// would take 2.5 times as long as the memory.  They run on the tensor cores in half
+// precision, three products for one: every operand is split into a high and a low half of
+// 11 bits each, hi hi + hi lo + lo hi, which leaves out 2^-22 of a product.  Half numbers
+// reach from 2^-24 to 2^16 only, so each row (a position's vector of x, y or z, a row of the
+// position-by-position matrix) is scaled by a power of two that brings its largest entry
+// to 2^13, and a state by one for all of it; the powers are put back in 32 bits.  Entries
+// far below their row's largest lose accuracy from 2^-20 of it on (they are good to 2^-38
+// of the largest).  (Measured, mma.sync: half 554, tf32 277 TFLOP/s; three products of
+// tf32 need no scaling, but would be bound by that rate.)  The state stays in 32-bit
+// registers, a chunk's products are added to it in 32 bits.
+//
+// NaN and infinities cannot take part: 0 times NaN would carry them to earlier positions
+// and other documents.  A chunk that holds one, or starts from a state that does, is
+// worked through position by position (rare_chunk).
+
+constexpr int kC = 64;                  // positions of a chunk
+constexpr int kThreads = 128;           // 4 warps of 16 positions
+constexpr int kTop = 13;                // a scaled row's largest entry is in [2^13, 2^14)
+
+__device__ __forceinline__ uint32_t smem_address(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void copy16(uint32_t to, const float* from, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from),
+               "r"(take ? 16 : 0));
+}
+__device__ __forceinline__ void copy4(uint32_t to, const float* from, bool take) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from),
+               "r"(take ? 4 : 0));
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ void load4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void load4_turned(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A product to 22 bits: the halves' but that of the two low ones, the small ones first.
+__device__ __forceinline__ void products(float (&c)[4], const uint32_t (&hi)[4],
+                                         const uint32_t (&lo)[4], uint32_t bh0, uint32_t bh1,
+                                         uint32_t bl0, uint32_t bl1) {
+  product(c, lo, bh0, bh1);
+  product(c, hi, bl0, bl1);
+  product(c, hi, bh0, bh1);
+}
+
+// The high and low halves of two numbers.
+__device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+__device__ __forceinline__ uint32_t size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+constexpr uint32_t kInfinite = 0x7f800000u;
+
+// The exponent of a row's largest entry; rows below 2^-100 are scaled as if at 2^-100.
+__device__ __forceinline__ int exponent(uint32_t bits) { return max((int)(bits >> 23) - 127, -100); }
+__device__ __forceinline__ float power2(int e) {            // -126 <= e <= 127
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+// v -> v f 2^e for any e, f about 1: in two steps of one sign, so that nothing is lost on
+// the way.
+struct Scale {
+  float first, then;
+  __device__ Scale(float f, int e) {
+    e = min(max(e, -250), 250);
+    first = f * power2(e / 2);
+    then = power2(e - e / 2);
+  }
+  __device__ __forceinline__ float operator()(float v) const { return v * first * then; }
+};
+
+// Tiles of W half numbers a row for ldmatrix: 16-byte pieces of a row exchanged so that
+// the same piece of 8 rows lies in 8 different sets of banks.
+template <int W>
+__device__ __forceinline__ uint32_t piece(int row, int q) {
+  const int turn = W == 32 ? (row >> 1) & 3 : row & 7;
+  return (uint32_t)(row * W * 2 + ((q ^ turn) << 4));
+}
+// Rows of W floats as copied: the even 16-byte pieces, then the odd ones, so that a lane's 8
+// neighbouring floats are read without conflicts.
+template <int W>
+__device__ __forceinline__ int raw_piece(int row, int q) {
+  const int at = (q >> 1) + (q & 1) * (W / 8);
+  return row * (W / 4) + (W == 32 ? at ^ ((row & 1) << 2) : at);
+}
+
+template <int P, int R>
+struct Layout {
+  static constexpr int kRawY = 0, kRawZ = kRawY + kC * P * 4;
+  static constexpr int kTiles = kRawZ + kC * R * 4;
+  // high halves, then low halves, of y, of y weighted for the state, of z, of the state
+  static constexpr int kY = kTiles, kW = kY + kC * P * 4, kZ = kW + kC * P * 4;
+  static constexpr int kX = kZ + kC * R * 4;
+  static constexpr int kBytes = kX + P * R * 4;
+  static_assert(P * R * 4 <= kX - kTiles, "rare_chunk's state lies in the tiles");
+  // tiles of the state that a warp keeps: rows of 16, columns of 8
+  static constexpr int kRowTiles = P >= 64 ? P / 64 : 1, kColTiles = P >= 64 ? R / 8 : R / 16;
+  static constexpr int kBlocks = P == 32 && R == 32 ? 4 : P <= 64 ? 2 : 1;     // on an SM
+};
+
+struct Segments {           // pieces of a row that are worked on side by side
+  int count, chunks;        // pieces, chunks of a piece
+  float* state;             // (passes, count - 1, B H, p * r): after each piece but the last
+  float* kept;              // (passes, count - 1, B H): what a piece does to the state before it
+};
+
+// The chunk's weights of decay and resets.
+struct Weights {
+  int first, last;          // of the resets after the chunk's first position, 64 and 0: none
+  unsigned long long inner;
+  int n, tail;              // positions; 1 where the state goes on past the chunk's end
+  bool drop;                // a reset there: the next chunk starts from zero
+  __device__ Weights(unsigned long long cuts, int n_, int tail_, bool drop_)
+      : inner(cuts & ~1ull), n(n_), tail(tail_), drop(drop_) {
+    first = inner ? __ffsll((long long)inner) - 1 : 64;
+    last = inner ? 63 - __clzll((long long)inner) : 0;
+  }
+  // exponents of l, -1: no weight
+  __device__ __forceinline__ int reach(int i, bool back) const {     // of the state, at i
+    return back ? (i >= last && i < n ? n - 1 - i : -1) : (i < first && i < n ? i : -1);
+  }
+  __device__ __forceinline__ int added(int j, bool back) const {     // of j, to the state
+    if (drop || j >= n) return -1;
+    return back ? (j < first ? j + 1 : -1) : (j >= last ? n - 1 - j + tail : -1);
+  }
+  __device__ __forceinline__ int kept(bool back) const {
+    return drop || inner ? -1 : n - 1 + (back ? 1 : tail);
+  }
+  __device__ __forceinline__ int document(int i) const {
+    return __popcll(inner & ((2ull << i) - 1));
+  }
+};
+
+// What a block works on, and the parts of shared memory that are not tiles.
+struct Small {
+  uint32_t max_y[kC], max_z[kC];        // bits of the rows' largest entries
+  uint32_t max_x[4];                    // of the state, by warp
+  float weight[kC];                     // 2^(exponents of y_j and z_j) below the largest
+  float power[kC + 1];                  // l^n
+  int document[kC];
+};
+
+// The passes of one launch: sweeps over the same B, T and H whose heads have the same
+// padded sizes.
+struct Passes {
+  Pass at[3];
+};
+
+// Position by position, for a chunk with numbers that are not finite: the state in shared
+// memory, columns over the lanes, rows over kThreads / R groups of threads.
+template <int P, int R, bool STATE>
+__device__ void rare_chunk(float* state, float* sums, const float* raw_y, const float* raw_z,
+                           const Pass& a, const Shape& s, const Weights& w, unsigned long long cuts,
+                           bool next_cut, Decay l, int64_t b, int h, int t0, int slice) {
+  constexpr int kGroups = kThreads / R;
+  const int c = threadIdx.x % R, group = threadIdx.x / R;
+  auto raw = [&](const float* p, int row, int i, auto width) {
+    constexpr int W = decltype(width)::value;
+    return p[raw_piece<W>(row, i >> 2) * 4 + (i & 3)];
+  };
+  for (int k = 0; k < w.n; ++k) {
+    const int i = a.back ? w.n - 1 - k : k;
+    const float z = raw(raw_z, i, c, std::integral_constant<int, R>{});
+    const float* x = a.x.p + b * a.x.bs + (t0 + i) * a.x.ts + (int64_t)h * a.p;
+    const bool on = k < w.n - 1 || a.back || w.tail;       // the state goes on from here
+    const bool cut = k < w.n - 1 ? (a.back ? cuts >> i & 1 : cuts >> (i + 1) & 1)
+                                 : (a.back ? cuts & 1 : next_cut);
+    float sum = 0.f;
+    for (int p = group; p < a.p; p += kGroups) {
+      float now = fmaf(a.y_scale * raw(raw_y, i, p, std::integral_constant<int, P>{}), z,
+                       state[p * R + c]);
+      if (!STATE) sum = fmaf(x[p], now, sum);
+      if (on) now = cut ? 0.f : l(now);
+      state[p * R + c] = now;
+    }
+    if (STATE) continue;
+    sums[threadIdx.x] = sum;
+    __syncthreads();
+    if (group == 0) {
+      for (int g = 1; g < kGroups; ++g) sum += sums[g * R + c];
+      const int r = slice * R + c;
+      if (r < a.r) a.out[((b * s.T + t0 + i) * s.H + h) * a.r + r] = a.out_scale * sum;
+    }
+    __syncthreads();
+  }
+}
+
+// A block: one sequence, head, slice of R columns of z and piece of the row; STATE: only
+// the state after the piece is wanted.
+template <int P, int R, bool STATE>
+__global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
+    chunk_kernel(const __grid_constant__ Passes passes, const Shape s, const Segments g,
+                 const unsigned per_pass) {
+  using L = Layout<P, R>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ Small m;
+  __shared__ float sums[kThreads];
+  const unsigned pass = blockIdx.x / per_pass;
+  const Pass& a = passes.at[pass];
+  unsigned at = blockIdx.x % per_pass;
+  const int slices = (a.r + R - 1) / R, pieces = STATE ? g.count - 1 : g.count;
+  const int slice = at % slices;
+  at /= slices;
+  const int seg = at % pieces;
+  at /= pieces;
+  const int h = at % s.H;
+  const int64_t b = at / s.H, heads = per_pass / (unsigned)(slices * pieces);   // B H
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, t = lane & 3;
+  const bool back = a.back;
+  const Decay l(s.log_decay[h]);
+  for (int i = threadIdx.x; i <= kC; i += kThreads)
+    m.power[i] = i == 0 ? 1.f : expf((float)i * s.log_decay[h]);
+
+  const int chunks = (s.T + kC - 1) / kC;
+  const int c0 = seg * g.chunks, c1 = min(c0 + g.chunks, chunks);
+  // pieces and chunks are counted in the direction of the sweep
+  auto start = [&](int c) { return (back ? chunks - 1 - c : c) * kC; };
+
+  // the state, in the layout of a product's result: rows row0 + 16 mt + quad (+ 8), columns
+  // col0 + 8 nt + 2 t (+ 1)
+  const int row0 = P >= 64 ? warp * (P / 4) : (warp & 1) * 16;
+  const int col0 = P >= 64 ? 0 : (warp >> 1) * (R / 2);
+  float X[L::kRowTiles][L::kColTiles][4];
+  {
+    const int64_t head = (b * s.H + h) * (int64_t)a.p * a.r;
+    const float* from = a.from ? a.from + head : nullptr;
+    bool drop = STATE && seg > 0;
+    int64_t ps = a.p_stride, rs = a.r_stride;
+    if (!STATE && seg > 0) {
+      from = g.state + ((pass * (int64_t)(g.count - 1) + seg - 1) * heads + b * s.H + h) * a.p * a.r;
+      ps = a.r;
+      rs = 1;
+    } else if (STATE) {
+      from = nullptr;
+    } else if (!back) {
+      drop = s.reset && s.reset[b * s.T] != 0;
+    }
+    const bool first = !STATE && seg == 0 && !back;          // its own step of the decay
+#pragma unroll
+    for (int mt = 0; mt < L::kRowTiles; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int p = row0 + mt * 16 + quad + (e >> 1) * 8;
+          const int r = slice * R + col0 + nt * 8 + 2 * t + (e & 1);
+          float v = from && !drop && p < a.p && r < a.r ? from[p * ps + r * rs] : 0.f;
+          X[mt][nt][e] = first ? l(v) : v;
+        }
+  }
+
+  float* raw_y = reinterpret_cast<float*>(smem + L::kRawY);
+  float* raw_z = reinterpret_cast<float*>(smem + L::kRawZ);
+  const uint32_t at_y = smem_address(smem + L::kY), at_w = smem_address(smem + L::kW),
+                 at_z = smem_address(smem + L::kZ), at_x = smem_address(smem + L::kX);
+  // 16-byte copies where every row allows them
+  auto whole = [&](const Operand& o, int width, int from) {
+    return ((reinterpret_cast<uintptr_t>(o.p) & 15) == 0) && ((o.bs | o.ts | width | from) & 3) == 0;
+  };
+  const bool wide_y = whole(a.y, a.p, 0), wide_z = whole(a.z, a.r, 0);
+  auto fetch_rows = [&](auto width, float* raw, const Operand& o, int columns, int from, int t0,
+                        bool wide) {
+    constexpr int W = decltype(width)::value;
+    const int n = min(kC, s.T - t0);
+    const float* p = o.p + b * o.bs + t0 * o.ts + (int64_t)h * columns + from;
+    const int here = columns - from;                      // columns from there on
+    if (wide) {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < kC * (W / 4); i += kThreads) {
+        const int row = i / (W / 4), q = i % (W / 4);
+        const bool take = row < n && q * 4 < here;
+        copy16(smem_address(raw) + raw_piece<W>(row, q) * 16, take ? p + row * o.ts + q * 4 : o.p,
+               take);
+      }
+    } else {
+      for (int i = threadIdx.x; i < kC * W; i += kThreads) {
+        const int row = i / W, col = i % W;
+        const bool take = row < n && col < here;
+        copy4(smem_address(raw) + raw_piece<W>(row, col >> 2) * 16 + (col & 3) * 4,
+              take ? p + row * o.ts + col : o.p, take);
+      }
+    }
+  };
+  auto fetch = [&](int c) {
+    fetch_rows(std::integral_constant<int, P>{}, raw_y, a.y, a.p, 0, start(c), wide_y);
+    fetch_rows(std::integral_constant<int, R>{}, raw_z, a.z, a.r, slice * R, start(c), wide_z);
+  };
+  const bool pairs_x = ((reinterpret_cast<uintptr_t>(a.x.p) & 7) == 0) &&
+                       ((a.x.bs | a.x.ts | a.p) & 1) == 0;
+  const bool pairs_o = ((reinterpret_cast<uintptr_t>(a.out) & 7) == 0) && (a.r & 1) == 0;
+
+  if (c0 < c1) fetch(c0);
+  float run = 1.f;                      // STATE: what the piece does to the state before it
+  auto publish = [&] {                  // the state's largest entry, of this warp
+    uint32_t most = 0;
+#pragma unroll
+    for (int mt = 0; mt < L::kRowTiles; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = max(most, size_bits(X[mt][nt][e]));
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) m.max_x[warp] = most;
+  };
+  publish();
+
+  for (int c = c0; c < c1; ++c) {
+    const int t0 = start(c), n = min(kC, s.T - t0);
+    // the resets of the chunk, and of the position after it
+    unsigned long long cuts = 0;
+    bool next_cut = false;
+    if (s.reset) {
+      const uint32_t* mark = s.reset + b * s.T + t0;
+      const unsigned lo = __ballot_sync(0xffffffffu, lane < n && mark[lane] != 0);
+      const unsigned hi = __ballot_sync(0xffffffffu, lane + 32 < n && mark[lane + 32] != 0);
+      cuts = (unsigned long long)hi << 32 | lo;
+      next_cut = !back && t0 + n < s.T && mark[n] != 0;
+    }
+    const Weights w(cuts, n, t0 + n < s.T, back ? cuts & 1 : next_cut);
+
+    // x of this warp's positions, in the layout of a product's left operand
+    float x[STATE ? 1 : P / 16][8];
+    uint32_t top_x[2] = {0, 0};
+    if (!STATE) {
+      const float* px = a.x.p + b * a.x.bs + t0 * a.x.ts + (int64_t)h * a.p;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int i = warp * 16 + quad + half * 8;
+        const float* row = px + i * a.x.ts;
+#pragma unroll
+        for (int k = 0; k < P / 16; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int col = k * 16 + e * 8 + 2 * t;
+            float2 v = make_float2(0.f, 0.f);
+            if (pairs_x) {
+              if (i < n && col < a.p) v = *reinterpret_cast<const float2*>(row + col);
+            } else {
+              if (i < n && col < a.p) v.x = row[col];
+              if (i < n && col + 1 < a.p) v.y = row[col + 1];
+            }
+            x[k][half * 2 + e * 4] = v.x;
+            x[k][half * 2 + e * 4 + 1] = v.y;
+          }
+      }
+    }
+    copies_done();
+    __syncthreads();       // y and z are here, the last chunk's tiles are read, max_x is known
+
+    uint32_t max_x = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) max_x = max(max_x, m.max_x[i]);
+    const int e_x = exponent(max_x);
+    if (!STATE && max_x < kInfinite && max_x > 0) {
+      const float up = power2(kTop - e_x);
+#pragma unroll
+      for (int mt = 0; mt < L::kRowTiles; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int row = row0 + mt * 16 + quad + half * 8;
+            uint32_t hi, lo;
+            split(up * X[mt][nt][half * 2], up * X[mt][nt][half * 2 + 1], hi, lo);
+            const uint32_t to = L::kX + piece<R>(row, col0 / 8 + nt) + 4 * t;
+            *reinterpret_cast<uint32_t*>(smem + to) = hi;
+            *reinterpret_cast<uint32_t*>(smem + to + P * R * 2) = lo;
+          }
+    }
+    // the rows' largest entries; a lane has 8 neighbouring columns of a row
+    constexpr int kLanesY = P / 8, kPassesY = kLanesY / 2, kLanesZ = R / 8, kPassesZ = kLanesZ / 2;
+    float y[kPassesY][8], z[kPassesZ][8];
+    uint32_t worst = max_x;
+    auto rows = [&](auto width, const float* raw, auto& v, uint32_t* max_row) {
+      constexpr int W = decltype(width)::value, kLanes = W / 8;
+#pragma unroll
+      for (int k = 0; k < kLanes / 2; ++k) {
+        const int row = warp * 16 + k * (32 / kLanes) + lane / kLanes, q = lane % kLanes;
+        const float4 u0 = reinterpret_cast<const float4*>(raw)[raw_piece<W>(row, 2 * q)];
+        const float4 u1 = reinterpret_cast<const float4*>(raw)[raw_piece<W>(row, 2 * q + 1)];
+        v[k][0] = u0.x, v[k][1] = u0.y, v[k][2] = u0.z, v[k][3] = u0.w;
+        v[k][4] = u1.x, v[k][5] = u1.y, v[k][6] = u1.z, v[k][7] = u1.w;
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = max(most, size_bits(v[k][i]));
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1)
+          most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if (q == 0) max_row[row] = most;
+        worst = max(worst, most);
+      }
+    };
+    rows(std::integral_constant<int, P>{}, raw_y, y, m.max_y);
+    rows(std::integral_constant<int, R>{}, raw_z, z, m.max_z);
+    if (!STATE) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int k = 0; k < P / 16; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            top_x[half] = max(top_x[half], max(size_bits(x[k][half * 2 + e * 4]),
+                                               size_bits(x[k][half * 2 + e * 4 + 1])));
+        top_x[half] = max(top_x[half], __shfl_xor_sync(0xffffffffu, top_x[half], 1));
+        top_x[half] = max(top_x[half], __shfl_xor_sync(0xffffffffu, top_x[half], 2));
+        worst = max(worst, top_x[half]);
+      }
+    }
+    if (__syncthreads_or(worst >= kInfinite)) {
+      float* state = reinterpret_cast<float*>(smem + L::kTiles);
+      auto each = [&](auto f) {
+#pragma unroll
+        for (int mt = 0; mt < L::kRowTiles; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              f(X[mt][nt][e], state[(row0 + mt * 16 + quad + (e >> 1) * 8) * R + col0 + nt * 8 +
+                                    2 * t + (e & 1)]);
+      };
+      each([](float& v, float& kept) { kept = v; });
+      __syncthreads();
+      rare_chunk<P, R, STATE>(state, sums, raw_y, raw_z, a, s, w, cuts, next_cut, l, b, h, t0, slice);
+      __syncthreads();
+      each([](float& v, float& kept) { v = kept; });
+      __syncthreads();
+      if (c + 1 < c1) fetch(c + 1);
+    } else {
+      // what the rows weigh: lane looks at rows lane and lane + 32
+      int most = -1000, most_added = -1000;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int j = lane + 32 * k;
+        if (j >= n) continue;
+        const int e = exponent(m.max_y[j]) + exponent(m.max_z[j]), u = w.added(j, back);
+        most = max(most, e);
+        if (u >= 0) most_added = max(most_added, e + exponent(size_bits(m.power[u])));
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      most_added = __reduce_max_sync(0xffffffffu, most_added);
+      if (!STATE && warp < 2) {
+        const int j = threadIdx.x;
+        const int e = exponent(m.max_y[j]) + exponent(m.max_z[j]) - most;
+        m.weight[j] = e < -126 || j >= n ? 0.f : power2(e);
+        m.document[j] = w.document(j);
+      }
+      // the tiles
+#pragma unroll
+      for (int k = 0; k < kPassesY; ++k) {
+        const int row = warp * 16 + k * (32 / kLanesY) + lane / kLanesY, q = lane % kLanesY;
+        const int e = exponent(m.max_y[row]), u = w.added(row, back);
+        const float up = power2(kTop - e);
+        float by = 0.f;
+        if (u >= 0) {
+          const int below = e + exponent(m.max_z[row]) - most_added;
+          by = below < -126 ? 0.f : m.power[u] * power2(min(below, 126));
+        }
+        uint32_t hi[4], lo[4], whi[4], wlo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float u0 = up * y[k][2 * i], u1 = up * y[k][2 * i + 1];
+          if (!STATE) split(u0, u1, hi[i], lo[i]);
+          split(by * u0, by * u1, whi[i], wlo[i]);
+        }
+        const uint32_t to = piece<P>(row, q);
+        if (!STATE) {
+          *reinterpret_cast<uint4*>(smem + L::kY + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(smem + L::kY + kC * P * 2 + to) =
+              make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        *reinterpret_cast<uint4*>(smem + L::kW + to) = make_uint4(whi[0], whi[1], whi[2], whi[3]);
+        *reinterpret_cast<uint4*>(smem + L::kW + kC * P * 2 + to) =
+            make_uint4(wlo[0], wlo[1], wlo[2], wlo[3]);
+      }
+#pragma unroll
+      for (int k = 0; k < kPassesZ; ++k) {
+        const int row = warp * 16 + k * (32 / kLanesZ) + lane / kLanesZ, q = lane % kLanesZ;
+        const float up = power2(kTop - exponent(m.max_z[row]));
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split(up * z[k][2 * i], up * z[k][2 * i + 1], hi[i], lo[i]);
+        const uint32_t to = piece<R>(row, q);
+        *reinterpret_cast<uint4*>(smem + L::kZ + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(smem + L::kZ + kC * R * 2 + to) =
+            make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      __syncthreads();
+      if (c + 1 < c1) fetch(c + 1);
+
+      const int mat = lane >> 3, mat_row = lane & 7;
+      if (!STATE) {
+        int e_row[2];
+        uint32_t xh[P / 16][4], xl[P / 16][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          e_row[half] = exponent(top_x[half]);
+          const float up = power2(kTop - e_row[half]);
+#pragma unroll
+          for (int k = 0; k < P / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              split(up * x[k][half * 2 + e * 4], up * x[k][half * 2 + e * 4 + 1],
+                    xh[k][half + 2 * e], xl[k][half + 2 * e]);
+        }
+        float o[R / 8][4];
+#pragma unroll
+        for (int nt = 0; nt < R / 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
+        if (max_x > 0) {
+#pragma unroll
+          for (int k = 0; k < P / 16; ++k)
+#pragma unroll
+            for (int nb = 0; nb < R / 16; ++nb) {
+              uint32_t bh[4], bl[4];
+              const uint32_t from =
+                  at_x + piece<R>(k * 16 + (mat & 1) * 8 + mat_row, 2 * nb + (mat >> 1));
+              load4_turned(bh, from);
+              load4_turned(bl, from + P * R * 2);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                products(o[2 * nb + e], xh[k], xl[k], bh[2 * e], bh[2 * e + 1], bl[2 * e],
+                         bl[2 * e + 1]);
+              }
+            }
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int u = w.reach(warp * 16 + quad + half * 8, back);
+            const Scale by(u < 0 ? 0.f : m.power[u], e_row[half] + e_x - 2 * kTop);
+#pragma unroll
+            for (int nt = 0; nt < R / 8; ++nt) {
+              o[nt][half * 2] = by(o[nt][half * 2]);
+              o[nt][half * 2 + 1] = by(o[nt][half * 2 + 1]);
+            }
+          }
+        }
+        // x y^T for the positions up to (back: from) this warp's own
+        float S[kC / 8][4];
+#pragma unroll
+        for (int jb = 0; jb < kC / 16; ++jb) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[2 * jb][e] = S[2 * jb + 1][e] = 0.f;
+          if (back ? jb < warp : jb > warp) continue;
+#pragma unroll
+          for (int k = 0; k < P / 16; ++k) {
+            uint32_t bh[4], bl[4];
+            const uint32_t from =
+                at_y + piece<P>(jb * 16 + (mat >> 1) * 8 + mat_row, 2 * k + (mat & 1));
+            load4(bh, from);
+            load4(bl, from + kC * P * 2);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              products(S[2 * jb + e], xh[k], xl[k], bh[2 * e], bh[2 * e + 1], bl[2 * e],
+                       bl[2 * e + 1]);
+            }
+          }
+        }
+        // its weights, and the rows' scales
+        uint32_t most_p[2] = {0, 0};
+#pragma unroll
+        for (int jt = 0; jt < kC / 8; ++jt) {
+          if (back ? jt / 2 < warp : jt / 2 > warp) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = warp * 16 + quad + (e >> 1) * 8, j = jt * 8 + 2 * t + (e & 1);
+            const int apart = back ? j - i : i - j;
+            float v = apart < 0 ? 0.f : S[jt][e] * (m.power[max(apart, 0)] * m.weight[j]);
+            if (w.inner && m.document[i] != m.document[j]) v = 0.f;
+            S[jt][e] = v;
+            most_p[e >> 1] = max(most_p[e >> 1], size_bits(v));
+          }
+        }
+        int e_p[2];
+        float up[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          most_p[half] = max(most_p[half], __shfl_xor_sync(0xffffffffu, most_p[half], 1));
+          most_p[half] = max(most_p[half], __shfl_xor_sync(0xffffffffu, most_p[half], 2));
+          e_p[half] = exponent(most_p[half]);
+          up[half] = power2(kTop - e_p[half]);
+        }
+        float v[R / 8][4];
+#pragma unroll
+        for (int nt = 0; nt < R / 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[nt][e] = 0.f;
+#pragma unroll
+        for (int jb = 0; jb < kC / 16; ++jb) {
+          if (back ? jb < warp : jb > warp) continue;
+          uint32_t ph[4], pl[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = up[e & 1];
+            split(f * S[2 * jb + (e >> 1)][(e & 1) * 2], f * S[2 * jb + (e >> 1)][(e & 1) * 2 + 1],
+                  ph[e], pl[e]);
+          }
+#pragma unroll
+          for (int nb = 0; nb < R / 16; ++nb) {
+            uint32_t bh[4], bl[4];
+            const uint32_t from =
+                at_z + piece<R>(jb * 16 + (mat & 1) * 8 + mat_row, 2 * nb + (mat >> 1));
+            load4_turned(bh, from);
+            load4_turned(bl, from + kC * R * 2);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              products(v[2 * nb + e], ph, pl, bh[2 * e], bh[2 * e + 1], bl[2 * e], bl[2 * e + 1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int i = warp * 16 + quad + half * 8;
+          const Scale by(a.y_scale, e_row[half] + e_p[half] + most - 4 * kTop);
+          float* out = a.out + ((b * s.T + t0 + i) * s.H + h) * a.r + slice * R;
+#pragma unroll
+          for (int nt = 0; nt < R / 8; ++nt) {
+            const int r = nt * 8 + 2 * t, room = a.r - slice * R;
+            const float v0 = a.out_scale * (by(v[nt][half * 2]) + o[nt][half * 2]);
+            const float v1 = a.out_scale * (by(v[nt][half * 2 + 1]) + o[nt][half * 2 + 1]);
+            if (i >= n) continue;
+            if (pairs_o) {
+              if (r < room) *reinterpret_cast<float2*>(out + r) = make_float2(v0, v1);
+            } else {
+              if (r < room) out[r] = v0;
+              if (r + 1 < room) out[r + 1] = v1;
+            }
+          }
+        }
+      }
+      // the state: its chunk's products, then in 32 bits
+      const Scale by(a.y_scale, most_added - 2 * kTop);
+      const int u = w.kept(back);
+      const float kept = u < 0 ? 0.f : m.power[u];
+#pragma unroll
+      for (int mt = 0; mt < L::kRowTiles; ++mt) {
+        float d[L::kColTiles][4];
+#pragma unroll
+        for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < kC / 16; ++k) {
+          uint32_t ah[4], al[4];
+          const uint32_t from = at_w + piece<P>(k * 16 + (mat >> 1) * 8 + mat_row,
+                                                (row0 + mt * 16) / 8 + (mat & 1));
+          load4_turned(ah, from);
+          load4_turned(al, from + kC * P * 2);
+#pragma unroll
+          for (int nb = 0; nb < L::kColTiles / 2; ++nb) {
+            uint32_t bh[4], bl[4];
+            const uint32_t zat = at_z + piece<R>(k * 16 + (mat & 1) * 8 + mat_row,
+                                                 col0 / 8 + 2 * nb + (mat >> 1));
+            load4_turned(bh, zat);
+            load4_turned(bl, zat + kC * R * 2);
+            products(d[2 * nb], ah, al, bh[0], bh[1], bl[0], bl[1]);
+            products(d[2 * nb + 1], ah, al, bh[2], bh[3], bl[2], bl[3]);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) X[mt][nt][e] = fmaf(kept, X[mt][nt][e], by(d[nt][e]));
+      }
+    }
+    if (STATE) {
+      const int u = w.kept(back);
+      run *= u < 0 ? 0.f : m.power[u];
+    }
+    publish();
+  }
+
+  const bool keep = STATE || (a.last && seg == pieces - 1);
+  float* to = STATE ? g.state + ((pass * (int64_t)pieces + seg) * heads + b * s.H + h) * a.p * a.r
+                    : a.last + (b * s.H + h) * (int64_t)a.p * a.r;
+  const int64_t ps = STATE ? a.r : a.p_stride, rs = STATE ? 1 : a.r_stride;
+#pragma unroll
+  for (int mt = 0; mt < L::kRowTiles; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int p = row0 + mt * 16 + quad + (e >> 1) * 8;
+        const int r = slice * R + col0 + nt * 8 + 2 * t + (e & 1);
+        if (keep && p < a.p && r < a.r) to[p * ps + r * rs] = X[mt][nt][e];
+      }
+  if (STATE && threadIdx.x == 0)
+    g.kept[(pass * (int64_t)pieces + seg) * heads + b * s.H + h] = run;
+}
+
+// The states before the pieces, from what each piece adds to a state and keeps of it, in
+// place: a thread an entry, one piece after the other.
+__global__ void __launch_bounds__(kT)
+    join_kernel(const __grid_constant__ Passes passes, const Shape s, const Segments g,
+                const int64_t heads, const int64_t total) {
+  const int64_t i = (int64_t)blockIdx.x * kT + threadIdx.x;
+  if (i >= total) return;
+  const int pass = blockIdx.y;
+  const Pass& a = passes.at[pass];
+  const int64_t size = (int64_t)a.p * a.r, head = i / size;
+  const int p = (int)(i % size) / a.r, r = (int)(i % size) % a.r;
+  const int64_t b = head / s.H;
+  float X = a.from ? a.from[head * size + p * a.p_stride + r * a.r_stride] : 0.f;
+  if (!a.back)
+    X = s.reset && s.reset[b * s.T] != 0 ? 0.f : Decay(s.log_decay[head % s.H])(X);
+  for (int k = 0; k < g.count - 1; ++k) {
+    float* E = g.state + (pass * (int64_t)(g.count - 1) + k) * total + i;
+    const float kept = g.kept[(pass * (int64_t)(g.count - 1) + k) * heads + head];
+    X = kept == 0.f ? *E : fmaf(kept, X, *E);
+    *E = X;
+  }
+}
+
 // One position a sequence: a block per sequence, head and 32 columns of the state.
 __global__ void __launch_bounds__(kT)
     step_kernel(float* __restrict__ o, float* __restrict__ state, const float* __restrict__ q,
@@ -164,16 +921,102 @@ int check_sizes(const char* what, int64_t B, int64_t T, int64_t H, int64_t dk, i
 }
 
 int sweep(const Pass& a, const Shape& s, int64_t B) {
-  const unsigned grid = (unsigned)(B * s.H * ((a.r + 31) / 32));
-  if (a.p <= 32)
-    sweep_kernel<4><<<grid, kT, 0, wxx::stream()>>>(a, s);
-  else if (a.p <= 64)
-    sweep_kernel<8><<<grid, kT, 0, wxx::stream()>>>(a, s);
-  else if (a.p <= 128)
-    sweep_kernel<16><<<grid, kT, 0, wxx::stream()>>>(a, s);
-  else
-    sweep_kernel<32><<<grid, kT, 0, wxx::stream()>>>(a, s);
+  sweep_kernel<32><<<(unsigned)(B * s.H * ((a.r + 31) / 32)), kT, 0, wxx::stream()>>>(a, s);
   return wxx::after_launch(__FILE__, __LINE__);
+}
+
+// Room for a kernel's tiles, asked for once for each.
+template <class K>
+int allow_smem(K kernel, int bytes) {
+  static std::mutex lock;
+  static K done[16] = {};           // kernels of this type that have it
+  std::lock_guard<std::mutex> hold(lock);
+  for (K& k : done) {
+    if (k == kernel) return WXX_OK;
+    if (k) continue;
+    WXX_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    k = kernel;
+    return WXX_OK;
+  }
+  return WXX_OK;
+}
+
+// n passes of one padded size in one launch, the rows in pieces where there are too few
+// sequences and heads to fill the SMs: first what every piece but the last adds to a state,
+// then the states before the pieces, then the outputs.
+template <int P, int R>
+int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
+  using L = Layout<P, R>;
+  const Pass& a = passes.at[0];
+  int slices = 0;
+  for (int i = 0; i < n; ++i) slices = std::max(slices, (passes.at[i].r + R - 1) / R);
+  const int64_t heads = B * s.H, blocks = heads * slices, chunks = (s.T + kC - 1) / kC;
+  const int64_t resident = (int64_t)wxx::num_sms() * L::kBlocks;
+  Segments g{1, (int)chunks, nullptr, nullptr};
+  if (blocks * n < resident) {
+    int64_t size = (chunks * blocks * n + resident - 1) / resident;
+    if (size < 4) size = 4;
+    g.count = (int)((chunks + size - 1) / size);
+    g.chunks = (int)size;
+  }
+  if (int st = allow_smem(chunk_kernel<P, R, true>, L::kBytes)) return st;
+  if (int st = allow_smem(chunk_kernel<P, R, false>, L::kBytes)) return st;
+  void* scratch = nullptr;
+  if (g.count > 1) {
+    const int64_t states = n * (g.count - 1) * heads;
+    if (int st = wxx_malloc(&scratch, (uint64_t)(states * (a.p * a.r + 1)) * sizeof(float)))
+      return st;
+    g.state = static_cast<float*>(scratch);
+    g.kept = g.state + states * a.p * a.r;
+    const unsigned per = (unsigned)(blocks * (g.count - 1));
+    chunk_kernel<P, R, true><<<per * n, kThreads, L::kBytes, wxx::stream()>>>(passes, s, g, per);
+    int st = wxx::after_launch(__FILE__, __LINE__);
+    if (st == WXX_OK) {
+      const int64_t total = heads * a.p * a.r;
+      join_kernel<<<dim3((unsigned)((total + kT - 1) / kT), n), kT, 0, wxx::stream()>>>(
+          passes, s, g, heads, total);
+      st = wxx::after_launch(__FILE__, __LINE__);
+    }
+    if (st != WXX_OK) {
+      wxx_free(scratch);
+      return st;
+    }
+  }
+  const unsigned per = (unsigned)(blocks * g.count);
+  chunk_kernel<P, R, false><<<per * n, kThreads, L::kBytes, wxx::stream()>>>(passes, s, g, per);
+  const int st = wxx::after_launch(__FILE__, __LINE__);
+  if (scratch) wxx_free(scratch);
+  return st;
+}
+
+int padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+// Passes of the same sizes side by side.
+int run_passes(const Pass* a, int n, const Shape& s, int64_t B) {
+  for (int i = 0; i < n;) {
+    const int P = padded(a[i].p), R = a[i].r <= 32 ? 32 : 64;
+    Passes same;
+    int k = 0;
+    for (; i < n && k < 3; ++i, ++k) {
+      if (padded(a[i].p) != P || (a[i].r <= 32 ? 32 : 64) != R ||
+          (a[i].r + 63) / 64 != (a[i - k].r + 63) / 64)
+        break;
+      same.at[k] = a[i];
+    }
+    int st;
+    if (P == 256) {
+      st = WXX_OK;
+      for (int j = 0; j < k && st == WXX_OK; ++j) st = sweep(same.at[j], s, B);
+    } else if (R == 32) {
+      st = P == 32 ? chunked<32, 32>(same, k, s, B) : P == 64 ? chunked<64, 32>(same, k, s, B)
+                                                              : chunked<128, 32>(same, k, s, B);
+    } else {
+      st = P == 32 ? chunked<32, 64>(same, k, s, B) : P == 64 ? chunked<64, 64>(same, k, s, B)
+                                                              : chunked<128, 64>(same, k, s, B);
+    }
+    if (st != WXX_OK) return st;
+  }
+  return WXX_OK;
 }
 
 int copy_state(float* to, const float* from, int64_t n) {
@@ -206,7 +1049,7 @@ WXX_EXPORT int wxx_linear_attention(float* o, float* last, const float* q, int64
   const Shape s{log_decay, reset, (int)T, (int)H};
   const Pass a{{q, q_bs, q_ts}, {k, k_bs, k_ts}, {v, v_bs, v_ts}, o, h0, last, dv, 1,
                (int)dk, (int)dv, 1.f, scale, 0};
-  return sweep(a, s, B);
+  return run_passes(&a, 1, s, B);
 }
 
 // dq, dk_out, dv_out (like q, k, v, dense) and dh0 (NULL: not wanted) from d_o, the
@@ -233,9 +1076,7 @@ WXX_EXPORT int wxx_linear_attention_backward(
       {od, ov, ok, dq, h0, nullptr, 1, dv, V, K, 1.f, scale, 0},
       {ok, oq, od, dv_out, dlast, dh0, dv, 1, K, V, scale, 1.f, 1},
       {ov, od, oq, dk_out, dlast, nullptr, 1, dv, V, K, scale, 1.f, 1}};
-  for (const Pass& a : passes)
-    if (int st = sweep(a, s, B)) return st;
-  return WXX_OK;
+  return run_passes(passes, 3, s, B);
 }
 
 // One position a sequence, in place: state (B, H, dk, dv) <- l state + k v^T, o (B, H dv) =
