@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kT) sweep_kernel(const Pass a, const Shape s) 
 // worked through position by position (rare_chunk).
 
 constexpr int kC = 64;                  // positions of a chunk
-constexpr int kThreads = 128;           // 4 warps of 16 positions
+constexpr int kThreads = 256;           // 8 warps: 4 groups of 16 positions by 2 halves
 constexpr int kTop = 13;                // a scaled row's largest entry is in [2^13, 2^14)
 
 __device__ __forceinline__ uint32_t smem_address(const void* p) {
@@ -179,6 +179,9 @@ __device__ __forceinline__ void copy4(uint32_t to, const float* from, bool take)
                "r"(take ? 4 : 0));
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void pair_barrier(int group) {      // the two warps of a group
+  asm volatile("bar.sync %0, 64;" ::"r"(group + 1) : "memory");
+}
 
 __device__ __forceinline__ void load4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -194,20 +197,23 @@ __device__ __forceinline__ void load4_turned(uint32_t (&r)[4], uint32_t at) {
 }
 __device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A product to 22 bits: the halves' but that of the two low ones, the small ones first.
-__device__ __forceinline__ void products(float (&c)[4], const uint32_t (&hi)[4],
-                                         const uint32_t (&lo)[4], uint32_t bh0, uint32_t bh1,
-                                         uint32_t bl0, uint32_t bl1) {
-  product(c, lo, bh0, bh1);
-  product(c, hi, bl0, bl1);
-  product(c, hi, bh0, bh1);
+// Products to 22 bits of a left operand with two right ones next to each other: the halves'
+// but that of the two low ones, the small ones first.
+__device__ __forceinline__ void products(float (&c0)[4], float (&c1)[4], const uint32_t (&hi)[4],
+                                         const uint32_t (&lo)[4], const uint32_t (&bh)[4],
+                                         const uint32_t (&bl)[4]) {
+  product(c0, lo, bh[0], bh[1]);
+  product(c1, lo, bh[2], bh[3]);
+  product(c0, hi, bl[0], bl[1]);
+  product(c1, hi, bl[2], bl[3]);
+  product(c0, hi, bh[0], bh[1]);
+  product(c1, hi, bh[2], bh[3]);
 }
 
 // The high and low halves of two numbers.
@@ -218,12 +224,16 @@ __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& 
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
-
-__device__ __forceinline__ uint32_t size_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-constexpr uint32_t kInfinite = 0x7f800000u;
+__device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {      // two halves each
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 
 // The exponent of a row's largest entry; rows below 2^-100 are scaled as if at 2^-100.
-__device__ __forceinline__ int exponent(uint32_t bits) { return max((int)(bits >> 23) - 127, -100); }
+__device__ __forceinline__ int exponent(float size) {
+  return max((int)(__float_as_uint(size) >> 23) - 127, -100);
+}
 __device__ __forceinline__ float power2(int e) {            // -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
@@ -258,14 +268,22 @@ template <int P, int R>
 struct Layout {
   static constexpr int kRawY = 0, kRawZ = kRawY + kC * P * 4;
   static constexpr int kTiles = kRawZ + kC * R * 4;
-  // high halves, then low halves, of y, of y weighted for the state, of z, of the state
-  static constexpr int kY = kTiles, kW = kY + kC * P * 4, kZ = kW + kC * P * 4;
-  static constexpr int kX = kZ + kC * R * 4;
-  static constexpr int kBytes = kX + P * R * 4;
-  static_assert(P * R * 4 <= kX - kTiles, "rare_chunk's state lies in the tiles");
-  // tiles of the state that a warp keeps: rows of 16, columns of 8
-  static constexpr int kRowTiles = P >= 64 ? P / 64 : 1, kColTiles = P >= 64 ? R / 8 : R / 16;
-  static constexpr int kBlocks = P == 32 && R == 32 ? 4 : P <= 64 ? 2 : 1;     // on an SM
+  // high halves, then low halves, of x, y, z and the state
+  static constexpr int kX = kTiles, kY = kX + kC * P * 4, kZ = kY + kC * P * 4;
+  static constexpr int kState = kZ + kC * R * 4;
+  static constexpr int kEnd = kState + P * R * 4;
+  // where the two halves of a group exchange their sums: x's tile of these positions, which
+  // both have read by then, where it is large enough
+  static constexpr bool kShared = P >= R;
+  static constexpr int kSums = kShared ? kX : kEnd, kGroup = kShared ? 16 * P * 2 : 16 * R * 4;
+  static constexpr int kHalf = kShared ? kC * P * 2 : 16 * R * 2;
+  static constexpr int kBytes = kShared ? kEnd : kEnd + 8 * 16 * R * 2;
+  static_assert(P * R * 4 <= kState - kTiles, "rare_chunk's state lies in the tiles");
+  // the warps' parts of the state: 16 rows by kColTiles tiles of 8 columns
+  static constexpr int kRowGroups = P / 16 < 8 ? P / 16 : 8;
+  static constexpr int kColGroups = 8 / kRowGroups > R / 16 ? R / 16 : 8 / kRowGroups;
+  static constexpr int kColTiles = R / 8 / kColGroups;
+  static constexpr int kBlocks = P == 128 ? 1 : P == 32 && R == 32 ? 3 : 2;    // on an SM
 };
 
 struct Segments {           // pieces of a row that are worked on side by side
@@ -276,8 +294,8 @@ struct Segments {           // pieces of a row that are worked on side by side
 
 // The chunk's weights of decay and resets.
 struct Weights {
-  int first, last;          // of the resets after the chunk's first position, 64 and 0: none
-  unsigned long long inner;
+  unsigned long long inner; // the resets after the chunk's first position
+  int first, last;          // of these; 64 and 0: none
   int n, tail;              // positions; 1 where the state goes on past the chunk's end
   bool drop;                // a reset there: the next chunk starts from zero
   __device__ Weights(unsigned long long cuts, int n_, int tail_, bool drop_)
@@ -301,11 +319,27 @@ struct Weights {
   }
 };
 
-// What a block works on, and the parts of shared memory that are not tiles.
-struct Small {
-  uint32_t max_y[kC], max_z[kC];        // bits of the rows' largest entries
-  uint32_t max_x[4];                    // of the state, by warp
-  float weight[kC];                     // 2^(exponents of y_j and z_j) below the largest
+// A weight of the state, l^u, as rest 2^e with rest in [1, 2); below 2^-126 there is none.
+struct Decayed {
+  bool any;
+  int e;
+  float rest;
+  __device__ Decayed(const float* power, int u) {
+    const uint32_t bits = u < 0 ? 0u : __float_as_uint(power[u]);
+    any = bits >= 0x00800000u;
+    e = any ? (int)(bits >> 23) - 127 : 0;
+    rest = any ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : 1.f;
+  }
+};
+
+// The parts of shared memory that are not tiles.
+struct alignas(16) Small {
+  float max_x[kC], max_y[kC], max_z[kC];    // the rows' largest entries
+  float max_state[8];                   // of the state, by warp
+  // per position j: 2^(exponents of y_j and z_j, below the largest) / what z_j's scale has more,
+  // and that times l^(15 - j % 16) (back: l^(j % 16))
+  float2 weight[kC];
+  uint16_t added[2][kC];                // j's weight in the state, as a product of two halves
   float power[kC + 1];                  // l^n
   int document[kC];
 };
@@ -319,26 +353,22 @@ struct Passes {
 // Position by position, for a chunk with numbers that are not finite: the state in shared
 // memory, columns over the lanes, rows over kThreads / R groups of threads.
 template <int P, int R, bool STATE>
-__device__ void rare_chunk(float* state, float* sums, const float* raw_y, const float* raw_z,
-                           const Pass& a, const Shape& s, const Weights& w, unsigned long long cuts,
-                           bool next_cut, Decay l, int64_t b, int h, int t0, int slice) {
+__device__ void rare_chunk(float* state, float* sums, const Pass& a, const Shape& s,
+                           const Weights& w, unsigned long long cuts, bool next_cut, Decay l,
+                           int64_t b, int h, int t0, int slice) {
   constexpr int kGroups = kThreads / R;
-  const int c = threadIdx.x % R, group = threadIdx.x / R;
-  auto raw = [&](const float* p, int row, int i, auto width) {
-    constexpr int W = decltype(width)::value;
-    return p[raw_piece<W>(row, i >> 2) * 4 + (i & 3)];
-  };
+  const int c = threadIdx.x % R, group = threadIdx.x / R, r = slice * R + c;
   for (int k = 0; k < w.n; ++k) {
     const int i = a.back ? w.n - 1 - k : k;
-    const float z = raw(raw_z, i, c, std::integral_constant<int, R>{});
     const float* x = a.x.p + b * a.x.bs + (t0 + i) * a.x.ts + (int64_t)h * a.p;
+    const float* y = a.y.p + b * a.y.bs + (t0 + i) * a.y.ts + (int64_t)h * a.p;
+    const float z = r < a.r ? a.z.p[b * a.z.bs + (t0 + i) * a.z.ts + (int64_t)h * a.r + r] : 0.f;
     const bool on = k < w.n - 1 || a.back || w.tail;       // the state goes on from here
     const bool cut = k < w.n - 1 ? (a.back ? cuts >> i & 1 : cuts >> (i + 1) & 1)
                                  : (a.back ? cuts & 1 : next_cut);
     float sum = 0.f;
     for (int p = group; p < a.p; p += kGroups) {
-      float now = fmaf(a.y_scale * raw(raw_y, i, p, std::integral_constant<int, P>{}), z,
-                       state[p * R + c]);
+      float now = fmaf(a.y_scale * y[p], z, state[p * R + c]);
       if (!STATE) sum = fmaf(x[p], now, sum);
       if (on) now = cut ? 0.f : l(now);
       state[p * R + c] = now;
@@ -348,7 +378,6 @@ __device__ void rare_chunk(float* state, float* sums, const float* raw_y, const 
     __syncthreads();
     if (group == 0) {
       for (int g = 1; g < kGroups; ++g) sum += sums[g * R + c];
-      const int r = slice * R + c;
       if (r < a.r) a.out[((b * s.T + t0 + i) * s.H + h) * a.r + r] = a.out_scale * sum;
     }
     __syncthreads();
@@ -356,7 +385,10 @@ __device__ void rare_chunk(float* state, float* sums, const float* raw_y, const 
 }
 
 // A block: one sequence, head, slice of R columns of z and piece of the row; STATE: only
-// the state after the piece is wanted.
+// the state after the piece is wanted.  Warps w and w + 4 have the same 16 positions: each
+// takes every other 16 positions of y and z and half of the state's rows, and they add
+// their sums at the end (so no warp has more than two of the four position blocks, and the
+// operands' registers are few enough for two blocks on an SM).
 template <int P, int R, bool STATE>
 __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
     chunk_kernel(const __grid_constant__ Passes passes, const Shape s, const Segments g,
@@ -364,7 +396,6 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
   using L = Layout<P, R>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Small m;
-  __shared__ float sums[kThreads];
   const unsigned pass = blockIdx.x / per_pass;
   const Pass& a = passes.at[pass];
   unsigned at = blockIdx.x % per_pass;
@@ -376,6 +407,8 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
   const int h = at % s.H;
   const int64_t b = at / s.H, heads = per_pass / (unsigned)(slices * pieces);   // B H
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, t = lane & 3;
+  const int group = warp & 3, half = warp >> 2;
+  const int mat = lane >> 3, mat_row = lane & 7;
   const bool back = a.back;
   const Decay l(s.log_decay[h]);
   for (int i = threadIdx.x; i <= kC; i += kThreads)
@@ -385,49 +418,61 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
   const int c0 = seg * g.chunks, c1 = min(c0 + g.chunks, chunks);
   // pieces and chunks are counted in the direction of the sweep
   auto start = [&](int c) { return (back ? chunks - 1 - c : c) * kC; };
+  const uint32_t* marks = s.reset ? s.reset + b * s.T : nullptr;
+  auto resets = [&](int c, bool& next) {
+    const int t0 = start(c), n = min(kC, s.T - t0);
+    next = false;
+    if (!marks) return 0ull;
+    const unsigned lo = __ballot_sync(0xffffffffu, lane < n && marks[t0 + lane] != 0);
+    const unsigned hi = __ballot_sync(0xffffffffu, lane + 32 < n && marks[t0 + lane + 32] != 0);
+    next = !back && t0 + n < s.T && marks[t0 + n] != 0;
+    return (unsigned long long)hi << 32 | lo;
+  };
+  auto weights = [&](int c, unsigned long long cuts, bool next) {
+    const int t0 = start(c), n = min(kC, s.T - t0);
+    return Weights(cuts, n, t0 + n < s.T, back ? cuts & 1 : next);
+  };
 
-  // the state, in the layout of a product's result: rows row0 + 16 mt + quad (+ 8), columns
-  // col0 + 8 nt + 2 t (+ 1)
-  const int row0 = P >= 64 ? warp * (P / 4) : (warp & 1) * 16;
-  const int col0 = P >= 64 ? 0 : (warp >> 1) * (R / 2);
-  float X[L::kRowTiles][L::kColTiles][4];
+  // the state, in the layout of a product's result: rows row0 + quad (+ 8), columns col0 + 8 nt
+  // + 2 t (+ 1); warps without a part keep zeros
+  const int row0 = (warp % L::kRowGroups) * 16;
+  const bool has_state = warp / L::kRowGroups < L::kColGroups;
+  const int col0 = has_state ? warp / L::kRowGroups * L::kColTiles * 8 : 0;
+  float X[L::kColTiles][4], d[L::kColTiles][4];
   {
     const int64_t head = (b * s.H + h) * (int64_t)a.p * a.r;
     const float* from = a.from ? a.from + head : nullptr;
-    bool drop = STATE && seg > 0;
     int64_t ps = a.p_stride, rs = a.r_stride;
-    if (!STATE && seg > 0) {
+    bool drop = !has_state;
+    if (STATE) {
+      from = nullptr;
+    } else if (seg > 0) {
       from = g.state + ((pass * (int64_t)(g.count - 1) + seg - 1) * heads + b * s.H + h) * a.p * a.r;
       ps = a.r;
       rs = 1;
-    } else if (STATE) {
-      from = nullptr;
     } else if (!back) {
-      drop = s.reset && s.reset[b * s.T] != 0;
+      drop = drop || (marks && marks[0] != 0);
     }
     const bool first = !STATE && seg == 0 && !back;          // its own step of the decay
 #pragma unroll
-    for (int mt = 0; mt < L::kRowTiles; ++mt)
+    for (int nt = 0; nt < L::kColTiles; ++nt)
 #pragma unroll
-      for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int p = row0 + mt * 16 + quad + (e >> 1) * 8;
-          const int r = slice * R + col0 + nt * 8 + 2 * t + (e & 1);
-          float v = from && !drop && p < a.p && r < a.r ? from[p * ps + r * rs] : 0.f;
-          X[mt][nt][e] = first ? l(v) : v;
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int p = row0 + quad + (e >> 1) * 8, r = slice * R + col0 + nt * 8 + 2 * t + (e & 1);
+        const float v = from && !drop && p < a.p && r < a.r ? from[p * ps + r * rs] : 0.f;
+        X[nt][e] = first ? l(v) : v;
+        d[nt][e] = 0.f;
+      }
   }
 
   float* raw_y = reinterpret_cast<float*>(smem + L::kRawY);
   float* raw_z = reinterpret_cast<float*>(smem + L::kRawZ);
-  const uint32_t at_y = smem_address(smem + L::kY), at_w = smem_address(smem + L::kW),
-                 at_z = smem_address(smem + L::kZ), at_x = smem_address(smem + L::kX);
-  // 16-byte copies where every row allows them
-  auto whole = [&](const Operand& o, int width, int from) {
-    return ((reinterpret_cast<uintptr_t>(o.p) & 15) == 0) && ((o.bs | o.ts | width | from) & 3) == 0;
+  const uint32_t base = smem_address(smem);
+  // 16-byte accesses where every row allows them
+  auto whole = [&](const Operand& o, int width) {
+    return ((reinterpret_cast<uintptr_t>(o.p) & 15) == 0) && ((o.bs | o.ts | width) & 3) == 0;
   };
-  const bool wide_y = whole(a.y, a.p, 0), wide_z = whole(a.z, a.r, 0);
+  const bool wide_x = !STATE && whole(a.x, a.p), wide_y = whole(a.y, a.p), wide_z = whole(a.z, a.r);
   auto fetch_rows = [&](auto width, float* raw, const Operand& o, int columns, int from, int t0,
                         bool wide) {
     constexpr int W = decltype(width)::value;
@@ -435,9 +480,9 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
     const float* p = o.p + b * o.bs + t0 * o.ts + (int64_t)h * columns + from;
     const int here = columns - from;                      // columns from there on
     if (wide) {
-#pragma unroll 4
-      for (int i = threadIdx.x; i < kC * (W / 4); i += kThreads) {
-        const int row = i / (W / 4), q = i % (W / 4);
+#pragma unroll
+      for (int k = 0; k < kC * (W / 4) / kThreads; ++k) {
+        const int i = threadIdx.x + k * kThreads, row = i / (W / 4), q = i % (W / 4);
         const bool take = row < n && q * 4 < here;
         copy16(smem_address(raw) + raw_piece<W>(row, q) * 16, take ? p + row * o.ts + q * 4 : o.p,
                take);
@@ -455,338 +500,368 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
     fetch_rows(std::integral_constant<int, P>{}, raw_y, a.y, a.p, 0, start(c), wide_y);
     fetch_rows(std::integral_constant<int, R>{}, raw_z, a.z, a.r, slice * R, start(c), wide_z);
   };
-  const bool pairs_x = ((reinterpret_cast<uintptr_t>(a.x.p) & 7) == 0) &&
-                       ((a.x.bs | a.x.ts | a.p) & 1) == 0;
+  // A lane's share of x, y and z: 8 neighbouring columns of a row, W / 32 rows in turn of the
+  // warp's 8.
+  auto row_of = [&](int W, int k) { return warp * 8 + k * (256 / W) + lane / (W / 8); };
+  constexpr int kPassesX = P / 32, kPassesZ = R / 32;
+  float x[STATE ? 1 : kPassesX][8];
+  auto fetch_x = [&](int c) {
+    const int t0 = start(c), n = min(kC, s.T - t0), col = lane % (P / 8) * 8;
+#pragma unroll
+    for (int k = 0; k < kPassesX; ++k) {
+      const int row = row_of(P, k);
+      const float* p = a.x.p + b * a.x.bs + (t0 + row) * a.x.ts + (int64_t)h * a.p + col;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[k][e] = 0.f;
+      if (row < n) {
+        if (wide_x) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            if (col + 4 * q >= a.p) continue;
+            const float4 v = *reinterpret_cast<const float4*>(p + 4 * q);
+            x[k][4 * q] = v.x, x[k][4 * q + 1] = v.y, x[k][4 * q + 2] = v.z, x[k][4 * q + 3] = v.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + e < a.p) x[k][e] = p[e];
+        }
+      }
+    }
+  };
   const bool pairs_o = ((reinterpret_cast<uintptr_t>(a.out) & 7) == 0) && (a.r & 1) == 0;
 
-  if (c0 < c1) fetch(c0);
+  fetch(c0);
+  if constexpr (!STATE) fetch_x(c0);
   float run = 1.f;                      // STATE: what the piece does to the state before it
-  auto publish = [&] {                  // the state's largest entry, of this warp
-    uint32_t most = 0;
-#pragma unroll
-    for (int mt = 0; mt < L::kRowTiles; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) most = max(most, size_bits(X[mt][nt][e]));
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) m.max_x[warp] = most;
-  };
-  publish();
+  float kept = 1.f, odd = 0.f;          // of the last chunk; odd: 0 unless something is not finite
+  Scale by_d(0.f, 0);
 
-  for (int c = c0; c < c1; ++c) {
-    const int t0 = start(c), n = min(kC, s.T - t0);
-    // the resets of the chunk, and of the position after it
-    unsigned long long cuts = 0;
-    bool next_cut = false;
-    if (s.reset) {
-      const uint32_t* mark = s.reset + b * s.T + t0;
-      const unsigned lo = __ballot_sync(0xffffffffu, lane < n && mark[lane] != 0);
-      const unsigned hi = __ballot_sync(0xffffffffu, lane + 32 < n && mark[lane + 32] != 0);
-      cuts = (unsigned long long)hi << 32 | lo;
-      next_cut = !back && t0 + n < s.T && mark[n] != 0;
-    }
-    const Weights w(cuts, n, t0 + n < s.T, back ? cuts & 1 : next_cut);
-
-    // x of this warp's positions, in the layout of a product's left operand
-    float x[STATE ? 1 : P / 16][8];
-    uint32_t top_x[2] = {0, 0};
-    if (!STATE) {
-      const float* px = a.x.p + b * a.x.bs + t0 * a.x.ts + (int64_t)h * a.p;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int i = warp * 16 + quad + half * 8;
-        const float* row = px + i * a.x.ts;
-#pragma unroll
-        for (int k = 0; k < P / 16; ++k)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int col = k * 16 + e * 8 + 2 * t;
-            float2 v = make_float2(0.f, 0.f);
-            if (pairs_x) {
-              if (i < n && col < a.p) v = *reinterpret_cast<const float2*>(row + col);
-            } else {
-              if (i < n && col < a.p) v.x = row[col];
-              if (i < n && col + 1 < a.p) v.y = row[col + 1];
-            }
-            x[k][half * 2 + e * 4] = v.x;
-            x[k][half * 2 + e * 4 + 1] = v.y;
-          }
-      }
-    }
+  for (int c = c0;; ++c) {
     copies_done();
-    __syncthreads();       // y and z are here, the last chunk's tiles are read, max_x is known
-
-    uint32_t max_x = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) max_x = max(max_x, m.max_x[i]);
-    const int e_x = exponent(max_x);
-    if (!STATE && max_x < kInfinite && max_x > 0) {
-      const float up = power2(kTop - e_x);
-#pragma unroll
-      for (int mt = 0; mt < L::kRowTiles; ++mt)
-#pragma unroll
-        for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int row = row0 + mt * 16 + quad + half * 8;
-            uint32_t hi, lo;
-            split(up * X[mt][nt][half * 2], up * X[mt][nt][half * 2 + 1], hi, lo);
-            const uint32_t to = L::kX + piece<R>(row, col0 / 8 + nt) + 4 * t;
-            *reinterpret_cast<uint32_t*>(smem + to) = hi;
-            *reinterpret_cast<uint32_t*>(smem + to + P * R * 2) = lo;
-          }
-    }
-    // the rows' largest entries; a lane has 8 neighbouring columns of a row
-    constexpr int kLanesY = P / 8, kPassesY = kLanesY / 2, kLanesZ = R / 8, kPassesZ = kLanesZ / 2;
-    float y[kPassesY][8], z[kPassesZ][8];
-    uint32_t worst = max_x;
-    auto rows = [&](auto width, const float* raw, auto& v, uint32_t* max_row) {
-      constexpr int W = decltype(width)::value, kLanes = W / 8;
-#pragma unroll
-      for (int k = 0; k < kLanes / 2; ++k) {
-        const int row = warp * 16 + k * (32 / kLanes) + lane / kLanes, q = lane % kLanes;
-        const float4 u0 = reinterpret_cast<const float4*>(raw)[raw_piece<W>(row, 2 * q)];
-        const float4 u1 = reinterpret_cast<const float4*>(raw)[raw_piece<W>(row, 2 * q + 1)];
-        v[k][0] = u0.x, v[k][1] = u0.y, v[k][2] = u0.z, v[k][3] = u0.w;
-        v[k][4] = u1.x, v[k][5] = u1.y, v[k][6] = u1.z, v[k][7] = u1.w;
-        uint32_t most = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) most = max(most, size_bits(v[k][i]));
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1)
-          most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        if (q == 0) max_row[row] = most;
-        worst = max(worst, most);
-      }
-    };
-    rows(std::integral_constant<int, P>{}, raw_y, y, m.max_y);
-    rows(std::integral_constant<int, R>{}, raw_z, z, m.max_z);
-    if (!STATE) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-#pragma unroll
-        for (int k = 0; k < P / 16; ++k)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            top_x[half] = max(top_x[half], max(size_bits(x[k][half * 2 + e * 4]),
-                                               size_bits(x[k][half * 2 + e * 4 + 1])));
-        top_x[half] = max(top_x[half], __shfl_xor_sync(0xffffffffu, top_x[half], 1));
-        top_x[half] = max(top_x[half], __shfl_xor_sync(0xffffffffu, top_x[half], 2));
-        worst = max(worst, top_x[half]);
-      }
-    }
-    if (__syncthreads_or(worst >= kInfinite)) {
+    // y and z are here, the last chunk's tiles are read
+    if (__syncthreads_or(!(odd == 0.f))) {
+      bool next;
+      const unsigned long long cuts = resets(c - 1, next);
       float* state = reinterpret_cast<float*>(smem + L::kTiles);
       auto each = [&](auto f) {
 #pragma unroll
-        for (int mt = 0; mt < L::kRowTiles; ++mt)
+        for (int nt = 0; nt < L::kColTiles; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              f(X[mt][nt][e], state[(row0 + mt * 16 + quad + (e >> 1) * 8) * R + col0 + nt * 8 +
-                                    2 * t + (e & 1)]);
+          for (int e = 0; e < 4; ++e)
+            f(X[nt][e], state[(row0 + quad + (e >> 1) * 8) * R + col0 + nt * 8 + 2 * t + (e & 1)]);
       };
-      each([](float& v, float& kept) { kept = v; });
+      if (has_state) each([](float& v, float& to) { to = v; });
       __syncthreads();
-      rare_chunk<P, R, STATE>(state, sums, raw_y, raw_z, a, s, w, cuts, next_cut, l, b, h, t0, slice);
+      rare_chunk<P, R, STATE>(state, state + P * R, a, s, weights(c - 1, cuts, next), cuts, next, l,
+                              b, h, start(c - 1), slice);
       __syncthreads();
-      each([](float& v, float& kept) { v = kept; });
+      if (has_state) each([](float& v, float& to) { v = to; });
       __syncthreads();
-      if (c + 1 < c1) fetch(c + 1);
-    } else {
-      // what the rows weigh: lane looks at rows lane and lane + 32
-      int most = -1000, most_added = -1000;
+    } else if (c > c0) {
+#pragma unroll
+      for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) X[nt][e] = fmaf(kept, X[nt][e], by_d(d[nt][e]));
+    }
+    if (c == c1) break;
+    odd = 0.f;
+    bool next;
+    const unsigned long long cuts = resets(c, next);
+    const Weights w = weights(c, cuts, next);
+    const int t0 = start(c), n = w.n;
+
+    if (!STATE) {                       // the state's largest entry
+      float most = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2)
+          most = fmax3(most, fabsf(X[nt][e]), fabsf(X[nt][e + 1]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (lane == 0) m.max_state[warp] = most;
+    }
+    // the rows' largest entries
+    auto largest = [&](auto width, const float (&v)[8], int row, float* max_row) {
+      constexpr int kLanes = decltype(width)::value / 8;
+      float most = fmax3(fabsf(v[0]), fabsf(v[1]), fabsf(v[2]));
+      most = fmax3(most, fabsf(v[3]), fabsf(v[4]));
+      most = fmax3(most, fabsf(v[5]), fabsf(v[6]));
+      most = fmaxf(most, fabsf(v[7]));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1)
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      if (lane % kLanes == 0) max_row[row] = most;
+    };
+    float y[kPassesX][8], z[kPassesZ][8];
+    auto read = [&](auto width, const float* raw, float (&v)[8], int row) {
+      constexpr int W = decltype(width)::value;
+      const int q = lane % (W / 8);
+      const float4 u0 = reinterpret_cast<const float4*>(raw)[raw_piece<W>(row, 2 * q)];
+      const float4 u1 = reinterpret_cast<const float4*>(raw)[raw_piece<W>(row, 2 * q + 1)];
+      v[0] = u0.x, v[1] = u0.y, v[2] = u0.z, v[3] = u0.w;
+      v[4] = u1.x, v[5] = u1.y, v[6] = u1.z, v[7] = u1.w;
+    };
+#pragma unroll
+    for (int k = 0; k < kPassesX; ++k)
+      read(std::integral_constant<int, P>{}, raw_y, y[k], row_of(P, k));
+#pragma unroll
+    for (int k = 0; k < kPassesZ; ++k)
+      read(std::integral_constant<int, R>{}, raw_z, z[k], row_of(R, k));
+#pragma unroll
+    for (int k = 0; k < kPassesX; ++k)
+      largest(std::integral_constant<int, P>{}, y[k], row_of(P, k), m.max_y);
+#pragma unroll
+    for (int k = 0; k < kPassesZ; ++k)
+      largest(std::integral_constant<int, R>{}, z[k], row_of(R, k), m.max_z);
+    if constexpr (!STATE) {
+#pragma unroll
+      for (int k = 0; k < kPassesX; ++k)
+        largest(std::integral_constant<int, P>{}, x[k], row_of(P, k), m.max_x);
+    }
+    __syncthreads();
+
+    // what the rows weigh: lane looks at rows lane and lane + 32
+    int most = -1000, most_added = -1000;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int j = lane + 32 * k;
+      const float my = m.max_y[j], mz = m.max_z[j];
+      if (my == 0.f || mz == 0.f) continue;               // nothing there
+      const int e = exponent(my) + exponent(mz);
+      const Decayed u(m.power, w.added(j, back));
+      most = max(most, e);
+      if (u.any) most_added = max(most_added, e + u.e);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    most_added = __reduce_max_sync(0xffffffffu, most_added);
+    if (most == -1000) most = 0;
+    if (most_added == -1000) most_added = 0;
+    if (threadIdx.x < kC) {
+      // the power of two of l^u goes into the weight, the rest into z's scale
+      const int j = threadIdx.x, e = exponent(m.max_y[j]) + exponent(m.max_z[j]);
+      const Decayed u(m.power, w.added(j, back));
+      const float one = e - most < -126 ? 0.f : a.y_scale * power2(min(e - most, 0)) / u.rest;
+      m.weight[j] = make_float2(one, one * m.power[back ? j & 15 : 15 - (j & 15)]);
+      const int below = u.any ? min(e + u.e - most_added, 0) : -1000;
+      // 2^below as two halves, each 2^-24 at least (0: less than 2^-38 of the largest)
+      const int first = max(below, -24), then = max(below - first, -24);
+      m.added[0][j] = below < -38 ? 0 : __half_as_ushort(__float2half_rn(power2(first)));
+      m.added[1][j] = __half_as_ushort(__float2half_rn(power2(then)));
+      m.document[j] = w.document(j);
+    }
+    const bool far = __any_sync(0xffffffffu, [&] {        // a weight below one half number
+      bool any = false;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int j = lane + 32 * k;
-        if (j >= n) continue;
-        const int e = exponent(m.max_y[j]) + exponent(m.max_z[j]), u = w.added(j, back);
-        most = max(most, e);
-        if (u >= 0) most_added = max(most_added, e + exponent(size_bits(m.power[u])));
+        const Decayed u(m.power, w.added(j, back));
+        const int below = exponent(m.max_y[j]) + exponent(m.max_z[j]) + u.e - most_added;
+        any = any || (u.any && below < -24);
       }
-      most = __reduce_max_sync(0xffffffffu, most);
-      most_added = __reduce_max_sync(0xffffffffu, most_added);
-      if (!STATE && warp < 2) {
-        const int j = threadIdx.x;
-        const int e = exponent(m.max_y[j]) + exponent(m.max_z[j]) - most;
-        m.weight[j] = e < -126 || j >= n ? 0.f : power2(e);
-        m.document[j] = w.document(j);
-      }
-      // the tiles
+      return any;
+    }());
+    // the tiles
+    auto tile = [&](auto width, int to, const float (&v)[8], int row, float up) {
+      constexpr int W = decltype(width)::value;
+      uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int k = 0; k < kPassesY; ++k) {
-        const int row = warp * 16 + k * (32 / kLanesY) + lane / kLanesY, q = lane % kLanesY;
-        const int e = exponent(m.max_y[row]), u = w.added(row, back);
-        const float up = power2(kTop - e);
-        float by = 0.f;
-        if (u >= 0) {
-          const int below = e + exponent(m.max_z[row]) - most_added;
-          by = below < -126 ? 0.f : m.power[u] * power2(min(below, 126));
-        }
-        uint32_t hi[4], lo[4], whi[4], wlo[4];
+      for (int i = 0; i < 4; ++i) split(up * v[2 * i], up * v[2 * i + 1], hi[i], lo[i]);
+      unsigned char* p = smem + to + piece<W>(row, lane % (W / 8));
+      *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(p + kC * W * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    };
+    float max_state = 0.f;
+    int e_state = 0;
+    if constexpr (!STATE) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float u0 = up * y[k][2 * i], u1 = up * y[k][2 * i + 1];
-          if (!STATE) split(u0, u1, hi[i], lo[i]);
-          split(by * u0, by * u1, whi[i], wlo[i]);
-        }
-        const uint32_t to = piece<P>(row, q);
-        if (!STATE) {
-          *reinterpret_cast<uint4*>(smem + L::kY + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(smem + L::kY + kC * P * 2 + to) =
-              make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        *reinterpret_cast<uint4*>(smem + L::kW + to) = make_uint4(whi[0], whi[1], whi[2], whi[3]);
-        *reinterpret_cast<uint4*>(smem + L::kW + kC * P * 2 + to) =
-            make_uint4(wlo[0], wlo[1], wlo[2], wlo[3]);
+      for (int i = 0; i < 8; ++i) max_state = fmaxf(max_state, m.max_state[i]);
+      e_state = exponent(max_state);
+      if (has_state && max_state > 0.f) {
+        const float up = power2(kTop - e_state);
+#pragma unroll
+        for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t hi, lo;
+            split(up * X[nt][e * 2], up * X[nt][e * 2 + 1], hi, lo);
+            unsigned char* p = smem + L::kState + piece<R>(row0 + quad + e * 8, col0 / 8 + nt) + 4 * t;
+            *reinterpret_cast<uint32_t*>(p) = hi;
+            *reinterpret_cast<uint32_t*>(p + P * R * 2) = lo;
+          }
       }
 #pragma unroll
-      for (int k = 0; k < kPassesZ; ++k) {
-        const int row = warp * 16 + k * (32 / kLanesZ) + lane / kLanesZ, q = lane % kLanesZ;
-        const float up = power2(kTop - exponent(m.max_z[row]));
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) split(up * z[k][2 * i], up * z[k][2 * i + 1], hi[i], lo[i]);
-        const uint32_t to = piece<R>(row, q);
-        *reinterpret_cast<uint4*>(smem + L::kZ + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(smem + L::kZ + kC * R * 2 + to) =
-            make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      for (int k = 0; k < kPassesX; ++k) {
+        const int row = row_of(P, k);
+        tile(std::integral_constant<int, P>{}, L::kX, x[k], row, power2(kTop - exponent(m.max_x[row])));
       }
-      __syncthreads();
-      if (c + 1 < c1) fetch(c + 1);
+    }
+#pragma unroll
+    for (int k = 0; k < kPassesX; ++k) {
+      const int row = row_of(P, k);
+      tile(std::integral_constant<int, P>{}, L::kY, y[k], row, power2(kTop - exponent(m.max_y[row])));
+    }
+#pragma unroll
+    for (int k = 0; k < kPassesZ; ++k) {
+      const int row = row_of(R, k);
+      tile(std::integral_constant<int, R>{}, L::kZ, z[k], row,
+           Decayed(m.power, w.added(row, back)).rest * power2(kTop - exponent(m.max_z[row])));
+    }
+    __syncthreads();
+    if (c + 1 < c1) fetch(c + 1);
 
-      const int mat = lane >> 3, mat_row = lane & 7;
-      if (!STATE) {
-        int e_row[2];
-        uint32_t xh[P / 16][4], xl[P / 16][4];
+    if constexpr (!STATE) {
+      uint32_t xh[P / 16][4], xl[P / 16][4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          e_row[half] = exponent(top_x[half]);
-          const float up = power2(kTop - e_row[half]);
+      for (int k = 0; k < P / 16; ++k) {
+        const uint32_t from =
+            base + L::kX + piece<P>(group * 16 + (mat & 1) * 8 + mat_row, 2 * k + (mat >> 1));
+        load4(xh[k], from);
+        load4(xl[k], from + kC * P * 2);
+      }
+      // x y^T for every other 16 positions up to (back: from) this group's own
+      float S[2][2][4];
+      float most_p[2] = {0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < P / 16; ++k)
+      for (int q = 0; q < 2; ++q) {
+        const int jb = half + 2 * q;
+        if (back ? jb < group : jb > group) continue;
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              split(up * x[k][half * 2 + e * 4], up * x[k][half * 2 + e * 4 + 1],
-                    xh[k][half + 2 * e], xl[k][half + 2 * e]);
+        for (int e = 0; e < 4; ++e) S[q][0][e] = S[q][1][e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < P / 16; ++k) {
+          uint32_t bh[4], bl[4];
+          const uint32_t from =
+              base + L::kY + piece<P>(jb * 16 + (mat >> 1) * 8 + mat_row, 2 * k + (mat & 1));
+          load4(bh, from);
+          load4(bl, from + kC * P * 2);
+          products(S[q][0], S[q][1], xh[k], xl[k], bh, bl);
         }
-        float o[R / 8][4];
+        // its weights, and the rows' largest: l^(i - j) is looked up in the group's own
+        // positions, elsewhere it is a product of three powers of at least 0
+        const float gap = jb == group ? 1.f : m.power[16 * abs(group - jb) - 15];
+        const float side[2] = {gap * m.power[back ? 15 - quad : quad],
+                               gap * m.power[back ? 7 - quad : quad + 8]};
 #pragma unroll
-        for (int nt = 0; nt < R / 8; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
-        if (max_x > 0) {
-#pragma unroll
-          for (int k = 0; k < P / 16; ++k)
-#pragma unroll
-            for (int nb = 0; nb < R / 16; ++nb) {
-              uint32_t bh[4], bl[4];
-              const uint32_t from =
-                  at_x + piece<R>(k * 16 + (mat & 1) * 8 + mat_row, 2 * nb + (mat >> 1));
-              load4_turned(bh, from);
-              load4_turned(bl, from + P * R * 2);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                products(o[2 * nb + e], xh[k], xl[k], bh[2 * e], bh[2 * e + 1], bl[2 * e],
-                         bl[2 * e + 1]);
-              }
-            }
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int u = w.reach(warp * 16 + quad + half * 8, back);
-            const Scale by(u < 0 ? 0.f : m.power[u], e_row[half] + e_x - 2 * kTop);
-#pragma unroll
-            for (int nt = 0; nt < R / 8; ++nt) {
-              o[nt][half * 2] = by(o[nt][half * 2]);
-              o[nt][half * 2 + 1] = by(o[nt][half * 2 + 1]);
-            }
-          }
-        }
-        // x y^T for the positions up to (back: from) this warp's own
-        float S[kC / 8][4];
-#pragma unroll
-        for (int jb = 0; jb < kC / 16; ++jb) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) S[2 * jb][e] = S[2 * jb + 1][e] = 0.f;
-          if (back ? jb < warp : jb > warp) continue;
-#pragma unroll
-          for (int k = 0; k < P / 16; ++k) {
-            uint32_t bh[4], bl[4];
-            const uint32_t from =
-                at_y + piece<P>(jb * 16 + (mat >> 1) * 8 + mat_row, 2 * k + (mat & 1));
-            load4(bh, from);
-            load4(bl, from + kC * P * 2);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              products(S[2 * jb + e], xh[k], xl[k], bh[2 * e], bh[2 * e + 1], bl[2 * e],
-                       bl[2 * e + 1]);
-            }
-          }
-        }
-        // its weights, and the rows' scales
-        uint32_t most_p[2] = {0, 0};
-#pragma unroll
-        for (int jt = 0; jt < kC / 8; ++jt) {
-          if (back ? jt / 2 < warp : jt / 2 > warp) continue;
+        for (int jt = 0; jt < 2; ++jt) {
+          const int j = jb * 16 + jt * 8 + 2 * t;
+          const float4 v = *reinterpret_cast<const float4*>(&m.weight[j]);
+          const float one[2] = {v.x, v.z}, other[2] = {v.y, v.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int i = warp * 16 + quad + (e >> 1) * 8, j = jt * 8 + 2 * t + (e & 1);
-            const int apart = back ? j - i : i - j;
-            float v = apart < 0 ? 0.f : S[jt][e] * (m.power[max(apart, 0)] * m.weight[j]);
-            if (w.inner && m.document[i] != m.document[j]) v = 0.f;
-            S[jt][e] = v;
-            most_p[e >> 1] = max(most_p[e >> 1], size_bits(v));
+            float value = S[q][jt][e];
+            if (jb == group) {
+              const int i = quad + (e >> 1) * 8, k = jt * 8 + 2 * t + (e & 1);
+              const int apart = back ? k - i : i - k;
+              value = apart < 0 ? 0.f : value * (m.power[max(apart, 0)] * one[e & 1]);
+            } else {
+              value *= side[e >> 1] * other[e & 1];
+            }
+            if (w.inner && m.document[group * 16 + quad + (e >> 1) * 8] != m.document[j + (e & 1)])
+              value = 0.f;
+            S[q][jt][e] = value;
           }
+          most_p[0] = fmax3(most_p[0], fabsf(S[q][jt][0]), fabsf(S[q][jt][1]));
+          most_p[1] = fmax3(most_p[1], fabsf(S[q][jt][2]), fabsf(S[q][jt][3]));
         }
-        int e_p[2];
-        float up[2];
+      }
+      // x X over this half of the state's rows
+      float o[R / 8][4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          most_p[half] = max(most_p[half], __shfl_xor_sync(0xffffffffu, most_p[half], 1));
-          most_p[half] = max(most_p[half], __shfl_xor_sync(0xffffffffu, most_p[half], 2));
-          e_p[half] = exponent(most_p[half]);
-          up[half] = power2(kTop - e_p[half]);
-        }
-        float v[R / 8][4];
+      for (int nt = 0; nt < R / 8; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < R / 8; ++nt)
+        for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
+      if (max_state > 0.f) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[nt][e] = 0.f;
-#pragma unroll
-        for (int jb = 0; jb < kC / 16; ++jb) {
-          if (back ? jb < warp : jb > warp) continue;
-          uint32_t ph[4], pl[4];
+        for (int k = 0; k < P / 32; ++k) {
+          const int kk = half * (P / 32) + k;
+          uint32_t ah[4], al[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float f = up[e & 1];
-            split(f * S[2 * jb + (e >> 1)][(e & 1) * 2], f * S[2 * jb + (e >> 1)][(e & 1) * 2 + 1],
-                  ph[e], pl[e]);
+            ah[e] = half ? xh[P / 32 + k][e] : xh[k][e];
+            al[e] = half ? xl[P / 32 + k][e] : xl[k][e];
           }
 #pragma unroll
           for (int nb = 0; nb < R / 16; ++nb) {
             uint32_t bh[4], bl[4];
-            const uint32_t from =
-                at_z + piece<R>(jb * 16 + (mat & 1) * 8 + mat_row, 2 * nb + (mat >> 1));
+            const uint32_t from = base + L::kState +
+                                  piece<R>(kk * 16 + (mat & 1) * 8 + mat_row, 2 * nb + (mat >> 1));
             load4_turned(bh, from);
-            load4_turned(bl, from + kC * R * 2);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              products(v[2 * nb + e], ph, pl, bh[2 * e], bh[2 * e + 1], bl[2 * e], bl[2 * e + 1]);
-            }
+            load4_turned(bl, from + P * R * 2);
+            products(o[2 * nb], o[2 * nb + 1], ah, al, bh, bl);
           }
         }
+      }
+      // Both sums in one scale: the larger's, whichever part it comes from.
+      Scale by[2] = {Scale(0.f, 0), Scale(0.f, 0)};
+      float up[2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int i = warp * 16 + quad + half * 8;
-          const Scale by(a.y_scale, e_row[half] + e_p[half] + most - 4 * kTop);
+      for (int side = 0; side < 2; ++side) {
+        const int i = group * 16 + quad + side * 8, u = w.reach(i, back);
+        most_p[side] = fmaxf(most_p[side], __shfl_xor_sync(0xffffffffu, most_p[side], 1));
+        most_p[side] = fmaxf(most_p[side], __shfl_xor_sync(0xffffffffu, most_p[side], 2));
+        int e_p = exponent(most_p[side]);
+        const float decay = u < 0 ? 0.f : m.power[u];
+        const int apart = e_state + 2 * kTop - most;
+        if (max_state > 0.f && decay > 0.f) e_p = max(e_p, apart + exponent(decay) - kTop);
+        const Scale in(decay, apart - e_p);
+#pragma unroll
+        for (int nt = 0; nt < R / 8; ++nt) {
+          o[nt][2 * side] = in(o[nt][2 * side]);
+          o[nt][2 * side + 1] = in(o[nt][2 * side + 1]);
+        }
+        up[side] = kTop - e_p < -126 ? 0.f : power2(kTop - e_p);
+        by[side] = Scale(a.out_scale, e_p + exponent(m.max_x[i]) + most - 4 * kTop);
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int jb = half + 2 * q;
+        if (back ? jb < group : jb > group) continue;
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float f = up[e & 1];
+          split(f * S[q][e >> 1][(e & 1) * 2], f * S[q][e >> 1][(e & 1) * 2 + 1], ph[e], pl[e]);
+        }
+#pragma unroll
+        for (int nb = 0; nb < R / 16; ++nb) {
+          uint32_t bh[4], bl[4];
+          const uint32_t from =
+              base + L::kZ + piece<R>(jb * 16 + (mat & 1) * 8 + mat_row, 2 * nb + (mat >> 1));
+          load4_turned(bh, from);
+          load4_turned(bl, from + kC * R * 2);
+          products(o[2 * nb], o[2 * nb + 1], ph, pl, bh, bl);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < R / 8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][e] = by[e >> 1](o[nt][e]);
+      // each half of the group writes half of the columns
+      pair_barrier(group);                                // both have read x's tile
+      auto finish = [&](auto which) {
+        constexpr int kMine = decltype(which)::value * (R / 16), kOther = R / 16 - kMine;
+        float2* sums = reinterpret_cast<float2*>(smem + L::kSums + group * L::kGroup);
+        constexpr int kApart = L::kHalf / (int)sizeof(float2);
+#pragma unroll
+        for (int k = 0; k < R / 16; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            sums[decltype(which)::value * kApart + (2 * k + e) * 32 + lane] =
+                make_float2(o[kOther + k][2 * e], o[kOther + k][2 * e + 1]);
+        pair_barrier(group);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = group * 16 + quad + e * 8;
           float* out = a.out + ((b * s.T + t0 + i) * s.H + h) * a.r + slice * R;
 #pragma unroll
-          for (int nt = 0; nt < R / 8; ++nt) {
-            const int r = nt * 8 + 2 * t, room = a.r - slice * R;
-            const float v0 = a.out_scale * (by(v[nt][half * 2]) + o[nt][half * 2]);
-            const float v1 = a.out_scale * (by(v[nt][half * 2 + 1]) + o[nt][half * 2 + 1]);
+          for (int k = 0; k < R / 16; ++k) {
+            const float2 more = sums[(1 - decltype(which)::value) * kApart + (2 * k + e) * 32 + lane];
+            const float v0 = o[kMine + k][2 * e] + more.x, v1 = o[kMine + k][2 * e + 1] + more.y;
+            const int r = (kMine + k) * 8 + 2 * t, room = a.r - slice * R;
+            odd = fmaf(v0, 0.f, odd);
+            odd = fmaf(v1, 0.f, odd);
             if (i >= n) continue;
             if (pairs_o) {
               if (r < room) *reinterpret_cast<float2*>(out + r) = make_float2(v0, v1);
@@ -796,63 +871,70 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
             }
           }
         }
-      }
-      // the state: its chunk's products, then in 32 bits
-      const Scale by(a.y_scale, most_added - 2 * kTop);
-      const int u = w.kept(back);
-      const float kept = u < 0 ? 0.f : m.power[u];
+      };
+      if (half == 0)
+        finish(std::integral_constant<int, 0>{});
+      else
+        finish(std::integral_constant<int, 1>{});
+      if (c + 1 < c1) fetch_x(c + 1);
+    }
+    // what the chunk adds to the state
 #pragma unroll
-      for (int mt = 0; mt < L::kRowTiles; ++mt) {
-        float d[L::kColTiles][4];
+    for (int nt = 0; nt < L::kColTiles; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < L::kColTiles; ++nt)
+      for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
+    if (has_state) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
+      for (int k = 0; k < kC / 16; ++k) {
+        uint32_t ah[4], al[4];
+        const uint32_t from =
+            base + L::kY + piece<P>(k * 16 + (mat >> 1) * 8 + mat_row, row0 / 8 + (mat & 1));
+        load4_turned(ah, from);
+        load4_turned(al, from + kC * P * 2);
 #pragma unroll
-        for (int k = 0; k < kC / 16; ++k) {
-          uint32_t ah[4], al[4];
-          const uint32_t from = at_w + piece<P>(k * 16 + (mat >> 1) * 8 + mat_row,
-                                                (row0 + mt * 16) / 8 + (mat & 1));
-          load4_turned(ah, from);
-          load4_turned(al, from + kC * P * 2);
-#pragma unroll
-          for (int nb = 0; nb < L::kColTiles / 2; ++nb) {
-            uint32_t bh[4], bl[4];
-            const uint32_t zat = at_z + piece<R>(k * 16 + (mat & 1) * 8 + mat_row,
-                                                 col0 / 8 + 2 * nb + (mat >> 1));
-            load4_turned(bh, zat);
-            load4_turned(bl, zat + kC * R * 2);
-            products(d[2 * nb], ah, al, bh[0], bh[1], bl[0], bl[1]);
-            products(d[2 * nb + 1], ah, al, bh[2], bh[3], bl[2], bl[3]);
+        for (int e = 0; e < 4; ++e) {
+          const int j = k * 16 + (e >> 1) * 8 + 2 * t;
+          const uint32_t f = *reinterpret_cast<const uint32_t*>(&m.added[0][j]);
+          ah[e] = times(ah[e], f);
+          al[e] = times(al[e], f);
+          if (far) {
+            const uint32_t f2 = *reinterpret_cast<const uint32_t*>(&m.added[1][j]);
+            ah[e] = times(ah[e], f2);
+            al[e] = times(al[e], f2);
           }
         }
 #pragma unroll
-        for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) X[mt][nt][e] = fmaf(kept, X[mt][nt][e], by(d[nt][e]));
+        for (int nb = 0; nb < L::kColTiles / 2; ++nb) {
+          uint32_t bh[4], bl[4];
+          const uint32_t zat = base + L::kZ + piece<R>(k * 16 + (mat & 1) * 8 + mat_row,
+                                                       col0 / 8 + 2 * nb + (mat >> 1));
+          load4_turned(bh, zat);
+          load4_turned(bl, zat + kC * R * 2);
+          products(d[2 * nb], d[2 * nb + 1], ah, al, bh, bl);
+        }
       }
     }
-    if (STATE) {
-      const int u = w.kept(back);
-      run *= u < 0 ? 0.f : m.power[u];
-    }
-    publish();
+    by_d = Scale(a.y_scale, most_added - 2 * kTop);
+    const int u = w.kept(back);
+    kept = u < 0 ? 0.f : m.power[u];
+    if (STATE) run *= kept;
+#pragma unroll
+    for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd = fmaf(d[nt][e], 0.f, fmaf(X[nt][e], 0.f, odd));
   }
 
-  const bool keep = STATE || (a.last && seg == pieces - 1);
+  const bool keep = has_state && (STATE || (a.last && seg == pieces - 1));
   float* to = STATE ? g.state + ((pass * (int64_t)pieces + seg) * heads + b * s.H + h) * a.p * a.r
                     : a.last + (b * s.H + h) * (int64_t)a.p * a.r;
   const int64_t ps = STATE ? a.r : a.p_stride, rs = STATE ? 1 : a.r_stride;
 #pragma unroll
-  for (int mt = 0; mt < L::kRowTiles; ++mt)
+  for (int nt = 0; nt < L::kColTiles; ++nt)
 #pragma unroll
-    for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int p = row0 + mt * 16 + quad + (e >> 1) * 8;
-        const int r = slice * R + col0 + nt * 8 + 2 * t + (e & 1);
-        if (keep && p < a.p && r < a.r) to[p * ps + r * rs] = X[mt][nt][e];
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int p = row0 + quad + (e >> 1) * 8, r = slice * R + col0 + nt * 8 + 2 * t + (e & 1);
+      if (keep && p < a.p && r < a.r) to[p * ps + r * rs] = X[nt][e];
+    }
   if (STATE && threadIdx.x == 0)
     g.kept[(pass * (int64_t)pieces + seg) * heads + b * s.H + h] = run;
 }
@@ -953,8 +1035,9 @@ int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
   const int64_t heads = B * s.H, blocks = heads * slices, chunks = (s.T + kC - 1) / kC;
   const int64_t resident = (int64_t)wxx::num_sms() * L::kBlocks;
   Segments g{1, (int)chunks, nullptr, nullptr};
-  if (blocks * n < resident) {
-    int64_t size = (chunks * blocks * n + resident - 1) / resident;
+  const int64_t most = resident / (blocks * n);
+  if (most >= 2) {
+    int64_t size = (chunks + most - 1) / most;
     if (size < 4) size = 4;
     g.count = (int)((chunks + size - 1) / size);
     g.chunks = (int)size;
