@@ -14,6 +14,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 WXX_EXPORT int wxx_malloc(void** out, uint64_t nbytes);
@@ -58,6 +60,43 @@ __device__ __forceinline__ float slope(float v) {
     return v > 10.f ? 1.f : v < -10.f ? 0.f : r;
   }
   return 1.f;
+}
+
+// The same where the activation is one branch for all threads (memory-bound kernels).
+__device__ __forceinline__ float act(int code, float v) {
+  return code == kSilu ? act<kSilu>(v) : code == kGelu ? act<kGelu>(v) : code == kRelu ? act<kRelu>(v) : v;
+}
+__device__ __forceinline__ float slope(int code, float v) {
+  return code == kSilu   ? slope<kSilu>(v)
+         : code == kGelu ? slope<kGelu>(v)
+         : code == kRelu ? slope<kRelu>(v)
+                         : 1.f;
+}
+
+template <int V>
+struct Pack {
+  float v[V];
+};
+template <int V>
+__device__ __forceinline__ Pack<V> load(const float* p) {
+  Pack<V> out;
+  if constexpr (V == 4) {
+    const float4 t = *reinterpret_cast<const float4*>(p);
+    out.v[0] = t.x, out.v[1] = t.y, out.v[2] = t.z, out.v[3] = t.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out.v[e] = p[e];
+  }
+  return out;
+}
+template <int V>
+__device__ __forceinline__ void store(float* p, const Pack<V>& a) {
+  if constexpr (V == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(a.v[0], a.v[1], a.v[2], a.v[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) p[e] = a.v[e];
+  }
 }
 
 // A count of values with their mean and the sum of their squared distances from it.
@@ -286,6 +325,398 @@ __global__ void __launch_bounds__(kT)
   }
 }
 
+// ------------------------------------------------------------------ one position a sample
+//
+// A group is `lanes` threads' registers (a power of two up to 32, K pieces of V channels
+// each), so x, the gate and dy are read once.  Backward a thread keeps its channels from
+// sample to sample and with them the sums for dgamma and dbeta: `rows` samples are under
+// way at once, and as many partial sums are added up by column_sums_kernel.
+
+struct Few {
+  int64_t N;
+  int C, G, per, lanes, rows, code;
+  float eps;
+};
+
+template <int K, int V>
+__device__ __forceinline__ float over_lanes(float v, int lanes) {
+  for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <int V, int K, bool GATED>
+__global__ void __launch_bounds__(kT)
+    token_kernel(float* __restrict__ y, float* __restrict__ mean, float* __restrict__ inv,
+                 const float* __restrict__ x, const float* __restrict__ gate,
+                 const float* __restrict__ gamma, const float* __restrict__ beta, const Few f) {
+  const unsigned total = (unsigned)(f.N * f.G), step = gridDim.x * kT / f.lanes;
+  const int lane = threadIdx.x % f.lanes;
+  for (unsigned u0 = (blockIdx.x * kT + threadIdx.x) / 32 * 32 / f.lanes; u0 < total; u0 += step) {
+    const unsigned u = u0 + threadIdx.x % 32 / f.lanes;      // a warp's groups go on together
+    const bool on = u < total;
+    const int64_t n = u / f.G;
+    const int g = (int)(u - n * f.G);
+    const int64_t at = n * f.C + g * f.per;
+    Pack<V> v[K], w[GATED ? K : 1];
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * f.lanes + lane) * V;
+      const bool in = on && c < f.per;
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[k].v[e] = 0.f;
+      if (in) v[k] = load<V>(x + at + c);
+      if (GATED && in) w[k] = load<V>(gate + at + c);
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum += v[k].v[e];
+    }
+    const float mu = over_lanes<K, V>(sum, f.lanes) / (float)f.per;
+    float square = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool in = (k * f.lanes + lane) * V < f.per;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[k].v[e] -= mu;
+        if (in) square = fmaf(v[k].v[e], v[k].v[e], square);
+      }
+    }
+    const float is = 1.0f / sqrtf(over_lanes<K, V>(square, f.lanes) / (float)f.per + f.eps);
+    if (!on) continue;
+    if (lane == 0) {
+      mean[u] = mu;
+      inv[u] = is;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * f.lanes + lane) * V;
+      if (c >= f.per) continue;
+      Pack<V> ga, be;
+#pragma unroll
+      for (int e = 0; e < V; ++e) ga.v[e] = 1.f, be.v[e] = 0.f;
+      if (gamma) ga = load<V>(gamma + g * f.per + c);
+      if (beta) be = load<V>(beta + g * f.per + c);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float t = fmaf(v[k].v[e] * is, ga.v[e], be.v[e]);
+        v[k].v[e] = GATED ? t * act(f.code, w[k].v[e]) : act(f.code, t);
+      }
+      store<V>(y + at + c, v[k]);
+    }
+  }
+}
+
+// The gradient of n at one place, and where GATED that of the gate.
+template <bool GATED>
+__device__ __forceinline__ float inner_gradient(int code, float dy, float z, float gamma,
+                                                float beta, float gate, float* dgate) {
+  const float v = fmaf(z, gamma, beta);
+  if (!GATED) return dy * slope(code, v);
+  *dgate = dy * v * slope(code, gate);
+  return dy * act(code, gate);
+}
+
+template <int V, int K, bool GATED>
+__global__ void __launch_bounds__(kT)
+    token_backward_kernel(float* __restrict__ dx, float* __restrict__ dgate,
+                          float* __restrict__ part, const float* __restrict__ dy,
+                          const float* __restrict__ x, const float* __restrict__ gate,
+                          const float* __restrict__ mean, const float* __restrict__ inv,
+                          const float* __restrict__ gamma, const float* __restrict__ beta,
+                          const Few f) {
+  // a thread's group of channels, and its first sample
+  const unsigned slot = (blockIdx.x * kT + threadIdx.x) / f.lanes;
+  const int lane = threadIdx.x % f.lanes, g = slot % f.G, row = slot / f.G;
+  const bool here = row < f.rows;
+  Pack<V> ga[K], be[K], sum_n[K], sum_z[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * f.lanes + lane) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) ga[k].v[e] = 1.f, be[k].v[e] = sum_n[k].v[e] = sum_z[k].v[e] = 0.f;
+    if (gamma && c < f.per) ga[k] = load<V>(gamma + g * f.per + c);
+    if (beta && c < f.per) be[k] = load<V>(beta + g * f.per + c);
+  }
+  // every lane of a warp takes as many turns (rows differ by one at most)
+  for (int64_t n0 = row; __any_sync(0xffffffffu, here && n0 < f.N); n0 += f.rows) {
+    const bool on = here && n0 < f.N;
+    const int64_t at = n0 * f.C + g * f.per;
+    const float mu = on ? mean[n0 * f.G + g] : 0.f, is = on ? inv[n0 * f.G + g] : 0.f;
+    Pack<V> z[K], d[K], w[GATED ? K : 1];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * f.lanes + lane) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[k].v[e] = mu, d[k].v[e] = 0.f;
+      if (GATED)
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[k].v[e] = 0.f;
+      if (on && c < f.per) {
+        z[k] = load<V>(x + at + c);
+        d[k] = load<V>(dy + at + c);
+        if (GATED) w[k] = load<V>(gate + at + c);
+      }
+    }
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        z[k].v[e] = (z[k].v[e] - mu) * is;
+        float dg = 0.f;
+        const float dn = inner_gradient<GATED>(f.code, d[k].v[e], z[k].v[e], ga[k].v[e], be[k].v[e],
+                                               GATED ? w[k].v[e] : 0.f, &dg);
+        if (GATED) w[k].v[e] = dg;
+        sum_n[k].v[e] += dn;
+        sum_z[k].v[e] = fmaf(dn, z[k].v[e], sum_z[k].v[e]);
+        d[k].v[e] = ga[k].v[e] * dn;
+        a += d[k].v[e];
+        b = fmaf(d[k].v[e], z[k].v[e], b);
+      }
+    a = over_lanes<K, V>(a, f.lanes) / (float)f.per;
+    b = over_lanes<K, V>(b, f.lanes) / (float)f.per;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * f.lanes + lane) * V;
+      if (!on || c >= f.per) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[k].v[e] = is * (d[k].v[e] - a - z[k].v[e] * b);
+      store<V>(dx + at + c, d[k]);
+      if (GATED) store<V>(dgate + at + c, w[k]);
+    }
+  }
+  if (!here) return;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * f.lanes + lane) * V;
+    if (c >= f.per) continue;
+    float* out = part + (int64_t)row * 2 * f.C + g * f.per + c;
+    store<V>(out, sum_n[k]);
+    store<V>(out + f.C, sum_z[k]);
+  }
+}
+
+// ------------------------------------------------------------------ maps in registers
+//
+// A block has `wide` channels (whole groups) of all positions of a sample in its
+// registers, K pieces of V channels a thread: `across` pieces of a position by `rows`
+// positions at a time.  Sums go over the threads through shared memory in a fixed order.
+
+struct Slab {
+  int64_t N;
+  int S, C, G, per, wide, spans, across, rows, split, code;
+  float eps;
+};
+
+// Sums over a block's positions of M numbers per channel: every thread's `v` (M, V), of
+// channels q V ..; out (M, split, wide): `split` partial sums of each.
+template <int M, int V>
+__device__ __forceinline__ void channel_sums(float* scratch, float* out, const float (&v)[M][V],
+                                             int q, int row, bool on, const Slab& f) {
+  __syncthreads();                                   // whoever read out and scratch is done
+  if (on)
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) scratch[(i * f.rows + row) * f.wide + q * V + e] = v[i][e];
+  __syncthreads();
+  for (int t = threadIdx.x; t < M * f.split * f.wide; t += blockDim.x) {
+    const int c = t % f.wide, j = t / f.wide % f.split, i = t / f.wide / f.split;
+    float sum = 0.f;
+    for (int r = j; r < f.rows; r += f.split) sum += scratch[(i * f.rows + r) * f.wide + c];
+    out[t] = sum;
+  }
+  __syncthreads();
+}
+
+template <int V, int K, bool GATED>
+__global__ void __launch_bounds__(512)
+    slab_kernel(float* __restrict__ y, float* __restrict__ mean, float* __restrict__ inv,
+                const float* __restrict__ x, const float* __restrict__ gate,
+                const float* __restrict__ gamma, const float* __restrict__ beta, const Slab f) {
+  extern __shared__ float smem[];
+  float* scratch = smem;                             // (rows, wide)
+  float* sums = scratch + f.rows * f.wide;           // (split, wide)
+  float* group = sums + f.split * f.wide;            // (wide / per) twice
+  const int64_t n = blockIdx.x / f.spans;
+  const int c0 = blockIdx.x % f.spans * f.wide, wide = min(f.wide, f.C - c0), groups = wide / f.per;
+  const int q = threadIdx.x % f.across, row = threadIdx.x / f.across;
+  const bool on = row < f.rows, in = on && q * V < wide;
+  const int64_t at = n * f.S * f.C + c0 + q * V;
+  Pack<V> v[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int p = row + k * f.rows;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[k].v[e] = 0.f;
+    if (in && p < f.S) v[k] = load<V>(x + at + (int64_t)p * f.C);
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float count = (float)f.S * (float)f.per;
+  auto over_groups = [&](float* to, auto finish) {
+    for (int g = warp; g < groups; g += blockDim.x >> 5) {
+      float sum = 0.f;
+      for (int i = lane; i < f.per * f.split; i += 32)
+        sum += sums[i / f.per * f.wide + g * f.per + i % f.per];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) to[g] = finish(sum / count);
+    }
+    __syncthreads();
+  };
+  int of[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) of[e] = in ? (q * V + e) / f.per : 0;
+  float part[1][V] = {};
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int e = 0; e < V; ++e) part[0][e] += v[k].v[e];
+  channel_sums<1, V>(scratch, sums, part, q, row, on, f);
+  over_groups(group, [](float m) { return m; });
+  float mu[V], is[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) mu[e] = group[of[e]], part[0][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      v[k].v[e] -= mu[e];
+      if (row + k * f.rows < f.S) part[0][e] = fmaf(v[k].v[e], v[k].v[e], part[0][e]);
+    }
+  if (!in)
+#pragma unroll
+    for (int e = 0; e < V; ++e) part[0][e] = 0.f;
+  channel_sums<1, V>(scratch, sums, part, q, row, on, f);
+  over_groups(group + groups, [&](float m) { return 1.0f / sqrtf(m + f.eps); });
+  for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+    mean[n * f.G + c0 / f.per + g] = group[g];
+    inv[n * f.G + c0 / f.per + g] = group[groups + g];
+  }
+  if (!in) return;
+  float ga[V], be[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    is[e] = group[groups + of[e]];
+    ga[e] = (gamma ? gamma[c0 + q * V + e] : 1.f);
+    be[e] = beta ? beta[c0 + q * V + e] : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int p = row + k * f.rows;
+    if (p >= f.S) continue;
+    Pack<V> w;
+    if (GATED) w = load<V>(gate + at + (int64_t)p * f.C);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float t = fmaf(v[k].v[e] * is[e], ga[e], be[e]);
+      v[k].v[e] = GATED ? t * act(f.code, w.v[e]) : act(f.code, t);
+    }
+    store<V>(y + at + (int64_t)p * f.C, v[k]);
+  }
+}
+
+template <int V, int K, bool GATED>
+__global__ void __launch_bounds__(512)
+    slab_backward_kernel(float* __restrict__ dx, float* __restrict__ dgate,
+                         float* __restrict__ part, const float* __restrict__ dy,
+                         const float* __restrict__ x, const float* __restrict__ gate,
+                         const float* __restrict__ mean, const float* __restrict__ inv,
+                         const float* __restrict__ gamma, const float* __restrict__ beta,
+                         const Slab f) {
+  extern __shared__ float smem[];
+  float* scratch = smem;                             // (2, rows, wide)
+  float* sums = scratch + 2 * f.rows * f.wide;       // (2, split, wide)
+  float2* group = reinterpret_cast<float2*>(sums + 2 * f.split * f.wide);   // (wide / per)
+  const int64_t n = blockIdx.x / f.spans;
+  const int c0 = blockIdx.x % f.spans * f.wide, wide = min(f.wide, f.C - c0), groups = wide / f.per;
+  const int q = threadIdx.x % f.across, row = threadIdx.x / f.across;
+  const bool on = row < f.rows, in = on && q * V < wide;
+  const int64_t at = n * f.S * f.C + c0 + q * V;
+  Pack<V> z[K], d[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int p = row + k * f.rows;
+#pragma unroll
+    for (int e = 0; e < V; ++e) z[k].v[e] = d[k].v[e] = 0.f;
+    if (in && p < f.S) {
+      z[k] = load<V>(x + at + (int64_t)p * f.C);
+      d[k] = load<V>(dy + at + (int64_t)p * f.C);
+    }
+  }
+  float mu[V], is[V], ga[V], be[V];
+  int of[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    of[e] = in ? (q * V + e) / f.per : 0;
+    mu[e] = in ? mean[n * f.G + c0 / f.per + of[e]] : 0.f;
+    is[e] = in ? inv[n * f.G + c0 / f.per + of[e]] : 0.f;
+    ga[e] = in && gamma ? gamma[c0 + q * V + e] : 1.f;
+    be[e] = in && beta ? beta[c0 + q * V + e] : 0.f;
+  }
+  float both[2][V] = {};
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int p = row + k * f.rows;
+    if (!in || p >= f.S) continue;
+    Pack<V> w;
+    if (GATED) w = load<V>(gate + at + (int64_t)p * f.C);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      z[k].v[e] = (z[k].v[e] - mu[e]) * is[e];
+      float dg = 0.f;
+      d[k].v[e] = inner_gradient<GATED>(f.code, d[k].v[e], z[k].v[e], ga[e], be[e],
+                                        GATED ? w.v[e] : 0.f, &dg);
+      if (GATED) w.v[e] = dg;
+      both[0][e] += d[k].v[e];
+      both[1][e] = fmaf(d[k].v[e], z[k].v[e], both[1][e]);
+    }
+    if (GATED) store<V>(dgate + at + (int64_t)p * f.C, w);
+  }
+  channel_sums<2, V>(scratch, sums, both, q, row, on, f);
+  // dbeta's and dgamma's share of this sample
+  for (int c = threadIdx.x; c < wide; c += blockDim.x) {
+    float a = 0.f, b = 0.f;
+    for (int j = 0; j < f.split; ++j) {
+      a += sums[j * f.wide + c];
+      b += sums[(f.split + j) * f.wide + c];
+    }
+    part[n * 2 * f.C + c0 + c] = a;
+    part[n * 2 * f.C + f.C + c0 + c] = b;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float count = (float)f.S * (float)f.per;
+  for (int g = warp; g < groups; g += blockDim.x >> 5) {
+    float a = 0.f, b = 0.f;
+    for (int i = lane; i < f.per * f.split; i += 32) {
+      const int c = g * f.per + i % f.per, j = i / f.per;
+      const float w = gamma ? gamma[c0 + c] : 1.f;
+      a = fmaf(w, sums[j * f.wide + c], a);
+      b = fmaf(w, sums[(f.split + j) * f.wide + c], b);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    if (lane == 0) group[g] = make_float2(a / count, b / count);
+  }
+  __syncthreads();
+  if (!in) return;
+  float2 m[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) m[e] = group[of[e]];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int p = row + k * f.rows;
+    if (p >= f.S) continue;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      d[k].v[e] = is[e] * (ga[e] * d[k].v[e] - m[e].x - z[k].v[e] * m[e].y);
+    store<V>(dx + at + (int64_t)p * f.C, d[k]);
+  }
+}
+
 // Calls f with the activation and whether there is a gate as constants.
 template <int V>
 struct Const {
@@ -331,6 +762,78 @@ int plan(const char* what, Shape& s, int64_t N, int64_t S, int64_t C, int64_t G,
   return WXX_OK;
 }
 
+// Whether rows of `per` channels and all the given memory can be taken 4 channels at a time.
+bool fours(const void* const (&memory)[8], int64_t per) {
+  uintptr_t all = 0;
+  for (const void* p : memory) all |= reinterpret_cast<uintptr_t>(p);
+  return (all & 15) == 0 && per % 4 == 0;
+}
+
+// A group of one position in the registers of up to 32 threads, if it fits.
+bool plan_few(Few& f, int& v, int& k, const Shape& s, int code, bool four) {
+  if (s.S != 1 || s.N * s.G >= (int64_t(1) << 31)) return false;
+  v = four ? 4 : 1;
+  const int pieces = (s.per + v - 1) / v;
+  int lanes = 1;
+  while (lanes < 32 && lanes < pieces) lanes <<= 1;
+  k = 1;
+  while (k * lanes < pieces) k <<= 1;
+  if (k > 8) return false;
+  f = Few{s.N, s.C, s.G, s.per, lanes, 0, code, s.eps};
+  return true;
+}
+
+// Whole groups of a sample's positions in a block's registers, K pieces a thread at most, if they
+// fit: as wide as that allows (long pieces of a position), 256 threads, or 512 where one
+// group needs them.
+bool plan_slab(Slab& f, int& v, int& k, int& threads, const Shape& s, int code, bool four, int most,
+               int sums) {
+  if (s.S == 1 || s.S > (1 << 20)) return false;
+  v = four ? 4 : 1;
+  int unit = s.per;                                  // channels of whole groups and pieces
+  while (unit % v) unit += s.per;
+  for (threads = 256; threads <= 512; threads *= 2) {
+    int wide = 0;
+    for (int w = unit; w <= s.C + unit - 1 && w / v <= threads; w += unit) {
+      const int rows = threads / (w / v);
+      const int64_t bytes = (int64_t)(sums * (rows + 16) + 2) * w * 4;
+      if ((s.S + rows - 1) / rows > most || bytes > 48 * 1024) break;
+      wide = w;
+      // blocks enough for the SMs before pieces of more than 64 bytes
+      if (w * 4 >= 64 && s.N * ((s.C + w - 1) / w) < 2 * wxx::num_sms()) break;
+    }
+    if (wide == 0) continue;
+    const int across = wide / v;
+    int rows = threads / across;
+    if (rows > s.S) rows = (int)s.S;
+    k = (int)((s.S + rows - 1) / rows);
+    int split = threads / wide;
+    if (split > 16) split = 16;
+    if (split > rows) split = rows;
+    if (split < 1) split = 1;
+    f = Slab{s.N, (int)s.S, s.C, s.G, s.per, wide, (s.C + wide - 1) / wide, across, rows, split, code,
+             s.eps};
+    return s.N * f.spans < (int64_t(1) << 31);
+  }
+  return false;
+}
+
+template <int K>
+using Pieces = std::integral_constant<int, K>;
+template <class F>
+void with_pieces(int v, int k, F f) {
+  auto with_k = [&](auto vv) {
+    if (k <= 1) return f(vv, Pieces<1>{});
+    if (k <= 2) return f(vv, Pieces<2>{});
+    if (k <= 4) return f(vv, Pieces<4>{});
+    return f(vv, Pieces<8>{});
+  };
+  if (v == 4)
+    with_k(Pieces<4>{});
+  else
+    with_k(Pieces<1>{});
+}
+
 }  // namespace
 
 // y, mean and inv (N, G) from x (N, S, C); gamma, beta (C) and gate (like x) may be NULL.
@@ -347,6 +850,31 @@ WXX_EXPORT int wxx_group_norm(float* y, float* mean, float* inv, const float* x,
       WXX_CUDA_CHECK(cudaMemsetAsync(mean, 0, (size_t)(N * G) * sizeof(float), wxx::stream()));
       WXX_CUDA_CHECK(cudaMemsetAsync(inv, 0, (size_t)(N * G) * sizeof(float), wxx::stream()));
     }
+    return WXX_OK;
+  }
+  const bool four = fours({y, x, gate, gamma, beta, nullptr, nullptr, nullptr}, C);
+  Few few;
+  Slab slab;
+  int v, k, threads;
+  if (plan_few(few, v, k, s, activation, four && s.per % 4 == 0)) {
+    const unsigned grid = wxx::grid_for(N * G * few.lanes, kT, 32);
+    with_pieces(v, k, [&](auto vv, auto kk) {
+      constexpr int V = decltype(vv)::value, K = decltype(kk)::value;
+      auto kernel = gate ? token_kernel<V, K, true> : token_kernel<V, K, false>;
+      kernel<<<grid, kT, 0, wxx::stream()>>>(y, mean, inv, x, gate, gamma, beta, few);
+    });
+    WXX_LAUNCH_CHECK();
+    return WXX_OK;
+  }
+  if (plan_slab(slab, v, k, threads, s, activation, four, 8, 1)) {
+    const size_t bytes = ((size_t)(slab.rows + slab.split + 2) * slab.wide) * sizeof(float);
+    with_pieces(v, k, [&](auto vv, auto kk) {
+      constexpr int V = decltype(vv)::value, K = decltype(kk)::value;
+      auto kernel = gate ? slab_kernel<V, K, true> : slab_kernel<V, K, false>;
+      kernel<<<(unsigned)(N * slab.spans), threads, bytes, wxx::stream()>>>(y, mean, inv, x, gate, gamma,
+                                                                           beta, slab);
+    });
+    WXX_LAUNCH_CHECK();
     return WXX_OK;
   }
   void* part = nullptr;
@@ -385,6 +913,49 @@ WXX_EXPORT int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, f
       WXX_CUDA_CHECK(cudaMemsetAsync(dbeta, 0, (size_t)C * sizeof(float), wxx::stream()));
     }
     return WXX_OK;
+  }
+  const bool four = fours({dx, dgate, dy, x, gate, gamma, beta, nullptr}, C);
+  Few few;
+  Slab slab;
+  int v, k, threads;
+  const bool tokens = plan_few(few, v, k, s, activation, four && s.per % 4 == 0);
+  if (tokens || plan_slab(slab, v, k, threads, s, activation, four, 8, 2)) {
+    unsigned grid;
+    int64_t rows = N;
+    if (tokens) {
+      // samples under way at once: enough threads for the SMs, two samples a thread at
+      // least where there are so many
+      const int64_t row = (int64_t)G * few.lanes, most = (N + 1) / 2;
+      rows = (int64_t)wxx::num_sms() * 1024 / row;
+      if (rows > most) rows = most;
+      if (rows < 1) rows = 1;
+      few.rows = (int)rows;
+      grid = (unsigned)((rows * row + kT - 1) / kT);
+    }
+    void* scratch = nullptr;
+    if (int st = wxx_malloc(&scratch, (uint64_t)(rows * 2 * C) * sizeof(float))) return st;
+    float* part = static_cast<float*>(scratch);
+    with_pieces(v, k, [&](auto vv, auto kk) {
+      constexpr int V = decltype(vv)::value, K = decltype(kk)::value;
+      if (tokens) {
+        auto kernel = gate ? token_backward_kernel<V, K, true> : token_backward_kernel<V, K, false>;
+        kernel<<<grid, kT, 0, wxx::stream()>>>(dx, dgate, part, dy, x, gate, mean, inv, gamma, beta, few);
+      } else {
+        const size_t bytes =
+            ((size_t)(2 * (slab.rows + slab.split) + 2) * slab.wide) * sizeof(float);
+        auto kernel = gate ? slab_backward_kernel<V, K, true> : slab_backward_kernel<V, K, false>;
+        kernel<<<(unsigned)(N * slab.spans), threads, bytes, wxx::stream()>>>(
+            dx, dgate, part, dy, x, gate, mean, inv, gamma, beta, slab);
+      }
+    });
+    int st = wxx::after_launch(__FILE__, __LINE__);
+    if (st == WXX_OK) {
+      column_sums_kernel<<<(unsigned)((2 * C + 31) / 32), kT, 0, wxx::stream()>>>(dbeta, dgamma, part,
+                                                                                 rows, (int)C);
+      st = wxx::after_launch(__FILE__, __LINE__);
+    }
+    wxx_free(scratch);
+    return st;
   }
   const int64_t rows = N * s.chunks;
   void* scratch = nullptr;
