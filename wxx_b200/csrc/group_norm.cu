@@ -27,11 +27,34 @@ constexpr int kT = 256;
 
 enum Act { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
 
-// 1 / (1 + exp(-v)), good to a few ulp: exp is the library's, and infinite where the
-// quotient is 0.
-__device__ __forceinline__ float logistic(float v) { return 1.0f / (1.0f + expf(-v)); }
+// sigmoid(v) and sigmoid(-v), each good to a few ulp of itself, from e = exp(-|v|) <= 1: e = 2^y
+// 2^r with y = -|v| log2 e rounded and r what the product and the constant lost (alone y would
+// cost e |y| half ulps), so little that 2^r is 1 + r log 2; 1 + e is what the approximate
+// reciprocal takes to an ulp.  From |v| = 104 on e is 0.  (With the library's exponential and
+// division the forward over 8192 x 1024 was bound by its instructions: 28.7 us.)
+struct Sigmoid {
+  float of, rest;
+};
+__device__ __forceinline__ Sigmoid sigmoid(float v) {
+  constexpr float kC = -1.4426950408889634f;
+  constexpr float kLow = (float)(-1.4426950408889634 - (double)kC);
+  float t, r;
+  asm("min.NaN.f32 %0, %1, 0f42D00000;" : "=f"(t) : "f"(fabsf(v)));   // 104
+  const float y = t * kC;
+  const float lost = fmaf(t, kLow, fmaf(t, kC, -y));
+  const float e = fast_exp2(y) * fmaf(lost, 0.6931471805599453f, 1.0f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  const float small = e * r;
+  return v >= 0.f ? Sigmoid{r, small} : Sigmoid{small, r};
+}
 
-// GELU is the tanh form with the clamps of gelu_tanh, as x s(2 u).
+// 1 / sqrt(a) of a normal number: the approximation and one step of Newton's method.
+__device__ __forceinline__ float inverse_root(float a) {
+  const float r = rsqrtf(a);
+  return fmaf(r * 0.5f, fmaf(-a * r, r, 1.0f), r);
+}
+
+// GELU is the tanh form with the clamps of gelu_tanh, as v sigmoid(2 u).
 __device__ __forceinline__ float gelu_argument(float v) {
   return 2.0f * 0.7978845608f * (v + 0.044715f * v * v * v);
 }
@@ -39,38 +62,45 @@ __device__ __forceinline__ float gelu_argument(float v) {
 template <int ACT>
 __device__ __forceinline__ float act(float v) {
   if (ACT == kRelu) return v < 0.f ? 0.f : v;
-  if (ACT == kSilu) return v * logistic(v);
+  if (ACT == kSilu) return v * sigmoid(v).of;
   if (ACT == kGelu) {
-    const float r = v * logistic(gelu_argument(v));
+    const float r = v * sigmoid(gelu_argument(v)).of;
     return v > 10.f ? v : v < -10.f ? 0.f : r;
   }
   return v;
 }
 
+// The activation and its slope.
+struct Both {
+  float value, slope;
+};
 template <int ACT>
-__device__ __forceinline__ float slope(float v) {
-  if (ACT == kRelu) return v > 0.f ? 1.f : 0.f;
+__device__ __forceinline__ Both act_slope(float v) {
+  if (ACT == kRelu) return {v < 0.f ? 0.f : v, v > 0.f ? 1.f : 0.f};
   if (ACT == kSilu) {
-    const float p = logistic(v);
-    return p * (1.0f + v * (1.0f - p));
+    const Sigmoid p = sigmoid(v);
+    return {v * p.of, fmaf(v * p.of, p.rest, p.of)};
   }
   if (ACT == kGelu) {
-    const float p = logistic(gelu_argument(v));
-    const float r = p + v * p * (1.0f - p) * (2.0f * 0.7978845608f) * (1.0f + 0.134145f * v * v);
-    return v > 10.f ? 1.f : v < -10.f ? 0.f : r;
+    const Sigmoid p = sigmoid(gelu_argument(v));
+    const float du = (2.0f * 0.7978845608f) * fmaf(0.134145f * v, v, 1.0f), value = v * p.of;
+    const float r = fmaf(value * p.rest, du, p.of);
+    if (v > 10.f) return {v, 1.f};
+    if (v < -10.f) return {0.f, 0.f};
+    return {value, r};
   }
-  return 1.f;
+  return {v, 1.f};
 }
 
-// The same where the activation is one branch for all threads (memory-bound kernels).
+// The same where the activation is one branch for all threads.
 __device__ __forceinline__ float act(int code, float v) {
   return code == kSilu ? act<kSilu>(v) : code == kGelu ? act<kGelu>(v) : code == kRelu ? act<kRelu>(v) : v;
 }
-__device__ __forceinline__ float slope(int code, float v) {
-  return code == kSilu   ? slope<kSilu>(v)
-         : code == kGelu ? slope<kGelu>(v)
-         : code == kRelu ? slope<kRelu>(v)
-                         : 1.f;
+__device__ __forceinline__ Both act_slope(int code, float v) {
+  return code == kSilu   ? act_slope<kSilu>(v)
+         : code == kGelu ? act_slope<kGelu>(v)
+         : code == kRelu ? act_slope<kRelu>(v)
+                         : act_slope<kNone>(v);
 }
 
 template <int V>
@@ -181,7 +211,7 @@ __global__ void __launch_bounds__(kT)
   Moments m = {0.f, 0.f, 0.f};
   for (int k = 0; k < s.chunks; ++k) m = join(m, part[(n * s.chunks + k) * s.G + g]);
   mean[i] = m.mean;
-  inv[i] = 1.0f / sqrtf(m.m2 / ((float)s.S * (float)s.per) + s.eps);
+  inv[i] = inverse_root(m.m2 / ((float)s.S * (float)s.per) + s.eps);
 }
 
 template <int ACT, bool GATED>
@@ -207,9 +237,9 @@ template <int ACT, bool GATED>
 __device__ __forceinline__ float inner_gradient(float dy, float z, float gamma, float beta,
                                                 float gate, float* dgate) {
   const float v = fmaf(z, gamma, beta);
-  if (!GATED) return dy * slope<ACT>(v);
-  *dgate = dy * v * slope<ACT>(gate);
-  return dy * act<ACT>(gate);
+  const Both f = act_slope<ACT>(GATED ? gate : v);
+  *dgate = dy * v * f.slope;
+  return dy * (GATED ? f.value : f.slope);
 }
 
 // For every channel the sums of dn and dn z over a piece of a sample: part (N, chunks,
@@ -306,23 +336,33 @@ __global__ void __launch_bounds__(kT)
   }
 }
 
-// out (2, C) from rows of 2 C partial sums, in a fixed order: 32 columns by 8 parts of
-// the rows a block.  first: dbeta, then dgamma.
-__global__ void __launch_bounds__(kT)
+// out (2, C) from rows of 2 C partial sums, in a fixed order: 32 columns by 32 parts of
+// the rows a block.  First dbeta, then dgamma.
+__global__ void __launch_bounds__(1024)
     column_sums_kernel(float* __restrict__ dbeta, float* __restrict__ dgamma,
                        const float* __restrict__ part, int64_t rows, int C) {
-  __shared__ float sums[8][33];
+  __shared__ float sums[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float a = 0.f;
-  if (c < 2 * C)
-    for (int64_t r = warp; r < rows; r += 8) a += part[r * 2 * C + c];
+  if (c < 2 * C) {
+    const float* p = part + c;
+    int64_t r = warp;
+    for (; r + 96 < rows; r += 128) {
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = p[(r + 32 * k) * 2 * C];
+      a += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    for (; r < rows; r += 32) a += p[r * 2 * C];
+  }
   sums[warp][lane] = a;
   __syncthreads();
-  if (warp == 0 && c < 2 * C) {
-    for (int w = 1; w < 8; ++w) a += sums[w][lane];
-    (c < C ? dbeta[c] : dgamma[c - C]) = a;
-  }
+  float v = sums[lane][warp];                        // a warp a column now
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int own = blockIdx.x * 32 + warp;
+  if (lane == 0 && own < 2 * C) (own < C ? dbeta[own] : dgamma[own - C]) = v;
 }
 
 // ------------------------------------------------------------------ one position a sample
@@ -338,7 +378,6 @@ struct Few {
   float eps;
 };
 
-template <int K, int V>
 __device__ __forceinline__ float over_lanes(float v, int lanes) {
   for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -349,13 +388,23 @@ __global__ void __launch_bounds__(kT)
     token_kernel(float* __restrict__ y, float* __restrict__ mean, float* __restrict__ inv,
                  const float* __restrict__ x, const float* __restrict__ gate,
                  const float* __restrict__ gamma, const float* __restrict__ beta, const Few f) {
-  const unsigned total = (unsigned)(f.N * f.G), step = gridDim.x * kT / f.lanes;
-  const int lane = threadIdx.x % f.lanes;
-  for (unsigned u0 = (blockIdx.x * kT + threadIdx.x) / 32 * 32 / f.lanes; u0 < total; u0 += step) {
-    const unsigned u = u0 + threadIdx.x % 32 / f.lanes;      // a warp's groups go on together
-    const bool on = u < total;
-    const int64_t n = u / f.G;
-    const int g = (int)(u - n * f.G);
+  // a thread's group of channels, and its first sample
+  const unsigned slot = (blockIdx.x * kT + threadIdx.x) / f.lanes;
+  const int lane = threadIdx.x % f.lanes, g = slot % f.G, row = slot / f.G;
+  const bool here = row < f.rows;
+  const float share = 1.0f / (float)f.per;
+  Pack<V> ga[K], be[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * f.lanes + lane) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) ga[k].v[e] = 1.f, be[k].v[e] = 0.f;
+    if (gamma && c < f.per) ga[k] = load<V>(gamma + g * f.per + c);
+    if (beta && c < f.per) be[k] = load<V>(beta + g * f.per + c);
+  }
+  // every lane of a warp takes as many turns (rows differ by one at most)
+  for (int64_t n = row; __any_sync(0xffffffffu, here && n < f.N); n += f.rows) {
+    const bool on = here && n < f.N;
     const int64_t at = n * f.C + g * f.per;
     Pack<V> v[K], w[GATED ? K : 1];
     float sum = 0.f;
@@ -367,10 +416,12 @@ __global__ void __launch_bounds__(kT)
       for (int e = 0; e < V; ++e) v[k].v[e] = 0.f;
       if (in) v[k] = load<V>(x + at + c);
       if (GATED && in) w[k] = load<V>(gate + at + c);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int e = 0; e < V; ++e) sum += v[k].v[e];
-    }
-    const float mu = over_lanes<K, V>(sum, f.lanes) / (float)f.per;
+    const float mu = over_lanes(sum, f.lanes) * share;
     float square = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -381,24 +432,19 @@ __global__ void __launch_bounds__(kT)
         if (in) square = fmaf(v[k].v[e], v[k].v[e], square);
       }
     }
-    const float is = 1.0f / sqrtf(over_lanes<K, V>(square, f.lanes) / (float)f.per + f.eps);
+    const float is = inverse_root(fmaf(over_lanes(square, f.lanes), share, f.eps));
     if (!on) continue;
     if (lane == 0) {
-      mean[u] = mu;
-      inv[u] = is;
+      mean[n * f.G + g] = mu;
+      inv[n * f.G + g] = is;
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * f.lanes + lane) * V;
       if (c >= f.per) continue;
-      Pack<V> ga, be;
-#pragma unroll
-      for (int e = 0; e < V; ++e) ga.v[e] = 1.f, be.v[e] = 0.f;
-      if (gamma) ga = load<V>(gamma + g * f.per + c);
-      if (beta) be = load<V>(beta + g * f.per + c);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float t = fmaf(v[k].v[e] * is, ga.v[e], be.v[e]);
+        const float t = fmaf(v[k].v[e] * is, ga[k].v[e], be[k].v[e]);
         v[k].v[e] = GATED ? t * act(f.code, w[k].v[e]) : act(f.code, t);
       }
       store<V>(y + at + c, v[k]);
@@ -411,9 +457,9 @@ template <bool GATED>
 __device__ __forceinline__ float inner_gradient(int code, float dy, float z, float gamma,
                                                 float beta, float gate, float* dgate) {
   const float v = fmaf(z, gamma, beta);
-  if (!GATED) return dy * slope(code, v);
-  *dgate = dy * v * slope(code, gate);
-  return dy * act(code, gate);
+  const Both f = act_slope(code, GATED ? gate : v);
+  *dgate = dy * v * f.slope;
+  return dy * (GATED ? f.value : f.slope);
 }
 
 template <int V, int K, bool GATED>
@@ -428,6 +474,7 @@ __global__ void __launch_bounds__(kT)
   const unsigned slot = (blockIdx.x * kT + threadIdx.x) / f.lanes;
   const int lane = threadIdx.x % f.lanes, g = slot % f.G, row = slot / f.G;
   const bool here = row < f.rows;
+  const float share = 1.0f / (float)f.per;
   Pack<V> ga[K], be[K], sum_n[K], sum_z[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -473,8 +520,8 @@ __global__ void __launch_bounds__(kT)
         a += d[k].v[e];
         b = fmaf(d[k].v[e], z[k].v[e], b);
       }
-    a = over_lanes<K, V>(a, f.lanes) / (float)f.per;
-    b = over_lanes<K, V>(b, f.lanes) / (float)f.per;
+    a = over_lanes(a, f.lanes) * share;
+    b = over_lanes(b, f.lanes) * share;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * f.lanes + lane) * V;
@@ -505,28 +552,45 @@ __global__ void __launch_bounds__(kT)
 struct Slab {
   int64_t N;
   int S, C, G, per, wide, spans, across, rows, split, code;
+  bool folded;
   float eps;
 };
 
-// Sums over a block's positions of M numbers per channel: every thread's `v` (M, V), of
-// channels q V ..; out (M, split, wide): `split` partial sums of each.
+// Partial sums over a block's positions of M numbers per channel, from every thread's v (M,
+// V) of channels q V ..: (M, split, wide) numbers, at the address that is returned.  Threads
+// of a warp with the same channels add theirs first where there is a power of two of them
+// (f.folded); up to 16 rows are left as they are, more are added to f.split.
 template <int M, int V>
-__device__ __forceinline__ void channel_sums(float* scratch, float* out, const float (&v)[M][V],
-                                             int q, int row, bool on, const Slab& f) {
-  __syncthreads();                                   // whoever read out and scratch is done
+__device__ __forceinline__ const float* channel_sums(float* scratch, float (&v)[M][V], int q,
+                                                     int row, bool on, const Slab& f) {
+  int rows = f.rows;
+  if (f.folded) {
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        for (int o = 16; o >= f.across; o >>= 1) v[i][e] += __shfl_xor_sync(0xffffffffu, v[i][e], o);
+    rows = blockDim.x >> 5;
+    row = threadIdx.x >> 5;
+    on = (threadIdx.x & 31) < f.across;
+  }
+  __syncthreads();                                   // whoever read the last sums is done
   if (on)
 #pragma unroll
     for (int i = 0; i < M; ++i)
 #pragma unroll
-      for (int e = 0; e < V; ++e) scratch[(i * f.rows + row) * f.wide + q * V + e] = v[i][e];
+      for (int e = 0; e < V; ++e) scratch[(i * rows + row) * f.wide + q * V + e] = v[i][e];
   __syncthreads();
+  if (rows == f.split) return scratch;
+  float* out = scratch + M * rows * f.wide;
   for (int t = threadIdx.x; t < M * f.split * f.wide; t += blockDim.x) {
     const int c = t % f.wide, j = t / f.wide % f.split, i = t / f.wide / f.split;
     float sum = 0.f;
-    for (int r = j; r < f.rows; r += f.split) sum += scratch[(i * f.rows + r) * f.wide + c];
+    for (int r = j; r < rows; r += f.split) sum += scratch[(i * rows + r) * f.wide + c];
     out[t] = sum;
   }
   __syncthreads();
+  return out;
 }
 
 template <int V, int K, bool GATED>
@@ -535,9 +599,8 @@ __global__ void __launch_bounds__(512)
                 const float* __restrict__ x, const float* __restrict__ gate,
                 const float* __restrict__ gamma, const float* __restrict__ beta, const Slab f) {
   extern __shared__ float smem[];
-  float* scratch = smem;                             // (rows, wide)
-  float* sums = scratch + f.rows * f.wide;           // (split, wide)
-  float* group = sums + f.split * f.wide;            // (wide / per) twice
+  float* group = smem;                               // (wide / per) twice
+  float* scratch = smem + 2 * f.wide;
   const int64_t n = blockIdx.x / f.spans;
   const int c0 = blockIdx.x % f.spans * f.wide, wide = min(f.wide, f.C - c0), groups = wide / f.per;
   const int q = threadIdx.x % f.across, row = threadIdx.x / f.across;
@@ -553,11 +616,18 @@ __global__ void __launch_bounds__(512)
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float count = (float)f.S * (float)f.per;
-  auto over_groups = [&](float* to, auto finish) {
+  // a lane's values of a group are every 32nd of split * per
+  const int first_j = lane / f.per, first_c = lane % f.per, step_j = 32 / f.per, step_c = 32 % f.per;
+  auto over_groups = [&](const float* sums, float* to, auto finish) {
     for (int g = warp; g < groups; g += blockDim.x >> 5) {
       float sum = 0.f;
-      for (int i = lane; i < f.per * f.split; i += 32)
-        sum += sums[i / f.per * f.wide + g * f.per + i % f.per];
+      for (int j = first_j, c = first_c; j < f.split; j += step_j, c += step_c) {
+        if (c >= f.per) {
+          c -= f.per;
+          if (++j >= f.split) break;
+        }
+        sum += sums[j * f.wide + g * f.per + c];
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane == 0) to[g] = finish(sum / count);
@@ -572,8 +642,8 @@ __global__ void __launch_bounds__(512)
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int e = 0; e < V; ++e) part[0][e] += v[k].v[e];
-  channel_sums<1, V>(scratch, sums, part, q, row, on, f);
-  over_groups(group, [](float m) { return m; });
+  const float* sums = channel_sums<1, V>(scratch, part, q, row, on, f);
+  over_groups(sums, group, [](float m) { return m; });
   float mu[V], is[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) mu[e] = group[of[e]], part[0][e] = 0.f;
@@ -587,8 +657,8 @@ __global__ void __launch_bounds__(512)
   if (!in)
 #pragma unroll
     for (int e = 0; e < V; ++e) part[0][e] = 0.f;
-  channel_sums<1, V>(scratch, sums, part, q, row, on, f);
-  over_groups(group + groups, [&](float m) { return 1.0f / sqrtf(m + f.eps); });
+  sums = channel_sums<1, V>(scratch, part, q, row, on, f);
+  over_groups(sums, group + groups, [&](float m) { return inverse_root(m + f.eps); });
   for (int g = threadIdx.x; g < groups; g += blockDim.x) {
     mean[n * f.G + c0 / f.per + g] = group[g];
     inv[n * f.G + c0 / f.per + g] = group[groups + g];
@@ -625,9 +695,8 @@ __global__ void __launch_bounds__(512)
                          const float* __restrict__ gamma, const float* __restrict__ beta,
                          const Slab f) {
   extern __shared__ float smem[];
-  float* scratch = smem;                             // (2, rows, wide)
-  float* sums = scratch + 2 * f.rows * f.wide;       // (2, split, wide)
-  float2* group = reinterpret_cast<float2*>(sums + 2 * f.split * f.wide);   // (wide / per)
+  float2* group = reinterpret_cast<float2*>(smem);   // (wide / per)
+  float* scratch = smem + 2 * f.wide;
   const int64_t n = blockIdx.x / f.spans;
   const int c0 = blockIdx.x % f.spans * f.wide, wide = min(f.wide, f.C - c0), groups = wide / f.per;
   const int q = threadIdx.x % f.across, row = threadIdx.x / f.across;
@@ -673,7 +742,7 @@ __global__ void __launch_bounds__(512)
     }
     if (GATED) store<V>(dgate + at + (int64_t)p * f.C, w);
   }
-  channel_sums<2, V>(scratch, sums, both, q, row, on, f);
+  const float* sums = channel_sums<2, V>(scratch, both, q, row, on, f);
   // dbeta's and dgamma's share of this sample
   for (int c = threadIdx.x; c < wide; c += blockDim.x) {
     float a = 0.f, b = 0.f;
@@ -688,8 +757,12 @@ __global__ void __launch_bounds__(512)
   const float count = (float)f.S * (float)f.per;
   for (int g = warp; g < groups; g += blockDim.x >> 5) {
     float a = 0.f, b = 0.f;
-    for (int i = lane; i < f.per * f.split; i += 32) {
-      const int c = g * f.per + i % f.per, j = i / f.per;
+    for (int j = lane / f.per, k = lane % f.per; j < f.split; j += 32 / f.per, k += 32 % f.per) {
+      if (k >= f.per) {
+        k -= f.per;
+        if (++j >= f.split) break;
+      }
+      const int c = g * f.per + k;
       const float w = gamma ? gamma[c0 + c] : 1.f;
       a = fmaf(w, sums[j * f.wide + c], a);
       b = fmaf(w, sums[(f.split + j) * f.wide + c], b);
@@ -783,6 +856,17 @@ bool plan_few(Few& f, int& v, int& k, const Shape& s, int code, bool four) {
   return true;
 }
 
+// Samples under way at once: two a thread (forward, least = 1), or (backward, where each costs
+// a partial sum of every channel) threads enough for the SMs, and `least` samples a thread
+// where there are so many.
+unsigned few_grid(Few& f, int least) {
+  const int64_t row = (int64_t)f.G * f.lanes, most = (f.N + least - 1) / least;
+  int64_t rows = least == 1 ? (f.N + 1) / 2 : ((int64_t)wxx::num_sms() * 1024 + row - 1) / row;
+  if (rows > most) rows = most;
+  f.rows = (int)rows;
+  return (unsigned)((rows * row + kT - 1) / kT);
+}
+
 // Whole groups of a sample's positions in a block's registers, K pieces a thread at most, if they
 // fit: as wide as that allows (long pieces of a position), 256 threads, or 512 where one
 // group needs them.
@@ -807,15 +891,24 @@ bool plan_slab(Slab& f, int& v, int& k, int& threads, const Shape& s, int code, 
     int rows = threads / across;
     if (rows > s.S) rows = (int)s.S;
     k = (int)((s.S + rows - 1) / rows);
-    int split = threads / wide;
-    if (split > 16) split = 16;
-    if (split > rows) split = rows;
-    if (split < 1) split = 1;
-    f = Slab{s.N, (int)s.S, s.C, s.G, s.per, wide, (s.C + wide - 1) / wide, across, rows, split, code,
-             s.eps};
+    const bool folded = across <= 16 && (across & (across - 1)) == 0;
+    int split = folded ? threads / 32 : rows;
+    if (split > 16) {
+      split = threads / wide;
+      if (split > 16) split = 16;
+      if (split < 1) split = 1;
+    }
+    f = Slab{s.N,    (int)s.S, s.C,  s.G,   s.per, wide,  (s.C + wide - 1) / wide,
+             across, rows,     split, code, folded, s.eps};
     return s.N * f.spans < (int64_t(1) << 31);
   }
   return false;
+}
+
+// Shared memory of a block: the groups' results, the threads' sums and partial sums of them.
+size_t slab_bytes(const Slab& f, int threads, int sums) {
+  const size_t rows = f.folded ? threads / 32 : f.rows;
+  return (2 + sums * (rows + f.split)) * f.wide * sizeof(float);
 }
 
 template <int K>
@@ -857,7 +950,7 @@ WXX_EXPORT int wxx_group_norm(float* y, float* mean, float* inv, const float* x,
   Slab slab;
   int v, k, threads;
   if (plan_few(few, v, k, s, activation, four && s.per % 4 == 0)) {
-    const unsigned grid = wxx::grid_for(N * G * few.lanes, kT, 32);
+    const unsigned grid = few_grid(few, 1);
     with_pieces(v, k, [&](auto vv, auto kk) {
       constexpr int V = decltype(vv)::value, K = decltype(kk)::value;
       auto kernel = gate ? token_kernel<V, K, true> : token_kernel<V, K, false>;
@@ -867,7 +960,7 @@ WXX_EXPORT int wxx_group_norm(float* y, float* mean, float* inv, const float* x,
     return WXX_OK;
   }
   if (plan_slab(slab, v, k, threads, s, activation, four, 8, 1)) {
-    const size_t bytes = ((size_t)(slab.rows + slab.split + 2) * slab.wide) * sizeof(float);
+    const size_t bytes = slab_bytes(slab, threads, 1);
     with_pieces(v, k, [&](auto vv, auto kk) {
       constexpr int V = decltype(vv)::value, K = decltype(kk)::value;
       auto kernel = gate ? slab_kernel<V, K, true> : slab_kernel<V, K, false>;
@@ -920,18 +1013,8 @@ WXX_EXPORT int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, f
   int v, k, threads;
   const bool tokens = plan_few(few, v, k, s, activation, four && s.per % 4 == 0);
   if (tokens || plan_slab(slab, v, k, threads, s, activation, four, 8, 2)) {
-    unsigned grid;
-    int64_t rows = N;
-    if (tokens) {
-      // samples under way at once: enough threads for the SMs, two samples a thread at
-      // least where there are so many
-      const int64_t row = (int64_t)G * few.lanes, most = (N + 1) / 2;
-      rows = (int64_t)wxx::num_sms() * 1024 / row;
-      if (rows > most) rows = most;
-      if (rows < 1) rows = 1;
-      few.rows = (int)rows;
-      grid = (unsigned)((rows * row + kT - 1) / kT);
-    }
+    const unsigned grid = tokens ? few_grid(few, 2) : 0;
+    const int64_t rows = tokens ? few.rows : N;
     void* scratch = nullptr;
     if (int st = wxx_malloc(&scratch, (uint64_t)(rows * 2 * C) * sizeof(float))) return st;
     float* part = static_cast<float*>(scratch);
@@ -941,8 +1024,7 @@ WXX_EXPORT int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, f
         auto kernel = gate ? token_backward_kernel<V, K, true> : token_backward_kernel<V, K, false>;
         kernel<<<grid, kT, 0, wxx::stream()>>>(dx, dgate, part, dy, x, gate, mean, inv, gamma, beta, few);
       } else {
-        const size_t bytes =
-            ((size_t)(2 * (slab.rows + slab.split) + 2) * slab.wide) * sizeof(float);
+        const size_t bytes = slab_bytes(slab, threads, 2);
         auto kernel = gate ? slab_backward_kernel<V, K, true> : slab_backward_kernel<V, K, false>;
         kernel<<<(unsigned)(N * slab.spans), threads, bytes, wxx::stream()>>>(
             dx, dgate, part, dy, x, gate, mean, inv, gamma, beta, slab);
@@ -950,7 +1032,7 @@ WXX_EXPORT int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, f
     });
     int st = wxx::after_launch(__FILE__, __LINE__);
     if (st == WXX_OK) {
-      column_sums_kernel<<<(unsigned)((2 * C + 31) / 32), kT, 0, wxx::stream()>>>(dbeta, dgamma, part,
+      column_sums_kernel<<<(unsigned)((2 * C + 31) / 32), 1024, 0, wxx::stream()>>>(dbeta, dgamma, part,
                                                                                  rows, (int)C);
       st = wxx::after_launch(__FILE__, __LINE__);
     }
@@ -983,7 +1065,7 @@ WXX_EXPORT int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, f
     st = wxx::after_launch(__FILE__, __LINE__);
   }
   if (st == WXX_OK) {
-    column_sums_kernel<<<(unsigned)((2 * C + 31) / 32), kT, 0, wxx::stream()>>>(dbeta, dgamma, part,
+    column_sums_kernel<<<(unsigned)((2 * C + 31) / 32), 1024, 0, wxx::stream()>>>(dbeta, dgamma, part,
                                                                                rows, (int)C);
     st = wxx::after_launch(__FILE__, __LINE__);
   }

@@ -962,33 +962,83 @@ __global__ void __launch_bounds__(kT)
   }
 }
 
-// One position a sequence: a block per sequence, head and 32 columns of the state.
+// One position a sequence: a block per sequence, head and 16 V columns of the state, V columns
+// a thread (16 threads a row) and every 16th row.  Bound by the state's read and write; a
+// thread's loads of up to 4 rows are under way together.
+template <int V>
 __global__ void __launch_bounds__(kT)
     step_kernel(float* __restrict__ o, float* __restrict__ state, const float* __restrict__ q,
                 int64_t q_ld, const float* __restrict__ k, int64_t k_ld,
                 const float* __restrict__ v, int64_t v_ld, const float* __restrict__ log_decay,
                 int H, int dk, int dv, float scale) {
-  __shared__ float part[8][32];
-  const int slices = (dv + 31) / 32;
+  constexpr int kRows = 16, kAhead = 4;
+  __shared__ float part[kT / 32][16 * V];
+  const int slices = (dv + 16 * V - 1) / (16 * V);
   const int slice = blockIdx.x % slices, h = blockIdx.x / slices % H;
   const int64_t b = blockIdx.x / slices / H;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = slice * 32 + lane;
-  const Decay l(log_decay[h]);
-  float* S = state + (b * H + h) * dk * dv;
-  float sum = 0.f;
-  if (c < dv) {
-    const float z = v[b * v_ld + h * dv + c];
-    for (int p = warp; p < dk; p += 8) {
-      const float now = fmaf(k[b * k_ld + h * dk + p], z, l(S[(int64_t)p * dv + c]));
-      S[(int64_t)p * dv + c] = now;
-      sum = fmaf(q[b * q_ld + h * dk + p], now, sum);
+  const int row = threadIdx.x / 16, c = slice * 16 * V + threadIdx.x % 16 * V;
+  float* S = state + (b * H + h) * dk * dv + c;
+  const float *qh = q + b * q_ld + h * dk, *kh = k + b * k_ld + h * dk;
+  const bool in = c < dv;
+  float z[V], sum[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) sum[e] = 0.f;
+  for (int p0 = row; p0 < dk; p0 += kRows * kAhead) {
+    float now[kAhead][V], x[kAhead], y[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int p = p0 + i * kRows;
+      const bool here = in && p < dk;
+      x[i] = here ? qh[p] : 0.f;
+      y[i] = here ? kh[p] : 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) now[i][e] = 0.f;
+      if (!here) continue;
+      if constexpr (V == 4) {
+        const float4 t = *reinterpret_cast<const float4*>(S + (int64_t)p * dv);
+        now[i][0] = t.x, now[i][1] = t.y, now[i][2] = t.z, now[i][3] = t.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) now[i][e] = S[(int64_t)p * dv + e];
+      }
+    }
+    if (p0 == row) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[e] = in ? v[b * v_ld + h * dv + c + e] : 0.f;
+    }
+    const Decay l(log_decay[h]);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int p = p0 + i * kRows;
+      if (!in || p >= dk) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        now[i][e] = fmaf(y[i], z[e], l(now[i][e]));
+        sum[e] = fmaf(x[i], now[i][e], sum[e]);
+      }
+      if constexpr (V == 4) {
+        *reinterpret_cast<float4*>(S + (int64_t)p * dv) =
+            make_float4(now[i][0], now[i][1], now[i][2], now[i][3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) S[(int64_t)p * dv + e] = now[i][e];
+      }
     }
   }
-  part[warp][lane] = sum;
+  // over a warp's two rows, then over the warps
+  const int warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
+    if ((threadIdx.x & 16) == 0) part[warp][threadIdx.x % 16 * V + e] = sum[e];
+  }
   __syncthreads();
-  if (warp == 0 && c < dv) {
-    for (int w = 1; w < 8; ++w) sum += part[w][lane];
-    o[(b * H + h) * dv + c] = scale * sum;
+  const int r = slice * 16 * V + threadIdx.x;
+  if (threadIdx.x < 16 * V && r < dv) {
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kT / 32; ++w) all += part[w][threadIdx.x];
+    o[(b * H + h) * dv + r] = scale * all;
   }
 }
 
@@ -997,7 +1047,7 @@ int check_sizes(const char* what, int64_t B, int64_t T, int64_t H, int64_t dk, i
   WXX_REQUIRE(dk <= 256 && dv <= 256, "%s: heads of %lld and %lld channels (256 at most)", what,
               (long long)dk, (long long)dv);
   WXX_REQUIRE(T < (int64_t(1) << 31) - 256 && H < (int64_t(1) << 22) &&
-                  B * H * 8 < (int64_t(1) << 31),
+                  B * H * 16 < (int64_t(1) << 31),
               "%s: too many positions, sequences or heads", what);
   return WXX_OK;
 }
@@ -1171,7 +1221,10 @@ WXX_EXPORT int wxx_linear_attention_step(float* o, float* state, const float* q,
   WXX_REQUIRE_INIT();
   if (int st = check_sizes("wxx_linear_attention_step", B, 1, H, dk, dv)) return st;
   if (B * H * dv == 0) return WXX_OK;
-  step_kernel<<<(unsigned)(B * H * ((dv + 31) / 32)), kT, 0, wxx::stream()>>>(
+  const bool fours = dv % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15) == 0;
+  auto kernel = fours ? step_kernel<4> : step_kernel<1>;
+  const int64_t wide = fours ? 64 : 16;
+  kernel<<<(unsigned)(B * H * ((dv + wide - 1) / wide)), kT, 0, wxx::stream()>>>(
       o, state, q, q_ld, k, k_ld, v, v_ld, log_decay, (int)H, (int)dk, (int)dv, scale);
   WXX_LAUNCH_CHECK();
   return WXX_OK;

@@ -21,7 +21,20 @@ namespace {
 constexpr int kT = 256;
 constexpr int kMostPairs = 256;
 constexpr int kSinCos = 4096;        // pairs of a block, at most (32 KB)
-constexpr int kElements = 8192;      // channels of a block's positions, about
+constexpr int kElements = 4096;      // channels of a block's positions, about
+
+// n / d for n < 2^31 as a product: d <= 2^s, m = ceil(2^(31 + s) / d) < 2^32.
+struct Divider {
+  unsigned m, s;
+  static Divider of(unsigned d) {
+    unsigned s = 0;
+    while ((1ull << s) < d) ++s;
+    return {(unsigned)(((1ull << (31 + s)) + d - 1) / d), 31 + s};
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return (int)(((unsigned long long)(unsigned)n * m) >> s);
+  }
+};
 
 struct Turns {
   double per[kMostPairs];            // full turns a position, per pair
@@ -37,6 +50,7 @@ struct Shape {
   int tiles;                         // blocks of a sequence
   float gain;                        // m
   float sign;                        // 1, or -1: the gradient
+  Divider by_pairs, by_row, by_items;    // pairs of a head, items of a position and a head
 };
 
 // cos and sin of `turns` full turns: the quarter taken off in 64 bits, so that the
@@ -95,7 +109,7 @@ __global__ void __launch_bounds__(kT)
   const int b = blockIdx.x / s.tiles, t0 = (blockIdx.x % s.tiles) * s.at_once;
   const int n = min(s.at_once, s.T - t0), pairs = s.r / 2;
   for (int e = threadIdx.x; e < n * pairs; e += kT) {
-    const int at = e / pairs, i = e - at * pairs;
+    const int at = s.by_pairs(e), i = e - at * pairs;
     int64_t p = s.offset;
     p += s.positions ? (int64_t)s.positions[b * s.p_bs + t0 + at] : (int64_t)(t0 + at);
     const float2 cs = cos_sin((double)p * turns.per[i]);
@@ -107,30 +121,43 @@ __global__ void __launch_bounds__(kT)
   const int row = s.heads * items, D = s.heads * s.d;
   const float* xb = x + b * s.x_bs + t0 * s.x_ts;
   float* yb = y + ((int64_t)b * s.T + t0) * D;
-  for (int e = threadIdx.x; e < n * row; e += kT) {
-    const int at = e / row, h = (e - at * row) / items, k = e - at * row - h * items;
-    const float* from = xb + at * s.x_ts + h * s.d;
-    float* to = yb + (int64_t)at * D + h * s.d;
-    const float2* cs = table + at * pairs + k * kPairs;
-    if (k >= turned) {
-      const int c = s.r + (k - turned) * V;
-      store<V>(to + c, load<V>(from + c));
-    } else if (APART) {
-      Pack<V> p = load<V>(from + k * V), q = load<V>(from + pairs + k * V);
+  // U items under way together
+  constexpr int U = V == 4 ? 2 : 4, kBoth = APART || V == 1 ? 2 : 1;
+  for (int e0 = threadIdx.x; e0 < n * row; e0 += U * kT) {
+    Pack<V> p[U][kBoth];
+    const float2* cs[U];
+    float* to[U];
+    int apart[U];                    // of the item's two packs; 0: copied or absent
+    bool here[U];
 #pragma unroll
-      for (int i = 0; i < V; ++i) turn(p.v[i], q.v[i], cs[i]);
-      store<V>(to + k * V, p);
-      store<V>(to + pairs + k * V, q);
-    } else if (V == 1) {
-      float p = from[2 * k], q = from[2 * k + 1];
-      turn(p, q, cs[0]);
-      to[2 * k] = p;
-      to[2 * k + 1] = q;
-    } else {
-      Pack<V> p = load<V>(from + k * V);
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kT;
+      here[u] = e < n * row;
+      if (!here[u]) continue;
+      const int at = s.by_row(e), h = s.by_items(e - at * row), k = e - at * row - h * items;
+      const bool turns = k < turned;
+      const int c = turns ? (APART ? k * V : 2 * k * kPairs) : s.r + (k - turned) * V;
+      const float* from = xb + at * s.x_ts + h * s.d + c;
+      to[u] = yb + (int64_t)at * D + h * s.d + c;
+      cs[u] = table + at * pairs + k * kPairs;
+      apart[u] = turns ? (APART ? pairs : 1) : 0;
+      p[u][0] = load<V>(from);
+      if (kBoth == 2 && turns) p[u][kBoth - 1] = load<V>(from + apart[u]);
+    }
 #pragma unroll
-      for (int i = 0; i + 1 < V; i += 2) turn(p.v[i], p.v[i + 1], cs[i / 2]);
-      store<V>(to + k * V, p);
+    for (int u = 0; u < U; ++u) {
+      if (!here[u]) continue;
+      if (apart[u]) {
+        if (kBoth == 2) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) turn(p[u][0].v[i], p[u][kBoth - 1].v[i], cs[u][i]);
+          store<V>(to[u] + apart[u], p[u][kBoth - 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i + 1 < V; i += 2) turn(p[u][0].v[i], p[u][0].v[i + 1], cs[u][i / 2]);
+        }
+      }
+      store<V>(to[u], p[u][0]);
     }
   }
 }
@@ -179,8 +206,6 @@ WXX_EXPORT int wxx_rotary(float* y, const float* x, int64_t x_bs, int64_t x_ts,
   if (at_once > T) at_once = T;
   const int64_t tiles = (T + at_once - 1) / at_once;
   WXX_REQUIRE(B * tiles < (int64_t(1) << 31), "wxx_rotary: too many positions");
-  Shape s{x_bs, x_ts, positions, p_bs, offset, (int)T, (int)heads, (int)d, r, (int)at_once,
-          (int)tiles, gain, back ? -1.0f : 1.0f};
   // Channels at a time: as many as divide a head's parts and every row's alignment.
   const uint64_t address = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y);
   auto fits = [&](int v) {
@@ -188,6 +213,10 @@ WXX_EXPORT int wxx_rotary(float* y, const float* x, int64_t x_bs, int64_t x_ts,
            (apart ? r / 2 : r) % v == 0;
   };
   const int v = fits(4) ? 4 : fits(2) ? 2 : 1;
+  const int kept = (int)d - r, items = (apart || v == 1 ? r / 2 / v : r / v) + kept / v;
+  const Shape s{x_bs, x_ts, positions, p_bs, offset, (int)T, (int)heads, (int)d, r, (int)at_once,
+                (int)tiles, gain, back ? -1.0f : 1.0f, Divider::of((unsigned)(r > 1 ? r / 2 : 1)),
+                Divider::of((unsigned)(heads * items)), Divider::of((unsigned)items)};
   const unsigned grid = (unsigned)(B * tiles);
   if (apart)
     launch<true>(v, grid, y, x, table, s);
