@@ -35,17 +35,25 @@ enum Act { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
 struct Sigmoid {
   float of, rest;
 };
-__device__ __forceinline__ Sigmoid sigmoid(float v) {
+// For two numbers, so that products and sums go in pairs.
+__device__ __forceinline__ void sigmoid2(float v0, float v1, Sigmoid& s0, Sigmoid& s1) {
   constexpr float kC = -1.4426950408889634f;
   constexpr float kLow = (float)(-1.4426950408889634 - (double)kC);
-  float t, r;
-  asm("min.NaN.f32 %0, %1, 0f42D00000;" : "=f"(t) : "f"(fabsf(v)));   // 104
-  const float y = t * kC;
-  const float lost = fmaf(t, kLow, fmaf(t, kC, -y));
-  const float e = fast_exp2(y) * fmaf(lost, 0.6931471805599453f, 1.0f);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  const float small = e * r;
-  return v >= 0.f ? Sigmoid{r, small} : Sigmoid{small, r};
+  constexpr float kLog2 = 0.6931471805599453f;
+  float t0, t1, y0, y1, l0, l1, e0, e1, d0, d1, r0, r1, m0, m1;
+  asm("min.NaN.f32 %0, %1, 0f42D00000;" : "=f"(t0) : "f"(fabsf(v0)));   // 104
+  asm("min.NaN.f32 %0, %1, 0f42D00000;" : "=f"(t1) : "f"(fabsf(v1)));
+  mul2(y0, y1, t0, t1, kC, kC);
+  fma2(l0, l1, t0, t1, kC, kC, -y0, -y1);
+  fma2(l0, l1, t0, t1, kLow, kLow, l0, l1);
+  fma2(l0, l1, l0, l1, kLog2, kLog2, 1.0f, 1.0f);
+  mul2(e0, e1, fast_exp2(y0), fast_exp2(y1), l0, l1);
+  add2(d0, d1, e0, e1, 1.0f, 1.0f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(d0));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(d1));
+  mul2(m0, m1, e0, e1, r0, r1);
+  s0 = v0 >= 0.f ? Sigmoid{r0, m0} : Sigmoid{m0, r0};
+  s1 = v1 >= 0.f ? Sigmoid{r1, m1} : Sigmoid{m1, r1};
 }
 
 // 1 / sqrt(a) of a normal number: the approximation and one step of Newton's method.
@@ -55,52 +63,99 @@ __device__ __forceinline__ float inverse_root(float a) {
 }
 
 // GELU is the tanh form with the clamps of gelu_tanh, as v sigmoid(2 u).
-__device__ __forceinline__ float gelu_argument(float v) {
-  return 2.0f * 0.7978845608f * (v + 0.044715f * v * v * v);
+__device__ __forceinline__ void gelu_arguments(float v0, float v1, float& u0, float& u1) {
+  constexpr float k2C = 2.0f * 0.7978845608f;
+  mul2(u0, u1, v0, v1, v0, v1);
+  fma2(u0, u1, u0, u1, 0.044715f, 0.044715f, 1.0f, 1.0f);
+  mul2(u0, u1, u0, u1, v0, v1);
+  mul2(u0, u1, u0, u1, k2C, k2C);
+}
+__device__ __forceinline__ float clamped(float v, float high, float middle, float low) {
+  return v > 10.f ? high : v < -10.f ? low : middle;
 }
 
+// The activations of two numbers, in place.
 template <int ACT>
-__device__ __forceinline__ float act(float v) {
-  if (ACT == kRelu) return v < 0.f ? 0.f : v;
-  if (ACT == kSilu) return v * sigmoid(v).of;
-  if (ACT == kGelu) {
-    const float r = v * sigmoid(gelu_argument(v)).of;
-    return v > 10.f ? v : v < -10.f ? 0.f : r;
+__device__ __forceinline__ void act2(float& v0, float& v1) {
+  if (ACT == kRelu) {
+    v0 = v0 < 0.f ? 0.f : v0;
+    v1 = v1 < 0.f ? 0.f : v1;
+  } else if (ACT != kNone) {
+    float u0 = v0, u1 = v1;
+    Sigmoid p0, p1;
+    if (ACT == kGelu) gelu_arguments(v0, v1, u0, u1);
+    sigmoid2(u0, u1, p0, p1);
+    mul2(u0, u1, v0, v1, p0.of, p1.of);
+    v0 = ACT == kGelu ? clamped(v0, v0, u0, 0.f) : u0;
+    v1 = ACT == kGelu ? clamped(v1, v1, u1, 0.f) : u1;
   }
-  return v;
 }
 
-// The activation and its slope.
-struct Both {
-  float value, slope;
-};
+// The activations of two numbers, in place, and their slopes.
 template <int ACT>
-__device__ __forceinline__ Both act_slope(float v) {
-  if (ACT == kRelu) return {v < 0.f ? 0.f : v, v > 0.f ? 1.f : 0.f};
-  if (ACT == kSilu) {
-    const Sigmoid p = sigmoid(v);
-    return {v * p.of, fmaf(v * p.of, p.rest, p.of)};
+__device__ __forceinline__ void act_slope2(float& v0, float& v1, float& s0, float& s1) {
+  s0 = s1 = 1.f;
+  if (ACT == kRelu) {
+    s0 = v0 > 0.f ? 1.f : 0.f;
+    s1 = v1 > 0.f ? 1.f : 0.f;
+    v0 = v0 < 0.f ? 0.f : v0;
+    v1 = v1 < 0.f ? 0.f : v1;
+  } else if (ACT == kSilu) {
+    Sigmoid p0, p1;
+    sigmoid2(v0, v1, p0, p1);
+    mul2(v0, v1, v0, v1, p0.of, p1.of);
+    fma2(s0, s1, v0, v1, p0.rest, p1.rest, p0.of, p1.of);
+  } else if (ACT == kGelu) {
+    constexpr float k2C = 2.0f * 0.7978845608f;
+    Sigmoid p0, p1;
+    float u0, u1, w0, w1;
+    gelu_arguments(v0, v1, u0, u1);
+    sigmoid2(u0, u1, p0, p1);
+    mul2(u0, u1, v0, v1, v0, v1);
+    fma2(u0, u1, u0, u1, 0.134145f * k2C, 0.134145f * k2C, k2C, k2C);     // of the argument
+    mul2(w0, w1, v0, v1, p0.of, p1.of);
+    mul2(u0, u1, u0, u1, p0.rest, p1.rest);
+    fma2(s0, s1, w0, w1, u0, u1, p0.of, p1.of);
+    s0 = clamped(v0, 1.f, s0, 0.f);
+    s1 = clamped(v1, 1.f, s1, 0.f);
+    v0 = clamped(v0, v0, w0, 0.f);
+    v1 = clamped(v1, v1, w1, 0.f);
   }
-  if (ACT == kGelu) {
-    const Sigmoid p = sigmoid(gelu_argument(v));
-    const float du = (2.0f * 0.7978845608f) * fmaf(0.134145f * v, v, 1.0f), value = v * p.of;
-    const float r = fmaf(value * p.rest, du, p.of);
-    if (v > 10.f) return {v, 1.f};
-    if (v < -10.f) return {0.f, 0.f};
-    return {value, r};
-  }
-  return {v, 1.f};
 }
 
-// The same where the activation is one branch for all threads.
-__device__ __forceinline__ float act(int code, float v) {
-  return code == kSilu ? act<kSilu>(v) : code == kGelu ? act<kGelu>(v) : code == kRelu ? act<kRelu>(v) : v;
+// For V numbers where the activation is one branch for all threads.
+template <int ACT, int V>
+__device__ __forceinline__ void act_all(float (&v)[V]) {
+  float unused = 0.f;
+#pragma unroll
+  for (int e = 0; e < V; e += 2) act2<ACT>(v[e], e + 1 < V ? v[e + 1] : unused);
 }
-__device__ __forceinline__ Both act_slope(int code, float v) {
-  return code == kSilu   ? act_slope<kSilu>(v)
-         : code == kGelu ? act_slope<kGelu>(v)
-         : code == kRelu ? act_slope<kRelu>(v)
-                         : act_slope<kNone>(v);
+template <int V>
+__device__ __forceinline__ void act_all(int code, float (&v)[V]) {
+  if (code == kSilu)
+    act_all<kSilu, V>(v);
+  else if (code == kGelu)
+    act_all<kGelu, V>(v);
+  else if (code == kRelu)
+    act_all<kRelu, V>(v);
+}
+template <int ACT, int V>
+__device__ __forceinline__ void act_slope_all(float (&v)[V], float (&s)[V]) {
+  float unused = 0.f, none;
+#pragma unroll
+  for (int e = 0; e < V; e += 2)
+    act_slope2<ACT>(v[e], e + 1 < V ? v[e + 1] : unused, s[e], e + 1 < V ? s[e + 1] : none);
+}
+template <int V>
+__device__ __forceinline__ void act_slope_all(int code, float (&v)[V], float (&s)[V]) {
+  if (code == kSilu)
+    act_slope_all<kSilu, V>(v, s);
+  else if (code == kGelu)
+    act_slope_all<kGelu, V>(v, s);
+  else if (code == kRelu)
+    act_slope_all<kRelu, V>(v, s);
+  else
+    act_slope_all<kNone, V>(v, s);
 }
 
 template <int V>
@@ -214,12 +269,12 @@ __global__ void __launch_bounds__(kT)
   inv[i] = inverse_root(m.m2 / ((float)s.S * (float)s.per) + s.eps);
 }
 
-template <int ACT, bool GATED>
+template <bool GATED>
 __global__ void __launch_bounds__(kT)
     apply_kernel(float* __restrict__ y, const float* __restrict__ x,
                  const float* __restrict__ gate, const float* __restrict__ mean,
                  const float* __restrict__ inv, const float* __restrict__ gamma,
-                 const float* __restrict__ beta, const Shape s) {
+                 const float* __restrict__ beta, const Shape s, const int code) {
   const int64_t sample = s.S * s.C, total = s.N * sample;
   for (int64_t i = (int64_t)blockIdx.x * kT + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * kT) {
@@ -227,30 +282,41 @@ __global__ void __launch_bounds__(kT)
     const int c = (int)((i - n * sample) % s.C);
     const int64_t g = n * s.G + c / s.per;
     const float z = (x[i] - mean[g]) * inv[g];
-    const float v = fmaf(z, gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f);
-    y[i] = GATED ? v * act<ACT>(gate[i]) : act<ACT>(v);
+    const float normal = fmaf(z, gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f);
+    float v[1] = {GATED ? gate[i] : normal};
+    act_all<1>(code, v);
+    y[i] = GATED ? normal * v[0] : v[0];
   }
 }
 
-// The gradient of n at one place, and where GATED that of the gate.
-template <int ACT, bool GATED>
-__device__ __forceinline__ float inner_gradient(float dy, float z, float gamma, float beta,
-                                                float gate, float* dgate) {
-  const float v = fmaf(z, gamma, beta);
-  const Both f = act_slope<ACT>(GATED ? gate : v);
-  *dgate = dy * v * f.slope;
-  return dy * (GATED ? f.value : f.slope);
+// From dy the gradients of n and, where GATED, of the gate (in its place), at V places.
+template <int V, bool GATED>
+__device__ __forceinline__ void inner_gradient(int code, float (&d)[V], const float (&z)[V],
+                                               const float (&gamma)[V], const float (&beta)[V],
+                                               float (&gate)[V]) {
+  float n[V], value[V], slope[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    n[e] = fmaf(z[e], gamma[e], beta[e]);
+    value[e] = GATED ? gate[e] : n[e];
+  }
+  act_slope_all<V>(code, value, slope);
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if (GATED) gate[e] = d[e] * n[e] * slope[e];
+    d[e] *= GATED ? value[e] : slope[e];
+  }
 }
 
 // For every channel the sums of dn and dn z over a piece of a sample: part (N, chunks,
 // 2, C).
-template <int ACT, bool GATED>
+template <bool GATED>
 __global__ void __launch_bounds__(kT)
     channel_sums_kernel(float* __restrict__ part, const float* __restrict__ dy,
                         const float* __restrict__ x, const float* __restrict__ gate,
                         const float* __restrict__ mean, const float* __restrict__ inv,
                         const float* __restrict__ gamma, const float* __restrict__ beta,
-                        const Shape s) {
+                        const Shape s, const int code) {
   __shared__ float sums[2][kT];
   const int64_t n = blockIdx.x / s.chunks;
   const int64_t p0 = (blockIdx.x % s.chunks) * s.piece;
@@ -263,15 +329,14 @@ __global__ void __launch_bounds__(kT)
     if (l.row < l.rows && c < s.C) {
       const int64_t g = n * s.G + c / s.per;
       const float mu = mean[g], is = inv[g];
-      const float ga = gamma ? gamma[c] : 1.f, be = beta ? beta[c] : 0.f;
+      const float ga[1] = {gamma ? gamma[c] : 1.f}, be[1] = {beta ? beta[c] : 0.f};
       for (int64_t p = p0 + l.row; p < p1; p += l.rows) {
         const int64_t i = at + p * s.C + c;
-        const float z = (x[i] - mu) * is;
-        float unused;
-        const float dn = inner_gradient<ACT, GATED>(dy[i], z, ga, be, GATED ? gate[i] : 0.f,
-                                                    &unused);
-        a += dn;
-        b = fmaf(dn, z, b);
+        const float z[1] = {(x[i] - mu) * is};
+        float dn[1] = {dy[i]}, w[1] = {GATED ? gate[i] : 0.f};
+        inner_gradient<1, GATED>(code, dn, z, ga, be, w);
+        a += dn[0];
+        b = fmaf(dn[0], z[0], b);
       }
     }
     sums[0][threadIdx.x] = a;
@@ -311,28 +376,27 @@ __global__ void __launch_bounds__(kT)
   sums[i] = make_float2(a / count, b / count);
 }
 
-template <int ACT, bool GATED>
+template <bool GATED>
 __global__ void __launch_bounds__(kT)
     input_gradient_kernel(float* __restrict__ dx, float* __restrict__ dgate,
                           const float* __restrict__ dy, const float* __restrict__ x,
                           const float* __restrict__ gate, const float* __restrict__ mean,
                           const float* __restrict__ inv, const float* __restrict__ gamma,
                           const float* __restrict__ beta, const float2* __restrict__ sums,
-                          const Shape s) {
+                          const Shape s, const int code) {
   const int64_t sample = s.S * s.C, total = s.N * sample;
   for (int64_t i = (int64_t)blockIdx.x * kT + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * kT) {
     const int64_t n = i / sample;
     const int c = (int)((i - n * sample) % s.C);
     const int64_t g = n * s.G + c / s.per;
-    const float is = inv[g], z = (x[i] - mean[g]) * is;
-    const float ga = gamma ? gamma[c] : 1.f;
-    float dg;
-    const float dn = inner_gradient<ACT, GATED>(dy[i], z, ga, beta ? beta[c] : 0.f,
-                                                GATED ? gate[i] : 0.f, &dg);
+    const float is = inv[g], z[1] = {(x[i] - mean[g]) * is};
+    const float ga[1] = {gamma ? gamma[c] : 1.f}, be[1] = {beta ? beta[c] : 0.f};
+    float dn[1] = {dy[i]}, w[1] = {GATED ? gate[i] : 0.f};
+    inner_gradient<1, GATED>(code, dn, z, ga, be, w);
     const float2 m = sums[g];
-    dx[i] = is * (ga * dn - m.x - z * m.y);
-    if (GATED) dgate[i] = dg;
+    dx[i] = is * (ga[0] * dn[0] - m.x - z[0] * m.y);
+    if (GATED) dgate[i] = w[0];
   }
 }
 
@@ -443,23 +507,17 @@ __global__ void __launch_bounds__(kT)
       const int c = (k * f.lanes + lane) * V;
       if (c >= f.per) continue;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float t = fmaf(v[k].v[e] * is, ga[k].v[e], be[k].v[e]);
-        v[k].v[e] = GATED ? t * act(f.code, w[k].v[e]) : act(f.code, t);
+      for (int e = 0; e < V; ++e) v[k].v[e] = fmaf(v[k].v[e] * is, ga[k].v[e], be[k].v[e]);
+      if constexpr (GATED) {
+        act_all<V>(f.code, w[k].v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[k].v[e] *= w[k].v[e];
+      } else {
+        act_all<V>(f.code, v[k].v);
       }
       store<V>(y + at + c, v[k]);
     }
   }
-}
-
-// The gradient of n at one place, and where GATED that of the gate.
-template <bool GATED>
-__device__ __forceinline__ float inner_gradient(int code, float dy, float z, float gamma,
-                                                float beta, float gate, float* dgate) {
-  const float v = fmaf(z, gamma, beta);
-  const Both f = act_slope(code, GATED ? gate : v);
-  *dgate = dy * v * f.slope;
-  return dy * (GATED ? f.value : f.slope);
 }
 
 template <int V, int K, bool GATED>
@@ -506,20 +564,19 @@ __global__ void __launch_bounds__(kT)
     }
     float a = 0.f, b = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[k].v[e] = (z[k].v[e] - mu) * is;
+      inner_gradient<V, GATED>(f.code, d[k].v, z[k].v, ga[k].v, be[k].v, w[GATED ? k : 0].v);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        z[k].v[e] = (z[k].v[e] - mu) * is;
-        float dg = 0.f;
-        const float dn = inner_gradient<GATED>(f.code, d[k].v[e], z[k].v[e], ga[k].v[e], be[k].v[e],
-                                               GATED ? w[k].v[e] : 0.f, &dg);
-        if (GATED) w[k].v[e] = dg;
-        sum_n[k].v[e] += dn;
-        sum_z[k].v[e] = fmaf(dn, z[k].v[e], sum_z[k].v[e]);
-        d[k].v[e] = ga[k].v[e] * dn;
+        sum_n[k].v[e] += d[k].v[e];
+        sum_z[k].v[e] = fmaf(d[k].v[e], z[k].v[e], sum_z[k].v[e]);
+        d[k].v[e] *= ga[k].v[e];
         a += d[k].v[e];
         b = fmaf(d[k].v[e], z[k].v[e], b);
       }
+    }
     a = over_lanes(a, f.lanes) * share;
     b = over_lanes(b, f.lanes) * share;
 #pragma unroll
@@ -678,9 +735,13 @@ __global__ void __launch_bounds__(512)
     Pack<V> w;
     if (GATED) w = load<V>(gate + at + (int64_t)p * f.C);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float t = fmaf(v[k].v[e] * is[e], ga[e], be[e]);
-      v[k].v[e] = GATED ? t * act(f.code, w.v[e]) : act(f.code, t);
+    for (int e = 0; e < V; ++e) v[k].v[e] = fmaf(v[k].v[e] * is[e], ga[e], be[e]);
+    if constexpr (GATED) {
+      act_all<V>(f.code, w.v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[k].v[e] *= w.v[e];
+    } else {
+      act_all<V>(f.code, v[k].v);
     }
     store<V>(y + at + (int64_t)p * f.C, v[k]);
   }
@@ -731,12 +792,10 @@ __global__ void __launch_bounds__(512)
     Pack<V> w;
     if (GATED) w = load<V>(gate + at + (int64_t)p * f.C);
 #pragma unroll
+    for (int e = 0; e < V; ++e) z[k].v[e] = (z[k].v[e] - mu[e]) * is[e];
+    inner_gradient<V, GATED>(f.code, d[k].v, z[k].v, ga, be, w.v);
+#pragma unroll
     for (int e = 0; e < V; ++e) {
-      z[k].v[e] = (z[k].v[e] - mu[e]) * is[e];
-      float dg = 0.f;
-      d[k].v[e] = inner_gradient<GATED>(f.code, d[k].v[e], z[k].v[e], ga[e], be[e],
-                                        GATED ? w.v[e] : 0.f, &dg);
-      if (GATED) w.v[e] = dg;
       both[0][e] += d[k].v[e];
       both[1][e] = fmaf(d[k].v[e], z[k].v[e], both[1][e]);
     }
@@ -788,27 +847,6 @@ __global__ void __launch_bounds__(512)
       d[k].v[e] = is[e] * (ga[e] * d[k].v[e] - m[e].x - z[k].v[e] * m[e].y);
     store<V>(dx + at + (int64_t)p * f.C, d[k]);
   }
-}
-
-// Calls f with the activation and whether there is a gate as constants.
-template <int V>
-struct Const {
-  static constexpr int value = V;
-};
-template <class F>
-void with_form(int activation, bool gated, F f) {
-  auto with_act = [&](auto g) {
-    switch (activation) {
-      case kRelu: return f(Const<kRelu>{}, g);
-      case kSilu: return f(Const<kSilu>{}, g);
-      case kGelu: return f(Const<kGelu>{}, g);
-      default: return f(Const<kNone>{}, g);
-    }
-  };
-  if (gated)
-    with_act(Const<1>{});
-  else
-    with_act(Const<0>{});
 }
 
 int plan(const char* what, Shape& s, int64_t N, int64_t S, int64_t C, int64_t G, int activation,
@@ -981,11 +1019,9 @@ WXX_EXPORT int wxx_group_norm(float* y, float* mean, float* inv, const float* x,
   }
   wxx_free(part);
   if (st != WXX_OK) return st;
-  with_form(activation, gate != nullptr, [&](auto a, auto g) {
-    apply_kernel<decltype(a)::value, decltype(g)::value>
-        <<<wxx::grid_for(N * S * C, kT), kT, 0, wxx::stream()>>>(y, x, gate, mean, inv, gamma, beta,
-                                                                 s);
-  });
+  auto apply = gate ? apply_kernel<true> : apply_kernel<false>;
+  apply<<<wxx::grid_for(N * S * C, kT), kT, 0, wxx::stream()>>>(y, x, gate, mean, inv, gamma, beta, s,
+                                                               activation);
   WXX_LAUNCH_CHECK();
   return WXX_OK;
 }
@@ -1046,10 +1082,8 @@ WXX_EXPORT int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, f
     return st;
   float2* sums = static_cast<float2*>(scratch);
   float* part = reinterpret_cast<float*>(sums + N * G);
-  with_form(activation, gate != nullptr, [&](auto a, auto g) {
-    channel_sums_kernel<decltype(a)::value, decltype(g)::value>
-        <<<(unsigned)rows, kT, 0, wxx::stream()>>>(part, dy, x, gate, mean, inv, gamma, beta, s);
-  });
+  auto sum = gate ? channel_sums_kernel<true> : channel_sums_kernel<false>;
+  sum<<<(unsigned)rows, kT, 0, wxx::stream()>>>(part, dy, x, gate, mean, inv, gamma, beta, s, activation);
   int st = wxx::after_launch(__FILE__, __LINE__);
   if (st == WXX_OK) {
     group_sums_kernel<<<(unsigned)((N * G + kT - 1) / kT), kT, 0, wxx::stream()>>>(sums, part,
@@ -1057,11 +1091,9 @@ WXX_EXPORT int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, f
     st = wxx::after_launch(__FILE__, __LINE__);
   }
   if (st == WXX_OK) {
-    with_form(activation, gate != nullptr, [&](auto a, auto g) {
-      input_gradient_kernel<decltype(a)::value, decltype(g)::value>
-          <<<wxx::grid_for(N * S * C, kT), kT, 0, wxx::stream()>>>(dx, dgate, dy, x, gate, mean,
-                                                                   inv, gamma, beta, sums, s);
-    });
+    auto input = gate ? input_gradient_kernel<true> : input_gradient_kernel<false>;
+    input<<<wxx::grid_for(N * S * C, kT), kT, 0, wxx::stream()>>>(dx, dgate, dy, x, gate, mean, inv,
+                                                                 gamma, beta, sums, s, activation);
     st = wxx::after_launch(__FILE__, __LINE__);
   }
   if (st == WXX_OK) {
