@@ -22,6 +22,10 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "tc_gemm.cuh"
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
 WXX_EXPORT int wxx_malloc(void** out, uint64_t nbytes);
 WXX_EXPORT int wxx_free(void* p);
@@ -152,36 +156,36 @@ __global__ void __launch_bounds__(kT) sweep_kernel(const Pass a, const Shape s) 
 // precision, three products for one: every operand is split into a high and a low half of
 // 11 bits each, hi hi + hi lo + lo hi, which leaves out 2^-22 of a product.  Half numbers
 // reach from 2^-24 to 2^16 only, so each row (a position's vector of x, y or z, a row of the
-// position-by-position matrix) is scaled by a power of two that brings its largest entry
-// to 2^13, and a state by one for all of it; the powers are put back in 32 bits.  Entries
-// far below their row's largest lose accuracy from 2^-20 of it on (they are good to 2^-38
-// of the largest).  (Measured, mma.sync: half 554, tf32 277 TFLOP/s; three products of
-// tf32 need no scaling, but would be bound by that rate.)  The state stays in 32-bit
-// registers, a chunk's products are added to it in 32 bits.
+// position-by-position matrix) is scaled by a power of two that brings its length (in the
+// matrix its largest entry) to 2^13, and a state by one for all of it; the powers are put
+// back in 32 bits.  Entries far below their row's length lose accuracy from 2^-20 of it on
+// (they are good to 2^-38 of it).  (Measured, mma.sync: half 554, tf32 277 TFLOP/s; three
+// products of tf32 need no scaling, but would be bound by that rate.  On tcgen05, kind::tf32
+// with sums in TMEM, chunks of 128 took as long, and the truncated sums made the error 1.6e-6
+// instead of 4.6e-7.)  The state stays in 32-bit registers, a chunk's products are added to
+// it in 32 bits.
 //
 // NaN and infinities cannot take part: 0 times NaN would carry them to earlier positions
-// and other documents.  A chunk that holds one, or starts from a state that does, is
-// worked through position by position (rare_chunk).
+// and other documents.  A chunk with a row whose length is not between 2^-60 and 2^63 (or 0),
+// or such a state, is worked through position by position (rare_chunk).
+
+using wxx_tc::mbar_arrive_expect_tx;
+using wxx_tc::mbar_init;
+using wxx_tc::mbar_wait;
+using wxx_tc::tma_load_4d;
 
 constexpr int kC = 64;                  // positions of a chunk
-constexpr int kThreads = 256;           // 8 warps: 4 groups of 16 positions by 2 halves
-constexpr int kTop = 13;                // a scaled row's largest entry is in [2^13, 2^14)
+constexpr int kThreads = 128;           // 4 warps of 16 positions
+constexpr int kTop = 13;                // a scaled row's length is in [2^13, 2^14)
 
 __device__ __forceinline__ uint32_t smem_address(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void copy16(uint32_t to, const float* from, bool take) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from),
-               "r"(take ? 16 : 0));
 }
 __device__ __forceinline__ void copy4(uint32_t to, const float* from, bool take) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from),
                "r"(take ? 4 : 0));
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-__device__ __forceinline__ void pair_barrier(int group) {      // the two warps of a group
-  asm volatile("bar.sync %0, 64;" ::"r"(group + 1) : "memory");
-}
 
 __device__ __forceinline__ void load4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -216,11 +220,13 @@ __device__ __forceinline__ void products(float (&c0)[4], float (&c1)[4], const u
   product(c1, hi, bh[2], bh[3]);
 }
 
-// The high and low halves of two numbers.
-__device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+// The high and low halves of two numbers times `up`.
+__device__ __forceinline__ void split(float a, float b, float up, uint32_t& hi, uint32_t& lo) {
+  mul2(a, b, a, b, up, up);
   const __half2 h = __floats2half2_rn(a, b);
   const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+  sub2(a, b, a, b, f.x, f.y);
+  const __half2 l = __floats2half2_rn(a, b);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -230,23 +236,28 @@ __device__ __forceinline__ uint32_t times(uint32_t a, uint32_t b) {      // two 
   return d;
 }
 
-// The exponent of a row's largest entry; rows below 2^-100 are scaled as if at 2^-100.
-__device__ __forceinline__ int exponent(float size) {
-  return max((int)(__float_as_uint(size) >> 23) - 127, -100);
+// Sums of squares, in two parts.
+__device__ __forceinline__ void square2(float& s0, float& s1, float a, float b) {
+  fma2(s0, s1, a, b, a, b, s0, s1);
+}
+// Whether a row (or the state) of this square cannot be scaled; 0 alone says nothing yet.
+constexpr float kShort = 0x1p-120f, kLong = 0x1p126f;
+// The exponent of a length with this square.
+__device__ __forceinline__ int exponent(float square) {
+  return ((int)(__float_as_uint(square) >> 23) - 127) >> 1;
 }
 __device__ __forceinline__ float power2(int e) {            // -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
-// v -> v f 2^e for any e, f about 1: in two steps of one sign, so that nothing is lost on
-// the way.
+// f 2^e, f about 1, in two steps: the second is 1 unless 2^e is out of range.
 struct Scale {
   float first, then;
   __device__ Scale(float f, int e) {
     e = min(max(e, -250), 250);
-    first = f * power2(e / 2);
-    then = power2(e - e / 2);
+    const int one = min(max(e, -125), 125);
+    first = f * power2(one);
+    then = power2(e - one);
   }
-  __device__ __forceinline__ float operator()(float v) const { return v * first * then; }
 };
 
 // Tiles of W half numbers a row for ldmatrix: 16-byte pieces of a row exchanged so that
@@ -256,34 +267,21 @@ __device__ __forceinline__ uint32_t piece(int row, int q) {
   const int turn = W == 32 ? (row >> 1) & 3 : row & 7;
   return (uint32_t)(row * W * 2 + ((q ^ turn) << 4));
 }
-// Rows of W floats as copied: the even 16-byte pieces, then the odd ones, so that a lane's 8
-// neighbouring floats are read without conflicts.
-template <int W>
-__device__ __forceinline__ int raw_piece(int row, int q) {
-  const int at = (q >> 1) + (q & 1) * (W / 8);
-  return row * (W / 4) + (W == 32 ? at ^ ((row & 1) << 2) : at);
-}
+// 32 columns of all positions as the copy engine leaves them, 16-byte pieces exchanged.
+__device__ __forceinline__ int raw_piece(int row, int q) { return row * 8 + (q ^ (row & 7)); }
+constexpr int kRaw = kC * 128;          // their bytes
 
 template <int P, int R>
 struct Layout {
-  static constexpr int kRawY = 0, kRawZ = kRawY + kC * P * 4;
-  static constexpr int kTiles = kRawZ + kC * R * 4;
-  // high halves, then low halves, of x, y, z and the state
-  static constexpr int kX = kTiles, kY = kX + kC * P * 4, kZ = kY + kC * P * 4;
-  static constexpr int kState = kZ + kC * R * 4;
-  static constexpr int kEnd = kState + P * R * 4;
-  // where the two halves of a group exchange their sums: x's tile of these positions, which
-  // both have read by then, where it is large enough
-  static constexpr bool kShared = P >= R;
-  static constexpr int kSums = kShared ? kX : kEnd, kGroup = kShared ? 16 * P * 2 : 16 * R * 4;
-  static constexpr int kHalf = kShared ? kC * P * 2 : 16 * R * 2;
-  static constexpr int kBytes = kShared ? kEnd : kEnd + 8 * 16 * R * 2;
-  static_assert(P * R * 4 <= kState - kTiles, "rare_chunk's state lies in the tiles");
-  // the warps' parts of the state: 16 rows by kColTiles tiles of 8 columns
-  static constexpr int kRowGroups = P / 16 < 8 ? P / 16 : 8;
-  static constexpr int kColGroups = 8 / kRowGroups > R / 16 ? R / 16 : 8 / kRowGroups;
-  static constexpr int kColTiles = R / 8 / kColGroups;
-  static constexpr int kBlocks = P == 128 ? 1 : P == 32 && R == 32 ? 3 : 2;    // on an SM
+  static constexpr int kRawX = 0, kRawY = kRawX + P / 32 * kRaw, kRawZ = kRawY + P / 32 * kRaw;
+  static constexpr int kTiles = kRawZ + R / 32 * kRaw;
+  // high halves, then low halves, of y, z and the state
+  static constexpr int kY = kTiles, kZ = kY + kC * P * 4, kState = kZ + kC * R * 4;
+  static constexpr int kEnd = kState + P * R * 4, kBytes = kEnd + 1024;
+  static_assert((P * R + kThreads) * 4 + kC <= kState - kTiles, "rare_chunk's room");
+  // the warps' parts of the state: kRowTiles times 16 rows by kColTiles tiles of 8 columns
+  static constexpr int kRowTiles = P >= 64 ? P / 64 : 1, kColTiles = P >= 64 ? R / 8 : R / 16;
+  static constexpr int kBlocks = P == 128 ? 1 : P == 64 && R == 64 ? 2 : P == 32 && R == 32 ? 4 : 3;
 };
 
 struct Segments {           // pieces of a row that are worked on side by side
@@ -319,7 +317,7 @@ struct Weights {
   }
 };
 
-// A weight of the state, l^u, as rest 2^e with rest in [1, 2); below 2^-126 there is none.
+// A power of l as rest 2^e with rest in [1, 2); below 2^-126 it is none.
 struct Decayed {
   bool any;
   int e;
@@ -334,38 +332,43 @@ struct Decayed {
 
 // The parts of shared memory that are not tiles.
 struct alignas(16) Small {
-  float max_x[kC], max_y[kC], max_z[kC];    // the rows' largest entries
-  float max_state[8];                   // of the state, by warp
+  float square_y[kC], square_z[kC];     // of the rows
+  float square_state[4];                // by warp
   // per position j: 2^(exponents of y_j and z_j, below the largest) / what z_j's scale has more,
   // and that times l^(15 - j % 16) (back: l^(j % 16))
   float2 weight[kC];
   uint16_t added[2][kC];                // j's weight in the state, as a product of two halves
-  float power[kC + 1];                  // l^n
+  float power[kC + 4];                  // l^n
   int document[kC];
+  uint64_t arrived;                     // y, z and x are here
+  int abort;
 };
 
 // The passes of one launch: sweeps over the same B, T and H whose heads have the same
-// padded sizes.
+// padded sizes; and the maps of their operands, where the copy engine takes them.
 struct Passes {
   Pass at[3];
 };
+struct Maps {
+  CUtensorMap x[3], y[3], z[3];
+};
 
-// Position by position, for a chunk with numbers that are not finite: the state in shared
-// memory, columns over the lanes, rows over kThreads / R groups of threads.
-template <int P, int R, bool STATE>
-__device__ void rare_chunk(float* state, float* sums, const Pass& a, const Shape& s,
-                           const Weights& w, unsigned long long cuts, bool next_cut, Decay l,
-                           int64_t b, int h, int t0, int slice) {
+// Position by position, for a chunk with numbers that are not finite or that cannot be
+// scaled: the state in shared memory, columns over the lanes, rows over kThreads / R groups
+// of threads.
+template <int R, bool STATE>
+__device__ void rare_chunk(float* state, float* sums, const unsigned char* cuts, const Pass& a,
+                           const Shape& s, int n, bool tail, bool next_cut, Decay l, int64_t b,
+                           int h, int t0, int slice) {
   constexpr int kGroups = kThreads / R;
   const int c = threadIdx.x % R, group = threadIdx.x / R, r = slice * R + c;
-  for (int k = 0; k < w.n; ++k) {
-    const int i = a.back ? w.n - 1 - k : k;
+  for (int k = 0; k < n; ++k) {
+    const int i = a.back ? n - 1 - k : k;
     const float* x = a.x.p + b * a.x.bs + (t0 + i) * a.x.ts + (int64_t)h * a.p;
     const float* y = a.y.p + b * a.y.bs + (t0 + i) * a.y.ts + (int64_t)h * a.p;
     const float z = r < a.r ? a.z.p[b * a.z.bs + (t0 + i) * a.z.ts + (int64_t)h * a.r + r] : 0.f;
-    const bool on = k < w.n - 1 || a.back || w.tail;       // the state goes on from here
-    const bool cut = k < w.n - 1 ? (a.back ? cuts >> i & 1 : cuts >> (i + 1) & 1)
-                                 : (a.back ? cuts & 1 : next_cut);
+    const bool on = k < n - 1 || a.back || tail;           // the state goes on from here
+    const bool cut = a.back ? cuts[i] : k < n - 1 ? cuts[i + 1] : next_cut;
     float sum = 0.f;
     for (int p = group; p < a.p; p += kGroups) {
       float now = fmaf(a.y_scale * y[p], z, state[p * R + c]);
@@ -385,17 +388,19 @@ __device__ void rare_chunk(float* state, float* sums, const Pass& a, const Shape
 }
 
 // A block: one sequence, head, slice of R columns of z and piece of the row; STATE: only
-// the state after the piece is wanted.  Warps w and w + 4 have the same 16 positions: each
-// takes every other 16 positions of y and z and half of the state's rows, and they add
-// their sums at the end (so no warp has more than two of the four position blocks, and the
-// operands' registers are few enough for two blocks on an SM).
+// the state after the piece is wanted.  A warp has 16 positions of x and their outputs, and
+// a part of the state; y and z are split by all warps and read by all.  The next chunk's
+// operands are copied meanwhile.
 template <int P, int R, bool STATE>
 __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
-    chunk_kernel(const __grid_constant__ Passes passes, const Shape s, const Segments g,
-                 const unsigned per_pass) {
+    chunk_kernel(const __grid_constant__ Passes passes, const __grid_constant__ Maps maps,
+                 const bool tma, const Shape s, const Segments g, const unsigned per_pass,
+                 int* err) {
   using L = Layout<P, R>;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char raw_smem[];
   __shared__ Small m;
+  unsigned char* smem = raw_smem + ((1024 - (smem_address(raw_smem) & 1023)) & 1023);
+  const uint32_t base = smem_address(smem);
   const unsigned pass = blockIdx.x / per_pass;
   const Pass& a = passes.at[pass];
   unsigned at = blockIdx.x % per_pass;
@@ -407,328 +412,323 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
   const int h = at % s.H;
   const int64_t b = at / s.H, heads = per_pass / (unsigned)(slices * pieces);   // B H
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, t = lane & 3;
-  const int group = warp & 3, half = warp >> 2;
   const int mat = lane >> 3, mat_row = lane & 7;
   const bool back = a.back;
   const Decay l(s.log_decay[h]);
-  for (int i = threadIdx.x; i <= kC; i += kThreads)
-    m.power[i] = i == 0 ? 1.f : expf((float)i * s.log_decay[h]);
+  if (threadIdx.x <= kC)
+    m.power[threadIdx.x] =
+        threadIdx.x == 0 ? 1.f : expf((float)threadIdx.x * s.log_decay[h]);
 
   const int chunks = (s.T + kC - 1) / kC;
   const int c0 = seg * g.chunks, c1 = min(c0 + g.chunks, chunks);
   // pieces and chunks are counted in the direction of the sweep
   auto start = [&](int c) { return (back ? chunks - 1 - c : c) * kC; };
   const uint32_t* marks = s.reset ? s.reset + b * s.T : nullptr;
-  auto resets = [&](int c, bool& next) {
-    const int t0 = start(c), n = min(kC, s.T - t0);
-    next = false;
-    if (!marks) return 0ull;
-    const unsigned lo = __ballot_sync(0xffffffffu, lane < n && marks[t0 + lane] != 0);
-    const unsigned hi = __ballot_sync(0xffffffffu, lane + 32 < n && marks[t0 + lane + 32] != 0);
-    next = !back && t0 + n < s.T && marks[t0 + n] != 0;
-    return (unsigned long long)hi << 32 | lo;
-  };
-  auto weights = [&](int c, unsigned long long cuts, bool next) {
-    const int t0 = start(c), n = min(kC, s.T - t0);
-    return Weights(cuts, n, t0 + n < s.T, back ? cuts & 1 : next);
-  };
 
-  // the state, in the layout of a product's result: rows row0 + quad (+ 8), columns col0 + 8 nt
-  // + 2 t (+ 1); warps without a part keep zeros
-  const int row0 = (warp % L::kRowGroups) * 16;
-  const bool has_state = warp / L::kRowGroups < L::kColGroups;
-  const int col0 = has_state ? warp / L::kRowGroups * L::kColTiles * 8 : 0;
-  float X[L::kColTiles][4], d[L::kColTiles][4];
+  // x, y and z of a chunk into shared memory, 32 columns of all positions at a time
+  auto fetch = [&](int c) {
+    const int t0 = start(c);
+    if (tma) {
+      if (threadIdx.x == 0) {
+        mbar_arrive_expect_tx(&m.arrived, ((STATE ? 1 : 2) * (P / 32) + R / 32) * kRaw);
+#pragma unroll
+        for (int k = 0; k < P / 32; ++k) {
+          if (!STATE)
+            tma_load_4d(base + L::kRawX + k * kRaw, &maps.x[pass], &m.arrived, 32 * k, h, t0, (int)b);
+          tma_load_4d(base + L::kRawY + k * kRaw, &maps.y[pass], &m.arrived, 32 * k, h, t0, (int)b);
+        }
+#pragma unroll
+        for (int k = 0; k < R / 32; ++k)
+          tma_load_4d(base + L::kRawZ + k * kRaw, &maps.z[pass], &m.arrived, slice * R + 32 * k, h,
+                      t0, (int)b);
+      }
+      return;
+    }
+    auto rows = [&](int to, const Operand& o, int columns, int from, int width) {
+      const int n = min(kC, s.T - t0);
+      const float* p = o.p + b * o.bs + t0 * o.ts + (int64_t)h * columns + from;
+      for (int i = threadIdx.x; i < kC * width; i += kThreads) {
+        const int row = i / width, col = i % width;
+        const bool take = row < n && col < columns - from;
+        copy4(base + to + (col >> 5) * kRaw + raw_piece(row, (col & 31) >> 2) * 16 + (col & 3) * 4,
+              take ? p + row * o.ts + col : o.p, take);
+      }
+    };
+    if (!STATE) rows(L::kRawX, a.x, a.p, 0, P);
+    rows(L::kRawY, a.y, a.p, 0, P);
+    rows(L::kRawZ, a.z, a.r, slice * R, R);
+  };
+  if (threadIdx.x == 0) {
+    mbar_init(&m.arrived, 1);
+    m.abort = 0;
+    wxx_tc::fence_barrier_init();
+  }
+  __syncthreads();
+  fetch(c0);
+
+  // the state, in the layout of a product's result: rows row0 + 16 mt + quad (+ 8), columns
+  // col0 + 8 nt + 2 t (+ 1)
+  const int row0 = P >= 64 ? warp * (P / 4) : (warp & 1) * 16;
+  const int col0 = P >= 64 ? 0 : (warp >> 1) * (R / 2);
+  float X[L::kRowTiles][L::kColTiles][4];
+  auto each = [&](auto f) {             // f(entry, row, column)
+#pragma unroll
+    for (int mt = 0; mt < L::kRowTiles; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          f(X[mt][nt][e], row0 + mt * 16 + quad + (e >> 1) * 8, col0 + nt * 8 + 2 * t + (e & 1));
+  };
   {
     const int64_t head = (b * s.H + h) * (int64_t)a.p * a.r;
-    const float* from = a.from ? a.from + head : nullptr;
+    const float* from = STATE || !a.from ? nullptr : a.from + head;
     int64_t ps = a.p_stride, rs = a.r_stride;
-    bool drop = !has_state;
-    if (STATE) {
-      from = nullptr;
-    } else if (seg > 0) {
+    if (!STATE && seg > 0) {
       from = g.state + ((pass * (int64_t)(g.count - 1) + seg - 1) * heads + b * s.H + h) * a.p * a.r;
       ps = a.r;
       rs = 1;
-    } else if (!back) {
-      drop = drop || (marks && marks[0] != 0);
     }
     const bool first = !STATE && seg == 0 && !back;          // its own step of the decay
-#pragma unroll
-    for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int p = row0 + quad + (e >> 1) * 8, r = slice * R + col0 + nt * 8 + 2 * t + (e & 1);
-        const float v = from && !drop && p < a.p && r < a.r ? from[p * ps + r * rs] : 0.f;
-        X[nt][e] = first ? l(v) : v;
-        d[nt][e] = 0.f;
-      }
+    if (first && marks && marks[0] != 0) from = nullptr;
+    each([&](float& v, int p, int c) {
+      const int r = slice * R + c;
+      v = from && p < a.p && r < a.r ? from[p * ps + r * rs] : 0.f;
+      if (first) v = l(v);
+    });
   }
+  const bool pairs_o = ((reinterpret_cast<uintptr_t>(a.out) & 7) == 0) && (a.r & 1) == 0;
+  float run = 1.f;                      // STATE: what the piece does to the state before it
 
-  float* raw_y = reinterpret_cast<float*>(smem + L::kRawY);
-  float* raw_z = reinterpret_cast<float*>(smem + L::kRawZ);
-  const uint32_t base = smem_address(smem);
-  // 16-byte accesses where every row allows them
-  auto whole = [&](const Operand& o, int width) {
-    return ((reinterpret_cast<uintptr_t>(o.p) & 15) == 0) && ((o.bs | o.ts | width) & 3) == 0;
-  };
-  const bool wide_x = !STATE && whole(a.x, a.p), wide_y = whole(a.y, a.p), wide_z = whole(a.z, a.r);
-  auto fetch_rows = [&](auto width, float* raw, const Operand& o, int columns, int from, int t0,
-                        bool wide) {
-    constexpr int W = decltype(width)::value;
-    const int n = min(kC, s.T - t0);
-    const float* p = o.p + b * o.bs + t0 * o.ts + (int64_t)h * columns + from;
-    const int here = columns - from;                      // columns from there on
-    if (wide) {
-#pragma unroll
-      for (int k = 0; k < kC * (W / 4) / kThreads; ++k) {
-        const int i = threadIdx.x + k * kThreads, row = i / (W / 4), q = i % (W / 4);
-        const bool take = row < n && q * 4 < here;
-        copy16(smem_address(raw) + raw_piece<W>(row, q) * 16, take ? p + row * o.ts + q * 4 : o.p,
-               take);
-      }
-    } else {
-      for (int i = threadIdx.x; i < kC * W; i += kThreads) {
-        const int row = i / W, col = i % W;
-        const bool take = row < n && col < here;
-        copy4(smem_address(raw) + raw_piece<W>(row, col >> 2) * 16 + (col & 3) * 4,
-              take ? p + row * o.ts + col : o.p, take);
-      }
+  for (int c = c0; c < c1; ++c) {
+    const int t0 = start(c), n = min(kC, s.T - t0);
+    // the resets of the chunk, and of the position after it
+    unsigned long long cuts = 0;
+    bool next = false;
+    if (marks) {
+      const unsigned lo = __ballot_sync(0xffffffffu, lane < n && marks[t0 + lane] != 0);
+      const unsigned hi = __ballot_sync(0xffffffffu, lane + 32 < n && marks[t0 + lane + 32] != 0);
+      next = !back && t0 + n < s.T && marks[t0 + n] != 0;
+      cuts = (unsigned long long)hi << 32 | lo;
     }
-  };
-  auto fetch = [&](int c) {
-    fetch_rows(std::integral_constant<int, P>{}, raw_y, a.y, a.p, 0, start(c), wide_y);
-    fetch_rows(std::integral_constant<int, R>{}, raw_z, a.z, a.r, slice * R, start(c), wide_z);
-  };
-  // A lane's share of x, y and z: 8 neighbouring columns of a row, W / 32 rows in turn of the
-  // warp's 8.
-  auto row_of = [&](int W, int k) { return warp * 8 + k * (256 / W) + lane / (W / 8); };
-  constexpr int kPassesX = P / 32, kPassesZ = R / 32;
-  float x[STATE ? 1 : kPassesX][8];
-  auto fetch_x = [&](int c) {
-    const int t0 = start(c), n = min(kC, s.T - t0), col = lane % (P / 8) * 8;
+    const Weights w(cuts, n, t0 + n < s.T, back ? cuts & 1 : next);
+    bool odd = false;                   // a row that cannot be scaled
+    {
+      float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-    for (int k = 0; k < kPassesX; ++k) {
-      const int row = row_of(P, k);
-      const float* p = a.x.p + b * a.x.bs + (t0 + row) * a.x.ts + (int64_t)h * a.p + col;
+      for (int mt = 0; mt < L::kRowTiles; ++mt)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[k][e] = 0.f;
-      if (row < n) {
-        if (wide_x) {
+        for (int nt = 0; nt < L::kColTiles; ++nt) {
+          square2(s0, s1, X[mt][nt][0], X[mt][nt][1]);
+          square2(s0, s1, X[mt][nt][2], X[mt][nt][3]);
+        }
+      s0 += s1;
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            if (col + 4 * q >= a.p) continue;
-            const float4 v = *reinterpret_cast<const float4*>(p + 4 * q);
-            x[k][4 * q] = v.x, x[k][4 * q + 1] = v.y, x[k][4 * q + 2] = v.z, x[k][4 * q + 3] = v.w;
+      for (int o = 16; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+      odd = !(s0 < kLong);
+      if (s0 < kShort) {                // a state may be shorter than its square tells
+        bool any = false;
+        each([&](float v, int, int) { any = any || v != 0.f; });
+        if (__any_sync(0xffffffffu, any)) s0 = 0x1p-126f;
+      }
+      if (lane == 0) m.square_state[warp] = s0;
+    }
+    if (tma)
+      mbar_wait(&m.arrived, (c - c0) & 1, &m.abort, err);
+    else
+      copies_done();
+    __syncthreads();       // the operands are here, the last chunk's tiles are read
+
+    // y and z by rows: a lane has 4 of every 32 columns; a pass of a warp takes 4 of its 16
+    // rows (64 columns and more: two of them 4 apart, for the banks of the tiles)
+    const int piece_of = lane & 7, sub = lane >> 3;
+    auto row_of = [&](int W, int k) {
+      return warp * 16 + (W == 32 ? 4 * k + sub : (k >> 1) * 8 + (k & 1) * 2 + (sub & 1) * 4 + (sub >> 1));
+    };
+    float4 y[4][P / 32], z[4][R / 32];
+    auto read = [&](auto width, int raw, auto& v, float* squares) {
+      constexpr int W = decltype(width)::value;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = row_of(W, k);
+#pragma unroll
+        for (int i = 0; i < W / 32; ++i)
+          v[k][i] = reinterpret_cast<const float4*>(smem + raw + i * kRaw)[raw_piece(row, piece_of)];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < W / 32; ++i) {
+          square2(s0, s1, v[k][i].x, v[k][i].y);
+          square2(s0, s1, v[k][i].z, v[k][i].w);
+        }
+        s0 += s1;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+        if (!(s0 >= kShort && s0 < kLong)) {
+          odd = odd || !(s0 < kLong);
+#pragma unroll
+          for (int i = 0; i < W / 32; ++i)
+            odd = odd || v[k][i].x != 0.f || v[k][i].y != 0.f || v[k][i].z != 0.f || v[k][i].w != 0.f;
+        }
+        if (piece_of == 0) squares[row_of(W, k)] = s0;
+      }
+    };
+    read(std::integral_constant<int, P>{}, L::kRawY, y, m.square_y);
+    read(std::integral_constant<int, R>{}, L::kRawZ, z, m.square_z);
+    // x of this warp's positions, in the layout of a product's left operand
+    float2 x[STATE ? 1 : P / 16][4];
+    float square_x[2] = {0.f, 0.f};
+    if constexpr (!STATE) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = warp * 16 + quad + half * 8;
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < P / 16; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const unsigned char* p = smem + L::kRawX + (k >> 1) * kRaw +
+                                     raw_piece(row, 4 * (k & 1) + 2 * e + (t >> 1)) * 16 + (t & 1) * 8;
+            const float2 v = *reinterpret_cast<const float2*>(p);
+            x[k][half + 2 * e] = v;
+            square2(s0, s1, v.x, v.y);
           }
-        } else {
+        s0 += s1;
+        s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
+        s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
+        square_x[half] = s0;
+        if (!(s0 >= kShort && s0 < kLong)) {
+          odd = odd || !(s0 < kLong);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (col + e < a.p) x[k][e] = p[e];
+          for (int k = 0; k < P / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              odd = odd || x[k][half + 2 * e].x != 0.f || x[k][half + 2 * e].y != 0.f;
         }
       }
     }
-  };
-  const bool pairs_o = ((reinterpret_cast<uintptr_t>(a.out) & 7) == 0) && (a.r & 1) == 0;
-
-  fetch(c0);
-  if constexpr (!STATE) fetch_x(c0);
-  float run = 1.f;                      // STATE: what the piece does to the state before it
-  float kept = 1.f, odd = 0.f;          // of the last chunk; odd: 0 unless something is not finite
-  Scale by_d(0.f, 0);
-
-  for (int c = c0;; ++c) {
-    copies_done();
-    // y and z are here, the last chunk's tiles are read
-    if (__syncthreads_or(!(odd == 0.f))) {
-      bool next;
-      const unsigned long long cuts = resets(c - 1, next);
+    odd = __syncthreads_or(odd);        // the squares are here, the operands are read
+    if (c + 1 < c1) fetch(c + 1);
+    const int kept_power = w.kept(back);
+    const float kept = kept_power < 0 ? 0.f : m.power[kept_power];
+    if (STATE) run *= kept;
+    const float square_state =
+        (m.square_state[0] + m.square_state[1]) + (m.square_state[2] + m.square_state[3]);
+    if (odd || (square_state > 0.f && square_state < kShort)) {
       float* state = reinterpret_cast<float*>(smem + L::kTiles);
-      auto each = [&](auto f) {
-#pragma unroll
-        for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            f(X[nt][e], state[(row0 + quad + (e >> 1) * 8) * R + col0 + nt * 8 + 2 * t + (e & 1)]);
-      };
-      if (has_state) each([](float& v, float& to) { to = v; });
+      unsigned char* cut = smem + L::kTiles + (P * R + kThreads) * 4;
+      if (threadIdx.x < kC) cut[threadIdx.x] = cuts >> threadIdx.x & 1;
+      each([&](float v, int p, int c) { state[p * R + c] = v; });
       __syncthreads();
-      rare_chunk<P, R, STATE>(state, state + P * R, a, s, weights(c - 1, cuts, next), cuts, next, l,
-                              b, h, start(c - 1), slice);
+      rare_chunk<R, STATE>(state, state + P * R, cut, a, s, n, w.tail, next, l, b, h, t0, slice);
       __syncthreads();
-      if (has_state) each([](float& v, float& to) { v = to; });
-      __syncthreads();
-    } else if (c > c0) {
-#pragma unroll
-      for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) X[nt][e] = fmaf(kept, X[nt][e], by_d(d[nt][e]));
+      each([&](float& v, int p, int c) { v = state[p * R + c]; });
+      continue;
     }
-    if (c == c1) break;
-    odd = 0.f;
-    bool next;
-    const unsigned long long cuts = resets(c, next);
-    const Weights w = weights(c, cuts, next);
-    const int t0 = start(c), n = w.n;
-
-    if (!STATE) {                       // the state's largest entry
-      float most = 0.f;
-#pragma unroll
-      for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2)
-          most = fmax3(most, fabsf(X[nt][e]), fabsf(X[nt][e + 1]));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (lane == 0) m.max_state[warp] = most;
-    }
-    // the rows' largest entries
-    auto largest = [&](auto width, const float (&v)[8], int row, float* max_row) {
-      constexpr int kLanes = decltype(width)::value / 8;
-      float most = fmax3(fabsf(v[0]), fabsf(v[1]), fabsf(v[2]));
-      most = fmax3(most, fabsf(v[3]), fabsf(v[4]));
-      most = fmax3(most, fabsf(v[5]), fabsf(v[6]));
-      most = fmaxf(most, fabsf(v[7]));
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1)
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (lane % kLanes == 0) max_row[row] = most;
-    };
-    float y[kPassesX][8], z[kPassesZ][8];
-    auto read = [&](auto width, const float* raw, float (&v)[8], int row) {
-      constexpr int W = decltype(width)::value;
-      const int q = lane % (W / 8);
-      const float4 u0 = reinterpret_cast<const float4*>(raw)[raw_piece<W>(row, 2 * q)];
-      const float4 u1 = reinterpret_cast<const float4*>(raw)[raw_piece<W>(row, 2 * q + 1)];
-      v[0] = u0.x, v[1] = u0.y, v[2] = u0.z, v[3] = u0.w;
-      v[4] = u1.x, v[5] = u1.y, v[6] = u1.z, v[7] = u1.w;
-    };
-#pragma unroll
-    for (int k = 0; k < kPassesX; ++k)
-      read(std::integral_constant<int, P>{}, raw_y, y[k], row_of(P, k));
-#pragma unroll
-    for (int k = 0; k < kPassesZ; ++k)
-      read(std::integral_constant<int, R>{}, raw_z, z[k], row_of(R, k));
-#pragma unroll
-    for (int k = 0; k < kPassesX; ++k)
-      largest(std::integral_constant<int, P>{}, y[k], row_of(P, k), m.max_y);
-#pragma unroll
-    for (int k = 0; k < kPassesZ; ++k)
-      largest(std::integral_constant<int, R>{}, z[k], row_of(R, k), m.max_z);
-    if constexpr (!STATE) {
-#pragma unroll
-      for (int k = 0; k < kPassesX; ++k)
-        largest(std::integral_constant<int, P>{}, x[k], row_of(P, k), m.max_x);
-    }
-    __syncthreads();
 
     // what the rows weigh: lane looks at rows lane and lane + 32
     int most = -1000, most_added = -1000;
+    int e_row[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int j = lane + 32 * k;
-      const float my = m.max_y[j], mz = m.max_z[j];
-      if (my == 0.f || mz == 0.f) continue;               // nothing there
-      const int e = exponent(my) + exponent(mz);
+      const float sy = m.square_y[j], sz = m.square_z[j];
+      e_row[k] = exponent(sy) + exponent(sz);
+      if (sy == 0.f || sz == 0.f) e_row[k] = -1000;         // nothing there
       const Decayed u(m.power, w.added(j, back));
-      most = max(most, e);
-      if (u.any) most_added = max(most_added, e + u.e);
+      most = max(most, e_row[k]);
+      e_row[k] = u.any ? e_row[k] + u.e : -1000;
+      most_added = max(most_added, e_row[k]);
     }
     most = __reduce_max_sync(0xffffffffu, most);
     most_added = __reduce_max_sync(0xffffffffu, most_added);
-    if (most == -1000) most = 0;
-    if (most_added == -1000) most_added = 0;
+    // a weight in the state that one half number does not hold
+    const bool far = __any_sync(0xffffffffu, (e_row[0] > -500 && e_row[0] - most_added < -24) ||
+                                                 (e_row[1] > -500 && e_row[1] - most_added < -24));
+    if (most < -500) most = 0;
+    if (most_added < -500) most_added = 0;
     if (threadIdx.x < kC) {
       // the power of two of l^u goes into the weight, the rest into z's scale
-      const int j = threadIdx.x, e = exponent(m.max_y[j]) + exponent(m.max_z[j]);
+      const int j = threadIdx.x;
+      const float sy = m.square_y[j], sz = m.square_z[j];
+      const bool any = sy != 0.f && sz != 0.f;
+      const int e = exponent(sy) + exponent(sz);
       const Decayed u(m.power, w.added(j, back));
-      const float one = e - most < -126 ? 0.f : a.y_scale * power2(min(e - most, 0)) / u.rest;
+      const float one = !any || e - most < -126 ? 0.f : __fdividef(a.y_scale * power2(e - most), u.rest);
       m.weight[j] = make_float2(one, one * m.power[back ? j & 15 : 15 - (j & 15)]);
-      const int below = u.any ? min(e + u.e - most_added, 0) : -1000;
+      const int below = any && u.any ? e + u.e - most_added : -1000;
       // 2^below as two halves, each 2^-24 at least (0: less than 2^-38 of the largest)
       const int first = max(below, -24), then = max(below - first, -24);
       m.added[0][j] = below < -38 ? 0 : __half_as_ushort(__float2half_rn(power2(first)));
       m.added[1][j] = __half_as_ushort(__float2half_rn(power2(then)));
       m.document[j] = w.document(j);
     }
-    const bool far = __any_sync(0xffffffffu, [&] {        // a weight below one half number
-      bool any = false;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int j = lane + 32 * k;
-        const Decayed u(m.power, w.added(j, back));
-        const int below = exponent(m.max_y[j]) + exponent(m.max_z[j]) + u.e - most_added;
-        any = any || (u.any && below < -24);
-      }
-      return any;
-    }());
-    // the tiles
-    auto tile = [&](auto width, int to, const float (&v)[8], int row, float up) {
+    // the tiles: y, and the state (z waits for its scales)
+    auto tile = [&](auto width, int to, const auto& v, auto up_of) {
       constexpr int W = decltype(width)::value;
-      uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) split(up * v[2 * i], up * v[2 * i + 1], hi[i], lo[i]);
-      unsigned char* p = smem + to + piece<W>(row, lane % (W / 8));
-      *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(p + kC * W * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      for (int k = 0; k < 4; ++k) {
+        const int row = row_of(W, k);
+        const float up = up_of(row);
+#pragma unroll
+        for (int i = 0; i < W / 32; ++i) {
+          uint2 hi, lo;
+          split(v[k][i].x, v[k][i].y, up, hi.x, lo.x);
+          split(v[k][i].z, v[k][i].w, up, hi.y, lo.y);
+          unsigned char* p = smem + to + piece<W>(row, 4 * i + (piece_of >> 1)) + (piece_of & 1) * 8;
+          *reinterpret_cast<uint2*>(p) = hi;
+          *reinterpret_cast<uint2*>(p + kC * W * 2) = lo;
+        }
+      }
     };
-    float max_state = 0.f;
-    int e_state = 0;
+    auto up_of = [](float square) { return square == 0.f ? 0.f : power2(kTop - exponent(square)); };
+    tile(std::integral_constant<int, P>{}, L::kY, y, [&](int row) { return up_of(m.square_y[row]); });
     if constexpr (!STATE) {
+      if (square_state > 0.f) {
+        const float up = up_of(square_state);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) max_state = fmaxf(max_state, m.max_state[i]);
-      e_state = exponent(max_state);
-      if (has_state && max_state > 0.f) {
-        const float up = power2(kTop - e_state);
+        for (int mt = 0; mt < L::kRowTiles; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < L::kColTiles; ++nt)
+          for (int nt = 0; nt < L::kColTiles; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t hi, lo;
-            split(up * X[nt][e * 2], up * X[nt][e * 2 + 1], hi, lo);
-            unsigned char* p = smem + L::kState + piece<R>(row0 + quad + e * 8, col0 / 8 + nt) + 4 * t;
-            *reinterpret_cast<uint32_t*>(p) = hi;
-            *reinterpret_cast<uint32_t*>(p + P * R * 2) = lo;
-          }
-      }
-#pragma unroll
-      for (int k = 0; k < kPassesX; ++k) {
-        const int row = row_of(P, k);
-        tile(std::integral_constant<int, P>{}, L::kX, x[k], row, power2(kTop - exponent(m.max_x[row])));
+            for (int half = 0; half < 2; ++half) {
+              uint32_t hi, lo;
+              split(X[mt][nt][half * 2], X[mt][nt][half * 2 + 1], up, hi, lo);
+              unsigned char* p = smem + L::kState +
+                                 piece<R>(row0 + mt * 16 + quad + half * 8, col0 / 8 + nt) + 4 * t;
+              *reinterpret_cast<uint32_t*>(p) = hi;
+              *reinterpret_cast<uint32_t*>(p + P * R * 2) = lo;
+            }
       }
     }
-#pragma unroll
-    for (int k = 0; k < kPassesX; ++k) {
-      const int row = row_of(P, k);
-      tile(std::integral_constant<int, P>{}, L::kY, y[k], row, power2(kTop - exponent(m.max_y[row])));
-    }
-#pragma unroll
-    for (int k = 0; k < kPassesZ; ++k) {
-      const int row = row_of(R, k);
-      tile(std::integral_constant<int, R>{}, L::kZ, z[k], row,
-           Decayed(m.power, w.added(row, back)).rest * power2(kTop - exponent(m.max_z[row])));
-    }
+    tile(std::integral_constant<int, R>{}, L::kZ, z, [&](int row) {
+      return Decayed(m.power, w.added(row, back)).rest * up_of(m.square_z[row]);
+    });
     __syncthreads();
-    if (c + 1 < c1) fetch(c + 1);
 
     if constexpr (!STATE) {
+      int e_x[2];
       uint32_t xh[P / 16][4], xl[P / 16][4];
 #pragma unroll
-      for (int k = 0; k < P / 16; ++k) {
-        const uint32_t from =
-            base + L::kX + piece<P>(group * 16 + (mat & 1) * 8 + mat_row, 2 * k + (mat >> 1));
-        load4(xh[k], from);
-        load4(xl[k], from + kC * P * 2);
+      for (int half = 0; half < 2; ++half) {
+        e_x[half] = square_x[half] == 0.f ? 0 : exponent(square_x[half]);
+        const float up = power2(kTop - e_x[half]);
+#pragma unroll
+        for (int k = 0; k < P / 16; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            split(x[k][half + 2 * e].x, x[k][half + 2 * e].y, up, xh[k][half + 2 * e],
+                  xl[k][half + 2 * e]);
       }
-      // x y^T for every other 16 positions up to (back: from) this group's own
-      float S[2][2][4];
-      float most_p[2] = {0.f, 0.f};
+      // x y^T for the positions up to (back: from) this warp's own
+      float S[kC / 8][4];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int jb = half + 2 * q;
-        if (back ? jb < group : jb > group) continue;
+      for (int jb = 0; jb < kC / 16; ++jb) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) S[q][0][e] = S[q][1][e] = 0.f;
+        for (int e = 0; e < 4; ++e) S[2 * jb][e] = S[2 * jb + 1][e] = 0.f;
+        if (back ? jb < warp : jb > warp) continue;
 #pragma unroll
         for (int k = 0; k < P / 16; ++k) {
           uint32_t bh[4], bl[4];
@@ -736,94 +736,96 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
               base + L::kY + piece<P>(jb * 16 + (mat >> 1) * 8 + mat_row, 2 * k + (mat & 1));
           load4(bh, from);
           load4(bl, from + kC * P * 2);
-          products(S[q][0], S[q][1], xh[k], xl[k], bh, bl);
-        }
-        // its weights, and the rows' largest: l^(i - j) is looked up in the group's own
-        // positions, elsewhere it is a product of three powers of at least 0
-        const float gap = jb == group ? 1.f : m.power[16 * abs(group - jb) - 15];
-        const float side[2] = {gap * m.power[back ? 15 - quad : quad],
-                               gap * m.power[back ? 7 - quad : quad + 8]};
-#pragma unroll
-        for (int jt = 0; jt < 2; ++jt) {
-          const int j = jb * 16 + jt * 8 + 2 * t;
-          const float4 v = *reinterpret_cast<const float4*>(&m.weight[j]);
-          const float one[2] = {v.x, v.z}, other[2] = {v.y, v.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float value = S[q][jt][e];
-            if (jb == group) {
-              const int i = quad + (e >> 1) * 8, k = jt * 8 + 2 * t + (e & 1);
-              const int apart = back ? k - i : i - k;
-              value = apart < 0 ? 0.f : value * (m.power[max(apart, 0)] * one[e & 1]);
-            } else {
-              value *= side[e >> 1] * other[e & 1];
-            }
-            if (w.inner && m.document[group * 16 + quad + (e >> 1) * 8] != m.document[j + (e & 1)])
-              value = 0.f;
-            S[q][jt][e] = value;
-          }
-          most_p[0] = fmax3(most_p[0], fabsf(S[q][jt][0]), fabsf(S[q][jt][1]));
-          most_p[1] = fmax3(most_p[1], fabsf(S[q][jt][2]), fabsf(S[q][jt][3]));
+          products(S[2 * jb], S[2 * jb + 1], xh[k], xl[k], bh, bl);
         }
       }
-      // x X over this half of the state's rows
+      // x X
       float o[R / 8][4];
 #pragma unroll
       for (int nt = 0; nt < R / 8; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
-      if (max_state > 0.f) {
+      if (square_state > 0.f) {
 #pragma unroll
-        for (int k = 0; k < P / 32; ++k) {
-          const int kk = half * (P / 32) + k;
-          uint32_t ah[4], al[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            ah[e] = half ? xh[P / 32 + k][e] : xh[k][e];
-            al[e] = half ? xl[P / 32 + k][e] : xl[k][e];
-          }
+        for (int k = 0; k < P / 16; ++k)
 #pragma unroll
           for (int nb = 0; nb < R / 16; ++nb) {
             uint32_t bh[4], bl[4];
             const uint32_t from = base + L::kState +
-                                  piece<R>(kk * 16 + (mat & 1) * 8 + mat_row, 2 * nb + (mat >> 1));
+                                  piece<R>(k * 16 + (mat & 1) * 8 + mat_row, 2 * nb + (mat >> 1));
             load4_turned(bh, from);
             load4_turned(bl, from + P * R * 2);
-            products(o[2 * nb], o[2 * nb + 1], ah, al, bh, bl);
+            products(o[2 * nb], o[2 * nb + 1], xh[k], xl[k], bh, bl);
           }
+      }
+      // The weights of x y^T, and the rows' largest: l^(i - j) is looked up in the warp's
+      // own positions, elsewhere it is a product of three powers of at least 0.
+      float most_p[2] = {0.f, 0.f};
+#pragma unroll
+      for (int jb = 0; jb < kC / 16; ++jb) {
+        if (back ? jb < warp : jb > warp) continue;
+        const float gap = jb == warp ? 1.f : m.power[16 * abs(warp - jb) - 15];
+        const float side[2] = {gap * m.power[back ? 15 - quad : quad],
+                               gap * m.power[back ? 7 - quad : quad + 8]};
+#pragma unroll
+        for (int jt = 0; jt < 2; ++jt) {
+          float(&v)[4] = S[2 * jb + jt];
+          const int j = jb * 16 + jt * 8 + 2 * t;
+          const float4 f = *reinterpret_cast<const float4*>(&m.weight[j]);
+          if (jb == warp) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = quad + (e >> 1) * 8, k = jt * 8 + 2 * t + (e & 1);
+              const int apart = back ? k - i : i - k;
+              v[e] = apart < 0 ? 0.f : v[e] * (m.power[max(apart, 0)] * (e & 1 ? f.z : f.x));
+            }
+          } else {
+            mul2(v[0], v[1], v[0], v[1], f.y, f.w);
+            mul2(v[2], v[3], v[2], v[3], f.y, f.w);
+            mul2(v[0], v[1], v[0], v[1], side[0], side[0]);
+            mul2(v[2], v[3], v[2], v[3], side[1], side[1]);
+          }
+          if (w.inner) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (m.document[warp * 16 + quad + (e >> 1) * 8] != m.document[j + (e & 1)]) v[e] = 0.f;
+          }
+          most_p[0] = fmax3(most_p[0], fabsf(v[0]), fabsf(v[1]));
+          most_p[1] = fmax3(most_p[1], fabsf(v[2]), fabsf(v[3]));
         }
       }
       // Both sums in one scale: the larger's, whichever part it comes from.
-      Scale by[2] = {Scale(0.f, 0), Scale(0.f, 0)};
       float up[2];
+      float by[2], then[2];
+      const int apart = (square_state > 0.f ? exponent(square_state) : 0) + 2 * kTop - most;
 #pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        const int i = group * 16 + quad + side * 8, u = w.reach(i, back);
-        most_p[side] = fmaxf(most_p[side], __shfl_xor_sync(0xffffffffu, most_p[side], 1));
-        most_p[side] = fmaxf(most_p[side], __shfl_xor_sync(0xffffffffu, most_p[side], 2));
-        int e_p = exponent(most_p[side]);
-        const float decay = u < 0 ? 0.f : m.power[u];
-        const int apart = e_state + 2 * kTop - most;
-        if (max_state > 0.f && decay > 0.f) e_p = max(e_p, apart + exponent(decay) - kTop);
-        const Scale in(decay, apart - e_p);
+      for (int half = 0; half < 2; ++half) {
+        const int i = warp * 16 + quad + half * 8;
+        most_p[half] = fmaxf(most_p[half], __shfl_xor_sync(0xffffffffu, most_p[half], 1));
+        most_p[half] = fmaxf(most_p[half], __shfl_xor_sync(0xffffffffu, most_p[half], 2));
+        int e_p = max((int)(__float_as_uint(most_p[half]) >> 23) - 127, -110);
+        const Decayed u(m.power, w.reach(i, back));
+        if (square_state > 0.f) {
+          if (u.any) e_p = max(e_p, apart + u.e - kTop);
+          const int e_in = u.e + apart - e_p;
+          const float in = !u.any || e_in < -126 ? 0.f : u.rest * power2(e_in);
 #pragma unroll
-        for (int nt = 0; nt < R / 8; ++nt) {
-          o[nt][2 * side] = in(o[nt][2 * side]);
-          o[nt][2 * side + 1] = in(o[nt][2 * side + 1]);
+          for (int nt = 0; nt < R / 8; ++nt)
+            mul2(o[nt][2 * half], o[nt][2 * half + 1], o[nt][2 * half], o[nt][2 * half + 1], in, in);
         }
-        up[side] = kTop - e_p < -126 ? 0.f : power2(kTop - e_p);
-        by[side] = Scale(a.out_scale, e_p + exponent(m.max_x[i]) + most - 4 * kTop);
+        up[half] = kTop - e_p < -126 ? 0.f : power2(kTop - e_p);
+        const Scale scale(a.out_scale, e_p + e_x[half] + most - 4 * kTop);
+        by[half] = scale.first;
+        then[half] = scale.then;
       }
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int jb = half + 2 * q;
-        if (back ? jb < group : jb > group) continue;
+      for (int jb = 0; jb < kC / 16; ++jb) {
+        if (back ? jb < warp : jb > warp) continue;
         uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float f = up[e & 1];
-          split(f * S[q][e >> 1][(e & 1) * 2], f * S[q][e >> 1][(e & 1) * 2 + 1], ph[e], pl[e]);
-        }
+        for (int e = 0; e < 4; ++e)
+          split(S[2 * jb + (e >> 1)][(e & 1) * 2], S[2 * jb + (e >> 1)][(e & 1) * 2 + 1], up[e & 1],
+                ph[e], pl[e]);
 #pragma unroll
         for (int nb = 0; nb < R / 16; ++nb) {
           uint32_t bh[4], bl[4];
@@ -834,73 +836,59 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
           products(o[2 * nb], o[2 * nb + 1], ph, pl, bh, bl);
         }
       }
+      const bool twice = __any_sync(0xffffffffu, then[0] != 1.f || then[1] != 1.f);
 #pragma unroll
-      for (int nt = 0; nt < R / 8; ++nt)
+      for (int half = 0; half < 2; ++half) {
+        const int i = warp * 16 + quad + half * 8, room = a.r - slice * R;
+        float* out = a.out + ((b * s.T + t0 + i) * s.H + h) * a.r + slice * R + 2 * t;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[nt][e] = by[e >> 1](o[nt][e]);
-      // each half of the group writes half of the columns
-      pair_barrier(group);                                // both have read x's tile
-      auto finish = [&](auto which) {
-        constexpr int kMine = decltype(which)::value * (R / 16), kOther = R / 16 - kMine;
-        float2* sums = reinterpret_cast<float2*>(smem + L::kSums + group * L::kGroup);
-        constexpr int kApart = L::kHalf / (int)sizeof(float2);
-#pragma unroll
-        for (int k = 0; k < R / 16; ++k)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            sums[decltype(which)::value * kApart + (2 * k + e) * 32 + lane] =
-                make_float2(o[kOther + k][2 * e], o[kOther + k][2 * e + 1]);
-        pair_barrier(group);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = group * 16 + quad + e * 8;
-          float* out = a.out + ((b * s.T + t0 + i) * s.H + h) * a.r + slice * R;
-#pragma unroll
-          for (int k = 0; k < R / 16; ++k) {
-            const float2 more = sums[(1 - decltype(which)::value) * kApart + (2 * k + e) * 32 + lane];
-            const float v0 = o[kMine + k][2 * e] + more.x, v1 = o[kMine + k][2 * e + 1] + more.y;
-            const int r = (kMine + k) * 8 + 2 * t, room = a.r - slice * R;
-            odd = fmaf(v0, 0.f, odd);
-            odd = fmaf(v1, 0.f, odd);
-            if (i >= n) continue;
-            if (pairs_o) {
-              if (r < room) *reinterpret_cast<float2*>(out + r) = make_float2(v0, v1);
-            } else {
-              if (r < room) out[r] = v0;
-              if (r + 1 < room) out[r + 1] = v1;
-            }
+        for (int nt = 0; nt < R / 8; ++nt) {
+          float v0, v1;
+          mul2(v0, v1, o[nt][half * 2], o[nt][half * 2 + 1], by[half], by[half]);
+          if (twice) mul2(v0, v1, v0, v1, then[half], then[half]);
+          const int r = nt * 8 + 2 * t;
+          if (i >= n) continue;
+          if (pairs_o) {
+            if (r < room) *reinterpret_cast<float2*>(out + nt * 8) = make_float2(v0, v1);
+          } else {
+            if (r < room) out[nt * 8] = v0;
+            if (r + 1 < room) out[nt * 8 + 1] = v1;
           }
         }
-      };
-      if (half == 0)
-        finish(std::integral_constant<int, 0>{});
-      else
-        finish(std::integral_constant<int, 1>{});
-      if (c + 1 < c1) fetch_x(c + 1);
+      }
     }
-    // what the chunk adds to the state
+    // the state: what the chunk adds, then in 32 bits
+    const Scale by(a.y_scale, most_added - 2 * kTop);
 #pragma unroll
-    for (int nt = 0; nt < L::kColTiles; ++nt)
+    for (int mt = 0; mt < L::kRowTiles; ++mt) {
+      float d[L::kColTiles][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
-    if (has_state) {
+      for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
 #pragma unroll
       for (int k = 0; k < kC / 16; ++k) {
         uint32_t ah[4], al[4];
-        const uint32_t from =
-            base + L::kY + piece<P>(k * 16 + (mat >> 1) * 8 + mat_row, row0 / 8 + (mat & 1));
+        const uint32_t from = base + L::kY + piece<P>(k * 16 + (mat >> 1) * 8 + mat_row,
+                                                      (row0 + mt * 16) / 8 + (mat & 1));
         load4_turned(ah, from);
         load4_turned(al, from + kC * P * 2);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = k * 16 + (e >> 1) * 8 + 2 * t;
+        for (int half = 0; half < 2; ++half) {
+          const int j = k * 16 + half * 8 + 2 * t;
           const uint32_t f = *reinterpret_cast<const uint32_t*>(&m.added[0][j]);
-          ah[e] = times(ah[e], f);
-          al[e] = times(al[e], f);
+#pragma unroll
+          for (int e = 2 * half; e < 2 * half + 2; ++e) {
+            ah[e] = times(ah[e], f);
+            al[e] = times(al[e], f);
+          }
           if (far) {
             const uint32_t f2 = *reinterpret_cast<const uint32_t*>(&m.added[1][j]);
-            ah[e] = times(ah[e], f2);
-            al[e] = times(al[e], f2);
+#pragma unroll
+            for (int e = 2 * half; e < 2 * half + 2; ++e) {
+              ah[e] = times(ah[e], f2);
+              al[e] = times(al[e], f2);
+            }
           }
         }
 #pragma unroll
@@ -913,28 +901,32 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
           products(d[2 * nb], d[2 * nb + 1], ah, al, bh, bl);
         }
       }
+      if (by.then != 1.f) {
+#pragma unroll
+        for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[nt][e] *= by.then;
+      }
+#pragma unroll
+      for (int nt = 0; nt < L::kColTiles; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          float(&v)[4] = X[mt][nt];
+          mul2(v[e], v[e + 1], v[e], v[e + 1], kept, kept);
+          fma2(v[e], v[e + 1], d[nt][e], d[nt][e + 1], by.first, by.first, v[e], v[e + 1]);
+        }
     }
-    by_d = Scale(a.y_scale, most_added - 2 * kTop);
-    const int u = w.kept(back);
-    kept = u < 0 ? 0.f : m.power[u];
-    if (STATE) run *= kept;
-#pragma unroll
-    for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) odd = fmaf(d[nt][e], 0.f, fmaf(X[nt][e], 0.f, odd));
   }
 
-  const bool keep = has_state && (STATE || (a.last && seg == pieces - 1));
-  float* to = STATE ? g.state + ((pass * (int64_t)pieces + seg) * heads + b * s.H + h) * a.p * a.r
-                    : a.last + (b * s.H + h) * (int64_t)a.p * a.r;
-  const int64_t ps = STATE ? a.r : a.p_stride, rs = STATE ? 1 : a.r_stride;
-#pragma unroll
-  for (int nt = 0; nt < L::kColTiles; ++nt)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int p = row0 + quad + (e >> 1) * 8, r = slice * R + col0 + nt * 8 + 2 * t + (e & 1);
-      if (keep && p < a.p && r < a.r) to[p * ps + r * rs] = X[nt][e];
-    }
+  if (STATE || (a.last && seg == pieces - 1)) {
+    float* to = STATE ? g.state + ((pass * (int64_t)pieces + seg) * heads + b * s.H + h) * a.p * a.r
+                      : a.last + (b * s.H + h) * (int64_t)a.p * a.r;
+    const int64_t ps = STATE ? a.r : a.p_stride, rs = STATE ? 1 : a.r_stride;
+    each([&](float v, int p, int c) {
+      const int r = slice * R + c;
+      if (p < a.p && r < a.r) to[p * ps + r * rs] = v;
+    });
+  }
   if (STATE && threadIdx.x == 0)
     g.kept[(pass * (int64_t)pieces + seg) * heads + b * s.H + h] = run;
 }
@@ -1073,6 +1065,55 @@ int allow_smem(K kernel, int bytes) {
   return WXX_OK;
 }
 
+// How many pieces a row of `chunks` is worked on in, for `blocks` rows (sequences, heads, slices
+// and passes) on `resident` places: the fewest turns of the outputs' launch and, with more
+// than one piece, of the states' one (half as long a chunk; a start is about a chunk, the
+// launches in between one and a half).
+int pieces_of(int64_t blocks, int64_t chunks, int64_t resident) {
+  double least = 0;
+  int best = 1;
+  for (int m = 1; m <= 64 && 2 * m <= chunks + 1; ++m) {
+    const int64_t size = (chunks + m - 1) / m;
+    if ((chunks + size - 1) / size != m) continue;
+    auto turns = [&](int64_t n) { return (double)((n + resident - 1) / resident); };
+    double cost = turns(blocks * m) * (size + 1);
+    if (m > 1) cost += turns(blocks * (m - 1)) * (0.5 * size + 1) + 1.5;
+    if (m == 1 || cost < least) least = cost, best = m;
+  }
+  return best;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault,
+                                         &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    cudaGetLastError();
+  });
+  return fn;
+}
+
+// A map of boxes of 32 channels of a head by 64 positions, where the copy engine takes the
+// operand: a 16-byte aligned base and strides.
+bool encode(CUtensorMap* map, const Operand& o, int64_t B, int64_t T, int64_t H, int64_t width) {
+  auto enc = get_encode();
+  const int64_t bs = B > 1 ? o.bs : T * o.ts;
+  if (!enc || (reinterpret_cast<uintptr_t>(o.p) & 15) || (o.ts | bs | width) & 3 || o.ts <= 0 ||
+      bs <= 0 || o.ts >= (int64_t(1) << 37) || bs >= (int64_t(1) << 37))
+    return false;
+  cuuint64_t dims[4] = {(cuuint64_t)width, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)width * 4, (cuuint64_t)o.ts * 4, (cuuint64_t)bs * 4};
+  cuuint32_t box[4] = {32, 1, kC, 1}, ones[4] = {1, 1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, const_cast<float*>(o.p), dims, strides, box,
+             ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // n passes of one padded size in one launch, the rows in pieces where there are too few
 // sequences and heads to fill the SMs: first what every piece but the last adds to a state,
 // then the states before the pieces, then the outputs.
@@ -1080,20 +1121,21 @@ template <int P, int R>
 int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
   using L = Layout<P, R>;
   const Pass& a = passes.at[0];
-  int slices = 0;
-  for (int i = 0; i < n; ++i) slices = std::max(slices, (passes.at[i].r + R - 1) / R);
+  const int slices = (a.r + R - 1) / R;
   const int64_t heads = B * s.H, blocks = heads * slices, chunks = (s.T + kC - 1) / kC;
-  const int64_t resident = (int64_t)wxx::num_sms() * L::kBlocks;
-  Segments g{1, (int)chunks, nullptr, nullptr};
-  const int64_t most = resident / (blocks * n);
-  if (most >= 2) {
-    int64_t size = (chunks + most - 1) / most;
-    if (size < 4) size = 4;
-    g.count = (int)((chunks + size - 1) / size);
-    g.chunks = (int)size;
+  Segments g{pieces_of(blocks * n, chunks, (int64_t)wxx::num_sms() * L::kBlocks), 0, nullptr, nullptr};
+  g.chunks = (int)((chunks + g.count - 1) / g.count);
+  WXX_REQUIRE(blocks * n * g.count < (int64_t(1) << 31), "linear attention: too many sequences");
+  Maps maps{};
+  bool tma = true;
+  for (int i = 0; i < n; ++i) {
+    const Pass& p = passes.at[i];
+    tma = tma && encode(&maps.x[i], p.x, B, s.T, s.H, p.p) &&
+          encode(&maps.y[i], p.y, B, s.T, s.H, p.p) && encode(&maps.z[i], p.z, B, s.T, s.H, p.r);
   }
   if (int st = allow_smem(chunk_kernel<P, R, true>, L::kBytes)) return st;
   if (int st = allow_smem(chunk_kernel<P, R, false>, L::kBytes)) return st;
+  int* err = wxx::device_error_word();
   void* scratch = nullptr;
   if (g.count > 1) {
     const int64_t states = n * (g.count - 1) * heads;
@@ -1102,7 +1144,8 @@ int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
     g.state = static_cast<float*>(scratch);
     g.kept = g.state + states * a.p * a.r;
     const unsigned per = (unsigned)(blocks * (g.count - 1));
-    chunk_kernel<P, R, true><<<per * n, kThreads, L::kBytes, wxx::stream()>>>(passes, s, g, per);
+    chunk_kernel<P, R, true><<<per * n, kThreads, L::kBytes, wxx::stream()>>>(passes, maps, tma, s, g,
+                                                                            per, err);
     int st = wxx::after_launch(__FILE__, __LINE__);
     if (st == WXX_OK) {
       const int64_t total = heads * a.p * a.r;
@@ -1116,7 +1159,8 @@ int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
     }
   }
   const unsigned per = (unsigned)(blocks * g.count);
-  chunk_kernel<P, R, false><<<per * n, kThreads, L::kBytes, wxx::stream()>>>(passes, s, g, per);
+  chunk_kernel<P, R, false><<<per * n, kThreads, L::kBytes, wxx::stream()>>>(passes, maps, tma, s, g,
+                                                                           per, err);
   const int st = wxx::after_launch(__FILE__, __LINE__);
   if (scratch) wxx_free(scratch);
   return st;
