@@ -199,6 +199,11 @@ __device__ __forceinline__ void load4_turned(uint32_t (&r)[4], uint32_t at) {
                : "r"(at)
                : "memory");
 }
+__device__ __forceinline__ void store4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a),
+               "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
 __device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
@@ -261,7 +266,8 @@ struct Scale {
 };
 
 // Tiles of W half numbers a row for ldmatrix: 16-byte pieces of a row exchanged so that
-// the same piece of 8 rows lies in 8 different sets of banks.
+// the same piece of 8 rows lies in 8 different sets of banks.  (q ^ k << 1 is the address of q
+// with k << 5 exchanged: how the products below step through a row.)
 template <int W>
 __device__ __forceinline__ uint32_t piece(int row, int q) {
   const int turn = W == 32 ? (row >> 1) & 3 : row & 7;
@@ -500,6 +506,18 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
   const bool pairs_o = ((reinterpret_cast<uintptr_t>(a.out) & 7) == 0) && (a.r & 1) == 0;
   float run = 1.f;                      // STATE: what the piece does to the state before it
 
+  // Where this lane reads y (and, across rows, y^T), z and the state for the products: the
+  // first 16 rows, the first 16 columns; 16 columns on is an address with 1 << 5 exchanged.
+  const uint32_t read_y = base + L::kY + piece<P>((mat >> 1) * 8 + mat_row, mat & 1);
+  const uint32_t read_z = base + L::kZ + piece<R>((mat & 1) * 8 + mat_row, mat >> 1);
+  const uint32_t read_state = base + L::kState + piece<R>((mat & 1) * 8 + mat_row, mat >> 1);
+  // y and z by rows: a lane has 4 of every 32 columns; a pass of a warp takes 4 of its 16
+  // rows (64 columns and more: two of them 4 apart, for the banks of the tiles)
+  const int piece_of = lane & 7, sub = lane >> 3;
+  auto first_row = [&](int W) { return warp * 16 + (W == 32 ? sub : (sub & 1) * 4 + (sub >> 1)); };
+  auto next_row = [](int W, int k) { return W == 32 ? 4 * k : (k >> 1) * 8 + (k & 1) * 2; };
+  auto row_of = [&](int W, int k) { return first_row(W) + next_row(W, k); };
+
   for (int c = c0; c < c1; ++c) {
     const int t0 = start(c), n = min(kC, s.T - t0);
     // the resets of the chunk, and of the position after it
@@ -539,21 +557,17 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
       copies_done();
     __syncthreads();       // the operands are here, the last chunk's tiles are read
 
-    // y and z by rows: a lane has 4 of every 32 columns; a pass of a warp takes 4 of its 16
-    // rows (64 columns and more: two of them 4 apart, for the banks of the tiles)
-    const int piece_of = lane & 7, sub = lane >> 3;
-    auto row_of = [&](int W, int k) {
-      return warp * 16 + (W == 32 ? 4 * k + sub : (k >> 1) * 8 + (k & 1) * 2 + (sub & 1) * 4 + (sub >> 1));
-    };
+    bool rare = false;                  // a row's square is out of range
     float4 y[4][P / 32], z[4][R / 32];
     auto read = [&](auto width, int raw, auto& v, float* squares) {
       constexpr int W = decltype(width)::value;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int row = row_of(W, k);
+        const int from = (raw_piece(first_row(W), piece_of) * 16 ^ ((k & 1) << (W == 32 ? 6 : 5))) +
+                         next_row(W, k) * 128;
 #pragma unroll
         for (int i = 0; i < W / 32; ++i)
-          v[k][i] = reinterpret_cast<const float4*>(smem + raw + i * kRaw)[raw_piece(row, piece_of)];
+          v[k][i] = *reinterpret_cast<const float4*>(smem + raw + i * kRaw + from);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -566,12 +580,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
         s0 += s1;
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-        if (!(s0 >= kShort && s0 < kLong)) {
-          odd = odd || !(s0 < kLong);
-#pragma unroll
-          for (int i = 0; i < W / 32; ++i)
-            odd = odd || v[k][i].x != 0.f || v[k][i].y != 0.f || v[k][i].z != 0.f || v[k][i].w != 0.f;
-        }
+        rare = rare || !(s0 >= kShort && s0 < kLong);
         if (piece_of == 0) squares[row_of(W, k)] = s0;
       }
     };
@@ -583,14 +592,15 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
     if constexpr (!STATE) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int row = warp * 16 + quad + half * 8;
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int k = 0; k < P / 16; ++k)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const unsigned char* p = smem + L::kRawX + (k >> 1) * kRaw +
-                                     raw_piece(row, 4 * (k & 1) + 2 * e + (t >> 1)) * 16 + (t & 1) * 8;
+            const unsigned char* p =
+                smem + L::kRawX + (k >> 1) * kRaw +
+                ((raw_piece(warp * 16 + quad, t >> 1) * 16 + (t & 1) * 8) ^ ((4 * (k & 1) + 2 * e) << 4)) +
+                half * 8 * 128;
             const float2 v = *reinterpret_cast<const float2*>(p);
             x[k][half + 2 * e] = v;
             square2(s0, s1, v.x, v.y);
@@ -599,14 +609,31 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
         s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
         s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
         square_x[half] = s0;
-        if (!(s0 >= kShort && s0 < kLong)) {
-          odd = odd || !(s0 < kLong);
+        rare = rare || !(s0 >= kShort && s0 < kLong);
+      }
+    }
+    if (__any_sync(0xffffffffu, rare)) {       // rows of zeros are fine
+      auto look = [&](const float* squares, int W, int row, float v0, float v1, float v2, float v3) {
+        const float s0 = squares[row];
+        odd = odd || !(s0 < kLong) ||
+              (s0 < kShort && (v0 != 0.f || v1 != 0.f || v2 != 0.f || v3 != 0.f));
+      };
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int i = 0; i < P / 32; ++i)
+          look(m.square_y, P, row_of(P, k), y[k][i].x, y[k][i].y, y[k][i].z, y[k][i].w);
+#pragma unroll
+        for (int i = 0; i < R / 32; ++i)
+          look(m.square_z, R, row_of(R, k), z[k][i].x, z[k][i].y, z[k][i].z, z[k][i].w);
+      }
+      if constexpr (!STATE) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int k = 0; k < P / 16; ++k)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              odd = odd || x[k][half + 2 * e].x != 0.f || x[k][half + 2 * e].y != 0.f;
-        }
+            look(square_x, 1, half, x[k][half].x, x[k][half].y, x[k][half + 2].x, x[k][half + 2].y);
       }
     }
     odd = __syncthreads_or(odd);        // the squares are here, the operands are read
@@ -677,7 +704,9 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
           uint2 hi, lo;
           split(v[k][i].x, v[k][i].y, up, hi.x, lo.x);
           split(v[k][i].z, v[k][i].w, up, hi.y, lo.y);
-          unsigned char* p = smem + to + piece<W>(row, 4 * i + (piece_of >> 1)) + (piece_of & 1) * 8;
+          unsigned char* p = smem + to + next_row(W, k) * W * 2 +
+                             ((piece<W>(first_row(W), piece_of >> 1) + (piece_of & 1) * 8) ^
+                              ((k & 1) << 5) ^ (i << 6));
           *reinterpret_cast<uint2*>(p) = hi;
           *reinterpret_cast<uint2*>(p + kC * W * 2) = lo;
         }
@@ -691,16 +720,16 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
         for (int mt = 0; mt < L::kRowTiles; ++mt)
 #pragma unroll
-          for (int nt = 0; nt < L::kColTiles; ++nt)
+          for (int nt = 0; nt < L::kColTiles; nt += 2) {
+            uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              uint32_t hi, lo;
-              split(X[mt][nt][half * 2], X[mt][nt][half * 2 + 1], up, hi, lo);
-              unsigned char* p = smem + L::kState +
-                                 piece<R>(row0 + mt * 16 + quad + half * 8, col0 / 8 + nt) + 4 * t;
-              *reinterpret_cast<uint32_t*>(p) = hi;
-              *reinterpret_cast<uint32_t*>(p + P * R * 2) = lo;
-            }
+            for (int e = 0; e < 4; ++e)
+              split(X[mt][nt + (e >> 1)][(e & 1) * 2], X[mt][nt + (e >> 1)][(e & 1) * 2 + 1], up, hi[e],
+                    lo[e]);
+            const uint32_t to = (read_state ^ ((col0 / 16 + nt / 2) << 5)) + (row0 + mt * 16) * R * 2;
+            store4(to, hi[0], hi[1], hi[2], hi[3]);
+            store4(to + P * R * 2, lo[0], lo[1], lo[2], lo[3]);
+          }
       }
     }
     tile(std::integral_constant<int, R>{}, L::kZ, z, [&](int row) {
@@ -726,17 +755,29 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
       float S[kC / 8][4];
 #pragma unroll
       for (int jb = 0; jb < kC / 16; ++jb) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) S[2 * jb][e] = S[2 * jb + 1][e] = 0.f;
         if (back ? jb < warp : jb > warp) continue;
+        float small[2][4];                // the products with low halves
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          S[2 * jb][e] = S[2 * jb + 1][e] = small[0][e] = small[1][e] = 0.f;
 #pragma unroll
         for (int k = 0; k < P / 16; ++k) {
           uint32_t bh[4], bl[4];
-          const uint32_t from =
-              base + L::kY + piece<P>(jb * 16 + (mat >> 1) * 8 + mat_row, 2 * k + (mat & 1));
+          const uint32_t from = (read_y ^ (k << 5)) + jb * 16 * P * 2;
           load4(bh, from);
           load4(bl, from + kC * P * 2);
-          products(S[2 * jb], S[2 * jb + 1], xh[k], xl[k], bh, bl);
+          product(small[0], xl[k], bh[0], bh[1]);
+          product(small[1], xl[k], bh[2], bh[3]);
+          product(S[2 * jb], xh[k], bh[0], bh[1]);
+          product(S[2 * jb + 1], xh[k], bh[2], bh[3]);
+          product(small[0], xh[k], bl[0], bl[1]);
+          product(small[1], xh[k], bl[2], bl[3]);
+        }
+#pragma unroll
+        for (int jt = 0; jt < 2; ++jt) {
+          float(&v)[4] = S[2 * jb + jt];
+          add2(v[0], v[1], v[0], v[1], small[jt][0], small[jt][1]);
+          add2(v[2], v[3], v[2], v[3], small[jt][2], small[jt][3]);
         }
       }
       // x X
@@ -751,8 +792,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
           for (int nb = 0; nb < R / 16; ++nb) {
             uint32_t bh[4], bl[4];
-            const uint32_t from = base + L::kState +
-                                  piece<R>(k * 16 + (mat & 1) * 8 + mat_row, 2 * nb + (mat >> 1));
+            const uint32_t from = (read_state ^ (nb << 5)) + k * 16 * R * 2;
             load4_turned(bh, from);
             load4_turned(bl, from + P * R * 2);
             products(o[2 * nb], o[2 * nb + 1], xh[k], xl[k], bh, bl);
@@ -785,14 +825,23 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
             mul2(v[0], v[1], v[0], v[1], side[0], side[0]);
             mul2(v[2], v[3], v[2], v[3], side[1], side[1]);
           }
-          if (w.inner) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (m.document[warp * 16 + quad + (e >> 1) * 8] != m.document[j + (e & 1)]) v[e] = 0.f;
-          }
-          most_p[0] = fmax3(most_p[0], fabsf(v[0]), fabsf(v[1]));
-          most_p[1] = fmax3(most_p[1], fabsf(v[2]), fabsf(v[3]));
         }
+      }
+      if (w.inner) {
+#pragma unroll
+        for (int jt = 0; jt < kC / 8; ++jt) {
+          if (back ? jt / 2 < warp : jt / 2 > warp) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (m.document[warp * 16 + quad + (e >> 1) * 8] != m.document[jt * 8 + 2 * t + (e & 1)])
+              S[jt][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int jt = 0; jt < kC / 8; ++jt) {
+        if (back ? jt / 2 < warp : jt / 2 > warp) continue;
+        most_p[0] = fmax3(most_p[0], fabsf(S[jt][0]), fabsf(S[jt][1]));
+        most_p[1] = fmax3(most_p[1], fabsf(S[jt][2]), fabsf(S[jt][3]));
       }
       // Both sums in one scale: the larger's, whichever part it comes from.
       float up[2];
@@ -829,32 +878,41 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
         for (int nb = 0; nb < R / 16; ++nb) {
           uint32_t bh[4], bl[4];
-          const uint32_t from =
-              base + L::kZ + piece<R>(jb * 16 + (mat & 1) * 8 + mat_row, 2 * nb + (mat >> 1));
+          const uint32_t from = (read_z ^ (nb << 5)) + jb * 16 * R * 2;
           load4_turned(bh, from);
           load4_turned(bl, from + kC * R * 2);
           products(o[2 * nb], o[2 * nb + 1], ph, pl, bh, bl);
         }
       }
-      const bool twice = __any_sync(0xffffffffu, then[0] != 1.f || then[1] != 1.f);
+      const int room = a.r - slice * R;
+      const bool plain = pairs_o && n == kC && room >= R;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int i = warp * 16 + quad + half * 8, room = a.r - slice * R;
-        float* out = a.out + ((b * s.T + t0 + i) * s.H + h) * a.r + slice * R + 2 * t;
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int nt = 0; nt < R / 8; ++nt)
+          mul2(o[nt][half * 2], o[nt][half * 2 + 1], o[nt][half * 2], o[nt][half * 2 + 1], by[half],
+               by[half]);
+      if (__any_sync(0xffffffffu, then[0] != 1.f || then[1] != 1.f)) {
+#pragma unroll
+        for (int nt = 0; nt < R / 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][e] *= then[e >> 1];
+      }
+      float* out = a.out + ((b * s.T + t0 + warp * 16 + quad) * s.H + h) * a.r + slice * R + 2 * t;
+      const int64_t eight = (int64_t)8 * s.H * a.r;
+      if (plain) {
 #pragma unroll
         for (int nt = 0; nt < R / 8; ++nt) {
-          float v0, v1;
-          mul2(v0, v1, o[nt][half * 2], o[nt][half * 2 + 1], by[half], by[half]);
-          if (twice) mul2(v0, v1, v0, v1, then[half], then[half]);
-          const int r = nt * 8 + 2 * t;
-          if (i >= n) continue;
-          if (pairs_o) {
-            if (r < room) *reinterpret_cast<float2*>(out + nt * 8) = make_float2(v0, v1);
-          } else {
-            if (r < room) out[nt * 8] = v0;
-            if (r + 1 < room) out[nt * 8 + 1] = v1;
-          }
+          *reinterpret_cast<float2*>(out + nt * 8) = make_float2(o[nt][0], o[nt][1]);
+          *reinterpret_cast<float2*>(out + eight + nt * 8) = make_float2(o[nt][2], o[nt][3]);
         }
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < R / 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (warp * 16 + quad + (e >> 1) * 8 < n && nt * 8 + 2 * t + (e & 1) < room)
+              out[(e >> 1) * eight + nt * 8 + (e & 1)] = o[nt][e];
       }
     }
     // the state: what the chunk adds, then in 32 bits
@@ -869,8 +927,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
       for (int k = 0; k < kC / 16; ++k) {
         uint32_t ah[4], al[4];
-        const uint32_t from = base + L::kY + piece<P>(k * 16 + (mat >> 1) * 8 + mat_row,
-                                                      (row0 + mt * 16) / 8 + (mat & 1));
+        const uint32_t from = (read_y ^ ((row0 / 16 + mt) << 5)) + k * 16 * P * 2;
         load4_turned(ah, from);
         load4_turned(al, from + kC * P * 2);
 #pragma unroll
@@ -894,8 +951,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
         for (int nb = 0; nb < L::kColTiles / 2; ++nb) {
           uint32_t bh[4], bl[4];
-          const uint32_t zat = base + L::kZ + piece<R>(k * 16 + (mat & 1) * 8 + mat_row,
-                                                       col0 / 8 + 2 * nb + (mat >> 1));
+          const uint32_t zat = (read_z ^ ((col0 / 16 + nb) << 5)) + k * 16 * R * 2;
           load4_turned(bh, zat);
           load4_turned(bl, zat + kC * R * 2);
           products(d[2 * nb], d[2 * nb + 1], ah, al, bh, bl);
