@@ -187,22 +187,34 @@ __device__ __forceinline__ void copy4(uint32_t to, const float* from, bool take)
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// Four 8 x 8 matrices of halves at `at` and a constant; turned: each the other way round.
+template <int OFF>
 __device__ __forceinline__ void load4(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4 + %5];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(at)
+               : "r"(at), "n"(OFF)
                : "memory");
 }
+template <int OFF>
 __device__ __forceinline__ void load4_turned(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4 + %5];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(at)
+               : "r"(at), "n"(OFF)
                : "memory");
 }
+template <int OFF>
 __device__ __forceinline__ void store4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a),
-               "r"(b), "r"(c), "r"(d)
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0 + %5], {%1, %2, %3, %4};" ::"r"(at),
+               "r"(a), "r"(b), "r"(c), "r"(d), "n"(OFF)
                : "memory");
+}
+// f with each of 0 to N - 1 as a constant.
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void for_each(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    for_each<N, I + 1>(f);
+  }
 }
 __device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
@@ -559,7 +571,9 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 
     bool rare = false;                  // a row's square is out of range
     float4 y[4][P / 32], z[4][R / 32];
-    auto read = [&](auto width, int raw, auto& v, float* squares) {
+    auto up_of = [](float square) { return square == 0.f ? 0.f : power2(kTop - exponent(square)); };
+    float up_y[4], up_z[4];
+    auto read = [&](auto width, int raw, auto& v, float* squares, float (&up)[4]) {
       constexpr int W = decltype(width)::value;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -581,11 +595,12 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
         rare = rare || !(s0 >= kShort && s0 < kLong);
+        up[k] = up_of(s0);
         if (piece_of == 0) squares[row_of(W, k)] = s0;
       }
     };
-    read(std::integral_constant<int, P>{}, L::kRawY, y, m.square_y);
-    read(std::integral_constant<int, R>{}, L::kRawZ, z, m.square_z);
+    read(std::integral_constant<int, P>{}, L::kRawY, y, m.square_y, up_y);
+    read(std::integral_constant<int, R>{}, L::kRawZ, z, m.square_z, up_z);
     // x of this warp's positions, in the layout of a product's left operand
     float2 x[STATE ? 1 : P / 16][4];
     float square_x[2] = {0.f, 0.f};
@@ -693,12 +708,11 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
       m.document[j] = w.document(j);
     }
     // the tiles: y, and the state (z waits for its scales)
-    auto tile = [&](auto width, int to, const auto& v, auto up_of) {
+    auto tile = [&](auto width, int to, const auto& v, const float (&ups)[4]) {
       constexpr int W = decltype(width)::value;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int row = row_of(W, k);
-        const float up = up_of(row);
+        const float up = ups[k];
 #pragma unroll
         for (int i = 0; i < W / 32; ++i) {
           uint2 hi, lo;
@@ -712,8 +726,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
         }
       }
     };
-    auto up_of = [](float square) { return square == 0.f ? 0.f : power2(kTop - exponent(square)); };
-    tile(std::integral_constant<int, P>{}, L::kY, y, [&](int row) { return up_of(m.square_y[row]); });
+    tile(std::integral_constant<int, P>{}, L::kY, y, up_y);
     if constexpr (!STATE) {
       if (square_state > 0.f) {
         const float up = up_of(square_state);
@@ -727,14 +740,14 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
               split(X[mt][nt + (e >> 1)][(e & 1) * 2], X[mt][nt + (e >> 1)][(e & 1) * 2 + 1], up, hi[e],
                     lo[e]);
             const uint32_t to = (read_state ^ ((col0 / 16 + nt / 2) << 5)) + (row0 + mt * 16) * R * 2;
-            store4(to, hi[0], hi[1], hi[2], hi[3]);
-            store4(to + P * R * 2, lo[0], lo[1], lo[2], lo[3]);
+            store4<0>(to, hi[0], hi[1], hi[2], hi[3]);
+            store4<P * R * 2>(to, lo[0], lo[1], lo[2], lo[3]);
           }
       }
     }
-    tile(std::integral_constant<int, R>{}, L::kZ, z, [&](int row) {
-      return Decayed(m.power, w.added(row, back)).rest * up_of(m.square_z[row]);
-    });
+#pragma unroll
+    for (int k = 0; k < 4; ++k) up_z[k] *= Decayed(m.power, w.added(row_of(R, k), back)).rest;
+    tile(std::integral_constant<int, R>{}, L::kZ, z, up_z);
     __syncthreads();
 
     if constexpr (!STATE) {
@@ -753,9 +766,9 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
       }
       // x y^T for the positions up to (back: from) this warp's own
       float S[kC / 8][4];
-#pragma unroll
-      for (int jb = 0; jb < kC / 16; ++jb) {
-        if (back ? jb < warp : jb > warp) continue;
+      for_each<kC / 16>([&](auto block) {
+        constexpr int jb = decltype(block)::value;
+        if (back ? jb < warp : jb > warp) return;
         float small[2][4];                // the products with low halves
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -763,9 +776,8 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
         for (int k = 0; k < P / 16; ++k) {
           uint32_t bh[4], bl[4];
-          const uint32_t from = (read_y ^ (k << 5)) + jb * 16 * P * 2;
-          load4(bh, from);
-          load4(bl, from + kC * P * 2);
+          load4<jb * 16 * P * 2>(bh, read_y ^ (k << 5));
+          load4<jb * 16 * P * 2 + kC * P * 2>(bl, read_y ^ (k << 5));
           product(small[0], xl[k], bh[0], bh[1]);
           product(small[1], xl[k], bh[2], bh[3]);
           product(S[2 * jb], xh[k], bh[0], bh[1]);
@@ -779,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
           add2(v[0], v[1], v[0], v[1], small[jt][0], small[jt][1]);
           add2(v[2], v[3], v[2], v[3], small[jt][2], small[jt][3]);
         }
-      }
+      });
       // x X
       float o[R / 8][4];
 #pragma unroll
@@ -787,16 +799,16 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][e] = 0.f;
       if (square_state > 0.f) {
-#pragma unroll
-        for (int k = 0; k < P / 16; ++k)
+        for_each<P / 16>([&](auto depth) {
+          constexpr int k = decltype(depth)::value;
 #pragma unroll
           for (int nb = 0; nb < R / 16; ++nb) {
             uint32_t bh[4], bl[4];
-            const uint32_t from = (read_state ^ (nb << 5)) + k * 16 * R * 2;
-            load4_turned(bh, from);
-            load4_turned(bl, from + P * R * 2);
+            load4_turned<k * 16 * R * 2>(bh, read_state ^ (nb << 5));
+            load4_turned<k * 16 * R * 2 + P * R * 2>(bl, read_state ^ (nb << 5));
             products(o[2 * nb], o[2 * nb + 1], xh[k], xl[k], bh, bl);
           }
+        });
       }
       // The weights of x y^T, and the rows' largest: l^(i - j) is looked up in the warp's
       // own positions, elsewhere it is a product of three powers of at least 0.
@@ -867,9 +879,9 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
         by[half] = scale.first;
         then[half] = scale.then;
       }
-#pragma unroll
-      for (int jb = 0; jb < kC / 16; ++jb) {
-        if (back ? jb < warp : jb > warp) continue;
+      for_each<kC / 16>([&](auto block) {
+        constexpr int jb = decltype(block)::value;
+        if (back ? jb < warp : jb > warp) return;
         uint32_t ph[4], pl[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -878,12 +890,11 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
         for (int nb = 0; nb < R / 16; ++nb) {
           uint32_t bh[4], bl[4];
-          const uint32_t from = (read_z ^ (nb << 5)) + jb * 16 * R * 2;
-          load4_turned(bh, from);
-          load4_turned(bl, from + kC * R * 2);
+          load4_turned<jb * 16 * R * 2>(bh, read_z ^ (nb << 5));
+          load4_turned<jb * 16 * R * 2 + kC * R * 2>(bl, read_z ^ (nb << 5));
           products(o[2 * nb], o[2 * nb + 1], ph, pl, bh, bl);
         }
-      }
+      });
       const int room = a.r - slice * R;
       const bool plain = pairs_o && n == kC && room >= R;
 #pragma unroll
@@ -924,12 +935,12 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
       for (int nt = 0; nt < L::kColTiles; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
-#pragma unroll
-      for (int k = 0; k < kC / 16; ++k) {
+      for_each<kC / 16>([&](auto depth) {
+        constexpr int k = decltype(depth)::value;
         uint32_t ah[4], al[4];
-        const uint32_t from = (read_y ^ ((row0 / 16 + mt) << 5)) + k * 16 * P * 2;
-        load4_turned(ah, from);
-        load4_turned(al, from + kC * P * 2);
+        const uint32_t from = read_y ^ ((row0 / 16 + mt) << 5);
+        load4_turned<k * 16 * P * 2>(ah, from);
+        load4_turned<k * 16 * P * 2 + kC * P * 2>(al, from);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int j = k * 16 + half * 8 + 2 * t;
@@ -951,12 +962,12 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
         for (int nb = 0; nb < L::kColTiles / 2; ++nb) {
           uint32_t bh[4], bl[4];
-          const uint32_t zat = (read_z ^ ((col0 / 16 + nb) << 5)) + k * 16 * R * 2;
-          load4_turned(bh, zat);
-          load4_turned(bl, zat + kC * R * 2);
+          const uint32_t zat = read_z ^ ((col0 / 16 + nb) << 5);
+          load4_turned<k * 16 * R * 2>(bh, zat);
+          load4_turned<k * 16 * R * 2 + kC * R * 2>(bl, zat);
           products(d[2 * nb], d[2 * nb + 1], ah, al, bh, bl);
         }
-      }
+      });
       if (by.then != 1.f) {
 #pragma unroll
         for (int nt = 0; nt < L::kColTiles; ++nt)
@@ -1121,19 +1132,27 @@ int allow_smem(K kernel, int bytes) {
   return WXX_OK;
 }
 
-// How many pieces a row of `chunks` is worked on in, for `blocks` rows (sequences, heads, slices
-// and passes) on `resident` places: the fewest turns of the outputs' launch and, with more
-// than one piece, of the states' one (half as long a chunk; a start is about a chunk, the
-// launches in between one and a half).
-int pieces_of(int64_t blocks, int64_t chunks, int64_t resident) {
+// How many pieces a row of `chunks` is worked on in, for `rows` rows (sequences, heads, slices
+// and passes) and `blocks` blocks on an SM: the least of the outputs' launch and, with more
+// than one piece, the states' one (half as long a chunk) and what lies between.  In units
+// of an SM's time for a chunk when it is full; a block by itself takes 0.8 blocks times as
+// long, a start is about a chunk.  Measured, forward with heads of 64: 128 rows of 16 chunks
+// in 1 and 2 pieces 108 and 116 us; 64 of 16 in 1, 2, 3 and 4 pieces 106, 92, 83 and 66; 64
+// of 128 in 3, 4 and 8 pieces 483, 387 and 390; 16 of 128 in 8, 16 and 32 pieces 175, 123
+// and 135.
+int pieces_of(int64_t rows, int64_t chunks, int blocks) {
+  const int64_t sms = wxx::num_sms();
+  auto turns = [&](int64_t n) {
+    const double full = (double)((n + sms - 1) / sms), alone = 0.8 * blocks;
+    return full > alone ? full : alone;
+  };
   double least = 0;
   int best = 1;
-  for (int m = 1; m <= 64 && 2 * m <= chunks + 1; ++m) {
+  for (int m = 1; m <= 128 && 2 * m <= chunks + 1; ++m) {
     const int64_t size = (chunks + m - 1) / m;
     if ((chunks + size - 1) / size != m) continue;
-    auto turns = [&](int64_t n) { return (double)((n + resident - 1) / resident); };
-    double cost = turns(blocks * m) * (size + 1);
-    if (m > 1) cost += turns(blocks * (m - 1)) * (0.5 * size + 1) + 1.5;
+    double cost = turns(rows * m) * (size + 1);
+    if (m > 1) cost += turns(rows * (m - 1)) * (0.5 * size + 1) + 2.5;
     if (m == 1 || cost < least) least = cost, best = m;
   }
   return best;
@@ -1179,7 +1198,7 @@ int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
   const Pass& a = passes.at[0];
   const int slices = (a.r + R - 1) / R;
   const int64_t heads = B * s.H, blocks = heads * slices, chunks = (s.T + kC - 1) / kC;
-  Segments g{pieces_of(blocks * n, chunks, (int64_t)wxx::num_sms() * L::kBlocks), 0, nullptr, nullptr};
+  Segments g{pieces_of(blocks * n, chunks, L::kBlocks), 0, nullptr, nullptr};
   g.chunks = (int)((chunks + g.count - 1) / g.count);
   WXX_REQUIRE(blocks * n * g.count < (int64_t(1) << 31), "linear attention: too many sequences");
   Maps maps{};
