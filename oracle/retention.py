@@ -133,3 +133,57 @@ def group_norm_backward(dy, x, groups, gamma=None, beta=None, activation=None, g
     dx = inv * (u - u.mean((1, 3), keepdims=True) - z * (u * z).mean((1, 3), keepdims=True))
     return (dx.reshape(x.shape), (dn * z).sum((0, 1)).reshape(-1), dn.sum((0, 1)).reshape(-1),
             dgate)
+
+
+def retention_forward(sd, pre, x, heads, log_decay, reset=None, off=None):
+    """The retention layer ``pre`` of a state_dict on x (B, T, D), in 64 bits.  ``off(value,
+    terms)``: what stands in for a value whose terms' sizes sum up to ``terms``."""
+    D = x.shape[-1]
+    hd = D // heads
+    off = off or (lambda value, terms: value)
+    f = 10000.0 ** (-2 * np.arange(hd // 2) / hd)
+
+    def lin(name, x):
+        w = np.asarray(sd[pre + name + ".weight"], np.float64)
+        return off(x @ w, np.abs(x) @ np.abs(w))
+
+    q, k = (rotary(lin(n, x), heads, f) for n in ("q", "k"))
+    v = lin("v", x)
+    scale = hd ** -0.5
+    o = off(linear_attention(q, k, v, log_decay, None, reset, scale)[0],
+            linear_attention(np.abs(q), np.abs(k), np.abs(v), log_decay, None, reset, scale)[0])
+    rows = (-1, D)
+    y = group_norm(o.reshape(rows), heads, sd[pre + "norm.weight"], sd[pre + "norm.bias"], "silu",
+                   lin("gate", x).reshape(rows))[0]
+    return lin("out", y.reshape(x.shape))
+
+
+def lm_forward(sd, ids, n_layers, heads, log_decay, reset=None, off=None):
+    """Logits of a RecurrentLM whose mixers are retentions, in 64 bits."""
+    from .recurrent import _gelu, _layernorm
+
+    w = {k: np.asarray(v, np.float64) for k, v in sd.items()}
+    h = w["tok_emb.weight"][np.asarray(ids, np.int64)]
+    for i in range(n_layers):
+        p = f"blocks.{i}."
+        n = _layernorm(h, w[p + "ln1.weightg"], w[p + "ln1.weightb"])
+        h = h + retention_forward(w, p + "mixer.", n, heads, log_decay, reset, off)
+        n = _layernorm(h, w[p + "ln2.weightg"], w[p + "ln2.weightb"])
+        h = h + _gelu(n @ w[p + "mlp.0.weight"] + w[p + "mlp.0.bias"]) @ w[p + "mlp.2.weight"] \
+            + w[p + "mlp.2.bias"]
+    h = _layernorm(h, w["ln_f.weightg"], w["ln_f.weightb"])
+    return h @ w["tok_emb.weight"].T
+
+
+def lm_error(sd, ids, n_layers, heads, log_decay, reset=None, part=2.0 ** -20, draws=4):
+    """(B, T): by how much a position's logits move when every value of the mixers is off by up to ``part`` of
+    its terms' sizes: the norm of a head divides by the head's own size, so outputs that
+    cancel pass their errors on enlarged."""
+    ref = lm_forward(sd, ids, n_layers, heads, log_decay, reset)
+    rng = np.random.default_rng(0)
+
+    def off(value, terms):
+        return value + rng.uniform(-part, part, value.shape) * terms
+
+    return np.max([np.abs(lm_forward(sd, ids, n_layers, heads, log_decay, reset, off) - ref).max(-1)
+                   for _ in range(draws)], 0)

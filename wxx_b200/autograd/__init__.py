@@ -516,6 +516,53 @@ class gated_recurrence(Function):
         return tuple(g if n else None for g, n in zip(grads, need))
 
 
+class rotary(Function):
+    """``functional.rotary`` of a tensor (batch, time, channels)."""
+
+    def forward(self, x, n_heads, frequencies, positions=None, offset=0, layout="half"):
+        if any(self.needs_input_grad):
+            self.saved = (n_heads, frequencies, positions, offset, layout)
+        return self._track(functional.rotary(x, n_heads, frequencies, positions, offset, layout))
+
+    def backward(self, grad_output):
+        saved, self.saved = self.saved, None
+        return functional.rotary_backward(grad_output, *saved)
+
+
+class linear_attention(Function):
+    """The outputs of linear attention with a decay for each head; constructed with q, k, v and,
+    when it needs a gradient, h0.  ``log_decay`` is a constant of the model."""
+
+    def forward(self, q, k, v, log_decay, h0=None, reset=None, scale=1.0):
+        if context.MODE == 0 and log_decay.requires_grad:
+            raise ValueError("linear_attention: log_decay receives no gradient")
+        o, _ = functional.linear_attention(q, k, v, log_decay, h0, reset, scale)
+        if any(self.needs_input_grad):
+            self.saved = (q, k, v, log_decay, h0, reset, None, scale)
+        return self._track(o)
+
+    def backward(self, grad_output):
+        saved, self.saved = self.saved, None
+        grads = functional.linear_attention_backward(grad_output, *saved)
+        return tuple(g if n else None for g, n in zip(grads, self.needs_input_grad))
+
+
+class group_norm(Function):
+    """``functional.group_norm``; constructed with x, gamma, beta and, where there is one, the
+    gate."""
+
+    def forward(self, x, groups, gamma, beta, activation=None, gate=None, eps=1e-5):
+        y, mean, inv = functional.group_norm(x, groups, gamma, beta, activation, gate, eps)
+        if any(self.needs_input_grad):
+            self.saved = (x, mean, inv, groups, gamma, beta, activation, gate)
+        return self._track(y)
+
+    def backward(self, grad_output):
+        saved, self.saved = self.saved, None
+        grads = functional.group_norm_backward(grad_output, *saved)
+        return tuple(g if n else None for g, n in zip(grads, self.needs_input_grad))
+
+
 def _training_op(name):
     class _T(Function):
         def forward(self, *args, **kwargs):

@@ -23,6 +23,7 @@ from .module import (
     Conv2DTranspose,
     Dropout,
     Embedding,
+    GroupNorm,
     LayerNorm,
     Linear,
     MaxPool1d,
@@ -35,7 +36,7 @@ from .module import (
 )
 from .loss import CCELoss, DistillLoss, MAELoss, loss
 from .optimizer import AdamW, Optimizer, SGD
-from .recurrent import GatedRecurrence, RecurrentBlock, RecurrentLM
+from .recurrent import GatedRecurrence, RecurrentBlock, RecurrentLM, Retention
 from .resnet import ResBlock, ResNet18
 
 __all__ = [
@@ -45,5 +46,5 @@ __all__ = [
     "MaxPool2d", "Module", "ModuleList", "MultiHeadAttention", "PositionalEncoding", "RMSNorm",
     "ResBlock", "ResNet18", "Sequential", "Sine", "SwiGLU", "TiedLinear",
     "loss", "CCELoss", "DistillLoss", "MAELoss", "Optimizer", "SGD", "AdamW",
-    "GatedRecurrence", "RecurrentBlock", "RecurrentLM",
+    "GatedRecurrence", "GroupNorm", "RecurrentBlock", "RecurrentLM", "Retention",
 ]

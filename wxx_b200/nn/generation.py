@@ -215,7 +215,9 @@ class _CacheDecoder:
 
 
 class _StateDecoder:
-    """The recurrent model's decode steps: one vector per layer and sequence."""
+    """The recurrent model's decode steps: one state per layer and sequence.  The tokens
+    so far are one more than those before the newest, so the prompt's positions start at
+    1 (a retention's products depend on distances alone)."""
 
     def __init__(self, model, rows, total):
         self.model, self.rows, self.total = model, rows, total
@@ -227,14 +229,14 @@ class _StateDecoder:
 
         model = self.model
         states = model.new_states(ids.shape[0])
-        h = model.hidden(ids, None, states)
+        h = model.hidden(ids, None, states, 1)
         for full, s in zip(self.vectors, states):
             functional.assign(full[::beams], s)
         last = h.narrow(1, ids.shape[1] - 1, 1).reshape((ids.shape[0], h.shape[-1]))
         return model.head(last)
 
     def step(self, state):
-        return self.model.decode(state.last, self.vectors)
+        return self.model.decode(state.last, self.vectors, state.cur_len)
 
 
 class _BeamState:

@@ -227,6 +227,28 @@ class LayerNorm(Module):
                                       feeds_tf32=True)[0]
 
 
+class GroupNorm(Module):
+    """Group norm over trailing channels with an activation (``functional.group_norm``; no
+    reference counterpart): (samples, ..., channels), ``activation`` of the result, or of the
+    ``gate`` given to ``forward``, which multiplies the result."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, activation=None):
+        super().__init__()
+        if num_groups < 1 or num_channels % num_groups:
+            raise ValueError(f"{num_channels} channels cannot be split over {num_groups} groups")
+        self.num_groups = num_groups
+        self.num_channels = num_channels
+        self.eps = eps
+        self.activation = activation
+        self.weight = Parameter(Tensor((num_channels,), value=1.0))
+        self.bias = Parameter(Tensor((num_channels,), value=0.0))
+
+    def forward(self, x, gate=None):
+        given = (x, self.weight, self.bias) + (() if gate is None else (gate,))
+        return autograd.group_norm(*given).forward(x, self.num_groups, self.weight, self.bias,
+                                                   self.activation, gate, self.eps)
+
+
 class RMSNorm(Module):
     """RMSNorm over the last dim (kernel eps 1e-6, as in the reference)."""
 
