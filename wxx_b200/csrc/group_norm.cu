@@ -158,6 +158,47 @@ __device__ __forceinline__ void act_slope_all(int code, float (&v)[V], float (&s
     act_slope_all<kNone, V>(v, s);
 }
 
+// V numbers at a time, in pairs.
+template <int V>
+__device__ __forceinline__ void add_all(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+#pragma unroll
+  for (int e = 0; e + 1 < V; e += 2) add2(d[e], d[e + 1], a[e], a[e + 1], b[e], b[e + 1]);
+  if (V % 2) d[V - 1] = a[V - 1] + b[V - 1];
+}
+template <int V>
+__device__ __forceinline__ void sub_all(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+#pragma unroll
+  for (int e = 0; e + 1 < V; e += 2) sub2(d[e], d[e + 1], a[e], a[e + 1], b[e], b[e + 1]);
+  if (V % 2) d[V - 1] = a[V - 1] - b[V - 1];
+}
+template <int V>
+__device__ __forceinline__ void mul_all(float (&d)[V], const float (&a)[V], const float (&b)[V]) {
+#pragma unroll
+  for (int e = 0; e + 1 < V; e += 2) mul2(d[e], d[e + 1], a[e], a[e + 1], b[e], b[e + 1]);
+  if (V % 2) d[V - 1] = a[V - 1] * b[V - 1];
+}
+template <int V>
+__device__ __forceinline__ void fma_all(float (&d)[V], const float (&a)[V], const float (&b)[V],
+                                        const float (&c)[V]) {
+#pragma unroll
+  for (int e = 0; e + 1 < V; e += 2)
+    fma2(d[e], d[e + 1], a[e], a[e + 1], b[e], b[e + 1], c[e], c[e + 1]);
+  if (V % 2) d[V - 1] = fmaf(a[V - 1], b[V - 1], c[V - 1]);
+}
+template <int V>
+__device__ __forceinline__ void fill(float (&d)[V], float v) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) d[e] = v;
+}
+template <int V>
+__device__ __forceinline__ float total(const float (&v)[V]) {
+  if constexpr (V == 4) return (v[0] + v[1]) + (v[2] + v[3]);
+  float sum = v[0];
+#pragma unroll
+  for (int e = 1; e < V; ++e) sum += v[e];
+  return sum;
+}
+
 template <int V>
 struct Pack {
   float v[V];
@@ -295,16 +336,16 @@ __device__ __forceinline__ void inner_gradient(int code, float (&d)[V], const fl
                                                const float (&gamma)[V], const float (&beta)[V],
                                                float (&gate)[V]) {
   float n[V], value[V], slope[V];
+  fma_all<V>(n, z, gamma, beta);
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    n[e] = fmaf(z[e], gamma[e], beta[e]);
-    value[e] = GATED ? gate[e] : n[e];
-  }
+  for (int e = 0; e < V; ++e) value[e] = GATED ? gate[e] : n[e];
   act_slope_all<V>(code, value, slope);
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if (GATED) gate[e] = d[e] * n[e] * slope[e];
-    d[e] *= GATED ? value[e] : slope[e];
+  if constexpr (GATED) {
+    mul_all<V>(n, n, slope);
+    mul_all<V>(gate, n, d);
+    mul_all<V>(d, d, value);
+  } else {
+    mul_all<V>(d, d, slope);
   }
 }
 
@@ -412,6 +453,12 @@ __global__ void __launch_bounds__(1024)
   if (c < 2 * C) {
     const float* p = part + c;
     int64_t r = warp;
+    for (; r + 224 < rows; r += 256) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = p[(r + 32 * k) * 2 * C];
+      a += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
     for (; r + 96 < rows; r += 128) {
       float v[4];
 #pragma unroll
@@ -443,7 +490,9 @@ struct Few {
 };
 
 __device__ __forceinline__ float over_lanes(float v, int lanes) {
-  for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
@@ -471,7 +520,8 @@ __global__ void __launch_bounds__(kT)
     const bool on = here && n < f.N;
     const int64_t at = n * f.C + g * f.per;
     Pack<V> v[K], w[GATED ? K : 1];
-    float sum = 0.f;
+    float sums[V], means[V];
+    fill<V>(sums, 0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * f.lanes + lane) * V;
@@ -482,21 +532,16 @@ __global__ void __launch_bounds__(kT)
       if (GATED && in) w[k] = load<V>(gate + at + c);
     }
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum += v[k].v[e];
-    const float mu = over_lanes(sum, f.lanes) * share;
-    float square = 0.f;
+    for (int k = 0; k < K; ++k) add_all<V>(sums, sums, v[k].v);
+    const float mu = over_lanes(total<V>(sums), f.lanes) * share;
+    fill<V>(means, mu);
+    fill<V>(sums, 0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const bool in = (k * f.lanes + lane) * V < f.per;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        v[k].v[e] -= mu;
-        if (in) square = fmaf(v[k].v[e], v[k].v[e], square);
-      }
+      sub_all<V>(v[k].v, v[k].v, means);
+      if ((k * f.lanes + lane) * V < f.per) fma_all<V>(sums, v[k].v, v[k].v, sums);
     }
-    const float is = inverse_root(fmaf(over_lanes(square, f.lanes), share, f.eps));
+    const float is = inverse_root(fmaf(over_lanes(total<V>(sums), f.lanes), share, f.eps));
     if (!on) continue;
     if (lane == 0) {
       mean[n * f.G + g] = mu;
@@ -506,12 +551,13 @@ __global__ void __launch_bounds__(kT)
     for (int k = 0; k < K; ++k) {
       const int c = (k * f.lanes + lane) * V;
       if (c >= f.per) continue;
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[k].v[e] = fmaf(v[k].v[e] * is, ga[k].v[e], be[k].v[e]);
+      float scales[V];
+      fill<V>(scales, is);
+      mul_all<V>(v[k].v, v[k].v, scales);
+      fma_all<V>(v[k].v, v[k].v, ga[k].v, be[k].v);
       if constexpr (GATED) {
         act_all<V>(f.code, w[k].v);
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[k].v[e] *= w[k].v[e];
+        mul_all<V>(v[k].v, v[k].v, w[k].v);
       } else {
         act_all<V>(f.code, v[k].v);
       }
@@ -562,29 +608,31 @@ __global__ void __launch_bounds__(kT)
         if (GATED) w[k] = load<V>(gate + at + c);
       }
     }
-    float a = 0.f, b = 0.f;
+    float as[V], bs[V], means[V], scales[V];
+    fill<V>(as, 0.f);
+    fill<V>(bs, 0.f);
+    fill<V>(means, mu);
+    fill<V>(scales, is);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) z[k].v[e] = (z[k].v[e] - mu) * is;
+      sub_all<V>(z[k].v, z[k].v, means);
+      mul_all<V>(z[k].v, z[k].v, scales);
       inner_gradient<V, GATED>(f.code, d[k].v, z[k].v, ga[k].v, be[k].v, w[GATED ? k : 0].v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        sum_n[k].v[e] += d[k].v[e];
-        sum_z[k].v[e] = fmaf(d[k].v[e], z[k].v[e], sum_z[k].v[e]);
-        d[k].v[e] *= ga[k].v[e];
-        a += d[k].v[e];
-        b = fmaf(d[k].v[e], z[k].v[e], b);
-      }
+      add_all<V>(sum_n[k].v, sum_n[k].v, d[k].v);
+      fma_all<V>(sum_z[k].v, d[k].v, z[k].v, sum_z[k].v);
+      mul_all<V>(d[k].v, d[k].v, ga[k].v);
+      add_all<V>(as, as, d[k].v);
+      fma_all<V>(bs, d[k].v, z[k].v, bs);
     }
-    a = over_lanes(a, f.lanes) * share;
-    b = over_lanes(b, f.lanes) * share;
+    fill<V>(as, over_lanes(total<V>(as), f.lanes) * share);
+    fill<V>(bs, -over_lanes(total<V>(bs), f.lanes) * share);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * f.lanes + lane) * V;
       if (!on || c >= f.per) continue;
-#pragma unroll
-      for (int e = 0; e < V; ++e) d[k].v[e] = is * (d[k].v[e] - a - z[k].v[e] * b);
+      sub_all<V>(d[k].v, d[k].v, as);
+      fma_all<V>(d[k].v, z[k].v, bs, d[k].v);
+      mul_all<V>(d[k].v, d[k].v, scales);
       store<V>(dx + at + c, d[k]);
       if (GATED) store<V>(dgate + at + c, w[k]);
     }
@@ -609,6 +657,7 @@ __global__ void __launch_bounds__(kT)
 struct Slab {
   int64_t N;
   int S, C, G, per, wide, spans, across, rows, split, code;
+  int step_j, step_c;       // 32 / per and 32 % per
   bool folded;
   float eps;
 };
@@ -622,11 +671,11 @@ __device__ __forceinline__ const float* channel_sums(float* scratch, float (&v)[
                                                      int row, bool on, const Slab& f) {
   int rows = f.rows;
   if (f.folded) {
+    for (int o = 16; o >= f.across; o >>= 1)
 #pragma unroll
-    for (int i = 0; i < M; ++i)
+      for (int i = 0; i < M; ++i)
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        for (int o = 16; o >= f.across; o >>= 1) v[i][e] += __shfl_xor_sync(0xffffffffu, v[i][e], o);
+        for (int e = 0; e < V; ++e) v[i][e] += __shfl_xor_sync(0xffffffffu, v[i][e], o);
     rows = blockDim.x >> 5;
     row = threadIdx.x >> 5;
     on = (threadIdx.x & 31) < f.across;
@@ -650,8 +699,39 @@ __device__ __forceinline__ const float* channel_sums(float* scratch, float (&v)[
   return out;
 }
 
+// The places of a lane's partial sums of the first group: every 32nd of split * per.
+template <class F>
+__device__ __forceinline__ void each_of_group(const Slab& f, int lane, F take) {
+  int j = lane / f.per, c = lane - j * f.per;
+#pragma unroll 4
+  for (int i = lane; i < f.split * f.per; i += 32) {
+    take(j * f.wide + c, c);
+    j += f.step_j;
+    c += f.step_c;
+    const bool on = c >= f.per;
+    j += on;
+    c -= on ? f.per : 0;
+  }
+}
+
+// The groups of channels c to c + V - 1.
+template <int V>
+__device__ __forceinline__ void groups_of(int (&of)[V], int c, int per) {
+  of[0] = c / per;
+  c -= of[0] * per;
+#pragma unroll
+  for (int e = 1; e < V; ++e) {
+    c = c + 1 == per ? 0 : c + 1;
+    of[e] = of[e - 1] + (c == 0);
+  }
+}
+
+// (64 registers a thread, four blocks of 256 on an SM: over 16 x 4096 x 64 19.9 -> 16.4 us, 64 x
+// 1024 x 128 gated 35.7 -> 30.5; over 128 x 1024 x 64, whose pieces of a position are 32 bytes,
+// 21.6 -> 22.1, where 3 TB/s go through it: phases of reading, two sums and writing that four
+// blocks hide from one another only in part.)
 template <int V, int K, bool GATED>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(512, 2)
     slab_kernel(float* __restrict__ y, float* __restrict__ mean, float* __restrict__ inv,
                 const float* __restrict__ x, const float* __restrict__ gate,
                 const float* __restrict__ gamma, const float* __restrict__ beta, const Slab f) {
@@ -673,18 +753,10 @@ __global__ void __launch_bounds__(512)
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float count = (float)f.S * (float)f.per;
-  // a lane's values of a group are every 32nd of split * per
-  const int first_j = lane / f.per, first_c = lane % f.per, step_j = 32 / f.per, step_c = 32 % f.per;
   auto over_groups = [&](const float* sums, float* to, auto finish) {
     for (int g = warp; g < groups; g += blockDim.x >> 5) {
       float sum = 0.f;
-      for (int j = first_j, c = first_c; j < f.split; j += step_j, c += step_c) {
-        if (c >= f.per) {
-          c -= f.per;
-          if (++j >= f.split) break;
-        }
-        sum += sums[j * f.wide + g * f.per + c];
-      }
+      each_of_group(f, lane, [&](int i, int) { sum += sums[i + g * f.per]; });
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane == 0) to[g] = finish(sum / count);
@@ -692,25 +764,20 @@ __global__ void __launch_bounds__(512)
     __syncthreads();
   };
   int of[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) of[e] = in ? (q * V + e) / f.per : 0;
+  groups_of<V>(of, in ? q * V : 0, f.per);
   float part[1][V] = {};
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int e = 0; e < V; ++e) part[0][e] += v[k].v[e];
+  for (int k = 0; k < K; ++k) add_all<V>(part[0], part[0], v[k].v);
   const float* sums = channel_sums<1, V>(scratch, part, q, row, on, f);
   over_groups(sums, group, [](float m) { return m; });
   float mu[V], is[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) mu[e] = group[of[e]], part[0][e] = 0.f;
 #pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      v[k].v[e] -= mu[e];
-      if (row + k * f.rows < f.S) part[0][e] = fmaf(v[k].v[e], v[k].v[e], part[0][e]);
-    }
+  for (int k = 0; k < K; ++k) {
+    sub_all<V>(v[k].v, v[k].v, mu);
+    if (row + k * f.rows < f.S) fma_all<V>(part[0], v[k].v, v[k].v, part[0]);
+  }
   if (!in)
 #pragma unroll
     for (int e = 0; e < V; ++e) part[0][e] = 0.f;
@@ -728,22 +795,37 @@ __global__ void __launch_bounds__(512)
     ga[e] = (gamma ? gamma[c0 + q * V + e] : 1.f);
     be[e] = beta ? beta[c0 + q * V + e] : 0.f;
   }
+  // (single channels two positions at a time, for the pairs)
+  constexpr int J = V == 1 && K > 1 ? 2 : 1;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int p = row + k * f.rows;
-    if (p >= f.S) continue;
-    Pack<V> w;
-    if (GATED) w = load<V>(gate + at + (int64_t)p * f.C);
+  for (int k = 0; k < K; k += J) {
+    if (row + k * f.rows >= f.S) continue;
+    float now[J * V], w[J * V];
+    fill<J * V>(w, 0.f);
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[k].v[e] = fmaf(v[k].v[e] * is[e], ga[e], be[e]);
-    if constexpr (GATED) {
-      act_all<V>(f.code, w.v);
+    for (int j = 0; j < J; ++j) {
+      const int p = row + (k + j) * f.rows;
+      mul_all<V>(v[k + j].v, v[k + j].v, is);
+      fma_all<V>(v[k + j].v, v[k + j].v, ga, be);
+      Pack<V> gates;
+      fill<V>(gates.v, 0.f);
+      if (GATED && p < f.S) gates = load<V>(gate + at + (int64_t)p * f.C);
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[k].v[e] *= w.v[e];
-    } else {
-      act_all<V>(f.code, v[k].v);
+      for (int e = 0; e < V; ++e) now[j * V + e] = v[k + j].v[e], w[j * V + e] = gates.v[e];
     }
-    store<V>(y + at + (int64_t)p * f.C, v[k]);
+    if constexpr (GATED) {
+      act_all<J * V>(f.code, w);
+      mul_all<J * V>(now, now, w);
+    } else {
+      act_all<J * V>(f.code, now);
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int p = row + (k + j) * f.rows;
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[k + j].v[e] = now[j * V + e];
+      if (p < f.S) store<V>(y + at + (int64_t)p * f.C, v[k + j]);
+    }
   }
 }
 
@@ -776,30 +858,51 @@ __global__ void __launch_bounds__(512)
   }
   float mu[V], is[V], ga[V], be[V];
   int of[V];
+  groups_of<V>(of, in ? q * V : 0, f.per);
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    of[e] = in ? (q * V + e) / f.per : 0;
     mu[e] = in ? mean[n * f.G + c0 / f.per + of[e]] : 0.f;
     is[e] = in ? inv[n * f.G + c0 / f.per + of[e]] : 0.f;
     ga[e] = in && gamma ? gamma[c0 + q * V + e] : 1.f;
     be[e] = in && beta ? beta[c0 + q * V + e] : 0.f;
   }
   float both[2][V] = {};
+  // (single channels two positions at a time, for the pairs)
+  constexpr int J = V == 1 && K > 1 ? 2 : 1;
+  float gammas[J * V], betas[J * V];
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int p = row + k * f.rows;
-    if (!in || p >= f.S) continue;
-    Pack<V> w;
-    if (GATED) w = load<V>(gate + at + (int64_t)p * f.C);
+  for (int e = 0; e < J * V; ++e) gammas[e] = ga[e % V], betas[e] = be[e % V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) z[k].v[e] = (z[k].v[e] - mu[e]) * is[e];
-    inner_gradient<V, GATED>(f.code, d[k].v, z[k].v, ga, be, w.v);
+  for (int k = 0; k < K; k += J) {
+    if (!in || row + k * f.rows >= f.S) continue;
+    float zs[J * V], ds[J * V], ws[J * V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      both[0][e] += d[k].v[e];
-      both[1][e] = fmaf(d[k].v[e], z[k].v[e], both[1][e]);
+    for (int j = 0; j < J; ++j) {
+      const int p = row + (k + j) * f.rows;
+      sub_all<V>(z[k + j].v, z[k + j].v, mu);
+      mul_all<V>(z[k + j].v, z[k + j].v, is);
+      Pack<V> gates;
+      fill<V>(gates.v, 0.f);
+      if (GATED && p < f.S) gates = load<V>(gate + at + (int64_t)p * f.C);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        zs[j * V + e] = z[k + j].v[e];
+        ds[j * V + e] = d[k + j].v[e];
+        ws[j * V + e] = gates.v[e];
+      }
     }
-    if (GATED) store<V>(dgate + at + (int64_t)p * f.C, w);
+    inner_gradient<J * V, GATED>(f.code, ds, zs, gammas, betas, ws);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int p = row + (k + j) * f.rows;
+      Pack<V> gates;
+#pragma unroll
+      for (int e = 0; e < V; ++e) d[k + j].v[e] = ds[j * V + e], gates.v[e] = ws[j * V + e];
+      if (j > 0 && p >= f.S) continue;
+      add_all<V>(both[0], both[0], d[k + j].v);
+      fma_all<V>(both[1], d[k + j].v, z[k + j].v, both[1]);
+      if (GATED) store<V>(dgate + at + (int64_t)p * f.C, gates);
+    }
   }
   const float* sums = channel_sums<2, V>(scratch, both, q, row, on, f);
   // dbeta's and dgamma's share of this sample
@@ -816,16 +919,11 @@ __global__ void __launch_bounds__(512)
   const float count = (float)f.S * (float)f.per;
   for (int g = warp; g < groups; g += blockDim.x >> 5) {
     float a = 0.f, b = 0.f;
-    for (int j = lane / f.per, k = lane % f.per; j < f.split; j += 32 / f.per, k += 32 % f.per) {
-      if (k >= f.per) {
-        k -= f.per;
-        if (++j >= f.split) break;
-      }
-      const int c = g * f.per + k;
-      const float w = gamma ? gamma[c0 + c] : 1.f;
-      a = fmaf(w, sums[j * f.wide + c], a);
-      b = fmaf(w, sums[(f.split + j) * f.wide + c], b);
-    }
+    each_of_group(f, lane, [&](int i, int c) {
+      const float w = gamma ? gamma[c0 + g * f.per + c] : 1.f;
+      a = fmaf(w, sums[i + g * f.per], a);
+      b = fmaf(w, sums[f.split * f.wide + i + g * f.per], b);
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       a += __shfl_xor_sync(0xffffffffu, a, o);
@@ -835,16 +933,21 @@ __global__ void __launch_bounds__(512)
   }
   __syncthreads();
   if (!in) return;
-  float2 m[V];
+  // is (ga d - mean of u - z mean of u z)
+  float a[V], b[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) m[e] = group[of[e]];
+  for (int e = 0; e < V; ++e) {
+    const float2 m = group[of[e]];
+    a[e] = -is[e] * m.x;
+    b[e] = -is[e] * m.y;
+    ga[e] *= is[e];
+  }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int p = row + k * f.rows;
     if (p >= f.S) continue;
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      d[k].v[e] = is[e] * (ga[e] * d[k].v[e] - m[e].x - z[k].v[e] * m[e].y);
+    fma_all<V>(d[k].v, d[k].v, ga, a);
+    fma_all<V>(d[k].v, z[k].v, b, d[k].v);
     store<V>(dx + at + (int64_t)p * f.C, d[k]);
   }
 }
@@ -881,12 +984,15 @@ bool fours(const void* const (&memory)[8], int64_t per) {
 }
 
 // A group of one position in the registers of up to 32 threads, if it fits.
-bool plan_few(Few& f, int& v, int& k, const Shape& s, int code, bool four) {
+bool plan_few(Few& f, int& v, int& k, const Shape& s, int code, bool four, bool two) {
   if (s.S != 1 || s.N * s.G >= (int64_t(1) << 31)) return false;
   v = four ? 4 : 1;
   const int pieces = (s.per + v - 1) / v;
   int lanes = 1;
-  while (lanes < 32 && lanes < pieces) lanes <<= 1;
+  // `two` pieces of 4 a thread where they still are whole 128 bytes.  (Over 8192 x 1024 gated:
+  // forward 21.6 -> 19.0 us; backward, which then has too many registers, 36.1 -> 39.8.)
+  while (lanes < 32 && lanes < pieces && (lanes < 8 || v == 1 || !two || 2 * lanes < pieces))
+    lanes <<= 1;
   k = 1;
   while (k * lanes < pieces) k <<= 1;
   if (k > 8) return false;
@@ -937,7 +1043,7 @@ bool plan_slab(Slab& f, int& v, int& k, int& threads, const Shape& s, int code, 
       if (split < 1) split = 1;
     }
     f = Slab{s.N,    (int)s.S, s.C,  s.G,   s.per, wide,  (s.C + wide - 1) / wide,
-             across, rows,     split, code, folded, s.eps};
+             across, rows,     split, code, 32 / s.per, 32 % s.per, folded, s.eps};
     return s.N * f.spans < (int64_t(1) << 31);
   }
   return false;
@@ -987,7 +1093,7 @@ WXX_EXPORT int wxx_group_norm(float* y, float* mean, float* inv, const float* x,
   Few few;
   Slab slab;
   int v, k, threads;
-  if (plan_few(few, v, k, s, activation, four && s.per % 4 == 0)) {
+  if (plan_few(few, v, k, s, activation, four && s.per % 4 == 0, true)) {
     const unsigned grid = few_grid(few, 1);
     with_pieces(v, k, [&](auto vv, auto kk) {
       constexpr int V = decltype(vv)::value, K = decltype(kk)::value;
@@ -1047,7 +1153,7 @@ WXX_EXPORT int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, f
   Few few;
   Slab slab;
   int v, k, threads;
-  const bool tokens = plan_few(few, v, k, s, activation, four && s.per % 4 == 0);
+  const bool tokens = plan_few(few, v, k, s, activation, four && s.per % 4 == 0, false);
   if (tokens || plan_slab(slab, v, k, threads, s, activation, four, 8, 2)) {
     const unsigned grid = tokens ? few_grid(few, 2) : 0;
     const int64_t rows = tokens ? few.rows : N;
