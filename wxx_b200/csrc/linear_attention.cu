@@ -293,17 +293,17 @@ __device__ __forceinline__ uint32_t piece(int row, int q) {
 __device__ __forceinline__ int raw_piece(int row, int q) { return row * 8 + (q ^ (row & 7)); }
 constexpr int kRaw = kC * 128;          // their bytes
 
-template <int P, int R>
+template <int P, int R, bool AHEAD>
 struct Layout {
   static constexpr int kRawX = 0, kRawY = kRawX + P / 32 * kRaw, kRawZ = kRawY + P / 32 * kRaw;
-  static constexpr int kTiles = kRawZ + R / 32 * kRaw;
-  // high halves, then low halves, of y, z and the state
-  static constexpr int kY = kTiles, kZ = kY + kC * P * 4, kState = kZ + kC * R * 4;
+  // high halves, then low halves, of y and z (AHEAD: not where the copies go) and the state
+  static constexpr int kY = AHEAD ? kRawZ + R / 32 * kRaw : kRawY, kZ = kY + kC * P * 4;
+  static constexpr int kState = kZ + kC * R * 4, kTiles = AHEAD ? kY : 0;
   static constexpr int kEnd = kState + P * R * 4, kBytes = kEnd + 1024;
-  static_assert((P * R + kThreads) * 4 + kC <= kState - kTiles, "rare_chunk's room");
+  static_assert((P * R + kThreads) * 4 + kC <= (AHEAD ? kState : kEnd) - kTiles, "rare_chunk's room");
   // the warps' parts of the state: kRowTiles times 16 rows by kColTiles tiles of 8 columns
   static constexpr int kRowTiles = P >= 64 ? P / 64 : 1, kColTiles = P >= 64 ? R / 8 : R / 16;
-  static constexpr int kBlocks = P == 128 ? 1 : P == 64 && R == 64 ? 2 : P == 32 && R == 32 ? 4 : 3;
+  static constexpr int kBlocks = P == 128 ? 1 : P == 64 && R == 64 ? (AHEAD ? 2 : 3) : P == 32 && R == 32 ? 4 : 3;
 };
 
 struct Segments {           // pieces of a row that are worked on side by side
@@ -411,14 +411,15 @@ __device__ void rare_chunk(float* state, float* sums, const unsigned char* cuts,
 
 // A block: one sequence, head, slice of R columns of z and piece of the row; STATE: only
 // the state after the piece is wanted.  A warp has 16 positions of x and their outputs, and
-// a part of the state; y and z are split by all warps and read by all.  The next chunk's
-// operands are copied meanwhile.
-template <int P, int R, bool STATE>
-__global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
+// a part of the state; y and z are split by all warps and read by all.  AHEAD: the next
+// chunk's operands are copied meanwhile; else they are copied, and split, in the place of this
+// chunk's, which more blocks on an SM have room for (plan_of chooses).
+template <int P, int R, bool STATE, bool AHEAD>
+__global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
     chunk_kernel(const __grid_constant__ Passes passes, const __grid_constant__ Maps maps,
                  const bool tma, const Shape s, const Segments g, const unsigned per_pass,
                  int* err) {
-  using L = Layout<P, R>;
+  using L = Layout<P, R, AHEAD>;
   extern __shared__ __align__(1024) unsigned char raw_smem[];
   __shared__ Small m;
   unsigned char* smem = raw_smem + ((1024 - (smem_address(raw_smem) & 1023)) & 1023);
@@ -534,6 +535,12 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
   auto next_row = [](int W, int k) { return W == 32 ? 4 * k : (k >> 1) * 8 + (k & 1) * 2; };
   auto row_of = [&](int W, int k) { return first_row(W) + next_row(W, k); };
 
+  auto turn_over = [&](int c) {         // not AHEAD: this chunk's operands are done with
+    if (AHEAD || c + 1 >= c1) return;
+    wxx_tc::fence_proxy_async_smem();
+    __syncthreads();
+    fetch(c + 1);
+  };
   for (int c = c0; c < c1; ++c) {
     const int t0 = start(c), n = min(kC, s.T - t0);
     // the resets of the chunk, and of the position after it
@@ -605,9 +612,16 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
     };
     read(std::integral_constant<int, P>{}, L::kRawY, y, m.square_y, up_y);
     read(std::integral_constant<int, R>{}, L::kRawZ, z, m.square_z, up_z);
-    // x of this warp's positions, in the layout of a product's left operand
+    // x of this warp's positions, in the layout of a product's left operand (not AHEAD: read
+    // again for the products, for the registers)
     float2 x[STATE ? 1 : P / 16][4];
     float square_x[2] = {0.f, 0.f};
+    auto x_at = [&](int half, int k, int e) {
+      return *reinterpret_cast<const float2*>(
+          smem + L::kRawX + (k >> 1) * kRaw +
+          ((raw_piece(warp * 16 + quad, t >> 1) * 16 + (t & 1) * 8) ^ ((4 * (k & 1) + 2 * e) << 4)) +
+          half * 8 * 128);
+    };
     if constexpr (!STATE) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -616,12 +630,8 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
         for (int k = 0; k < P / 16; ++k)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const unsigned char* p =
-                smem + L::kRawX + (k >> 1) * kRaw +
-                ((raw_piece(warp * 16 + quad, t >> 1) * 16 + (t & 1) * 8) ^ ((4 * (k & 1) + 2 * e) << 4)) +
-                half * 8 * 128;
-            const float2 v = *reinterpret_cast<const float2*>(p);
-            x[k][half + 2 * e] = v;
+            const float2 v = x_at(half, k, e);
+            if (AHEAD) x[k][half + 2 * e] = v;
             square2(s0, s1, v.x, v.y);
           }
         s0 += s1;
@@ -651,12 +661,15 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int k = 0; k < P / 16; ++k)
-            look(square_x, 1, half, x[k][half].x, x[k][half].y, x[k][half + 2].x, x[k][half + 2].y);
+          for (int k = 0; k < P / 16; ++k) {
+            const float2 u = AHEAD ? x[k][half] : x_at(half, k, 0);
+            const float2 v = AHEAD ? x[k][half + 2] : x_at(half, k, 1);
+            look(square_x, 1, half, u.x, u.y, v.x, v.y);
+          }
       }
     }
     odd = __syncthreads_or(odd);        // the squares are here, the operands are read
-    if (c + 1 < c1) fetch(c + 1);
+    if (AHEAD && c + 1 < c1) fetch(c + 1);
     const int kept_power = w.kept(back);
     const float kept = kept_power < 0 ? 0.f : m.power[kept_power];
     if (STATE) run *= kept;
@@ -671,6 +684,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
       rare_chunk<R, STATE>(state, state + P * R, cut, a, s, n, w.tail, next, l, b, h, t0, slice);
       __syncthreads();
       each([&](float& v, int p, int c) { v = state[p * R + c]; });
+      turn_over(c);
       continue;
     }
 
@@ -764,9 +778,10 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
 #pragma unroll
         for (int k = 0; k < P / 16; ++k)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            split(x[k][half + 2 * e].x, x[k][half + 2 * e].y, up, xh[k][half + 2 * e],
-                  xl[k][half + 2 * e]);
+          for (int e = 0; e < 2; ++e) {
+            const float2 v = AHEAD ? x[k][half + 2 * e] : x_at(half, k, e);
+            split(v.x, v.y, up, xh[k][half + 2 * e], xl[k][half + 2 * e]);
+          }
       }
       // x y^T for the positions up to (back: from) this warp's own
       float S[kC / 8][4];
@@ -987,6 +1002,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R>::kBlocks)
           fma2(v[e], v[e + 1], d[nt][e], d[nt][e + 1], by.first, by.first, v[e], v[e + 1]);
         }
     }
+    turn_over(c);
   }
 
   if (STATE || (a.last && seg == pieces - 1)) {
@@ -1137,27 +1153,40 @@ int allow_smem(K kernel, int bytes) {
 }
 
 // How many pieces a row of `chunks` is worked on in, for `rows` rows (sequences, heads, slices
-// and passes) and `blocks` blocks on an SM: the least of the outputs' launch and, with more
-// than one piece, the states' one (half as long a chunk) and what lies between.  In units
-// of an SM's time for a chunk when it is full; a block by itself takes 0.8 blocks times as
-// long, a start is about a chunk.  Measured, forward with heads of 64: 128 rows of 16 chunks
-// in 1 and 2 pieces 108 and 116 us; 64 of 16 in 1, 2, 3 and 4 pieces 106, 92, 83 and 66; 64
-// of 128 in 3, 4 and 8 pieces 483, 387 and 390; 16 of 128 in 8, 16 and 32 pieces 175, 123
-// and 135.
-int pieces_of(int64_t rows, int64_t chunks, int blocks) {
+// and passes), and whether with the next chunk's operands ahead, `blocks` blocks on an SM, or
+// in place, `more` of them: the least of the outputs' launch and, with more than one piece, the
+// states' one (half as long a chunk) and what lies between.  In units of a full SM's time for
+// one block's chunk; a start is about a chunk.  Measured, heads of 64, 16 chunks a row, 1, 2 and
+// 3 blocks on every SM: ahead 106 and 135 us (and 247: two turns), in place 129, 172 and 207; so
+// 384 rows take 243 and 195 us, 592 rows 261 and 369.  In 1 and 2 pieces 128 rows of 16 chunks
+// 108 and 116 us; 64 of 128 chunks in 3, 4 and 8 pieces 463, 377 and 380; 16 of 128 in 8, 16 and
+// 32 pieces 175, 123 and 135.
+struct Plan {
+  int pieces;
+  bool ahead;
+};
+Plan plan_of(int64_t rows, int64_t chunks, int blocks, int more) {
   const int64_t sms = wxx::num_sms();
-  auto turns = [&](int64_t n) {
-    const double full = (double)((n + sms - 1) / sms), alone = 0.8 * blocks;
-    return full > alone ? full : alone;
+  // n blocks, `fit` on an SM at a time: a full SM takes `full`, a block by itself `alone`
+  auto turns = [&](int64_t n, int fit, double alone, double full) {
+    const int64_t times = n / (sms * fit), rest = (n - times * sms * fit + sms - 1) / sms;
+    const double last = rest == 0   ? 0.
+                        : fit == 1 ? full
+                                   : alone + (full - alone) * (double)(rest - 1) / (fit - 1);
+    return times * full + last;
   };
+  auto ahead = [&](int64_t n) { return turns(n, blocks, 0.8 * blocks, blocks); };
   double least = 0;
-  int best = 1;
+  Plan best{1, true};
   for (int m = 1; m <= 128 && 2 * m <= chunks + 1; ++m) {
     const int64_t size = (chunks + m - 1) / m;
     if ((chunks + size - 1) / size != m) continue;
-    double cost = turns(rows * m) * (size + 1);
-    if (m > 1) cost += turns(rows * (m - 1)) * (0.5 * size + 1) + 2.5;
-    if (m == 1 || cost < least) least = cost, best = m;
+    const double states = m > 1 ? ahead(rows * (m - 1)) * (0.5 * size + 1) + 2.5 : 0.;
+    const double a = states + ahead(rows * m) * (size + 1);
+    if (m == 1 || a < least) least = a, best = {m, true};
+    if (more == blocks) continue;
+    const double i = states + turns(rows * m, more, 0.95 * blocks, 1.03 * more) * (size + 1);
+    if (i < least) least = i, best = {m, false};
   }
   return best;
 }
@@ -1198,11 +1227,13 @@ bool encode(CUtensorMap* map, const Operand& o, int64_t B, int64_t T, int64_t H,
 // then the states before the pieces, then the outputs.
 template <int P, int R>
 int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
-  using L = Layout<P, R>;
+  using L = Layout<P, R, true>;
+  using InPlace = Layout<P, R, P != 64 || R != 64>;     // (other sizes: measured no faster)
   const Pass& a = passes.at[0];
   const int slices = (a.r + R - 1) / R;
   const int64_t heads = B * s.H, blocks = heads * slices, chunks = (s.T + kC - 1) / kC;
-  Segments g{pieces_of(blocks * n, chunks, L::kBlocks), 0, nullptr, nullptr};
+  const Plan plan = plan_of(blocks * n, chunks, L::kBlocks, InPlace::kBlocks);
+  Segments g{plan.pieces, 0, nullptr, nullptr};
   g.chunks = (int)((chunks + g.count - 1) / g.count);
   WXX_REQUIRE(blocks * n * g.count < (int64_t(1) << 31), "linear attention: too many sequences");
   Maps maps{};
@@ -1212,8 +1243,11 @@ int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
     tma = tma && encode(&maps.x[i], p.x, B, s.T, s.H, p.p) &&
           encode(&maps.y[i], p.y, B, s.T, s.H, p.p) && encode(&maps.z[i], p.z, B, s.T, s.H, p.r);
   }
-  if (int st = allow_smem(chunk_kernel<P, R, true>, L::kBytes)) return st;
-  if (int st = allow_smem(chunk_kernel<P, R, false>, L::kBytes)) return st;
+  constexpr bool kIn = InPlace::kBlocks == L::kBlocks;  // there is no such kernel
+  auto kernel = plan.ahead ? chunk_kernel<P, R, false, true> : chunk_kernel<P, R, false, kIn>;
+  const int bytes = plan.ahead ? L::kBytes : InPlace::kBytes;
+  if (int st = allow_smem(chunk_kernel<P, R, true, true>, L::kBytes)) return st;
+  if (int st = allow_smem(kernel, bytes)) return st;
   int* err = wxx::device_error_word();
   void* scratch = nullptr;
   if (g.count > 1) {
@@ -1223,7 +1257,7 @@ int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
     g.state = static_cast<float*>(scratch);
     g.kept = g.state + states * a.p * a.r;
     const unsigned per = (unsigned)(blocks * (g.count - 1));
-    chunk_kernel<P, R, true><<<per * n, kThreads, L::kBytes, wxx::stream()>>>(passes, maps, tma, s, g,
+    chunk_kernel<P, R, true, true><<<per * n, kThreads, L::kBytes, wxx::stream()>>>(passes, maps, tma, s, g,
                                                                             per, err);
     int st = wxx::after_launch(__FILE__, __LINE__);
     if (st == WXX_OK) {
@@ -1238,7 +1272,7 @@ int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
     }
   }
   const unsigned per = (unsigned)(blocks * g.count);
-  chunk_kernel<P, R, false><<<per * n, kThreads, L::kBytes, wxx::stream()>>>(passes, maps, tma, s, g,
+  kernel<<<per * n, kThreads, bytes, wxx::stream()>>>(passes, maps, tma, s, g,
                                                                            per, err);
   const int st = wxx::after_launch(__FILE__, __LINE__);
   if (scratch) wxx_free(scratch);
