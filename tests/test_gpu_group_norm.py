@@ -207,6 +207,33 @@ def test_empty_and_captured(rng):
     g.close()
 
 
+def test_more_than_32_bits_of_numbers(rng):
+    """Tokens and maps of more than 2^31 numbers, and more threads' places than 32 bits count:
+    zeros, whose result is beta, but for a few rows."""
+    import wxx_b200 as wxx
+
+    F = _F()
+    for shape, G, per in [((2100003, 1024), 16, 64), ((131100, 128, 128), 8, 16),
+                          (((1 << 25) + 5, 144), 16, 9)]:
+        x = wxx.Tensor(shape, value=0.0)
+        N, C = shape[0], shape[-1]
+        assert N * np.prod(shape[1:]) > 2 ** 31
+        rows = [0, N // 2, N // 2 + 1, N - 1]
+        some = rng.standard_normal((4, *shape[1:])).astype(np.float32)
+        for i, r in enumerate(rows):
+            F.assign(x.narrow(0, r, 1), up(some[i:i + 1]))
+        gamma, beta = (rng.standard_normal(C).astype(np.float32) for _ in range(2))
+        y, mean, inv = F.group_norm(x, G, up(gamma), up(beta))
+        ref, rmean, _ = retention.group_norm(some, G, gamma, beta)
+        for i, r in enumerate(rows):
+            near(y.narrow(0, r, 1).numpy()[0], ref[i], 1e-5)
+            near(mean.narrow(0, r, 1).numpy()[0], rmean[i], 1e-5, None)
+        for r in (1, N // 4, N // 2 + 2, 3 * (N // 4), N - 2):
+            got = y.narrow(0, r, 1).numpy()[0]
+            assert np.array_equal(got, np.broadcast_to(beta, got.shape))
+        del x, y, mean, inv
+
+
 def test_refusals():
     F = _F()
     x = up(np.zeros((4, 6), np.float32))

@@ -1007,6 +1007,8 @@ unsigned few_grid(Few& f, int least) {
   const int64_t row = (int64_t)f.G * f.lanes, most = (f.N + least - 1) / least;
   int64_t rows = least == 1 ? (f.N + 1) / 2 : ((int64_t)wxx::num_sms() * 1024 + row - 1) / row;
   if (rows > most) rows = most;
+  const int64_t counted = ((int64_t(1) << 31) - kT) / row;     // threads are counted in 32 bits
+  if (rows > counted) rows = counted;
   f.rows = (int)rows;
   return (unsigned)((rows * row + kT - 1) / kT);
 }
