@@ -118,6 +118,73 @@ def test_forward_and_backward(B, T, H, dk, dv, h0, reset, rng):
     check(rng, B, T, H, dk, dv, h0, reset)
 
 
+@pytest.mark.parametrize("B,T,H,dk,dv", [(24, 130, 16, 64, 64), (8, 200, 16, 64, 64),
+                                         (24, 70, 16, 63, 62), (10, 90, 32, 64, 40)])
+def test_more_rows_than_fit_at_a_time(B, T, H, dk, dv, rng):
+    """Hundreds of sequences and heads: three blocks on an SM, with the operands in place
+    (forward from 300 rows on, backward, whose passes run side by side, from 100)."""
+    check(rng, B, T, H, dk, dv, True, True)
+
+
+def test_non_finite_values_among_many_rows(rng):
+    F = _F()
+    B, T, H, d = 24, 150, 16, 64
+    q, k, v, h0, reset = inputs(rng, B, T, H, d, d, True, True)
+
+    def run(k):
+        o, last = F.linear_attention(up(q), up(k), up(v), up(decays(H)), up(h0), up(reset, np.uint32))
+        return o.numpy().reshape(B, T, H, d), last.numpy()
+
+    good, good_last = run(k)
+    bad = k.copy()
+    bad[7, 80, 3 * d + 5] = np.nan                  # head 3
+    got, last = run(bad)
+    hit = ~np.isfinite(got)
+    behind = np.flatnonzero(reset[7, 81:])
+    end = 81 + behind[0] if behind.size else T
+    want = np.zeros_like(hit)
+    want[7, 80:end, 3] = True
+    assert np.array_equal(hit, want)
+    others = np.ones((B, H), bool)
+    others[7, 3] = False
+    assert np.array_equal(got.transpose(0, 2, 1, 3)[others], good.transpose(0, 2, 1, 3)[others])
+    assert np.array_equal(last[others], good_last[others])
+
+
+def test_operands_and_states_past_32_bits(rng):
+    """Sequences more than 2^31 numbers apart in one buffer, and states of more than 2^31
+    numbers; rows behind the last sequence stay as they were."""
+    import wxx_b200 as wxx
+
+    F = _F()
+    T, H, d = 70, 2, 32
+    far = wxx.Tensor._empty([2, 1 << 21, 1100])             # 18 GB, only a corner is used
+    corner = far.narrow(1, 0, T).narrow(2, 8, 3 * H * d)
+    x = rng.standard_normal((2, T, 3 * H * d)).astype(np.float32)
+    F.assign(corner, up(x))
+    q, k, v = (corner.narrow(2, i * H * d, H * d) for i in range(3))
+    assert q.stride[0] > 2 ** 31
+    n = [np.ascontiguousarray(x[:, :, i * H * d:(i + 1) * H * d]) for i in range(3)]
+    for a, b in zip(F.linear_attention(q, k, v, up(decays(H))),
+                    F.linear_attention(*(up(t) for t in n), up(decays(H)))):
+        assert np.array_equal(a.numpy(), b.numpy())
+    f = F.rotary_frequencies(d)
+    assert np.array_equal(F.rotary(q, H, f).numpy(), F.rotary(up(n[0]), H, f).numpy())
+    del far, corner, q, k, v
+    B, d = 33000, 256
+    state = wxx.Tensor((B + 1, 1, d, d), value=0.25)
+    qkv = rng.standard_normal((3, B, d)).astype(np.float32)
+    o = F.linear_attention_step(*(up(t) for t in qkv), up(np.float32([-0.5])), state.narrow(0, 0, B))
+    for b in (0, B - 1):
+        ref = np.float64(np.exp(np.float64(-0.5))) * 0.25 + np.outer(qkv[1, b], qkv[2, b].astype(np.float64))
+        got = state.narrow(0, b, 1).numpy().reshape(d, d)
+        assert np.abs(got - ref).max() < 4 * U * np.abs(ref).max()
+        out = qkv[0, b] @ ref
+        assert np.abs(o.narrow(0, b, 1).numpy() - out).max() < (4 + d) * U * (
+            np.abs(qkv[0, b]) @ np.abs(ref)).max()
+    assert (state.narrow(0, B, 1).numpy() == 0.25).all()
+
+
 @pytest.mark.parametrize("value", [0.0, -1e-6, -0.7, -20.0, -200.0, -np.inf])
 def test_extreme_decays(value, rng):
     """No decay, almost none, and decays that forget everything: at 0 the state is a plain

@@ -154,8 +154,8 @@ def test_parameter_gradients_against_differences():
 
 def test_training_step_replays_from_a_graph():
     """Recorded steps on new batches end where the eager ones do (the embedding gradient's
-    atomic adds may reorder 32-bit sums, hence a tolerance), with an eager graph of another
-    model's operators alive meanwhile."""
+    atomic adds may reorder 32-bit sums, hence a tolerance), with an eager forward of
+    the same parameters alive meanwhile."""
     wxx = _wxx()
     F = wxx.functional
     V, D, H, L, S, B = 64, 32, 2, 2, 70, 2
@@ -184,9 +184,8 @@ def test_training_step_replays_from_a_graph():
     for k in range(4):
         load(ids, tgt, k)
         last_eager = float(step().numpy().reshape(-1)[0])
-    other, _ = build(V, D, H, L)
-    alive = other(u32(batches[0]))
     m_graph, ids, tgt, step = make()
+    alive = m_graph(ids)
     g = wxx.graph.capture(step)                 # its warm-up run is step 1 (batch 0)
     try:
         for k in range(1, 4):
@@ -295,7 +294,7 @@ def test_rotary_linear_attention_and_norm_in_a_row(rng):
 def test_refusals():
     wxx = _wxx()
     F = wxx.functional
-    for args in ((30, 16, None, 1), (30, 16, 3, 1), (30, 18, 2, 1)):
+    for args in ((30, 16, None, 1), (30, 16, 3, 1), (30, 18, 2, 1), (30, 514, 1, 1)):
         with pytest.raises(ValueError):
             wxx.nn.RecurrentLM(*args, mixer="retention")
     with pytest.raises(ValueError):

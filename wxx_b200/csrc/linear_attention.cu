@@ -1149,6 +1149,7 @@ int allow_smem(K kernel, int bytes) {
     k = kernel;
     return WXX_OK;
   }
+  WXX_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   return WXX_OK;
 }
 

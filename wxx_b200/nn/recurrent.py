@@ -83,9 +83,9 @@ class Retention(Module):
     def __init__(self, d_model, n_heads, base=10000.0):
         super().__init__()
         n_heads = int(n_heads)
-        if n_heads < 1 or d_model % n_heads or d_model // n_heads % 2:
+        if n_heads < 1 or d_model % n_heads or d_model // n_heads % 2 or d_model > 256 * n_heads:
             raise ValueError(f"{d_model} channels cannot be split over {n_heads} heads of an even "
-                             "number of them")
+                             "number of them, 256 at most")
         self.d_model = d_model
         self.n_heads = n_heads
         self.head_dim = d_model // n_heads
