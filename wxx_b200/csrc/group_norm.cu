@@ -441,38 +441,38 @@ __global__ void __launch_bounds__(kT)
   }
 }
 
-// out (2, C) from rows of 2 C partial sums, in a fixed order: 32 columns by 32 parts of
-// the rows a block.  First dbeta, then dgamma.
+// out (2, C) from rows of 2 C partial sums, in a fixed order: 16 columns by 64 parts of
+// the rows a block (32 by 32 has half as many blocks and twice the rows a thread, 0.8 us longer over
+// 592 rows of 2 x 1024).  First dbeta, then dgamma.
 __global__ void __launch_bounds__(1024)
     column_sums_kernel(float* __restrict__ dbeta, float* __restrict__ dgamma,
                        const float* __restrict__ part, int64_t rows, int C) {
-  __shared__ float sums[32][33];
+  __shared__ float sums[64][17];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+  const int column = threadIdx.x & 15, share = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + column;
   float a = 0.f;
   if (c < 2 * C) {
     const float* p = part + c;
-    int64_t r = warp;
-    for (; r + 224 < rows; r += 256) {
+    int64_t r = share;
+    for (; r + 448 < rows; r += 512) {
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = p[(r + 32 * k) * 2 * C];
+      for (int k = 0; k < 8; ++k) v[k] = p[(r + 64 * k) * 2 * C];
       a += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
     }
-    for (; r + 96 < rows; r += 128) {
-      float v[4];
+    float v[7];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = p[(r + 32 * k) * 2 * C];
-      a += (v[0] + v[1]) + (v[2] + v[3]);
-    }
-    for (; r < rows; r += 32) a += p[r * 2 * C];
+    for (int k = 0; k < 7; ++k) v[k] = r + 64 * k < rows ? p[(r + 64 * k) * 2 * C] : 0.f;
+    a += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + v[6]);
   }
-  sums[warp][lane] = a;
+  sums[share][column] = a;
   __syncthreads();
-  float v = sums[lane][warp];                        // a warp a column now
+  if (warp >= 16) return;
+  float v = sums[lane][warp] + sums[lane + 32][warp];      // a warp a column now
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int own = blockIdx.x * 32 + warp;
+  const int own = blockIdx.x * 16 + warp;
   if (lane == 0 && own < 2 * C) (own < C ? dbeta[own] : dgamma[own - C]) = v;
 }
 
@@ -1176,7 +1176,7 @@ WXX_EXPORT int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, f
     });
     int st = wxx::after_launch(__FILE__, __LINE__);
     if (st == WXX_OK) {
-      column_sums_kernel<<<(unsigned)((2 * C + 31) / 32), 1024, 0, wxx::stream()>>>(dbeta, dgamma, part,
+      column_sums_kernel<<<(unsigned)((2 * C + 15) / 16), 1024, 0, wxx::stream()>>>(dbeta, dgamma, part,
                                                                                  rows, (int)C);
       st = wxx::after_launch(__FILE__, __LINE__);
     }
@@ -1205,7 +1205,7 @@ WXX_EXPORT int wxx_group_norm_backward(float* dx, float* dgamma, float* dbeta, f
     st = wxx::after_launch(__FILE__, __LINE__);
   }
   if (st == WXX_OK) {
-    column_sums_kernel<<<(unsigned)((2 * C + 31) / 32), 1024, 0, wxx::stream()>>>(dbeta, dgamma, part,
+    column_sums_kernel<<<(unsigned)((2 * C + 15) / 16), 1024, 0, wxx::stream()>>>(dbeta, dgamma, part,
                                                                                rows, (int)C);
     st = wxx::after_launch(__FILE__, __LINE__);
   }
