@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kT) sweep_kernel(const Pass a, const Shape s) 
 // (they are good to 2^-38 of it).  (Measured, mma.sync: half 554, tf32 277 TFLOP/s; three
 // products of tf32 need no scaling, but would be bound by that rate.  On tcgen05, kind::tf32
 // with sums in TMEM, chunks of 128 took as long, and the truncated sums made the error 1.6e-6
-// instead of 4.6e-7.)  The state stays in 32-bit registers, a chunk's products are added to
+// instead of 5e-7 to 7e-7.)  The state stays in 32-bit registers, a chunk's products are added to
 // it in 32 bits.
 //
 // NaN and infinities cannot take part: 0 times NaN would carry them to earlier positions
@@ -811,7 +811,12 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
           add2(v[2], v[3], v[2], v[3], small[jt][2], small[jt][3]);
         }
       });
-      // x X
+      // x X.  A sum in a product loses up to an ulp each time (it is cut off, not rounded), so 128
+      // channels take all the small products first, while the sum is small: error 9.5e-7 ->
+      // 7.2e-7, 164 -> 170 us over 8 x 1024 tokens of 8 heads of 128.  In place it is also
+      // faster (193 -> 188 us backward over 8 x 1024 tokens of 16 heads of 64), ahead, whose
+      // error is 7.4e-7 at 64 channels, slower (261 -> 268 forward over 37 x 1024).
+      constexpr bool kSmallFirst = P == 128 || !AHEAD;
       float o[R / 8][4];
 #pragma unroll
       for (int nt = 0; nt < R / 8; ++nt)
@@ -825,7 +830,24 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
             uint32_t bh[4], bl[4];
             load4_turned<k * 16 * R * 2>(bh, read_state ^ (nb << 5));
             load4_turned<k * 16 * R * 2 + P * R * 2>(bl, read_state ^ (nb << 5));
-            products(o[2 * nb], o[2 * nb + 1], xh[k], xl[k], bh, bl);
+            if constexpr (kSmallFirst) {
+              product(o[2 * nb], xl[k], bh[0], bh[1]);
+              product(o[2 * nb + 1], xl[k], bh[2], bh[3]);
+              product(o[2 * nb], xh[k], bl[0], bl[1]);
+              product(o[2 * nb + 1], xh[k], bl[2], bl[3]);
+            } else {
+              products(o[2 * nb], o[2 * nb + 1], xh[k], xl[k], bh, bl);
+            }
+          }
+        });
+        for_each<kSmallFirst ? P / 16 : 0>([&](auto depth) {
+          constexpr int k = decltype(depth)::value;
+#pragma unroll
+          for (int nb = 0; nb < R / 16; ++nb) {
+            uint32_t bh[4];
+            load4_turned<k * 16 * R * 2>(bh, read_state ^ (nb << 5));
+            product(o[2 * nb], xh[k], bh[0], bh[1]);
+            product(o[2 * nb + 1], xh[k], bh[2], bh[3]);
           }
         });
       }
@@ -1158,8 +1180,8 @@ int allow_smem(K kernel, int bytes) {
 // in place, `more` of them: the least of the outputs' launch and, with more than one piece, the
 // states' one (half as long a chunk) and what lies between.  In units of a full SM's time for
 // one block's chunk; a start is about a chunk.  Measured, heads of 64, 16 chunks a row, 1, 2 and
-// 3 blocks on every SM: ahead 106 and 135 us (and 247: two turns), in place 129, 172 and 207; so
-// 384 rows take 243 and 195 us, 592 rows 261 and 369.  In 1 and 2 pieces 128 rows of 16 chunks
+// 3 blocks on every SM: ahead 106 and 135 us (and 247: two turns), in place 129, 172 and 196; so
+// 384 rows take 243 and 188 us, 592 rows 261 and 369.  In 1 and 2 pieces 128 rows of 16 chunks
 // 108 and 116 us; 64 of 128 chunks in 3, 4 and 8 pieces 463, 377 and 380; 16 of 128 in 8, 16 and
 // 32 pieces 175, 123 and 135.
 struct Plan {
@@ -1186,7 +1208,7 @@ Plan plan_of(int64_t rows, int64_t chunks, int blocks, int more) {
     const double a = states + ahead(rows * m) * (size + 1);
     if (m == 1 || a < least) least = a, best = {m, true};
     if (more == blocks) continue;
-    const double i = states + turns(rows * m, more, 0.95 * blocks, 1.03 * more) * (size + 1);
+    const double i = states + turns(rows * m, more, 0.95 * blocks, 0.97 * more) * (size + 1);
     if (i < least) least = i, best = {m, false};
   }
   return best;
