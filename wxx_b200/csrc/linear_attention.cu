@@ -535,6 +535,16 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
   auto next_row = [](int W, int k) { return W == 32 ? 4 * k : (k >> 1) * 8 + (k & 1) * 2; };
   auto row_of = [&](int W, int k) { return first_row(W) + next_row(W, k); };
 
+  // the resets, read a chunk ahead (waited for at the chunk: 394 instead of 368 us forward over 16
+  // x 8192 packed tokens of 4 heads of 64)
+  uint32_t mark[3] = {0, 0, 0};
+  auto read_marks = [&](int c) {
+    const int t0 = start(c), n = min(kC, s.T - t0);
+    mark[0] = lane < n ? __ldg(marks + t0 + lane) : 0;
+    mark[1] = lane + 32 < n ? __ldg(marks + t0 + lane + 32) : 0;
+    mark[2] = !back && t0 + n < s.T ? __ldg(marks + t0 + n) : 0;
+  };
+  if (marks) read_marks(c0);
   auto turn_over = [&](int c) {         // not AHEAD: this chunk's operands are done with
     if (AHEAD || c + 1 >= c1) return;
     wxx_tc::fence_proxy_async_smem();
@@ -547,9 +557,9 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
     unsigned long long cuts = 0;
     bool next = false;
     if (marks) {
-      const unsigned lo = __ballot_sync(0xffffffffu, lane < n && marks[t0 + lane] != 0);
-      const unsigned hi = __ballot_sync(0xffffffffu, lane + 32 < n && marks[t0 + lane + 32] != 0);
-      next = !back && t0 + n < s.T && marks[t0 + n] != 0;
+      const unsigned lo = __ballot_sync(0xffffffffu, mark[0] != 0);
+      const unsigned hi = __ballot_sync(0xffffffffu, mark[1] != 0);
+      next = mark[2] != 0;
       cuts = (unsigned long long)hi << 32 | lo;
     }
     const Weights w(cuts, n, t0 + n < s.T, back ? cuts & 1 : next);
@@ -670,6 +680,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
     }
     odd = __syncthreads_or(odd);        // the squares are here, the operands are read
     if (AHEAD && c + 1 < c1) fetch(c + 1);
+    if (marks && c + 1 < c1) read_marks(c + 1);
     const int kept_power = w.kept(back);
     const float kept = kept_power < 0 ? 0.f : m.power[kept_power];
     if (STATE) run *= kept;
@@ -1180,8 +1191,8 @@ int allow_smem(K kernel, int bytes) {
 // in place, `more` of them: the least of the outputs' launch and, with more than one piece, the
 // states' one (half as long a chunk) and what lies between.  In units of a full SM's time for
 // one block's chunk; a start is about a chunk.  Measured, heads of 64, 16 chunks a row, 1, 2 and
-// 3 blocks on every SM: ahead 106 and 135 us (and 247: two turns), in place 129, 172 and 196; so
-// 384 rows take 243 and 188 us, 592 rows 261 and 369.  In 1 and 2 pieces 128 rows of 16 chunks
+// 3 blocks on every SM: ahead 106 and 135 us (and 247: two turns), in place 129, 172 and 188; so
+// 384 rows take 243 and 180 us, 592 rows 261 and 369.  In 1 and 2 pieces 128 rows of 16 chunks
 // 108 and 116 us; 64 of 128 chunks in 3, 4 and 8 pieces 463, 377 and 380; 16 of 128 in 8, 16 and
 // 32 pieces 175, 123 and 135.
 struct Plan {
