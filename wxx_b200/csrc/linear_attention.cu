@@ -536,7 +536,9 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
   auto row_of = [&](int W, int k) { return first_row(W) + next_row(W, k); };
 
   // the resets, read a chunk ahead (waited for at the chunk: 394 instead of 368 us forward over 16
-  // x 8192 packed tokens of 4 heads of 64)
+  // x 8192 packed tokens of 4 heads of 64) where there are registers for them (four blocks of
+  // 32 by 32: 205 us without any over 65536 positions of 8 heads, else 199)
+  constexpr bool kMarksAhead = L::kBlocks < 4;
   uint32_t mark[3] = {0, 0, 0};
   auto read_marks = [&](int c) {
     const int t0 = start(c), n = min(kC, s.T - t0);
@@ -544,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
     mark[1] = lane + 32 < n ? __ldg(marks + t0 + lane + 32) : 0;
     mark[2] = !back && t0 + n < s.T ? __ldg(marks + t0 + n) : 0;
   };
-  if (marks) read_marks(c0);
+  if (kMarksAhead && marks) read_marks(c0);
   auto turn_over = [&](int c) {         // not AHEAD: this chunk's operands are done with
     if (AHEAD || c + 1 >= c1) return;
     wxx_tc::fence_proxy_async_smem();
@@ -557,6 +559,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
     unsigned long long cuts = 0;
     bool next = false;
     if (marks) {
+      if (!kMarksAhead) read_marks(c);
       const unsigned lo = __ballot_sync(0xffffffffu, mark[0] != 0);
       const unsigned hi = __ballot_sync(0xffffffffu, mark[1] != 0);
       next = mark[2] != 0;
@@ -680,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
     }
     odd = __syncthreads_or(odd);        // the squares are here, the operands are read
     if (AHEAD && c + 1 < c1) fetch(c + 1);
-    if (marks && c + 1 < c1) read_marks(c + 1);
+    if (kMarksAhead && marks && c + 1 < c1) read_marks(c + 1);
     const int kept_power = w.kept(back);
     const float kept = kept_power < 0 ? 0.f : m.power[kept_power];
     if (STATE) run *= kept;
