@@ -73,10 +73,10 @@ struct Decay {
 };
 
 // A block per sequence, head and 32 columns of X: lane = column, warp = every 8th row,
-// K rows a thread.  One position after the other.
-template <int K>
+// K rows a thread.  One position after the other: for heads of more than 128 channels, whose
+// state the chunks' kernel has no room for.
 __global__ void __launch_bounds__(kT) sweep_kernel(const Pass a, const Shape s) {
-  constexpr int kTile = K > 16 ? 8 : 16;      // positions of a tile
+  constexpr int K = 32, kTile = 8;      // rows, positions of a tile
   __shared__ float sx[kTile][8 * K], sy[kTile][8 * K], sz[kTile][32], part[8][kTile][32];
   __shared__ int cut[kTile];
   const int slices = (a.r + 31) / 32;
@@ -1168,7 +1168,7 @@ int check_sizes(const char* what, int64_t B, int64_t T, int64_t H, int64_t dk, i
 }
 
 int sweep(const Pass& a, const Shape& s, int64_t B) {
-  sweep_kernel<32><<<(unsigned)(B * s.H * ((a.r + 31) / 32)), kT, 0, wxx::stream()>>>(a, s);
+  sweep_kernel<<<(unsigned)(B * s.H * ((a.r + 31) / 32)), kT, 0, wxx::stream()>>>(a, s);
   return wxx::after_launch(__FILE__, __LINE__);
 }
 
