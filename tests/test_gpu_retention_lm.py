@@ -202,6 +202,31 @@ def test_training_step_replays_from_a_graph():
     assert wxx.backend.device_status() == 0
 
 
+def test_a_parameter_listed_twice_is_stepped_once():
+    """LayerNorm's parameters have two names each; AdamW steps them like any other, to the bit,
+    however its blocks are scheduled."""
+    wxx = _wxx()
+    F = wxx.functional
+    rng = np.random.default_rng(5)
+    sizes = [32, 4096, 70000]
+    w0 = [rng.standard_normal(n).astype(np.float32) for n in sizes]
+    grads = [[rng.standard_normal(n).astype(np.float32) for n in sizes] for _ in range(5)]
+
+    def run(times):
+        params = [wxx.Parameter(F.from_numpy(w)) for w in w0]
+        opt = wxx.nn.AdamW([("", p) for p in params for _ in range(times)], lr=1e-2)
+        for g in grads:
+            for p, t in zip(params, g):
+                p.grad = F.from_numpy(t)
+            opt.step()
+        return [p.numpy() for p in params]
+
+    once = run(1)
+    for _ in range(10):
+        for a, b in zip(run(2), once):
+            assert np.array_equal(a, b)
+
+
 @pytest.mark.parametrize("beams,n,stop", [(1, 12, None), (3, 12, None), (4, 16, 11), (8, 6, None)])
 def test_beam_search_over_states(beams, n, stop):
     wxx = _wxx()

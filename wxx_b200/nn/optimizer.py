@@ -75,9 +75,14 @@ class AdamW(Optimizer):
               "adamw_advance")
         rows = []
         keep = []
+        seen = set()
         for (_, w), st in zip(self.params, self.state):
-            if w.grad is None:
+            # A parameter listed again (LayerNorm registers weightg as weight, too) is stepped
+            # once: its two entries would run side by side in the launch and now and then
+            # see each other's half of a step.
+            if w.grad is None or id(w) in seen:
                 continue
+            seen.add(id(w))
             g = functional.contiguous(w.grad)
             if tuple(g.shape) != tuple(w.shape):
                 raise ValueError(f"adamw: grad shape {tuple(g.shape)} != {tuple(w.shape)}")
