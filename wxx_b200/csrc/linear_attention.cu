@@ -293,17 +293,23 @@ __device__ __forceinline__ uint32_t piece(int row, int q) {
 __device__ __forceinline__ int raw_piece(int row, int q) { return row * 8 + (q ^ (row & 7)); }
 constexpr int kRaw = kC * 128;          // their bytes
 
-template <int P, int R, bool AHEAD>
+// (STATE does without x and the state's tile, which makes room for a third block of 64 by 64: 366
+// -> 338 us forward over 16 x 8192 tokens of 4 heads of 64, 110 -> 92 over 3 x 4097 of 5 heads of
+// 40 by 72.)
+template <int P, int R, bool STATE, bool AHEAD>
 struct Layout {
-  static constexpr int kRawX = 0, kRawY = kRawX + P / 32 * kRaw, kRawZ = kRawY + P / 32 * kRaw;
+  static constexpr int kRawX = 0, kRawY = STATE ? 0 : P / 32 * kRaw, kRawZ = kRawY + P / 32 * kRaw;
   // high halves, then low halves, of y and z (AHEAD: not where the copies go) and the state
   static constexpr int kY = AHEAD ? kRawZ + R / 32 * kRaw : kRawY, kZ = kY + kC * P * 4;
   static constexpr int kState = kZ + kC * R * 4, kTiles = AHEAD ? kY : 0;
-  static constexpr int kEnd = kState + P * R * 4, kBytes = kEnd + 1024;
+  static constexpr int kEnd = kState + (STATE ? 0 : P * R * 4), kBytes = kEnd + 1024;
   static_assert((P * R + kThreads) * 4 + kC <= (AHEAD ? kState : kEnd) - kTiles, "rare_chunk's room");
   // the warps' parts of the state: kRowTiles times 16 rows by kColTiles tiles of 8 columns
   static constexpr int kRowTiles = P >= 64 ? P / 64 : 1, kColTiles = P >= 64 ? R / 8 : R / 16;
-  static constexpr int kBlocks = P == 128 ? 1 : P == 64 && R == 64 ? (AHEAD ? 2 : 3) : P == 32 && R == 32 ? 4 : 3;
+  static constexpr int kBlocks = P == 128                ? (STATE ? 2 : 1)
+                                 : P == 64 && R == 64 ? (AHEAD && !STATE ? 2 : 3)
+                                 : P == 32 && R == 32 ? 4
+                                                      : 3;
 };
 
 struct Segments {           // pieces of a row that are worked on side by side
@@ -415,11 +421,11 @@ __device__ void rare_chunk(float* state, float* sums, const unsigned char* cuts,
 // chunk's operands are copied meanwhile; else they are copied, and split, in the place of this
 // chunk's, which more blocks on an SM have room for (plan_of chooses).
 template <int P, int R, bool STATE, bool AHEAD>
-__global__ void __launch_bounds__(kThreads, Layout<P, R, AHEAD>::kBlocks)
+__global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
     chunk_kernel(const __grid_constant__ Passes passes, const __grid_constant__ Maps maps,
                  const bool tma, const Shape s, const Segments g, const unsigned per_pass,
                  int* err) {
-  using L = Layout<P, R, AHEAD>;
+  using L = Layout<P, R, STATE, AHEAD>;
   extern __shared__ __align__(1024) unsigned char raw_smem[];
   __shared__ Small m;
   unsigned char* smem = raw_smem + ((1024 - (smem_address(raw_smem) & 1023)) & 1023);
@@ -1196,13 +1202,13 @@ int allow_smem(K kernel, int bytes) {
 // one block's chunk; a start is about a chunk.  Measured, heads of 64, 16 chunks a row, 1, 2 and
 // 3 blocks on every SM: ahead 106 and 135 us (and 247: two turns), in place 129, 172 and 188; so
 // 384 rows take 243 and 180 us, 592 rows 261 and 369.  In 1 and 2 pieces 128 rows of 16 chunks
-// 108 and 116 us; 64 of 128 chunks in 3, 4 and 8 pieces 463, 377 and 380; 16 of 128 in 8, 16 and
-// 32 pieces 175, 123 and 135.
+// 108 and 116 us; with two of the states' blocks on an SM 64 of 128 chunks in 3, 4 and 8 pieces 463,
+// 377 and 380, 16 of 128 in 8, 16 and 32 pieces 175, 123 and 135.
 struct Plan {
   int pieces;
   bool ahead;
 };
-Plan plan_of(int64_t rows, int64_t chunks, int blocks, int more) {
+Plan plan_of(int64_t rows, int64_t chunks, int blocks, int more, int of_states) {
   const int64_t sms = wxx::num_sms();
   // n blocks, `fit` on an SM at a time: a full SM takes `full`, a block by itself `alone`
   auto turns = [&](int64_t n, int fit, double alone, double full) {
@@ -1218,7 +1224,7 @@ Plan plan_of(int64_t rows, int64_t chunks, int blocks, int more) {
   for (int m = 1; m <= 128 && 2 * m <= chunks + 1; ++m) {
     const int64_t size = (chunks + m - 1) / m;
     if ((chunks + size - 1) / size != m) continue;
-    const double states = m > 1 ? ahead(rows * (m - 1)) * (0.5 * size + 1) + 2.5 : 0.;
+    const double states = m > 1 ? turns(rows * (m - 1), of_states, 0.8 * blocks, of_states) * (0.5 * size + 1) + 2.5 : 0.;
     const double a = states + ahead(rows * m) * (size + 1);
     if (m == 1 || a < least) least = a, best = {m, true};
     if (more == blocks) continue;
@@ -1264,12 +1270,13 @@ bool encode(CUtensorMap* map, const Operand& o, int64_t B, int64_t T, int64_t H,
 // then the states before the pieces, then the outputs.
 template <int P, int R>
 int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
-  using L = Layout<P, R, true>;
-  using InPlace = Layout<P, R, P != 64 || R != 64>;     // (other sizes: measured no faster)
+  using L = Layout<P, R, false, true>;
+  using States = Layout<P, R, true, true>;
+  using InPlace = Layout<P, R, false, P != 64 || R != 64>;     // (other sizes: measured no faster)
   const Pass& a = passes.at[0];
   const int slices = (a.r + R - 1) / R;
   const int64_t heads = B * s.H, blocks = heads * slices, chunks = (s.T + kC - 1) / kC;
-  const Plan plan = plan_of(blocks * n, chunks, L::kBlocks, InPlace::kBlocks);
+  const Plan plan = plan_of(blocks * n, chunks, L::kBlocks, InPlace::kBlocks, States::kBlocks);
   Segments g{plan.pieces, 0, nullptr, nullptr};
   g.chunks = (int)((chunks + g.count - 1) / g.count);
   WXX_REQUIRE(blocks * n * g.count < (int64_t(1) << 31), "linear attention: too many sequences");
@@ -1283,7 +1290,7 @@ int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
   constexpr bool kIn = InPlace::kBlocks == L::kBlocks;  // there is no such kernel
   auto kernel = plan.ahead ? chunk_kernel<P, R, false, true> : chunk_kernel<P, R, false, kIn>;
   const int bytes = plan.ahead ? L::kBytes : InPlace::kBytes;
-  if (int st = allow_smem(chunk_kernel<P, R, true, true>, L::kBytes)) return st;
+  if (int st = allow_smem(chunk_kernel<P, R, true, true>, States::kBytes)) return st;
   if (int st = allow_smem(kernel, bytes)) return st;
   int* err = wxx::device_error_word();
   void* scratch = nullptr;
@@ -1294,7 +1301,7 @@ int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
     g.state = static_cast<float*>(scratch);
     g.kept = g.state + states * a.p * a.r;
     const unsigned per = (unsigned)(blocks * (g.count - 1));
-    chunk_kernel<P, R, true, true><<<per * n, kThreads, L::kBytes, wxx::stream()>>>(passes, maps, tma, s, g,
+    chunk_kernel<P, R, true, true><<<per * n, kThreads, States::kBytes, wxx::stream()>>>(passes, maps, tma, s, g,
                                                                             per, err);
     int st = wxx::after_launch(__FILE__, __LINE__);
     if (st == WXX_OK) {
