@@ -1,0 +1,61 @@
+"""Linear attention over rows long enough to be worked on in many pieces, against its 64-bit
+restatement: what reaches a piece from the ones before it."""
+
+import numpy as np
+import pytest
+
+from oracle import retention
+
+pytestmark = pytest.mark.gpu
+
+
+def _F():
+    import wxx_b200 as wxx
+
+    return wxx.functional
+
+
+def up(a, dtype=np.float32):
+    return None if a is None else _F().from_numpy(np.asarray(a), dtype=dtype)
+
+
+def normals(rng, *shapes):
+    return [rng.standard_normal(s).astype(np.float32) for s in shapes]
+
+
+@pytest.mark.parametrize("memory", [2, 8, 2000])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("d,T", [(32, 20000), (64, 9000)])
+def test_only_a_reset_ends_a_value_that_is_not_finite(d, T, bad, memory, rng):
+    """A NaN or an infinity near a row's start (backward: its end) reaches all that follows in
+    its document, in all pieces, also where the decays over a piece are below 2^-149."""
+    F = _F()
+    H = 2
+    q, k, v, do = normals(rng, *[(1, T, H * d)] * 4)
+    h0, dlast = normals(rng, *[(1, H, d, d)] * 2)
+    decay = np.log1p(-1 / np.full(H, memory, np.float64)).astype(np.float32)
+    with_reset = np.zeros((1, T), np.uint32)
+    with_reset[0, T // 2] = 1
+    for reset in (None, with_reset):
+        r = up(reset, np.uint32)
+        for name in ("v", "h0"):
+            given = {"v": v.copy(), "h0": h0.copy()}
+            given[name][(0, 70, 3) if name == "v" else (0, 0, 2, 3)] = bad    # head 0, column 3
+            o, last = F.linear_attention(up(q), up(k), up(given["v"]), up(decay), up(given["h0"]), r)
+            hit = ~np.isfinite(o.numpy())
+            want = np.zeros((1, T, H * d), bool)
+            want[0, 70 if name == "v" else 0:T if reset is None else T // 2, 3] = True
+            assert np.array_equal(hit, want)
+            hit = ~np.isfinite(last.numpy())
+            want = np.zeros((1, H, d, d), bool)
+            if reset is None:
+                want[0, 0, slice(None) if name == "v" else 2, 3] = True
+            assert np.array_equal(hit, want)
+        for name in ("do", "dlast"):
+            given = {"do": do.copy(), "dlast": dlast.copy()}
+            given[name][(0, T - 70, 3) if name == "do" else (0, 0, 2, 3)] = bad
+            dv = F.linear_attention_backward(up(given["do"]), up(q), up(k), up(v), up(decay), up(h0),
+                                             r, up(given["dlast"]))[2].numpy()
+            want = np.zeros((1, T, H * d), bool)
+            want[0, 0 if reset is None else T // 2:T - 69 if name == "do" else T, 3] = True
+            assert np.array_equal(~np.isfinite(dv), want)

@@ -315,7 +315,8 @@ struct Layout {
 struct Segments {           // pieces of a row that are worked on side by side
   int count, chunks;        // pieces, chunks of a piece
   float* state;             // (passes, count - 1, B H, p * r): after each piece but the last
-  float* kept;              // (passes, count - 1, B H): what a piece does to the state before it
+  float* kept;              // (passes, count - 1, B H): what a piece leaves of the state before it,
+                            // -1: a reset is in it (0 is a decay too small for 32 bits)
 };
 
 // The chunk's weights of decay and resets.
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
     });
   }
   const bool pairs_o = ((reinterpret_cast<uintptr_t>(a.out) & 7) == 0) && (a.r & 1) == 0;
-  float run = 1.f;                      // STATE: what the piece does to the state before it
+  float run = 1.f;                      // STATE: what the piece leaves of the state before it
 
   // Where this lane reads y (and, across rows, y^T), z and the state for the products: the
   // first 16 rows, the first 16 columns; 16 columns on is an address with 1 << 5 exchanged.
@@ -692,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
     if (kMarksAhead && marks && c + 1 < c1) read_marks(c + 1);
     const int kept_power = w.kept(back);
     const float kept = kept_power < 0 ? 0.f : m.power[kept_power];
-    if (STATE) run *= kept;
+    if (STATE) run = run < 0.f || kept_power < 0 ? -1.f : run * kept;
     const float square_state =
         (m.square_state[0] + m.square_state[1]) + (m.square_state[2] + m.square_state[3]);
     if (odd || (square_state > 0.f && square_state < kShort)) {
@@ -1061,7 +1062,8 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
 }
 
 // The states before the pieces, from what each piece adds to a state and keeps of it, in
-// place: a thread an entry, one piece after the other.
+// place: a thread an entry, one piece after the other.  Only a reset ends a NaN or an infinity,
+// however little the decays leave of a number.
 __global__ void __launch_bounds__(kT)
     join_kernel(const __grid_constant__ Passes passes, const Shape s, const Segments g,
                 const int64_t heads, const int64_t total) {
@@ -1073,12 +1075,12 @@ __global__ void __launch_bounds__(kT)
   const int p = (int)(i % size) / a.r, r = (int)(i % size) % a.r;
   const int64_t b = head / s.H;
   float X = a.from ? a.from[head * size + p * a.p_stride + r * a.r_stride] : 0.f;
-  if (!a.back)
-    X = s.reset && s.reset[b * s.T] != 0 ? 0.f : Decay(s.log_decay[head % s.H])(X);
+  const Decay l(s.log_decay[head % s.H]);
+  if (!a.back) X = s.reset && s.reset[b * s.T] != 0 ? 0.f : l(X);
   for (int k = 0; k < g.count - 1; ++k) {
     float* E = g.state + (pass * (int64_t)(g.count - 1) + k) * total + i;
     const float kept = g.kept[(pass * (int64_t)(g.count - 1) + k) * heads + head];
-    X = kept == 0.f ? *E : fmaf(kept, X, *E);
+    X = kept < 0.f ? *E : fabsf(X) < INFINITY ? fmaf(kept, X, *E) : l(X) + *E;
     *E = X;
   }
 }
