@@ -67,6 +67,43 @@ def linear_attention_backward(do, q, k, v, log_decay, h0=None, reset=None, dlast
     return dq.reshape(B, T, -1), dkey.reshape(B, T, -1), dval.reshape(B, T, -1), R
 
 
+def _swept(x, y, z, log_decay, start, chunk=128):
+    """``(out, last)`` of X_t = l X_{t-1} + y_t z_t^T, out_t = X_t^T x_t a chunk of positions at a
+    time; x, y (B, T, H, p), z (B, T, H, r), start (B, H, p, r)."""
+    ld = np.asarray(log_decay, np.float64)
+    X, out = start, np.empty(z.shape)
+    for a in range(0, z.shape[1], chunk):
+        xs, ys, zs = (t[:, a:a + chunk].transpose(0, 2, 1, 3) for t in (x, y, z))
+        i = np.arange(xs.shape[2])
+        n = len(i)
+        apart = i[:, None] - i
+        w = np.where(apart >= 0, np.exp(np.maximum(apart, 0) * ld[:, None, None]), 0.0)
+        before = np.exp((i + 1) * ld[:, None])[..., None]
+        left = np.exp((n - 1 - i) * ld[:, None])[..., None]
+        out[:, a:a + chunk] = (((xs @ ys.swapaxes(2, 3)) * w) @ zs
+                               + before * (xs @ X)).transpose(0, 2, 1, 3)
+        X = np.exp(n * ld)[:, None, None] * X + (left * ys).swapaxes(2, 3) @ zs
+    return out, X
+
+
+def linear_attention_long(do, q, k, v, log_decay, h0, dlast):
+    """(o, last, dq, dk, dv, dh0) of ``linear_attention`` and its backward without resets, for rows
+    too long to go through position by position."""
+    H = len(log_decay)
+    q, k, v, do = (_heads(t, H) for t in (q, k, v, do))
+    h0, R = np.asarray(h0, np.float64), np.asarray(dlast, np.float64)
+    o, last = _swept(q, k, v, log_decay, h0)
+    dq = _swept(do, v, k, log_decay, h0.swapaxes(2, 3))[0]
+    # backwards the decay comes after a position: before the first one it is taken off again
+    lam = np.exp(np.asarray(log_decay, np.float64))[:, None, None]
+    turned = [t[:, ::-1] for t in (q, k, v, do)]
+    dv, last_R = _swept(turned[1], turned[0], turned[3], log_decay, R / lam)
+    dk = _swept(turned[2], turned[3], turned[0], log_decay, R.swapaxes(2, 3) / lam)[0]
+    flat = (t.reshape(*t.shape[:2], -1) for t in (o, dq, dk[:, ::-1], dv[:, ::-1]))
+    o, dq, dk, dv = flat
+    return o, last, dq, dk, dv, lam * last_R
+
+
 def _logistic(v):
     e = np.exp(-np.abs(v))
     return np.where(v >= 0, 1 / (1 + e), e / (1 + e))

@@ -59,3 +59,43 @@ def test_only_a_reset_ends_a_value_that_is_not_finite(d, T, bad, memory, rng):
             want = np.zeros((1, T, H * d), bool)
             want[0, 0 if reset is None else T // 2:T - 69 if name == "do" else T, 3] = True
             assert np.array_equal(~np.isfinite(dv), want)
+
+
+@pytest.mark.parametrize("memory", [2 ** 14, 2 ** 16, 2 ** 18])
+@pytest.mark.parametrize("B,H,d", [(1, 2, 32), (1, 2, 64), (150, 1, 32)])
+def test_long_memories(B, H, d, memory, rng):
+    """Memories of 2^14 positions and more over 32768, in many pieces and (150 sequences) in few.
+    A state is rounded once a chunk of 64 positions, 512 times, independently: sqrt(512) u / 2 = 12
+    u of it; its products 8 u, its decays a few u for all chunks together: below 64 u = 4e-6 in the
+    2-norm.  Decays that are rounded alike in every chunk, u / 2 of the state each, would be off by up
+    to 256 u."""
+    F = _F()
+    T = 32768
+    rows = min(B, 2)                             # these again and again
+    q, k, v, do = normals(rng, *[(rows, T, H * d)] * 4)
+    k, v, q, do = k + 0.5, v + 0.5, q + 0.5, do + 0.5
+    h0, dlast = normals(rng, *[(rows, H, d, d)] * 2)
+    h0, dlast = 100 * h0, 100 * dlast
+    decay = np.full(H, np.log1p(-1 / memory), np.float32)
+
+    def many(t):
+        return up(np.ascontiguousarray(np.broadcast_to(t, (B // rows,) + t.shape)).reshape(
+            (B,) + t.shape[1:]))
+
+    def close(got, ref, what):
+        got = got.numpy().astype(np.float64)
+        for at in {0, B // rows - 1}:
+            part = got[at * rows:(at + 1) * rows]
+            e = np.linalg.norm(part - ref) / np.linalg.norm(ref)
+            assert e < 4e-6, (what, e)
+
+    refs = retention.linear_attention_long(do, q, k, v, decay, h0, dlast)
+    args = [many(t) for t in (q, k, v)] + [up(decay), many(h0)]
+    got = (*F.linear_attention(*args),
+           *F.linear_attention_backward(many(do), *args, None, many(dlast)))
+    for name, g, ref in zip(("o", "last", "dq", "dk", "dv", "dh0"), got, refs):
+        close(g, ref, name)
+    # what is left of h0 alone
+    none = np.zeros_like(v)
+    o, last = F.linear_attention(many(q), many(k), many(none), up(decay), many(h0))
+    close(last, np.exp(T * decay.astype(np.float64))[None, :, None, None] * h0, "h0")

@@ -204,3 +204,18 @@ def test_refusals():
                       ((u(4, 5, 6), x, m, m, 2), TypeError), ((x, x, m, m, 4), ValueError)]:
         with pytest.raises(err):
             F.group_norm_backward(*args)
+
+
+def test_linear_attention_a_chunk_at_a_time(rng):
+    """The form for long rows against the one that goes position by position."""
+    B, T, H, dk, dv = 2, 300, 3, 4, 6
+    q, k = (rng.standard_normal((B, T, H * dk)) for _ in range(2))
+    v, do = (rng.standard_normal((B, T, H * dv)) for _ in range(2))
+    h0, dlast = (rng.standard_normal((B, H, dk, dv)) for _ in range(2))
+    decay = np.array([-0.5, -0.01, 0.0])
+    got = retention.linear_attention_long(do, q, k, v, decay, h0, dlast)
+    want = (retention.linear_attention(q, k, v, decay, h0)
+            + retention.linear_attention_backward(do, q, k, v, decay, h0, None, dlast))
+    for a, b in zip(got, want):
+        assert a.shape == b.shape
+        assert np.abs(a - b).max() < 1e-11 * np.abs(b).max()

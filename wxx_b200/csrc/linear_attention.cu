@@ -62,11 +62,17 @@ constexpr int kT = 256;
 // One position's decay of a state, l X.  A decay near 1 is applied as X + (l - 1) X: l alone
 // is rounded to 2^-25, which n positions in a row make n 2^-25.
 // (An infinite state takes l itself: of the two terms' signs one is the other's opposite.)
+// The same for n positions at once, with n log l in the place of log l: a chunk's l^64, rounded
+// alike in every chunk, left a state after 32768 positions with a memory of 2^18 off by 7e-6, h0's
+// part of it by 1.5e-5; now 2.4e-7 and 3e-7.
+__device__ __forceinline__ float whole_of(float log_decay) { return log_decay > -0.5f ? 1.f : 0.f; }
+__device__ __forceinline__ float less_of(float log_decay) {
+  return log_decay > -0.5f ? expm1f(log_decay) : expf(log_decay);
+}
 struct Decay {
   float l, less, whole;
   __device__ explicit Decay(float log_decay)
-      : l(expf(log_decay)), less(log_decay > -0.5f ? expm1f(log_decay) : l),
-        whole(log_decay > -0.5f ? 1.f : 0.f) {}
+      : l(expf(log_decay)), less(less_of(log_decay)), whole(whole_of(log_decay)) {}
   __device__ __forceinline__ float operator()(float X) const {
     return fabsf(X) < INFINITY ? fmaf(less, X, whole * X) : l * X;
   }
@@ -315,8 +321,8 @@ struct Layout {
 struct Segments {           // pieces of a row that are worked on side by side
   int count, chunks;        // pieces, chunks of a piece
   float* state;             // (passes, count - 1, B H, p * r): after each piece but the last
-  float* kept;              // (passes, count - 1, B H): what a piece leaves of the state before it,
-                            // -1: a reset is in it (0 is a decay too small for 32 bits)
+  float2* kept;             // (passes, count - 1, B H): what a piece leaves of a state X before it,
+                            // x X + y X as in Decay; y = -1: nothing, a reset is in it
 };
 
 // The chunk's weights of decay and resets.
@@ -368,6 +374,7 @@ struct alignas(16) Small {
   float2 weight[kC];
   uint16_t added[2][kC];                // j's weight in the state, as a product of two halves
   float power[kC + 4];                  // l^n
+  float2 kept[kC + 4];                  // what n positions leave of a state: Decay's less and whole
   int document[kC];
   uint64_t arrived;                     // y, z and x are here
   int abort;
@@ -445,9 +452,12 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
   const int mat = lane >> 3, mat_row = lane & 7;
   const bool back = a.back;
   const Decay l(s.log_decay[h]);
-  if (threadIdx.x <= kC)
-    m.power[threadIdx.x] =
-        threadIdx.x == 0 ? 1.f : expf((float)threadIdx.x * s.log_decay[h]);
+  if (threadIdx.x <= kC) {
+    const float n_log = (float)threadIdx.x * s.log_decay[h];
+    const float power = threadIdx.x == 0 ? 1.f : expf(n_log), whole = whole_of(n_log);
+    m.power[threadIdx.x] = power;
+    m.kept[threadIdx.x] = make_float2(whole != 0.f ? expm1f(n_log) : power, whole);
+  }
 
   const int chunks = (s.T + kC - 1) / kC;
   const int c0 = seg * g.chunks, c1 = min(c0 + g.chunks, chunks);
@@ -528,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
     });
   }
   const bool pairs_o = ((reinterpret_cast<uintptr_t>(a.out) & 7) == 0) && (a.r & 1) == 0;
-  float run = 1.f;                      // STATE: what the piece leaves of the state before it
+  int run = 0;                          // STATE: the piece's decays, -1: a reset is in it
 
   // Where this lane reads y (and, across rows, y^T), z and the state for the products: the
   // first 16 rows, the first 16 columns; 16 columns on is an address with 1 << 5 exchanged.
@@ -692,8 +702,8 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
     if (AHEAD && c + 1 < c1) fetch(c + 1);
     if (kMarksAhead && marks && c + 1 < c1) read_marks(c + 1);
     const int kept_power = w.kept(back);
-    const float kept = kept_power < 0 ? 0.f : m.power[kept_power];
-    if (STATE) run = run < 0.f || kept_power < 0 ? -1.f : run * kept;
+    const float2 kept = kept_power < 0 ? make_float2(0.f, 0.f) : m.kept[kept_power];
+    if (STATE) run = run < 0 || kept_power < 0 ? -1 : run + kept_power;
     const float square_state =
         (m.square_state[0] + m.square_state[1]) + (m.square_state[2] + m.square_state[3]);
     if (odd || (square_state > 0.f && square_state < kShort)) {
@@ -1041,8 +1051,10 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           float(&v)[4] = X[mt][nt];
-          mul2(v[e], v[e + 1], v[e], v[e + 1], kept, kept);
-          fma2(v[e], v[e + 1], d[nt][e], d[nt][e + 1], by.first, by.first, v[e], v[e + 1]);
+          float t0, t1;
+          mul2(t0, t1, v[e], v[e + 1], kept.x, kept.x);
+          fma2(t0, t1, d[nt][e], d[nt][e + 1], by.first, by.first, t0, t1);
+          fma2(v[e], v[e + 1], v[e], v[e + 1], kept.y, kept.y, t0, t1);
         }
     }
     turn_over(c);
@@ -1057,8 +1069,11 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
       if (p < a.p && r < a.r) to[p * ps + r * rs] = v;
     });
   }
-  if (STATE && threadIdx.x == 0)
-    g.kept[(pass * (int64_t)pieces + seg) * heads + b * s.H + h] = run;
+  if (STATE && threadIdx.x == 0) {
+    const float run_log = (float)run * s.log_decay[h];
+    g.kept[(pass * (int64_t)pieces + seg) * heads + b * s.H + h] =
+        run < 0 ? make_float2(0.f, -1.f) : make_float2(less_of(run_log), whole_of(run_log));
+  }
 }
 
 // The states before the pieces, from what each piece adds to a state and keeps of it, in
@@ -1077,11 +1092,21 @@ __global__ void __launch_bounds__(kT)
   float X = a.from ? a.from[head * size + p * a.p_stride + r * a.r_stride] : 0.f;
   const Decay l(s.log_decay[head % s.H]);
   if (!a.back) X = s.reset && s.reset[b * s.T] != 0 ? 0.f : l(X);
+  float* E = g.state + pass * (int64_t)(g.count - 1) * total + i;
+  const float2* kept = g.kept + pass * (int64_t)(g.count - 1) * heads + head;
+  // a piece's numbers are read before the one before it is written
+  float own = *E;
+  float2 left = __ldg(kept);
   for (int k = 0; k < g.count - 1; ++k) {
-    float* E = g.state + (pass * (int64_t)(g.count - 1) + k) * total + i;
-    const float kept = g.kept[(pass * (int64_t)(g.count - 1) + k) * heads + head];
-    X = kept < 0.f ? *E : fabsf(X) < INFINITY ? fmaf(kept, X, *E) : l(X) + *E;
+    const bool more = k + 1 < g.count - 1;
+    const float next = more ? E[total] : 0.f;
+    const float2 next_left = more ? __ldg(kept + heads) : left;
+    X = left.y < 0.f             ? own
+        : fabsf(X) < INFINITY ? fmaf(left.y, X, fmaf(left.x, X, own))
+                                 : l(X) + own;
     *E = X;
+    own = next, left = next_left;
+    E += total, kept += heads;
   }
 }
 
@@ -1298,10 +1323,10 @@ int chunked(const Passes& passes, int n, const Shape& s, int64_t B) {
   void* scratch = nullptr;
   if (g.count > 1) {
     const int64_t states = n * (g.count - 1) * heads;
-    if (int st = wxx_malloc(&scratch, (uint64_t)(states * (a.p * a.r + 1)) * sizeof(float)))
+    if (int st = wxx_malloc(&scratch, (uint64_t)(states * (a.p * a.r + 2)) * sizeof(float)))
       return st;
-    g.state = static_cast<float*>(scratch);
-    g.kept = g.state + states * a.p * a.r;
+    g.kept = static_cast<float2*>(scratch);
+    g.state = reinterpret_cast<float*>(g.kept + states);
     const unsigned per = (unsigned)(blocks * (g.count - 1));
     chunk_kernel<P, R, true, true><<<per * n, kThreads, States::kBytes, wxx::stream()>>>(passes, maps, tma, s, g,
                                                                             per, err);
