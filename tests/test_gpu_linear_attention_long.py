@@ -99,3 +99,31 @@ def test_long_memories(B, H, d, memory, rng):
     none = np.zeros_like(v)
     o, last = F.linear_attention(many(q), many(k), many(none), up(decay), many(h0))
     close(last, np.exp(T * decay.astype(np.float64))[None, :, None, None] * h0, "h0")
+
+
+@pytest.mark.parametrize("d", [32, 64])
+def test_sizes_of_a_chunk_do_not_meet(d, rng):
+    """Positions of a chunk whose keys and values are more than 2^126 apart, the large ones
+    later, or in another document: each output is as good as its own terms allow."""
+    F = _F()
+    T, H = 64, 1
+    q, k, v = normals(rng, *[(1, T, d)] * 3)
+    size = np.where(np.arange(T) < 20, 1e-10, np.where(np.arange(T) < 40, 1e12, 1e-12))
+    k, v = ((t * size[None, :, None]).astype(np.float32) for t in (k, v))
+    reset = np.zeros((1, T), np.uint32)
+    reset[0, 40] = 1
+    decay = np.float32([-0.01])
+    for back in (False, True):
+        if back:
+            got = F.linear_attention_backward(up(v), up(k), up(q), up(q), up(decay), None,
+                                              up(reset, np.uint32))[2].numpy()
+            ref = retention.linear_attention_backward(v, k, q, q, decay, None, reset)[2]
+            top = retention.linear_attention_backward(*map(np.abs, (v, k, q, q)), decay, None, reset)[2]
+        else:
+            got = F.linear_attention(up(q), up(k), up(v), up(decay), None, up(reset, np.uint32))[0].numpy()
+            ref = retention.linear_attention(q, k, v, decay, None, reset)[0]
+            top = retention.linear_attention(*map(np.abs, (q, k, v)), decay, None, reset)[0]
+        # 3 * 2^-22 of the rows' lengths for halves, (64 + 8 sqrt(64) + d) u for the sums
+        tol = (3 * 2.0 ** -22 + (128 + d) * 2.0 ** -24) * d
+        worst = np.abs(got - ref).max(-1) / top.max(-1)
+        assert worst.max() < tol, (back, worst)

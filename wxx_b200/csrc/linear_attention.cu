@@ -173,7 +173,9 @@ __global__ void __launch_bounds__(kT) sweep_kernel(const Pass a, const Shape s) 
 //
 // NaN and infinities cannot take part: 0 times NaN would carry them to earlier positions
 // and other documents.  A chunk with a row whose length is not between 2^-60 and 2^63 (or 0),
-// or such a state, is worked through position by position (rare_chunk).
+// or such a state, is worked through position by position (rare_chunk); and one whose products
+// of lengths |y_j| |z_j| are more than 2^110 apart, so that a later position, or another
+// document's, cannot cost one its value.
 
 using wxx_tc::mbar_arrive_expect_tx;
 using wxx_tc::mbar_init;
@@ -269,6 +271,9 @@ __device__ __forceinline__ void square2(float& s0, float& s1, float a, float b) 
 }
 // Whether a row (or the state) of this square cannot be scaled; 0 alone says nothing yet.
 constexpr float kShort = 0x1p-120f, kLong = 0x1p126f;
+// Rows of y and z with squares between these are not too far apart.
+constexpr float kBelow = 0x1p-54f, kAbove = 0x1p54f;
+constexpr int kApart = 110;
 // The exponent of a length with this square.
 __device__ __forceinline__ int exponent(float square) {
   return ((int)(__float_as_uint(square) >> 23) - 127) >> 1;
@@ -365,6 +370,20 @@ struct Decayed {
   }
 };
 
+// Whether the products of the lengths of a chunk's rows are too far apart, from their squares.
+__device__ __forceinline__ bool far_apart(const float* square_y, const float* square_z) {
+  int most = -1000, least = 1000;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int j = (threadIdx.x & 31) + 32 * k;
+    if (square_y[j] == 0.f || square_z[j] == 0.f) continue;          // nothing there
+    const int e = exponent(square_y[j]) + exponent(square_z[j]);
+    most = max(most, e);
+    least = min(least, e);
+  }
+  return __reduce_max_sync(0xffffffffu, most) - __reduce_min_sync(0xffffffffu, least) > kApart;
+}
+
 // The parts of shared memory that are not tiles.
 struct alignas(16) Small {
   float square_y[kC], square_z[kC];     // of the rows
@@ -377,6 +396,7 @@ struct alignas(16) Small {
   float2 kept[kC + 4];                  // what n positions leave of a state: Decay's less and whole
   int document[kC];
   uint64_t arrived;                     // y, z and x are here
+  int look;                             // the last chunk that may have rows too far apart
   int abort;
 };
 
@@ -501,6 +521,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
   if (threadIdx.x == 0) {
     mbar_init(&m.arrived, 1);
     m.abort = 0;
+    m.look = -1;
     wxx_tc::fence_barrier_init();
   }
   __syncthreads();
@@ -610,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
       copies_done();
     __syncthreads();       // the operands are here, the last chunk's tiles are read
 
-    bool rare = false;                  // a row's square is out of range
+    bool rare = false;                  // a row's square is out of range, or far from the middle
     float4 y[4][P / 32], z[4][R / 32];
     auto up_of = [](float square) { return square == 0.f ? 0.f : power2(kTop - exponent(square)); };
     float up_y[4], up_z[4];
@@ -635,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
         s0 += s1;
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-        rare = rare || !(s0 >= kShort && s0 < kLong);
+        rare = rare || !(s0 >= kBelow && s0 < kAbove);
         up[k] = up_of(s0);
         if (piece_of == 0) squares[row_of(W, k)] = s0;
       }
@@ -672,6 +693,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
       }
     }
     if (__any_sync(0xffffffffu, rare)) {       // rows of zeros are fine
+      if (lane == 0) m.look = c;
       auto look = [&](const float* squares, int W, int row, float v0, float v1, float v2, float v3) {
         const float s0 = squares[row];
         odd = odd || !(s0 < kLong) ||
@@ -706,6 +728,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
     if (STATE) run = run < 0 || kept_power < 0 ? -1 : run + kept_power;
     const float square_state =
         (m.square_state[0] + m.square_state[1]) + (m.square_state[2] + m.square_state[3]);
+    if (!STATE && m.look == c) odd = odd || far_apart(m.square_y, m.square_z);
     if (odd || (square_state > 0.f && square_state < kShort)) {
       float* state = reinterpret_cast<float*>(smem + L::kTiles);
       unsigned char* cut = smem + L::kTiles + (P * R + kThreads) * 4;
@@ -747,7 +770,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
       const bool any = sy != 0.f && sz != 0.f;
       const int e = exponent(sy) + exponent(sz);
       const Decayed u(m.power, w.added(j, back));
-      const float one = !any || e - most < -126 ? 0.f : __fdividef(a.y_scale * power2(e - most), u.rest);
+      const float one = !any ? 0.f : __fdividef(a.y_scale * power2(e - most), u.rest);
       m.weight[j] = make_float2(one, one * m.power[back ? j & 15 : 15 - (j & 15)]);
       const int below = any && u.any ? e + u.e - most_added : -1000;
       // 2^below as two halves, each 2^-24 at least (0: less than 2^-38 of the largest)
