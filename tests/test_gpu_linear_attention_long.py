@@ -127,3 +127,24 @@ def test_sizes_of_a_chunk_do_not_meet(d, rng):
         tol = (3 * 2.0 ** -22 + (128 + d) * 2.0 ** -24) * d
         worst = np.abs(got - ref).max(-1) / top.max(-1)
         assert worst.max() < tol, (back, worst)
+
+
+@pytest.mark.parametrize("d,scale", [(64, 1e-36), (64, -1e-30), (32, 1e30), (32, 1e-33), (200, 1e-36)])
+def test_scales_near_the_ends_of_the_range(d, scale, rng):
+    """A scale multiplies: outputs and gradients are those of scale 1 times it, each term rounded
+    as there (two roundings more), the states free of it."""
+    F = _F()
+    B, T, H = 2, 150, 2
+    q, k, v, do = normals(rng, *[(B, T, H * d)] * 4)
+    h0, dlast = normals(rng, *[(B, H, d, d)] * 2)
+    dlast *= np.float32(scale)
+    decay = np.log1p(-1 / np.float32([8, 100])).astype(np.float32)
+    args = [up(t) for t in (q, k, v, decay, h0)]
+    o, last = F.linear_attention(*args, scale=scale)
+    scale = float(np.float32(scale))
+    refs = (*retention.linear_attention(q, k, v, decay, h0, None, scale),
+            *retention.linear_attention_backward(do, q, k, v, decay, h0, None, dlast, scale))
+    got = (o, last, *F.linear_attention_backward(up(do), *args, None, up(dlast), scale=scale))
+    for g, ref in zip(got, refs):
+        e = np.linalg.norm(g.numpy().astype(np.float64) - ref) / np.linalg.norm(ref)
+        assert e < 4e-6, e

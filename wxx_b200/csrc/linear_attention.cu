@@ -18,6 +18,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <type_traits>
 
@@ -49,7 +50,15 @@ struct Pass {
   int p, r;
   float y_scale, out_scale;
   int back;
+  // the scales as units in [1, 2) (or 0) and powers of two, which stay in range beside others
+  float y_unit, out_unit;
+  int y_exp, out_exp;
 };
+float unit_of(float scale, int& exp) {
+  const float half = frexpf(scale, &exp);
+  --exp;
+  return 2.f * half;
+}
 
 struct Shape {
   const float* log_decay;   // (H)
@@ -770,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
       const bool any = sy != 0.f && sz != 0.f;
       const int e = exponent(sy) + exponent(sz);
       const Decayed u(m.power, w.added(j, back));
-      const float one = !any ? 0.f : __fdividef(a.y_scale * power2(e - most), u.rest);
+      const float one = !any ? 0.f : __fdividef(a.y_unit * power2(e - most), u.rest);
       m.weight[j] = make_float2(one, one * m.power[back ? j & 15 : 15 - (j & 15)]);
       const int below = any && u.any ? e + u.e - most_added : -1000;
       // 2^below as two halves, each 2^-24 at least (0: less than 2^-38 of the largest)
@@ -953,7 +962,8 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
       // Both sums in one scale: the larger's, whichever part it comes from.
       float up[2];
       float by[2], then[2];
-      const int apart = (square_state > 0.f ? exponent(square_state) : 0) + 2 * kTop - most;
+      const int unit = most + a.y_exp;
+      const int apart = (square_state > 0.f ? exponent(square_state) : 0) + 2 * kTop - unit;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int i = warp * 16 + quad + half * 8;
@@ -970,7 +980,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
             mul2(o[nt][2 * half], o[nt][2 * half + 1], o[nt][2 * half], o[nt][2 * half + 1], in, in);
         }
         up[half] = kTop - e_p < -126 ? 0.f : power2(kTop - e_p);
-        const Scale scale(a.out_scale, e_p + e_x[half] + most - 4 * kTop);
+        const Scale scale(a.out_unit, e_p + e_x[half] + unit + a.out_exp - 4 * kTop);
         by[half] = scale.first;
         then[half] = scale.then;
       }
@@ -1022,7 +1032,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
       }
     }
     // the state: what the chunk adds, then in 32 bits
-    const Scale by(a.y_scale, most_added - 2 * kTop);
+    const Scale by(a.y_unit, most_added + a.y_exp - 2 * kTop);
 #pragma unroll
     for (int mt = 0; mt < L::kRowTiles; ++mt) {
       float d[L::kColTiles][4];
@@ -1386,6 +1396,8 @@ int run_passes(const Pass* a, int n, const Shape& s, int64_t B) {
           (a[i].r + 63) / 64 != (a[i - k].r + 63) / 64)
         break;
       same.at[k] = a[i];
+      same.at[k].y_unit = unit_of(a[i].y_scale, same.at[k].y_exp);
+      same.at[k].out_unit = unit_of(a[i].out_scale, same.at[k].out_exp);
     }
     int st;
     if (P == 256) {
