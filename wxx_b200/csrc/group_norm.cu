@@ -74,6 +74,14 @@ __device__ __forceinline__ float clamped(float v, float high, float middle, floa
   return v > 10.f ? high : v < -10.f ? low : middle;
 }
 
+// Sums for a mean are made of 2^-16 of the numbers: as good, and those of 2^14 numbers of 2^126 fit.
+// Squared distances from the mean overflow from 2^64 / sqrt(n) on: their sum is then made again of
+// distances in units of 2^80, of which 2^24 fit.
+constexpr float kDown = 0x1p-16f, kUp = 0x1p16f, kFar = 0x1p-80f;
+__device__ __forceinline__ float far_inverse(float variance, float eps) {
+  return inverse_root(fmaf(eps * kFar, kFar, variance)) * kFar;
+}
+
 // The activations of two numbers, in place.
 template <int ACT>
 __device__ __forceinline__ void act2(float& v0, float& v1) {
@@ -299,15 +307,50 @@ __global__ void __launch_bounds__(kT)
 // mean and inv (N, G) from the pieces' moments.
 __global__ void __launch_bounds__(kT)
     statistics_kernel(float* __restrict__ mean, float* __restrict__ inv,
-                      const Moments* __restrict__ part, const Shape s) {
+                      const Moments* __restrict__ part, const float* __restrict__ x, const Shape s) {
+  __shared__ bool far[kT];
+  __shared__ float sums[kT / 32];
   const int64_t i = (int64_t)blockIdx.x * kT + threadIdx.x;
-  if (i >= s.N * s.G) return;
-  const int64_t n = i / s.G;
-  const int g = (int)(i - n * s.G);
-  Moments m = {0.f, 0.f, 0.f};
-  for (int k = 0; k < s.chunks; ++k) m = join(m, part[(n * s.chunks + k) * s.G + g]);
-  mean[i] = m.mean;
-  inv[i] = inverse_root(m.m2 / ((float)s.S * (float)s.per) + s.eps);
+  const float count = (float)s.S * (float)s.per;
+  bool range = true;
+  if (i < s.N * s.G) {
+    const int64_t n = i / s.G;
+    const int g = (int)(i - n * s.G);
+    Moments m = {0.f, 0.f, 0.f};
+    for (int k = 0; k < s.chunks; ++k) m = join(m, part[(n * s.chunks + k) * s.G + g]);
+    const float variance = m.m2 / count;
+    mean[i] = m.mean;
+    inv[i] = inverse_root(variance + s.eps);
+    range = variance < INFINITY;
+  }
+  far[threadIdx.x] = !range;
+  if (!__syncthreads_or(!range)) return;
+  // the groups out of range one after the other, by all threads
+  auto block_sum = [&](float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kT / 32; ++w) all += sums[w];
+    __syncthreads();
+    return all;
+  };
+  for (int t = 0; t < kT; ++t) {
+    if (!far[t]) continue;
+    const int64_t j = (int64_t)blockIdx.x * kT + t, n = j / s.G;
+    const float* group = x + n * s.S * s.C + (j - n * s.G) * s.per;
+    const int64_t numbers = s.S * s.per;
+    const float mu = mean[j];
+    float squares = 0.f;
+    for (int64_t k = threadIdx.x; k < numbers; k += kT) {
+      const float d = (group[k / s.per * s.C + k % s.per] - mu) * kFar;
+      squares = fmaf(d, d, squares);
+    }
+    const float all = block_sum(squares);
+    if (threadIdx.x == 0) inv[j] = far_inverse(all / count, s.eps);
+  }
 }
 
 template <bool GATED>
@@ -496,6 +539,21 @@ __device__ __forceinline__ float over_lanes(float v, int lanes) {
   return v;
 }
 
+// The sum of squares of a group's distances in units of 2^80, over the group's lanes alone.
+template <int V, int K>
+__device__ __forceinline__ float far_squares(const Pack<V> (&v)[K], int lane, const Few& f) {
+  const unsigned group = f.lanes == 32 ? 0xffffffffu
+                                       : ((1u << f.lanes) - 1) << (threadIdx.x & 31 & -f.lanes);
+  float far = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if ((k * f.lanes + lane) * V < f.per)
+#pragma unroll
+      for (int e = 0; e < V; ++e) far = fmaf(v[k].v[e] * kFar, v[k].v[e] * kFar, far);
+  for (int o = f.lanes >> 1; o > 0; o >>= 1) far += __shfl_xor_sync(group, far, o);
+  return far;
+}
+
 template <int V, int K, bool GATED>
 __global__ void __launch_bounds__(kT)
     token_kernel(float* __restrict__ y, float* __restrict__ mean, float* __restrict__ inv,
@@ -520,8 +578,9 @@ __global__ void __launch_bounds__(kT)
     const bool on = here && n < f.N;
     const int64_t at = n * f.C + g * f.per;
     Pack<V> v[K], w[GATED ? K : 1];
-    float sums[V], means[V];
+    float sums[V], means[V], downs[V];
     fill<V>(sums, 0.f);
+    fill<V>(downs, kDown);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (k * f.lanes + lane) * V;
@@ -532,8 +591,8 @@ __global__ void __launch_bounds__(kT)
       if (GATED && in) w[k] = load<V>(gate + at + c);
     }
 #pragma unroll
-    for (int k = 0; k < K; ++k) add_all<V>(sums, sums, v[k].v);
-    const float mu = over_lanes(total<V>(sums), f.lanes) * share;
+    for (int k = 0; k < K; ++k) fma_all<V>(sums, v[k].v, downs, sums);
+    const float mu = over_lanes(total<V>(sums), f.lanes) * (share * kUp);
     fill<V>(means, mu);
     fill<V>(sums, 0.f);
 #pragma unroll
@@ -541,8 +600,10 @@ __global__ void __launch_bounds__(kT)
       sub_all<V>(v[k].v, v[k].v, means);
       if ((k * f.lanes + lane) * V < f.per) fma_all<V>(sums, v[k].v, v[k].v, sums);
     }
-    const float is = inverse_root(fmaf(over_lanes(total<V>(sums), f.lanes), share, f.eps));
+    const float squares = over_lanes(total<V>(sums), f.lanes);
+    float is = inverse_root(fmaf(squares, share, f.eps));
     if (!on) continue;
+    if (!(squares < INFINITY)) is = far_inverse(far_squares<V, K>(v, lane, f) * share, f.eps);
     if (lane == 0) {
       mean[n * f.G + g] = mu;
       inv[n * f.G + g] = is;
@@ -759,17 +820,18 @@ __global__ void __launch_bounds__(512, 2)
       each_of_group(f, lane, [&](int i, int) { sum += sums[i + g * f.per]; });
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) to[g] = finish(sum / count);
+      if (lane == 0) to[g] = finish(sum / count, g);
     }
     __syncthreads();
   };
   int of[V];
   groups_of<V>(of, in ? q * V : 0, f.per);
-  float part[1][V] = {};
+  float part[1][V] = {}, downs[V];
+  fill<V>(downs, kDown);
 #pragma unroll
-  for (int k = 0; k < K; ++k) add_all<V>(part[0], part[0], v[k].v);
+  for (int k = 0; k < K; ++k) fma_all<V>(part[0], v[k].v, downs, part[0]);
   const float* sums = channel_sums<1, V>(scratch, part, q, row, on, f);
-  over_groups(sums, group, [](float m) { return m; });
+  over_groups(sums, group, [](float m, int) { return m * kUp; });
   float mu[V], is[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) mu[e] = group[of[e]], part[0][e] = 0.f;
@@ -782,7 +844,17 @@ __global__ void __launch_bounds__(512, 2)
 #pragma unroll
     for (int e = 0; e < V; ++e) part[0][e] = 0.f;
   sums = channel_sums<1, V>(scratch, part, q, row, on, f);
-  over_groups(sums, group + groups, [&](float m) { return inverse_root(m + f.eps); });
+  over_groups(sums, group + groups, [&](float m, int g) {
+    if (m < INFINITY) return inverse_root(m + f.eps);
+    const float* own = x + n * f.S * f.C + c0 + g * f.per;
+    float far = 0.f;
+    for (int p = 0; p < f.S; ++p)
+      for (int c = 0; c < f.per; ++c) {
+        const float d = (own[(int64_t)p * f.C + c] - group[g]) * kFar;
+        far = fmaf(d, d, far);
+      }
+    return far_inverse(far / count, f.eps);
+  });
   for (int g = threadIdx.x; g < groups; g += blockDim.x) {
     mean[n * f.G + c0 / f.per + g] = group[g];
     inv[n * f.G + c0 / f.per + g] = group[groups + g];
@@ -1122,7 +1194,7 @@ WXX_EXPORT int wxx_group_norm(float* y, float* mean, float* inv, const float* x,
   moments_kernel<<<(unsigned)(N * s.chunks), kT, 0, wxx::stream()>>>(m, x, s);
   int st = wxx::after_launch(__FILE__, __LINE__);
   if (st == WXX_OK) {
-    statistics_kernel<<<(unsigned)((N * G + kT - 1) / kT), kT, 0, wxx::stream()>>>(mean, inv, m, s);
+    statistics_kernel<<<(unsigned)((N * G + kT - 1) / kT), kT, 0, wxx::stream()>>>(mean, inv, m, x, s);
     st = wxx::after_launch(__FILE__, __LINE__);
   }
   wxx_free(part);

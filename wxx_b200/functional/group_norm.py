@@ -5,6 +5,8 @@ kernels in ``csrc/group_norm.cu``).
 normalised over all its positions, ``z = (x - mean) / sqrt(var + eps)``, ``n = gamma z +
 beta``.  The result is ``act(n)``, or with a gate ``n act(gate)``.  Tokens that are
 normalised each by itself are samples: ``x.reshape((batch * time, channels))``.
+Numbers of up to 2^126 in size, whose squares 32 bits do not hold, are normalised as any other;
+a NaN or an infinity makes its group's results NaN.
 """
 
 import math
