@@ -148,3 +148,51 @@ def test_scales_near_the_ends_of_the_range(d, scale, rng):
     for g, ref in zip(got, refs):
         e = np.linalg.norm(g.numpy().astype(np.float64) - ref) / np.linalg.norm(ref)
         assert e < 4e-6, e
+
+
+def test_documents_after_their_last_token_take_as_long_as_others(rng):
+    """Sequences that end early (keys and values of 0 from there on; backward: no gradient after
+    the prompt): the state decays below 2^-60 there and goes on as any other, to the formula's
+    values, and in about the time of a row of ordinary numbers."""
+    import wxx_b200 as wxx
+
+    F = _F()
+    B, T, H, d, n = 40, 4096, 1, 64, 512
+    q, k, v, do = normals(rng, *[(B, T, H * d)] * 4)
+    kz, vz, doz = k.copy(), v.copy(), do.copy()
+    kz[:, n:] = vz[:, n:] = 0
+    doz[:, :T - n] = 0
+    decay = np.log1p(-1 / np.float32([8])).astype(np.float32)
+    ld, uq = up(decay), up(q)
+    plain, ended = [up(t) for t in (k, v, do)], [up(t) for t in (kz, vz, doz)]
+    o, last = F.linear_attention(uq, ended[0], ended[1], ld)
+    grads = F.linear_attention_backward(ended[2], uq, plain[0], plain[1], ld)
+    row = slice(3, 4)
+    ro, rlast = retention.linear_attention(q[row], kz[row], vz[row], decay)
+    refs = retention.linear_attention_backward(doz[row], q[row], k[row], v[row], decay)
+    # Rows of an output against their own lengths: the decays over t positions, each good to t
+    # log(memory) u, as far as a number and its state (times up to 2^4) are normal ones
+    for got, ref in ((o, ro), (grads[1], refs[1]), (grads[2], refs[2])):
+        got, ref = got.numpy()[row].astype(np.float64)[0], ref[0]
+        size, off = np.linalg.norm(ref, axis=-1), np.linalg.norm(got - ref, axis=-1)
+        normal = size > 2.0 ** -110
+        assert normal.sum() > 1000 and (off[normal] < 1e-4 * size[normal]).all()
+        assert (off[~normal] < 2.0 ** -109).all()
+    assert np.abs(last.numpy()[row] - rlast).max() < 2.0 ** -120
+
+    def ms(call):
+        times = []
+        for _ in range(6):
+            a = wxx.backend.device.Event().record()
+            keep = call()
+            b = wxx.backend.device.Event().record()
+            wxx.backend.device.synchronize()
+            times.append(a.elapsed_ms(b))
+            del keep
+        return min(times)
+
+    # (position by position the forward took 11 times as long)
+    assert ms(lambda: F.linear_attention(uq, ended[0], ended[1], ld)) < \
+        4 * ms(lambda: F.linear_attention(uq, plain[0], plain[1], ld))
+    assert ms(lambda: F.linear_attention_backward(ended[2], uq, plain[0], plain[1], ld)) < \
+        4 * ms(lambda: F.linear_attention_backward(plain[2], uq, plain[0], plain[1], ld))
