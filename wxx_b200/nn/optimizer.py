@@ -10,8 +10,13 @@ from ..functional.utils import mark_written
 
 
 class Optimizer:
+    """A parameter that is listed again (LayerNorm registers weightg as weight, too) is kept, and
+    stepped, once, by its first name."""
+
     def __init__(self, parameters):
-        self.parameters = list(parameters)
+        seen = set()
+        self.parameters = [(name, w) for name, w in parameters
+                           if not (id(w) in seen or seen.add(id(w)))]
 
     def step(self):
         raise NotImplementedError
@@ -39,8 +44,8 @@ class SGD(Optimizer):
 
 
 class AdamW(Optimizer):
-    """Adam with decoupled weight decay, one ``wxx_adamw_device`` launch per
-    parameter: ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
+    """Adam with decoupled weight decay, all parameters in one launch (per 128 of
+    them): ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
     ``w -= lr (m / bc1 / (sqrt(v / bc2) + eps) + weight_decay w)`` with the bias
     corrections bc = 1 - beta^t (nn/optimizer.py:38-84, adamw.wgsl).
 
@@ -75,14 +80,9 @@ class AdamW(Optimizer):
               "adamw_advance")
         rows = []
         keep = []
-        seen = set()
         for (_, w), st in zip(self.params, self.state):
-            # A parameter listed again (LayerNorm registers weightg as weight, too) is stepped
-            # once: its two entries would run side by side in the launch and now and then
-            # see each other's half of a step.
-            if w.grad is None or id(w) in seen:
+            if w.grad is None:
                 continue
-            seen.add(id(w))
             g = functional.contiguous(w.grad)
             if tuple(g.shape) != tuple(w.shape):
                 raise ValueError(f"adamw: grad shape {tuple(g.shape)} != {tuple(w.shape)}")
