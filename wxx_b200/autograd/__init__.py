@@ -49,6 +49,17 @@ class Function:
         return out
 
 
+def _given(op, *tensors):
+    """Refuses a tensor of ``forward`` that needs a gradient and is not the constructor's in its
+    place, where its gradient would be lost."""
+    if context.MODE != 0:
+        return
+    for i, t in enumerate(tensors):
+        if getattr(t, "requires_grad", False) and not (i < len(op.inputs) and op.inputs[i] is t):
+            raise ValueError(f"{type(op).__name__}: tensor {i} needs a gradient, but the function is "
+                             "not constructed with it in that place")
+
+
 def _op(name, fn, doc):
     """A forward-only op (no backward in this backend)."""
     def forward(self, *a, **k):
@@ -520,6 +531,7 @@ class rotary(Function):
     """``functional.rotary`` of a tensor (batch, time, channels)."""
 
     def forward(self, x, n_heads, frequencies, positions=None, offset=0, layout="half"):
+        _given(self, x)
         if any(self.needs_input_grad):
             self.saved = (n_heads, frequencies, positions, offset, layout)
         return self._track(functional.rotary(x, n_heads, frequencies, positions, offset, layout))
@@ -531,11 +543,13 @@ class rotary(Function):
 
 class linear_attention(Function):
     """The outputs of linear attention with a decay for each head; constructed with q, k, v and,
-    when it needs a gradient, h0.  ``log_decay`` is a constant of the model."""
+    when it needs a gradient, h0.  ``log_decay`` is a constant of the model.  The last state is not
+    among the results: ``functional.linear_attention_backward`` takes its gradient."""
 
     def forward(self, q, k, v, log_decay, h0=None, reset=None, scale=1.0):
         if context.MODE == 0 and log_decay.requires_grad:
             raise ValueError("linear_attention: log_decay receives no gradient")
+        _given(self, q, k, v, h0)
         o, _ = functional.linear_attention(q, k, v, log_decay, h0, reset, scale)
         if any(self.needs_input_grad):
             self.saved = (q, k, v, log_decay, h0, reset, None, scale)
@@ -548,10 +562,11 @@ class linear_attention(Function):
 
 
 class group_norm(Function):
-    """``functional.group_norm``; constructed with x, gamma, beta and, where there is one, the
-    gate."""
+    """``functional.group_norm``; constructed with x, gamma, beta (or None for either) and, where
+    there is one that needs a gradient, the gate."""
 
     def forward(self, x, groups, gamma, beta, activation=None, gate=None, eps=1e-5):
+        _given(self, x, gamma, beta, gate)
         y, mean, inv = functional.group_norm(x, groups, gamma, beta, activation, gate, eps)
         if any(self.needs_input_grad):
             self.saved = (x, mean, inv, groups, gamma, beta, activation, gate)
