@@ -219,3 +219,20 @@ def test_linear_attention_a_chunk_at_a_time(rng):
     for a, b in zip(got, want):
         assert a.shape == b.shape
         assert np.abs(a - b).max() < 1e-11 * np.abs(b).max()
+
+
+def test_numbers_that_32_bits_do_not_hold_are_refused():
+    """The kernels take them in 32 bits, where 1e39 is infinite and 1e-50 is 0."""
+    import wxx_b200.functional as F
+
+    f = lambda *s: _Fake(s)  # noqa: E731
+    for call in (lambda v: F.RotaryFrequencies((1.0,), v),
+                 lambda v: F.linear_attention(f(2, 3, 8), f(2, 3, 8), f(2, 3, 12), f(2), scale=v),
+                 lambda v: F.linear_attention_backward(f(2, 3, 12), f(2, 3, 8), f(2, 3, 8), f(2, 3, 12),
+                                                       f(2), scale=v),
+                 lambda v: F.linear_attention_step(f(2, 8), f(2, 8), f(2, 12), f(2), f(2, 2, 4, 6), v),
+                 lambda v: F.group_norm(f(4, 6), 2, eps=v)):
+        with pytest.raises(ValueError):
+            call(1e39)
+    with pytest.raises(ValueError):
+        F.group_norm(f(4, 6), 2, eps=1e-50)

@@ -57,6 +57,11 @@ def compact(t):
     return t
 
 
+def finite32(value):
+    """Whether a number is finite as the 32-bit one that a kernel takes."""
+    return abs(value) <= 3.4028234663852886e38
+
+
 def ptr_or_none(t):
     return None if t is None else t.ptr
 
@@ -112,6 +117,7 @@ __all__ = [
     "empty",
     "empty_group",
     "F",
+    "finite32",
     "get_matmul_mode",
     "manual_seed",
     "matmul_mode_code",

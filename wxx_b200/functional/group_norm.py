@@ -11,7 +11,7 @@ a NaN or an infinity makes its group's results NaN.
 
 import math
 
-from ._common import F, check, compact, empty, empty_group, ptr_or_none
+from ._common import F, check, compact, empty, empty_group, finite32, ptr_or_none
 
 _SMALL = 1 << 20
 _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
@@ -45,7 +45,7 @@ def group_norm(x, groups, gamma=None, beta=None, activation=None, gate=None, eps
     the result's, or with ``gate`` (like ``x``) the gate's, which multiplies the result."""
     x, gamma, beta, gate, groups, code, N, S, C = _operands("group_norm", x, groups, gamma, beta,
                                                             activation, gate)
-    if not 0.0 < eps < math.inf:
+    if not (2.0 ** -149 <= eps and finite32(eps)):
         raise ValueError(f"group_norm: eps must be positive, got {eps}")
     # A small call takes as long as its host work: one allocation (14.7 -> 12 us).  A large
     # result must not be kept by the statistics.

@@ -12,9 +12,7 @@ new document starts: the state before such a position is zero, so documents pack
 one row do not see each other, not even their NaN.  Heads have up to 256 channels.
 """
 
-import math
-
-from ._common import F, check, compact, empty, ptr_or_none
+from ._common import F, check, compact, empty, finite32, ptr_or_none
 from .utils import mark_written
 
 _MOST = 256
@@ -64,8 +62,8 @@ def _operands(what, q, k, v, log_decay, h0, reset, scale):
     if reset is not None and tuple(reset.shape) != (B, T):
         raise ValueError(f"{what}: reset {tuple(reset.shape)} is not {(B, T)}")
     scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"{what}: the scale must be finite, got {scale}")
+    if not finite32(scale):
+        raise ValueError(f"{what}: the scale must be finite in 32 bits, got {scale}")
     given = [None if t is None else compact(t) for t in (log_decay, h0, reset)]
     return (*(_inner_dense(t) for t in (q, k, v)), *given, scale, B, T, H, dk, dv)
 
@@ -122,8 +120,8 @@ def linear_attention_step(q, k, v, log_decay, state, scale=1.0):
     if not state.is_dense():
         raise ValueError(f"{what}: the state is updated in place and must be dense")
     scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"{what}: the scale must be finite, got {scale}")
+    if not finite32(scale):
+        raise ValueError(f"{what}: the scale must be finite in 32 bits, got {scale}")
     q, k, v, log_decay = (_inner_dense(t) for t in (q, k, v, log_decay))
     o = empty((B, H * dv))
     check(F.wxx_linear_attention_step(o.buffer.ptr, state.ptr, q.ptr, q.stride[0], k.ptr,

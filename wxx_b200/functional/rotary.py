@@ -10,7 +10,7 @@ they are:
 import ctypes
 import math
 
-from ._common import F, check, compact, empty, ptr_or_none
+from ._common import F, check, compact, empty, finite32, ptr_or_none
 
 _MOST = 512
 _SCALINGS = ("linear", "ntk", "yarn")
@@ -25,7 +25,7 @@ class RotaryFrequencies:
         self.gain = float(gain)
         if not 1 <= len(self.frequencies) <= _MOST // 2:
             raise ValueError(f"rotary: 1 to {_MOST // 2} frequencies, got {len(self.frequencies)}")
-        if not all(math.isfinite(f) for f in self.frequencies) or not math.isfinite(self.gain):
+        if not all(math.isfinite(f) for f in self.frequencies) or not finite32(self.gain):
             raise ValueError("rotary: the frequencies and the gain must be finite")
         self.dim = 2 * len(self.frequencies)
         self._turns = (ctypes.c_double * len(self.frequencies))(
