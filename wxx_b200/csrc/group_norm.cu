@@ -75,7 +75,7 @@ __device__ __forceinline__ float clamped(float v, float high, float middle, floa
 }
 
 // Sums for a mean are made of 2^-16 of the numbers: as good, and those of 2^14 numbers of 2^126 fit.
-// Squared distances from the mean overflow from 2^64 / sqrt(n) on: their sum is then made again of
+// Squared distances from the mean overflow from 2^64 / sqrt(n) on: their sum is then made of
 // distances in units of 2^80, of which 2^24 fit.
 constexpr float kDown = 0x1p-16f, kUp = 0x1p16f, kFar = 0x1p-80f;
 __device__ __forceinline__ float far_inverse(float variance, float eps) {
@@ -573,21 +573,6 @@ struct Few {
   float eps;
 };
 
-// The sum of squares of a group's distances in units of 2^80, over the group's lanes alone.
-template <int V, int K>
-__device__ __forceinline__ float far_squares(const Pack<V> (&v)[K], int lane, const Few& f) {
-  const unsigned group = f.lanes == 32 ? 0xffffffffu
-                                       : ((1u << f.lanes) - 1) << (threadIdx.x & 31 & -f.lanes);
-  float far = 0.f;
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-    if ((k * f.lanes + lane) * V < f.per)
-#pragma unroll
-      for (int e = 0; e < V; ++e) far = fmaf(v[k].v[e] * kFar, v[k].v[e] * kFar, far);
-  for (int o = f.lanes >> 1; o > 0; o >>= 1) far += __shfl_xor_sync(group, far, o);
-  return far;
-}
-
 template <int V, int K, bool GATED>
 __global__ void __launch_bounds__(kT)
     token_kernel(float* __restrict__ y, float* __restrict__ mean, float* __restrict__ inv,
@@ -598,6 +583,8 @@ __global__ void __launch_bounds__(kT)
   const int lane = threadIdx.x % f.lanes, g = slot % f.G, row = slot / f.G;
   const bool here = row < f.rows;
   const float share = 1.0f / (float)f.per;
+  const unsigned group = f.lanes == 32 ? 0xffffffffu                // the lanes of this group
+                                       : ((1u << f.lanes) - 1) << (threadIdx.x & 31 & -f.lanes);
   Pack<V> ga[K], be[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -612,7 +599,7 @@ __global__ void __launch_bounds__(kT)
     const bool on = here && n < f.N;
     const int64_t at = n * f.C + g * f.per;
     Pack<V> v[K], w[GATED ? K : 1];
-    float sums[V], means[V], downs[V];
+    float sums[V], means[V], downs[V], units[V];
     fill<V>(sums, 0.f);
     fill<V>(downs, kDown);
 #pragma unroll
@@ -629,15 +616,28 @@ __global__ void __launch_bounds__(kT)
     const float mu = over_lanes(total<V>(sums), f.lanes) * (share * kUp);
     fill<V>(means, mu);
     fill<V>(sums, 0.f);
+    // (the unit of a group by a vote; a branch that makes the sum again, and its code between the
+    // rest, cost one position of 32 x 1024 0.5 us)
+    float top = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       sub_all<V>(v[k].v, v[k].v, means);
-      if ((k * f.lanes + lane) * V < f.per) fma_all<V>(sums, v[k].v, v[k].v, sums);
+      if ((k * f.lanes + lane) * V < f.per)
+#pragma unroll
+        for (int e = 0; e < V; ++e) top = fmaxf(top, fabsf(v[k].v[e]));
     }
-    const float squares = over_lanes(total<V>(sums), f.lanes);
-    float is = inverse_root(fmaf(squares, share, f.eps));
+    const bool far = (__ballot_sync(0xffffffffu, top >= 0x1p58f) & group) != 0;
+    const float unit = far ? kFar : 1.f;
+    fill<V>(units, unit);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if ((k * f.lanes + lane) * V < f.per) {
+        float d[V];
+        mul_all<V>(d, v[k].v, units);
+        fma_all<V>(sums, d, d, sums);
+      }
+    const float is = inverse_root(fmaf(over_lanes(total<V>(sums), f.lanes), share, f.eps * unit * unit)) * unit;
     if (!on) continue;
-    if (!(squares < INFINITY)) is = far_inverse(far_squares<V, K>(v, lane, f) * share, f.eps);
     if (lane == 0) {
       mean[n * f.G + g] = mu;
       inv[n * f.G + g] = is;
