@@ -284,12 +284,12 @@ constexpr float kShort = 0x1p-120f, kLong = 0x1p126f;
 // Rows of y and z with squares between these are not too far apart.
 constexpr float kBelow = 0x1p-54f, kAbove = 0x1p54f;
 constexpr int kApart = 110;
-// A state shorter than 2^-60, as the decays leave it behind a sequence's last token, is multiplied by
-// this while it is an operand.  (Position by position a row of 4096 positions whose last 3584 have
-// keys and values of 0 took 1490 us instead of 141, 64 channels, 40 sequences; backward 12.0 ms instead
-// of 0.4.)
-constexpr int kLifted = 80, kNoState = -1000;
-constexpr float kLift = 0x1p80f;
+// A state shorter than 2^-60, as the decays leave it behind a sequence's last token, is scaled by its
+// largest entry (times 64: its length is 90 of them at most), and by 2^127 at most: halves then leave
+// out less than 2^-150, which 32 bits cannot say either.  (Position by position a row of 4096
+// positions whose last 3584 have keys and values of 0 took 1490 us instead of 141, 64 channels, 40
+// sequences; backward 12.0 ms instead of 0.4.)
+constexpr int kNoState = -1000;
 // The exponent of a length with this square.
 __device__ __forceinline__ int exponent(float square) {
   return ((int)(__float_as_uint(square) >> 23) - 127) >> 1;
@@ -403,7 +403,7 @@ __device__ __forceinline__ bool far_apart(const float* square_y, const float* sq
 // The parts of shared memory that are not tiles.
 struct alignas(16) Small {
   float square_y[kC], square_z[kC];     // of the rows
-  float square_state[4];                // by warp; of a short one, minus that of kLift times it
+  float square_state[4];                // by warp; where that is short, minus the largest entry
   // per position j: 2^(exponents of y_j and z_j, below the largest) / what z_j's scale has more,
   // and that times l^(15 - j % 16) (back: l^(j % 16))
   float2 weight[kC];
@@ -634,11 +634,10 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
       odd = !(s0 < kLong);
-      if (s0 < kShort) {                // a state may be shorter than its square tells: by its
-        float top = 0.f;                // largest entry, times 64 (a part's length is 46 at most)
+      if (s0 < kShort) {                // a state may be shorter than its square tells
+        float top = 0.f;
         each([&](float v, int, int) { top = fmaxf(top, fabsf(v)); });
-        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))) * (kLift * 64.f);
-        s0 = -top * top;
+        s0 = -__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
       }
       if (lane == 0) m.square_state[warp] = s0;
     }
@@ -748,8 +747,8 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
                                (fmaxf(parts.z, 0.f) + fmaxf(parts.w, 0.f));
     int e_state = exponent(square_state);
     if (square_state == 0.f) {
-      const float lifted = -((parts.x + parts.y) + (parts.z + parts.w));
-      e_state = lifted > 0.f ? exponent(lifted) - kLifted : kNoState;
+      const float top = -fminf(fminf(parts.x, parts.y), fminf(parts.z, parts.w));
+      e_state = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127 + 6, kTop - 127) : kNoState;
     }
     if (!STATE && m.look == c) odd = odd || far_apart(m.square_y, m.square_z);
     if (odd) {
@@ -824,37 +823,20 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
     tile(std::integral_constant<int, P>{}, L::kY, y, up_y);
     if constexpr (!STATE) {
       if (e_state != kNoState) {
-        if (e_state < -100) {            // 2^(kTop - e_state) in two steps
-          const float up = power2(kTop - kLifted - e_state);
+        const float up = power2(kTop - e_state);
 #pragma unroll
-          for (int mt = 0; mt < L::kRowTiles; ++mt)
+        for (int mt = 0; mt < L::kRowTiles; ++mt)
 #pragma unroll
-            for (int nt = 0; nt < L::kColTiles; ++nt)
+          for (int nt = 0; nt < L::kColTiles; nt += 2) {
+            uint32_t hi[4], lo[4];
 #pragma unroll
-              for (int e = 0; e < 4; e += 2) {
-                uint32_t hi, lo;
-                split(X[mt][nt][e] * kLift, X[mt][nt][e + 1] * kLift, up, hi, lo);
-                unsigned char* to = smem + L::kState + 4 * t +
-                                    piece<R>(row0 + mt * 16 + quad + e * 4, col0 / 8 + nt);
-                *reinterpret_cast<uint32_t*>(to) = hi;
-                *reinterpret_cast<uint32_t*>(to + P * R * 2) = lo;
-              }
-        } else {
-          const float up = power2(kTop - e_state);
-#pragma unroll
-          for (int mt = 0; mt < L::kRowTiles; ++mt)
-#pragma unroll
-            for (int nt = 0; nt < L::kColTiles; nt += 2) {
-              uint32_t hi[4], lo[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                split(X[mt][nt + (e >> 1)][(e & 1) * 2], X[mt][nt + (e >> 1)][(e & 1) * 2 + 1], up, hi[e],
-                      lo[e]);
-              const uint32_t to = (read_state ^ ((col0 / 16 + nt / 2) << 5)) + (row0 + mt * 16) * R * 2;
-              store4<0>(to, hi[0], hi[1], hi[2], hi[3]);
-              store4<P * R * 2>(to, lo[0], lo[1], lo[2], lo[3]);
-            }
-        }
+            for (int e = 0; e < 4; ++e)
+              split(X[mt][nt + (e >> 1)][(e & 1) * 2], X[mt][nt + (e >> 1)][(e & 1) * 2 + 1], up, hi[e],
+                    lo[e]);
+            const uint32_t to = (read_state ^ ((col0 / 16 + nt / 2) << 5)) + (row0 + mt * 16) * R * 2;
+            store4<0>(to, hi[0], hi[1], hi[2], hi[3]);
+            store4<P * R * 2>(to, lo[0], lo[1], lo[2], lo[3]);
+          }
       }
     }
 #pragma unroll
