@@ -42,7 +42,9 @@ def group_norm(x, groups, gamma=None, beta=None, activation=None, gate=None, eps
     """``(y, mean, inv)``: the result like ``x``, and the groups' means and 1 / sqrt(var + eps)
     (samples, groups), which the backward takes.  ``gamma`` and ``beta`` (channels) default
     to 1 and 0; ``activation`` (None, ``"relu"``, ``"silu"`` or ``"gelu"``, the tanh form) is
-    the result's, or with ``gate`` (like ``x``) the gate's, which multiplies the result."""
+    the result's, or with ``gate`` (like ``x``) the gate's, which multiplies the result.  Up to
+    2^20 numbers share one allocation with their statistics, which is kept while any of the three
+    is."""
     x, gamma, beta, gate, groups, code, N, S, C = _operands("group_norm", x, groups, gamma, beta,
                                                             activation, gate)
     if not (2.0 ** -149 <= eps and finite32(eps)):

@@ -10,6 +10,12 @@ strides whose channels are dense (column slices of a projection are read in plac
 the model and receives no gradient.  ``reset`` (batch, time), u32, marks positions where a
 new document starts: the state before such a position is zero, so documents packed into
 one row do not see each other, not even their NaN.  Heads have up to 256 channels.
+
+Operands enter the products as pairs of half-precision numbers, 22 bits of each row (and of the
+state) relative to its length: results are good to about 6e-7 of their terms.  Rows that are not
+0 but shorter than 2^-60, or longer than 2^63, sizes 2^110 apart within 64 positions, an infinity or
+a NaN, and heads of more than 128 channels are worked through position by position, which takes
+longer.
 """
 
 from ._common import F, check, compact, empty, finite32, ptr_or_none
