@@ -196,3 +196,30 @@ def test_documents_after_their_last_token_take_as_long_as_others(rng):
         4 * ms(lambda: F.linear_attention(uq, plain[0], plain[1], ld))
     assert ms(lambda: F.linear_attention_backward(ended[2], uq, plain[0], plain[1], ld)) < \
         4 * ms(lambda: F.linear_attention_backward(plain[2], uq, plain[0], plain[1], ld))
+
+
+@pytest.mark.parametrize("d,log_decay,T", [(32, -3.0, 200), (64, -1.5, 200), (64, -0.1, 12000),
+                                           (32, -2.0, 12000)])
+def test_large_numbers_behind_small_decays(d, log_decay, T, rng):
+    """Keys and values of 1e12 to 1e15 at a row's first positions, little after them, queries of
+    1e6: their part of later outputs counts where the decay itself is below 2^-126.  A position's
+    decay, rounded each time, is off by up to t |log decay| u after t of them, t |log decay| below
+    120 where the terms are above 1e-15: with the products and sums (128 + 2 d) u of the terms."""
+    F = _F()
+    H = 1
+    q, k, v, do = normals(rng, *[(1, T, H * d)] * 4)
+    q *= np.float32(1e6)
+    k[:, :3] *= np.float32(1e12)
+    v[:, :3] *= np.float32(1e15)
+    k[:, 3:] *= np.float32(1e-15)
+    v[:, 3:] *= np.float32(1e-10)
+    decay = np.float32([log_decay])
+    terms = [np.abs(t) for t in (q, k, v)]
+    o, last = F.linear_attention(up(q), up(k), up(v), up(decay))
+    ro, rlast = retention.linear_attention(q, k, v, decay)
+    mo, mlast = retention.linear_attention(*terms, decay)
+    for got, ref, size in ((o, ro, mo), (last, rlast, mlast)):
+        off = np.abs(got.numpy() - ref)
+        counts = size > 1e-15
+        # halves: 3 * 2^-22 of the rows' lengths, up to d / 2 of their entries' products
+        assert (off <= (3 * 2.0 ** -22 * d + (248 + 2 * d) * 2.0 ** -24) * size)[counts].all()

@@ -281,7 +281,9 @@ __device__ __forceinline__ void square2(float& s0, float& s1, float a, float b) 
 // Whether a row of this square (or a state, of the larger one) cannot be scaled; 0 alone says
 // nothing yet.
 constexpr float kShort = 0x1p-120f, kLong = 0x1p126f;
-// Rows of y and z with squares between these are not too far apart.
+// Rows of y and z with squares between these are not too far apart, and with x up to the larger and a
+// state up to its square what decays below 2^-126 is below 2^-45, and taken as 0; in a chunk beyond
+// them such decays are worked through position by position.
 constexpr float kBelow = 0x1p-54f, kAbove = 0x1p54f;
 constexpr int kApart = 110;
 // A state shorter than 2^-60, as the decays leave it behind a sequence's last token, is scaled by its
@@ -342,8 +344,8 @@ struct Layout {
 struct Segments {           // pieces of a row that are worked on side by side
   int count, chunks;        // pieces, chunks of a piece
   float* state;             // (passes, count - 1, B H, p * r): after each piece but the last
-  float2* kept;             // (passes, count - 1, B H): what a piece leaves of a state X before it,
-                            // x X + y X as in Decay; y = -1: nothing, a reset is in it
+  float2* kept;             // (passes, count - 1, B H): what a piece leaves of a state X before it, y =
+                            // 1: X + x X; 0: x^2 X (l^n may be out of range); -1: 0, a reset is in it
 };
 
 // The chunk's weights of decay and resets.
@@ -633,7 +635,10 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
       s0 += s1;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-      odd = !(s0 < kLong);
+      if (!(s0 < kAbove * kAbove)) {
+        odd = !(s0 < kLong);
+        if (lane == 0) m.look = c;
+      }
       if (s0 < kShort) {                // a state may be shorter than its square tells
         float top = 0.f;
         each([&](float v, int, int) { top = fmaxf(top, fabsf(v)); });
@@ -705,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
         s0 += __shfl_xor_sync(0xffffffffu, s0, 1);
         s0 += __shfl_xor_sync(0xffffffffu, s0, 2);
         square_x[half] = s0;
-        rare = rare || !(s0 >= kShort && s0 < kLong);
+        rare = rare || !(s0 >= kShort && s0 < kAbove);
       }
     }
     if (__any_sync(0xffffffffu, rare)) {       // rows of zeros are fine
@@ -750,7 +755,8 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
       const float top = -fminf(fminf(parts.x, parts.y), fminf(parts.z, parts.w));
       e_state = top > 0.f ? max((int)(__float_as_uint(top) >> 23) - 127 + 6, kTop - 127) : kNoState;
     }
-    if (!STATE && m.look == c) odd = odd || far_apart(m.square_y, m.square_z);
+    if (m.look == c)
+      odd = odd || m.power[kC] < 0x1p-126f || (!STATE && far_apart(m.square_y, m.square_z));
     if (odd) {
       float* state = reinterpret_cast<float*>(smem + L::kTiles);
       unsigned char* cut = smem + L::kTiles + (P * R + kThreads) * 4;
@@ -1118,7 +1124,9 @@ __global__ void __launch_bounds__(kThreads, Layout<P, R, STATE, AHEAD>::kBlocks)
   if (STATE && threadIdx.x == 0) {
     const float run_log = (float)run * s.log_decay[h];
     g.kept[(pass * (int64_t)pieces + seg) * heads + b * s.H + h] =
-        run < 0 ? make_float2(0.f, -1.f) : make_float2(less_of(run_log), whole_of(run_log));
+        run < 0                      ? make_float2(0.f, -1.f)
+        : whole_of(run_log) != 0.f ? make_float2(expm1f(run_log), 1.f)
+                                     : make_float2(expf(0.5f * run_log), 0.f);
   }
 }
 
@@ -1148,8 +1156,9 @@ __global__ void __launch_bounds__(kT)
     const float next = more ? E[total] : 0.f;
     const float2 next_left = more ? __ldg(kept + heads) : left;
     X = left.y < 0.f             ? own
-        : fabsf(X) < INFINITY ? fmaf(left.y, X, fmaf(left.x, X, own))
-                                 : l(X) + own;
+        : !(fabsf(X) < INFINITY) ? l(X) + own
+        : left.y > 0.f           ? X + fmaf(left.x, X, own)
+                                 : fmaf(left.x * X, left.x, own);
     *E = X;
     own = next, left = next_left;
     E += total, kept += heads;
